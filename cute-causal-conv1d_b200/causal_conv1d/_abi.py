@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -87,6 +88,14 @@ SIGNATURES = {
     "cc1d_update_launch": (c_i32, [ctypes.POINTER(UpdateParams), c_void_p]),
     "cc1d_varlen_states_launch": (c_i32, [ctypes.POINTER(VarlenParams), c_void_p]),
     "cc1d_fwd_varlen_states_launch": (c_i32, [ctypes.POINTER(FwdVarlenStatesParams), c_void_p]),
+    # the params of these are packed as flat 64-bit words (_words)
+    "cc1d_recurrence_fwd_launch": (c_i32, [c_void_p, c_void_p]),
+    "cc1d_recurrence_bwd_workspace_bytes": (c_i64, [c_void_p]),
+    "cc1d_recurrence_bwd_launch": (c_i32, [c_void_p, c_void_p]),
+    "cc1d_recurrence_update_launch": (c_i32, [c_void_p, c_void_p]),
+    "cc1d_add_norm_fwd_launch": (c_i32, [c_void_p, c_void_p]),
+    "cc1d_add_norm_bwd_workspace_bytes": (c_i64, [c_void_p]),
+    "cc1d_add_norm_bwd_launch": (c_i32, [c_void_p, c_void_p]),
     "cc1d_last_error": (ctypes.c_char_p, []),
     "cc1d_status_string": (ctypes.c_char_p, [c_i32]),
     "cc1d_abi_version": (c_i32, []),
@@ -312,6 +321,146 @@ def fwd_varlen_states(x, weight, bias, seq_idx, cu_seqlens, states, out, silu: b
     p = FwdVarlenStatesParams(f, states.shape[0], states.shape[2], _ct(cu_seqlens), _ct(states))
     with _Guard(dev) as stream:
         _check(lib.cc1d_fwd_varlen_states_launch(ctypes.byref(p), stream))
+
+
+# ------------------------------------------------- recurrent-block operators
+# Their params structs are made of 64-bit words only (a cc1d_tensor is five: data, dtype
+# with the reserved half zero, three strides), so one struct.pack fills them: a decode
+# step is short enough for the host's time per call to count.
+RECURRENCE_CHUNK = 64  # CC1D_RECURRENCE_CHUNK
+_NONE = (0, 0, 0, 0, 0)
+RECURRENCE_PARAMS = struct.Struct("<78q")
+RECURRENCE_UPDATE_PARAMS = struct.Struct("<39q")
+ADD_NORM_PARAMS = struct.Struct("<55q2d")
+
+
+def _words(t: torch.Tensor | None) -> tuple:
+    if t is None:
+        return _NONE
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {t.dtype}")
+    s = t.stride()
+    n = len(s)
+    if n == 3:
+        return (t.data_ptr(), code, *s)
+    return (t.data_ptr(), code, *s, *_NONE[n:3])
+
+
+def _recurrence_shapes(x, gate, z, bias, seq_idx, states):
+    """Checks the shapes of a recurrence's tensors against x; ``states`` are (name, tensor)
+    pairs that must all be (nstates, dim).  Returns (B, D, L, nstates)."""
+    _expect_dims("x", x, 3)
+    shape = x.shape
+    B, D, L = shape
+    _expect("gate", gate, shape)
+    _expect("z", z, shape)
+    _expect("gate_bias", bias, (D,))
+    _expect("seq_idx", seq_idx, (B, L))
+    n = B if seq_idx is None else None
+    for name, t in states:
+        if t is not None:
+            _expect_dims(name, t, 2)
+            if n is None:
+                n = t.shape[0]
+            _expect(name, t, (n, D))
+    return B, D, L, 0 if n is None else n
+
+
+def recurrence_fwd(x, gate, z, bias, seq_idx, initial_states, final_states, checkpoints, out) -> None:
+    B, D, L, n = _recurrence_shapes(x, gate, z, bias, seq_idx,
+                                    (("initial_states", initial_states), ("final_states", final_states)))
+    _expect("out", out, (B, D, L))
+    if checkpoints is not None:
+        _expect("checkpoints", checkpoints, (B, -(-L // RECURRENCE_CHUNK), D))
+    lib = load_library()
+    dev = _device_of(x, gate, z, bias, seq_idx, initial_states, final_states, checkpoints, out)
+    p = RECURRENCE_PARAMS.pack(
+        B, D, L, n, *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(seq_idx), *_words(initial_states),
+        *_words(final_states), *_words(out), *_NONE * 6, 0, 0 if checkpoints is None else checkpoints.data_ptr(), 0, 0)
+    with _Guard(dev) as stream:
+        _check(lib.cc1d_recurrence_fwd_launch(p, stream))
+
+
+def recurrence_bwd(x, gate, z, bias, seq_idx, initial_states, checkpoints, dout, dfinal_states, dx, dgate, dz,
+                   dinitial_states, dbias) -> None:
+    B, D, L, n = _recurrence_shapes(x, gate, z, bias, seq_idx,
+                                    (("initial_states", initial_states), ("dfinal_states", dfinal_states),
+                                     ("dinitial_states", dinitial_states)))
+    for name, t in (("dout", dout), ("dx", dx), ("dgate", dgate), ("dz", dz)):
+        _expect(name, t, (B, D, L))
+    _expect("checkpoints", checkpoints, (B, -(-L // RECURRENCE_CHUNK), D))
+    _expect("dbias", dbias, (D,))
+    lib = load_library()
+    dev = _device_of(x, gate, z, bias, seq_idx, initial_states, checkpoints, dout, dfinal_states, dx, dgate, dz,
+                     dinitial_states, dbias)
+    words = (
+        B, D, L, n, *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(seq_idx), *_words(initial_states),
+        *_NONE * 2, *_words(dout), *_words(dfinal_states), *_words(dx), *_words(dgate), *_words(dz),
+        *_words(dinitial_states), 0 if dbias is None else dbias.data_ptr(), checkpoints.data_ptr())
+    with _Guard(dev) as stream:
+        need = lib.cc1d_recurrence_bwd_workspace_bytes(RECURRENCE_PARAMS.pack(*words, 0, 0))
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+        p = RECURRENCE_PARAMS.pack(*words, 0 if workspace is None else workspace.data_ptr(), max(need, 0))
+        _check(lib.cc1d_recurrence_bwd_launch(p, stream))
+
+
+def recurrence_update(x, gate, z, bias, state, state_indices, out) -> None:
+    _expect_dims("x", x, 3)
+    _expect_dims("state", state, 2)
+    shape = x.shape
+    B, D, T = shape
+    _expect("gate", gate, shape)
+    _expect("z", z, shape)
+    _expect("gate_bias", bias, (D,))
+    _expect("state", state, (B if state_indices is None else state.shape[0], D))
+    _expect("state_indices", state_indices, (B,))
+    _expect("out", out, shape)
+    lib = load_library()
+    dev = _device_of(x, gate, z, bias, state, state_indices, out)
+    p = RECURRENCE_UPDATE_PARAMS.pack(
+        B, D, T, state.shape[0], *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(state),
+        *_words(state_indices), *_words(out))
+    with _Guard(dev) as stream:
+        _check(lib.cc1d_recurrence_update_launch(p, stream))
+
+
+def add_norm_fwd(x, residual, weight, rng_state, out, residual_out, eps: float, dropout_p: float) -> None:
+    _expect_dims("x", x, 2)
+    shape = x.shape
+    for name, t in (("residual", residual), ("out", out), ("residual_out", residual_out)):
+        _expect(name, t, shape)
+    _expect("weight", weight, (shape[1],))
+    _expect("rng_state", rng_state, (2,))
+    lib = load_library()
+    dev = _device_of(x, residual, weight, rng_state, out, residual_out)
+    p = ADD_NORM_PARAMS.pack(
+        *shape, *_words(x), *_words(residual), *_words(weight), *_words(rng_state), *_words(out),
+        *_words(residual_out), *_NONE * 4, 0, 0, 0, eps, dropout_p)
+    with _Guard(dev) as stream:
+        _check(lib.cc1d_add_norm_fwd_launch(p, stream))
+
+
+def add_norm_bwd(x_dtype, residual_out, weight, rng_state, dout, dresidual_out, dx, dresidual, dweight,
+                 eps: float, dropout_p: float) -> None:
+    _expect_dims("residual_out", residual_out, 2)
+    shape = residual_out.shape
+    for name, t in (("dout", dout), ("dresidual_out", dresidual_out), ("dx", dx), ("dresidual", dresidual)):
+        _expect(name, t, shape)
+    _expect("weight", weight, (shape[1],))
+    _expect("dweight", dweight, (shape[1],))
+    _expect("rng_state", rng_state, (2,))
+    lib = load_library()
+    dev = _device_of(residual_out, weight, rng_state, dout, dresidual_out, dx, dresidual, dweight)
+    words = (
+        *shape, 0, _DTYPES[x_dtype], 0, 0, 0, *_NONE, *_words(weight), *_words(rng_state), *_NONE,
+        *_words(residual_out), *_words(dout), *_words(dresidual_out), *_words(dx), *_words(dresidual),
+        0 if dweight is None else dweight.data_ptr())
+    with _Guard(dev) as stream:
+        need = lib.cc1d_add_norm_bwd_workspace_bytes(ADD_NORM_PARAMS.pack(*words, 0, 0, eps, dropout_p))
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+        p = ADD_NORM_PARAMS.pack(*words, 0 if workspace is None else workspace.data_ptr(), max(need, 0), eps, dropout_p)
+        _check(lib.cc1d_add_norm_bwd_launch(p, stream))
 
 
 def launch_count() -> int:

@@ -35,9 +35,11 @@ UNITS = [
     ("cc1d_update.cu", [], "cc1d_update.o"),
     ("cc1d_decode.cu", [], "cc1d_decode.o"),
     ("cc1d_static.cu", [], "cc1d_static.o"),
+    ("cc1d_block_abi.cu", [], "cc1d_block_abi.o"),
 ] + [
     (src, [f"-DCC1D_DT={dt}"], f"{src[:-3]}_{name}.o")
-    for src in ("cc1d_fwd.cu", "cc1d_bwd.cu", "cc1d_rows.cu", "cc1d_rowwalk.cu")
+    for src in ("cc1d_fwd.cu", "cc1d_bwd.cu", "cc1d_rows.cu", "cc1d_rowwalk.cu",
+                "cc1d_recurrence.cu", "cc1d_add_norm.cu")
     for dt, name in ((0, "f32"), (1, "f16"), (2, "bf16"))
 ]
 

@@ -381,6 +381,7 @@ cc1d_status check_conv_common(int64_t B, int64_t D, int64_t L, int64_t W, const 
 }  // namespace
 
 void set_last_error(const char* msg) { g_last_error = msg; }
+void count_launches(int n) { g_launches.fetch_add(n); }
 
 cudaError_t allow_dynamic_smem(const void* kernel, size_t bytes) {
   if (bytes <= 48 * 1024) return cudaSuccess;

@@ -1,0 +1,294 @@
+// extern "C" launchers of the recurrent-block operators: the gated recurrence, its token
+// update, and dropout + residual add + RMSNorm.  Argument checks happen here, before any
+// launch; include/causal_conv1d_b200.h states the contract.
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+#include "cc1d_block_launch.h"
+
+namespace cc1d {
+namespace {
+
+cc1d_status fail(cc1d_status code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+cc1d_status fail(cc1d_status code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  try {
+    set_last_error(buf);
+  } catch (...) {  // out of memory for the message: the status alone has to do
+  }
+  return code;
+}
+
+cc1d_status launched(cudaError_t e, const char* what, int kernels) {
+  if (e != cudaSuccess)
+    return fail(CC1D_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorString(e), cudaGetErrorName(e));
+  count_launches(kernels);
+  return CC1D_OK;
+}
+
+bool is_float(int dt) { return dt == CC1D_FLOAT32 || dt == CC1D_FLOAT16 || dt == CC1D_BFLOAT16; }
+constexpr int64_t kMax31 = (int64_t{1} << 31) - 1;
+
+// Sizes whose products stay far inside 64 bits, so that the launchers' own arithmetic cannot wrap.
+bool sizes_ok(int64_t a, int64_t b, int64_t c) {
+  return a >= 0 && b >= 0 && c >= 0 && a <= kMax31 && b <= kMax31 && c <= kMax31 &&
+         static_cast<double>(a) * static_cast<double>(b) * static_cast<double>(c) < 4e18;
+}
+
+template <typename Args>
+cudaError_t by_type(int dtype, const Args& a, cudaStream_t s, cudaError_t (*f32)(const Args&, cudaStream_t),
+                    cudaError_t (*f16)(const Args&, cudaStream_t), cudaError_t (*bf16)(const Args&, cudaStream_t)) {
+  switch (dtype) {
+    case CC1D_FLOAT32: return f32(a, s);
+    case CC1D_FLOAT16: return f16(a, s);
+    default: return bf16(a, s);
+  }
+}
+
+#define CC1D_REQUIRE(t, name) \
+  if (!(t).data) return fail(CC1D_ERR_VALUE, "%s is required", name)
+#define CC1D_SAME_TYPE(t, name)                            \
+  if ((t).data && (t).dtype != p->x.dtype) return fail(CC1D_ERR_TYPE, "%s must have x's dtype", name)
+#define CC1D_FP32(t, name) \
+  if ((t).data && (t).dtype != CC1D_FLOAT32) return fail(CC1D_ERR_TYPE, "%s must be float32", name)
+
+cc1d_status rec_check(const cc1d_recurrence_params* p, bool bwd, RecArgs* a) {
+  if (!p) return fail(CC1D_ERR_VALUE, "params is NULL");
+  const int64_t B = p->batch, D = p->dim, L = p->seqlen, N = p->nstates;
+  if (!sizes_ok(B, D, L) || !sizes_ok(N, D, 1))
+    return fail(CC1D_ERR_VALUE, "sizes must be >= 0 and below 2^31");
+  if (!is_float(p->x.dtype)) return fail(CC1D_ERR_TYPE, "x must be float32, float16 or bfloat16");
+  CC1D_SAME_TYPE(p->gate, "gate");
+  CC1D_SAME_TYPE(p->z, "z");
+  if (p->bias.data && !is_float(p->bias.dtype)) return fail(CC1D_ERR_TYPE, "bias must be a float tensor");
+  if (p->seq_idx.data && p->seq_idx.dtype != CC1D_INT32) return fail(CC1D_ERR_TYPE, "seq_idx must be int32");
+  CC1D_FP32(p->initial_states, "initial_states");
+  if (!p->seq_idx.data && (p->initial_states.data || p->final_states.data || p->dfinal_states.data ||
+                           p->dinitial_states.data) && N != B)
+    return fail(CC1D_ERR_VALUE, "without seq_idx there is one state for each batch row");
+  if (!bwd) {
+    CC1D_SAME_TYPE(p->out, "out");
+    CC1D_FP32(p->final_states, "final_states");
+  } else {
+    CC1D_SAME_TYPE(p->dout, "dout");
+    CC1D_SAME_TYPE(p->dx, "dx");
+    CC1D_SAME_TYPE(p->dgate, "dgate");
+    CC1D_SAME_TYPE(p->dz, "dz");
+    CC1D_FP32(p->dfinal_states, "dfinal_states");
+    CC1D_FP32(p->dinitial_states, "dinitial_states");
+  }
+  if (B > 0 && D > 0 && L > 0) {
+    CC1D_REQUIRE(p->x, "x");
+    CC1D_REQUIRE(p->gate, "gate");
+    if (!bwd) {
+      CC1D_REQUIRE(p->out, "out");
+    } else {
+      CC1D_REQUIRE(p->dout, "dout");
+      CC1D_REQUIRE(p->dx, "dx");
+      CC1D_REQUIRE(p->dgate, "dgate");
+      if (p->z.data) CC1D_REQUIRE(p->dz, "dz");
+      if (!p->checkpoints) return fail(CC1D_ERR_VALUE, "checkpoints are required");
+    }
+  }
+  a->batch = B;
+  a->dim = D;
+  a->seqlen = L;
+  a->nstates = N;
+  a->nchunks = (L + kRecChunk - 1) / kRecChunk;
+  a->x = tensor_arg(p->x);
+  a->gate = tensor_arg(p->gate);
+  a->z = tensor_arg(p->z);
+  a->bias = tensor_arg(p->bias);
+  a->seq_idx = tensor_arg(p->seq_idx);
+  a->init = tensor_arg(p->initial_states);
+  a->final_states = bwd ? TensorArg{} : tensor_arg(p->final_states);
+  a->out = tensor_arg(p->out);
+  a->dout = tensor_arg(p->dout);
+  a->dfinal = tensor_arg(p->dfinal_states);
+  a->dx = tensor_arg(p->dx);
+  a->dgate = tensor_arg(p->dgate);
+  a->dz = tensor_arg(p->dz);
+  a->dinit = tensor_arg(p->dinitial_states);
+  a->dbias = bwd ? p->dbias : nullptr;
+  a->checkpoints = p->checkpoints;
+  a->partials = static_cast<float*>(p->workspace);
+  return CC1D_OK;
+}
+
+cc1d_status add_norm_check(const cc1d_add_norm_params* p, bool bwd, AddNormArgs* a) {
+  if (!p) return fail(CC1D_ERR_VALUE, "params is NULL");
+  if (!sizes_ok(p->rows, p->dim, 1)) return fail(CC1D_ERR_VALUE, "sizes must be >= 0 and below 2^31");
+  if (!is_float(p->x.dtype)) return fail(CC1D_ERR_TYPE, "x must be float32, float16 or bfloat16");
+  const int rt = p->residual_out.dtype;
+  if (rt != p->x.dtype && rt != CC1D_FLOAT32)
+    return fail(CC1D_ERR_TYPE, "residual_out must have x's dtype or be float32");
+  if (!is_float(p->weight.dtype)) return fail(CC1D_ERR_TYPE, "weight must be a float tensor");
+  if (!(p->dropout_p >= 0.0 && p->dropout_p < 1.0)) return fail(CC1D_ERR_VALUE, "dropout_p must be in [0, 1)");
+  if (!(p->eps >= 0.0)) return fail(CC1D_ERR_VALUE, "eps must be >= 0");
+  if (p->rng_state.data && p->rng_state.dtype != CC1D_INT64) return fail(CC1D_ERR_TYPE, "rng_state must be int64");
+  if (p->dropout_p > 0.0) CC1D_REQUIRE(p->rng_state, "rng_state");
+  const struct { const cc1d_tensor& t; const char* name; bool stream; } all[] = {
+      {p->x, "x", false},       {p->residual, "residual", true},           {p->out, "out", false},
+      {p->residual_out, "residual_out", true}, {p->dout, "dout", false}, {p->dresidual_out, "dresidual_out", true},
+      {p->dx, "dx", false},     {p->dresidual, "dresidual", true}};
+  for (const auto& e : all) {
+    if (!e.t.data) continue;
+    if (e.t.dtype != (e.stream ? rt : p->x.dtype))
+      return fail(CC1D_ERR_TYPE, "%s must have %s dtype", e.name, e.stream ? "residual_out's" : "x's");
+    if (p->dim > 1 && e.t.stride[1] != 1) return fail(CC1D_ERR_VALUE, "%s must have channel stride 1", e.name);
+  }
+  if (p->rows > 0 && p->dim > 0) {
+    CC1D_REQUIRE(p->weight, "weight");
+    CC1D_REQUIRE(p->residual_out, "residual_out");
+    if (!bwd) {
+      CC1D_REQUIRE(p->x, "x");
+      CC1D_REQUIRE(p->out, "out");
+    }
+  }
+  a->rows = p->rows;
+  a->dim = p->dim;
+  a->x = tensor_arg(p->x);
+  a->residual = tensor_arg(p->residual);
+  a->weight = tensor_arg(p->weight);
+  a->out = tensor_arg(p->out);
+  a->residual_out = tensor_arg(p->residual_out);
+  a->dout = tensor_arg(p->dout);
+  a->dresidual_out = tensor_arg(p->dresidual_out);
+  a->dx = tensor_arg(p->dx);
+  a->dresidual = tensor_arg(p->dresidual);
+  a->rng = p->dropout_p > 0.0 ? static_cast<const int64_t*>(p->rng_state.data) : nullptr;
+  a->rng_stride = p->rng_state.stride[0];
+  a->dweight = p->dweight;
+  a->partials = static_cast<float*>(p->workspace);
+  a->eps = static_cast<float>(p->eps);
+  a->keep_scale = static_cast<float>(1.0 / (1.0 - p->dropout_p));
+  a->keep_from = static_cast<unsigned>(p->dropout_p * 4294967296.0);
+  return CC1D_OK;
+}
+
+cc1d_status workspace_ok(const void* ws, int64_t bytes, int64_t need) {
+  if (need > 0 && (!ws || bytes < need))
+    return fail(CC1D_ERR_VALUE, "workspace too small: %lld bytes needed", (long long)need);
+  if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & 15u)) return fail(CC1D_ERR_VALUE, "workspace must be 16-byte aligned");
+  return CC1D_OK;
+}
+
+}  // namespace
+}  // namespace cc1d
+
+using namespace cc1d;
+
+extern "C" {
+
+cc1d_status cc1d_recurrence_fwd_launch(const cc1d_recurrence_params* p, void* stream) {
+  set_last_error("");
+  RecArgs a;
+  const cc1d_status st = rec_check(p, false, &a);
+  if (st != CC1D_OK || a.batch == 0 || a.dim == 0 || a.seqlen == 0) return st;
+  return launched(by_type(p->x.dtype, a, static_cast<cudaStream_t>(stream), rec_fwd_f32, rec_fwd_f16, rec_fwd_bf16),
+                  "gated recurrence forward launch", 1);
+}
+
+int64_t cc1d_recurrence_bwd_workspace_bytes(const cc1d_recurrence_params* p) {
+  set_last_error("");
+  RecArgs a;
+  if (rec_check(p, true, &a) != CC1D_OK) return -1;
+  if (a.batch == 0 || a.dim == 0 || a.seqlen == 0 || !a.dbias) return 0;
+  return rec_bwd_partial_floats(a) * static_cast<int64_t>(sizeof(float));
+}
+
+cc1d_status cc1d_recurrence_bwd_launch(const cc1d_recurrence_params* p, void* stream) {
+  set_last_error("");
+  RecArgs a;
+  cc1d_status st = rec_check(p, true, &a);
+  if (st != CC1D_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a.batch == 0 || a.dim == 0 || a.seqlen == 0) {
+    if (!a.dbias || a.dim == 0) return CC1D_OK;
+    return launched(cudaMemsetAsync(a.dbias, 0, a.dim * sizeof(float), s), "gated recurrence zero fill", 0);
+  }
+  if (a.dbias) {
+    st = workspace_ok(p->workspace, p->workspace_bytes, rec_bwd_partial_floats(a) * static_cast<int64_t>(sizeof(float)));
+    if (st != CC1D_OK) return st;
+  }
+  return launched(by_type(p->x.dtype, a, s, rec_bwd_f32, rec_bwd_f16, rec_bwd_bf16), "gated recurrence backward launch",
+                  a.dbias ? 2 : 1);
+}
+
+cc1d_status cc1d_recurrence_update_launch(const cc1d_recurrence_update_params* p, void* stream) {
+  set_last_error("");
+  if (!p) return fail(CC1D_ERR_VALUE, "params is NULL");
+  const int64_t B = p->batch, D = p->dim, T = p->seqlen, N = p->nstates;
+  if (!sizes_ok(B, D, T) || !sizes_ok(N, D, 1)) return fail(CC1D_ERR_VALUE, "sizes must be >= 0 and below 2^31");
+  if (!is_float(p->x.dtype)) return fail(CC1D_ERR_TYPE, "x must be float32, float16 or bfloat16");
+  CC1D_SAME_TYPE(p->gate, "gate");
+  CC1D_SAME_TYPE(p->z, "z");
+  CC1D_SAME_TYPE(p->out, "out");
+  if (p->bias.data && !is_float(p->bias.dtype)) return fail(CC1D_ERR_TYPE, "bias must be a float tensor");
+  CC1D_FP32(p->state, "state");
+  if (p->state_indices.data && p->state_indices.dtype != CC1D_INT32)
+    return fail(CC1D_ERR_TYPE, "state_indices must be int32");
+  if (!p->state_indices.data && N != B) return fail(CC1D_ERR_VALUE, "without state_indices there is one state for each batch row");
+  if (B == 0 || D == 0 || T == 0) return CC1D_OK;
+  CC1D_REQUIRE(p->x, "x");
+  CC1D_REQUIRE(p->gate, "gate");
+  CC1D_REQUIRE(p->out, "out");
+  if (N > 0) CC1D_REQUIRE(p->state, "state");
+  RecUpdateArgs a;
+  a.batch = B;
+  a.dim = D;
+  a.seqlen = T;
+  a.nstates = N;
+  a.x = tensor_arg(p->x);
+  a.gate = tensor_arg(p->gate);
+  a.z = tensor_arg(p->z);
+  a.bias = tensor_arg(p->bias);
+  a.state = tensor_arg(p->state);
+  a.out = tensor_arg(p->out);
+  a.indices = static_cast<const int32_t*>(p->state_indices.data);
+  a.indices_stride = p->state_indices.stride[0];
+  return launched(by_type(p->x.dtype, a, static_cast<cudaStream_t>(stream), rec_update_f32, rec_update_f16, rec_update_bf16),
+                  "gated recurrence update launch", 1);
+}
+
+cc1d_status cc1d_add_norm_fwd_launch(const cc1d_add_norm_params* p, void* stream) {
+  set_last_error("");
+  AddNormArgs a;
+  const cc1d_status st = add_norm_check(p, false, &a);
+  if (st != CC1D_OK || a.rows == 0 || a.dim == 0) return st;
+  return launched(by_type(p->x.dtype, a, static_cast<cudaStream_t>(stream), add_norm_fwd_f32, add_norm_fwd_f16, add_norm_fwd_bf16),
+                  "dropout_add_rms_norm forward launch", 1);
+}
+
+int64_t cc1d_add_norm_bwd_workspace_bytes(const cc1d_add_norm_params* p) {
+  set_last_error("");
+  AddNormArgs a;
+  if (add_norm_check(p, true, &a) != CC1D_OK) return -1;
+  if (a.rows == 0 || a.dim == 0 || !a.dweight) return 0;
+  return add_norm_bwd_partial_floats(a) * static_cast<int64_t>(sizeof(float));
+}
+
+cc1d_status cc1d_add_norm_bwd_launch(const cc1d_add_norm_params* p, void* stream) {
+  set_last_error("");
+  AddNormArgs a;
+  cc1d_status st = add_norm_check(p, true, &a);
+  if (st != CC1D_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a.rows == 0 || a.dim == 0) {
+    if (!a.dweight || a.dim == 0) return CC1D_OK;
+    return launched(cudaMemsetAsync(a.dweight, 0, a.dim * sizeof(float), s), "dropout_add_rms_norm zero fill", 0);
+  }
+  if (a.dweight) {
+    st = workspace_ok(p->workspace, p->workspace_bytes, add_norm_bwd_partial_floats(a) * static_cast<int64_t>(sizeof(float)));
+    if (st != CC1D_OK) return st;
+  }
+  return launched(by_type(p->x.dtype, a, s, add_norm_bwd_f32, add_norm_bwd_f16, add_norm_bwd_bf16),
+                  "dropout_add_rms_norm backward launch", a.dweight ? 2 : 1);
+}
+
+}  // extern "C"

@@ -1,0 +1,71 @@
+// Element-wise mathematics shared by the recurrent-block kernels.
+#pragma once
+
+#include "cc1d_common.cuh"
+
+namespace cc1d {
+
+// min(v, 1e30) that keeps a NaN: 1 + e and e / (1 + e) stay finite where exp overflows, and
+// the other sigmoid is then 1e-30, zero to working precision.
+__device__ __forceinline__ float clamp_exp(float v) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(1e30f));
+  return r;
+}
+
+// exp(-u), at most 1e30.  For 16-bit tensors 2^v by the hardware's approximation (relative
+// error about 2^-22, plus the rounding of u log2(e)); for fp32 the library's exp.
+template <typename T>
+__device__ __forceinline__ float exp_minus(float u) {
+  if constexpr (std::is_same<T, float>::value) return clamp_exp(expf(-u));
+  else return clamp_exp(ex2_approx(-kLog2e * u));
+}
+template <typename T>
+__device__ __forceinline__ float reciprocal(float v) {
+  if constexpr (std::is_same<T, float>::value) return __frcp_rn(v);
+  else return rcp_approx(v);
+}
+
+// a = sigmoid(u) and c = 1 - a = sigmoid(-u), each to full relative precision.
+template <typename T>
+__device__ __forceinline__ void sigmoid_pair(float u, float& a, float& c) {
+  const float e = exp_minus<T>(u);
+  a = reciprocal<T>(1.f + e);
+  c = e * a;
+}
+
+template <typename T>
+__device__ __forceinline__ float silu_of(float z) {
+  return z * reciprocal<T>(1.f + exp_minus<T>(z));
+}
+// silu(z) and its derivative sigmoid(z) (1 + z sigmoid(-z)).
+template <typename T>
+__device__ __forceinline__ void silu_and_grad(float z, float& s, float& ds) {
+  float p, q;
+  sigmoid_pair<T>(z, p, q);
+  s = z * p;
+  ds = p * fmaf(z, q, 1.f);
+}
+
+// ---------------------------------------------------------------------- Philox4x32-10
+// Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3" (2011):
+// four 32-bit words for a 128-bit counter under a 64-bit key.
+__device__ __forceinline__ uint4 philox(uint64_t key, uint64_t block, uint64_t stream) {
+  uint32_t k0 = static_cast<uint32_t>(key), k1 = static_cast<uint32_t>(key >> 32);
+  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32);
+  uint32_t c2 = static_cast<uint32_t>(stream), c3 = static_cast<uint32_t>(stream >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t p0 = static_cast<uint64_t>(c0) * 0xD2511F53u;
+    const uint64_t p1 = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
+    c0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ k0;
+    c1 = static_cast<uint32_t>(p1);
+    c2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ k1;
+    c3 = static_cast<uint32_t>(p0);
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+}  // namespace cc1d

@@ -84,6 +84,8 @@ inline cudaError_t launch_dependent(Kernel kernel, dim3 grid, dim3 block, size_t
 
 // Sets the message returned by cc1d_last_error() on the calling thread.
 void set_last_error(const char* msg);
+// Adds n to cc1d_launch_count().
+void count_launches(int n);
 
 cudaError_t rows_f32(bool bwd, const ConvArgs&, const LaunchShape&, cudaStream_t);
 cudaError_t rows_f16(bool bwd, const ConvArgs&, const LaunchShape&, cudaStream_t);

@@ -235,6 +235,135 @@ typedef struct cc1d_fwd_varlen_states_params {
 
 cc1d_status cc1d_fwd_varlen_states_launch(const cc1d_fwd_varlen_states_params* params, void* stream);
 
+/* ---------------------------------------------------------- gated recurrence
+ * The linear recurrence that follows the convolution in a recurrent block:
+ *     u[b, d, t] = gate[b, d, t] + bias[d]
+ *     h[b, d, t] = sigmoid(u) * h[b, d, t-1] + (1 - sigmoid(u)) * x[b, d, t]
+ *     out[b, d, t] = h[b, d, t] * silu(z[b, d, t])          (out = h without z)
+ * computed and carried in fp32 and rounded once, on the stores.
+ *
+ * Any strides are accepted; channel-last (stride[1] == 1) and (batch, dim, seqlen)
+ * contiguous (stride[2] == 1) tensors that all have the same layout are the fast ones.
+ *   x, gate, z, out (batch, dim, seqlen)   one float dtype; z optional
+ *   bias            (dim,)                 any float dtype, optional
+ *   seq_idx         (batch, seqlen)        int32, optional: a run of equal non-negative ids is one
+ *                                          sequence, and the id its row in the states (an id >=
+ *                                          nstates starts from zero and is stored nowhere); a
+ *                                          negative id is padding: out = 0, nothing is carried
+ *                                          across it, and whatever x, gate and z hold is ignored
+ *   initial_states  (nstates, dim) fp32    optional, h before the first position
+ *   final_states    (nstates, dim) fp32    optional output, h at the last position.  With seq_idx
+ *                                          only the rows of sequences that have positions are
+ *                                          written: fill the others beforehand
+ *   checkpoints     (batch, ceil(seqlen / CC1D_RECURRENCE_CHUNK), dim) fp32 contiguous: h before
+ *                                          each chunk; written by the forward if given, read by the
+ *                                          backward
+ * Without seq_idx nstates == batch.  The gradients of out and of final_states give
+ *   dx, dgate, dz   (batch, dim, seqlen)   outputs, x's dtype (dz iff z)
+ *   dinitial_states (nstates, dim) fp32    optional output; with seq_idx as final_states
+ *   dbias           (dim,) fp32            optional output, summed in a fixed order
+ *   workspace       device scratch of cc1d_recurrence_bwd_workspace_bytes(params) bytes, 16-byte
+ *                   aligned, contents need not be initialised
+ * dout (batch, dim, seqlen) has x's dtype; dfinal_states (nstates, dim) fp32 is optional.
+ * The forward ignores the gradient fields and the backward final_states and out.
+ */
+#define CC1D_RECURRENCE_CHUNK 64
+
+typedef struct cc1d_recurrence_params {
+  int64_t batch, dim, seqlen, nstates;
+  cc1d_tensor x;
+  cc1d_tensor gate;
+  cc1d_tensor z;
+  cc1d_tensor bias;
+  cc1d_tensor seq_idx;
+  cc1d_tensor initial_states;
+  cc1d_tensor final_states;
+  cc1d_tensor out;
+  cc1d_tensor dout;
+  cc1d_tensor dfinal_states;
+  cc1d_tensor dx;
+  cc1d_tensor dgate;
+  cc1d_tensor dz;
+  cc1d_tensor dinitial_states;
+  float* dbias;
+  float* checkpoints;
+  void* workspace;
+  int64_t workspace_bytes;
+} cc1d_recurrence_params;
+
+cc1d_status cc1d_recurrence_fwd_launch(const cc1d_recurrence_params* params, void* stream);
+/* Scratch bytes of the backward, or -1 with cc1d_last_error() set if the params are invalid. */
+int64_t cc1d_recurrence_bwd_workspace_bytes(const cc1d_recurrence_params* params);
+cc1d_status cc1d_recurrence_bwd_launch(const cc1d_recurrence_params* params, void* stream);
+
+/* --------------------------------------------------- gated recurrence, decoding
+ * The same recurrence for a few tokens of each row against a pool of states.
+ *   x, gate, z, out (batch, dim, seqlen)   as above, any strides
+ *   state           (nstates, dim) fp32    updated in place
+ *   state_indices   (batch,) int32         optional: state row of each batch row; a row outside
+ *                                          [0, nstates) is padding: out = 0, no state is touched.
+ *                                          Two batch rows must not name the same state row.
+ * Without state_indices nstates == batch.
+ */
+typedef struct cc1d_recurrence_update_params {
+  int64_t batch, dim, seqlen, nstates;
+  cc1d_tensor x;
+  cc1d_tensor gate;
+  cc1d_tensor z;
+  cc1d_tensor bias;
+  cc1d_tensor state;
+  cc1d_tensor state_indices;
+  cc1d_tensor out;
+} cc1d_recurrence_update_params;
+
+cc1d_status cc1d_recurrence_update_launch(const cc1d_recurrence_update_params* params, void* stream);
+
+/* --------------------------------------------- dropout + residual add + RMSNorm
+ * The residual connection between two blocks, on (rows, dim) matrices:
+ *     residual_out = residual + keep * x / (1 - dropout_p)        stored in residual_out's dtype
+ *     out          = residual_out / sqrt(mean(residual_out^2) + eps) * weight
+ * computed in fp32; what is normalised is residual_out as stored, so the backward, which
+ * reads it, differentiates exactly what the forward computed.
+ *
+ * keep is a function of the generator's state and the place alone and is never stored:
+ * element (row, col) takes word col % 4 of the Philox4x32-10 block with counter
+ * row * ceil(dim / 4) + col / 4 (low 64 bits) and rng_state[1] (high 64 bits) under the key
+ * rng_state[0], and is kept if that word is >= floor(dropout_p * 2^32).
+ *   x, out          (rows, dim)   one float dtype, channel stride 1
+ *   residual        (rows, dim)   optional, residual_out's dtype
+ *   residual_out    (rows, dim)   x's dtype or fp32: output of the forward, input of the backward
+ *   weight          (dim,)        any float dtype
+ *   rng_state       (2,) int64 on the device; needed iff dropout_p > 0
+ *   dropout_p       in [0, 1)
+ * Backward: dout (x's dtype) and dresidual_out (residual_out's dtype), each optional (absent
+ * means zero), give
+ *   dx              (rows, dim)   optional output, x's dtype
+ *   dresidual       (rows, dim)   optional output, residual_out's dtype
+ *   dweight         (dim,) fp32   optional output, summed in a fixed order
+ *   workspace       cc1d_add_norm_bwd_workspace_bytes(params) bytes, 16-byte aligned
+ */
+typedef struct cc1d_add_norm_params {
+  int64_t rows, dim;
+  cc1d_tensor x;
+  cc1d_tensor residual;
+  cc1d_tensor weight;
+  cc1d_tensor rng_state;
+  cc1d_tensor out;
+  cc1d_tensor residual_out;
+  cc1d_tensor dout;
+  cc1d_tensor dresidual_out;
+  cc1d_tensor dx;
+  cc1d_tensor dresidual;
+  float* dweight;
+  void* workspace;
+  int64_t workspace_bytes;
+  double eps, dropout_p;
+} cc1d_add_norm_params;
+
+cc1d_status cc1d_add_norm_fwd_launch(const cc1d_add_norm_params* params, void* stream);
+int64_t cc1d_add_norm_bwd_workspace_bytes(const cc1d_add_norm_params* params);
+cc1d_status cc1d_add_norm_bwd_launch(const cc1d_add_norm_params* params, void* stream);
+
 /* ------------------------------------------------------------------- utility */
 /* Message of the last error on the calling thread ("" if none). */
 const char* cc1d_last_error(void);
