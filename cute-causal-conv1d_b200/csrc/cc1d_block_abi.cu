@@ -50,6 +50,74 @@ cudaError_t by_type(int dtype, const Args& a, cudaStream_t s, cudaError_t (*f32)
   }
 }
 
+// ------------------------------------------------------------------ recurrence plan
+// 16-byte packets along the tensor's unit-stride dimension are legal.
+bool packets_ok(const TensorArg& t, const RecArgs& a) {
+  if (!t.data) return true;
+  const int64_t n = t.dtype == CC1D_FLOAT32 ? 4 : 8;
+  auto step_ok = [&](int64_t s, int64_t extent) { return extent <= 1 || s % n == 0; };
+  return (reinterpret_cast<uintptr_t>(t.data) & 15u) == 0 && step_ok(t.s0, a.batch) &&
+         (a.rows ? t.s2 == 1 && step_ok(t.s1, a.dim) : t.s1 == 1 && step_ok(t.s2, a.seqlen));
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return 148;
+  }
+  return n;
+}
+
+// CTAs that share a tile.  Each takes 1/cluster of the chunks; two CTAs fit an SM.  The
+// estimate counts chunk times: a CTA pays its start (about 3 chunks until its first tiles
+// are there), a cluster's barrier lengthens a chunk by a fifth, and an SM with one CTA
+// takes 0.6 of the time that two need for a chunk each.
+int choose_cluster(int64_t tiles, int64_t chunks) {
+  const int64_t sms = sm_count(), slots = 2 * sms;
+  double best = 0;
+  int pick = 1;
+  for (int c = 1; c <= 16 && c <= chunks; c *= 2) {
+    const int64_t ctas = tiles * c, rest = ctas % slots;
+    const double per_cta = (static_cast<double>((chunks + c - 1) / c) + 3.0) * (c > 1 ? 1.2 : 1.0);
+    const double cost = per_cta * (static_cast<double>(ctas / slots) + (rest == 0 ? 0.0 : rest <= sms ? 0.6 : 1.0));
+    if (c == 1 || cost < best) {
+      best = cost;
+      pick = c;
+    }
+  }
+  return pick;
+}
+
+// Layout, packets and cluster of a recurrence.  Rows: every tensor has unit stride along the
+// sequence; anything else goes element by element through the channel-last kernel unless all
+// have unit channel stride and alignment.
+cc1d_status rec_plan(RecArgs* a, bool bwd) {
+  const TensorArg* const all[] = {&a->x, &a->gate, &a->z, bwd ? &a->dout : &a->out, bwd ? &a->dx : nullptr,
+                                  bwd ? &a->dgate : nullptr, bwd ? &a->dz : nullptr};
+  bool last = true, rows = true;
+  for (const TensorArg* t : all) {
+    if (!t || !t->data) continue;
+    last = last && (t->s1 == 1 || a->dim == 1);
+    rows = rows && (t->s2 == 1 || a->seqlen == 1);
+  }
+  a->rows = rows && (!last || a->dim == 1);
+  a->packed = true;
+  for (const TensorArg* t : all)
+    if (t) a->packed = a->packed && packets_ok(*t, *a);
+  const int64_t channels = a->x.dtype == CC1D_FLOAT32 ? 32 : 64;
+  a->dtiles = (a->dim + channels - 1) / channels;
+  const int64_t tiles = a->batch * a->dtiles;
+  a->cluster = choose_cluster(tiles, a->nchunks);
+  if (tiles * a->cluster > kMax31) return fail(CC1D_ERR_VALUE, "batch * dim is too large");
+  return CC1D_OK;
+}
+
+int64_t rec_partial_bytes(const RecArgs& a) {
+  return a.batch * a.cluster * a.dim * static_cast<int64_t>(sizeof(float));
+}
+
 #define CC1D_REQUIRE(t, name) \
   if (!(t).data) return fail(CC1D_ERR_VALUE, "%s is required", name)
 #define CC1D_SAME_TYPE(t, name)                            \
@@ -188,8 +256,9 @@ extern "C" {
 cc1d_status cc1d_recurrence_fwd_launch(const cc1d_recurrence_params* p, void* stream) {
   set_last_error("");
   RecArgs a;
-  const cc1d_status st = rec_check(p, false, &a);
+  cc1d_status st = rec_check(p, false, &a);
   if (st != CC1D_OK || a.batch == 0 || a.dim == 0 || a.seqlen == 0) return st;
+  if ((st = rec_plan(&a, false)) != CC1D_OK) return st;
   return launched(by_type(p->x.dtype, a, static_cast<cudaStream_t>(stream), rec_fwd_f32, rec_fwd_f16, rec_fwd_bf16),
                   "gated recurrence forward launch", 1);
 }
@@ -199,7 +268,7 @@ int64_t cc1d_recurrence_bwd_workspace_bytes(const cc1d_recurrence_params* p) {
   RecArgs a;
   if (rec_check(p, true, &a) != CC1D_OK) return -1;
   if (a.batch == 0 || a.dim == 0 || a.seqlen == 0 || !a.dbias) return 0;
-  return rec_bwd_partial_floats(a) * static_cast<int64_t>(sizeof(float));
+  return rec_plan(&a, true) == CC1D_OK ? rec_partial_bytes(a) : -1;
 }
 
 cc1d_status cc1d_recurrence_bwd_launch(const cc1d_recurrence_params* p, void* stream) {
@@ -212,10 +281,8 @@ cc1d_status cc1d_recurrence_bwd_launch(const cc1d_recurrence_params* p, void* st
     if (!a.dbias || a.dim == 0) return CC1D_OK;
     return launched(cudaMemsetAsync(a.dbias, 0, a.dim * sizeof(float), s), "gated recurrence zero fill", 0);
   }
-  if (a.dbias) {
-    st = workspace_ok(p->workspace, p->workspace_bytes, rec_bwd_partial_floats(a) * static_cast<int64_t>(sizeof(float)));
-    if (st != CC1D_OK) return st;
-  }
+  if ((st = rec_plan(&a, true)) != CC1D_OK) return st;
+  if (a.dbias && (st = workspace_ok(p->workspace, p->workspace_bytes, rec_partial_bytes(a))) != CC1D_OK) return st;
   return launched(by_type(p->x.dtype, a, s, rec_bwd_f32, rec_bwd_f16, rec_bwd_bf16), "gated recurrence backward launch",
                   a.dbias ? 2 : 1);
 }

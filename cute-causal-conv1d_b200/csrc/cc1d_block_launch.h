@@ -14,7 +14,12 @@ struct RecArgs {
   TensorArg dout, dfinal, dx, dgate, dz, dinit;
   float* dbias;
   float* checkpoints;
-  float* partials;  // backward: sums of dgate to add up for dbias
+  float* partials;  // backward: (batch * cluster, dim) sums of dgate to add up for dbias
+  // the plan (rec_plan): tiles of channels, CTAs that share one, memory layout, and whether
+  // every tensor moves in 16-byte packets
+  int64_t dtiles;
+  int cluster;
+  bool rows, packed;
 };
 
 struct RecUpdateArgs {
@@ -49,7 +54,6 @@ CC1D_DECLARE(add_norm_bwd, AddNormArgs)
 #undef CC1D_DECLARE
 
 // fp32 values of workspace the backward kernels need.
-int64_t rec_bwd_partial_floats(const RecArgs& a);
 int64_t add_norm_bwd_partial_floats(const AddNormArgs& a);
 
 }  // namespace cc1d
