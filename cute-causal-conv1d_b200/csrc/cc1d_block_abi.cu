@@ -51,13 +51,22 @@ cudaError_t by_type(int dtype, const Args& a, cudaStream_t s, cudaError_t (*f32)
 }
 
 // ------------------------------------------------------------------ recurrence plan
-// 16-byte packets along the tensor's unit-stride dimension are legal.
+// Unit stride along the layout's dimension, the others not negative and small enough for a
+// 32-bit byte offset within a tile.
+bool strips_ok(const TensorArg& t, const RecArgs& a) {
+  if (!t.data) return true;
+  const int64_t size = t.dtype == CC1D_FLOAT32 ? 4 : 2;
+  const int64_t unit = a.rows ? t.s2 : t.s1, step = a.rows ? t.s1 : t.s2;
+  const bool steps = (a.rows ? a.dim : a.seqlen) > 1;
+  return (unit == 1 || (a.rows ? a.seqlen : a.dim) == 1) && t.s0 >= 0 && (!steps || (step >= 0 && step < (int64_t{1} << 32) / 64 / size));
+}
+// Every strip of it starts on a 16-byte boundary.
 bool packets_ok(const TensorArg& t, const RecArgs& a) {
   if (!t.data) return true;
   const int64_t n = t.dtype == CC1D_FLOAT32 ? 4 : 8;
   auto step_ok = [&](int64_t s, int64_t extent) { return extent <= 1 || s % n == 0; };
   return (reinterpret_cast<uintptr_t>(t.data) & 15u) == 0 && step_ok(t.s0, a.batch) &&
-         (a.rows ? t.s2 == 1 && step_ok(t.s1, a.dim) : t.s1 == 1 && step_ok(t.s2, a.seqlen));
+         (a.rows ? step_ok(t.s1, a.dim) : step_ok(t.s2, a.seqlen));
 }
 
 int sm_count() {
@@ -90,9 +99,8 @@ int choose_cluster(int64_t tiles, int64_t chunks) {
   return pick;
 }
 
-// Layout, packets and cluster of a recurrence.  Rows: every tensor has unit stride along the
-// sequence; anything else goes element by element through the channel-last kernel unless all
-// have unit channel stride and alignment.
+// Layout, way of moving and cluster of a recurrence.  Rows: every tensor has unit stride along
+// the sequence; all others take the channel-last kernel.
 cc1d_status rec_plan(RecArgs* a, bool bwd) {
   const TensorArg* const all[] = {&a->x, &a->gate, &a->z, bwd ? &a->dout : &a->out, bwd ? &a->dx : nullptr,
                                   bwd ? &a->dgate : nullptr, bwd ? &a->dz : nullptr};
@@ -103,9 +111,15 @@ cc1d_status rec_plan(RecArgs* a, bool bwd) {
     rows = rows && (t->s2 == 1 || a->seqlen == 1);
   }
   a->rows = rows && (!last || a->dim == 1);
+  bool strips = true;
   a->packed = true;
-  for (const TensorArg* t : all)
-    if (t) a->packed = a->packed && packets_ok(*t, *a);
+  for (const TensorArg* t : all) {
+    if (!t) continue;
+    strips = strips && strips_ok(*t, *a);
+    a->packed = a->packed && packets_ok(*t, *a);
+  }
+  a->packed = a->packed && strips;
+  a->skew = strips && !a->packed && a->x.dtype != CC1D_FLOAT32;
   const int64_t channels = a->x.dtype == CC1D_FLOAT32 ? 32 : 64;
   a->dtiles = (a->dim + channels - 1) / channels;
   const int64_t tiles = a->batch * a->dtiles;

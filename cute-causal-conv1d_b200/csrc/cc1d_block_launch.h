@@ -15,11 +15,12 @@ struct RecArgs {
   float* dbias;
   float* checkpoints;
   float* partials;  // backward: (batch * cluster, dim) sums of dgate to add up for dbias
-  // the plan (rec_plan): tiles of channels, CTAs that share one, memory layout, and whether
-  // every tensor moves in 16-byte packets
+  // the plan (rec_plan): tiles of channels, CTAs that share one, memory layout, and how the
+  // tensors move: in 16-byte packets, in 4-byte words that may cut an element's pair in two
+  // (skew, 16-bit types), or else element by element
   int64_t dtiles;
   int cluster;
-  bool rows, packed;
+  bool rows, packed, skew;
 };
 
 struct RecUpdateArgs {

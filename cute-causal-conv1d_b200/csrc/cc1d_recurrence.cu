@@ -53,10 +53,10 @@ __device__ __forceinline__ void gates(const Lane<V> (&g)[kRecSteps], const Lane<
 }
 
 template <typename T, int LAYOUT>
-__device__ __forceinline__ Lane<Tile<T, LAYOUT>::V> gate_offset(const RecArgs& a, int64_t d0, int lane) {
-  Lane<Tile<T, LAYOUT>::V> nb;
+__device__ __forceinline__ Lane<4 / sizeof(T)> gate_offset(const RecArgs& a, int64_t d0, int lane) {
+  Lane<4 / sizeof(T)> nb;
 #pragma unroll
-  for (int i = 0; i < Tile<T, LAYOUT>::V; ++i) {
+  for (int i = 0; i < static_cast<int>(4 / sizeof(T)); ++i) {
     const int64_t d = d0 + lane_channel<T, LAYOUT>(lane, i);
     const float b = a.bias.data && d < a.dim ? load_any(a.bias.data, a.bias.dtype, d * a.bias.s0) : 0.f;
     el(nb, i) = std::is_same<T, float>::value ? b : -kLog2e * b;
@@ -64,69 +64,141 @@ __device__ __forceinline__ Lane<Tile<T, LAYOUT>::V> gate_offset(const RecArgs& a
   return nb;
 }
 
-// The 8-bit mask of a warp's positions t .. t + 7 below len.
-__device__ __forceinline__ unsigned below(int64_t t, int64_t len) {
-  const int64_t n = len - t;
-  return n >= kRecSteps ? 0xffu : n <= 0 ? 0u : (1u << n) - 1u;
+// Positions of a chunk or of a warp, t .. t + n - 1, that lie within the sequence (may be <= 0).
+__device__ __forceinline__ int within(int64_t t, int64_t len, int n) {
+  return static_cast<int>(max(static_cast<int64_t>(-1), min(len - t, static_cast<int64_t>(n))));
+}
+__device__ __forceinline__ unsigned below(int n) { return n >= kRecSteps ? 0xffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// What a CTA is: a tile of channels of a batch row, and its place in the cluster.
+struct Place {
+  int64_t b, d0;
+  int nd, cluster, rank, rounds;
+};
+template <int CHANNELS>
+__device__ __forceinline__ Place place_of(const RecArgs& a) {
+  Place p;
+  p.cluster = a.cluster;
+  p.rank = a.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const unsigned tile = blockIdx.x / static_cast<unsigned>(a.cluster), n = static_cast<unsigned>(a.dtiles);
+  p.b = tile / n;
+  p.d0 = static_cast<int64_t>(tile % n) * CHANNELS;
+  p.nd = static_cast<int>(min(a.dim - p.d0, static_cast<int64_t>(CHANNELS)));
+  p.rounds = static_cast<int>((a.nchunks + a.cluster - 1) / a.cluster);
+  return p;
 }
 
-template <typename T, int LAYOUT, bool SEQ, bool Z>
+// The maps of the warps before warp w (FORWARD: lower warps first) after each other, applied to h.
+template <int V, bool SEQ, bool FORWARD>
+__device__ __forceinline__ Lane<V> through_warps(const Map<V>* sums, int w, int lane, Lane<V> h) {
+#pragma unroll
+  for (int i = 0; i < kRecWarps - 1; ++i) {
+    const int q = FORWARD ? i : kRecWarps - 1 - i;
+    const Map<V> m = sums[q * 32 + lane];
+    const Lane<V> r = apply<V, SEQ>(m.A, m.H, h);
+    if (FORWARD ? q < w : q > w) h = r;
+  }
+  return h;
+}
+
+// The state that warp w's positions start from, for a CTA of a cluster.  Takes the CTA's maps,
+// sends their composition to the cluster's CTAs and joins theirs; `carry` is the state the
+// round starts from, and becomes the one that the next starts from.
+template <int V, bool SEQ, bool FORWARD>
+__device__ __forceinline__ Lane<V> through_cluster(const Map<V>* sums, Map<V>* far, unsigned bar, unsigned parity, const Place& p,
+                                                   int w, int lane, Lane<V>& carry) {
+  Map<V> all, mine;
+  all.A = splat(1.f, Lane<V>{});
+  all.H = splat(0.f, Lane<V>{});
+  mine = all;
+#pragma unroll
+  for (int i = 0; i < kRecWarps; ++i) {
+    const int q = FORWARD ? i : kRecWarps - 1 - i;
+    if (q == w) mine = all;
+    const Map<V> m = sums[q * 32 + lane];
+    all.H = apply<V, SEQ>(m.A, m.H, all.H);
+    all.A = chain<V, SEQ>(m.A, all.A);
+  }
+  if (threadIdx.x == 0) mbar_expect(bar, p.cluster * 32 * sizeof(Map<V>));
+  const unsigned slot = static_cast<unsigned>(__cvta_generic_to_shared(far + p.rank * 32 + lane));
+  for (int r = w; r < p.cluster; r += kRecWarps) send_map<V>(slot, bar, r, all);
+  // a partner that never answers leaves NaN in the results instead of a hang
+  Lane<V> h = mbar_wait(bar, parity) ? carry : splat(__int_as_float(0x7fc00000), carry);
+  Lane<V> start = h;
+#pragma unroll 4
+  for (int i = 0; i < p.cluster; ++i) {
+    const int r = FORWARD ? i : p.cluster - 1 - i;
+    if (r == p.rank) start = h;
+    const Map<V> m = far[r * 32 + lane];
+    h = apply<V, SEQ>(m.A, m.H, h);
+  }
+  carry = h;
+  return apply<V, SEQ>(mine.A, mine.H, start);
+}
+
+template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z>
 __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const RecArgs a) {
-  using C = Tile<T, LAYOUT>;
+  using C = Tile<T, LAYOUT, SKEW>;
   constexpr int V = C::V, NT = Z ? 3 : 2, S = kFwdStages;
   using L = Lane<V>;
   extern __shared__ __align__(128) unsigned char smem[];
-  unsigned char* const ring = smem;
-  L* const sumA = reinterpret_cast<L*>(smem + S * NT * C::kBytes);  // [2][warps][32]
-  L* const sumH = sumA + 2 * kRecWarps * 32;
-  L* const farA = sumH + 2 * kRecWarps * 32;  // [2][cluster][32]
-  L* const farH = farA + 2 * a.cluster * 32;
+  // ring of tiles (gate, x, z) | maps of the warps [2][warps][32] | maps of the cluster [2][cluster][32]
+  Map<V>* const sums = reinterpret_cast<Map<V>*>(smem + S * NT * C::kBytes);
+  Map<V>* const far = sums + 2 * kRecWarps * 32;
+  __shared__ L handed[2][32];     // without a cluster: the state after the last warp's positions
+  __shared__ uint64_t bars[2];
+  const unsigned ring = static_cast<unsigned>(__cvta_generic_to_shared(smem));
+  const unsigned bar = static_cast<unsigned>(__cvta_generic_to_shared(bars));
 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const unsigned cluster = a.cluster, rank = cluster > 1 ? cluster_rank() : 0;
-  const int64_t tile = blockIdx.x / cluster;
-  const int64_t b = tile / a.dtiles, d0 = (tile - b * a.dtiles) * C::kChannels;
-  const int64_t rounds = (a.nchunks + cluster - 1) / cluster;
+  const Place p = place_of<C::kChannels>(a);
   grid_dependency_wait();
+  const Strip<T> gt = strip_of<T, LAYOUT, SKEW>(a.gate, p.b, p.d0), xt = strip_of<T, LAYOUT, SKEW>(a.x, p.b, p.d0);
+  const Strip<T> zt = Z ? strip_of<T, LAYOUT, SKEW>(a.z, p.b, p.d0) : gt, ot = strip_of<T, LAYOUT, SKEW>(a.out, p.b, p.d0);
+  const int nch = p.nd - lane * V;
 
-  const T* const xp = static_cast<const T*>(a.x.data) + b * a.x.s0;
-  const T* const gp = static_cast<const T*>(a.gate.data) + b * a.gate.s0;
-  const T* const zp = Z ? static_cast<const T*>(a.z.data) + b * a.z.s0 : nullptr;
-  T* const op = static_cast<T*>(a.out.data) + b * a.out.s0;
-  const int dl = lane_channel<T, LAYOUT>(lane, 0);
-  const int nch = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(V), a.dim - d0 - dl)));
-
-  auto load = [&](int64_t k) {
-    const int64_t c = k * cluster + rank;
-    if (k < rounds && c < a.nchunks) {
-      unsigned char* t = ring + (k % S) * NT * C::kBytes;
-      load_tile<T, LAYOUT>(t, gp, a.gate.s1, a.gate.s2, d0, c * kRecChunk, a.dim, a.seqlen, a.packed);
-      load_tile<T, LAYOUT>(t + C::kBytes, xp, a.x.s1, a.x.s2, d0, c * kRecChunk, a.dim, a.seqlen, a.packed);
-      if constexpr (Z) load_tile<T, LAYOUT>(t + 2 * C::kBytes, zp, a.z.s1, a.z.s2, d0, c * kRecChunk, a.dim, a.seqlen, a.packed);
+  int load_slot = 0;
+  auto load = [&](int k) {
+    const int64_t t0 = (static_cast<int64_t>(k) * p.cluster + p.rank) * kRecChunk;
+    const int nt = within(t0, a.seqlen, kRecChunk), o = load_slot * NT * C::kBytes;
+    if (k < p.rounds && nt > 0) {
+      load_tile<T, LAYOUT, SKEW>(ring + o, smem + o, gt, t0, p.nd, nt, a.packed);
+      load_tile<T, LAYOUT, SKEW>(ring + o + C::kBytes, smem + o + C::kBytes, xt, t0, p.nd, nt, a.packed);
+      if constexpr (Z) load_tile<T, LAYOUT, SKEW>(ring + o + 2 * C::kBytes, smem + o + 2 * C::kBytes, zt, t0, p.nd, nt, a.packed);
     }
     cp_async_commit();
+    if (++load_slot == S) load_slot = 0;
   };
 #pragma unroll
   for (int k = 0; k < S - 1; ++k) load(k);
-  if (cluster > 1) {  // the others' shared memory may be written once they have all begun
-    cluster_arrive();
-    cluster_wait();
+  if (p.cluster > 1) {
+    if (threadIdx.x == 0) {
+      mbar_init(bar);
+      mbar_init(bar + 8);
+      mbar_init_done();
+    }
+    cluster_sync();  // the barriers are there before a partner's first map arrives
   }
-  const L nb = gate_offset<T, LAYOUT>(a, d0, lane);
-  L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.init, b, a.nstates, d0, a.dim, lane);
-  int ids = SEQ ? load_ids(a, b, static_cast<int64_t>(rank) * kRecChunk + w * kRecSteps, lane) : 0;
+  const L nb = gate_offset<T, LAYOUT>(a, p.d0, lane);
+  L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.init, p.b, a.nstates, p.d0, a.dim, lane);
+  if (w == 0) handed[0][lane] = carry;
+  int ids = SEQ ? load_ids(a, p.b, static_cast<int64_t>(p.rank) * kRecChunk + w * kRecSteps, lane) : 0;
 
-  for (int64_t k = 0; k < rounds; ++k) {
-    const int64_t c = k * cluster + rank;
+  int slot = 0;
+  for (int k = 0; k < p.rounds; ++k) {
+    const int64_t c = static_cast<int64_t>(k) * p.cluster + p.rank;
     const int64_t t0 = c * kRecChunk, tw = t0 + w * kRecSteps;
-    unsigned char* const now = ring + (k % S) * NT * C::kBytes;
-    const int buf = static_cast<int>(k & 1);
+    const int left = within(tw, a.seqlen, kRecSteps);
+    unsigned char* const now = smem + slot * NT * C::kBytes;
+    const int buf = k & 1;
     cp_async_wait<S - 2>();
     if constexpr (C::kRows) {
       __syncthreads();
-      if (k > 0)
-        store_tile<T>(ring + ((k - 1) % S) * NT * C::kBytes + C::kBytes, op, a.out.s1, a.out.s2, d0, t0 - static_cast<int64_t>(cluster) * kRecChunk,
-                      a.dim, a.seqlen, a.packed);
+      if (k > 0) {
+        const int64_t tp = t0 - static_cast<int64_t>(p.cluster) * kRecChunk;
+        store_tile<T, SKEW>(smem + (slot == 0 ? S - 1 : slot - 1) * NT * C::kBytes + C::kBytes, ot, tp, p.nd, within(tp, a.seqlen, kRecChunk), a.packed);
+        if constexpr (SKEW) __syncthreads();
+      }
     } else {
       __syncwarp();
     }
@@ -135,34 +207,33 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const RecArgs a
     // the 8 positions' maps and their composition
     L ga[kRecSteps], gb[kRecSteps];
     {
-      L g[kRecSteps], x[kRecSteps];
-      read_steps<T, LAYOUT>(now, w, lane, g);
-      read_steps<T, LAYOUT>(now + C::kBytes, w, lane, x);
-      L gc[kRecSteps];
+      L g[kRecSteps], x[kRecSteps], gc[kRecSteps];
+      read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, g);
       gates<T, V>(g, nb, ga, gc);
+      read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, x);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gc[j], x[j]);
     }
     Edges e;
-    unsigned valid = below(tw, a.seqlen);
+    unsigned valid = below(left);
     if constexpr (SEQ) {
       e = edges_of(ids);
       valid = e.valid;
-      ids = load_ids(a, b, tw + static_cast<int64_t>(cluster) * kRecChunk, lane);
+      ids = load_ids(a, p.b, tw + static_cast<int64_t>(p.cluster) * kRecChunk, lane);
     }
-    L A, H;
+    Map<V> m;
     const bool whole = valid == 0xffu && !(SEQ && e.first);
     if (whole) {
-      A = ga[0];
-      H = gb[0];
+      m.A = ga[0];
+      m.H = gb[0];
 #pragma unroll
       for (int j = 1; j < kRecSteps; ++j) {
-        A = mul(ga[j], A);
-        H = fma(ga[j], H, gb[j]);
+        m.A = mul(ga[j], m.A);
+        m.H = fma(ga[j], m.H, gb[j]);
       }
     } else {
-      A = splat(1.f, L{});
-      H = splat(0.f, L{});
+      m.A = splat(1.f, L{});
+      m.H = splat(0.f, L{});
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
         if (!(valid >> j & 1u)) {  // no token: the state passes
@@ -170,57 +241,23 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const RecArgs a
           gb[j] = splat(0.f, L{});
         }
         if (SEQ && (e.first >> j & 1u)) {
-          H = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, d0, a.dim, lane);
-          A = splat(-1.f, L{});
+          m.H = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
+          m.A = splat(-1.f, L{});
         }
-        A = mul(ga[j], A);
-        H = fma(ga[j], H, gb[j]);
+        m.A = mul(ga[j], m.A);
+        m.H = fma(ga[j], m.H, gb[j]);
       }
     }
-    sumA[(buf * kRecWarps + w) * 32 + lane] = A;
-    sumH[(buf * kRecWarps + w) * 32 + lane] = H;
+    Map<V>* const sum = sums + buf * kRecWarps * 32;
+    sum[w * 32 + lane] = m;
     __syncthreads();
-
-    L h = carry;
-    if (cluster == 1) {
-      L p = carry;
-#pragma unroll
-      for (int q = 0; q < kRecWarps; ++q) {
-        if (q == w) h = p;
-        p = apply<V, SEQ>(sumA[(buf * kRecWarps + q) * 32 + lane], sumH[(buf * kRecWarps + q) * 32 + lane], p);
-      }
-      carry = p;
-    } else {
-      L pa = splat(1.f, L{}), ph = splat(0.f, L{}), wa = pa, wh = ph;
-#pragma unroll
-      for (int q = 0; q < kRecWarps; ++q) {
-        if (q == w) wa = pa, wh = ph;
-        const L qa = sumA[(buf * kRecWarps + q) * 32 + lane];
-        ph = apply<V, SEQ>(qa, sumH[(buf * kRecWarps + q) * 32 + lane], ph);
-        pa = chain<V, SEQ>(qa, pa);
-      }
-      for (unsigned r = w; r < cluster; r += kRecWarps) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          store_remote(&el(farA[(buf * cluster + rank) * 32 + lane], i), r, el(pa, i));
-          store_remote(&el(farH[(buf * cluster + rank) * 32 + lane], i), r, el(ph, i));
-        }
-      }
-      cluster_arrive();
-      cluster_wait();
-      L p = carry;
-      for (unsigned r = 0; r < cluster; ++r) {
-        if (r == rank) h = p;
-        p = apply<V, SEQ>(farA[(buf * cluster + r) * 32 + lane], farH[(buf * cluster + r) * 32 + lane], p);
-      }
-      carry = p;
-      h = apply<V, SEQ>(wa, wh, h);
-    }
+    L h = p.cluster == 1 ? through_warps<V, SEQ, true>(sum, w, lane, handed[buf][lane])
+                         : through_cluster<V, SEQ, true>(sum, far + buf * p.cluster * 32, bar + 8 * buf, (k >> 1) & 1, p, w, lane, carry);
     if (w == 0 && a.checkpoints && c < a.nchunks) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int64_t d = d0 + lane_channel<T, LAYOUT>(lane, i);
-        if (d < a.dim) a.checkpoints[(b * a.nchunks + c) * a.dim + d] = el(h, i);
+        const int64_t d = p.d0 + lane_channel<T, LAYOUT>(lane, i);
+        if (d < a.dim) a.checkpoints[(p.b * a.nchunks + c) * a.dim + d] = el(h, i);
       }
     }
 
@@ -228,19 +265,20 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const RecArgs a
 #pragma unroll
     for (int j = 0; j < kRecSteps; ++j) {
       if (SEQ && !whole && (e.first >> j & 1u))
-        h = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, d0, a.dim, lane);
+        h = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
       h = fma(ga[j], h, gb[j]);
       gb[j] = h;
     }
+    if (p.cluster == 1 && w == kRecWarps - 1) handed[buf ^ 1][lane] = h;
     if (SEQ && e.last && a.final_states.data) {
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j)
         if (e.last >> j & 1u)
-          store_state<T, LAYOUT>(a.final_states, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, d0, a.dim, lane, gb[j]);
+          store_state<T, LAYOUT>(a.final_states, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane, gb[j]);
     }
     if constexpr (Z) {
       L z[kRecSteps];
-      read_steps<T, LAYOUT>(now + 2 * C::kBytes, w, lane, z);
+      read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, zt, t0, w, lane, z);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
         L s;
@@ -255,112 +293,117 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const RecArgs a
         if (!(valid >> j & 1u)) gb[j] = splat(0.f, L{});
     }
     if constexpr (C::kRows) {
-      write_steps<T, LAYOUT>(now + C::kBytes, w, lane, gb);
+      write_steps<T, SKEW>(now + C::kBytes, w, lane, gb);
     } else {
-      T* o = op + (d0 + dl) * a.out.s1 + tw * a.out.s2;
-      if (tw + kRecSteps <= a.seqlen) {
-#pragma unroll
-        for (int j = 0; j < kRecSteps; ++j) store_step<T>(o + j * a.out.s2, a.out.s1, nch, a.packed, gb[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kRecSteps; ++j)
-          if (tw + j < a.seqlen) store_step<T>(o + j * a.out.s2, a.out.s1, nch, a.packed, gb[j]);
-      }
+      store_steps<T, SKEW>(ot, tw, lane, nch, left, a.packed, gb);
     }
+    if (++slot == S) slot = 0;
   }
   if constexpr (C::kRows) {
     __syncthreads();
-    store_tile<T>(ring + ((rounds - 1) % S) * NT * C::kBytes + C::kBytes, op, a.out.s1, a.out.s2, d0,
-                  ((rounds - 1) * cluster + rank) * kRecChunk, a.dim, a.seqlen, a.packed);
+    const int64_t tp = (static_cast<int64_t>(p.rounds - 1) * p.cluster + p.rank) * kRecChunk;
+    store_tile<T, SKEW>(smem + (slot == 0 ? S - 1 : slot - 1) * NT * C::kBytes + C::kBytes, ot, tp, p.nd, within(tp, a.seqlen, kRecChunk), a.packed);
   }
-  if (!SEQ && w == 0 && rank == 0) store_state<T, LAYOUT>(a.final_states, b, a.nstates, d0, a.dim, lane, carry);
+  if (!SEQ && a.final_states.data && p.rank == 0) {
+    if (p.cluster == 1) {
+      __syncthreads();
+      carry = handed[p.rounds & 1][lane];
+    }
+    if (w == 0) store_state<T, LAYOUT>(a.final_states, p.b, a.nstates, p.d0, a.dim, lane, carry);
+  }
+  if (p.cluster > 1) cluster_sync();  // no CTA leaves while a partner may still write to it
 }
 
-template <typename T, int LAYOUT, bool SEQ, bool Z>
+template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z>
 __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a) {
-  using C = Tile<T, LAYOUT>;
+  using C = Tile<T, LAYOUT, SKEW>;
   constexpr int V = C::V, NT = Z ? 4 : 3, S = kBwdStages<LAYOUT>;
   using L = Lane<V>;
   extern __shared__ __align__(128) unsigned char smem[];
-  unsigned char* const ring = smem;  // gate, x, dout, z
-  L* const sumA = reinterpret_cast<L*>(smem + S * NT * C::kBytes);  // [2][warps][32], of h -> A h + H
-  L* const sumH = sumA + 2 * kRecWarps * 32;
-  L* const sumS = sumH + 2 * kRecWarps * 32;                 // of s -> R s + S, back through the warp's positions
-  L* const sumR = SEQ ? sumS + 2 * kRecWarps * 32 : sumA;    // the same product unless a sequence ends or starts
-  L* const farR = (SEQ ? sumR : sumS) + 2 * kRecWarps * 32;  // [2][cluster][32]
-  L* const farS = farR + 2 * a.cluster * 32;
+  // ring of tiles (gate, x, dout, z) | maps of the warps, forward and back [2][2][warps][32] |
+  // maps of the cluster, back [2][cluster][32]
+  Map<V>* const sums = reinterpret_cast<Map<V>*>(smem + S * NT * C::kBytes);
+  Map<V>* const far = sums + 4 * kRecWarps * 32;
+  __shared__ L handed[2][32];
+  __shared__ uint64_t bars[2];
+  const unsigned ring = static_cast<unsigned>(__cvta_generic_to_shared(smem));
+  const unsigned bar = static_cast<unsigned>(__cvta_generic_to_shared(bars));
 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const unsigned cluster = a.cluster, rank = cluster > 1 ? cluster_rank() : 0;
-  const int64_t tile = blockIdx.x / cluster;
-  const int64_t b = tile / a.dtiles, d0 = (tile - b * a.dtiles) * C::kChannels;
-  const int64_t rounds = (a.nchunks + cluster - 1) / cluster;
+  const Place p = place_of<C::kChannels>(a);
   grid_dependency_wait();
+  const Strip<T> gt = strip_of<T, LAYOUT, SKEW>(a.gate, p.b, p.d0), xt = strip_of<T, LAYOUT, SKEW>(a.x, p.b, p.d0);
+  const Strip<T> yt = strip_of<T, LAYOUT, SKEW>(a.dout, p.b, p.d0), zt = Z ? strip_of<T, LAYOUT, SKEW>(a.z, p.b, p.d0) : gt;
+  const Strip<T> dxt = strip_of<T, LAYOUT, SKEW>(a.dx, p.b, p.d0), dgt = strip_of<T, LAYOUT, SKEW>(a.dgate, p.b, p.d0);
+  const Strip<T> dzt = Z ? strip_of<T, LAYOUT, SKEW>(a.dz, p.b, p.d0) : dgt;
+  const int nch = p.nd - lane * V;
 
-  const T* const xp = static_cast<const T*>(a.x.data) + b * a.x.s0;
-  const T* const gp = static_cast<const T*>(a.gate.data) + b * a.gate.s0;
-  const T* const yp = static_cast<const T*>(a.dout.data) + b * a.dout.s0;
-  const T* const zp = Z ? static_cast<const T*>(a.z.data) + b * a.z.s0 : nullptr;
-  T* const dxp = static_cast<T*>(a.dx.data) + b * a.dx.s0;
-  T* const dgp = static_cast<T*>(a.dgate.data) + b * a.dgate.s0;
-  T* const dzp = Z ? static_cast<T*>(a.dz.data) + b * a.dz.s0 : nullptr;
-  const int dl = lane_channel<T, LAYOUT>(lane, 0);
-  const int nch = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(V), a.dim - d0 - dl)));
-
-  auto chunk_of = [&](int64_t k) { return (rounds - 1 - k) * cluster + rank; };
-  auto load = [&](int64_t k) {
-    const int64_t c = chunk_of(k);
-    if (k < rounds && c < a.nchunks) {
-      unsigned char* t = ring + (k % S) * NT * C::kBytes;
-      load_tile<T, LAYOUT>(t, gp, a.gate.s1, a.gate.s2, d0, c * kRecChunk, a.dim, a.seqlen, a.packed);
-      load_tile<T, LAYOUT>(t + C::kBytes, xp, a.x.s1, a.x.s2, d0, c * kRecChunk, a.dim, a.seqlen, a.packed);
-      load_tile<T, LAYOUT>(t + 2 * C::kBytes, yp, a.dout.s1, a.dout.s2, d0, c * kRecChunk, a.dim, a.seqlen, a.packed);
-      if constexpr (Z) load_tile<T, LAYOUT>(t + 3 * C::kBytes, zp, a.z.s1, a.z.s2, d0, c * kRecChunk, a.dim, a.seqlen, a.packed);
+  auto chunk_of = [&](int k) { return static_cast<int64_t>(p.rounds - 1 - k) * p.cluster + p.rank; };
+  int load_slot = 0;
+  auto load = [&](int k) {
+    const int64_t t0 = chunk_of(k) * kRecChunk;
+    const int nt = within(t0, a.seqlen, kRecChunk), o = load_slot * NT * C::kBytes;
+    if (k < p.rounds && nt > 0) {
+      load_tile<T, LAYOUT, SKEW>(ring + o, smem + o, gt, t0, p.nd, nt, a.packed);
+      load_tile<T, LAYOUT, SKEW>(ring + o + C::kBytes, smem + o + C::kBytes, xt, t0, p.nd, nt, a.packed);
+      load_tile<T, LAYOUT, SKEW>(ring + o + 2 * C::kBytes, smem + o + 2 * C::kBytes, yt, t0, p.nd, nt, a.packed);
+      if constexpr (Z) load_tile<T, LAYOUT, SKEW>(ring + o + 3 * C::kBytes, smem + o + 3 * C::kBytes, zt, t0, p.nd, nt, a.packed);
     }
     cp_async_commit();
+    if (++load_slot == S) load_slot = 0;
   };
-  auto store = [&](int64_t k) {  // rows: the gradients of round k, from the tiles they replaced
-    const int64_t c = chunk_of(k);
-    if (c >= a.nchunks) return;
-    const unsigned char* t = ring + (k % S) * NT * C::kBytes;
+  auto store = [&](int k, const unsigned char* t) {  // rows: the gradients of round k, from the tiles they replaced
     if constexpr (C::kRows) {
-      store_tile<T>(t, dgp, a.dgate.s1, a.dgate.s2, d0, c * kRecChunk, a.dim, a.seqlen, a.packed);
-      store_tile<T>(t + C::kBytes, dxp, a.dx.s1, a.dx.s2, d0, c * kRecChunk, a.dim, a.seqlen, a.packed);
-      if constexpr (Z) store_tile<T>(t + 3 * C::kBytes, dzp, a.dz.s1, a.dz.s2, d0, c * kRecChunk, a.dim, a.seqlen, a.packed);
+      const int64_t t0 = chunk_of(k) * kRecChunk;
+      const int nt = within(t0, a.seqlen, kRecChunk);
+      store_tile<T, SKEW>(t, dgt, t0, p.nd, nt, a.packed);
+      store_tile<T, SKEW>(t + C::kBytes, dxt, t0, p.nd, nt, a.packed);
+      if constexpr (Z) store_tile<T, SKEW>(t + 3 * C::kBytes, dzt, t0, p.nd, nt, a.packed);
     }
   };
-  auto checkpoint = [&](int64_t k) {
+  auto checkpoint = [&](int k) {
     L r = splat(0.f, L{});
     const int64_t c = chunk_of(k);
-    if (k < rounds && c < a.nchunks) {
+    if (k < p.rounds && c < a.nchunks) {
+      const float* from = a.checkpoints + (p.b * a.nchunks + c) * a.dim + p.d0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int64_t d = d0 + lane_channel<T, LAYOUT>(lane, i);
-        if (d < a.dim) el(r, i) = __ldg(a.checkpoints + (b * a.nchunks + c) * a.dim + d);
+        const int d = lane_channel<T, LAYOUT>(lane, i);
+        if (d < p.nd) el(r, i) = __ldg(from + d);
       }
     }
     return r;
   };
 #pragma unroll
   for (int k = 0; k < S - 1; ++k) load(k);
-  if (cluster > 1) {  // the others' shared memory may be written once they have all begun
-    cluster_arrive();
-    cluster_wait();
+  if (p.cluster > 1) {
+    if (threadIdx.x == 0) {
+      mbar_init(bar);
+      mbar_init(bar + 8);
+      mbar_init_done();
+    }
+    cluster_sync();
   }
-  const L nb = gate_offset<T, LAYOUT>(a, d0, lane);
-  L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.dfinal, b, a.nstates, d0, a.dim, lane);
+  const L nb = gate_offset<T, LAYOUT>(a, p.d0, lane);
+  L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.dfinal, p.b, a.nstates, p.d0, a.dim, lane);
+  if (w == 0) handed[0][lane] = carry;
   L start = checkpoint(0);
-  int ids = SEQ ? load_ids(a, b, chunk_of(0) * kRecChunk + w * kRecSteps, lane) : 0;
+  int ids = SEQ ? load_ids(a, p.b, chunk_of(0) * kRecChunk + w * kRecSteps, lane) : 0;
   L bias_sum = splat(0.f, L{});
 
-  for (int64_t k = 0; k < rounds; ++k) {
+  int slot = 0;
+  for (int k = 0; k < p.rounds; ++k) {
     const int64_t t0 = chunk_of(k) * kRecChunk, tw = t0 + w * kRecSteps;
-    unsigned char* const now = ring + (k % S) * NT * C::kBytes;
-    const int buf = static_cast<int>(k & 1);
+    const int left = within(tw, a.seqlen, kRecSteps);
+    unsigned char* const now = smem + slot * NT * C::kBytes;
+    const int buf = k & 1;
     cp_async_wait<S - 2>();
     if constexpr (C::kRows) {
       __syncthreads();
-      if (k > 0) store(k - 1);
+      if (k > 0) {
+        store(k - 1, smem + (slot == 0 ? S - 1 : slot - 1) * NT * C::kBytes);
+        if constexpr (SKEW) __syncthreads();
+      }
     } else {
       __syncwarp();
     }
@@ -369,14 +412,14 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a
     L ga[kRecSteps], gc[kRecSteps], x[kRecSteps], gy[kRecSteps], dz[kRecSteps];
     {
       L g[kRecSteps];
-      read_steps<T, LAYOUT>(now, w, lane, g);
+      read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, g);
       gates<T, V>(g, nb, ga, gc);
     }
-    read_steps<T, LAYOUT>(now + C::kBytes, w, lane, x);
-    read_steps<T, LAYOUT>(now + 2 * C::kBytes, w, lane, gy);
+    read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, x);
+    read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, yt, t0, w, lane, gy);
     if constexpr (Z) {
       L z[kRecSteps];
-      read_steps<T, LAYOUT>(now + 3 * C::kBytes, w, lane, z);
+      read_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, t0, w, lane, z);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
         L s, d;
@@ -387,29 +430,29 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a
       }
     }
     Edges e;
-    unsigned valid = below(tw, a.seqlen);
+    unsigned valid = below(left);
     if constexpr (SEQ) {
       e = edges_of(ids);
       valid = e.valid;
-      ids = load_ids(a, b, tw - static_cast<int64_t>(cluster) * kRecChunk, lane);
+      ids = load_ids(a, p.b, tw - static_cast<int64_t>(p.cluster) * kRecChunk, lane);
     }
     const bool whole = valid == 0xffu && !(SEQ && (e.first || e.last));
-    L A, H, R, B;
+    Map<V> f, r;  // h -> A h + H forward through the positions, s -> A s + H back
     if (whole) {
-      A = ga[0];
-      H = mul(gc[0], x[0]);
+      f.A = ga[0];
+      f.H = mul(gc[0], x[0]);
 #pragma unroll
       for (int j = 1; j < kRecSteps; ++j) {
-        A = mul(ga[j], A);
-        H = fma(ga[j], H, mul(gc[j], x[j]));
+        f.A = mul(ga[j], f.A);
+        f.H = fma(ga[j], f.H, mul(gc[j], x[j]));
       }
-      B = mul(ga[kRecSteps - 1], gy[kRecSteps - 1]);
+      r.H = mul(ga[kRecSteps - 1], gy[kRecSteps - 1]);
 #pragma unroll
-      for (int j = kRecSteps - 2; j >= 0; --j) B = mul(ga[j], add(gy[j], B));
-      R = A;
+      for (int j = kRecSteps - 2; j >= 0; --j) r.H = mul(ga[j], add(gy[j], r.H));
+      r.A = f.A;
     } else {
-      A = R = splat(1.f, L{});
-      H = B = splat(0.f, L{});
+      f.A = r.A = splat(1.f, L{});
+      f.H = r.H = splat(0.f, L{});
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
         if (!(valid >> j & 1u)) {
@@ -417,75 +460,38 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a
           gc[j] = x[j] = gy[j] = splat(0.f, L{});
         }
         if (SEQ && (e.first >> j & 1u)) {
-          H = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, d0, a.dim, lane);
-          A = splat(-1.f, L{});
+          f.H = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
+          f.A = splat(-1.f, L{});
         }
-        A = mul(ga[j], A);
-        H = fma(ga[j], H, mul(gc[j], x[j]));
+        f.A = mul(ga[j], f.A);
+        f.H = fma(ga[j], f.H, mul(gc[j], x[j]));
       }
 #pragma unroll
       for (int j = kRecSteps - 1; j >= 0; --j) {
         if (SEQ && (e.last >> j & 1u)) {
-          B = load_state<T, LAYOUT>(a.dfinal, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, d0, a.dim, lane);
-          R = splat(-1.f, L{});
+          r.H = load_state<T, LAYOUT>(a.dfinal, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
+          r.A = splat(-1.f, L{});
         }
-        R = mul(ga[j], R);
-        B = mul(ga[j], add(gy[j], B));
+        r.A = mul(ga[j], r.A);
+        r.H = mul(ga[j], add(gy[j], r.H));
       }
     }
-    sumA[(buf * kRecWarps + w) * 32 + lane] = A;
-    sumH[(buf * kRecWarps + w) * 32 + lane] = H;
-    sumS[(buf * kRecWarps + w) * 32 + lane] = B;
-    if constexpr (SEQ) sumR[(buf * kRecWarps + w) * 32 + lane] = R;
+    Map<V>* const ahead = sums + 2 * buf * kRecWarps * 32;
+    Map<V>* const back = ahead + kRecWarps * 32;
+    ahead[w * 32 + lane] = f;
+    back[w * 32 + lane] = r;
     __syncthreads();
-
-    L h = start;
-#pragma unroll
-    for (int q = 0; q < kRecWarps - 1; ++q)
-      if (q < w) h = apply<V, SEQ>(sumA[(buf * kRecWarps + q) * 32 + lane], sumH[(buf * kRecWarps + q) * 32 + lane], h);
+    L h = through_warps<V, SEQ, true>(ahead, w, lane, start);
     start = checkpoint(k + 1);
-    L s = carry;
-    if (cluster == 1) {
-      L p = carry;
-#pragma unroll
-      for (int q = kRecWarps - 1; q >= 0; --q) {
-        if (q == w) s = p;
-        p = apply<V, SEQ>(sumR[(buf * kRecWarps + q) * 32 + lane], sumS[(buf * kRecWarps + q) * 32 + lane], p);
-      }
-      carry = p;
-    } else {
-      L pr = splat(1.f, L{}), ps = splat(0.f, L{}), wr = pr, ws = ps;
-#pragma unroll
-      for (int q = kRecWarps - 1; q >= 0; --q) {
-        if (q == w) wr = pr, ws = ps;
-        const L qr = sumR[(buf * kRecWarps + q) * 32 + lane];
-        ps = apply<V, SEQ>(qr, sumS[(buf * kRecWarps + q) * 32 + lane], ps);
-        pr = chain<V, SEQ>(qr, pr);
-      }
-      for (unsigned r = w; r < cluster; r += kRecWarps) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          store_remote(&el(farR[(buf * cluster + rank) * 32 + lane], i), r, el(pr, i));
-          store_remote(&el(farS[(buf * cluster + rank) * 32 + lane], i), r, el(ps, i));
-        }
-      }
-      cluster_arrive();
-      cluster_wait();
-      L p = carry;
-      for (int r = static_cast<int>(cluster) - 1; r >= 0; --r) {
-        if (r == static_cast<int>(rank)) s = p;
-        p = apply<V, SEQ>(farR[(buf * cluster + r) * 32 + lane], farS[(buf * cluster + r) * 32 + lane], p);
-      }
-      carry = p;
-      s = apply<V, SEQ>(wr, ws, s);
-    }
+    L s = p.cluster == 1 ? through_warps<V, SEQ, false>(back, w, lane, handed[buf][lane])
+                         : through_cluster<V, SEQ, false>(back, far + buf * p.cluster * 32, bar + 8 * buf, (k >> 1) & 1, p, w, lane, carry);
 
     // forward through the positions: h before each, and dz
     L prev[kRecSteps];
 #pragma unroll
     for (int j = 0; j < kRecSteps; ++j) {
       if (SEQ && !whole && (e.first >> j & 1u))
-        h = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, d0, a.dim, lane);
+        h = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
       prev[j] = h;
       h = fma(ga[j], h, mul(gc[j], x[j]));
       if constexpr (Z) dz[j] = mul(dz[j], h);
@@ -494,7 +500,7 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a
 #pragma unroll
     for (int j = kRecSteps - 1; j >= 0; --j) {
       if (SEQ && !whole && (e.last >> j & 1u))
-        s = load_state<T, LAYOUT>(a.dfinal, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, d0, a.dim, lane);
+        s = load_state<T, LAYOUT>(a.dfinal, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
       const L dh = add(gy[j], s);
       gy[j] = mul(dh, gc[j]);
       s = mul(ga[j], dh);
@@ -505,40 +511,40 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a
       }
       bias_sum = add(bias_sum, prev[j]);
       if (SEQ && !whole && (e.first >> j & 1u))
-        store_state<T, LAYOUT>(a.dinit, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, d0, a.dim, lane, s);
+        store_state<T, LAYOUT>(a.dinit, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane, s);
     }
+    if (p.cluster == 1 && w == 0) handed[buf ^ 1][lane] = s;
     if constexpr (C::kRows) {
-      write_steps<T, LAYOUT>(now, w, lane, prev);
-      write_steps<T, LAYOUT>(now + C::kBytes, w, lane, gy);
-      if constexpr (Z) write_steps<T, LAYOUT>(now + 3 * C::kBytes, w, lane, dz);
+      write_steps<T, SKEW>(now, w, lane, prev);
+      write_steps<T, SKEW>(now + C::kBytes, w, lane, gy);
+      if constexpr (Z) write_steps<T, SKEW>(now + 3 * C::kBytes, w, lane, dz);
     } else {
-      const int64_t d = d0 + dl;
-#pragma unroll
-      for (int j = 0; j < kRecSteps; ++j) {
-        if (tw + j >= a.seqlen) break;
-        store_step<T>(dxp + d * a.dx.s1 + (tw + j) * a.dx.s2, a.dx.s1, nch, a.packed, gy[j]);
-        store_step<T>(dgp + d * a.dgate.s1 + (tw + j) * a.dgate.s2, a.dgate.s1, nch, a.packed, prev[j]);
-        if constexpr (Z) store_step<T>(dzp + d * a.dz.s1 + (tw + j) * a.dz.s2, a.dz.s1, nch, a.packed, dz[j]);
-      }
+      store_steps<T, SKEW>(dxt, tw, lane, nch, left, a.packed, gy);
+      store_steps<T, SKEW>(dgt, tw, lane, nch, left, a.packed, prev);
+      if constexpr (Z) store_steps<T, SKEW>(dzt, tw, lane, nch, left, a.packed, dz);
     }
+    if (++slot == S) slot = 0;
   }
   __syncthreads();
-  if constexpr (C::kRows) store(rounds - 1);
-  if (!SEQ && w == 0 && rank == 0) store_state<T, LAYOUT>(a.dinit, b, a.nstates, d0, a.dim, lane, carry);
+  if constexpr (C::kRows) store(p.rounds - 1, smem + (slot == 0 ? S - 1 : slot - 1) * NT * C::kBytes);
+  if (!SEQ && w == 0 && p.rank == 0)
+    store_state<T, LAYOUT>(a.dinit, p.b, a.nstates, p.d0, a.dim, lane, p.cluster == 1 ? handed[p.rounds & 1][lane] : carry);
   if (a.dbias) {
-    sumA[w * 32 + lane] = bias_sum;
+    L* const sum = reinterpret_cast<L*>(sums);
+    sum[w * 32 + lane] = bias_sum;
     __syncthreads();
     if (w == 0) {
-      L sum = sumA[lane];
+      L total = sum[lane];
 #pragma unroll
-      for (int q = 1; q < kRecWarps; ++q) sum = add(sum, sumA[q * 32 + lane]);
+      for (int q = 1; q < kRecWarps; ++q) total = add(total, sum[q * 32 + lane]);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int64_t d = d0 + lane_channel<T, LAYOUT>(lane, i);
-        if (d < a.dim) a.partials[(b * cluster + rank) * a.dim + d] = el(sum, i);
+        const int64_t d = p.d0 + lane_channel<T, LAYOUT>(lane, i);
+        if (d < a.dim) a.partials[(p.b * p.cluster + p.rank) * a.dim + d] = el(total, i);
       }
     }
   }
+  if (p.cluster > 1) cluster_sync();
 }
 
 // dbias[d] = the tiles' partial sums added up in order.
@@ -587,14 +593,14 @@ __global__ void __launch_bounds__(kThreads) rec_update_kernel(const RecUpdateArg
 
 unsigned blocks_for(int64_t threads) { return static_cast<unsigned>((threads + kThreads - 1) / kThreads); }
 
-template <typename T, int LAYOUT, bool BWD, bool SEQ, bool Z>
+template <typename T, int LAYOUT, bool SKEW, bool BWD, bool SEQ, bool Z>
 cudaError_t run(const RecArgs& a, cudaStream_t s) {
-  using C = Tile<T, LAYOUT>;
+  using C = Tile<T, LAYOUT, SKEW>;
   constexpr int NT = (BWD ? 3 : 2) + (Z ? 1 : 0);
   constexpr int stages = BWD ? kBwdStages<LAYOUT> : kFwdStages;
-  constexpr int sums = BWD ? (SEQ ? 4 : 3) : 2;
-  const size_t smem = static_cast<size_t>(stages) * NT * C::kBytes + sizeof(Lane<C::V>) * 32 * 2 * (sums * kRecWarps + (a.cluster > 1 ? 2 * a.cluster : 0));
-  auto kernel = BWD ? rec_bwd_kernel<T, LAYOUT, SEQ, Z> : rec_fwd_kernel<T, LAYOUT, SEQ, Z>;
+  const size_t smem = static_cast<size_t>(stages) * NT * C::kBytes +
+                      sizeof(Map<C::V>) * 32 * 2 * ((BWD ? 2 : 1) * kRecWarps + (a.cluster > 1 ? a.cluster : 0));
+  auto kernel = BWD ? rec_bwd_kernel<T, LAYOUT, SKEW, SEQ, Z> : rec_fwd_kernel<T, LAYOUT, SKEW, SEQ, Z>;
   const void* ptr = reinterpret_cast<const void*>(kernel);
   cudaError_t e = allow_dynamic_smem(ptr, smem);
   if (e == cudaSuccess && a.cluster > 8) e = cudaFuncSetAttribute(ptr, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -615,10 +621,18 @@ cudaError_t run(const RecArgs& a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-template <typename T, int LAYOUT, bool BWD>
+template <typename T, int LAYOUT, bool SKEW, bool BWD>
+cudaError_t pick_options(const RecArgs& a, cudaStream_t s) {
+  if (a.seq_idx.data)
+    return a.z.data ? run<T, LAYOUT, SKEW, BWD, true, true>(a, s) : run<T, LAYOUT, SKEW, BWD, true, false>(a, s);
+  return a.z.data ? run<T, LAYOUT, SKEW, BWD, false, true>(a, s) : run<T, LAYOUT, SKEW, BWD, false, false>(a, s);
+}
+template <typename T, bool BWD>
 cudaError_t pick(const RecArgs& a, cudaStream_t s) {
-  if (a.seq_idx.data) return a.z.data ? run<T, LAYOUT, BWD, true, true>(a, s) : run<T, LAYOUT, BWD, true, false>(a, s);
-  return a.z.data ? run<T, LAYOUT, BWD, false, true>(a, s) : run<T, LAYOUT, BWD, false, false>(a, s);
+  if constexpr (sizeof(T) == 2) {
+    if (a.skew) return a.rows ? pick_options<T, kLayoutRows, true, BWD>(a, s) : pick_options<T, kLayoutChannelLast, true, BWD>(a, s);
+  }
+  return a.rows ? pick_options<T, kLayoutRows, false, BWD>(a, s) : pick_options<T, kLayoutChannelLast, false, BWD>(a, s);
 }
 
 }  // namespace
@@ -626,10 +640,10 @@ cudaError_t pick(const RecArgs& a, cudaStream_t s) {
 using DT = CC1D_DT_TYPE;
 
 cudaError_t CC1D_DT_NAME(rec_fwd)(const RecArgs& a, cudaStream_t s) {
-  return a.rows ? pick<DT, kLayoutRows, false>(a, s) : pick<DT, kLayoutChannelLast, false>(a, s);
+  return pick<DT, false>(a, s);
 }
 cudaError_t CC1D_DT_NAME(rec_bwd)(const RecArgs& a, cudaStream_t s) {
-  cudaError_t e = a.rows ? pick<DT, kLayoutRows, true>(a, s) : pick<DT, kLayoutChannelLast, true>(a, s);
+  cudaError_t e = pick<DT, true>(a, s);
   if (e == cudaSuccess && a.dbias) e = launch_dependent(rec_bias_kernel, dim3(blocks_for(a.dim)), dim3(kThreads), 0, s, a);
   return e;
 }
