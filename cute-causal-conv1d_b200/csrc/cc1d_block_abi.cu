@@ -40,9 +40,8 @@ bool sizes_ok(int64_t a, int64_t b, int64_t c) {
          static_cast<double>(a) * static_cast<double>(b) * static_cast<double>(c) < 4e18;
 }
 
-template <typename Args>
-cudaError_t by_type(int dtype, const Args& a, cudaStream_t s, cudaError_t (*f32)(const Args&, cudaStream_t),
-                    cudaError_t (*f16)(const Args&, cudaStream_t), cudaError_t (*bf16)(const Args&, cudaStream_t)) {
+template <typename Args, typename Fn>
+cudaError_t by_type(int dtype, Args& a, cudaStream_t s, Fn f32, Fn f16, Fn bf16) {
   switch (dtype) {
     case CC1D_FLOAT32: return f32(a, s);
     case CC1D_FLOAT16: return f16(a, s);
@@ -51,14 +50,11 @@ cudaError_t by_type(int dtype, const Args& a, cudaStream_t s, cudaError_t (*f32)
 }
 
 // ------------------------------------------------------------------ recurrence plan
-// Unit stride along the layout's dimension, the others not negative and small enough for a
-// 32-bit byte offset within a tile.
+// Unit stride along the layout's dimension, the other strides not negative.
 bool strips_ok(const TensorArg& t, const RecArgs& a) {
   if (!t.data) return true;
-  const int64_t size = t.dtype == CC1D_FLOAT32 ? 4 : 2;
   const int64_t unit = a.rows ? t.s2 : t.s1, step = a.rows ? t.s1 : t.s2;
-  const bool steps = (a.rows ? a.dim : a.seqlen) > 1;
-  return (unit == 1 || (a.rows ? a.seqlen : a.dim) == 1) && t.s0 >= 0 && (!steps || (step >= 0 && step < (int64_t{1} << 32) / 64 / size));
+  return (unit == 1 || (a.rows ? a.seqlen : a.dim) == 1) && t.s0 >= 0 && ((a.rows ? a.dim : a.seqlen) <= 1 || step >= 0);
 }
 // Every strip of it starts on a 16-byte boundary.
 bool packets_ok(const TensorArg& t, const RecArgs& a) {
@@ -79,20 +75,22 @@ int sm_count() {
   return n;
 }
 
-// CTAs that share a tile.  Each takes 1/cluster of the chunks; two CTAs fit an SM.  The
-// estimate counts chunk times: a CTA pays its start (about 3 chunks until its first tiles
-// are there), a cluster's barrier lengthens a chunk by a fifth, and an SM with one CTA
-// takes 0.6 of the time that two need for a chunk each.
-int choose_cluster(int64_t tiles, int64_t chunks) {
-  const int64_t sms = sm_count(), slots = 2 * sms;
+// CTAs that share a tile.  Each takes 1/cluster of the chunks.  The estimate counts chunk
+// times: a CTA pays its start (about 3 chunks until its first tiles are there), a cluster's
+// exchange lengthens a chunk by a fifth, and an SM with one CTA takes 0.6 of the time that two
+// need for a chunk each.  Two CTAs fit an SM while their shared memory (`smem`, and 1 KB for
+// each CTA of the cluster) does.
+int choose_cluster(int64_t tiles, int64_t chunks, int64_t smem) {
+  const int64_t sms = sm_count();
   double best = 0;
   int pick = 1;
   for (int c = 1; c <= 16 && c <= chunks; c *= 2) {
-    const int64_t ctas = tiles * c, rest = ctas % slots;
+    const bool two = smem + (c > 1 ? c * 1024 : 0) <= 113 * 1024;
+    const int64_t ctas = tiles * c, slots = two ? 2 * sms : sms, rest = ctas % slots;
     const double per_cta = (static_cast<double>((chunks + c - 1) / c) + 3.0) * (c > 1 ? 1.2 : 1.0);
-    const double cost = per_cta * (static_cast<double>(ctas / slots) + (rest == 0 ? 0.0 : rest <= sms ? 0.6 : 1.0));
-    if (c == 1 || cost < best) {
-      best = cost;
+    const double waves = static_cast<double>(ctas / slots) * (two ? 1.0 : 0.6) + (rest == 0 ? 0.0 : rest <= sms ? 0.6 : 1.0);
+    if (c == 1 || per_cta * waves < best) {
+      best = per_cta * waves;
       pick = c;
     }
   }
@@ -111,19 +109,18 @@ cc1d_status rec_plan(RecArgs* a, bool bwd) {
     rows = rows && (t->s2 == 1 || a->seqlen == 1);
   }
   a->rows = rows && (!last || a->dim == 1);
-  bool strips = true;
-  a->packed = true;
+  bool strips = true, packets = true;
   for (const TensorArg* t : all) {
     if (!t) continue;
     strips = strips && strips_ok(*t, *a);
-    a->packed = a->packed && packets_ok(*t, *a);
+    packets = packets && packets_ok(*t, *a);
   }
-  a->packed = a->packed && strips;
-  a->skew = strips && !a->packed && a->x.dtype != CC1D_FLOAT32;
+  a->move = !strips ? kElements : packets ? kTma : a->x.dtype != CC1D_FLOAT32 ? kWords : kElements;
   const int64_t channels = a->x.dtype == CC1D_FLOAT32 ? 32 : 64;
   a->dtiles = (a->dim + channels - 1) / channels;
   const int64_t tiles = a->batch * a->dtiles;
-  a->cluster = choose_cluster(tiles, a->nchunks);
+  const int64_t tile = 8192 + (a->move == kWords ? 256 : 0), z = a->z.data ? 1 : 0;
+  a->cluster = choose_cluster(tiles, a->nchunks, bwd ? 3 * (3 + z) * tile + 13 * 1024 : 4 * (2 + z) * tile + 9 * 1024);
   if (tiles * a->cluster > kMax31) return fail(CC1D_ERR_VALUE, "batch * dim is too large");
   return CC1D_OK;
 }

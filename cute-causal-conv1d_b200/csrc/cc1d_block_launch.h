@@ -16,12 +16,16 @@ struct RecArgs {
   float* checkpoints;
   float* partials;  // backward: (batch * cluster, dim) sums of dgate to add up for dbias
   // the plan (rec_plan): tiles of channels, CTAs that share one, memory layout, and how the
-  // tensors move: in 16-byte packets, in 4-byte words that may cut an element's pair in two
-  // (skew, 16-bit types), or else element by element
+  // tensors move
   int64_t dtiles;
-  int cluster;
-  bool rows, packed, skew;
+  int cluster, move;
+  bool rows;
 };
+
+// How the recurrence's tensors move (RecArgs::move).  kTma: the TMA copies whole tiles both
+// ways (strips aligned to 16 bytes).  kWords: 4-byte words by cp.async, for strips of 16-bit
+// elements that may start in the middle of a word.  kElements: one by one, any strides.
+constexpr int kTma = 0, kWords = 1, kElements = 2;
 
 struct RecUpdateArgs {
   int64_t batch, dim, seqlen, nstates;
@@ -47,8 +51,13 @@ struct AddNormArgs {
   cudaError_t name##_f16(const Args&, cudaStream_t);   \
   cudaError_t name##_bf16(const Args&, cudaStream_t);
 
-CC1D_DECLARE(rec_fwd, RecArgs)
-CC1D_DECLARE(rec_bwd, RecArgs)
+// (RecArgs is changed only where a tensor turns out not to be one that the TMA can describe)
+cudaError_t rec_fwd_f32(RecArgs&, cudaStream_t);
+cudaError_t rec_fwd_f16(RecArgs&, cudaStream_t);
+cudaError_t rec_fwd_bf16(RecArgs&, cudaStream_t);
+cudaError_t rec_bwd_f32(RecArgs&, cudaStream_t);
+cudaError_t rec_bwd_f16(RecArgs&, cudaStream_t);
+cudaError_t rec_bwd_bf16(RecArgs&, cudaStream_t);
 CC1D_DECLARE(rec_update, RecUpdateArgs)
 CC1D_DECLARE(add_norm_fwd, AddNormArgs)
 CC1D_DECLARE(add_norm_bwd, AddNormArgs)

@@ -34,19 +34,16 @@ __device__ __forceinline__ void sigmoid_pair(float u, float& a, float& c) {
   c = e * a;
 }
 
+// sigmoid(z) alone needs no clamp: 1 / (1 + inf) is 0.
+template <typename T>
+__device__ __forceinline__ float sigmoid_of(float z) {
+  if constexpr (std::is_same<T, float>::value) return __frcp_rn(1.f + expf(-z));
+  else return rcp_approx(1.f + ex2_approx(-kLog2e * z));
+}
 template <typename T>
 __device__ __forceinline__ float silu_of(float z) {
-  return z * reciprocal<T>(1.f + exp_minus<T>(z));
+  return z * sigmoid_of<T>(z);
 }
-// silu(z) and its derivative sigmoid(z) (1 + z sigmoid(-z)).
-template <typename T>
-__device__ __forceinline__ void silu_and_grad(float z, float& s, float& ds) {
-  float p, q;
-  sigmoid_pair<T>(z, p, q);
-  s = z * p;
-  ds = p * fmaf(z, q, 1.f);
-}
-
 // ---------------------------------------------------------------------- Philox4x32-10
 // Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3" (2011):
 // four 32-bit words for a 128-bit counter under a 64-bit key.

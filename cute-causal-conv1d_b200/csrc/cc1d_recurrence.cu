@@ -21,14 +21,16 @@
 // take consecutive chunks and exchange the chunks' sums through distributed shared memory,
 // one cluster barrier per round.  No CTA waits for another outside its cluster, and results
 // do not depend on timing.
+#include <cudaTypedefs.h>
+
 #include "cc1d_recurrence.cuh"
 
 namespace cc1d {
 namespace {
 
-// Ring slots: chunks in flight and the one in work.
-constexpr int kFwdStages = 3;
-template <int LAYOUT> constexpr int kBwdStages = LAYOUT == kLayoutRows ? 2 : 3;
+// Ring slots: the chunk in work, the one before, whose results are still being stored from its
+// tiles, and one (backward) or two chunks that are being loaded.
+constexpr int kFwdStages = 4, kBwdStages = 3;
 
 // exp(-(gate + bias)), at most 1e30; nb is -bias log2(e) for 16-bit tensors, else the bias.
 template <typename T>
@@ -88,39 +90,56 @@ __device__ __forceinline__ Place place_of(const RecArgs& a) {
   return p;
 }
 
+// What the warps of a CTA tell each other about their positions: the product A of the a's, H
+// with h -> A h + H forward through them (and B with s -> A s + B back), and whether a
+// sequence starts (ends) among them: the map is then constant, also for an h that is infinite
+// or NaN.
+template <int V> struct Sums {
+  Lane<V> A[kRecWarps * 32], H[kRecWarps * 32];
+  unsigned cut[kRecWarps];
+};
+template <int V> struct SumsBack {
+  Lane<V> B[kRecWarps * 32];
+  unsigned cut[kRecWarps];
+};
+__device__ __forceinline__ unsigned cuts_of(const unsigned* cut, int lane) {
+  return __ballot_sync(0xffffffffu, lane < kRecWarps && cut[lane & (kRecWarps - 1)]);
+}
+
 // The maps of the warps before warp w (FORWARD: lower warps first) after each other, applied to h.
 template <int V, bool SEQ, bool FORWARD>
-__device__ __forceinline__ Lane<V> through_warps(const Map<V>* sums, int w, int lane, Lane<V> h) {
+__device__ __forceinline__ Lane<V> through_warps(const Lane<V>* A, const Lane<V>* H, unsigned cuts, int w, int lane, Lane<V> h) {
 #pragma unroll
   for (int i = 0; i < kRecWarps - 1; ++i) {
     const int q = FORWARD ? i : kRecWarps - 1 - i;
-    const Map<V> m = sums[q * 32 + lane];
-    const Lane<V> r = apply<V, SEQ>(m.A, m.H, h);
+    const Lane<V> c = H[q * 32 + lane];
+    Lane<V> r = fma(A[q * 32 + lane], h, c);
+    if (SEQ && (cuts >> q & 1u)) r = c;
     if (FORWARD ? q < w : q > w) h = r;
   }
   return h;
 }
 
-// The state that warp w's positions start from, for a CTA of a cluster.  Takes the CTA's maps,
-// sends their composition to the cluster's CTAs and joins theirs; `carry` is the state the
-// round starts from, and becomes the one that the next starts from.
+// The state that warp w's positions start from, for a CTA of a cluster.  Sends the composition
+// of the CTA's maps to the cluster's CTAs and joins theirs; `carry` is the state the round
+// starts from, and becomes the one that the next starts from.
 template <int V, bool SEQ, bool FORWARD>
-__device__ __forceinline__ Lane<V> through_cluster(const Map<V>* sums, Map<V>* far, unsigned bar, unsigned parity, const Place& p,
-                                                   int w, int lane, Lane<V>& carry) {
-  Map<V> all, mine;
+__device__ __forceinline__ Lane<V> through_cluster(const Lane<V>* A, const Lane<V>* H, unsigned cuts, Map<V>* far, unsigned bar,
+                                                   unsigned parity, const Place& p, int w, int lane, Lane<V>& carry) {
+  Map<V> all;
   all.A = splat(1.f, Lane<V>{});
   all.H = splat(0.f, Lane<V>{});
-  mine = all;
 #pragma unroll
   for (int i = 0; i < kRecWarps; ++i) {
     const int q = FORWARD ? i : kRecWarps - 1 - i;
-    if (q == w) mine = all;
-    const Map<V> m = sums[q * 32 + lane];
-    all.H = apply<V, SEQ>(m.A, m.H, all.H);
-    all.A = chain<V, SEQ>(m.A, all.A);
+    const Lane<V> m = A[q * 32 + lane], c = H[q * 32 + lane];
+    all.H = fma(m, all.H, c);
+    if (SEQ && (cuts >> q & 1u)) all.H = c;
+    all.A = mul(m, all.A);
   }
+  if (SEQ && cuts) all.A = splat(-1.f, all.A);
   if (threadIdx.x == 0) mbar_expect(bar, p.cluster * 32 * sizeof(Map<V>));
-  const unsigned slot = static_cast<unsigned>(__cvta_generic_to_shared(far + p.rank * 32 + lane));
+  const unsigned slot = shared_addr(far + p.rank * 32 + lane);
   for (int r = w; r < p.cluster; r += kRecWarps) send_map<V>(slot, bar, r, all);
   // a partner that never answers leaves NaN in the results instead of a hang
   Lane<V> h = mbar_wait(bar, parity) ? carry : splat(__int_as_float(0x7fc00000), carry);
@@ -129,135 +148,169 @@ __device__ __forceinline__ Lane<V> through_cluster(const Map<V>* sums, Map<V>* f
   for (int i = 0; i < p.cluster; ++i) {
     const int r = FORWARD ? i : p.cluster - 1 - i;
     if (r == p.rank) start = h;
-    const Map<V> m = far[r * 32 + lane];
-    h = apply<V, SEQ>(m.A, m.H, h);
+    h = apply<V, SEQ>(far[r * 32 + lane], h);
   }
   carry = h;
-  return apply<V, SEQ>(mine.A, mine.H, start);
+  return through_warps<V, SEQ, FORWARD>(A, H, cuts, w, lane, start);
+}
+
+// What else a CTA keeps in shared memory: without a cluster, the state that one round's last
+// positions hand to the next round; the barriers.
+template <int V> struct Common {
+  Lane<V> handed[2][32];
+  uint64_t bars[kFwdStages + 2];
+};
+
+// The barriers of the ring (one per slot) and of the cluster's exchange (two).
+template <int S>
+__device__ __forceinline__ void start_barriers(unsigned bars, bool tma, int cluster) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(bars + 8 * i, tma ? 1 : 2 * kRecThreads);
+    mbar_init(bars + 8 * S, 1);
+    mbar_init(bars + 8 * S + 8, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (cluster > 1) cluster_sync();  // they are there before a partner's first map arrives
+  else __syncthreads();
 }
 
 template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z>
-__global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const RecArgs a) {
+__global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int V = C::V, NT = Z ? 3 : 2, S = kFwdStages;
   using L = Lane<V>;
-  extern __shared__ __align__(128) unsigned char smem[];
-  // ring of tiles (gate, x, z) | maps of the warps [2][warps][32] | maps of the cluster [2][cluster][32]
-  Map<V>* const sums = reinterpret_cast<Map<V>*>(smem + S * NT * C::kBytes);
-  Map<V>* const far = sums + 2 * kRecWarps * 32;
-  __shared__ L handed[2][32];     // without a cluster: the state after the last warp's positions
-  __shared__ uint64_t bars[2];
-  const unsigned ring = static_cast<unsigned>(__cvta_generic_to_shared(smem));
-  const unsigned bar = static_cast<unsigned>(__cvta_generic_to_shared(bars));
+  extern __shared__ __align__(1024) unsigned char smem[];
+  // ring of tiles (gate, x, z) | sums of the warps [2] | maps of the cluster [2][cluster][32] | common
+  Sums<V>* const sums = reinterpret_cast<Sums<V>*>(smem + S * NT * C::kBytes);
+  Map<V>* const far = reinterpret_cast<Map<V>*>(sums + 2);
+  Common<V>& common = *reinterpret_cast<Common<V>*>(far + (a.cluster > 1 ? 2 * a.cluster * 32 : 0));
+  const unsigned ring = shared_addr(smem), bars = shared_addr(common.bars);
 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const Place p = place_of<C::kChannels>(a);
+  const bool tma = !SKEW && a.move == kTma;
+  start_barriers<S>(bars, tma, p.cluster);
   grid_dependency_wait();
-  const Strip<T> gt = strip_of<T, LAYOUT, SKEW>(a.gate, p.b, p.d0), xt = strip_of<T, LAYOUT, SKEW>(a.x, p.b, p.d0);
-  const Strip<T> zt = Z ? strip_of<T, LAYOUT, SKEW>(a.z, p.b, p.d0) : gt, ot = strip_of<T, LAYOUT, SKEW>(a.out, p.b, p.d0);
-  const int nch = p.nd - lane * V;
+  const Strip<T> gt = strip_of<T>(a.gate, maps.gate, p.b, p.d0), xt = strip_of<T>(a.x, maps.x, p.b, p.d0);
+  const Strip<T> zt = Z ? strip_of<T>(a.z, maps.z, p.b, p.d0) : gt, ot = strip_of<T>(a.out, maps.out, p.b, p.d0);
 
   int load_slot = 0;
-  auto load = [&](int k) {
-    const int64_t t0 = (static_cast<int64_t>(k) * p.cluster + p.rank) * kRecChunk;
-    const int nt = within(t0, a.seqlen, kRecChunk), o = load_slot * NT * C::kBytes;
-    if (k < p.rounds && nt > 0) {
-      load_tile<T, LAYOUT, SKEW>(ring + o, smem + o, gt, t0, p.nd, nt, a.packed);
-      load_tile<T, LAYOUT, SKEW>(ring + o + C::kBytes, smem + o + C::kBytes, xt, t0, p.nd, nt, a.packed);
-      if constexpr (Z) load_tile<T, LAYOUT, SKEW>(ring + o + 2 * C::kBytes, smem + o + 2 * C::kBytes, zt, t0, p.nd, nt, a.packed);
+  auto load = [&](int k) {  // the tiles of round k
+    if (k < p.rounds) {
+      const int64_t t0 = (static_cast<int64_t>(k) * p.cluster + p.rank) * kRecChunk;
+      const int nt = within(t0, a.seqlen, kRecChunk), o = load_slot * NT * C::kBytes;
+      const unsigned bar = bars + 8 * load_slot;
+      if (tma) {
+        if (threadIdx.x == 0) {
+          if (nt > 0) {
+            mbar_expect(bar, NT * C::kBytes);
+            tma_load<T, LAYOUT>(ring + o, gt.map, p.d0, t0, p.b, bar);
+            tma_load<T, LAYOUT>(ring + o + C::kBytes, xt.map, p.d0, t0, p.b, bar);
+            if constexpr (Z) tma_load<T, LAYOUT>(ring + o + 2 * C::kBytes, zt.map, p.d0, t0, p.b, bar);
+          } else {
+            mbar_arrive(bar);
+          }
+        }
+      } else {
+        if (nt > 0) {
+          load_tile<T, LAYOUT, SKEW>(smem + o, gt, t0, p.nd, nt);
+          load_tile<T, LAYOUT, SKEW>(smem + o + C::kBytes, xt, t0, p.nd, nt);
+          if constexpr (Z) load_tile<T, LAYOUT, SKEW>(smem + o + 2 * C::kBytes, zt, t0, p.nd, nt);
+        }
+        mbar_arrive_copies(bar);  // of the asynchronous copies
+        mbar_arrive(bar);         // and of the plain stores
+      }
     }
-    cp_async_commit();
     if (++load_slot == S) load_slot = 0;
   };
-#pragma unroll
-  for (int k = 0; k < S - 1; ++k) load(k);
-  if (p.cluster > 1) {
-    if (threadIdx.x == 0) {
-      mbar_init(bar);
-      mbar_init(bar + 8);
-      mbar_init_done();
+  auto store = [&](int k, int slot) {  // the results of round k, from the tiles of x
+    const int64_t t0 = (static_cast<int64_t>(k) * p.cluster + p.rank) * kRecChunk;
+    const int nt = within(t0, a.seqlen, kRecChunk), o = slot * NT * C::kBytes + C::kBytes;
+    if (tma) {
+      if (threadIdx.x == 0) {
+        if (nt > 0) tma_store<T, LAYOUT>(ring + o, ot.map, p.d0, t0, p.b);
+        tma_commit();
+      }
+    } else if (nt > 0) {
+      store_tile<T, LAYOUT, SKEW>(smem + o, ot, t0, p.nd, nt);
     }
-    cluster_sync();  // the barriers are there before a partner's first map arrives
-  }
+  };
+#pragma unroll
+  for (int k = 0; k < S - 2; ++k) load(k);
   const L nb = gate_offset<T, LAYOUT>(a, p.d0, lane);
   L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.init, p.b, a.nstates, p.d0, a.dim, lane);
-  if (w == 0) handed[0][lane] = carry;
+  if (w == 0) common.handed[0][lane] = carry;
   int ids = SEQ ? load_ids(a, p.b, static_cast<int64_t>(p.rank) * kRecChunk + w * kRecSteps, lane) : 0;
 
   int slot = 0;
+  unsigned parity = 0;
   for (int k = 0; k < p.rounds; ++k) {
     const int64_t c = static_cast<int64_t>(k) * p.cluster + p.rank;
     const int64_t t0 = c * kRecChunk, tw = t0 + w * kRecSteps;
-    const int left = within(tw, a.seqlen, kRecSteps);
     unsigned char* const now = smem + slot * NT * C::kBytes;
     const int buf = k & 1;
-    cp_async_wait<S - 2>();
-    if constexpr (C::kRows) {
-      __syncthreads();
-      if (k > 0) {
-        const int64_t tp = t0 - static_cast<int64_t>(p.cluster) * kRecChunk;
-        store_tile<T, SKEW>(smem + (slot == 0 ? S - 1 : slot - 1) * NT * C::kBytes + C::kBytes, ot, tp, p.nd, within(tp, a.seqlen, kRecChunk), a.packed);
-        if constexpr (SKEW) __syncthreads();
-      }
-    } else {
-      __syncwarp();
-    }
-    load(k + S - 1);
+    const bool there = mbar_wait(bars + 8 * slot, parity);
 
     // the 8 positions' maps and their composition
     L ga[kRecSteps], gb[kRecSteps];
     {
-      L g[kRecSteps], x[kRecSteps], gc[kRecSteps];
+      L g[kRecSteps], x[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, g);
-      gates<T, V>(g, nb, ga, gc);
       read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, x);
+      gates<T, V>(g, nb, ga, g);
 #pragma unroll
-      for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gc[j], x[j]);
+      for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(g[j], x[j]);
+      if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
     }
     Edges e;
-    unsigned valid = below(left);
+    unsigned valid = below(within(tw, a.seqlen, kRecSteps));
     if constexpr (SEQ) {
       e = edges_of(ids);
       valid = e.valid;
       ids = load_ids(a, p.b, tw + static_cast<int64_t>(p.cluster) * kRecChunk, lane);
     }
-    Map<V> m;
+    L A, H;
     const bool whole = valid == 0xffu && !(SEQ && e.first);
     if (whole) {
-      m.A = ga[0];
-      m.H = gb[0];
+      A = ga[0];
+      H = gb[0];
 #pragma unroll
       for (int j = 1; j < kRecSteps; ++j) {
-        m.A = mul(ga[j], m.A);
-        m.H = fma(ga[j], m.H, gb[j]);
+        A = mul(ga[j], A);
+        H = fma(ga[j], H, gb[j]);
       }
     } else {
-      m.A = splat(1.f, L{});
-      m.H = splat(0.f, L{});
+      A = splat(1.f, L{});
+      H = splat(0.f, L{});
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
         if (!(valid >> j & 1u)) {  // no token: the state passes
           ga[j] = splat(1.f, L{});
           gb[j] = splat(0.f, L{});
         }
-        if (SEQ && (e.first >> j & 1u)) {
-          m.H = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
-          m.A = splat(-1.f, L{});
-        }
-        m.A = mul(ga[j], m.A);
-        m.H = fma(ga[j], m.H, gb[j]);
+        if (SEQ && (e.first >> j & 1u))
+          H = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
+        A = mul(ga[j], A);
+        H = fma(ga[j], H, gb[j]);
       }
     }
-    Map<V>* const sum = sums + buf * kRecWarps * 32;
-    sum[w * 32 + lane] = m;
+    Sums<V>& sum = sums[buf];
+    sum.A[w * 32 + lane] = A;
+    sum.H[w * 32 + lane] = H;
+    if (SEQ && lane == 0) sum.cut[w] = e.first;
     __syncthreads();
-    L h = p.cluster == 1 ? through_warps<V, SEQ, true>(sum, w, lane, handed[buf][lane])
-                         : through_cluster<V, SEQ, true>(sum, far + buf * p.cluster * 32, bar + 8 * buf, (k >> 1) & 1, p, w, lane, carry);
+    if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
+    if (tma && threadIdx.x == 0) tma_wait_read<1>();  // the slot to be loaded was stored a round ago
+    load(k + S - 2);
+    const unsigned cuts = SEQ ? cuts_of(sum.cut, lane) : 0;
+    L h = p.cluster == 1 ? through_warps<V, SEQ, true>(sum.A, sum.H, cuts, w, lane, common.handed[buf][lane])
+                         : through_cluster<V, SEQ, true>(sum.A, sum.H, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), (k >> 1) & 1, p, w, lane, carry);
     if (w == 0 && a.checkpoints && c < a.nchunks) {
+      float* to = a.checkpoints + (p.b * a.nchunks + c) * a.dim + p.d0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int64_t d = p.d0 + lane_channel<T, LAYOUT>(lane, i);
-        if (d < a.dim) a.checkpoints[(p.b * a.nchunks + c) * a.dim + d] = el(h, i);
+        const int d = lane_channel<T, LAYOUT>(lane, i);
+        if (d < p.nd) to[d] = el(h, i);
       }
     }
 
@@ -269,7 +322,7 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const RecArgs a
       h = fma(ga[j], h, gb[j]);
       gb[j] = h;
     }
-    if (p.cluster == 1 && w == kRecWarps - 1) handed[buf ^ 1][lane] = h;
+    if (p.cluster == 1 && w == kRecWarps - 1) common.handed[buf ^ 1][lane] = h;
     if (SEQ && e.last && a.final_states.data) {
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j)
@@ -292,73 +345,90 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const RecArgs a
       for (int j = 0; j < kRecSteps; ++j)
         if (!(valid >> j & 1u)) gb[j] = splat(0.f, L{});
     }
-    if constexpr (C::kRows) {
-      write_steps<T, SKEW>(now + C::kBytes, w, lane, gb);
-    } else {
-      store_steps<T, SKEW>(ot, tw, lane, nch, left, a.packed, gb);
-    }
-    if (++slot == S) slot = 0;
+    write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gb);
+    if (tma) tma_fence();
+    if (++slot == S) slot = 0, parity ^= 1;
   }
-  if constexpr (C::kRows) {
-    __syncthreads();
-    const int64_t tp = (static_cast<int64_t>(p.rounds - 1) * p.cluster + p.rank) * kRecChunk;
-    store_tile<T, SKEW>(smem + (slot == 0 ? S - 1 : slot - 1) * NT * C::kBytes + C::kBytes, ot, tp, p.nd, within(tp, a.seqlen, kRecChunk), a.packed);
-  }
-  if (!SEQ && a.final_states.data && p.rank == 0) {
-    if (p.cluster == 1) {
-      __syncthreads();
-      carry = handed[p.rounds & 1][lane];
-    }
-    if (w == 0) store_state<T, LAYOUT>(a.final_states, p.b, a.nstates, p.d0, a.dim, lane, carry);
-  }
+  __syncthreads();
+  store(p.rounds - 1, slot == 0 ? S - 1 : slot - 1);
+  if (!SEQ && w == 0 && p.rank == 0)
+    store_state<T, LAYOUT>(a.final_states, p.b, a.nstates, p.d0, a.dim, lane, p.cluster == 1 ? common.handed[p.rounds & 1][lane] : carry);
+  if (tma && threadIdx.x == 0) tma_wait_read<0>();
   if (p.cluster > 1) cluster_sync();  // no CTA leaves while a partner may still write to it
 }
 
 template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z>
-__global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a) {
+__global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
   using C = Tile<T, LAYOUT, SKEW>;
-  constexpr int V = C::V, NT = Z ? 4 : 3, S = kBwdStages<LAYOUT>;
+  constexpr int V = C::V, NT = Z ? 4 : 3, S = kBwdStages;
   using L = Lane<V>;
-  extern __shared__ __align__(128) unsigned char smem[];
-  // ring of tiles (gate, x, dout, z) | maps of the warps, forward and back [2][2][warps][32] |
-  // maps of the cluster, back [2][cluster][32]
-  Map<V>* const sums = reinterpret_cast<Map<V>*>(smem + S * NT * C::kBytes);
-  Map<V>* const far = sums + 4 * kRecWarps * 32;
-  __shared__ L handed[2][32];
-  __shared__ uint64_t bars[2];
-  const unsigned ring = static_cast<unsigned>(__cvta_generic_to_shared(smem));
-  const unsigned bar = static_cast<unsigned>(__cvta_generic_to_shared(bars));
+  extern __shared__ __align__(1024) unsigned char smem[];
+  // ring of tiles (gate, x, dout, z) | sums of the warps, forward and back [2] | maps of the
+  // cluster, back [2][cluster][32] | common
+  Sums<V>* const sums = reinterpret_cast<Sums<V>*>(smem + S * NT * C::kBytes);
+  SumsBack<V>* const sums_back = reinterpret_cast<SumsBack<V>*>(sums + 2);
+  Map<V>* const far = reinterpret_cast<Map<V>*>(sums_back + 2);
+  Common<V>& common = *reinterpret_cast<Common<V>*>(far + (a.cluster > 1 ? 2 * a.cluster * 32 : 0));
+  const unsigned ring = shared_addr(smem), bars = shared_addr(common.bars);
 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const Place p = place_of<C::kChannels>(a);
+  const bool tma = !SKEW && a.move == kTma;
+  start_barriers<S>(bars, tma, p.cluster);
   grid_dependency_wait();
-  const Strip<T> gt = strip_of<T, LAYOUT, SKEW>(a.gate, p.b, p.d0), xt = strip_of<T, LAYOUT, SKEW>(a.x, p.b, p.d0);
-  const Strip<T> yt = strip_of<T, LAYOUT, SKEW>(a.dout, p.b, p.d0), zt = Z ? strip_of<T, LAYOUT, SKEW>(a.z, p.b, p.d0) : gt;
-  const Strip<T> dxt = strip_of<T, LAYOUT, SKEW>(a.dx, p.b, p.d0), dgt = strip_of<T, LAYOUT, SKEW>(a.dgate, p.b, p.d0);
-  const Strip<T> dzt = Z ? strip_of<T, LAYOUT, SKEW>(a.dz, p.b, p.d0) : dgt;
-  const int nch = p.nd - lane * V;
+  const Strip<T> gt = strip_of<T>(a.gate, maps.gate, p.b, p.d0), xt = strip_of<T>(a.x, maps.x, p.b, p.d0);
+  const Strip<T> yt = strip_of<T>(a.dout, maps.dout, p.b, p.d0), zt = Z ? strip_of<T>(a.z, maps.z, p.b, p.d0) : gt;
+  const Strip<T> dxt = strip_of<T>(a.dx, maps.dx, p.b, p.d0), dgt = strip_of<T>(a.dgate, maps.dgate, p.b, p.d0);
+  const Strip<T> dzt = Z ? strip_of<T>(a.dz, maps.dz, p.b, p.d0) : dgt;
 
   auto chunk_of = [&](int k) { return static_cast<int64_t>(p.rounds - 1 - k) * p.cluster + p.rank; };
   int load_slot = 0;
   auto load = [&](int k) {
-    const int64_t t0 = chunk_of(k) * kRecChunk;
-    const int nt = within(t0, a.seqlen, kRecChunk), o = load_slot * NT * C::kBytes;
-    if (k < p.rounds && nt > 0) {
-      load_tile<T, LAYOUT, SKEW>(ring + o, smem + o, gt, t0, p.nd, nt, a.packed);
-      load_tile<T, LAYOUT, SKEW>(ring + o + C::kBytes, smem + o + C::kBytes, xt, t0, p.nd, nt, a.packed);
-      load_tile<T, LAYOUT, SKEW>(ring + o + 2 * C::kBytes, smem + o + 2 * C::kBytes, yt, t0, p.nd, nt, a.packed);
-      if constexpr (Z) load_tile<T, LAYOUT, SKEW>(ring + o + 3 * C::kBytes, smem + o + 3 * C::kBytes, zt, t0, p.nd, nt, a.packed);
+    if (k < p.rounds) {
+      const int64_t t0 = chunk_of(k) * kRecChunk;
+      const int nt = within(t0, a.seqlen, kRecChunk), o = load_slot * NT * C::kBytes;
+      const unsigned bar = bars + 8 * load_slot;
+      if (tma) {
+        if (threadIdx.x == 0) {
+          if (nt > 0) {
+            mbar_expect(bar, NT * C::kBytes);
+            tma_load<T, LAYOUT>(ring + o, gt.map, p.d0, t0, p.b, bar);
+            tma_load<T, LAYOUT>(ring + o + C::kBytes, xt.map, p.d0, t0, p.b, bar);
+            tma_load<T, LAYOUT>(ring + o + 2 * C::kBytes, yt.map, p.d0, t0, p.b, bar);
+            if constexpr (Z) tma_load<T, LAYOUT>(ring + o + 3 * C::kBytes, zt.map, p.d0, t0, p.b, bar);
+          } else {
+            mbar_arrive(bar);
+          }
+        }
+      } else {
+        if (nt > 0) {
+          load_tile<T, LAYOUT, SKEW>(smem + o, gt, t0, p.nd, nt);
+          load_tile<T, LAYOUT, SKEW>(smem + o + C::kBytes, xt, t0, p.nd, nt);
+          load_tile<T, LAYOUT, SKEW>(smem + o + 2 * C::kBytes, yt, t0, p.nd, nt);
+          if constexpr (Z) load_tile<T, LAYOUT, SKEW>(smem + o + 3 * C::kBytes, zt, t0, p.nd, nt);
+        }
+        mbar_arrive_copies(bar);  // of the asynchronous copies
+        mbar_arrive(bar);         // and of the plain stores
+      }
     }
-    cp_async_commit();
     if (++load_slot == S) load_slot = 0;
   };
-  auto store = [&](int k, const unsigned char* t) {  // rows: the gradients of round k, from the tiles they replaced
-    if constexpr (C::kRows) {
-      const int64_t t0 = chunk_of(k) * kRecChunk;
-      const int nt = within(t0, a.seqlen, kRecChunk);
-      store_tile<T, SKEW>(t, dgt, t0, p.nd, nt, a.packed);
-      store_tile<T, SKEW>(t + C::kBytes, dxt, t0, p.nd, nt, a.packed);
-      if constexpr (Z) store_tile<T, SKEW>(t + 3 * C::kBytes, dzt, t0, p.nd, nt, a.packed);
+  auto store = [&](int k, int slot) {  // dgate, dx and dz of round k, from the tiles of gate, x and z
+    const int64_t t0 = chunk_of(k) * kRecChunk;
+    const int nt = within(t0, a.seqlen, kRecChunk), o = slot * NT * C::kBytes;
+    if (tma) {
+      if (threadIdx.x == 0) {
+        if (nt > 0) {
+          tma_store<T, LAYOUT>(ring + o, dgt.map, p.d0, t0, p.b);
+          tma_store<T, LAYOUT>(ring + o + C::kBytes, dxt.map, p.d0, t0, p.b);
+          if constexpr (Z) tma_store<T, LAYOUT>(ring + o + 3 * C::kBytes, dzt.map, p.d0, t0, p.b);
+        }
+        tma_commit();
+      }
+    } else if (nt > 0) {
+      store_tile<T, LAYOUT, SKEW>(smem + o, dgt, t0, p.nd, nt);
+      store_tile<T, LAYOUT, SKEW>(smem + o + C::kBytes, dxt, t0, p.nd, nt);
+      if constexpr (Z) store_tile<T, LAYOUT, SKEW>(smem + o + 3 * C::kBytes, dzt, t0, p.nd, nt);
     }
   };
   auto checkpoint = [&](int k) {
@@ -375,45 +445,28 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a
     return r;
   };
 #pragma unroll
-  for (int k = 0; k < S - 1; ++k) load(k);
-  if (p.cluster > 1) {
-    if (threadIdx.x == 0) {
-      mbar_init(bar);
-      mbar_init(bar + 8);
-      mbar_init_done();
-    }
-    cluster_sync();
-  }
+  for (int k = 0; k < S - 2; ++k) load(k);
   const L nb = gate_offset<T, LAYOUT>(a, p.d0, lane);
   L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.dfinal, p.b, a.nstates, p.d0, a.dim, lane);
-  if (w == 0) handed[0][lane] = carry;
+  if (w == 0) common.handed[0][lane] = carry;
   L start = checkpoint(0);
   int ids = SEQ ? load_ids(a, p.b, chunk_of(0) * kRecChunk + w * kRecSteps, lane) : 0;
   L bias_sum = splat(0.f, L{});
 
   int slot = 0;
+  unsigned parity = 0;
   for (int k = 0; k < p.rounds; ++k) {
     const int64_t t0 = chunk_of(k) * kRecChunk, tw = t0 + w * kRecSteps;
-    const int left = within(tw, a.seqlen, kRecSteps);
     unsigned char* const now = smem + slot * NT * C::kBytes;
     const int buf = k & 1;
-    cp_async_wait<S - 2>();
-    if constexpr (C::kRows) {
-      __syncthreads();
-      if (k > 0) {
-        store(k - 1, smem + (slot == 0 ? S - 1 : slot - 1) * NT * C::kBytes);
-        if constexpr (SKEW) __syncthreads();
-      }
-    } else {
-      __syncwarp();
-    }
-    load(k + S - 1);
+    const bool there = mbar_wait(bars + 8 * slot, parity);
 
     L ga[kRecSteps], gc[kRecSteps], x[kRecSteps], gy[kRecSteps], dz[kRecSteps];
     {
       L g[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, g);
       gates<T, V>(g, nb, ga, gc);
+      if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
     }
     read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, x);
     read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, yt, t0, w, lane, gy);
@@ -422,69 +475,73 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a
       read_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, t0, w, lane, z);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
-        L s, d;
+        // silu(z) = z p and silu'(z) = p (1 + z (1 - p)), p = sigmoid(z)
+        L p, one = splat(1.f, L{});
 #pragma unroll
-        for (int i = 0; i < V; ++i) silu_and_grad<T>(el(z[j], i), el(s, i), el(d, i));
-        dz[j] = mul(gy[j], d);
-        gy[j] = mul(gy[j], s);
+        for (int i = 0; i < V; ++i) el(p, i) = sigmoid_of<T>(el(z[j], i));
+        dz[j] = mul(gy[j], mul(p, fma(z[j], sub(one, p), one)));
+        gy[j] = mul(gy[j], mul(z[j], p));
       }
     }
     Edges e;
-    unsigned valid = below(left);
+    unsigned valid = below(within(tw, a.seqlen, kRecSteps));
     if constexpr (SEQ) {
       e = edges_of(ids);
       valid = e.valid;
       ids = load_ids(a, p.b, tw - static_cast<int64_t>(p.cluster) * kRecChunk, lane);
     }
     const bool whole = valid == 0xffu && !(SEQ && (e.first || e.last));
-    Map<V> f, r;  // h -> A h + H forward through the positions, s -> A s + H back
+    L A, H, B;
     if (whole) {
-      f.A = ga[0];
-      f.H = mul(gc[0], x[0]);
+      A = ga[0];
+      H = mul(gc[0], x[0]);
 #pragma unroll
       for (int j = 1; j < kRecSteps; ++j) {
-        f.A = mul(ga[j], f.A);
-        f.H = fma(ga[j], f.H, mul(gc[j], x[j]));
+        A = mul(ga[j], A);
+        H = fma(ga[j], H, mul(gc[j], x[j]));
       }
-      r.H = mul(ga[kRecSteps - 1], gy[kRecSteps - 1]);
+      B = mul(ga[kRecSteps - 1], gy[kRecSteps - 1]);
 #pragma unroll
-      for (int j = kRecSteps - 2; j >= 0; --j) r.H = mul(ga[j], add(gy[j], r.H));
-      r.A = f.A;
+      for (int j = kRecSteps - 2; j >= 0; --j) B = mul(ga[j], add(gy[j], B));
     } else {
-      f.A = r.A = splat(1.f, L{});
-      f.H = r.H = splat(0.f, L{});
+      A = splat(1.f, L{});
+      H = B = splat(0.f, L{});
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
         if (!(valid >> j & 1u)) {
           ga[j] = splat(1.f, L{});
           gc[j] = x[j] = gy[j] = splat(0.f, L{});
         }
-        if (SEQ && (e.first >> j & 1u)) {
-          f.H = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
-          f.A = splat(-1.f, L{});
-        }
-        f.A = mul(ga[j], f.A);
-        f.H = fma(ga[j], f.H, mul(gc[j], x[j]));
+        if (SEQ && (e.first >> j & 1u))
+          H = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
+        A = mul(ga[j], A);
+        H = fma(ga[j], H, mul(gc[j], x[j]));
       }
 #pragma unroll
       for (int j = kRecSteps - 1; j >= 0; --j) {
-        if (SEQ && (e.last >> j & 1u)) {
-          r.H = load_state<T, LAYOUT>(a.dfinal, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
-          r.A = splat(-1.f, L{});
-        }
-        r.A = mul(ga[j], r.A);
-        r.H = mul(ga[j], add(gy[j], r.H));
+        if (SEQ && (e.last >> j & 1u))
+          B = load_state<T, LAYOUT>(a.dfinal, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
+        B = mul(ga[j], add(gy[j], B));
       }
     }
-    Map<V>* const ahead = sums + 2 * buf * kRecWarps * 32;
-    Map<V>* const back = ahead + kRecWarps * 32;
-    ahead[w * 32 + lane] = f;
-    back[w * 32 + lane] = r;
+    Sums<V>& sum = sums[buf];
+    SumsBack<V>& sum_back = sums_back[buf];
+    sum.A[w * 32 + lane] = A;
+    sum.H[w * 32 + lane] = H;
+    sum_back.B[w * 32 + lane] = B;
+    if (SEQ && lane == 0) {
+      sum.cut[w] = e.first;
+      sum_back.cut[w] = e.last;
+    }
     __syncthreads();
-    L h = through_warps<V, SEQ, true>(ahead, w, lane, start);
+    if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
+    if (tma && threadIdx.x == 0) tma_wait_read<1>();
+    load(k + S - 2);
+    L h = through_warps<V, SEQ, true>(sum.A, sum.H, SEQ ? cuts_of(sum.cut, lane) : 0, w, lane, start);
     start = checkpoint(k + 1);
-    L s = p.cluster == 1 ? through_warps<V, SEQ, false>(back, w, lane, handed[buf][lane])
-                         : through_cluster<V, SEQ, false>(back, far + buf * p.cluster * 32, bar + 8 * buf, (k >> 1) & 1, p, w, lane, carry);
+    const unsigned cuts = SEQ ? cuts_of(sum_back.cut, lane) : 0;
+    L s = p.cluster == 1 ? through_warps<V, SEQ, false>(sum.A, sum_back.B, cuts, w, lane, common.handed[buf][lane])
+                         : through_cluster<V, SEQ, false>(sum.A, sum_back.B, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), (k >> 1) & 1, p, w, lane, carry);
 
     // forward through the positions: h before each, and dz
     L prev[kRecSteps];
@@ -513,24 +570,19 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a
       if (SEQ && !whole && (e.first >> j & 1u))
         store_state<T, LAYOUT>(a.dinit, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane, s);
     }
-    if (p.cluster == 1 && w == 0) handed[buf ^ 1][lane] = s;
-    if constexpr (C::kRows) {
-      write_steps<T, SKEW>(now, w, lane, prev);
-      write_steps<T, SKEW>(now + C::kBytes, w, lane, gy);
-      if constexpr (Z) write_steps<T, SKEW>(now + 3 * C::kBytes, w, lane, dz);
-    } else {
-      store_steps<T, SKEW>(dxt, tw, lane, nch, left, a.packed, gy);
-      store_steps<T, SKEW>(dgt, tw, lane, nch, left, a.packed, prev);
-      if constexpr (Z) store_steps<T, SKEW>(dzt, tw, lane, nch, left, a.packed, dz);
-    }
-    if (++slot == S) slot = 0;
+    if (p.cluster == 1 && w == 0) common.handed[buf ^ 1][lane] = s;
+    write_steps<T, LAYOUT, SKEW>(now, w, lane, prev);
+    write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gy);
+    if constexpr (Z) write_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, w, lane, dz);
+    if (tma) tma_fence();
+    if (++slot == S) slot = 0, parity ^= 1;
   }
   __syncthreads();
-  if constexpr (C::kRows) store(p.rounds - 1, smem + (slot == 0 ? S - 1 : slot - 1) * NT * C::kBytes);
+  store(p.rounds - 1, slot == 0 ? S - 1 : slot - 1);
   if (!SEQ && w == 0 && p.rank == 0)
-    store_state<T, LAYOUT>(a.dinit, p.b, a.nstates, p.d0, a.dim, lane, p.cluster == 1 ? handed[p.rounds & 1][lane] : carry);
+    store_state<T, LAYOUT>(a.dinit, p.b, a.nstates, p.d0, a.dim, lane, p.cluster == 1 ? common.handed[p.rounds & 1][lane] : carry);
   if (a.dbias) {
-    L* const sum = reinterpret_cast<L*>(sums);
+    L* const sum = sums[0].A;
     sum[w * 32 + lane] = bias_sum;
     __syncthreads();
     if (w == 0) {
@@ -544,19 +596,19 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const RecArgs a
       }
     }
   }
+  if (tma && threadIdx.x == 0) tma_wait_read<0>();
   if (p.cluster > 1) cluster_sync();
 }
 
 // dbias[d] = the tiles' partial sums added up in order.
-__global__ void __launch_bounds__(kThreads) rec_bias_kernel(const RecArgs a) {
+__global__ void __launch_bounds__(kThreads) rec_bias_kernel(const float* __restrict__ partials, int64_t n, int64_t dim, float* dbias) {
   grid_dependency_wait();
   const int64_t d = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (d >= a.dim) return;
-  const int64_t n = a.batch * a.cluster;
+  if (d >= dim) return;
   float s = 0.f;
 #pragma unroll 8
-  for (int64_t i = 0; i < n; ++i) s += a.partials[i * a.dim + d];
-  a.dbias[d] = s;
+  for (int64_t i = 0; i < n; ++i) s += partials[i * dim + d];
+  dbias[d] = s;
 }
 
 template <typename T>
@@ -593,13 +645,48 @@ __global__ void __launch_bounds__(kThreads) rec_update_kernel(const RecUpdateArg
 
 unsigned blocks_for(int64_t threads) { return static_cast<unsigned>((threads + kThreads - 1) / kThreads); }
 
+// The tensor map of a strip-wise aligned tensor; channel-last (dim, seqlen, batch), rows
+// (seqlen, dim, batch), boxes of 128 bytes by the tile's other extent.
+template <typename T, int LAYOUT>
+bool make_map(CUtensorMap* map, const TensorArg& t, const RecArgs& a) {
+  if (!t.data) return true;
+  using C = Tile<T, LAYOUT, false>;
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  if (!encode) return false;
+  const int64_t inner = C::kRows ? a.seqlen : a.dim, outer = C::kRows ? a.dim : a.seqlen, step = C::kRows ? t.s1 : t.s2;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(a.batch)};
+  // an extent of one never uses its stride, which may then be anything
+  const cuuint64_t strides[2] = {outer > 1 ? static_cast<cuuint64_t>(step) * sizeof(T) : 16, a.batch > 1 ? static_cast<cuuint64_t>(t.s0) * sizeof(T) : 16};
+  const cuuint32_t box[3] = {128 / sizeof(T), static_cast<cuuint32_t>(C::kRows ? C::kChannels : kRecChunk), 1};
+  const cuuint32_t one[3] = {1, 1, 1};
+  return encode(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, t.data, dims, strides, box, one,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, C::kRows ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int LAYOUT, bool SKEW, bool BWD, bool SEQ, bool Z>
-cudaError_t run(const RecArgs& a, cudaStream_t s) {
+cudaError_t run(RecArgs& a, cudaStream_t s) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int NT = (BWD ? 3 : 2) + (Z ? 1 : 0);
-  constexpr int stages = BWD ? kBwdStages<LAYOUT> : kFwdStages;
-  const size_t smem = static_cast<size_t>(stages) * NT * C::kBytes +
-                      sizeof(Map<C::V>) * 32 * 2 * ((BWD ? 2 : 1) * kRecWarps + (a.cluster > 1 ? a.cluster : 0));
+  constexpr int stages = BWD ? kBwdStages : kFwdStages;
+  RecMaps maps = {};
+  if (a.move == kTma) {
+    const bool ok = make_map<T, LAYOUT>(&maps.gate, a.gate, a) && make_map<T, LAYOUT>(&maps.x, a.x, a) && make_map<T, LAYOUT>(&maps.z, a.z, a) &&
+                    (BWD ? make_map<T, LAYOUT>(&maps.dout, a.dout, a) && make_map<T, LAYOUT>(&maps.dx, a.dx, a) &&
+                               make_map<T, LAYOUT>(&maps.dgate, a.dgate, a) && make_map<T, LAYOUT>(&maps.dz, a.dz, a)
+                         : make_map<T, LAYOUT>(&maps.out, a.out, a));
+    if (!ok) a.move = kElements;
+  }
+  const size_t smem = static_cast<size_t>(stages) * NT * C::kBytes + 2 * (sizeof(Sums<C::V>) + (BWD ? sizeof(SumsBack<C::V>) : 0)) +
+                      (a.cluster > 1 ? 2 * a.cluster * 32 * sizeof(Map<C::V>) : 0) + sizeof(Common<C::V>);
   auto kernel = BWD ? rec_bwd_kernel<T, LAYOUT, SKEW, SEQ, Z> : rec_fwd_kernel<T, LAYOUT, SKEW, SEQ, Z>;
   const void* ptr = reinterpret_cast<const void*>(kernel);
   cudaError_t e = allow_dynamic_smem(ptr, smem);
@@ -618,19 +705,19 @@ cudaError_t run(const RecArgs& a, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = a.cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<const RecArgs&>(a), static_cast<const RecMaps&>(maps));
 }
 
 template <typename T, int LAYOUT, bool SKEW, bool BWD>
-cudaError_t pick_options(const RecArgs& a, cudaStream_t s) {
+cudaError_t pick_options(RecArgs& a, cudaStream_t s) {
   if (a.seq_idx.data)
     return a.z.data ? run<T, LAYOUT, SKEW, BWD, true, true>(a, s) : run<T, LAYOUT, SKEW, BWD, true, false>(a, s);
   return a.z.data ? run<T, LAYOUT, SKEW, BWD, false, true>(a, s) : run<T, LAYOUT, SKEW, BWD, false, false>(a, s);
 }
 template <typename T, bool BWD>
-cudaError_t pick(const RecArgs& a, cudaStream_t s) {
+cudaError_t pick(RecArgs& a, cudaStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    if (a.skew) return a.rows ? pick_options<T, kLayoutRows, true, BWD>(a, s) : pick_options<T, kLayoutChannelLast, true, BWD>(a, s);
+    if (a.move == kWords) return a.rows ? pick_options<T, kLayoutRows, true, BWD>(a, s) : pick_options<T, kLayoutChannelLast, true, BWD>(a, s);
   }
   return a.rows ? pick_options<T, kLayoutRows, false, BWD>(a, s) : pick_options<T, kLayoutChannelLast, false, BWD>(a, s);
 }
@@ -639,13 +726,22 @@ cudaError_t pick(const RecArgs& a, cudaStream_t s) {
 
 using DT = CC1D_DT_TYPE;
 
-cudaError_t CC1D_DT_NAME(rec_fwd)(const RecArgs& a, cudaStream_t s) {
+cudaError_t CC1D_DT_NAME(rec_fwd)(RecArgs& a, cudaStream_t s) {
   return pick<DT, false>(a, s);
 }
-cudaError_t CC1D_DT_NAME(rec_bwd)(const RecArgs& a, cudaStream_t s) {
+cudaError_t CC1D_DT_NAME(rec_bwd)(RecArgs& a, cudaStream_t s) {
   cudaError_t e = pick<DT, true>(a, s);
-  if (e == cudaSuccess && a.dbias) e = launch_dependent(rec_bias_kernel, dim3(blocks_for(a.dim)), dim3(kThreads), 0, s, a);
-  return e;
+  if (e != cudaSuccess || !a.dbias) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks_for(a.dim));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, rec_bias_kernel, static_cast<const float*>(a.partials), a.batch * a.cluster, a.dim, a.dbias);
 }
 cudaError_t CC1D_DT_NAME(rec_update)(const RecUpdateArgs& a, cudaStream_t s) {
   return launch_dependent(rec_update_kernel<DT>, dim3(blocks_for(a.batch * a.dim)), dim3(kThreads), 0, s, a);

@@ -7,15 +7,20 @@
 // memory layouts.
 #pragma once
 
+#include <cuda.h>
+
 #include "cc1d_block_launch.h"
 #include "cc1d_block_math.cuh"
 
 namespace cc1d {
 
+struct RecMaps {
+  CUtensorMap gate, x, z, out, dout, dx, dgate, dz;
+};
+
 constexpr int kRecWarps = 8;
 constexpr int kRecThreads = 32 * kRecWarps;
 constexpr int kRecSteps = kRecChunk / kRecWarps;  // positions of a warp in a chunk
-constexpr int kRecMaxCluster = 16;
 static_assert(kRecSteps == 8, "the tiles' packets and the boundary masks hold 8 positions");
 
 // ------------------------------------------------------------------ V channels of a lane
@@ -41,43 +46,75 @@ template <int V> __device__ __forceinline__ float el(const Lane<V>& a, int i) { 
 // The affine map h -> A h + H of a stretch of positions.  A stretch in which a sequence
 // starts does not depend on h at all, not even where h is infinite or NaN: A then has its
 // sign bit set (a product of sigmoids never has).
+template <int V> struct alignas(8 * V) Map { Lane<V> A, H; };
+
 template <int V, bool SEQ>
-__device__ __forceinline__ Lane<V> apply(const Lane<V>& A, const Lane<V>& H, const Lane<V>& h) {
-  Lane<V> r = fma(A, h, H);
+__device__ __forceinline__ Lane<V> apply(const Map<V>& m, const Lane<V>& h) {
+  Lane<V> r = fma(m.A, h, m.H);
   if constexpr (SEQ) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (__float_as_int(el(A, i)) < 0) el(r, i) = el(H, i);
-  }
-  return r;
-}
-// A of the map (A2, .) after (A1, .).
-template <int V, bool SEQ>
-__device__ __forceinline__ Lane<V> chain(const Lane<V>& A2, const Lane<V>& A1) {
-  Lane<V> r = mul(A2, A1);
-  if constexpr (SEQ) {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (__float_as_int(el(A2, i)) < 0) el(r, i) = el(A2, i);
+      if (__float_as_int(el(m.A, i)) < 0) el(r, i) = el(m.H, i);
   }
   return r;
 }
 
+// -------------------------------------------------------------------------- barriers
+__device__ __forceinline__ unsigned shared_addr(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(unsigned bar, unsigned count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(unsigned bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(unsigned bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+// Arrives when all cp.async that this thread has issued are done.
+__device__ __forceinline__ void mbar_arrive_copies(unsigned bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+// Waits for the phase of that parity, at most 2^20 tries of the hardware's own waiting time;
+// returns whether it came.  What is waited for was issued by this CTA or by CTAs of its
+// cluster, which run at the same time, so it does come.
+__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
+  for (int i = 0; i < (1 << 20); ++i) {
+    unsigned done;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+
 // ----------------------------------------------------------------------------- the tiles
-// SKEW (16-bit only): rows that do not all start on a 4-byte boundary are copied in the
-// 4-byte words that cover them, so a row lies in its tile as it does in memory, half a word
-// late where it starts in the middle of one.
+// SKEW (kWords): a strip lies in its tile as it does in memory, half a word late where it
+// starts in the middle of one, so it takes 33 words.
+//
+// channel-last: 64 rows (positions) of 128 bytes of channels.
+// rows: a row of positions per channel, in 16-byte packets; packet p of row r is at p ^ (r % 8)
+// (the TMA's 128-byte swizzle), so that 8 lanes reading a packet of 8 channels use all banks.
+// fp32 has two such halves of 32 positions each.  SKEW: the 33rd words follow.
 template <typename T, int LAYOUT, bool SKEW> struct Tile {
   static constexpr int kSize = sizeof(T);
   static constexpr int V = 4 / kSize;                // channels per lane
   static constexpr int kChannels = 32 * V;           // 128 bytes
   static constexpr int kPacket = 16 / kSize;         // elements per 16 bytes
   static constexpr bool kRows = LAYOUT == kLayoutRows;
-  // channel-last: 64 rows of 128 bytes, rows 8w.. written and read by warp w alone.
-  // rows: a row of 64 positions per channel, 16 bytes longer so that the 16-byte reads of
-  // 8 lanes (8 channels) fall into different banks.
-  static constexpr int kPitch = kRows ? kRecChunk * kSize + 16 : SKEW ? 132 : 128;
-  static constexpr int kBytes = kRows ? kChannels * kPitch : kRecChunk * kPitch;
+  static constexpr int kBytes = 8192 + (SKEW ? 256 : 0);
+  static constexpr int kEnds = 8192;                 // SKEW: the 33rd words (of 64 strips)
+  // byte of element (channel, position) without a skew
+  static __device__ __forceinline__ int at(int ch, int pos) {
+    if constexpr (!kRows) return pos * 128 + ch * kSize;
+    const int byte = pos * kSize;
+    return (byte >> 7) * (kChannels * 128) + ch * 128 + ((((byte >> 4) & 7) ^ (ch & 7)) << 4) + (byte & 15);
+  }
+  // byte of word i (0 .. 31) of strip r: a position channel-last, a channel with rows
+  static __device__ __forceinline__ int word(int r, int i) {
+    return kRows ? r * 128 + ((((i >> 2) ^ r) & 7) << 4) + (i & 3) * 4 : r * 128 + i * 4;
+  }
 };
 
 // Channel of value i of a lane within the tile: neighbours share a 4-byte word of a
@@ -92,144 +129,101 @@ __device__ __forceinline__ int lane_channel(int lane, int i) {
 template <typename T>
 struct Strip {
   T* origin;
-  T* row;       // at channel d0, position 0
+  T* row;  // at channel d0, position 0
   int64_t s1, s2;
-  unsigned off; // packed: byte offset of the thread's first packet from (d0, t0)
+  const CUtensorMap* map;
 };
-
-__device__ __forceinline__ void cp16(unsigned dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+template <typename T>
+__device__ __forceinline__ Strip<T> strip_of(const TensorArg& t, const CUtensorMap& map, int64_t b, int64_t d0) {
+  T* const o = static_cast<T*>(t.data);
+  return {o, o + b * t.s0 + d0 * t.s1, t.s1, t.s2, &map};
 }
+
 __device__ __forceinline__ void cp4(unsigned dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-template <typename T, int LAYOUT, bool SKEW>
-__device__ __forceinline__ Strip<T> strip_of(const TensorArg& t, int64_t b, int64_t d0) {
-  using C = Tile<T, LAYOUT, SKEW>;
-  Strip<T> s;
-  s.origin = static_cast<T*>(t.data);
-  s.row = s.origin + b * t.s0 + d0 * t.s1;
-  s.s1 = t.s1;
-  s.s2 = t.s2;
-  // below 2^32 for packed tensors (rec_plan)
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  if constexpr (C::kRows) {
-    constexpr int PR = kRecChunk / C::kPacket;
-    s.off = (static_cast<unsigned>(threadIdx.x / PR) * static_cast<unsigned>(t.s1) + (threadIdx.x % PR) * C::kPacket) * C::kSize;
-  } else {
-    s.off = (static_cast<unsigned>(w * kRecSteps + (lane >> 3)) * static_cast<unsigned>(t.s2) + (lane & 7) * C::kPacket) * C::kSize;
-  }
-  return s;
+// kTma, one thread: the copy of a chunk into its tile, counted on `bar`; and back.
+template <typename T, int LAYOUT>
+__device__ __forceinline__ void tma_load(unsigned tile, const CUtensorMap* map, int d0, int t0, int b, unsigned bar) {
+  constexpr bool rows = LAYOUT == kLayoutRows;
+#pragma unroll
+  for (int h = 0; h < (rows ? static_cast<int>(sizeof(T)) / 2 : 1); ++h)
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(tile + h * 4096),
+                 "l"(map), "r"(rows ? t0 + h * 32 : d0), "r"(rows ? d0 : t0), "r"(b), "r"(bar) : "memory");
 }
+template <typename T, int LAYOUT>
+__device__ __forceinline__ void tma_store(unsigned tile, const CUtensorMap* map, int d0, int t0, int b) {
+  constexpr bool rows = LAYOUT == kLayoutRows;
+#pragma unroll
+  for (int h = 0; h < (rows ? static_cast<int>(sizeof(T)) / 2 : 1); ++h)
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n" ::"l"(map),
+                 "r"(rows ? t0 + h * 32 : d0), "r"(rows ? d0 : t0), "r"(b), "r"(tile + h * 4096) : "memory");
+}
+__device__ __forceinline__ void tma_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
+// At most N committed groups still read shared memory.
+template <int N> __device__ __forceinline__ void tma_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory"); }
+// What this thread wrote to shared memory is there for the TMA.
+__device__ __forceinline__ void tma_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-// Starts the copy of a chunk (positions t0 .. t0 + nt - 1 of nd channels) into its tile;
-// places outside are zero.  packed: 16-byte packets, aligned (rec_plan);
-// SKEW: 4-byte words; else element by element at any strides.  Channel-last: each warp
-// copies what it reads itself.
+// kWords and kElements, all threads: positions t0 .. t0 + nt - 1 of nd channels; places outside
+// are zero.
 template <typename T, int LAYOUT, bool SKEW>
-__device__ __forceinline__ void load_tile(unsigned tile, unsigned char* tile_ptr, const Strip<T>& t, int64_t t0, int nd, int nt, bool packed) {
+__device__ __forceinline__ void load_tile(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
   using C = Tile<T, LAYOUT, SKEW>;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const unsigned base = shared_addr(tile);
   if constexpr (SKEW) {
-    constexpr int R = C::kRows ? C::kChannels : kRecSteps;  // rows: the CTA's, or the warp's own
     const int64_t step = C::kRows ? t.s1 : t.s2;
-    const int first = C::kRows ? 0 : w * kRecSteps;
-    const int rows = C::kRows ? nd : nt, len = C::kRows ? nt : nd;
-    const T* const base = t.row + (C::kRows ? t0 : t0 * t.s2);
-    // word i of a row covers elements 2i - skew and 2i + 1 - skew
-    auto word = [&](int r, int i) {
-      const T* p = base + r * step;
-      const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1;
-      const int e = 2 * i - skew;  // its first element in the row
-      const int n = r < rows ? max(0, min(2, len - e)) : 0;
-      const unsigned dst = tile + r * C::kPitch + i * 4;
+    const int strips = C::kRows ? nd : nt, len = C::kRows ? nt : nd;
+    const T* const from = t.row + (C::kRows ? t0 : t0 * t.s2);
+    const T* const none = t.origin + (reinterpret_cast<uintptr_t>(t.origin) >> 1 & 1);  // aligned, not read
+    // word i of a strip covers its elements 2i - skew and 2i + 1 - skew
+    auto word = [&](int r, int i, int o) {
+      const T* p = from + r * step;
+      const int e = 2 * i - (static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1);
+      const int n = r < strips ? max(0, min(2, len - e)) : 0;
       if (n > 0 && p + e < t.origin) {  // half of the word lies before the tensor
-        *reinterpret_cast<uint32_t*>(tile_ptr + r * C::kPitch + i * 4) = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + e + 1)) << 16;
+        *reinterpret_cast<uint32_t*>(tile + o) = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + e + 1)) << 16;
       } else {
-        cp4(dst, n > 0 ? p + e : t.origin + (reinterpret_cast<uintptr_t>(t.origin) >> 1 & 1), n * 2);
+        cp4(base + o, n > 0 ? p + e : none, n * 2);
       }
     };
-    if constexpr (C::kRows) {
-#pragma unroll 4
-      for (int k = 0; k < R / kRecWarps; ++k) word(w * (R / kRecWarps) + k, lane);
-      if (threadIdx.x < R) word(threadIdx.x, 32);
-    } else {
 #pragma unroll
-      for (int k = 0; k < R; ++k) word(first + k, lane);
-      if (lane < R) word(first + lane, 32);
-    }
-    return;
+    for (int k = 0; k < 8; ++k) word(w * 8 + k, lane, C::word(w * 8 + k, lane));
+    if (threadIdx.x < 64) word(threadIdx.x, 32, C::kEnds + threadIdx.x * 4);
   } else {
-    if (packed) {
-      if constexpr (C::kRows) {
-        constexpr int PR = kRecChunk / C::kPacket;          // packets of a row
-        constexpr int CR = kRecThreads / PR;                // rows a pass of the threads covers
-        const char* const src = reinterpret_cast<const char*>(t.row + t0);
-        const int c0 = threadIdx.x / PR, p = (threadIdx.x % PR) * C::kPacket;
-        const int n = max(0, min(C::kPacket, nt - p)) * C::kSize;
-#pragma unroll
-        for (int k = 0; k < C::kChannels / CR; ++k) {
-          const int m = c0 + k * CR < nd ? n : 0;
-          cp16(tile + (c0 + k * CR) * C::kPitch + p * C::kSize, m ? src + k * CR * t.s1 * C::kSize + t.off : reinterpret_cast<const char*>(t.origin), m);
-        }
-      } else {
-        const int n = max(0, min(C::kPacket, nd - (lane & 7) * C::kPacket)) * C::kSize;
-        const char* const src = reinterpret_cast<const char*>(t.row + t0 * t.s2);
-        const int r = w * kRecSteps + (lane >> 3);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int m = r + 4 * k < nt ? n : 0;
-          cp16(tile + (r + 4 * k) * C::kPitch + (lane & 7) * 16, m ? src + 4 * k * t.s2 * C::kSize + t.off : reinterpret_cast<const char*>(t.origin), m);
-        }
-      }
-      return;
-    }
-    const T* src = t.row + t0 * t.s2;
-    constexpr int N = C::kRows ? C::kChannels * kRecChunk / kRecThreads : kRecSteps * C::V;
+    const T* const src = t.row + t0 * t.s2;
+    constexpr int N = C::kChannels * kRecChunk / kRecThreads;
 #pragma unroll 4
     for (int k = 0; k < N; ++k) {
-      int ch, p;
-      if constexpr (C::kRows) {
-        const int i = threadIdx.x + k * kRecThreads;
-        ch = i / kRecChunk;
-        p = i % kRecChunk;
-      } else {
-        ch = lane + 32 * (k % C::V);
-        p = w * kRecSteps + k / C::V;
-      }
+      const int i = threadIdx.x + k * kRecThreads;
+      const int ch = C::kRows ? i / kRecChunk : i % C::kChannels, p = C::kRows ? i % kRecChunk : i / C::kChannels;
       const bool in = ch < nd && p < nt;
-      const int o = C::kRows ? ch * C::kPitch + p * C::kSize : p * C::kPitch + ch * C::kSize;
       const T* from = in ? src + ch * t.s1 + p * t.s2 : t.origin;
       if constexpr (C::kSize == 4) {
-        cp4(tile + o, from, in ? 4 : 0);
+        cp4(base + C::at(ch, p), from, in ? 4 : 0);
       } else {
-        *reinterpret_cast<T*>(tile_ptr + o) = in ? *from : from_f32<T>(0.f);
+        *reinterpret_cast<T*>(tile + C::at(ch, p)) = in ? *from : from_f32<T>(0.f);
       }
     }
   }
-}
-
-template <typename T, int N>
-__device__ __forceinline__ void widen(const uint32_t (&r)[N], float2 (&v)[N]) {
-  unpack2<T, 2 * N>(*reinterpret_cast<const Packet<T, 2 * N>*>(&r), v);
 }
 
 // The 8 positions of warp w and the lane's V channels, as fp32.
 template <typename T, int LAYOUT, bool SKEW>
-__device__ __forceinline__ void read_steps(const unsigned char* tile, const Strip<T>& t, int64_t t0, int w, int lane,
-                                           Lane<Tile<T, LAYOUT, SKEW>::V> (&f)[kRecSteps]) {
+__device__ __forceinline__ void read_steps(const unsigned char* tile, const Strip<T>& t, int64_t t0, int w, int lane, Lane<4 / sizeof(T)> (&f)[kRecSteps]) {
   using C = Tile<T, LAYOUT, SKEW>;
   if constexpr (C::kRows) {
 #pragma unroll
     for (int i = 0; i < C::V; ++i) {
-      const unsigned char* p = tile + (lane + 32 * i) * C::kPitch + w * kRecSteps * C::kSize;
+      const int ch = lane + 32 * i;
 #pragma unroll
       for (int q = 0; q < kRecSteps / C::kPacket; ++q) {
-        uint4 u = *reinterpret_cast<const uint4*>(p + q * 16);
+        uint4 u = *reinterpret_cast<const uint4*>(tile + C::at(ch, w * kRecSteps + q * C::kPacket));
         if constexpr (SKEW) {
-          const uint32_t next = *reinterpret_cast<const uint32_t*>(p + 16);
-          const unsigned sh = (reinterpret_cast<uintptr_t>(t.row + t0 + (lane + 32 * i) * t.s1) & 2) * 8;
+          const uint32_t next = *reinterpret_cast<const uint32_t*>(tile + (w < 7 ? C::word(ch, 4 * w + 4) : C::kEnds + 4 * ch));
+          const unsigned sh = (reinterpret_cast<uintptr_t>(t.row + t0 + ch * t.s1) & 2) * 8;
           u = make_uint4(__funnelshift_r(u.x, u.y, sh), __funnelshift_r(u.y, u.z, sh), __funnelshift_r(u.z, u.w, sh),
                          __funnelshift_r(u.w, next, sh));
         }
@@ -243,132 +237,93 @@ __device__ __forceinline__ void read_steps(const unsigned char* tile, const Stri
       }
     }
   } else {
-    const unsigned char* p = tile + w * kRecSteps * C::kPitch + lane * 4;
+    const unsigned char* p = tile + w * kRecSteps * 128 + lane * 4;
 #pragma unroll
     for (int j = 0; j < kRecSteps; ++j) {
       if constexpr (C::V == 2) {
-        uint32_t u = *reinterpret_cast<const uint32_t*>(p + j * C::kPitch);
+        uint32_t u = *reinterpret_cast<const uint32_t*>(p + j * 128);
         if constexpr (SKEW) {
+          const uint32_t next = *reinterpret_cast<const uint32_t*>(lane < 31 ? p + j * 128 + 4 : tile + C::kEnds + (w * kRecSteps + j) * 4);
           const unsigned sh = (reinterpret_cast<uintptr_t>(t.row + (t0 + w * kRecSteps + j) * t.s2) & 2) * 8;
-          u = __funnelshift_r(u, *reinterpret_cast<const uint32_t*>(p + j * C::kPitch + 4), sh);
+          u = __funnelshift_r(u, next, sh);
         }
         float2 v[1];
         unpack2<T, 2>(*reinterpret_cast<const Packet<T, 2>*>(&u), v);
         f[j].v = v[0];
       } else {
-        f[j].v = *reinterpret_cast<const float*>(p + j * C::kPitch);
+        f[j].v = *reinterpret_cast<const float*>(p + j * 128);
       }
     }
   }
 }
 
-// rows: puts 8 positions back into a tile (without a skew), to be stored by store_tile.
-template <typename T, bool SKEW>
+// Puts 8 positions into a tile, without a skew.
+template <typename T, int LAYOUT, bool SKEW>
 __device__ __forceinline__ void write_steps(unsigned char* tile, int w, int lane, const Lane<4 / sizeof(T)> (&f)[kRecSteps]) {
-  using C = Tile<T, kLayoutRows, SKEW>;
+  using C = Tile<T, LAYOUT, SKEW>;
+  if constexpr (C::kRows) {
 #pragma unroll
-  for (int i = 0; i < C::V; ++i) {
-    unsigned char* p = tile + (lane + 32 * i) * C::kPitch + w * kRecSteps * C::kSize;
+    for (int i = 0; i < C::V; ++i) {
 #pragma unroll
-    for (int q = 0; q < kRecSteps / C::kPacket; ++q) {
-      float2 v[C::kPacket / 2];
+      for (int q = 0; q < kRecSteps / C::kPacket; ++q) {
+        float2 v[C::kPacket / 2];
 #pragma unroll
-      for (int j = 0; j < C::kPacket / 2; ++j)
-        v[j] = make_float2(el(f[q * C::kPacket + 2 * j], i), el(f[q * C::kPacket + 2 * j + 1], i));
-      *reinterpret_cast<Packet<T, C::kPacket>*>(p + q * 16) = pack2<T, C::kPacket>(v);
-    }
-  }
-}
-
-// rows: stores a tile.  Without a skew each thread takes the elements that it also loads, so a
-// load into the same tile may follow without a barrier.
-template <typename T, bool SKEW>
-__device__ __forceinline__ void store_tile(const unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt, bool packed) {
-  using C = Tile<T, kLayoutRows, SKEW>;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  if constexpr (SKEW) {
-    // words of the row in memory: element 2i - skew and its successor
-    auto word = [&](int r, int i) {
-      if (r >= nd) return;
-      T* p = t.row + t0 + r * t.s1;
-      const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1;
-      const int e = 2 * i - skew;
-      const unsigned char* s = tile + r * C::kPitch;
-      if (e >= 0 && e + 1 < nt) {
-        const uint32_t lo = *reinterpret_cast<const uint32_t*>(s + (e & ~1) * 2);
-        const uint32_t hi = *reinterpret_cast<const uint32_t*>(s + (e & ~1) * 2 + 4);
-        *reinterpret_cast<uint32_t*>(p + e) = __funnelshift_r(lo, hi, skew * 16);
-      } else {
-        if (e >= 0 && e < nt) p[e] = *reinterpret_cast<const T*>(s + e * 2);
-        if (e + 1 >= 0 && e + 1 < nt) p[e + 1] = *reinterpret_cast<const T*>(s + e * 2 + 2);
-      }
-    };
-#pragma unroll 4
-    for (int k = 0; k < C::kChannels / kRecWarps; ++k) word(w * (C::kChannels / kRecWarps) + k, lane);
-    if (threadIdx.x < C::kChannels) word(threadIdx.x, 32);
-  } else if (packed) {
-    constexpr int PR = kRecChunk / C::kPacket;
-    constexpr int CR = kRecThreads / PR;
-    char* const dst = reinterpret_cast<char*>(t.row + t0);
-    const int c0 = threadIdx.x / PR, p = (threadIdx.x % PR) * C::kPacket;
-#pragma unroll
-    for (int k = 0; k < C::kChannels / CR; ++k) {
-      if (c0 + k * CR >= nd || p >= nt) continue;
-      const Packet<T, C::kPacket> r = *reinterpret_cast<const Packet<T, C::kPacket>*>(tile + (c0 + k * CR) * C::kPitch + p * C::kSize);
-      T* o = reinterpret_cast<T*>(dst + k * CR * t.s1 * C::kSize + t.off);
-      if (p + C::kPacket <= nt) {
-        st_packet<T, C::kPacket>(o, r);
-      } else {
-#pragma unroll
-        for (int j = 0; j < C::kPacket; ++j)
-          if (p + j < nt) o[j] = r.v[j];
+        for (int j = 0; j < C::kPacket / 2; ++j)
+          v[j] = make_float2(el(f[q * C::kPacket + 2 * j], i), el(f[q * C::kPacket + 2 * j + 1], i));
+        *reinterpret_cast<Packet<T, C::kPacket>*>(tile + C::at(lane + 32 * i, w * kRecSteps + q * C::kPacket)) = pack2<T, C::kPacket>(v);
       }
     }
   } else {
-    T* dst = t.row + t0 * t.s2;
-#pragma unroll 4
-    for (int k = 0; k < C::kChannels * kRecChunk / kRecThreads; ++k) {
-      const int i = threadIdx.x + k * kRecThreads;
-      const int ch = i / kRecChunk, p = i % kRecChunk;
-      if (ch < nd && p < nt) dst[ch * t.s1 + p * t.s2] = *reinterpret_cast<const T*>(tile + ch * C::kPitch + p * C::kSize);
+    unsigned char* p = tile + w * kRecSteps * 128 + lane * 4;
+#pragma unroll
+    for (int j = 0; j < kRecSteps; ++j) {
+      if constexpr (C::V == 2) {
+        float2 v[1] = {f[j].v};
+        *reinterpret_cast<Packet<T, 2>*>(p + j * 128) = pack2<T, 2>(v);
+      } else {
+        *reinterpret_cast<float*>(p + j * 128) = f[j].v;
+      }
     }
   }
 }
 
-// channel-last: stores the 8 positions of warp w, nt of them within the sequence.  nch: how
-// many of the lane's channels there are.
-template <typename T, bool SKEW>
-__device__ __forceinline__ void store_steps(const Strip<T>& t, int64_t tw, int lane, int nch, int left, bool packed,
-                                            const Lane<4 / sizeof(T)> (&f)[kRecSteps]) {
-  constexpr int V = 4 / sizeof(T);
-  char* const row = reinterpret_cast<char*>(t.row + tw * t.s2);
-  if (!SKEW && packed && nch == V) {
-    const unsigned o = lane * 4u;
-    auto put = [&](int j) {
-      char* p = row + j * t.s2 * static_cast<int64_t>(sizeof(T)) + o;
-      if constexpr (V == 2) {
-        float2 v[1] = {f[j].v};
-        st_packet<T, 2>(reinterpret_cast<T*>(p), pack2<T, 2>(v));
+// kWords and kElements, all threads: stores what write_steps put into a tile.
+template <typename T, int LAYOUT, bool SKEW>
+__device__ __forceinline__ void store_tile(const unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
+  using C = Tile<T, LAYOUT, SKEW>;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  if constexpr (SKEW) {
+    const int64_t step = C::kRows ? t.s1 : t.s2;
+    const int strips = C::kRows ? nd : nt, len = C::kRows ? nt : nd;
+    T* const to = t.row + (C::kRows ? t0 : t0 * t.s2);
+    auto element = [&](int r, int e) {
+      return *reinterpret_cast<const uint16_t*>(tile + C::word(r, e >> 1) + (e & 1) * 2);
+    };
+    auto word = [&](int r, int i) {  // the words of the strip as it lies in memory
+      if (r >= strips) return;
+      T* p = to + r * step;
+      const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1;
+      const int e = 2 * i - skew;
+      if (e >= 0 && e + 1 < len) {
+        const uint32_t hi = *reinterpret_cast<const uint32_t*>(tile + C::word(r, i));
+        const uint32_t lo = skew ? *reinterpret_cast<const uint32_t*>(tile + C::word(r, i - 1)) : 0;
+        *reinterpret_cast<uint32_t*>(p + e) = skew ? __funnelshift_r(lo, hi, 16) : hi;
       } else {
-        *reinterpret_cast<float*>(p) = f[j].v;
+        if (e >= 0 && e < len) *reinterpret_cast<uint16_t*>(p + e) = element(r, e);
+        if (e + 1 >= 0 && e + 1 < len) *reinterpret_cast<uint16_t*>(p + e + 1) = element(r, e + 1);
       }
     };
-    if (left >= kRecSteps) {
 #pragma unroll
-      for (int j = 0; j < kRecSteps; ++j) put(j);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kRecSteps; ++j)
-        if (j < left) put(j);
+    for (int k = 0; k < 8; ++k) word(w * 8 + k, lane);
+    if (threadIdx.x < 64) word(threadIdx.x, 32);
+  } else {
+    T* const dst = t.row + t0 * t.s2;
+#pragma unroll 4
+    for (int k = 0; k < C::kChannels * kRecChunk / kRecThreads; ++k) {
+      const int i = threadIdx.x + k * kRecThreads;
+      const int ch = C::kRows ? i / kRecChunk : i % C::kChannels, p = C::kRows ? i % kRecChunk : i / C::kChannels;
+      if (ch < nd && p < nt) dst[ch * t.s1 + p * t.s2] = *reinterpret_cast<const T*>(tile + C::at(ch, p));
     }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < kRecSteps; ++j) {
-    if (j >= left) break;
-    T* p = t.row + (tw + j) * t.s2 + lane * V * t.s1;
-    if (nch > 0) p[0] = from_f32<T>(el(f[j], 0));
-    if (V > 1 && nch > 1) p[t.s1] = from_f32<T>(el(f[j], V - 1));
   }
 }
 
@@ -419,9 +374,6 @@ __device__ __forceinline__ void store_state(const TensorArg& s, int64_t n, int64
 }
 
 // ------------------------------------------------------------------------- clusters
-// A map of a stretch of positions, as it travels between warps and CTAs.
-template <int V> struct alignas(8 * V) Map { Lane<V> A, H; };
-
 __device__ __forceinline__ unsigned cluster_rank() {
   unsigned r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
@@ -429,26 +381,6 @@ __device__ __forceinline__ unsigned cluster_rank() {
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ void mbar_init(unsigned bar) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_init_done() { asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory"); }
-__device__ __forceinline__ void mbar_expect(unsigned bar, unsigned bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
-}
-// Waits for the phase of that parity, at most about 2^20 tries of the hardware's own waiting
-// time; returns whether it came.  The partners run at the same time (one cluster), so it does.
-__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
-  for (int i = 0; i < (1 << 20); ++i) {
-    unsigned done;
-    asm volatile(
-        "{\n.reg .pred p;\n"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    if (done) return true;
-  }
-  return false;
 }
 // Writes m to the place of `local` in the shared memory of CTA `rank`, and counts its bytes on
 // that CTA's barrier at the place of `bar`: data and signal in one, without a fence that
