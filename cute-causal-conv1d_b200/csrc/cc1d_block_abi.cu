@@ -120,7 +120,7 @@ cc1d_status rec_plan(RecArgs* a, bool bwd) {
   a->dtiles = (a->dim + channels - 1) / channels;
   const int64_t tiles = a->batch * a->dtiles;
   const int64_t tile = 8192 + (a->move == kWords ? 256 : 0), z = a->z.data ? 1 : 0;
-  a->cluster = choose_cluster(tiles, a->nchunks, bwd ? 3 * (3 + z) * tile + 13 * 1024 : 4 * (2 + z) * tile + 9 * 1024);
+  a->cluster = choose_cluster(tiles, a->nchunks, bwd ? 3 * (3 + z) * tile + 15 * 1024 : 4 * (2 + z) * tile + 11 * 1024);
   if (tiles * a->cluster > kMax31) return fail(CC1D_ERR_VALUE, "batch * dim is too large");
   return CC1D_OK;
 }

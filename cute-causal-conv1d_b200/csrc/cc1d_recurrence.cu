@@ -32,26 +32,29 @@ namespace {
 // tiles, and one (backward) or two chunks that are being loaded.
 constexpr int kFwdStages = 4, kBwdStages = 3;
 
-// exp(-(gate + bias)), at most 1e30; nb is -bias log2(e) for 16-bit tensors, else the bias.
-template <typename T>
-__device__ __forceinline__ float gate_exp(float gate, float nb) {
-  if constexpr (std::is_same<T, float>::value) return clamp_exp(expf(-(gate + nb)));
-  else return clamp_exp(ex2_approx(fmaf(gate, -kLog2e, nb)));
-}
-
-// a and c of the 8 positions from the gate's values.
-template <typename T, int V>
-__device__ __forceinline__ void gates(const Lane<V> (&g)[kRecSteps], const Lane<V>& nb, Lane<V> (&a)[kRecSteps], Lane<V> (&c)[kRecSteps]) {
+// 1 / (1 + exp(-v)) of a lane's channels; e, if wanted, is exp(-v), at most 1e30 so that e / (1 + e)
+// is right where exp overflows (1 / (1 + inf) needs no care).  For 16-bit tensors m and n give
+// -v log2(e) = v m + n, for fp32 n is added to v.
+template <typename T, int V, bool E>
+__device__ __forceinline__ Lane<V> sigmoids(const Lane<V>& v, const Lane<V>& n, Lane<V>* e) {
+  Lane<V> x, r;
+  if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-  for (int j = 0; j < kRecSteps; ++j) {
-    Lane<V> e;
+    for (int i = 0; i < V; ++i) el(x, i) = expf(-(el(v, i) + el(n, i)));
+  } else {
+    x = fma(v, splat(-kLog2e, v), n);
 #pragma unroll
-    for (int i = 0; i < V; ++i) el(e, i) = gate_exp<T>(el(g[j], i), el(nb, i));
-    const Lane<V> d = add(e, splat(1.f, e));
-#pragma unroll
-    for (int i = 0; i < V; ++i) el(a[j], i) = reciprocal<T>(el(d, i));
-    c[j] = mul(e, a[j]);
+    for (int i = 0; i < V; ++i) el(x, i) = ex2_approx(el(x, i));
   }
+  if constexpr (E) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) el(x, i) = clamp_exp(el(x, i));
+    *e = x;
+  }
+  r = add(x, splat(1.f, x));
+#pragma unroll
+  for (int i = 0; i < V; ++i) el(r, i) = reciprocal<T>(el(r, i));
+  return r;
 }
 
 template <typename T, int LAYOUT>
@@ -65,6 +68,10 @@ __device__ __forceinline__ Lane<4 / sizeof(T)> gate_offset(const RecArgs& a, int
   }
   return nb;
 }
+
+// A gate that holds the state: a = 1 and 1 - a = 0 whatever the bias.  Positions without a token
+// get it (and zeros for the rest), in shared memory, before they are read.
+constexpr float kHold = 60000.f;
 
 // Positions of a chunk or of a warp, t .. t + n - 1, that lie within the sequence (may be <= 0).
 __device__ __forceinline__ int within(int64_t t, int64_t len, int n) {
@@ -106,16 +113,33 @@ __device__ __forceinline__ unsigned cuts_of(const unsigned* cut, int lane) {
   return __ballot_sync(0xffffffffu, lane < kRecWarps && cut[lane & (kRecWarps - 1)]);
 }
 
+// h = m h + c if p, as one predicated instruction.
+__device__ __forceinline__ void fma_if(bool p, Lane<1>& h, const Lane<1>& m, const Lane<1>& c) {
+  asm("{.reg .pred p;\n setp.ne.s32 p, %3, 0;\n @p fma.rn.f32 %0, %1, %0, %2;\n}" : "+f"(h.v) : "f"(m.v), "f"(c.v), "r"(static_cast<int>(p)));
+}
+__device__ __forceinline__ void fma_if(bool p, Lane<2>& h, const Lane<2>& m, const Lane<2>& c) {
+  asm("{.reg .pred p;\n .reg .b64 h, m, c;\n setp.ne.s32 p, %6, 0;\n mov.b64 h, {%0, %1};\n mov.b64 m, {%2, %3};\n mov.b64 c, {%4, %5};\n"
+      "@p fma.rn.f32x2 h, m, h, c;\n mov.b64 {%0, %1}, h;\n}"
+      : "+f"(h.v.x), "+f"(h.v.y) : "f"(m.v.x), "f"(m.v.y), "f"(c.v.x), "f"(c.v.y), "r"(static_cast<int>(p)));
+}
+
 // The maps of the warps before warp w (FORWARD: lower warps first) after each other, applied to h.
 template <int V, bool SEQ, bool FORWARD>
 __device__ __forceinline__ Lane<V> through_warps(const Lane<V>* A, const Lane<V>* H, unsigned cuts, int w, int lane, Lane<V> h) {
+  if (!SEQ || cuts == 0) {
 #pragma unroll
-  for (int i = 0; i < kRecWarps - 1; ++i) {
-    const int q = FORWARD ? i : kRecWarps - 1 - i;
-    const Lane<V> c = H[q * 32 + lane];
-    Lane<V> r = fma(A[q * 32 + lane], h, c);
-    if (SEQ && (cuts >> q & 1u)) r = c;
-    if (FORWARD ? q < w : q > w) h = r;
+    for (int i = 0; i < kRecWarps - 1; ++i) {
+      const int q = FORWARD ? i : kRecWarps - 1 - i;
+      fma_if(FORWARD ? q < w : q > w, h, A[q * 32 + lane], H[q * 32 + lane]);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < kRecWarps - 1; ++i) {
+      const int q = FORWARD ? i : kRecWarps - 1 - i;
+      if (FORWARD ? q >= w : q <= w) break;
+      const Lane<V> c = H[q * 32 + lane];
+      h = cuts >> q & 1u ? c : fma(A[q * 32 + lane], h, c);
+    }
   }
   return h;
 }
@@ -156,10 +180,24 @@ __device__ __forceinline__ Lane<V> through_cluster(const Lane<V>* A, const Lane<
 
 // What else a CTA keeps in shared memory: without a cluster, the state that one round's last
 // positions hand to the next round; the barriers.
+// ids of positions t0 - 1 .. t0 + 64 and (backward) the state before position t0 of the chunks
+// of four rounds, copied two rounds ahead.
 template <int V> struct Common {
   Lane<V> handed[2][32];
+  Lane<V> start[4][32];
+  int ids[4][kRecChunk + 4];
   uint64_t bars[kFwdStages + 2];
 };
+
+// Starts the copy of a round's ids; the caller commits.  Outside the sequence they are -1.
+__device__ __forceinline__ void load_ids(const RecArgs& a, int64_t b, int64_t t0, int* ids) {
+  const int i = threadIdx.x;
+  if (i >= kRecChunk + 2) return;
+  const int64_t t = t0 - 1 + i;
+  const int* from = static_cast<const int*>(a.seq_idx.data) + b * a.seq_idx.s0 + t * a.seq_idx.s1;
+  if (t >= 0 && t < a.seqlen) cp4(shared_addr(ids + i), from, 4);
+  else ids[i] = -1;
+}
 
 // The barriers of the ring (one per slot) and of the cluster's exchange (two).
 template <int S>
@@ -240,7 +278,18 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
   const L nb = gate_offset<T, LAYOUT>(a, p.d0, lane);
   L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.init, p.b, a.nstates, p.d0, a.dim, lane);
   if (w == 0) common.handed[0][lane] = carry;
-  int ids = SEQ ? load_ids(a, p.b, static_cast<int64_t>(p.rank) * kRecChunk + w * kRecSteps, lane) : 0;
+  auto copy_ids = [&](int k) {
+    if constexpr (SEQ) {
+      if (k < p.rounds) load_ids(a, p.b, (static_cast<int64_t>(k) * p.cluster + p.rank) * kRecChunk, common.ids[k & 3]);
+      cp_async_commit();
+    }
+  };
+  if constexpr (SEQ) {
+    copy_ids(0);
+    copy_ids(1);
+    cp_async_wait<0>();
+    __syncthreads();
+  }
 
   int slot = 0;
   unsigned parity = 0;
@@ -251,46 +300,37 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
     const int buf = k & 1;
     const bool there = mbar_wait(bars + 8 * slot, parity);
 
+    Edges e;
+    if constexpr (SEQ) {
+      e = edges_of(lane < kRecSteps + 2 ? common.ids[k & 3][w * kRecSteps + lane] : -1);
+      if (e.valid != 0xffu) {  // rare: positions without a token pass the state on
+        set_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, ~e.valid, kHold);
+        set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, ~e.valid, 0.f);
+        __syncwarp();
+      }
+    }
     // the 8 positions' maps and their composition
     L ga[kRecSteps], gb[kRecSteps];
-    {
-      L g[kRecSteps], x[kRecSteps];
-      read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, g);
-      read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, x);
-      gates<T, V>(g, nb, ga, g);
+    read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, ga);
+    read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, gb);
 #pragma unroll
-      for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(g[j], x[j]);
-      if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
+    for (int j = 0; j < kRecSteps; ++j) {
+      // 1 - a from a: a + (1 - a) is then exactly one, and the error of 2^-24 is that of a itself
+      ga[j] = sigmoids<T, V, false>(ga[j], nb, nullptr);
+      gb[j] = mul(sub(splat(1.f, L{}), ga[j]), gb[j]);
     }
-    Edges e;
-    unsigned valid = below(within(tw, a.seqlen, kRecSteps));
-    if constexpr (SEQ) {
-      e = edges_of(ids);
-      valid = e.valid;
-      ids = load_ids(a, p.b, tw + static_cast<int64_t>(p.cluster) * kRecChunk, lane);
-    }
-    L A, H;
-    const bool whole = valid == 0xffu && !(SEQ && e.first);
-    if (whole) {
-      A = ga[0];
-      H = gb[0];
+    if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
+    L A = ga[0], H = gb[0];
 #pragma unroll
-      for (int j = 1; j < kRecSteps; ++j) {
-        A = mul(ga[j], A);
-        H = fma(ga[j], H, gb[j]);
-      }
-    } else {
-      A = splat(1.f, L{});
-      H = splat(0.f, L{});
+    for (int j = 1; j < kRecSteps; ++j) {
+      A = mul(ga[j], A);
+      H = fma(ga[j], H, gb[j]);
+    }
+    if (SEQ && e.first) {  // a sequence starts here: H again, from its initial state
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
-        if (!(valid >> j & 1u)) {  // no token: the state passes
-          ga[j] = splat(1.f, L{});
-          gb[j] = splat(0.f, L{});
-        }
-        if (SEQ && (e.first >> j & 1u))
+        if (e.first >> j & 1u)
           H = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
-        A = mul(ga[j], A);
         H = fma(ga[j], H, gb[j]);
       }
     }
@@ -298,7 +338,9 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
     sum.A[w * 32 + lane] = A;
     sum.H[w * 32 + lane] = H;
     if (SEQ && lane == 0) sum.cut[w] = e.first;
+    if (SEQ) cp_async_wait<0>();  // the ids of the next round, for all after the barrier
     __syncthreads();
+    copy_ids(k + 2);
     if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
     if (tma && threadIdx.x == 0) tma_wait_read<1>();  // the slot to be loaded was stored a round ago
     load(k + S - 2);
@@ -315,44 +357,46 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
     }
 
     // the states themselves
+    if (SEQ && e.first) {
 #pragma unroll
-    for (int j = 0; j < kRecSteps; ++j) {
-      if (SEQ && !whole && (e.first >> j & 1u))
-        h = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
-      h = fma(ga[j], h, gb[j]);
-      gb[j] = h;
+      for (int j = 0; j < kRecSteps; ++j) {
+        if (e.first >> j & 1u)
+          h = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
+        h = fma(ga[j], h, gb[j]);
+        gb[j] = h;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRecSteps; ++j) {
+        h = fma(ga[j], h, gb[j]);
+        gb[j] = h;
+      }
     }
     if (p.cluster == 1 && w == kRecWarps - 1) common.handed[buf ^ 1][lane] = h;
-    if (SEQ && e.last && a.final_states.data) {
+    if (a.final_states.data && (SEQ ? e.last != 0 : tw < a.seqlen && tw + kRecSteps >= a.seqlen)) {
 #pragma unroll
-      for (int j = 0; j < kRecSteps; ++j)
-        if (e.last >> j & 1u)
-          store_state<T, LAYOUT>(a.final_states, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane, gb[j]);
+      for (int j = 0; j < kRecSteps; ++j) {
+        if constexpr (SEQ) {
+          if (e.last >> j & 1u)
+            store_state<T, LAYOUT>(a.final_states, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane, gb[j]);
+        } else {
+          if (tw + j == a.seqlen - 1) store_state<T, LAYOUT>(a.final_states, p.b, a.nstates, p.d0, a.dim, lane, gb[j]);
+        }
+      }
     }
     if constexpr (Z) {
       L z[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, zt, t0, w, lane, z);
 #pragma unroll
-      for (int j = 0; j < kRecSteps; ++j) {
-        L s;
-#pragma unroll
-        for (int i = 0; i < V; ++i) el(s, i) = silu_of<T>(el(z[j], i));
-        gb[j] = mul(gb[j], s);
-      }
-    }
-    if (SEQ && valid != 0xffu) {
-#pragma unroll
-      for (int j = 0; j < kRecSteps; ++j)
-        if (!(valid >> j & 1u)) gb[j] = splat(0.f, L{});
+      for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gb[j], mul(z[j], sigmoids<T, V, false>(z[j], splat(0.f, L{}), nullptr)));
     }
     write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gb);
+    if (SEQ && e.valid != 0xffu) clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~e.valid);
     if (tma) tma_fence();
     if (++slot == S) slot = 0, parity ^= 1;
   }
   __syncthreads();
   store(p.rounds - 1, slot == 0 ? S - 1 : slot - 1);
-  if (!SEQ && w == 0 && p.rank == 0)
-    store_state<T, LAYOUT>(a.final_states, p.b, a.nstates, p.d0, a.dim, lane, p.cluster == 1 ? common.handed[p.rounds & 1][lane] : carry);
   if (tma && threadIdx.x == 0) tma_wait_read<0>();
   if (p.cluster > 1) cluster_sync();  // no CTA leaves while a partner may still write to it
 }
@@ -431,26 +475,31 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_co
       if constexpr (Z) store_tile<T, LAYOUT, SKEW>(smem + o + 3 * C::kBytes, dzt, t0, p.nd, nt);
     }
   };
-  auto checkpoint = [&](int k) {
-    L r = splat(0.f, L{});
-    const int64_t c = chunk_of(k);
-    if (k < p.rounds && c < a.nchunks) {
-      const float* from = a.checkpoints + (p.b * a.nchunks + c) * a.dim + p.d0;
+  auto copy_ahead = [&](int k) {  // what round k needs besides the tiles
+    if (k < p.rounds) {
+      const int64_t c = chunk_of(k);
+      if (w == kRecWarps - 1) {
+        const float* from = a.checkpoints + (p.b * a.nchunks + c) * a.dim + p.d0;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int d = lane_channel<T, LAYOUT>(lane, i);
-        if (d < p.nd) el(r, i) = __ldg(from + d);
+        for (int i = 0; i < V; ++i) {
+          const int d = lane_channel<T, LAYOUT>(lane, i);
+          const bool in = c < a.nchunks && d < p.nd;
+          cp4(shared_addr(&common.start[k & 3][lane]) + 4 * i, in ? from + d : a.checkpoints, in ? 4 : 0);
+        }
       }
+      if constexpr (SEQ) load_ids(a, p.b, c * kRecChunk, common.ids[k & 3]);
     }
-    return r;
+    cp_async_commit();
   };
 #pragma unroll
   for (int k = 0; k < S - 2; ++k) load(k);
   const L nb = gate_offset<T, LAYOUT>(a, p.d0, lane);
   L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.dfinal, p.b, a.nstates, p.d0, a.dim, lane);
   if (w == 0) common.handed[0][lane] = carry;
-  L start = checkpoint(0);
-  int ids = SEQ ? load_ids(a, p.b, chunk_of(0) * kRecChunk + w * kRecSteps, lane) : 0;
+  copy_ahead(0);
+  copy_ahead(1);
+  cp_async_wait<0>();
+  __syncthreads();
   L bias_sum = splat(0.f, L{});
 
   int slot = 0;
@@ -461,11 +510,30 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_co
     const int buf = k & 1;
     const bool there = mbar_wait(bars + 8 * slot, parity);
 
+    Edges e;
+    unsigned valid = below(within(tw, a.seqlen, kRecSteps));
+    if constexpr (SEQ) {
+      e = edges_of(lane < kRecSteps + 2 ? common.ids[k & 3][w * kRecSteps + lane] : -1);
+      valid = e.valid;
+    }
+    if (valid != 0xffu) {  // rare: positions without a token pass the gradient on
+      set_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, ~valid, kHold);
+      set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, ~valid, 0.f);
+      set_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, yt, t0, w, lane, ~valid, 0.f);
+      if constexpr (Z) set_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, t0, w, lane, ~valid, 0.f);
+      __syncwarp();
+    }
     L ga[kRecSteps], gc[kRecSteps], x[kRecSteps], gy[kRecSteps], dz[kRecSteps];
     {
       L g[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, g);
-      gates<T, V>(g, nb, ga, gc);
+#pragma unroll
+      for (int j = 0; j < kRecSteps; ++j) {
+        // the gradients have 1 - a as a factor, so it is taken to full relative precision
+        L ex;
+        ga[j] = sigmoids<T, V, true>(g[j], nb, &ex);
+        gc[j] = mul(ex, ga[j]);
+      }
       if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
     }
     read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, x);
@@ -475,53 +543,33 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_co
       read_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, t0, w, lane, z);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
-        // silu(z) = z p and silu'(z) = p (1 + z (1 - p)), p = sigmoid(z)
-        L p, one = splat(1.f, L{});
-#pragma unroll
-        for (int i = 0; i < V; ++i) el(p, i) = sigmoid_of<T>(el(z[j], i));
-        dz[j] = mul(gy[j], mul(p, fma(z[j], sub(one, p), one)));
-        gy[j] = mul(gy[j], mul(z[j], p));
+        // silu(z) = z p and silu'(z) = p + z p (1 - p), p = sigmoid(z)
+        const L s = sigmoids<T, V, false>(z[j], splat(0.f, L{}), nullptr), zs = mul(z[j], s);
+        dz[j] = mul(gy[j], fma(zs, sub(splat(1.f, L{}), s), s));
+        gy[j] = mul(gy[j], zs);
       }
     }
-    Edges e;
-    unsigned valid = below(within(tw, a.seqlen, kRecSteps));
-    if constexpr (SEQ) {
-      e = edges_of(ids);
-      valid = e.valid;
-      ids = load_ids(a, p.b, tw - static_cast<int64_t>(p.cluster) * kRecChunk, lane);
+    L A = ga[0], H = mul(gc[0], x[0]);
+#pragma unroll
+    for (int j = 1; j < kRecSteps; ++j) {
+      A = mul(ga[j], A);
+      H = fma(ga[j], H, mul(gc[j], x[j]));
     }
-    const bool whole = valid == 0xffu && !(SEQ && (e.first || e.last));
-    L A, H, B;
-    if (whole) {
-      A = ga[0];
-      H = mul(gc[0], x[0]);
+    L B = mul(ga[kRecSteps - 1], gy[kRecSteps - 1]);
 #pragma unroll
-      for (int j = 1; j < kRecSteps; ++j) {
-        A = mul(ga[j], A);
-        H = fma(ga[j], H, mul(gc[j], x[j]));
-      }
-      B = mul(ga[kRecSteps - 1], gy[kRecSteps - 1]);
-#pragma unroll
-      for (int j = kRecSteps - 2; j >= 0; --j) B = mul(ga[j], add(gy[j], B));
-    } else {
-      A = splat(1.f, L{});
-      H = B = splat(0.f, L{});
+    for (int j = kRecSteps - 2; j >= 0; --j) B = mul(ga[j], add(gy[j], B));
+    if (SEQ && (e.first | e.last)) {  // a sequence starts or ends here
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
-        if (!(valid >> j & 1u)) {
-          ga[j] = splat(1.f, L{});
-          gc[j] = x[j] = gy[j] = splat(0.f, L{});
-        }
-        if (SEQ && (e.first >> j & 1u))
+        if (e.first >> j & 1u)
           H = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
-        A = mul(ga[j], A);
-        H = fma(ga[j], H, mul(gc[j], x[j]));
+        H = j == 0 && !(e.first & 1u) ? mul(gc[0], x[0]) : fma(ga[j], H, mul(gc[j], x[j]));
       }
 #pragma unroll
       for (int j = kRecSteps - 1; j >= 0; --j) {
-        if (SEQ && (e.last >> j & 1u))
+        if (e.last >> j & 1u)
           B = load_state<T, LAYOUT>(a.dfinal, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
-        B = mul(ga[j], add(gy[j], B));
+        B = j == kRecSteps - 1 && !(e.last >> j & 1u) ? mul(ga[j], gy[j]) : mul(ga[j], add(gy[j], B));
       }
     }
     Sums<V>& sum = sums[buf];
@@ -533,47 +581,66 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_co
       sum.cut[w] = e.first;
       sum_back.cut[w] = e.last;
     }
+    cp_async_wait<0>();  // what the next round needs, for all after the barrier
     __syncthreads();
+    copy_ahead(k + 2);
     if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
     if (tma && threadIdx.x == 0) tma_wait_read<1>();
     load(k + S - 2);
-    L h = through_warps<V, SEQ, true>(sum.A, sum.H, SEQ ? cuts_of(sum.cut, lane) : 0, w, lane, start);
-    start = checkpoint(k + 1);
+    L h = through_warps<V, SEQ, true>(sum.A, sum.H, SEQ ? cuts_of(sum.cut, lane) : 0, w, lane, common.start[k & 3][lane]);
     const unsigned cuts = SEQ ? cuts_of(sum_back.cut, lane) : 0;
     L s = p.cluster == 1 ? through_warps<V, SEQ, false>(sum.A, sum_back.B, cuts, w, lane, common.handed[buf][lane])
                          : through_cluster<V, SEQ, false>(sum.A, sum_back.B, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), (k >> 1) & 1, p, w, lane, carry);
 
     // forward through the positions: h before each, and dz
     L prev[kRecSteps];
+    if (SEQ && e.first) {
 #pragma unroll
-    for (int j = 0; j < kRecSteps; ++j) {
-      if (SEQ && !whole && (e.first >> j & 1u))
-        h = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
-      prev[j] = h;
-      h = fma(ga[j], h, mul(gc[j], x[j]));
-      if constexpr (Z) dz[j] = mul(dz[j], h);
+      for (int j = 0; j < kRecSteps; ++j) {
+        if (e.first >> j & 1u)
+          h = load_state<T, LAYOUT>(a.init, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
+        prev[j] = h;
+        h = fma(ga[j], h, mul(gc[j], x[j]));
+        if constexpr (Z) dz[j] = mul(dz[j], h);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRecSteps; ++j) {
+        prev[j] = h;
+        h = fma(ga[j], h, mul(gc[j], x[j]));
+        if constexpr (Z) dz[j] = mul(dz[j], h);
+      }
     }
     // and back: dx (in gy) and dgate (in prev)
-#pragma unroll
-    for (int j = kRecSteps - 1; j >= 0; --j) {
-      if (SEQ && !whole && (e.last >> j & 1u))
-        s = load_state<T, LAYOUT>(a.dfinal, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
+    auto step_back = [&](int j) {
       const L dh = add(gy[j], s);
       gy[j] = mul(dh, gc[j]);
       s = mul(ga[j], dh);
       prev[j] = mul(mul(s, gc[j]), sub(prev[j], x[j]));
-      if (!whole && !(valid >> j & 1u)) {
-        gy[j] = prev[j] = splat(0.f, L{});
-        if constexpr (Z) dz[j] = splat(0.f, L{});
-      }
       bias_sum = add(bias_sum, prev[j]);
-      if (SEQ && !whole && (e.first >> j & 1u))
-        store_state<T, LAYOUT>(a.dinit, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane, s);
+    };
+    if (SEQ && (e.first | e.last)) {
+#pragma unroll
+      for (int j = kRecSteps - 1; j >= 0; --j) {
+        if (e.last >> j & 1u)
+          s = load_state<T, LAYOUT>(a.dfinal, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane);
+        step_back(j);
+        if (e.first >> j & 1u)
+          store_state<T, LAYOUT>(a.dinit, __shfl_sync(0xffffffffu, e.id, j + 1), a.nstates, p.d0, a.dim, lane, s);
+      }
+    } else {
+#pragma unroll
+      for (int j = kRecSteps - 1; j >= 0; --j) step_back(j);
     }
     if (p.cluster == 1 && w == 0) common.handed[buf ^ 1][lane] = s;
     write_steps<T, LAYOUT, SKEW>(now, w, lane, prev);
     write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gy);
     if constexpr (Z) write_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, w, lane, dz);
+    if (SEQ && valid != 0xffu) {
+      clear_steps<T, LAYOUT, SKEW>(now, w, lane, ~valid);
+      clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~valid);
+      if constexpr (Z) clear_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, w, lane, ~valid);
+    }
     if (tma) tma_fence();
     if (++slot == S) slot = 0, parity ^= 1;
   }

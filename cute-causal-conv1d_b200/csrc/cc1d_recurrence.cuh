@@ -82,7 +82,7 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
     unsigned done;
     asm volatile(
         "{\n.reg .pred p;\n"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         "selp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     if (done) return true;
   }
@@ -287,6 +287,41 @@ __device__ __forceinline__ void write_steps(unsigned char* tile, int w, int lane
   }
 }
 
+// Sets the positions of `mask` among the warp's 8 to a value, in a tile as it was loaded.
+template <typename T, int LAYOUT, bool SKEW>
+__device__ __forceinline__ void set_steps(unsigned char* tile, const Strip<T>& t, int64_t t0, int w, int lane, unsigned mask, float value) {
+  using C = Tile<T, LAYOUT, SKEW>;
+#pragma unroll 1
+  for (int j = 0; j < kRecSteps; ++j) {
+    if (!(mask >> j & 1u)) continue;
+    const int pos = w * kRecSteps + j;
+#pragma unroll
+    for (int i = 0; i < C::V; ++i) {
+      const int ch = lane_channel<T, LAYOUT>(lane, i);
+      int o = C::at(ch, pos);
+      if constexpr (SKEW) {
+        const int r = C::kRows ? ch : pos;
+        const T* p = t.row + (C::kRows ? t0 + ch * t.s1 : (t0 + pos) * t.s2);
+        const int e = (C::kRows ? pos : ch) + (static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1);
+        o = e < 64 ? C::word(r, e >> 1) + (e & 1) * 2 : C::kEnds + 4 * r;
+      }
+      *reinterpret_cast<T*>(tile + o) = from_f32<T>(value);
+    }
+  }
+}
+// Clears them in a tile of results.
+template <typename T, int LAYOUT, bool SKEW>
+__device__ __forceinline__ void clear_steps(unsigned char* tile, int w, int lane, unsigned mask) {
+  using C = Tile<T, LAYOUT, SKEW>;
+#pragma unroll 1
+  for (int j = 0; j < kRecSteps; ++j) {
+    if (!(mask >> j & 1u)) continue;
+#pragma unroll
+    for (int i = 0; i < C::V; ++i)
+      *reinterpret_cast<T*>(tile + C::at(lane_channel<T, LAYOUT>(lane, i), w * kRecSteps + j)) = from_f32<T>(0.f);
+  }
+}
+
 // kWords and kElements, all threads: stores what write_steps put into a tile.
 template <typename T, int LAYOUT, bool SKEW>
 __device__ __forceinline__ void store_tile(const unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
@@ -334,12 +369,7 @@ struct Edges {
   unsigned valid, first, last;
   int id;
 };
-// ids of positions t - 1 .. t + 8, one per lane 0 .. 9; -1 outside the sequence.
-__device__ __forceinline__ int load_ids(const RecArgs& a, int64_t b, int64_t t, int lane) {
-  const int64_t p = t - 1 + lane;
-  if (lane > 9 || p < 0 || p >= a.seqlen) return -1;
-  return __ldg(static_cast<const int*>(a.seq_idx.data) + b * a.seq_idx.s0 + p * a.seq_idx.s1);
-}
+// From the ids of positions t - 1 .. t + 8, in lanes 0 .. 9.
 __device__ __forceinline__ Edges edges_of(int id) {
   constexpr unsigned all = 0xffffffffu;
   const int before = __shfl_up_sync(all, id, 1), after = __shfl_down_sync(all, id, 1);
