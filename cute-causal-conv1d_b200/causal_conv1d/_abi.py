@@ -327,7 +327,7 @@ def fwd_varlen_states(x, weight, bias, seq_idx, cu_seqlens, states, out, silu: b
 # Their params structs are made of 64-bit words only (a cc1d_tensor is five: data, dtype
 # with the reserved half zero, three strides), so one struct.pack fills them: a decode
 # step is short enough for the host's time per call to count.
-RECURRENCE_CHUNK = 64  # CC1D_RECURRENCE_CHUNK
+RECURRENCE_CHUNK = 32  # CC1D_RECURRENCE_CHUNK
 _NONE = (0, 0, 0, 0, 0)
 RECURRENCE_PARAMS = struct.Struct("<78q")
 RECURRENCE_UPDATE_PARAMS = struct.Struct("<39q")

@@ -1,6 +1,7 @@
 // extern "C" launchers of the recurrent-block operators: the gated recurrence, its token
 // update, and dropout + residual add + RMSNorm.  Argument checks happen here, before any
 // launch; include/causal_conv1d_b200.h states the contract.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -76,19 +77,20 @@ int sm_count() {
 }
 
 // CTAs that share a tile.  Each takes 1/cluster of the chunks.  The estimate counts chunk
-// times: a CTA pays its start (about 3 chunks until its first tiles are there), a cluster's
-// exchange lengthens a chunk by a fifth, and an SM with one CTA takes 0.6 of the time that two
-// need for a chunk each.  Two CTAs fit an SM while their shared memory (`smem`, and 1 KB for
-// each CTA of the cluster) does.
+// times: a CTA pays its start (about 4 chunks until its first tiles are there), a cluster's
+// exchange lengthens a chunk by half, and n CTAs on an SM take (2 + n) / 3 of the time that one
+// needs for a chunk each.  As many fit as their shared memory (`smem`, and 1 KB for each CTA of
+// the cluster) allows, at most 4.
 int choose_cluster(int64_t tiles, int64_t chunks, int64_t smem) {
   const int64_t sms = sm_count();
   double best = 0;
   int pick = 1;
+  auto time = [](double n) { return (2.0 + n) / 3.0; };
   for (int c = 1; c <= 16 && c <= chunks; c *= 2) {
-    const bool two = smem + (c > 1 ? c * 1024 : 0) <= 113 * 1024;
-    const int64_t ctas = tiles * c, slots = two ? 2 * sms : sms, rest = ctas % slots;
-    const double per_cta = (static_cast<double>((chunks + c - 1) / c) + 3.0) * (c > 1 ? 1.2 : 1.0);
-    const double waves = static_cast<double>(ctas / slots) * (two ? 1.0 : 0.6) + (rest == 0 ? 0.0 : rest <= sms ? 0.6 : 1.0);
+    const int64_t bytes = smem + (c > 1 ? c * 1024 : 0) + 1024;
+    const int64_t fit = std::min<int64_t>(4, 228 * 1024 / bytes), slots = fit * sms, ctas = tiles * c, rest = ctas % slots;
+    const double per_cta = (static_cast<double>((chunks + c - 1) / c) + 4.0) * (c > 1 ? 1.5 : 1.0);
+    const double waves = static_cast<double>(ctas / slots) * time(fit) + (rest ? time((rest + sms - 1) / sms) : 0.0);
     if (c == 1 || per_cta * waves < best) {
       best = per_cta * waves;
       pick = c;
@@ -119,8 +121,8 @@ cc1d_status rec_plan(RecArgs* a, bool bwd) {
   const int64_t channels = a->x.dtype == CC1D_FLOAT32 ? 32 : 64;
   a->dtiles = (a->dim + channels - 1) / channels;
   const int64_t tiles = a->batch * a->dtiles;
-  const int64_t tile = 8192 + (a->move == kWords ? 256 : 0), z = a->z.data ? 1 : 0;
-  a->cluster = choose_cluster(tiles, a->nchunks, bwd ? 3 * (3 + z) * tile + 15 * 1024 : 4 * (2 + z) * tile + 11 * 1024);
+  const int64_t tile = 4096 + (a->move == kWords ? 256 : 0), z = a->z.data ? 1 : 0;
+  a->cluster = choose_cluster(tiles, a->nchunks, bwd ? 3 * (3 + z) * tile + 8064 : 4 * (2 + z) * tile + 6016);
   if (tiles * a->cluster > kMax31) return fail(CC1D_ERR_VALUE, "batch * dim is too large");
   return CC1D_OK;
 }

@@ -5,11 +5,18 @@
 
 namespace cc1d {
 
-// min(v, 1e30) that keeps a NaN: 1 + e and e / (1 + e) stay finite where exp overflows, and
-// the other sigmoid is then 1e-30, zero to working precision.
-__device__ __forceinline__ float clamp_exp(float v) {
+// min(v, most) that keeps a NaN: e / (1 + e) stays finite where exp overflows, and 1 / (1 + e)
+// is then zero to working precision.
+__device__ __forceinline__ float clamp_exp(float v, float most) {
   float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(1e30f));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+  return r;
+}
+
+// The larger of two, or NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
@@ -17,8 +24,8 @@ __device__ __forceinline__ float clamp_exp(float v) {
 // error about 2^-22, plus the rounding of u log2(e)); for fp32 the library's exp.
 template <typename T>
 __device__ __forceinline__ float exp_minus(float u) {
-  if constexpr (std::is_same<T, float>::value) return clamp_exp(expf(-u));
-  else return clamp_exp(ex2_approx(-kLog2e * u));
+  if constexpr (std::is_same<T, float>::value) return clamp_exp(expf(-u), 1e30f);
+  else return clamp_exp(ex2_approx(-kLog2e * u), 1e30f);
 }
 template <typename T>
 __device__ __forceinline__ float reciprocal(float v) {

@@ -11,7 +11,7 @@
 //
 // A position is the affine map h -> a h + c x, and maps compose, so a stretch of positions is
 // summed up by two numbers per channel.  Each warp does that for its 8 positions of a chunk,
-// from registers; the CTA's 8 warps exchange the sums through shared memory, and each then
+// from registers; the CTA's 4 warps exchange the sums through shared memory, and each then
 // knows the state its positions start from and goes through them once more, still from
 // registers.  The inputs are read once, into a ring of shared-memory tiles a few chunks
 // ahead.  The backward does the same in both directions at once: the forward direction from
@@ -32,29 +32,59 @@ namespace {
 // tiles, and one (backward) or two chunks that are being loaded.
 constexpr int kFwdStages = 4, kBwdStages = 3;
 
-// 1 / (1 + exp(-v)) of a lane's channels; e, if wanted, is exp(-v), at most 1e30 so that e / (1 + e)
-// is right where exp overflows (1 / (1 + inf) needs no care).  For 16-bit tensors m and n give
-// -v log2(e) = v m + n, for fp32 n is added to v.
-template <typename T, int V, bool E>
-__device__ __forceinline__ Lane<V> sigmoids(const Lane<V>& v, const Lane<V>& n, Lane<V>* e) {
-  Lane<V> x, r;
+// s = 1 / (1 + exp(-v)) at a warp's 8 positions, and e = exp(-v) if wanted.  For 16-bit tensors
+// -v log2(e) = v m + n with m = -log2(e), for fp32 n is added to v.
+//
+// 16-bit: four positions share one reciprocal, of the product of their 1 + e (the special
+// function unit would bound the forward otherwise: 4 of its operations per element, now 2.5).
+// So that the product stays finite e is at most 2^30 and a sigmoid at least 2^-30, which is
+// zero next to the other terms of a sum; the three more roundings leave 2^-22.  A NaN must not
+// reach the others of its four: the minimum drops it, and KEEP puts it back into its own
+// sigmoid (silu has it from z).
+template <typename T, int V, bool E, bool KEEP>
+__device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const Lane<V>& n, Lane<V> (&s)[kRecSteps], Lane<V>* e) {
   if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) el(x, i) = expf(-(el(v, i) + el(n, i)));
+    for (int j = 0; j < kRecSteps; ++j) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float x = clamp_exp(expf(-(el(v[j], i) + el(n, i))), 1e30f);
+        if constexpr (E) el(e[j], i) = x;
+        el(s[j], i) = __frcp_rn(1.f + x);
+      }
+    }
   } else {
-    x = fma(v, splat(-kLog2e, v), n);
 #pragma unroll
-    for (int i = 0; i < V; ++i) el(x, i) = ex2_approx(el(x, i));
+    for (int q = 0; q < kRecSteps; q += 4) {
+      Lane<V> d[4], raw[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        Lane<V> x = fma(v[q + j], splat(-kLog2e, n), n);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          el(raw[j], i) = ex2_approx(el(x, i));
+          el(x, i) = fminf(el(raw[j], i), 1073741824.f);
+        }
+        if constexpr (E) e[q + j] = x;
+        d[j] = add(x, splat(1.f, x));
+      }
+      const Lane<V> lo = mul(d[0], d[1]), hi = mul(d[2], d[3]);
+      Lane<V> r = mul(lo, hi);
+#pragma unroll
+      for (int i = 0; i < V; ++i) el(r, i) = rcp_approx(el(r, i));
+      const Lane<V> rlo = mul(r, hi), rhi = mul(r, lo);
+      s[q] = mul(rlo, d[1]);
+      s[q + 1] = mul(rlo, d[0]);
+      s[q + 2] = mul(rhi, d[3]);
+      s[q + 3] = mul(rhi, d[2]);
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) el(s[q + j], i) = max_nan(el(s[q + j], i), -el(raw[j], i));
+      }
+    }
   }
-  if constexpr (E) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) el(x, i) = clamp_exp(el(x, i));
-    *e = x;
-  }
-  r = add(x, splat(1.f, x));
-#pragma unroll
-  for (int i = 0; i < V; ++i) el(r, i) = reciprocal<T>(el(r, i));
-  return r;
 }
 
 template <typename T, int LAYOUT>
@@ -180,12 +210,12 @@ __device__ __forceinline__ Lane<V> through_cluster(const Lane<V>* A, const Lane<
 
 // What else a CTA keeps in shared memory: without a cluster, the state that one round's last
 // positions hand to the next round; the barriers.
-// ids of positions t0 - 1 .. t0 + 64 and (backward) the state before position t0 of the chunks
-// of four rounds, copied two rounds ahead.
+// ids of positions t0 - 1 .. t0 + 32 and (backward) the state before position t0 of the chunks
+// of three rounds, copied two rounds ahead.
 template <int V> struct Common {
   Lane<V> handed[2][32];
-  Lane<V> start[4][32];
-  int ids[4][kRecChunk + 4];
+  Lane<V> start[3][32];
+  int ids[3][kRecChunk + 4];
   uint64_t bars[kFwdStages + 2];
 };
 
@@ -213,7 +243,7 @@ __device__ __forceinline__ void start_barriers(unsigned bars, bool tma, int clus
 }
 
 template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z>
-__global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
+__global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int V = C::V, NT = Z ? 3 : 2, S = kFwdStages;
   using L = Lane<V>;
@@ -242,9 +272,9 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
         if (threadIdx.x == 0) {
           if (nt > 0) {
             mbar_expect(bar, NT * C::kBytes);
-            tma_load<T, LAYOUT>(ring + o, gt.map, p.d0, t0, p.b, bar);
-            tma_load<T, LAYOUT>(ring + o + C::kBytes, xt.map, p.d0, t0, p.b, bar);
-            if constexpr (Z) tma_load<T, LAYOUT>(ring + o + 2 * C::kBytes, zt.map, p.d0, t0, p.b, bar);
+            tma_load<LAYOUT>(ring + o, gt.map, p.d0, t0, p.b, bar);
+            tma_load<LAYOUT>(ring + o + C::kBytes, xt.map, p.d0, t0, p.b, bar);
+            if constexpr (Z) tma_load<LAYOUT>(ring + o + 2 * C::kBytes, zt.map, p.d0, t0, p.b, bar);
           } else {
             mbar_arrive(bar);
           }
@@ -266,7 +296,7 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
     const int nt = within(t0, a.seqlen, kRecChunk), o = slot * NT * C::kBytes + C::kBytes;
     if (tma) {
       if (threadIdx.x == 0) {
-        if (nt > 0) tma_store<T, LAYOUT>(ring + o, ot.map, p.d0, t0, p.b);
+        if (nt > 0) tma_store<LAYOUT>(ring + o, ot.map, p.d0, t0, p.b);
         tma_commit();
       }
     } else if (nt > 0) {
@@ -280,7 +310,7 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
   if (w == 0) common.handed[0][lane] = carry;
   auto copy_ids = [&](int k) {
     if constexpr (SEQ) {
-      if (k < p.rounds) load_ids(a, p.b, (static_cast<int64_t>(k) * p.cluster + p.rank) * kRecChunk, common.ids[k & 3]);
+      if (k < p.rounds) load_ids(a, p.b, (static_cast<int64_t>(k) * p.cluster + p.rank) * kRecChunk, common.ids[k % 3]);
       cp_async_commit();
     }
   };
@@ -302,7 +332,7 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
 
     Edges e;
     if constexpr (SEQ) {
-      e = edges_of(lane < kRecSteps + 2 ? common.ids[k & 3][w * kRecSteps + lane] : -1);
+      e = edges_of(lane < kRecSteps + 2 ? common.ids[k % 3][w * kRecSteps + lane] : -1);
       if (e.valid != 0xffu) {  // rare: positions without a token pass the state on
         set_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, ~e.valid, kHold);
         set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, ~e.valid, 0.f);
@@ -313,12 +343,10 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
     L ga[kRecSteps], gb[kRecSteps];
     read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, ga);
     read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, gb);
+    sigmoids<T, V, false, true>(ga, nb, ga, nullptr);
+    // 1 - a from a: a + (1 - a) is then exactly one, and the error of 2^-24 is that of a itself
 #pragma unroll
-    for (int j = 0; j < kRecSteps; ++j) {
-      // 1 - a from a: a + (1 - a) is then exactly one, and the error of 2^-24 is that of a itself
-      ga[j] = sigmoids<T, V, false>(ga[j], nb, nullptr);
-      gb[j] = mul(sub(splat(1.f, L{}), ga[j]), gb[j]);
-    }
+    for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(sub(splat(1.f, L{}), ga[j]), gb[j]);
     if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
     L A = ga[0], H = gb[0];
 #pragma unroll
@@ -385,10 +413,11 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
       }
     }
     if constexpr (Z) {
-      L z[kRecSteps];
+      L z[kRecSteps], s[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, zt, t0, w, lane, z);
+      sigmoids<T, V, false, false>(z, splat(0.f, L{}), s, nullptr);
 #pragma unroll
-      for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gb[j], mul(z[j], sigmoids<T, V, false>(z[j], splat(0.f, L{}), nullptr)));
+      for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gb[j], mul(z[j], s[j]));
     }
     write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gb);
     if (SEQ && e.valid != 0xffu) clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~e.valid);
@@ -402,7 +431,7 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_fwd_kernel(const __grid_co
 }
 
 template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z>
-__global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
+__global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int V = C::V, NT = Z ? 4 : 3, S = kBwdStages;
   using L = Lane<V>;
@@ -436,10 +465,10 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_co
         if (threadIdx.x == 0) {
           if (nt > 0) {
             mbar_expect(bar, NT * C::kBytes);
-            tma_load<T, LAYOUT>(ring + o, gt.map, p.d0, t0, p.b, bar);
-            tma_load<T, LAYOUT>(ring + o + C::kBytes, xt.map, p.d0, t0, p.b, bar);
-            tma_load<T, LAYOUT>(ring + o + 2 * C::kBytes, yt.map, p.d0, t0, p.b, bar);
-            if constexpr (Z) tma_load<T, LAYOUT>(ring + o + 3 * C::kBytes, zt.map, p.d0, t0, p.b, bar);
+            tma_load<LAYOUT>(ring + o, gt.map, p.d0, t0, p.b, bar);
+            tma_load<LAYOUT>(ring + o + C::kBytes, xt.map, p.d0, t0, p.b, bar);
+            tma_load<LAYOUT>(ring + o + 2 * C::kBytes, yt.map, p.d0, t0, p.b, bar);
+            if constexpr (Z) tma_load<LAYOUT>(ring + o + 3 * C::kBytes, zt.map, p.d0, t0, p.b, bar);
           } else {
             mbar_arrive(bar);
           }
@@ -463,9 +492,9 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_co
     if (tma) {
       if (threadIdx.x == 0) {
         if (nt > 0) {
-          tma_store<T, LAYOUT>(ring + o, dgt.map, p.d0, t0, p.b);
-          tma_store<T, LAYOUT>(ring + o + C::kBytes, dxt.map, p.d0, t0, p.b);
-          if constexpr (Z) tma_store<T, LAYOUT>(ring + o + 3 * C::kBytes, dzt.map, p.d0, t0, p.b);
+          tma_store<LAYOUT>(ring + o, dgt.map, p.d0, t0, p.b);
+          tma_store<LAYOUT>(ring + o + C::kBytes, dxt.map, p.d0, t0, p.b);
+          if constexpr (Z) tma_store<LAYOUT>(ring + o + 3 * C::kBytes, dzt.map, p.d0, t0, p.b);
         }
         tma_commit();
       }
@@ -484,10 +513,10 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_co
         for (int i = 0; i < V; ++i) {
           const int d = lane_channel<T, LAYOUT>(lane, i);
           const bool in = c < a.nchunks && d < p.nd;
-          cp4(shared_addr(&common.start[k & 3][lane]) + 4 * i, in ? from + d : a.checkpoints, in ? 4 : 0);
+          cp4(shared_addr(&common.start[k % 3][lane]) + 4 * i, in ? from + d : a.checkpoints, in ? 4 : 0);
         }
       }
-      if constexpr (SEQ) load_ids(a, p.b, c * kRecChunk, common.ids[k & 3]);
+      if constexpr (SEQ) load_ids(a, p.b, c * kRecChunk, common.ids[k % 3]);
     }
     cp_async_commit();
   };
@@ -513,7 +542,7 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_co
     Edges e;
     unsigned valid = below(within(tw, a.seqlen, kRecSteps));
     if constexpr (SEQ) {
-      e = edges_of(lane < kRecSteps + 2 ? common.ids[k & 3][w * kRecSteps + lane] : -1);
+      e = edges_of(lane < kRecSteps + 2 ? common.ids[k % 3][w * kRecSteps + lane] : -1);
       valid = e.valid;
     }
     if (valid != 0xffu) {  // rare: positions without a token pass the gradient on
@@ -527,25 +556,23 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_co
     {
       L g[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, g);
+      // the gradients have 1 - a as a factor, so it is taken to full relative precision
+      sigmoids<T, V, true, true>(g, nb, ga, gc);
 #pragma unroll
-      for (int j = 0; j < kRecSteps; ++j) {
-        // the gradients have 1 - a as a factor, so it is taken to full relative precision
-        L ex;
-        ga[j] = sigmoids<T, V, true>(g[j], nb, &ex);
-        gc[j] = mul(ex, ga[j]);
-      }
+      for (int j = 0; j < kRecSteps; ++j) gc[j] = mul(gc[j], ga[j]);
       if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
     }
     read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, x);
     read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, yt, t0, w, lane, gy);
     if constexpr (Z) {
-      L z[kRecSteps];
+      L z[kRecSteps], s[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, t0, w, lane, z);
+      sigmoids<T, V, false, false>(z, splat(0.f, L{}), s, nullptr);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
-        // silu(z) = z p and silu'(z) = p + z p (1 - p), p = sigmoid(z)
-        const L s = sigmoids<T, V, false>(z[j], splat(0.f, L{}), nullptr), zs = mul(z[j], s);
-        dz[j] = mul(gy[j], fma(zs, sub(splat(1.f, L{}), s), s));
+        // silu(z) = z s and silu'(z) = s + z s (1 - s), s = sigmoid(z)
+        const L zs = mul(z[j], s[j]);
+        dz[j] = mul(gy[j], fma(zs, sub(splat(1.f, L{}), s[j]), s[j]));
         gy[j] = mul(gy[j], zs);
       }
     }
@@ -587,7 +614,7 @@ __global__ void __launch_bounds__(kRecThreads, 2) rec_bwd_kernel(const __grid_co
     if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
     if (tma && threadIdx.x == 0) tma_wait_read<1>();
     load(k + S - 2);
-    L h = through_warps<V, SEQ, true>(sum.A, sum.H, SEQ ? cuts_of(sum.cut, lane) : 0, w, lane, common.start[k & 3][lane]);
+    L h = through_warps<V, SEQ, true>(sum.A, sum.H, SEQ ? cuts_of(sum.cut, lane) : 0, w, lane, common.start[k % 3][lane]);
     const unsigned cuts = SEQ ? cuts_of(sum_back.cut, lane) : 0;
     L s = p.cluster == 1 ? through_warps<V, SEQ, false>(sum.A, sum_back.B, cuts, w, lane, common.handed[buf][lane])
                          : through_cluster<V, SEQ, false>(sum.A, sum_back.B, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), (k >> 1) & 1, p, w, lane, carry);
@@ -713,7 +740,7 @@ __global__ void __launch_bounds__(kThreads) rec_update_kernel(const RecUpdateArg
 unsigned blocks_for(int64_t threads) { return static_cast<unsigned>((threads + kThreads - 1) / kThreads); }
 
 // The tensor map of a strip-wise aligned tensor; channel-last (dim, seqlen, batch), rows
-// (seqlen, dim, batch), boxes of 128 bytes by the tile's other extent.
+// (seqlen, dim, batch), boxes of a tile's strips.
 template <typename T, int LAYOUT>
 bool make_map(CUtensorMap* map, const TensorArg& t, const RecArgs& a) {
   if (!t.data) return true;
@@ -732,10 +759,10 @@ bool make_map(CUtensorMap* map, const TensorArg& t, const RecArgs& a) {
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(a.batch)};
   // an extent of one never uses its stride, which may then be anything
   const cuuint64_t strides[2] = {outer > 1 ? static_cast<cuuint64_t>(step) * sizeof(T) : 16, a.batch > 1 ? static_cast<cuuint64_t>(t.s0) * sizeof(T) : 16};
-  const cuuint32_t box[3] = {128 / sizeof(T), static_cast<cuuint32_t>(C::kRows ? C::kChannels : kRecChunk), 1};
+  const cuuint32_t box[3] = {C::kStripBytes / sizeof(T), static_cast<cuuint32_t>(C::kStrips), 1};
   const cuuint32_t one[3] = {1, 1, 1};
   return encode(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, t.data, dims, strides, box, one,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, C::kRows ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, !C::kRows ? CU_TENSOR_MAP_SWIZZLE_NONE : C::kStripBytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

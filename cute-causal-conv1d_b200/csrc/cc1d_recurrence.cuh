@@ -2,7 +2,7 @@
 // their loads and stores, sequence boundaries and the exchange within a cluster.
 //
 // A CTA owns a tile of 128 bytes of channels of one batch row and walks the sequence in
-// chunks of 64 positions; warp w has the 8 positions 8w .. 8w+7 of each chunk and its lanes
+// chunks of 32 positions; warp w has the 8 positions 8w .. 8w+7 of each chunk and its lanes
 // the tile's channels.  So every boundary between sequences is uniform over a warp, in both
 // memory layouts.
 #pragma once
@@ -18,7 +18,7 @@ struct RecMaps {
   CUtensorMap gate, x, z, out, dout, dx, dgate, dz;
 };
 
-constexpr int kRecWarps = 8;
+constexpr int kRecWarps = 4;
 constexpr int kRecThreads = 32 * kRecWarps;
 constexpr int kRecSteps = kRecChunk / kRecWarps;  // positions of a warp in a chunk
 static_assert(kRecSteps == 8, "the tiles' packets and the boundary masks hold 8 positions");
@@ -91,29 +91,32 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
 
 // ----------------------------------------------------------------------------- the tiles
 // SKEW (kWords): a strip lies in its tile as it does in memory, half a word late where it
-// starts in the middle of one, so it takes 33 words.
+// starts in the middle of one, so it takes one word more.
 //
-// channel-last: 64 rows (positions) of 128 bytes of channels.
-// rows: a row of positions per channel, in 16-byte packets; packet p of row r is at p ^ (r % 8)
-// (the TMA's 128-byte swizzle), so that 8 lanes reading a packet of 8 channels use all banks.
-// fp32 has two such halves of 32 positions each.  SKEW: the 33rd words follow.
+// channel-last: 32 strips (positions) of 128 bytes of channels.
+// rows: strips of 32 positions, one per channel, in 16-byte packets that are swapped around as
+// the TMA's swizzles do, so that 8 lanes reading the same packet of 8 channels use all banks.
 template <typename T, int LAYOUT, bool SKEW> struct Tile {
   static constexpr int kSize = sizeof(T);
   static constexpr int V = 4 / kSize;                // channels per lane
   static constexpr int kChannels = 32 * V;           // 128 bytes
   static constexpr int kPacket = 16 / kSize;         // elements per 16 bytes
   static constexpr bool kRows = LAYOUT == kLayoutRows;
-  static constexpr int kBytes = 8192 + (SKEW ? 256 : 0);
-  static constexpr int kEnds = 8192;                 // SKEW: the 33rd words (of 64 strips)
+  static constexpr int kStrips = kRows ? kChannels : kRecChunk;
+  static constexpr int kStripBytes = kRows ? kRecChunk * kSize : 128;
+  static constexpr int kStripWords = kStripBytes / 4;
+  static constexpr int kEnds = kStrips * kStripBytes;  // SKEW: the strips' last words
+  static constexpr int kBytes = kEnds + (SKEW ? kStrips * 4 : 0);
+  static_assert(kEnds == 4096 && (!kRows || kStripBytes == 64 || kStripBytes == 128), "");
+  // byte of word i of strip r, without the last
+  static __device__ __forceinline__ int word(int r, int i) {
+    const int swap = !kRows ? 0 : kStripBytes == 128 ? r & 7 : (r >> 1) & 3;
+    return r * kStripBytes + (((i >> 2) ^ swap) << 4) + (i & 3) * 4;
+  }
   // byte of element (channel, position) without a skew
   static __device__ __forceinline__ int at(int ch, int pos) {
-    if constexpr (!kRows) return pos * 128 + ch * kSize;
-    const int byte = pos * kSize;
-    return (byte >> 7) * (kChannels * 128) + ch * 128 + ((((byte >> 4) & 7) ^ (ch & 7)) << 4) + (byte & 15);
-  }
-  // byte of word i (0 .. 31) of strip r: a position channel-last, a channel with rows
-  static __device__ __forceinline__ int word(int r, int i) {
-    return kRows ? r * 128 + ((((i >> 2) ^ r) & 7) << 4) + (i & 3) * 4 : r * 128 + i * 4;
+    const int byte = (kRows ? pos : ch) * kSize;
+    return word(kRows ? ch : pos, byte >> 2) + (byte & 3);
   }
 };
 
@@ -144,21 +147,15 @@ __device__ __forceinline__ void cp4(unsigned dst, const void* src, int bytes) {
 }
 
 // kTma, one thread: the copy of a chunk into its tile, counted on `bar`; and back.
-template <typename T, int LAYOUT>
+template <int LAYOUT>
 __device__ __forceinline__ void tma_load(unsigned tile, const CUtensorMap* map, int d0, int t0, int b, unsigned bar) {
-  constexpr bool rows = LAYOUT == kLayoutRows;
-#pragma unroll
-  for (int h = 0; h < (rows ? static_cast<int>(sizeof(T)) / 2 : 1); ++h)
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(tile + h * 4096),
-                 "l"(map), "r"(rows ? t0 + h * 32 : d0), "r"(rows ? d0 : t0), "r"(b), "r"(bar) : "memory");
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(tile),
+               "l"(map), "r"(LAYOUT == kLayoutRows ? t0 : d0), "r"(LAYOUT == kLayoutRows ? d0 : t0), "r"(b), "r"(bar) : "memory");
 }
-template <typename T, int LAYOUT>
+template <int LAYOUT>
 __device__ __forceinline__ void tma_store(unsigned tile, const CUtensorMap* map, int d0, int t0, int b) {
-  constexpr bool rows = LAYOUT == kLayoutRows;
-#pragma unroll
-  for (int h = 0; h < (rows ? static_cast<int>(sizeof(T)) / 2 : 1); ++h)
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n" ::"l"(map),
-                 "r"(rows ? t0 + h * 32 : d0), "r"(rows ? d0 : t0), "r"(b), "r"(tile + h * 4096) : "memory");
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n" ::"l"(map),
+               "r"(LAYOUT == kLayoutRows ? t0 : d0), "r"(LAYOUT == kLayoutRows ? d0 : t0), "r"(b), "r"(tile) : "memory");
 }
 __device__ __forceinline__ void tma_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
 // At most N committed groups still read shared memory.
@@ -171,7 +168,6 @@ __device__ __forceinline__ void tma_fence() { asm volatile("fence.proxy.async.sh
 template <typename T, int LAYOUT, bool SKEW>
 __device__ __forceinline__ void load_tile(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
   using C = Tile<T, LAYOUT, SKEW>;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const unsigned base = shared_addr(tile);
   if constexpr (SKEW) {
     const int64_t step = C::kRows ? t.s1 : t.s2;
@@ -190,8 +186,11 @@ __device__ __forceinline__ void load_tile(unsigned char* tile, const Strip<T>& t
       }
     };
 #pragma unroll
-    for (int k = 0; k < 8; ++k) word(w * 8 + k, lane, C::word(w * 8 + k, lane));
-    if (threadIdx.x < 64) word(threadIdx.x, 32, C::kEnds + threadIdx.x * 4);
+    for (int k = 0; k < 1024 / kRecThreads; ++k) {
+      const int i = threadIdx.x + k * kRecThreads, r = i / C::kStripWords;
+      word(r, i % C::kStripWords, C::word(r, i % C::kStripWords));
+    }
+    if (threadIdx.x < C::kStrips) word(threadIdx.x, C::kStripWords, C::kEnds + threadIdx.x * 4);
   } else {
     const T* const src = t.row + t0 * t.s2;
     constexpr int N = C::kChannels * kRecChunk / kRecThreads;
@@ -222,7 +221,7 @@ __device__ __forceinline__ void read_steps(const unsigned char* tile, const Stri
       for (int q = 0; q < kRecSteps / C::kPacket; ++q) {
         uint4 u = *reinterpret_cast<const uint4*>(tile + C::at(ch, w * kRecSteps + q * C::kPacket));
         if constexpr (SKEW) {
-          const uint32_t next = *reinterpret_cast<const uint32_t*>(tile + (w < 7 ? C::word(ch, 4 * w + 4) : C::kEnds + 4 * ch));
+          const uint32_t next = *reinterpret_cast<const uint32_t*>(tile + (w < kRecWarps - 1 ? C::word(ch, 4 * w + 4) : C::kEnds + 4 * ch));
           const unsigned sh = (reinterpret_cast<uintptr_t>(t.row + t0 + ch * t.s1) & 2) * 8;
           u = make_uint4(__funnelshift_r(u.x, u.y, sh), __funnelshift_r(u.y, u.z, sh), __funnelshift_r(u.z, u.w, sh),
                          __funnelshift_r(u.w, next, sh));
@@ -303,7 +302,7 @@ __device__ __forceinline__ void set_steps(unsigned char* tile, const Strip<T>& t
         const int r = C::kRows ? ch : pos;
         const T* p = t.row + (C::kRows ? t0 + ch * t.s1 : (t0 + pos) * t.s2);
         const int e = (C::kRows ? pos : ch) + (static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1);
-        o = e < 64 ? C::word(r, e >> 1) + (e & 1) * 2 : C::kEnds + 4 * r;
+        o = e < 2 * C::kStripWords ? C::word(r, e >> 1) + (e & 1) * 2 : C::kEnds + 4 * r;
       }
       *reinterpret_cast<T*>(tile + o) = from_f32<T>(value);
     }
@@ -326,7 +325,6 @@ __device__ __forceinline__ void clear_steps(unsigned char* tile, int w, int lane
 template <typename T, int LAYOUT, bool SKEW>
 __device__ __forceinline__ void store_tile(const unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
   using C = Tile<T, LAYOUT, SKEW>;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   if constexpr (SKEW) {
     const int64_t step = C::kRows ? t.s1 : t.s2;
     const int strips = C::kRows ? nd : nt, len = C::kRows ? nt : nd;
@@ -349,8 +347,8 @@ __device__ __forceinline__ void store_tile(const unsigned char* tile, const Stri
       }
     };
 #pragma unroll
-    for (int k = 0; k < 8; ++k) word(w * 8 + k, lane);
-    if (threadIdx.x < 64) word(threadIdx.x, 32);
+    for (int k = 0; k < 1024 / kRecThreads; ++k) word((threadIdx.x + k * kRecThreads) / C::kStripWords, (threadIdx.x + k * kRecThreads) % C::kStripWords);
+    if (threadIdx.x < C::kStrips) word(threadIdx.x, C::kStripWords);
   } else {
     T* const dst = t.row + t0 * t.s2;
 #pragma unroll 4

@@ -267,7 +267,7 @@ cc1d_status cc1d_fwd_varlen_states_launch(const cc1d_fwd_varlen_states_params* p
  * dout (batch, dim, seqlen) has x's dtype; dfinal_states (nstates, dim) fp32 is optional.
  * The forward ignores the gradient fields and the backward final_states and out.
  */
-#define CC1D_RECURRENCE_CHUNK 64
+#define CC1D_RECURRENCE_CHUNK 32
 
 typedef struct cc1d_recurrence_params {
   int64_t batch, dim, seqlen, nstates;

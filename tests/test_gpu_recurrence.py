@@ -171,6 +171,38 @@ def test_nan_travels_within_its_sequence():
             assert bad[1, 3, 50:].all() and bad.sum() == 100 and torch.isnan(final).sum() == 1
 
 
+@pytest.mark.parametrize("layout", ["channel_last", "contiguous"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", ["x", "gate", "z", "dout"])
+def test_nan_does_not_travel_against_time(name, dtype, layout):
+    """A NaN reaches what depends on it and nothing else: not the positions beside it, other
+    channels, or a packed neighbour."""
+    D, L, at, ch = 70, 100, 45, 9
+    ids = np.zeros((1, L), np.int32)
+    ids[0, 40:60], ids[0, 60:] = 1, 2
+    t = _inputs(23, 1, D, L, dtype, layout, nstates=3)
+
+    def run(v):
+        leaves = [v[k].detach().requires_grad_() for k in ("x", "gate", "z")]
+        out = gated_recurrence_fn(*leaves, v["bias"], seq_idx=torch.from_numpy(ids).cuda(), initial_states=v["init"])
+        return [out, *torch.autograd.grad(out, leaves, v["dout"])]
+
+    want = run(t)
+    t[name][0, ch, at] = float("nan")
+    got = run(t)
+    # places of its own sequence, from it on (out) or up to it (what flows back), or all
+    own, before, after, here = (np.zeros(L, bool) for _ in range(4))
+    own[40:60], before[40:at + 1], after[at:60], here[at] = True, True, True, True
+    reach = {"x": (after, own, own, after), "gate": (after, own, own, after), "z": (here, before, before, here),
+             "dout": (here & False, before, before, here)}[name]
+    for what, g, w, may in zip(("out", "dx", "dgate", "dz"), got, want, reach):
+        same = torch.ones(1, D, L, dtype=torch.bool, device="cuda")
+        same[0, ch, torch.from_numpy(may).cuda()] = False
+        assert torch.equal(g[same], w[same]), what
+    if name != "dout":
+        assert torch.isnan(got[0][0, ch, at])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_extreme_gates(dtype):
     """Gates that hold on for ever and that let go at once, beyond exp's range."""
