@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
   };
 #pragma unroll
   for (int k = 0; k < S - 2; ++k) load(k);
+  if (tma) load(S - 2);
   const L nb = gate_offset<T, LAYOUT>(a, p.d0, lane);
   L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.init, p.b, a.nstates, p.d0, a.dim, lane);
   if (w == 0) common.handed[0][lane] = carry;
@@ -370,8 +371,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     __syncthreads();
     copy_ids(k + 2);
     if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
-    if (tma && threadIdx.x == 0) tma_wait_read<1>();  // the slot to be loaded was stored a round ago
-    load(k + S - 2);
+    if (!tma) load(k + S - 2);  // into the slot that was stored a round ago
     const unsigned cuts = SEQ ? cuts_of(sum.cut, lane) : 0;
     L h = p.cluster == 1 ? through_warps<V, SEQ, true>(sum.A, sum.H, cuts, w, lane, common.handed[buf][lane])
                          : through_cluster<V, SEQ, true>(sum.A, sum.H, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), (k >> 1) & 1, p, w, lane, carry);
@@ -421,7 +421,11 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     }
     write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gb);
     if (SEQ && e.valid != 0xffu) clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~e.valid);
-    if (tma) tma_fence();
+    if (tma) {
+      tma_fence();
+      if (threadIdx.x == 0) tma_wait_read<0>();  // by now the last round's tiles have been stored
+      load(k + S - 1);
+    }
     if (++slot == S) slot = 0, parity ^= 1;
   }
   __syncthreads();
@@ -522,6 +526,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
   };
 #pragma unroll
   for (int k = 0; k < S - 2; ++k) load(k);
+  if (tma) load(S - 2);
   const L nb = gate_offset<T, LAYOUT>(a, p.d0, lane);
   L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.dfinal, p.b, a.nstates, p.d0, a.dim, lane);
   if (w == 0) common.handed[0][lane] = carry;
@@ -612,8 +617,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     __syncthreads();
     copy_ahead(k + 2);
     if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
-    if (tma && threadIdx.x == 0) tma_wait_read<1>();
-    load(k + S - 2);
+    if (!tma) load(k + S - 2);
     L h = through_warps<V, SEQ, true>(sum.A, sum.H, SEQ ? cuts_of(sum.cut, lane) : 0, w, lane, common.start[k % 3][lane]);
     const unsigned cuts = SEQ ? cuts_of(sum_back.cut, lane) : 0;
     L s = p.cluster == 1 ? through_warps<V, SEQ, false>(sum.A, sum_back.B, cuts, w, lane, common.handed[buf][lane])
@@ -668,7 +672,11 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
       clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~valid);
       if constexpr (Z) clear_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, w, lane, ~valid);
     }
-    if (tma) tma_fence();
+    if (tma) {
+      tma_fence();
+      if (threadIdx.x == 0) tma_wait_read<0>();  // by now the last round's tiles have been stored
+      load(k + S - 1);
+    }
     if (++slot == S) slot = 0, parity ^= 1;
   }
   __syncthreads();
