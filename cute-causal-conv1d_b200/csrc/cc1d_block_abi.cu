@@ -76,23 +76,33 @@ int sm_count() {
   return n;
 }
 
-// CTAs that share a tile.  Each takes 1/cluster of the chunks.  The estimate counts chunk
-// times: a CTA pays its start (about 4 chunks until its first tiles are there), a cluster's
-// exchange lengthens a chunk by half, and n CTAs on an SM take (2 + n) / 3 of the time that one
-// needs for a chunk each.  As many fit as their shared memory (`smem`, and 1 KB for each CTA of
-// the cluster) allows, at most 4.
-int choose_cluster(int64_t tiles, int64_t chunks, int64_t smem) {
+// CTAs that share a tile.  Each takes 1/cluster of the chunks, so a long sequence of few
+// channels fills the GPU, but the cluster's exchange lengthens every chunk.  Measured on a
+// B200, with n CTAs on an SM, a chunk takes base + n * more microseconds:
+//
+//   cluster           1            2            4            8            16
+//   forward    .75 + .21n  1.15 + .15n  1.30 + .13n  1.30 + .22n  1.30 + .45n
+//   backward   .75 + .52n  1.40 + .25n  1.60 + .28n  1.75 + .37n  1.75 + .65n
+//
+// and a CTA about 6 microseconds to start.  As many fit an SM as their shared memory allows
+// (`smem`, and 1 KB for each CTA of the cluster), at most 4 (registers).  The estimate picks
+// the fastest: 256 tiles of 64 chunks run alone, 64 tiles of 256 chunks in clusters of 4
+// (forward 244 us alone, 100 in fours, 113 in eights).
+int choose_cluster(int64_t tiles, int64_t chunks, int64_t smem, bool bwd) {
+  static const double kBase[2][5] = {{.75, 1.15, 1.30, 1.30, 1.30}, {.75, 1.40, 1.60, 1.75, 1.75}};
+  static const double kMore[2][5] = {{.21, .15, .13, .22, .45}, {.52, .25, .28, .37, .65}};
   const int64_t sms = sm_count();
   double best = 0;
   int pick = 1;
-  auto time = [](double n) { return (2.0 + n) / 3.0; };
-  for (int c = 1; c <= 16 && c <= chunks; c *= 2) {
+  for (int i = 0, c = 1; c <= 16 && (c == 1 || c <= chunks); ++i, c *= 2) {
     const int64_t bytes = smem + (c > 1 ? c * 1024 : 0) + 1024;
-    const int64_t fit = std::min<int64_t>(4, 228 * 1024 / bytes), slots = fit * sms, ctas = tiles * c, rest = ctas % slots;
-    const double per_cta = (static_cast<double>((chunks + c - 1) / c) + 4.0) * (c > 1 ? 1.5 : 1.0);
-    const double waves = static_cast<double>(ctas / slots) * time(fit) + (rest ? time((rest + sms - 1) / sms) : 0.0);
-    if (c == 1 || per_cta * waves < best) {
-      best = per_cta * waves;
+    const int64_t fit = std::max<int64_t>(1, std::min<int64_t>(4, 228 * 1024 / bytes)), slots = fit * sms;
+    const int64_t ctas = tiles * c, rest = ctas % slots;
+    const double rounds = static_cast<double>((chunks + c - 1) / c);
+    auto wave = [&](int64_t n) { return 6.0 + rounds * (kBase[bwd][i] + kMore[bwd][i] * static_cast<double>(n)); };
+    const double cost = static_cast<double>(ctas / slots) * wave(fit) + (rest ? wave((rest + sms - 1) / sms) : 0.0);
+    if (c == 1 || cost < best) {
+      best = cost;
       pick = c;
     }
   }
@@ -117,12 +127,12 @@ cc1d_status rec_plan(RecArgs* a, bool bwd) {
     strips = strips && strips_ok(*t, *a);
     packets = packets && packets_ok(*t, *a);
   }
-  a->move = !strips ? kElements : packets ? kTma : a->x.dtype != CC1D_FLOAT32 ? kWords : kElements;
+  a->move = !strips ? kElements : packets ? kTma : a->x.dtype != CC1D_FLOAT32 ? kPackets : kElements;
   const int64_t channels = a->x.dtype == CC1D_FLOAT32 ? 32 : 64;
   a->dtiles = (a->dim + channels - 1) / channels;
   const int64_t tiles = a->batch * a->dtiles;
-  const int64_t tile = 4096 + (a->move == kWords ? 256 : 0), z = a->z.data ? 1 : 0;
-  a->cluster = choose_cluster(tiles, a->nchunks, bwd ? 3 * (3 + z) * tile + 8064 : 4 * (2 + z) * tile + 6016);
+  const int64_t tile = 4096 + (a->move == kPackets ? (a->rows ? 1024 : 512) : 0), z = a->z.data ? 1 : 0;
+  a->cluster = choose_cluster(tiles, a->nchunks, bwd ? 3 * (3 + z) * tile + 8064 : 4 * (2 + z) * tile + 6016, bwd);
   if (tiles * a->cluster > kMax31) return fail(CC1D_ERR_VALUE, "batch * dim is too large");
   return CC1D_OK;
 }

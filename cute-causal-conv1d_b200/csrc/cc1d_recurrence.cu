@@ -114,16 +114,16 @@ struct Place {
   int64_t b, d0;
   int nd, cluster, rank, rounds;
 };
-template <int CHANNELS>
+template <int CHANNELS, bool CLUSTER>
 __device__ __forceinline__ Place place_of(const RecArgs& a) {
   Place p;
-  p.cluster = a.cluster;
-  p.rank = a.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
-  const unsigned tile = blockIdx.x / static_cast<unsigned>(a.cluster), n = static_cast<unsigned>(a.dtiles);
+  p.cluster = CLUSTER ? a.cluster : 1;
+  p.rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0;
+  const unsigned tile = blockIdx.x / static_cast<unsigned>(p.cluster), n = static_cast<unsigned>(a.dtiles);
   p.b = tile / n;
   p.d0 = static_cast<int64_t>(tile % n) * CHANNELS;
   p.nd = static_cast<int>(min(a.dim - p.d0, static_cast<int64_t>(CHANNELS)));
-  p.rounds = static_cast<int>((a.nchunks + a.cluster - 1) / a.cluster);
+  p.rounds = static_cast<int>((a.nchunks + p.cluster - 1) / p.cluster);
   return p;
 }
 
@@ -174,12 +174,12 @@ __device__ __forceinline__ Lane<V> through_warps(const Lane<V>* A, const Lane<V>
   return h;
 }
 
-// The state that warp w's positions start from, for a CTA of a cluster.  Sends the composition
-// of the CTA's maps to the cluster's CTAs and joins theirs; `carry` is the state the round
-// starts from, and becomes the one that the next starts from.
+// A CTA of a cluster sends the composition of its maps to all of them, itself included.
 template <int V, bool SEQ, bool FORWARD>
-__device__ __forceinline__ Lane<V> through_cluster(const Lane<V>* A, const Lane<V>* H, unsigned cuts, Map<V>* far, unsigned bar,
-                                                   unsigned parity, const Place& p, int w, int lane, Lane<V>& carry) {
+__device__ __forceinline__ void send_to_cluster(const Lane<V>* A, const Lane<V>* H, unsigned cuts, Map<V>* far, unsigned bar,
+                                                const Place& p, int w, int lane) {
+  if (threadIdx.x == 0) mbar_expect(bar, p.cluster * 32 * sizeof(Map<V>));
+  if (w >= p.cluster) return;  // this warp sends to ranks w, w + 4, ...
   Map<V> all;
   all.A = splat(1.f, Lane<V>{});
   all.H = splat(0.f, Lane<V>{});
@@ -192,20 +192,28 @@ __device__ __forceinline__ Lane<V> through_cluster(const Lane<V>* A, const Lane<
     all.A = mul(m, all.A);
   }
   if (SEQ && cuts) all.A = splat(-1.f, all.A);
-  if (threadIdx.x == 0) mbar_expect(bar, p.cluster * 32 * sizeof(Map<V>));
   const unsigned slot = shared_addr(far + p.rank * 32 + lane);
   for (int r = w; r < p.cluster; r += kRecWarps) send_map<V>(slot, bar, r, all);
-  // a partner that never answers leaves NaN in the results instead of a hang
+}
+
+// The state that this CTA's chunk starts from.  `carry` is the state the round starts from, and
+// becomes the one that the next starts from.  A partner that never answers leaves NaN in the
+// results instead of a hang.
+template <int V, bool SEQ, bool FORWARD>
+__device__ __forceinline__ Lane<V> from_cluster(const Map<V>* far, unsigned bar, unsigned parity, const Place& p, int lane, Lane<V>& carry) {
   Lane<V> h = mbar_wait(bar, parity) ? carry : splat(__int_as_float(0x7fc00000), carry);
   Lane<V> start = h;
-#pragma unroll 4
-  for (int i = 0; i < p.cluster; ++i) {
+  const int mine = FORWARD ? p.rank : p.cluster - 1 - p.rank;  // how many come before this CTA
+  for (int i = 0; i < p.cluster; i += 2) {                     // (a power of two)
     const int r = FORWARD ? i : p.cluster - 1 - i;
-    if (r == p.rank) start = h;
-    h = apply<V, SEQ>(far[r * 32 + lane], h);
+    const Map<V> m0 = far[r * 32 + lane], m1 = far[(FORWARD ? r + 1 : r - 1) * 32 + lane];
+    if (i == mine) start = h;
+    h = apply<V, SEQ>(m0, h);
+    if (i + 1 == mine) start = h;
+    h = apply<V, SEQ>(m1, h);
   }
   carry = h;
-  return through_warps<V, SEQ, FORWARD>(A, H, cuts, w, lane, start);
+  return start;
 }
 
 // What else a CTA keeps in shared memory: without a cluster, the state that one round's last
@@ -230,19 +238,19 @@ __device__ __forceinline__ void load_ids(const RecArgs& a, int64_t b, int64_t t0
 }
 
 // The barriers of the ring (one per slot) and of the cluster's exchange (two).
-template <int S>
-__device__ __forceinline__ void start_barriers(unsigned bars, bool tma, int cluster) {
+template <int S, bool CLUSTER>
+__device__ __forceinline__ void start_barriers(unsigned bars, bool tma) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) mbar_init(bars + 8 * i, tma ? 1 : 2 * kRecThreads);
     mbar_init(bars + 8 * S, 1);
     mbar_init(bars + 8 * S + 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (cluster > 1) cluster_sync();  // they are there before a partner's first map arrives
+  if (CLUSTER) cluster_sync();  // they are there before a partner's first map arrives
   else __syncthreads();
 }
 
-template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z>
+template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z, bool CLUSTER>
 __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int V = C::V, NT = Z ? 3 : 2, S = kFwdStages;
@@ -251,13 +259,13 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
   // ring of tiles (gate, x, z) | sums of the warps [2] | maps of the cluster [2][cluster][32] | common
   Sums<V>* const sums = reinterpret_cast<Sums<V>*>(smem + S * NT * C::kBytes);
   Map<V>* const far = reinterpret_cast<Map<V>*>(sums + 2);
-  Common<V>& common = *reinterpret_cast<Common<V>*>(far + (a.cluster > 1 ? 2 * a.cluster * 32 : 0));
+  Common<V>& common = *reinterpret_cast<Common<V>*>(far + (CLUSTER ? 2 * a.cluster * 32 : 0));
   const unsigned ring = shared_addr(smem), bars = shared_addr(common.bars);
 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const Place p = place_of<C::kChannels>(a);
+  const Place p = place_of<C::kChannels, CLUSTER>(a);
   const bool tma = !SKEW && a.move == kTma;
-  start_barriers<S>(bars, tma, p.cluster);
+  start_barriers<S, CLUSTER>(bars, tma);
   grid_dependency_wait();
   const Strip<T> gt = strip_of<T>(a.gate, maps.gate, p.b, p.d0), xt = strip_of<T>(a.x, maps.x, p.b, p.d0);
   const Strip<T> zt = Z ? strip_of<T>(a.z, maps.z, p.b, p.d0) : gt, ot = strip_of<T>(a.out, maps.out, p.b, p.d0);
@@ -369,12 +377,23 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     if (SEQ && lane == 0) sum.cut[w] = e.first;
     if (SEQ) cp_async_wait<0>();  // the ids of the next round, for all after the barrier
     __syncthreads();
+    const unsigned cuts = SEQ ? cuts_of(sum.cut, lane) : 0;
+    if (CLUSTER) send_to_cluster<V, SEQ, true>(sum.A, sum.H, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), p, w, lane);
     copy_ids(k + 2);
     if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
     if (!tma) load(k + S - 2);  // into the slot that was stored a round ago
-    const unsigned cuts = SEQ ? cuts_of(sum.cut, lane) : 0;
-    L h = p.cluster == 1 ? through_warps<V, SEQ, true>(sum.A, sum.H, cuts, w, lane, common.handed[buf][lane])
-                         : through_cluster<V, SEQ, true>(sum.A, sum.H, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), (k >> 1) & 1, p, w, lane, carry);
+    L zs[kRecSteps];
+    auto silu = [&] {
+      L z[kRecSteps];
+      read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, zt, t0, w, lane, z);
+      sigmoids<T, V, false, false>(z, splat(0.f, L{}), zs, nullptr);
+#pragma unroll
+      for (int j = 0; j < kRecSteps; ++j) zs[j] = mul(zs[j], z[j]);
+    };
+    if constexpr (Z && CLUSTER) silu();  // while the cluster's maps are on their way
+    L h = !CLUSTER ? common.handed[buf][lane]
+                         : from_cluster<V, SEQ, true>(far + buf * p.cluster * 32, bars + 8 * (S + buf), (k >> 1) & 1, p, lane, carry);
+    h = through_warps<V, SEQ, true>(sum.A, sum.H, cuts, w, lane, h);
     if (w == 0 && a.checkpoints && c < a.nchunks) {
       float* to = a.checkpoints + (p.b * a.nchunks + c) * a.dim + p.d0;
 #pragma unroll
@@ -400,7 +419,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
         gb[j] = h;
       }
     }
-    if (p.cluster == 1 && w == kRecWarps - 1) common.handed[buf ^ 1][lane] = h;
+    if (!CLUSTER && w == kRecWarps - 1) common.handed[buf ^ 1][lane] = h;
     if (a.final_states.data && (SEQ ? e.last != 0 : tw < a.seqlen && tw + kRecSteps >= a.seqlen)) {
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
@@ -413,11 +432,9 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
       }
     }
     if constexpr (Z) {
-      L z[kRecSteps], s[kRecSteps];
-      read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, zt, t0, w, lane, z);
-      sigmoids<T, V, false, false>(z, splat(0.f, L{}), s, nullptr);
+      if constexpr (!CLUSTER) silu();
 #pragma unroll
-      for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gb[j], mul(z[j], s[j]));
+      for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gb[j], zs[j]);
     }
     write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gb);
     if (SEQ && e.valid != 0xffu) clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~e.valid);
@@ -431,10 +448,10 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
   __syncthreads();
   store(p.rounds - 1, slot == 0 ? S - 1 : slot - 1);
   if (tma && threadIdx.x == 0) tma_wait_read<0>();
-  if (p.cluster > 1) cluster_sync();  // no CTA leaves while a partner may still write to it
+  if (CLUSTER) cluster_sync();  // no CTA leaves while a partner may still write to it
 }
 
-template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z>
+template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z, bool CLUSTER>
 __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int V = C::V, NT = Z ? 4 : 3, S = kBwdStages;
@@ -445,13 +462,13 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
   Sums<V>* const sums = reinterpret_cast<Sums<V>*>(smem + S * NT * C::kBytes);
   SumsBack<V>* const sums_back = reinterpret_cast<SumsBack<V>*>(sums + 2);
   Map<V>* const far = reinterpret_cast<Map<V>*>(sums_back + 2);
-  Common<V>& common = *reinterpret_cast<Common<V>*>(far + (a.cluster > 1 ? 2 * a.cluster * 32 : 0));
+  Common<V>& common = *reinterpret_cast<Common<V>*>(far + (CLUSTER ? 2 * a.cluster * 32 : 0));
   const unsigned ring = shared_addr(smem), bars = shared_addr(common.bars);
 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const Place p = place_of<C::kChannels>(a);
+  const Place p = place_of<C::kChannels, CLUSTER>(a);
   const bool tma = !SKEW && a.move == kTma;
-  start_barriers<S>(bars, tma, p.cluster);
+  start_barriers<S, CLUSTER>(bars, tma);
   grid_dependency_wait();
   const Strip<T> gt = strip_of<T>(a.gate, maps.gate, p.b, p.d0), xt = strip_of<T>(a.x, maps.x, p.b, p.d0);
   const Strip<T> yt = strip_of<T>(a.dout, maps.dout, p.b, p.d0), zt = Z ? strip_of<T>(a.z, maps.z, p.b, p.d0) : gt;
@@ -615,13 +632,12 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     }
     cp_async_wait<0>();  // what the next round needs, for all after the barrier
     __syncthreads();
+    const unsigned cuts = SEQ ? cuts_of(sum_back.cut, lane) : 0;
+    if (CLUSTER) send_to_cluster<V, SEQ, false>(sum.A, sum_back.B, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), p, w, lane);
     copy_ahead(k + 2);
     if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
     if (!tma) load(k + S - 2);
     L h = through_warps<V, SEQ, true>(sum.A, sum.H, SEQ ? cuts_of(sum.cut, lane) : 0, w, lane, common.start[k % 3][lane]);
-    const unsigned cuts = SEQ ? cuts_of(sum_back.cut, lane) : 0;
-    L s = p.cluster == 1 ? through_warps<V, SEQ, false>(sum.A, sum_back.B, cuts, w, lane, common.handed[buf][lane])
-                         : through_cluster<V, SEQ, false>(sum.A, sum_back.B, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), (k >> 1) & 1, p, w, lane, carry);
 
     // forward through the positions: h before each, and dz
     L prev[kRecSteps];
@@ -643,6 +659,9 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
       }
     }
     // and back: dx (in gy) and dgate (in prev)
+    L s = !CLUSTER ? common.handed[buf][lane]
+                         : from_cluster<V, SEQ, false>(far + buf * p.cluster * 32, bars + 8 * (S + buf), (k >> 1) & 1, p, lane, carry);
+    s = through_warps<V, SEQ, false>(sum.A, sum_back.B, cuts, w, lane, s);
     auto step_back = [&](int j) {
       const L dh = add(gy[j], s);
       gy[j] = mul(dh, gc[j]);
@@ -663,7 +682,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
 #pragma unroll
       for (int j = kRecSteps - 1; j >= 0; --j) step_back(j);
     }
-    if (p.cluster == 1 && w == 0) common.handed[buf ^ 1][lane] = s;
+    if (!CLUSTER && w == 0) common.handed[buf ^ 1][lane] = s;
     write_steps<T, LAYOUT, SKEW>(now, w, lane, prev);
     write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gy);
     if constexpr (Z) write_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, w, lane, dz);
@@ -682,7 +701,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
   __syncthreads();
   store(p.rounds - 1, slot == 0 ? S - 1 : slot - 1);
   if (!SEQ && w == 0 && p.rank == 0)
-    store_state<T, LAYOUT>(a.dinit, p.b, a.nstates, p.d0, a.dim, lane, p.cluster == 1 ? common.handed[p.rounds & 1][lane] : carry);
+    store_state<T, LAYOUT>(a.dinit, p.b, a.nstates, p.d0, a.dim, lane, !CLUSTER ? common.handed[p.rounds & 1][lane] : carry);
   if (a.dbias) {
     L* const sum = sums[0].A;
     sum[w * 32 + lane] = bias_sum;
@@ -699,7 +718,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     }
   }
   if (tma && threadIdx.x == 0) tma_wait_read<0>();
-  if (p.cluster > 1) cluster_sync();
+  if (CLUSTER) cluster_sync();
 }
 
 // dbias[d] = the tiles' partial sums added up in order.
@@ -774,7 +793,7 @@ bool make_map(CUtensorMap* map, const TensorArg& t, const RecArgs& a) {
                 CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int LAYOUT, bool SKEW, bool BWD, bool SEQ, bool Z>
+template <typename T, int LAYOUT, bool SKEW, bool BWD, bool SEQ, bool Z, bool CLUSTER>
 cudaError_t run(RecArgs& a, cudaStream_t s) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int NT = (BWD ? 3 : 2) + (Z ? 1 : 0);
@@ -788,8 +807,8 @@ cudaError_t run(RecArgs& a, cudaStream_t s) {
     if (!ok) a.move = kElements;
   }
   const size_t smem = static_cast<size_t>(stages) * NT * C::kBytes + 2 * (sizeof(Sums<C::V>) + (BWD ? sizeof(SumsBack<C::V>) : 0)) +
-                      (a.cluster > 1 ? 2 * a.cluster * 32 * sizeof(Map<C::V>) : 0) + sizeof(Common<C::V>);
-  auto kernel = BWD ? rec_bwd_kernel<T, LAYOUT, SKEW, SEQ, Z> : rec_fwd_kernel<T, LAYOUT, SKEW, SEQ, Z>;
+                      (CLUSTER ? 2 * a.cluster * 32 * sizeof(Map<C::V>) : 0) + sizeof(Common<C::V>);
+  auto kernel = BWD ? rec_bwd_kernel<T, LAYOUT, SKEW, SEQ, Z, CLUSTER> : rec_fwd_kernel<T, LAYOUT, SKEW, SEQ, Z, CLUSTER>;
   const void* ptr = reinterpret_cast<const void*>(kernel);
   cudaError_t e = allow_dynamic_smem(ptr, smem);
   if (e == cudaSuccess && a.cluster > 8) e = cudaFuncSetAttribute(ptr, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -806,20 +825,24 @@ cudaError_t run(RecArgs& a, cudaStream_t s) {
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = a.cluster > 1 ? 2 : 1;
+  cfg.numAttrs = CLUSTER ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<const RecArgs&>(a), static_cast<const RecMaps&>(maps));
 }
 
+template <typename T, int LAYOUT, bool SKEW, bool BWD, bool SEQ, bool Z>
+cudaError_t pick_cluster(RecArgs& a, cudaStream_t s) {
+  return a.cluster > 1 ? run<T, LAYOUT, SKEW, BWD, SEQ, Z, true>(a, s) : run<T, LAYOUT, SKEW, BWD, SEQ, Z, false>(a, s);
+}
 template <typename T, int LAYOUT, bool SKEW, bool BWD>
 cudaError_t pick_options(RecArgs& a, cudaStream_t s) {
   if (a.seq_idx.data)
-    return a.z.data ? run<T, LAYOUT, SKEW, BWD, true, true>(a, s) : run<T, LAYOUT, SKEW, BWD, true, false>(a, s);
-  return a.z.data ? run<T, LAYOUT, SKEW, BWD, false, true>(a, s) : run<T, LAYOUT, SKEW, BWD, false, false>(a, s);
+    return a.z.data ? pick_cluster<T, LAYOUT, SKEW, BWD, true, true>(a, s) : pick_cluster<T, LAYOUT, SKEW, BWD, true, false>(a, s);
+  return a.z.data ? pick_cluster<T, LAYOUT, SKEW, BWD, false, true>(a, s) : pick_cluster<T, LAYOUT, SKEW, BWD, false, false>(a, s);
 }
 template <typename T, bool BWD>
 cudaError_t pick(RecArgs& a, cudaStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    if (a.move == kWords) return a.rows ? pick_options<T, kLayoutRows, true, BWD>(a, s) : pick_options<T, kLayoutChannelLast, true, BWD>(a, s);
+    if (a.move == kPackets) return a.rows ? pick_options<T, kLayoutRows, true, BWD>(a, s) : pick_options<T, kLayoutChannelLast, true, BWD>(a, s);
   }
   return a.rows ? pick_options<T, kLayoutRows, false, BWD>(a, s) : pick_options<T, kLayoutChannelLast, false, BWD>(a, s);
 }

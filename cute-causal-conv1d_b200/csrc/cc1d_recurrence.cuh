@@ -90,12 +90,13 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
 }
 
 // ----------------------------------------------------------------------------- the tiles
-// SKEW (kWords): a strip lies in its tile as it does in memory, half a word late where it
-// starts in the middle of one, so it takes one word more.
-//
 // channel-last: 32 strips (positions) of 128 bytes of channels.
 // rows: strips of 32 positions, one per channel, in 16-byte packets that are swapped around as
 // the TMA's swizzles do, so that 8 lanes reading the same packet of 8 channels use all banks.
+//
+// SKEW (kPackets): the aligned 16-byte packets that cover a strip, in order; the strip starts
+// as many bytes into them as it lies off a 16-byte boundary in memory.  Results are put there
+// without that offset.
 template <typename T, int LAYOUT, bool SKEW> struct Tile {
   static constexpr int kSize = sizeof(T);
   static constexpr int V = 4 / kSize;                // channels per lane
@@ -104,19 +105,14 @@ template <typename T, int LAYOUT, bool SKEW> struct Tile {
   static constexpr bool kRows = LAYOUT == kLayoutRows;
   static constexpr int kStrips = kRows ? kChannels : kRecChunk;
   static constexpr int kStripBytes = kRows ? kRecChunk * kSize : 128;
-  static constexpr int kStripWords = kStripBytes / 4;
-  static constexpr int kEnds = kStrips * kStripBytes;  // SKEW: the strips' last words
-  static constexpr int kBytes = kEnds + (SKEW ? kStrips * 4 : 0);
-  static_assert(kEnds == 4096 && (!kRows || kStripBytes == 64 || kStripBytes == 128), "");
-  // byte of word i of strip r, without the last
-  static __device__ __forceinline__ int word(int r, int i) {
-    const int swap = !kRows ? 0 : kStripBytes == 128 ? r & 7 : (r >> 1) & 3;
-    return r * kStripBytes + (((i >> 2) ^ swap) << 4) + (i & 3) * 4;
-  }
-  // byte of element (channel, position) without a skew
+  static constexpr int kPitch = kStripBytes + (SKEW ? 16 : 0);
+  static constexpr int kBytes = kStrips * kPitch;
+  static_assert(kStrips * kStripBytes == 4096 && (!kRows || kStripBytes == 64 || kStripBytes == 128), "");
+  // byte of element (channel, position), for SKEW of a result
   static __device__ __forceinline__ int at(int ch, int pos) {
-    const int byte = (kRows ? pos : ch) * kSize;
-    return word(kRows ? ch : pos, byte >> 2) + (byte & 3);
+    const int r = kRows ? ch : pos, byte = (kRows ? pos : ch) * kSize;
+    const int swap = !kRows || SKEW ? 0 : kStripBytes == 128 ? r & 7 : (r >> 1) & 3;
+    return r * kPitch + (((byte >> 4) ^ swap) << 4) + (byte & 15);
   }
 };
 
@@ -163,34 +159,34 @@ template <int N> __device__ __forceinline__ void tma_wait_read() { asm volatile(
 // What this thread wrote to shared memory is there for the TMA.
 __device__ __forceinline__ void tma_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-// kWords and kElements, all threads: positions t0 .. t0 + nt - 1 of nd channels; places outside
-// are zero.
+// kPackets and kElements, all threads: positions t0 .. t0 + nt - 1 of nd channels; places
+// outside are zero.
 template <typename T, int LAYOUT, bool SKEW>
 __device__ __forceinline__ void load_tile(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
   using C = Tile<T, LAYOUT, SKEW>;
   const unsigned base = shared_addr(tile);
   if constexpr (SKEW) {
-    const int64_t step = C::kRows ? t.s1 : t.s2;
-    const int strips = C::kRows ? nd : nt, len = C::kRows ? nt : nd;
-    const T* const from = t.row + (C::kRows ? t0 : t0 * t.s2);
-    const T* const none = t.origin + (reinterpret_cast<uintptr_t>(t.origin) >> 1 & 1);  // aligned, not read
-    // word i of a strip covers its elements 2i - skew and 2i + 1 - skew
-    auto word = [&](int r, int i, int o) {
-      const T* p = from + r * step;
-      const int e = 2 * i - (static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1);
-      const int n = r < strips ? max(0, min(2, len - e)) : 0;
-      if (n > 0 && p + e < t.origin) {  // half of the word lies before the tensor
-        *reinterpret_cast<uint32_t*>(tile + o) = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + e + 1)) << 16;
-      } else {
-        cp4(base + o, n > 0 ? p + e : none, n * 2);
-      }
-    };
+    constexpr int P = C::kPitch / 16, N = C::kStrips * P;
+    const int64_t step = (C::kRows ? t.s1 : t.s2) * C::kSize;
+    const int strips = C::kRows ? nd : nt, bytes = (C::kRows ? nt : nd) * C::kSize;
+    const char* const from = reinterpret_cast<const char*>(t.row + (C::kRows ? t0 : t0 * t.s2));
+    const char* const origin = reinterpret_cast<const char*>(t.origin);
 #pragma unroll
-    for (int k = 0; k < 1024 / kRecThreads; ++k) {
-      const int i = threadIdx.x + k * kRecThreads, r = i / C::kStripWords;
-      word(r, i % C::kStripWords, C::word(r, i % C::kStripWords));
+    for (int k = 0; k < (N + kRecThreads - 1) / kRecThreads; ++k) {
+      const int i = threadIdx.x + k * kRecThreads, r = i / P, c = i % P * 16;
+      if (N % kRecThreads && i >= N) break;
+      const char* const strip = from + r * step;
+      const int off = static_cast<int>(reinterpret_cast<uintptr_t>(strip)) & 15;
+      const int n = r < strips ? max(0, min(16, off + bytes - c)) : 0;  // up to the strip's end
+      const char* const src = strip - off + c;
+      const unsigned dst = base + r * C::kPitch + c;
+      if (n > 0 && src < origin) {  // the tensor begins within the packet
+        for (int e = off; e < n; e += C::kSize)
+          *reinterpret_cast<uint16_t*>(tile + r * C::kPitch + e) = *reinterpret_cast<const uint16_t*>(src + e);
+      } else {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(n > 0 ? src : reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(origin) & ~uintptr_t{15})), "r"(n) : "memory");
+      }
     }
-    if (threadIdx.x < C::kStrips) word(threadIdx.x, C::kStripWords, C::kEnds + threadIdx.x * 4);
   } else {
     const T* const src = t.row + t0 * t.s2;
     constexpr int N = C::kChannels * kRecChunk / kRecThreads;
@@ -209,6 +205,12 @@ __device__ __forceinline__ void load_tile(unsigned char* tile, const Strip<T>& t
   }
 }
 
+// The low half of the address of element p[i * step].
+template <typename T>
+__device__ __forceinline__ unsigned low_address(const T* p, int i, int64_t step) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)) + static_cast<unsigned>(i) * static_cast<unsigned>(step) * static_cast<unsigned>(sizeof(T));
+}
+
 // The 8 positions of warp w and the lane's V channels, as fp32.
 template <typename T, int LAYOUT, bool SKEW>
 __device__ __forceinline__ void read_steps(const unsigned char* tile, const Strip<T>& t, int64_t t0, int w, int lane, Lane<4 / sizeof(T)> (&f)[kRecSteps]) {
@@ -219,12 +221,14 @@ __device__ __forceinline__ void read_steps(const unsigned char* tile, const Stri
       const int ch = lane + 32 * i;
 #pragma unroll
       for (int q = 0; q < kRecSteps / C::kPacket; ++q) {
-        uint4 u = *reinterpret_cast<const uint4*>(tile + C::at(ch, w * kRecSteps + q * C::kPacket));
+        uint4 u;
         if constexpr (SKEW) {
-          const uint32_t next = *reinterpret_cast<const uint32_t*>(tile + (w < kRecWarps - 1 ? C::word(ch, 4 * w + 4) : C::kEnds + 4 * ch));
-          const unsigned sh = (reinterpret_cast<uintptr_t>(t.row + t0 + ch * t.s1) & 2) * 8;
-          u = make_uint4(__funnelshift_r(u.x, u.y, sh), __funnelshift_r(u.y, u.z, sh), __funnelshift_r(u.z, u.w, sh),
-                         __funnelshift_r(u.w, next, sh));
+          const unsigned off = low_address(t.row + t0, ch, t.s1) & 15, sh = (off & 2) * 8;
+          const uint32_t* p = reinterpret_cast<const uint32_t*>(tile + ch * C::kPitch + w * 16 + (off & 12));
+          const uint32_t w0 = p[0], w1 = p[1], w2 = p[2], w3 = p[3], w4 = p[4];
+          u = make_uint4(__funnelshift_r(w0, w1, sh), __funnelshift_r(w1, w2, sh), __funnelshift_r(w2, w3, sh), __funnelshift_r(w3, w4, sh));
+        } else {
+          u = *reinterpret_cast<const uint4*>(tile + C::at(ch, w * kRecSteps + q * C::kPacket));
         }
         float2 v[C::kPacket / 2];
         unpack2<T, C::kPacket>(*reinterpret_cast<const Packet<T, C::kPacket>*>(&u), v);
@@ -236,21 +240,23 @@ __device__ __forceinline__ void read_steps(const unsigned char* tile, const Stri
       }
     }
   } else {
-    const unsigned char* p = tile + w * kRecSteps * 128 + lane * 4;
+    const unsigned char* p = tile + w * kRecSteps * C::kPitch + lane * 4;
 #pragma unroll
     for (int j = 0; j < kRecSteps; ++j) {
       if constexpr (C::V == 2) {
-        uint32_t u = *reinterpret_cast<const uint32_t*>(p + j * 128);
+        uint32_t u;
         if constexpr (SKEW) {
-          const uint32_t next = *reinterpret_cast<const uint32_t*>(lane < 31 ? p + j * 128 + 4 : tile + C::kEnds + (w * kRecSteps + j) * 4);
-          const unsigned sh = (reinterpret_cast<uintptr_t>(t.row + (t0 + w * kRecSteps + j) * t.s2) & 2) * 8;
-          u = __funnelshift_r(u, next, sh);
+          const unsigned off = low_address(t.row + t0 * t.s2, w * kRecSteps + j, t.s2) & 15;
+          const uint32_t* q = reinterpret_cast<const uint32_t*>(p + j * C::kPitch + (off & 12));
+          u = __funnelshift_r(q[0], q[1], (off & 2) * 8);
+        } else {
+          u = *reinterpret_cast<const uint32_t*>(p + j * C::kPitch);
         }
         float2 v[1];
         unpack2<T, 2>(*reinterpret_cast<const Packet<T, 2>*>(&u), v);
         f[j].v = v[0];
       } else {
-        f[j].v = *reinterpret_cast<const float*>(p + j * 128);
+        f[j].v = *reinterpret_cast<const float*>(p + j * C::kPitch);
       }
     }
   }
@@ -273,14 +279,14 @@ __device__ __forceinline__ void write_steps(unsigned char* tile, int w, int lane
       }
     }
   } else {
-    unsigned char* p = tile + w * kRecSteps * 128 + lane * 4;
+    unsigned char* p = tile + w * kRecSteps * C::kPitch + lane * 4;
 #pragma unroll
     for (int j = 0; j < kRecSteps; ++j) {
       if constexpr (C::V == 2) {
         float2 v[1] = {f[j].v};
-        *reinterpret_cast<Packet<T, 2>*>(p + j * 128) = pack2<T, 2>(v);
+        *reinterpret_cast<Packet<T, 2>*>(p + j * C::kPitch) = pack2<T, 2>(v);
       } else {
-        *reinterpret_cast<float*>(p + j * 128) = f[j].v;
+        *reinterpret_cast<float*>(p + j * C::kPitch) = f[j].v;
       }
     }
   }
@@ -298,12 +304,7 @@ __device__ __forceinline__ void set_steps(unsigned char* tile, const Strip<T>& t
     for (int i = 0; i < C::V; ++i) {
       const int ch = lane_channel<T, LAYOUT>(lane, i);
       int o = C::at(ch, pos);
-      if constexpr (SKEW) {
-        const int r = C::kRows ? ch : pos;
-        const T* p = t.row + (C::kRows ? t0 + ch * t.s1 : (t0 + pos) * t.s2);
-        const int e = (C::kRows ? pos : ch) + (static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1);
-        o = e < 2 * C::kStripWords ? C::word(r, e >> 1) + (e & 1) * 2 : C::kEnds + 4 * r;
-      }
+      if constexpr (SKEW) o += C::kRows ? low_address(t.row + t0, ch, t.s1) & 15 : low_address(t.row + t0 * t.s2, pos, t.s2) & 15;
       *reinterpret_cast<T*>(tile + o) = from_f32<T>(value);
     }
   }
@@ -321,34 +322,33 @@ __device__ __forceinline__ void clear_steps(unsigned char* tile, int w, int lane
   }
 }
 
-// kWords and kElements, all threads: stores what write_steps put into a tile.
+// kPackets and kElements, all threads: stores what write_steps put into a tile.
 template <typename T, int LAYOUT, bool SKEW>
 __device__ __forceinline__ void store_tile(const unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
   using C = Tile<T, LAYOUT, SKEW>;
   if constexpr (SKEW) {
-    const int64_t step = C::kRows ? t.s1 : t.s2;
+    constexpr int W = C::kStripBytes / 4;  // words of a strip, and one more where it starts within a word
+    const int64_t step = (C::kRows ? t.s1 : t.s2) * C::kSize;
     const int strips = C::kRows ? nd : nt, len = C::kRows ? nt : nd;
-    T* const to = t.row + (C::kRows ? t0 : t0 * t.s2);
-    auto element = [&](int r, int e) {
-      return *reinterpret_cast<const uint16_t*>(tile + C::word(r, e >> 1) + (e & 1) * 2);
-    };
-    auto word = [&](int r, int i) {  // the words of the strip as it lies in memory
+    char* const to = reinterpret_cast<char*>(t.row + (C::kRows ? t0 : t0 * t.s2));
+    auto word = [&](int r, int i) {
       if (r >= strips) return;
-      T* p = to + r * step;
-      const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1;
-      const int e = 2 * i - skew;
+      char* const strip = to + r * step;
+      const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(strip) >> 1) & 1, e = 2 * i - skew;
+      const unsigned char* const s = tile + r * C::kPitch + 4 * i;  // the word that holds element 2i
       if (e >= 0 && e + 1 < len) {
-        const uint32_t hi = *reinterpret_cast<const uint32_t*>(tile + C::word(r, i));
-        const uint32_t lo = skew ? *reinterpret_cast<const uint32_t*>(tile + C::word(r, i - 1)) : 0;
-        *reinterpret_cast<uint32_t*>(p + e) = skew ? __funnelshift_r(lo, hi, 16) : hi;
+        uint32_t u = *reinterpret_cast<const uint32_t*>(s);
+        if (skew) u = __funnelshift_r(*reinterpret_cast<const uint32_t*>(s - 4), u, 16);
+        *reinterpret_cast<uint32_t*>(strip + 2 * e) = u;
       } else {
-        if (e >= 0 && e < len) *reinterpret_cast<uint16_t*>(p + e) = element(r, e);
-        if (e + 1 >= 0 && e + 1 < len) *reinterpret_cast<uint16_t*>(p + e + 1) = element(r, e + 1);
+        const unsigned char* const f = s - 2 * skew;
+        if (e >= 0 && e < len) *reinterpret_cast<uint16_t*>(strip + 2 * e) = *reinterpret_cast<const uint16_t*>(f);
+        if (e + 1 >= 0 && e + 1 < len) *reinterpret_cast<uint16_t*>(strip + 2 * e + 2) = *reinterpret_cast<const uint16_t*>(f + 2);
       }
     };
 #pragma unroll
-    for (int k = 0; k < 1024 / kRecThreads; ++k) word((threadIdx.x + k * kRecThreads) / C::kStripWords, (threadIdx.x + k * kRecThreads) % C::kStripWords);
-    if (threadIdx.x < C::kStrips) word(threadIdx.x, C::kStripWords);
+    for (int k = 0; k < C::kStrips * W / kRecThreads; ++k) word((threadIdx.x + k * kRecThreads) / W, (threadIdx.x + k * kRecThreads) % W);
+    if (threadIdx.x < C::kStrips) word(threadIdx.x, W);
   } else {
     T* const dst = t.row + t0 * t.s2;
 #pragma unroll 4
