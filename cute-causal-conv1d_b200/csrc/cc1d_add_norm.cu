@@ -6,128 +6,513 @@
 //   dr = dresidual_out + rstd (q - n mean(q n)),  dresidual = dr,  dx = keep dr / (1 - p),
 //   dw = sum over the rows of dout n.
 //
-// One CTA per row, element by element.
+// G threads take a row and hold it in registers between its sum and its use, so every element
+// is read and written once: a warp up to 1024 columns (512 in fp32), which needs no barrier,
+// else the whole CTA.  Each thread has E neighbouring columns per step, a multiple of the 4
+// that one Philox block decides: the mask costs about 20 integer instructions per element,
+// computed where it is used, forward and backward.  CTAs stay (a few per SM) and load their
+// next row before they work on the present one.
+//
+// Bound by HBM.  Rows too wide for the registers (16384 columns, backward 8192, and 8192 in
+// fp32 or off the 16-byte alignment) are read a second time, from L2.
 #include "cc1d_block_launch.h"
 #include "cc1d_block_math.cuh"
 
 namespace cc1d {
 namespace {
 
-constexpr int kRowsPerPartial = 64;
+constexpr int kWideElements = 4;  // columns of a thread per step, rows read twice
 
-__device__ __forceinline__ float cta_sum(float v, float* scratch) {
+// E neighbouring elements as they lie in memory.
+template <typename T, int E> struct alignas(16) Cols { T v[E]; };
+
+// n of E elements from p, zero beyond; VEC: 16-byte packets where all are there.
+template <typename T, int E, bool VEC>
+__device__ __forceinline__ void load_cols(const T* p, int n, Cols<T, E>& r) {
+  constexpr int P = 16 / sizeof(T);
+  if (VEC && n >= E) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.f;
+    for (int i = 0; i < E; i += P) *reinterpret_cast<uint4*>(&r.v[i]) = __ldg(reinterpret_cast<const uint4*>(p + i));
+  } else {
 #pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) s += scratch[i];
-  return s;
-}
-
-__device__ __forceinline__ float kept(const AddNormArgs& a, int64_t row, int64_t c) {
-  if (!a.rng) return 1.f;
-  const uint4 w = philox(static_cast<uint64_t>(a.rng[0]), static_cast<uint64_t>(row * ((a.dim + 3) / 4) + c / 4),
-                         static_cast<uint64_t>(a.rng[a.rng_stride]));
-  const unsigned v = (c & 3) == 0 ? w.x : (c & 3) == 1 ? w.y : (c & 3) == 2 ? w.z : w.w;
-  return v >= a.keep_from ? a.keep_scale : 0.f;
-}
-
-template <typename T, typename R>
-__global__ void __launch_bounds__(kThreads) add_norm_fwd_kernel(const AddNormArgs a) {
-  grid_dependency_wait();
-  __shared__ float scratch[kThreads / 32];
-  const int64_t row = blockIdx.x;
-  R* ro = static_cast<R*>(a.residual_out.data) + row * a.residual_out.s0;
-  float sum = 0.f;
-  for (int64_t c = threadIdx.x; c < a.dim; c += kThreads) {
-    const float m = kept(a, row, c);
-    float r = m == 0.f ? 0.f : m * to_f32(static_cast<const T*>(a.x.data)[row * a.x.s0 + c]);
-    if (a.residual.data) r += to_f32(static_cast<const R*>(a.residual.data)[row * a.residual.s0 + c]);
-    const R stored = from_f32<R>(r);
-    ro[c] = stored;
-    r = to_f32(stored);
-    sum = fmaf(r, r, sum);
+    for (int i = 0; i < E; ++i) r.v[i] = i < n ? p[i] : from_f32<T>(0.f);
   }
-  const float rstd = 1.f / sqrtf(cta_sum(sum, scratch) / static_cast<float>(a.dim) + a.eps);
-  for (int64_t c = threadIdx.x; c < a.dim; c += kThreads)
-    static_cast<T*>(a.out.data)[row * a.out.s0 + c] =
-        from_f32<T>(to_f32(ro[c]) * rstd * load_any(a.weight.data, a.weight.dtype, c * a.weight.s0));
+}
+template <typename T, int E>
+__device__ __forceinline__ void widen(const Cols<T, E>& r, float (&f)[E]) {
+  unpack<T, E>(*reinterpret_cast<const Packet<T, E>*>(&r), f);
+}
+template <typename T, int E, bool VEC>
+__device__ __forceinline__ void load_cols(const T* p, int n, float (&f)[E]) {
+  Cols<T, E> r;
+  load_cols<T, E, VEC>(p, n, r);
+  widen<T, E>(r, f);
+}
+template <typename T, int E, bool VEC>
+__device__ __forceinline__ void store_cols(T* p, int n, const float (&f)[E]) {
+  constexpr int P = 16 / sizeof(T);
+  if (VEC && n >= E) {
+#pragma unroll
+    for (int i = 0; i < E; i += P) {
+      float u[P];
+#pragma unroll
+      for (int j = 0; j < P; ++j) u[j] = f[i + j];
+      st_packet<T, P>(p + i, pack<T, P>(u));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < n) p[i] = from_f32<T>(f[i]);
+  }
+}
+// The weight's columns: contiguous and aligned in packets, else one by one.
+template <int E>
+__device__ __forceinline__ void load_weight(const TensorArg& w, int64_t c, int n, float (&f)[E]) {
+  if (n >= E && w.s0 == 1 && (reinterpret_cast<uintptr_t>(w.data) & 15) == 0) {
+    if (w.dtype == CC1D_FLOAT32) return load_cols<float, E, true>(static_cast<const float*>(w.data) + c, E, f);
+    if constexpr (E == 8) {
+      if (w.dtype == CC1D_FLOAT16) return load_cols<__half, E, true>(static_cast<const __half*>(w.data) + c, E, f);
+      return load_cols<__nv_bfloat16, E, true>(static_cast<const __nv_bfloat16*>(w.data) + c, E, f);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) f[i] = i < n ? load_any(w.data, w.dtype, (c + i) * w.s0) : 0.f;
 }
 
-template <typename T, typename R>
-__global__ void __launch_bounds__(kThreads) add_norm_bwd_kernel(const AddNormArgs a) {
-  grid_dependency_wait();
-  __shared__ float scratch[kThreads / 32];
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRowsPerPartial;
-  float* part = a.dweight ? a.partials + blockIdx.x * a.dim : nullptr;
-  if (part)
-    for (int64_t c = threadIdx.x; c < a.dim; c += kThreads) part[c] = 0.f;
-  for (int64_t row = row0; row < min(a.rows, row0 + kRowsPerPartial); ++row) {
-    const R* rp = static_cast<const R*>(a.residual_out.data) + row * a.residual_out.s0;
-    const T* dy = a.dout.data ? static_cast<const T*>(a.dout.data) + row * a.dout.s0 : nullptr;
-    const R* dro = a.dresidual_out.data ? static_cast<const R*>(a.dresidual_out.data) + row * a.dresidual_out.s0 : nullptr;
-    float sum = 0.f, dot = 0.f;
-    for (int64_t c = threadIdx.x; c < a.dim; c += kThreads) {
-      const float r = to_f32(rp[c]);
-      sum = fmaf(r, r, sum);
-      if (dy) dot = fmaf(r, to_f32(dy[c]) * load_any(a.weight.data, a.weight.dtype, c * a.weight.s0), dot);
+// keep / (1 - p) of E columns from c (a multiple of 4) of a row.
+template <int E>
+__device__ __forceinline__ void keep_cols(const AddNormArgs& a, uint64_t key, uint64_t stream, int64_t row, int64_t c, float (&m)[E]) {
+  const uint64_t block = static_cast<uint64_t>(row) * static_cast<uint64_t>((a.dim + 3) / 4) + static_cast<uint64_t>(c / 4);
+#pragma unroll
+  for (int i = 0; i < E; i += 4) {
+    const uint4 u = philox(key, block + i / 4, stream);
+    m[i] = u.x >= a.keep_from ? a.keep_scale : 0.f;
+    m[i + 1] = u.y >= a.keep_from ? a.keep_scale : 0.f;
+    m[i + 2] = u.z >= a.keep_from ? a.keep_scale : 0.f;
+    m[i + 3] = u.w >= a.keep_from ? a.keep_scale : 0.f;
+  }
+}
+
+// Sums over the G threads of a row: a warp, or the CTA through shared memory (two buffers, so
+// that one barrier is enough).
+template <int G, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float (*scratch)[N][kThreads / 32], int turn) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  if constexpr (G > 32) {
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) scratch[turn & 1][i][threadIdx.x >> 5] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kThreads / 32; ++k) v[i] += scratch[turn & 1][i][k];
     }
-    const float inv = 1.f / static_cast<float>(a.dim);
-    const float rstd = 1.f / sqrtf(cta_sum(sum, scratch) * inv + a.eps);
-    const float k = cta_sum(dot, scratch) * inv * rstd;  // mean(q n)
-    for (int64_t c = threadIdx.x; c < a.dim; c += kThreads) {
-      const float n = to_f32(rp[c]) * rstd;
-      const float g = dy ? to_f32(dy[c]) : 0.f;
-      const float q = dy ? g * load_any(a.weight.data, a.weight.dtype, c * a.weight.s0) : 0.f;
-      const float dr = (dro ? to_f32(dro[c]) : 0.f) + rstd * (q - n * k);
-      if (a.dresidual.data) static_cast<R*>(a.dresidual.data)[row * a.dresidual.s0 + c] = from_f32<R>(dr);
-      if (a.dx.data) {
-        const float m = kept(a, row, c);
-        static_cast<T*>(a.dx.data)[row * a.dx.s0 + c] = from_f32<T>(m == 0.f ? 0.f : m * dr);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T* row_of(const TensorArg& t, int64_t row) { return static_cast<T*>(t.data) + row * t.s0; }
+
+__device__ __forceinline__ int cols_left(int64_t dim, int64_t c) {
+  return static_cast<int>(max(static_cast<int64_t>(0), min(dim - c, static_cast<int64_t>(1 << 20))));
+}
+
+// CTAs of a kernel that holds `elements` columns in a thread that fit an SM (its registers).
+constexpr int fwd_ctas(int elements) { return elements <= 8 ? 5 : elements <= 16 ? 3 : elements <= 32 ? 2 : 1; }
+constexpr int bwd_ctas(int elements) { return elements <= 8 ? 3 : elements <= 16 ? 2 : 1; }
+
+template <typename T, typename R, int G, int VPT, int E, bool VEC>
+__global__ void __launch_bounds__(kThreads, fwd_ctas(VPT * E)) add_norm_fwd_kernel(const AddNormArgs a) {
+  __shared__ float scratch[2][1][kThreads / 32];
+  constexpr bool kHeld = VPT * E <= 16;  // the weight stays in registers
+  const int g = threadIdx.x % G;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / G);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
+  grid_dependency_wait();
+  const uint64_t key = a.rng ? static_cast<uint64_t>(a.rng[0]) : 0, stream = a.rng ? static_cast<uint64_t>(a.rng[a.rng_stride]) : 0;
+  Cols<T, E> x[VPT];
+  Cols<R, E> res[VPT];
+  auto load = [&](int64_t at) {
+    if (at >= a.rows) return;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = static_cast<int64_t>(v * G + g) * E;
+      const int n = cols_left(a.dim, c);
+      load_cols<T, E, VEC>(row_of<T>(a.x, at) + c, n, x[v]);
+      if (a.residual.data) load_cols<R, E, VEC>(row_of<R>(a.residual, at) + c, n, res[v]);
+    }
+  };
+  load(row);
+  float held[kHeld ? VPT : 1][E];
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = static_cast<int64_t>(v * G + g) * E;
+      load_weight<E>(a.weight, c, cols_left(a.dim, c), held[v]);
+    }
+  }
+  for (int turn = 0; row < a.rows; row += step, ++turn) {
+    float r[VPT][E];
+    float sum[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      widen<T, E>(x[v], r[v]);
+      const int64_t c = static_cast<int64_t>(v * G + g) * E;
+      if (a.rng && c < a.dim) {
+        float m[E];
+        keep_cols<E>(a, key, stream, row, c, m);
+#pragma unroll
+        for (int i = 0; i < E; ++i) r[v][i] = m[i] == 0.f ? 0.f : m[i] * r[v][i];  // what is dropped is not used, NaN or not
       }
-      if (part) part[c] += g * n;
+      if (a.residual.data) {
+        float f[E];
+        widen<R, E>(res[v], f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) r[v][i] += f[i];
+      }
+    }
+    load(row + step);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = static_cast<int64_t>(v * G + g) * E;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {  // columns beyond the row are zero
+        r[v][i] = to_f32(from_f32<R>(r[v][i]));
+        sum[0] = fmaf(r[v][i], r[v][i], sum[0]);
+      }
+      store_cols<R, E, VEC>(row_of<R>(a.residual_out, row) + c, cols_left(a.dim, c), r[v]);
+    }
+    row_sum<G, 1>(sum, scratch, turn);
+    const float rstd = 1.f / sqrtf(sum[0] / static_cast<float>(a.dim) + a.eps);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = static_cast<int64_t>(v * G + g) * E;
+      const int n = cols_left(a.dim, c);
+      float w[E];
+      if constexpr (kHeld) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) w[i] = held[v][i];
+      } else {
+        load_weight<E>(a.weight, c, n, w);
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) w[i] *= r[v][i] * rstd;
+      store_cols<T, E, VEC>(row_of<T>(a.out, row) + c, n, w);
     }
   }
 }
 
-__global__ void __launch_bounds__(kThreads) add_norm_weight_kernel(const AddNormArgs a, int64_t parts) {
+// Rows that do not fit the registers: the stored stream is read again for the output.
+template <typename T, typename R>
+__global__ void __launch_bounds__(kThreads) add_norm_fwd_wide_kernel(const AddNormArgs a) {
+  constexpr int E = kWideElements;
+  __shared__ float scratch[2][1][kThreads / 32];
+  const int64_t row = blockIdx.x;
   grid_dependency_wait();
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (c >= a.dim) return;
-  float s = 0.f;
-  for (int64_t i = 0; i < parts; ++i) s += a.partials[i * a.dim + c];
-  a.dweight[c] = s;
+  const uint64_t key = a.rng ? static_cast<uint64_t>(a.rng[0]) : 0, stream = a.rng ? static_cast<uint64_t>(a.rng[a.rng_stride]) : 0;
+  R* const ro = row_of<R>(a.residual_out, row);
+  float sum[1] = {0.f};
+  for (int64_t c = threadIdx.x * E; c < a.dim; c += kThreads * E) {
+    const int n = cols_left(a.dim, c);
+    float r[E], res[E];
+    load_cols<T, E, false>(row_of<T>(a.x, row) + c, n, r);
+    if (a.rng) {
+      float m[E];
+      keep_cols<E>(a, key, stream, row, c, m);
+#pragma unroll
+      for (int i = 0; i < E; ++i) r[i] = m[i] == 0.f ? 0.f : m[i] * r[i];
+    }
+    if (a.residual.data) load_cols<R, E, false>(row_of<R>(a.residual, row) + c, n, res);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (a.residual.data) r[i] += res[i];
+      r[i] = to_f32(from_f32<R>(r[i]));
+      if (i < n) sum[0] = fmaf(r[i], r[i], sum[0]);
+    }
+    store_cols<R, E, false>(ro + c, n, r);
+  }
+  row_sum<kThreads, 1>(sum, scratch, 0);
+  const float rstd = 1.f / sqrtf(sum[0] / static_cast<float>(a.dim) + a.eps);
+  for (int64_t c = threadIdx.x * E; c < a.dim; c += kThreads * E) {
+    const int n = cols_left(a.dim, c);
+    float w[E];
+    load_weight<E>(a.weight, c, n, w);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < n) w[i] *= to_f32(ro[c + i]) * rstd;  // this thread's own stores
+    store_cols<T, E, false>(row_of<T>(a.out, row) + c, n, w);
+  }
 }
 
-template <typename T, typename R>
-cudaError_t fwd(const AddNormArgs& a, cudaStream_t s) {
-  return launch_dependent(add_norm_fwd_kernel<T, R>, dim3(static_cast<unsigned>(a.rows)), dim3(kThreads), 0, s, a);
+// Backward: a CTA takes rows blockIdx.x * rows per CTA + k * rows of the grid and adds up its
+// share of dw in registers; the shares go to `partials`, one row of (dim) for each CTA.
+template <typename T, typename R, int G, int VPT, int E, bool VEC>
+__global__ void __launch_bounds__(kThreads, bwd_ctas(VPT * E)) add_norm_bwd_kernel(const AddNormArgs a) {
+  extern __shared__ float shares[];  // G == 32: [warps][columns]
+  __shared__ float scratch[2][2][kThreads / 32];
+  const int g = threadIdx.x % G;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / G);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
+  grid_dependency_wait();
+  const uint64_t key = a.rng ? static_cast<uint64_t>(a.rng[0]) : 0, stream = a.rng ? static_cast<uint64_t>(a.rng[a.rng_stride]) : 0;
+  const float inv = 1.f / static_cast<float>(a.dim);
+  Cols<R, E> r[VPT], dres[VPT];
+  Cols<T, E> dy[VPT];
+  auto load = [&](int64_t at) {
+    if (at >= a.rows) return;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = static_cast<int64_t>(v * G + g) * E;
+      const int n = cols_left(a.dim, c);
+      load_cols<R, E, VEC>(row_of<R>(a.residual_out, at) + c, n, r[v]);
+      load_cols<T, E, VEC>(row_of<T>(a.dout, at) + c, a.dout.data ? n : 0, dy[v]);
+      load_cols<R, E, VEC>(row_of<R>(a.dresidual_out, at) + c, a.dresidual_out.data ? n : 0, dres[v]);
+    }
+  };
+  load(row);
+  float w[VPT][E], dw[VPT][E];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int64_t c = static_cast<int64_t>(v * G + g) * E;
+    load_weight<E>(a.weight, c, cols_left(a.dim, c), w[v]);
+#pragma unroll
+    for (int i = 0; i < E; ++i) dw[v][i] = 0.f;
+  }
+  for (int turn = 0; row < a.rows; row += step, ++turn) {
+    float sum[2] = {0.f, 0.f};  // of r^2 and of q r
+    Cols<R, E> rn[VPT], dresn[VPT];
+    Cols<T, E> dyn[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      float rf[E], df[E];
+      widen<R, E>(rn[v] = r[v], rf);
+      widen<T, E>(dyn[v] = dy[v], df);
+      dresn[v] = dres[v];
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        sum[0] = fmaf(rf[i], rf[i], sum[0]);
+        sum[1] = fmaf(df[i] * w[v][i], rf[i], sum[1]);
+      }
+    }
+    load(row + step);
+    row_sum<G, 2>(sum, scratch, turn);
+    const float rstd = 1.f / sqrtf(sum[0] * inv + a.eps);
+    const float k = sum[1] * inv * rstd;  // mean(q n)
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = static_cast<int64_t>(v * G + g) * E;
+      const int n = cols_left(a.dim, c);
+      float rf[E], df[E], dr[E];
+      widen<R, E>(rn[v], rf);
+      widen<T, E>(dyn[v], df);
+      widen<R, E>(dresn[v], dr);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float nv = rf[i] * rstd;
+        dw[v][i] = fmaf(df[i], nv, dw[v][i]);
+        dr[i] = fmaf(rstd, fmaf(-nv, k, df[i] * w[v][i]), dr[i]);
+      }
+      if (a.dresidual.data) store_cols<R, E, VEC>(row_of<R>(a.dresidual, row) + c, n, dr);
+      if (a.dx.data) {
+        if (a.rng && n > 0) {
+          float m[E];
+          keep_cols<E>(a, key, stream, row, c, m);
+#pragma unroll
+          for (int i = 0; i < E; ++i) dr[i] = m[i] == 0.f ? 0.f : m[i] * dr[i];
+        }
+        store_cols<T, E, VEC>(row_of<T>(a.dx, row) + c, n, dr);
+      }
+    }
+  }
+  if (!a.dweight) return;
+  float* const part = a.partials + static_cast<int64_t>(blockIdx.x) * a.dim;
+  if constexpr (G == 32) {
+    constexpr int D = 32 * VPT * E;
+    const int warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+      for (int i = 0; i < E; ++i) shares[warp * D + (v * 32 + g) * E + i] = dw[v][i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.dim; c += kThreads) {
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < kThreads / 32; ++q) s += shares[q * D + c];
+      part[c] = s;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = static_cast<int64_t>(v * G + g) * E;
+      store_cols<float, E, false>(part + c, cols_left(a.dim, c), dw[v]);
+    }
+  }
 }
-int64_t parts_of(const AddNormArgs& a) { return (a.rows + kRowsPerPartial - 1) / kRowsPerPartial; }
+
+// Rows that do not fit the registers: read twice, the share of dw kept in `partials`.
 template <typename T, typename R>
-cudaError_t bwd(const AddNormArgs& a, cudaStream_t s) {
-  cudaError_t e = launch_dependent(add_norm_bwd_kernel<T, R>, dim3(static_cast<unsigned>(parts_of(a))), dim3(kThreads), 0, s, a);
-  if (e != cudaSuccess || !a.dweight) return e;
-  add_norm_weight_kernel<<<static_cast<unsigned>((a.dim + kThreads - 1) / kThreads), kThreads, 0, s>>>(a, parts_of(a));
-  return cudaGetLastError();
+__global__ void __launch_bounds__(kThreads) add_norm_bwd_wide_kernel(const AddNormArgs a) {
+  constexpr int E = kWideElements;
+  __shared__ float scratch[2][2][kThreads / 32];
+  grid_dependency_wait();
+  const uint64_t key = a.rng ? static_cast<uint64_t>(a.rng[0]) : 0, stream = a.rng ? static_cast<uint64_t>(a.rng[a.rng_stride]) : 0;
+  const float inv = 1.f / static_cast<float>(a.dim);
+  float* const part = a.dweight ? a.partials + static_cast<int64_t>(blockIdx.x) * a.dim : nullptr;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++turn) {
+    float sum[2] = {0.f, 0.f};
+    for (int64_t c = threadIdx.x * E; c < a.dim; c += kThreads * E) {
+      const int n = cols_left(a.dim, c);
+      float r[E], dy[E], w[E];
+      load_cols<R, E, false>(row_of<R>(a.residual_out, row) + c, n, r);
+      load_cols<T, E, false>(row_of<T>(a.dout, row) + c, a.dout.data ? n : 0, dy);
+      load_weight<E>(a.weight, c, n, w);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        sum[0] = fmaf(r[i], r[i], sum[0]);
+        sum[1] = fmaf(dy[i] * w[i], r[i], sum[1]);
+      }
+    }
+    row_sum<kThreads, 2>(sum, scratch, turn);
+    const float rstd = 1.f / sqrtf(sum[0] * inv + a.eps);
+    const float k = sum[1] * inv * rstd;
+    for (int64_t c = threadIdx.x * E; c < a.dim; c += kThreads * E) {
+      const int n = cols_left(a.dim, c);
+      float r[E], dy[E], w[E], dr[E], m[E];
+      load_cols<R, E, false>(row_of<R>(a.residual_out, row) + c, n, r);
+      load_cols<T, E, false>(row_of<T>(a.dout, row) + c, a.dout.data ? n : 0, dy);
+      load_cols<R, E, false>(row_of<R>(a.dresidual_out, row) + c, a.dresidual_out.data ? n : 0, dr);
+      load_weight<E>(a.weight, c, n, w);
+      if (a.rng) keep_cols<E>(a, key, stream, row, c, m);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float nv = r[i] * rstd;
+        if (part && i < n) part[c + i] = turn ? fmaf(dy[i], nv, part[c + i]) : dy[i] * nv;
+        dr[i] = fmaf(rstd, fmaf(-nv, k, dy[i] * w[i]), dr[i]);
+      }
+      if (a.dresidual.data) store_cols<R, E, false>(row_of<R>(a.dresidual, row) + c, n, dr);
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (a.rng) dr[i] = m[i] == 0.f ? 0.f : m[i] * dr[i];
+      if (a.dx.data) store_cols<T, E, false>(row_of<T>(a.dx, row) + c, n, dr);
+    }
+  }
+}
+
+// All of a row's tensors start on 16-byte boundaries.
+bool vectors_ok(const AddNormArgs& a) {
+  const TensorArg* const all[] = {&a.x, &a.residual, &a.out, &a.residual_out, &a.dout, &a.dresidual_out, &a.dx, &a.dresidual};
+  for (const TensorArg* t : all) {
+    const int64_t size = t->dtype == CC1D_FLOAT32 ? 4 : 2;
+    if (t->data && ((reinterpret_cast<uintptr_t>(t->data) & 15) || (a.rows > 1 && t->s0 * size % 16))) return false;
+  }
+  return true;
+}
+
+template <typename T, typename R, bool BWD, int G, int VPT, int E, bool VEC>
+cudaError_t run(const AddNormArgs& a, cudaStream_t s) {
+  if constexpr (BWD) {
+    const size_t smem = G == 32 && a.dweight ? kThreads / 32 * 32 * VPT * E * sizeof(float) : 0;
+    cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(add_norm_bwd_kernel<T, R, G, VPT, E, VEC>), smem);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(add_norm_bwd_kernel<T, R, G, VPT, E, VEC>, dim3(static_cast<unsigned>(a.ctas)), dim3(kThreads), smem, s, a);
+  } else {
+    return launch_dependent(add_norm_fwd_kernel<T, R, G, VPT, E, VEC>, dim3(static_cast<unsigned>(a.ctas)), dim3(kThreads), 0, s, a);
+  }
+}
+
+template <typename T, typename R, bool BWD, int E, bool VEC>
+cudaError_t pick_width(const AddNormArgs& a, cudaStream_t s) {
+  constexpr int N = kThreads;
+  if (a.group == 32) {
+    if (a.held == E) return run<T, R, BWD, 32, 1, E, VEC>(a, s);
+    if (a.held == 2 * E) return run<T, R, BWD, 32, 2, E, VEC>(a, s);
+    return run<T, R, BWD, 32, 4, E, VEC>(a, s);
+  }
+  if (a.held == E) return run<T, R, BWD, N, 1, E, VEC>(a, s);
+  if (a.held == 2 * E) return run<T, R, BWD, N, 2, E, VEC>(a, s);
+  if constexpr (!BWD || E == 4) {
+    if (a.held == 8 * E) return run<T, R, BWD, N, 8, E, VEC>(a, s);
+  }
+  return run<T, R, BWD, N, 4, E, VEC>(a, s);
+}
+
+template <typename T, typename R, bool BWD>
+cudaError_t pick(AddNormArgs& a, cudaStream_t s) {
+  if (a.group == 0)
+    return BWD ? launch_dependent(add_norm_bwd_wide_kernel<T, R>, dim3(static_cast<unsigned>(a.ctas)), dim3(kThreads), 0, s, static_cast<const AddNormArgs&>(a))
+               : launch_dependent(add_norm_fwd_wide_kernel<T, R>, dim3(static_cast<unsigned>(a.rows)), dim3(kThreads), 0, s, static_cast<const AddNormArgs&>(a));
+  if (a.vectors) return pick_width<T, R, BWD, 16 / sizeof(T), true>(a, s);
+  return pick_width<T, R, BWD, 4, false>(a, s);
 }
 
 }  // namespace
 
 using DT = CC1D_DT_TYPE;
 
-cudaError_t CC1D_DT_NAME(add_norm_fwd)(const AddNormArgs& a, cudaStream_t s) {
-  return a.residual_out.dtype == CC1D_FLOAT32 ? fwd<DT, float>(a, s) : fwd<DT, DT>(a, s);
+cudaError_t CC1D_DT_NAME(add_norm_fwd)(AddNormArgs& a, cudaStream_t s) {
+  return a.residual_out.dtype == CC1D_FLOAT32 ? pick<DT, float, false>(a, s) : pick<DT, DT, false>(a, s);
 }
-cudaError_t CC1D_DT_NAME(add_norm_bwd)(const AddNormArgs& a, cudaStream_t s) {
-  return a.residual_out.dtype == CC1D_FLOAT32 ? bwd<DT, float>(a, s) : bwd<DT, DT>(a, s);
+cudaError_t CC1D_DT_NAME(add_norm_bwd)(AddNormArgs& a, cudaStream_t s) {
+  cudaError_t e = a.residual_out.dtype == CC1D_FLOAT32 ? pick<DT, float, true>(a, s) : pick<DT, DT, true>(a, s);
+  if (e == cudaSuccess && a.dweight) e = sum_rows(a.partials, a.ctas, a.dim, a.dweight, s);
+  return e;
 }
 
 #if CC1D_DT == 0
-int64_t add_norm_bwd_partial_floats(const AddNormArgs& a) { return parts_of(a) * a.dim; }
+void add_norm_plan(AddNormArgs* a, int dtype, int sms, bool bwd) {
+  a->vectors = vectors_ok(*a);
+  const int e = a->vectors && dtype != CC1D_FLOAT32 ? 8 : 4;
+  const int64_t steps = (a->dim + e - 1) / e;
+  // 64 elements of a thread are too many for the backward's arrays of them
+  const int64_t most = (bwd && e == 8 ? 4 : 8) * kThreads;
+  a->group = steps <= 128 ? 32 : steps <= most ? kThreads : 0;
+  a->held = e;
+  while (a->group && a->held / e * a->group < steps) a->held *= 2;
+  const int64_t per = a->group == 32 ? kThreads / 32 : 1, need = (a->rows + per - 1) / per;
+  const int64_t fit = static_cast<int64_t>(sms) * (a->group == 0 ? 2 : bwd ? bwd_ctas(a->held) : fwd_ctas(a->held));
+  a->ctas = need < fit ? need : fit;
+}
+
+namespace {
+// out[d] = the partial sums of column d added up in a fixed order: 32 columns by 8 warps.
+__global__ void __launch_bounds__(kThreads) sum_rows_kernel(const float* __restrict__ partials, int64_t n, int64_t dim, float* out) {
+  __shared__ float part[kThreads / 32][32];
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t d = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  float s = 0.f;
+  if (d < dim) {
+#pragma unroll 8
+    for (int64_t i = w; i < n; i += kThreads / 32) s += partials[i * dim + d];
+  }
+  part[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && d < dim) {
+#pragma unroll
+    for (int q = 1; q < kThreads / 32; ++q) s += part[q][lane];
+    out[d] = s;
+  }
+}
+}  // namespace
+
+cudaError_t sum_rows(const float* partials, int64_t n, int64_t dim, float* out, cudaStream_t s) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((dim + 31) / 32));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sum_rows_kernel, partials, n, dim, out);
+}
 #endif
 
 }  // namespace cc1d

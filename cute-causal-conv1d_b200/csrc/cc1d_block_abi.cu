@@ -259,6 +259,7 @@ cc1d_status add_norm_check(const cc1d_add_norm_params* p, bool bwd, AddNormArgs*
   a->eps = static_cast<float>(p->eps);
   a->keep_scale = static_cast<float>(1.0 / (1.0 - p->dropout_p));
   a->keep_from = static_cast<unsigned>(p->dropout_p * 4294967296.0);
+  if (p->rows > 0 && p->dim > 0) add_norm_plan(a, p->x.dtype, sm_count(), bwd);
   return CC1D_OK;
 }
 
@@ -360,7 +361,7 @@ int64_t cc1d_add_norm_bwd_workspace_bytes(const cc1d_add_norm_params* p) {
   AddNormArgs a;
   if (add_norm_check(p, true, &a) != CC1D_OK) return -1;
   if (a.rows == 0 || a.dim == 0 || !a.dweight) return 0;
-  return add_norm_bwd_partial_floats(a) * static_cast<int64_t>(sizeof(float));
+  return a.ctas * a.dim * static_cast<int64_t>(sizeof(float));
 }
 
 cc1d_status cc1d_add_norm_bwd_launch(const cc1d_add_norm_params* p, void* stream) {
@@ -374,7 +375,7 @@ cc1d_status cc1d_add_norm_bwd_launch(const cc1d_add_norm_params* p, void* stream
     return launched(cudaMemsetAsync(a.dweight, 0, a.dim * sizeof(float), s), "dropout_add_rms_norm zero fill", 0);
   }
   if (a.dweight) {
-    st = workspace_ok(p->workspace, p->workspace_bytes, add_norm_bwd_partial_floats(a) * static_cast<int64_t>(sizeof(float)));
+    st = workspace_ok(p->workspace, p->workspace_bytes, a.ctas * a.dim * static_cast<int64_t>(sizeof(float)));
     if (st != CC1D_OK) return st;
   }
   return launched(by_type(p->x.dtype, a, s, add_norm_bwd_f32, add_norm_bwd_f16, add_norm_bwd_bf16),

@@ -44,26 +44,29 @@ struct AddNormArgs {
   float* partials;
   float eps, keep_scale;     // keep_scale = 1 / (1 - p)
   unsigned keep_from;        // a word below it is dropped
+  // the plan (add_norm_plan): threads that share a row (0: rows too wide for the registers),
+  // columns that each of them holds, CTAs, and whether every row moves in 16-byte packets
+  int group, held;
+  int64_t ctas;
+  bool vectors;
 };
 
-#define CC1D_DECLARE(name, Args)                       \
-  cudaError_t name##_f32(const Args&, cudaStream_t);   \
-  cudaError_t name##_f16(const Args&, cudaStream_t);   \
-  cudaError_t name##_bf16(const Args&, cudaStream_t);
+// The launches of one element type.  Args& is changed only where a recurrence's tensor turns
+// out not to be one that the TMA can describe.
+#define CC1D_DECLARE(name, Args)                 \
+  cudaError_t name##_f32(Args&, cudaStream_t);   \
+  cudaError_t name##_f16(Args&, cudaStream_t);   \
+  cudaError_t name##_bf16(Args&, cudaStream_t);
 
-// (RecArgs is changed only where a tensor turns out not to be one that the TMA can describe)
-cudaError_t rec_fwd_f32(RecArgs&, cudaStream_t);
-cudaError_t rec_fwd_f16(RecArgs&, cudaStream_t);
-cudaError_t rec_fwd_bf16(RecArgs&, cudaStream_t);
-cudaError_t rec_bwd_f32(RecArgs&, cudaStream_t);
-cudaError_t rec_bwd_f16(RecArgs&, cudaStream_t);
-cudaError_t rec_bwd_bf16(RecArgs&, cudaStream_t);
+CC1D_DECLARE(rec_fwd, RecArgs)
+CC1D_DECLARE(rec_bwd, RecArgs)
 CC1D_DECLARE(rec_update, RecUpdateArgs)
 CC1D_DECLARE(add_norm_fwd, AddNormArgs)
 CC1D_DECLARE(add_norm_bwd, AddNormArgs)
 #undef CC1D_DECLARE
 
-// fp32 values of workspace the backward kernels need.
-int64_t add_norm_bwd_partial_floats(const AddNormArgs& a);
+void add_norm_plan(AddNormArgs* a, int dtype, int sms, bool bwd);
+// out[d] = sum over n rows of partials (n, dim), in a fixed order.
+cudaError_t sum_rows(const float* partials, int64_t n, int64_t dim, float* out, cudaStream_t s);
 
 }  // namespace cc1d

@@ -721,17 +721,6 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
   if (CLUSTER) cluster_sync();
 }
 
-// dbias[d] = the tiles' partial sums added up in order.
-__global__ void __launch_bounds__(kThreads) rec_bias_kernel(const float* __restrict__ partials, int64_t n, int64_t dim, float* dbias) {
-  grid_dependency_wait();
-  const int64_t d = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (d >= dim) return;
-  float s = 0.f;
-#pragma unroll 8
-  for (int64_t i = 0; i < n; ++i) s += partials[i * dim + d];
-  dbias[d] = s;
-}
-
 template <typename T>
 __device__ __forceinline__ float at(const TensorArg& t, int64_t b, int64_t d, int64_t l) {
   return to_f32(static_cast<const T*>(t.data)[b * t.s0 + d * t.s1 + l * t.s2]);
@@ -856,20 +845,11 @@ cudaError_t CC1D_DT_NAME(rec_fwd)(RecArgs& a, cudaStream_t s) {
 }
 cudaError_t CC1D_DT_NAME(rec_bwd)(RecArgs& a, cudaStream_t s) {
   cudaError_t e = pick<DT, true>(a, s);
-  if (e != cudaSuccess || !a.dbias) return e;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks_for(a.dim));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, rec_bias_kernel, static_cast<const float*>(a.partials), a.batch * a.cluster, a.dim, a.dbias);
+  if (e == cudaSuccess && a.dbias) e = sum_rows(a.partials, a.batch * a.cluster, a.dim, a.dbias, s);
+  return e;
 }
-cudaError_t CC1D_DT_NAME(rec_update)(const RecUpdateArgs& a, cudaStream_t s) {
-  return launch_dependent(rec_update_kernel<DT>, dim3(blocks_for(a.batch * a.dim)), dim3(kThreads), 0, s, a);
+cudaError_t CC1D_DT_NAME(rec_update)(RecUpdateArgs& a, cudaStream_t s) {
+  return launch_dependent(rec_update_kernel<DT>, dim3(blocks_for(a.batch * a.dim)), dim3(kThreads), 0, s, static_cast<const RecUpdateArgs&>(a));
 }
 
 }  // namespace cc1d
