@@ -48,22 +48,27 @@ __device__ __forceinline__ void load_cols(const T* p, int n, float (&f)[E]) {
   load_cols<T, E, VEC>(p, n, r);
   widen<T, E>(r, f);
 }
+template <typename T, int E>
+__device__ __forceinline__ void narrow(const float (&f)[E], Cols<T, E>& r) {
+  *reinterpret_cast<Packet<T, E>*>(&r) = pack<T, E>(f);
+}
 template <typename T, int E, bool VEC>
-__device__ __forceinline__ void store_cols(T* p, int n, const float (&f)[E]) {
+__device__ __forceinline__ void store_cols(T* p, int n, const Cols<T, E>& r) {
   constexpr int P = 16 / sizeof(T);
   if (VEC && n >= E) {
 #pragma unroll
-    for (int i = 0; i < E; i += P) {
-      float u[P];
-#pragma unroll
-      for (int j = 0; j < P; ++j) u[j] = f[i + j];
-      st_packet<T, P>(p + i, pack<T, P>(u));
-    }
+    for (int i = 0; i < E; i += P) *reinterpret_cast<uint4*>(p + i) = *reinterpret_cast<const uint4*>(&r.v[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < E; ++i)
-      if (i < n) p[i] = from_f32<T>(f[i]);
+      if (i < n) p[i] = r.v[i];
   }
+}
+template <typename T, int E, bool VEC>
+__device__ __forceinline__ void store_cols(T* p, int n, const float (&f)[E]) {
+  Cols<T, E> r;
+  narrow<T, E>(f, r);
+  store_cols<T, E, VEC>(p, n, r);
 }
 // The weight's columns: contiguous and aligned in packets, else one by one.
 template <int E>
@@ -79,17 +84,44 @@ __device__ __forceinline__ void load_weight(const TensorArg& w, int64_t c, int n
   for (int i = 0; i < E; ++i) f[i] = i < n ? load_any(w.data, w.dtype, (c + i) * w.s0) : 0.f;
 }
 
-// keep / (1 - p) of E columns from c (a multiple of 4) of a row.
-template <int E>
-__device__ __forceinline__ void keep_cols(const AddNormArgs& a, uint64_t key, uint64_t stream, int64_t row, int64_t c, float (&m)[E]) {
-  const uint64_t block = static_cast<uint64_t>(row) * static_cast<uint64_t>((a.dim + 3) / 4) + static_cast<uint64_t>(c / 4);
+// Dropout of N vectors of E columns; c[n] (a multiple of 4) is the first column of vector n.
+// What is dropped is not used, NaN or not.
+template <int N, int E>
+__device__ __forceinline__ void drop_cols(const AddNormArgs& a, uint64_t key, uint64_t stream, int64_t row, const int64_t (&c)[N], float (&f)[N][E]) {
+  constexpr int B = E / 4;
+  const uint64_t first = static_cast<uint64_t>(row) * static_cast<uint64_t>((a.dim + 3) / 4);
+  uint64_t block[N * B];
+  uint32_t u[N * B][4];
 #pragma unroll
-  for (int i = 0; i < E; i += 4) {
-    const uint4 u = philox(key, block + i / 4, stream);
-    m[i] = u.x >= a.keep_from ? a.keep_scale : 0.f;
-    m[i + 1] = u.y >= a.keep_from ? a.keep_scale : 0.f;
-    m[i + 2] = u.z >= a.keep_from ? a.keep_scale : 0.f;
-    m[i + 3] = u.w >= a.keep_from ? a.keep_scale : 0.f;
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < B; ++i) block[n * B + i] = first + static_cast<uint64_t>(c[n] / 4 + i);
+  philox<N * B>(key, block, stream, u);
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < E; ++i) f[n][i] = u[n * B + i / 4][i & 3] >= a.keep_from ? f[n][i] * a.keep_scale : 0.f;
+}
+// All VPT vectors of a thread, as many at a time as make 4 Philox blocks.
+template <int VPT, int E, int G>
+__device__ __forceinline__ void drop_row(const AddNormArgs& a, uint64_t key, uint64_t stream, int64_t row, int g, float (&f)[VPT][E]) {
+  constexpr int N = VPT * E <= 16 ? VPT : 16 / E;
+#pragma unroll
+  for (int v = 0; v < VPT; v += N) {
+    int64_t c[N];
+    float h[N][E];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      c[n] = static_cast<int64_t>((v + n) * G + g) * E;
+#pragma unroll
+      for (int i = 0; i < E; ++i) h[n][i] = f[v + n][i];
+    }
+    if (c[0] >= a.dim) break;
+    drop_cols<N, E>(a, key, stream, row, c, h);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[v + n][i] = h[n][i];
   }
 }
 
@@ -162,13 +194,10 @@ __global__ void __launch_bounds__(kThreads, fwd_ctas(VPT * E)) add_norm_fwd_kern
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       widen<T, E>(x[v], r[v]);
-      const int64_t c = static_cast<int64_t>(v * G + g) * E;
-      if (a.rng && c < a.dim) {
-        float m[E];
-        keep_cols<E>(a, key, stream, row, c, m);
+    }
+    if (a.rng) drop_row<VPT, E, G>(a, key, stream, row, g, r);
 #pragma unroll
-        for (int i = 0; i < E; ++i) r[v][i] = m[i] == 0.f ? 0.f : m[i] * r[v][i];  // what is dropped is not used, NaN or not
-      }
+    for (int v = 0; v < VPT; ++v) {
       if (a.residual.data) {
         float f[E];
         widen<R, E>(res[v], f);
@@ -180,12 +209,12 @@ __global__ void __launch_bounds__(kThreads, fwd_ctas(VPT * E)) add_norm_fwd_kern
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int64_t c = static_cast<int64_t>(v * G + g) * E;
+      Cols<R, E> stored;
+      narrow<R, E>(r[v], stored);
+      store_cols<R, E, VEC>(row_of<R>(a.residual_out, row) + c, cols_left(a.dim, c), stored);
+      widen<R, E>(stored, r[v]);
 #pragma unroll
-      for (int i = 0; i < E; ++i) {  // columns beyond the row are zero
-        r[v][i] = to_f32(from_f32<R>(r[v][i]));
-        sum[0] = fmaf(r[v][i], r[v][i], sum[0]);
-      }
-      store_cols<R, E, VEC>(row_of<R>(a.residual_out, row) + c, cols_left(a.dim, c), r[v]);
+      for (int i = 0; i < E; ++i) sum[0] = fmaf(r[v][i], r[v][i], sum[0]);  // columns beyond the row are zero
     }
     row_sum<G, 1>(sum, scratch, turn);
     const float rstd = 1.f / sqrtf(sum[0] / static_cast<float>(a.dim) + a.eps);
@@ -221,12 +250,7 @@ __global__ void __launch_bounds__(kThreads) add_norm_fwd_wide_kernel(const AddNo
     const int n = cols_left(a.dim, c);
     float r[E], res[E];
     load_cols<T, E, false>(row_of<T>(a.x, row) + c, n, r);
-    if (a.rng) {
-      float m[E];
-      keep_cols<E>(a, key, stream, row, c, m);
-#pragma unroll
-      for (int i = 0; i < E; ++i) r[i] = m[i] == 0.f ? 0.f : m[i] * r[i];
-    }
+    if (a.rng) drop_cols<1, E>(a, key, stream, row, {c}, reinterpret_cast<float(&)[1][E]>(r));
     if (a.residual.data) load_cols<R, E, false>(row_of<R>(a.residual, row) + c, n, res);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -303,30 +327,28 @@ __global__ void __launch_bounds__(kThreads, bwd_ctas(VPT * E)) add_norm_bwd_kern
     row_sum<G, 2>(sum, scratch, turn);
     const float rstd = 1.f / sqrtf(sum[0] * inv + a.eps);
     const float k = sum[1] * inv * rstd;  // mean(q n)
+    float dr[VPT][E];
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int64_t c = static_cast<int64_t>(v * G + g) * E;
-      const int n = cols_left(a.dim, c);
-      float rf[E], df[E], dr[E];
+      float rf[E], df[E];
       widen<R, E>(rn[v], rf);
       widen<T, E>(dyn[v], df);
-      widen<R, E>(dresn[v], dr);
+      widen<R, E>(dresn[v], dr[v]);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const float nv = rf[i] * rstd;
         dw[v][i] = fmaf(df[i], nv, dw[v][i]);
-        dr[i] = fmaf(rstd, fmaf(-nv, k, df[i] * w[v][i]), dr[i]);
+        dr[v][i] = fmaf(rstd, fmaf(-nv, k, df[i] * w[v][i]), dr[v][i]);
       }
-      if (a.dresidual.data) store_cols<R, E, VEC>(row_of<R>(a.dresidual, row) + c, n, dr);
-      if (a.dx.data) {
-        if (a.rng && n > 0) {
-          float m[E];
-          keep_cols<E>(a, key, stream, row, c, m);
+      if (a.dresidual.data) store_cols<R, E, VEC>(row_of<R>(a.dresidual, row) + c, cols_left(a.dim, c), dr[v]);
+    }
+    if (!a.dx.data) continue;
+    if (a.rng) drop_row<VPT, E, G>(a, key, stream, row, g, dr);
 #pragma unroll
-          for (int i = 0; i < E; ++i) dr[i] = m[i] == 0.f ? 0.f : m[i] * dr[i];
-        }
-        store_cols<T, E, VEC>(row_of<T>(a.dx, row) + c, n, dr);
-      }
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = static_cast<int64_t>(v * G + g) * E;
+      store_cols<T, E, VEC>(row_of<T>(a.dx, row) + c, cols_left(a.dim, c), dr[v]);
     }
   }
   if (!a.dweight) return;
@@ -383,12 +405,11 @@ __global__ void __launch_bounds__(kThreads) add_norm_bwd_wide_kernel(const AddNo
     const float k = sum[1] * inv * rstd;
     for (int64_t c = threadIdx.x * E; c < a.dim; c += kThreads * E) {
       const int n = cols_left(a.dim, c);
-      float r[E], dy[E], w[E], dr[E], m[E];
+      float r[E], dy[E], w[E], dr[E];
       load_cols<R, E, false>(row_of<R>(a.residual_out, row) + c, n, r);
       load_cols<T, E, false>(row_of<T>(a.dout, row) + c, a.dout.data ? n : 0, dy);
       load_cols<R, E, false>(row_of<R>(a.dresidual_out, row) + c, a.dresidual_out.data ? n : 0, dr);
       load_weight<E>(a.weight, c, n, w);
-      if (a.rng) keep_cols<E>(a, key, stream, row, c, m);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const float nv = r[i] * rstd;
@@ -396,9 +417,7 @@ __global__ void __launch_bounds__(kThreads) add_norm_bwd_wide_kernel(const AddNo
         dr[i] = fmaf(rstd, fmaf(-nv, k, dy[i] * w[i]), dr[i]);
       }
       if (a.dresidual.data) store_cols<R, E, false>(row_of<R>(a.dresidual, row) + c, n, dr);
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (a.rng) dr[i] = m[i] == 0.f ? 0.f : m[i] * dr[i];
+      if (a.rng) drop_cols<1, E>(a, key, stream, row, {c}, reinterpret_cast<float(&)[1][E]>(dr));
       if (a.dx.data) store_cols<T, E, false>(row_of<T>(a.dx, row) + c, n, dr);
     }
   }

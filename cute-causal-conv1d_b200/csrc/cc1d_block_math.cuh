@@ -54,22 +54,32 @@ __device__ __forceinline__ float silu_of(float z) {
 // ---------------------------------------------------------------------- Philox4x32-10
 // Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3" (2011):
 // four 32-bit words for a 128-bit counter under a 64-bit key.
-__device__ __forceinline__ uint4 philox(uint64_t key, uint64_t block, uint64_t stream) {
+// N blocks from `block` on together, so that they share the rounds' keys.
+template <int N>
+__device__ __forceinline__ void philox(uint64_t key, const uint64_t (&block)[N], uint64_t stream, uint32_t (&words)[N][4]) {
   uint32_t k0 = static_cast<uint32_t>(key), k1 = static_cast<uint32_t>(key >> 32);
-  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32);
-  uint32_t c2 = static_cast<uint32_t>(stream), c3 = static_cast<uint32_t>(stream >> 32);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    words[n][0] = static_cast<uint32_t>(block[n]);
+    words[n][1] = static_cast<uint32_t>(block[n] >> 32);
+    words[n][2] = static_cast<uint32_t>(stream);
+    words[n][3] = static_cast<uint32_t>(stream >> 32);
+  }
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
-    const uint64_t p0 = static_cast<uint64_t>(c0) * 0xD2511F53u;
-    const uint64_t p1 = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-    c0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ k0;
-    c1 = static_cast<uint32_t>(p1);
-    c2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ k1;
-    c3 = static_cast<uint32_t>(p0);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      uint32_t(&c)[4] = words[n];
+      const uint64_t p0 = static_cast<uint64_t>(c[0]) * 0xD2511F53u;
+      const uint64_t p1 = static_cast<uint64_t>(c[2]) * 0xCD9E8D57u;
+      c[0] = static_cast<uint32_t>(p1 >> 32) ^ c[1] ^ k0;
+      c[1] = static_cast<uint32_t>(p1);
+      c[2] = static_cast<uint32_t>(p0 >> 32) ^ c[3] ^ k1;
+      c[3] = static_cast<uint32_t>(p0);
+    }
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  return make_uint4(c0, c1, c2, c3);
 }
 
 }  // namespace cc1d
