@@ -325,142 +325,178 @@ def fwd_varlen_states(x, weight, bias, seq_idx, cu_seqlens, states, out, silu: b
 
 # ------------------------------------------------- recurrent-block operators
 # Their params structs are made of 64-bit words only (a cc1d_tensor is five: data, dtype
-# with the reserved half zero, three strides), so one struct.pack fills them: a decode
-# step is short enough for the host's time per call to count.
+# with the reserved half zero, three strides), so one struct.pack fills them, and the
+# checks below are written for few Python operations: a decode step is short enough for the
+# host's time per call to count.
 RECURRENCE_CHUNK = 32  # CC1D_RECURRENCE_CHUNK
 _NONE = (0, 0, 0, 0, 0)
+_PAD = ((0, 0, 0), (0, 0), (0,), ())
 RECURRENCE_PARAMS = struct.Struct("<78q")
 RECURRENCE_UPDATE_PARAMS = struct.Struct("<39q")
 ADD_NORM_PARAMS = struct.Struct("<55q2d")
+_RECURRENCE_SCRATCH = struct.Struct("<2q")  # the last words: workspace, workspace_bytes
+_ADD_NORM_SCRATCH = struct.Struct("<2q2d")  # ... and eps, dropout_p
 
 
 def _words(t: torch.Tensor | None) -> tuple:
     if t is None:
         return _NONE
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"unsupported dtype {t.dtype}")
     s = t.stride()
-    n = len(s)
-    if n == 3:
-        return (t.data_ptr(), code, *s)
-    return (t.data_ptr(), code, *s, *_NONE[n:3])
+    try:
+        return (t.data_ptr(), _DTYPES[t.dtype], *s, *_PAD[len(s)])
+    except KeyError:
+        raise TypeError(f"unsupported dtype {t.dtype}") from None
 
 
-def _recurrence_shapes(x, gate, z, bias, seq_idx, states):
-    """Checks the shapes of a recurrence's tensors against x; ``states`` are (name, tensor)
-    pairs that must all be (nstates, dim).  Returns (B, D, L, nstates)."""
-    _expect_dims("x", x, 3)
-    shape = x.shape
-    B, D, L = shape
-    _expect("gate", gate, shape)
-    _expect("z", z, shape)
-    _expect("gate_bias", bias, (D,))
-    _expect("seq_idx", seq_idx, (B, L))
-    n = B if seq_idx is None else None
-    for name, t in states:
+def _check_all(tensors) -> int:
+    """The device index of (name, tensor, shape) triples after checking the shapes (as
+    ``_expect``) and that all are on one CUDA device.  The first must be there."""
+    dev = tensors[0][1].get_device()
+    same = dev >= 0
+    for name, t, shape in tensors:
         if t is not None:
-            _expect_dims(name, t, 2)
-            if n is None:
-                n = t.shape[0]
-            _expect(name, t, (n, D))
-    return B, D, L, 0 if n is None else n
+            if t.shape != shape:
+                raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+            same = same and t.get_device() == dev
+    if not same:
+        _device_of(*(t for _, t, _ in tensors))  # raises with the reason
+    return dev
+
+
+class _DeviceStream:
+    """The current stream's handle on device ``index``, which is current meanwhile."""
+
+    __slots__ = ("index", "prev")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.prev = torch._C._cuda_getDevice()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+def _recurrence_states(batch, seq_idx, states) -> int:
+    """Rows of the states: the batch's, or with packed sequences as many as the first of
+    them has (0 if there are none)."""
+    if seq_idx is None:
+        return batch
+    for t in states:
+        if t is not None:
+            return t.shape[0]
+    return 0
 
 
 def recurrence_fwd(x, gate, z, bias, seq_idx, initial_states, final_states, checkpoints, out) -> None:
-    B, D, L, n = _recurrence_shapes(x, gate, z, bias, seq_idx,
-                                    (("initial_states", initial_states), ("final_states", final_states)))
-    _expect("out", out, (B, D, L))
-    if checkpoints is not None:
-        _expect("checkpoints", checkpoints, (B, -(-L // RECURRENCE_CHUNK), D))
-    lib = load_library()
-    dev = _device_of(x, gate, z, bias, seq_idx, initial_states, final_states, checkpoints, out)
+    _expect_dims("x", x, 3)
+    shape = x.shape
+    B, D, L = shape
+    n = _recurrence_states(B, seq_idx, (initial_states, final_states))
+    dev = _check_all((("x", x, shape), ("gate", gate, shape), ("z", z, shape), ("gate_bias", bias, (D,)),
+                      ("seq_idx", seq_idx, (B, L)), ("initial_states", initial_states, (n, D)),
+                      ("final_states", final_states, (n, D)), ("out", out, shape),
+                      ("checkpoints", checkpoints, (B, -(-L // RECURRENCE_CHUNK), D))))
     p = RECURRENCE_PARAMS.pack(
         B, D, L, n, *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(seq_idx), *_words(initial_states),
         *_words(final_states), *_words(out), *_NONE * 6, 0, 0 if checkpoints is None else checkpoints.data_ptr(), 0, 0)
-    with _Guard(dev) as stream:
-        _check(lib.cc1d_recurrence_fwd_launch(p, stream))
+    lib = _lib or load_library()
+    with _DeviceStream(dev) as stream:
+        status = lib.cc1d_recurrence_fwd_launch(p, stream)
+        if status:
+            _check(status)
 
 
 def recurrence_bwd(x, gate, z, bias, seq_idx, initial_states, checkpoints, dout, dfinal_states, dx, dgate, dz,
                    dinitial_states, dbias) -> None:
-    B, D, L, n = _recurrence_shapes(x, gate, z, bias, seq_idx,
-                                    (("initial_states", initial_states), ("dfinal_states", dfinal_states),
-                                     ("dinitial_states", dinitial_states)))
-    for name, t in (("dout", dout), ("dx", dx), ("dgate", dgate), ("dz", dz)):
-        _expect(name, t, (B, D, L))
-    _expect("checkpoints", checkpoints, (B, -(-L // RECURRENCE_CHUNK), D))
-    _expect("dbias", dbias, (D,))
-    lib = load_library()
-    dev = _device_of(x, gate, z, bias, seq_idx, initial_states, checkpoints, dout, dfinal_states, dx, dgate, dz,
-                     dinitial_states, dbias)
-    words = (
+    _expect_dims("x", x, 3)
+    shape = x.shape
+    B, D, L = shape
+    n = _recurrence_states(B, seq_idx, (initial_states, dfinal_states, dinitial_states))
+    dev = _check_all((("x", x, shape), ("gate", gate, shape), ("z", z, shape), ("gate_bias", bias, (D,)),
+                      ("seq_idx", seq_idx, (B, L)), ("initial_states", initial_states, (n, D)),
+                      ("dout", dout, shape), ("dfinal_states", dfinal_states, (n, D)), ("dx", dx, shape),
+                      ("dgate", dgate, shape), ("dz", dz, shape), ("dinitial_states", dinitial_states, (n, D)),
+                      ("dbias", dbias, (D,)), ("checkpoints", checkpoints, (B, -(-L // RECURRENCE_CHUNK), D))))
+    p = RECURRENCE_PARAMS.pack(
         B, D, L, n, *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(seq_idx), *_words(initial_states),
         *_NONE * 2, *_words(dout), *_words(dfinal_states), *_words(dx), *_words(dgate), *_words(dz),
-        *_words(dinitial_states), 0 if dbias is None else dbias.data_ptr(), checkpoints.data_ptr())
-    with _Guard(dev) as stream:
-        need = lib.cc1d_recurrence_bwd_workspace_bytes(RECURRENCE_PARAMS.pack(*words, 0, 0))
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-        p = RECURRENCE_PARAMS.pack(*words, 0 if workspace is None else workspace.data_ptr(), max(need, 0))
-        _check(lib.cc1d_recurrence_bwd_launch(p, stream))
+        *_words(dinitial_states), 0 if dbias is None else dbias.data_ptr(), checkpoints.data_ptr(), 0, 0)
+    lib = _lib or load_library()
+    with _DeviceStream(dev) as stream:
+        need = lib.cc1d_recurrence_bwd_workspace_bytes(p)
+        if need > 0:
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+            p = p[:-16] + _RECURRENCE_SCRATCH.pack(workspace.data_ptr(), need)
+        status = lib.cc1d_recurrence_bwd_launch(p, stream)
+        if status:
+            _check(status)
 
 
 def recurrence_update(x, gate, z, bias, state, state_indices, out) -> None:
-    _expect_dims("x", x, 3)
-    _expect_dims("state", state, 2)
+    """x, gate, z, out: (batch, dim) or (batch, dim, tokens)."""
     shape = x.shape
-    B, D, T = shape
-    _expect("gate", gate, shape)
-    _expect("z", z, shape)
-    _expect("gate_bias", bias, (D,))
-    _expect("state", state, (B if state_indices is None else state.shape[0], D))
-    _expect("state_indices", state_indices, (B,))
-    _expect("out", out, shape)
-    lib = load_library()
-    dev = _device_of(x, gate, z, bias, state, state_indices, out)
+    if len(shape) == 2:
+        B, D = shape
+        T = 1
+    else:
+        _expect_dims("x", x, 3)
+        B, D, T = shape
+    _expect_dims("state", state, 2)
+    n = B if state_indices is None else state.shape[0]
+    dev = _check_all((("x", x, shape), ("gate", gate, shape), ("z", z, shape), ("gate_bias", bias, (D,)),
+                      ("state", state, (n, D)), ("state_indices", state_indices, (B,)), ("out", out, shape)))
     p = RECURRENCE_UPDATE_PARAMS.pack(
-        B, D, T, state.shape[0], *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(state),
-        *_words(state_indices), *_words(out))
-    with _Guard(dev) as stream:
-        _check(lib.cc1d_recurrence_update_launch(p, stream))
+        B, D, T, n, *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(state), *_words(state_indices),
+        *_words(out))
+    lib = _lib or load_library()
+    with _DeviceStream(dev) as stream:
+        status = lib.cc1d_recurrence_update_launch(p, stream)
+        if status:
+            _check(status)
 
 
 def add_norm_fwd(x, residual, weight, rng_state, out, residual_out, eps: float, dropout_p: float) -> None:
     _expect_dims("x", x, 2)
     shape = x.shape
-    for name, t in (("residual", residual), ("out", out), ("residual_out", residual_out)):
-        _expect(name, t, shape)
-    _expect("weight", weight, (shape[1],))
-    _expect("rng_state", rng_state, (2,))
-    lib = load_library()
-    dev = _device_of(x, residual, weight, rng_state, out, residual_out)
+    dev = _check_all((("x", x, shape), ("residual", residual, shape), ("weight", weight, (shape[1],)),
+                      ("rng_state", rng_state, (2,)), ("out", out, shape), ("residual_out", residual_out, shape)))
     p = ADD_NORM_PARAMS.pack(
         *shape, *_words(x), *_words(residual), *_words(weight), *_words(rng_state), *_words(out),
         *_words(residual_out), *_NONE * 4, 0, 0, 0, eps, dropout_p)
-    with _Guard(dev) as stream:
-        _check(lib.cc1d_add_norm_fwd_launch(p, stream))
+    lib = _lib or load_library()
+    with _DeviceStream(dev) as stream:
+        status = lib.cc1d_add_norm_fwd_launch(p, stream)
+        if status:
+            _check(status)
 
 
 def add_norm_bwd(x_dtype, residual_out, weight, rng_state, dout, dresidual_out, dx, dresidual, dweight,
                  eps: float, dropout_p: float) -> None:
     _expect_dims("residual_out", residual_out, 2)
     shape = residual_out.shape
-    for name, t in (("dout", dout), ("dresidual_out", dresidual_out), ("dx", dx), ("dresidual", dresidual)):
-        _expect(name, t, shape)
-    _expect("weight", weight, (shape[1],))
-    _expect("dweight", dweight, (shape[1],))
-    _expect("rng_state", rng_state, (2,))
-    lib = load_library()
-    dev = _device_of(residual_out, weight, rng_state, dout, dresidual_out, dx, dresidual, dweight)
-    words = (
+    dev = _check_all((("residual_out", residual_out, shape), ("weight", weight, (shape[1],)),
+                      ("rng_state", rng_state, (2,)), ("dout", dout, shape), ("dresidual_out", dresidual_out, shape),
+                      ("dx", dx, shape), ("dresidual", dresidual, shape), ("dweight", dweight, (shape[1],))))
+    p = ADD_NORM_PARAMS.pack(
         *shape, 0, _DTYPES[x_dtype], 0, 0, 0, *_NONE, *_words(weight), *_words(rng_state), *_NONE,
         *_words(residual_out), *_words(dout), *_words(dresidual_out), *_words(dx), *_words(dresidual),
-        0 if dweight is None else dweight.data_ptr())
-    with _Guard(dev) as stream:
-        need = lib.cc1d_add_norm_bwd_workspace_bytes(ADD_NORM_PARAMS.pack(*words, 0, 0, eps, dropout_p))
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-        p = ADD_NORM_PARAMS.pack(*words, 0 if workspace is None else workspace.data_ptr(), max(need, 0), eps, dropout_p)
-        _check(lib.cc1d_add_norm_bwd_launch(p, stream))
+        0 if dweight is None else dweight.data_ptr(), 0, 0, eps, dropout_p)
+    lib = _lib or load_library()
+    with _DeviceStream(dev) as stream:
+        need = lib.cc1d_add_norm_bwd_workspace_bytes(p)
+        if need > 0:
+            workspace = torch.empty(need, dtype=torch.uint8, device=weight.device)
+            p = p[:-32] + _ADD_NORM_SCRATCH.pack(workspace.data_ptr(), need, eps, dropout_p)
+        status = lib.cc1d_add_norm_bwd_launch(p, stream)
+        if status:
+            _check(status)
 
 
 def launch_count() -> int:

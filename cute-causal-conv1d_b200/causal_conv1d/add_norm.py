@@ -16,7 +16,8 @@ from causal_conv1d import _abi
 
 def _rows(t, dim):
     """t as a (rows, dim) matrix with channel stride 1."""
-    t = t.reshape(-1, dim) if t.dim() != 2 else t
+    if t.dim() != 2:
+        t = t.reshape(-1, dim)
     return t if t.stride(1) == 1 else t.contiguous()
 
 
@@ -30,12 +31,13 @@ def dropout_add_rms_norm_fwd_function(x, weight, residual, eps, dropout_p, rng_s
         raise ValueError("residual must be float32 with residual_in_fp32")
     dim = x.shape[-1]
     dtype = residual.dtype if residual is not None else torch.float32 if residual_in_fp32 else x.dtype
-    out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    residual_out = torch.empty(x.shape, device=x.device, dtype=dtype)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    residual_out = torch.empty_like(out, dtype=dtype)
     if dim == 0:
         return out, residual_out
-    _abi.add_norm_fwd(_rows(x, dim), None if residual is None else _rows(residual, dim), weight, rng_state,
-                      out.view(-1, dim), residual_out.view(-1, dim), eps, dropout_p)
+    flat = (out, residual_out) if out.dim() == 2 else (out.view(-1, dim), residual_out.view(-1, dim))
+    _abi.add_norm_fwd(_rows(x, dim), None if residual is None else _rows(residual, dim), weight, rng_state, *flat,
+                      eps, dropout_p)
     return out, residual_out
 
 

@@ -20,9 +20,11 @@ from causal_conv1d.cpp_functions import _like_layout
 
 def _laid_out(x, *others):
     """x with a unit stride along dim or seqlen, and the others in x's layout."""
-    if x.stride(1) != 1 and x.stride(2) != 1:
+    s = x.stride()
+    if s[1] != 1 and s[2] != 1:
         x = x.contiguous()
-    return x, *(t if t is None or t.dim() != 3 else _like_layout(t, x) for t in others)
+        s = x.stride()
+    return x, *(t if t is None or t.stride() == s or t.dim() != 3 else _like_layout(t, x) for t in others)
 
 
 def gated_recurrence_fwd_function(x, gate, z, gate_bias, seq_idx, initial_states, return_final_states,
@@ -139,17 +141,11 @@ def gated_recurrence_update(x, state, gate, z=None, gate_bias=None, state_indice
     state_indices[b]; an index outside the pool is padding (zero output, no state
     touched), and no row may be named twice.  Returns out with x's shape.
     """
-    flat = x.dim() == 2
-    if flat:
-        x = x.unsqueeze(-1)
-        gate = gate.unsqueeze(-1)
-        if z is not None:
-            z = z.unsqueeze(-1)
-    if state_indices is not None and state_indices.dtype != torch.int32:
+    if state_indices is not None and state_indices.dtype is not torch.int32:
         state_indices = state_indices.to(torch.int32)
     out = torch.empty_like(x)
     _abi.recurrence_update(x, gate, z, gate_bias, state, state_indices, out)
-    return out.squeeze(-1) if flat else out
+    return out
 
 
 def gated_recurrence_ref(x, gate, z=None, gate_bias=None, seq_idx=None, initial_states=None,
