@@ -39,7 +39,7 @@ UNITS = [
 ] + [
     (src, [f"-DCC1D_DT={dt}"], f"{src[:-3]}_{name}.o")
     for src in ("cc1d_fwd.cu", "cc1d_bwd.cu", "cc1d_rows.cu", "cc1d_rowwalk.cu",
-                "cc1d_recurrence.cu", "cc1d_add_norm.cu")
+                "cc1d_recurrence.cu", "cc1d_recurrence_update.cu", "cc1d_add_norm.cu")
     for dt, name in ((0, "f32"), (1, "f16"), (2, "bf16"))
 ]
 

@@ -132,7 +132,7 @@ cc1d_status rec_plan(RecArgs* a, bool bwd) {
   a->dtiles = (a->dim + channels - 1) / channels;
   const int64_t tiles = a->batch * a->dtiles;
   const int64_t tile = 4096 + (a->move == kPackets ? (a->rows ? 1024 : 512) : 0), z = a->z.data ? 1 : 0;
-  a->cluster = choose_cluster(tiles, a->nchunks, bwd ? 3 * (3 + z) * tile + 8064 : 4 * (2 + z) * tile + 6016, bwd);
+  a->cluster = choose_cluster(tiles, a->nchunks, bwd ? 3 * (3 + z) * tile + 8064 : (a->move == kPackets && !a->rows ? 3 : 4) * (2 + z) * tile + 6016, bwd);
   if (tiles * a->cluster > kMax31) return fail(CC1D_ERR_VALUE, "batch * dim is too large");
   return CC1D_OK;
 }
@@ -330,6 +330,7 @@ cc1d_status cc1d_recurrence_update_launch(const cc1d_recurrence_update_params* p
   CC1D_REQUIRE(p->gate, "gate");
   CC1D_REQUIRE(p->out, "out");
   if (N > 0) CC1D_REQUIRE(p->state, "state");
+  if (B * D > kMax31 * 256) return fail(CC1D_ERR_VALUE, "batch * dim is too large");
   RecUpdateArgs a;
   a.batch = B;
   a.dim = D;

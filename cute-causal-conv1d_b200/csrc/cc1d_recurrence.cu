@@ -30,7 +30,9 @@ namespace {
 
 // Ring slots: the chunk in work, the one before, whose results are still being stored from its
 // tiles, and one (backward) or two chunks that are being loaded.
-constexpr int kFwdStages = 4, kBwdStages = 3;
+// (strips off their alignment have larger tiles, and channel-last none that are stored from).
+template <bool SKEW, int LAYOUT> constexpr int kFwdStages = SKEW && LAYOUT != kLayoutRows ? 3 : 4;
+constexpr int kBwdStages = 3, kMostStages = 4;
 
 // s = 1 / (1 + exp(-v)) at a warp's 8 positions, and e = exp(-v) if wanted.  For 16-bit tensors
 // -v log2(e) = v m + n with m = -log2(e), for fp32 n is added to v.
@@ -102,6 +104,12 @@ __device__ __forceinline__ Lane<4 / sizeof(T)> gate_offset(const RecArgs& a, int
 // A gate that holds the state: a = 1 and 1 - a = 0 whatever the bias.  Positions without a token
 // get it (and zeros for the rest), in shared memory, before they are read.
 constexpr float kHold = 60000.f;
+
+template <typename T, int LAYOUT, bool SKEW>
+__device__ __forceinline__ void load_by_threads(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
+  if constexpr (SKEW) load_strips<T, LAYOUT>(tile, t, t0, nd, nt);
+  else load_tile<T, LAYOUT>(tile, t, t0, nd, nt);
+}
 
 // Positions of a chunk or of a warp, t .. t + n - 1, that lie within the sequence (may be <= 0).
 __device__ __forceinline__ int within(int64_t t, int64_t len, int n) {
@@ -224,7 +232,7 @@ template <int V> struct Common {
   Lane<V> handed[2][32];
   Lane<V> start[3][32];
   int ids[3][kRecChunk + 4];
-  uint64_t bars[kFwdStages + 2];
+  uint64_t bars[kMostStages + 2];
 };
 
 // Starts the copy of a round's ids; the caller commits.  Outside the sequence they are -1.
@@ -253,7 +261,7 @@ __device__ __forceinline__ void start_barriers(unsigned bars, bool tma) {
 template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z, bool CLUSTER>
 __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
   using C = Tile<T, LAYOUT, SKEW>;
-  constexpr int V = C::V, NT = Z ? 3 : 2, S = kFwdStages;
+  constexpr int V = C::V, NT = Z ? 3 : 2, S = kFwdStages<SKEW, LAYOUT>;
   using L = Lane<V>;
   extern __shared__ __align__(1024) unsigned char smem[];
   // ring of tiles (gate, x, z) | sums of the warps [2] | maps of the cluster [2][cluster][32] | common
@@ -265,6 +273,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const Place p = place_of<C::kChannels, CLUSTER>(a);
   const bool tma = !SKEW && a.move == kTma;
+  constexpr bool kDirect = SKEW && !C::kRows;  // results are stored from registers
   start_barriers<S, CLUSTER>(bars, tma);
   grid_dependency_wait();
   const Strip<T> gt = strip_of<T>(a.gate, maps.gate, p.b, p.d0), xt = strip_of<T>(a.x, maps.x, p.b, p.d0);
@@ -289,9 +298,9 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
         }
       } else {
         if (nt > 0) {
-          load_tile<T, LAYOUT, SKEW>(smem + o, gt, t0, p.nd, nt);
-          load_tile<T, LAYOUT, SKEW>(smem + o + C::kBytes, xt, t0, p.nd, nt);
-          if constexpr (Z) load_tile<T, LAYOUT, SKEW>(smem + o + 2 * C::kBytes, zt, t0, p.nd, nt);
+          load_by_threads<T, LAYOUT, SKEW>(smem + o, gt, t0, p.nd, nt);
+          load_by_threads<T, LAYOUT, SKEW>(smem + o + C::kBytes, xt, t0, p.nd, nt);
+          if constexpr (Z) load_by_threads<T, LAYOUT, SKEW>(smem + o + 2 * C::kBytes, zt, t0, p.nd, nt);
         }
         mbar_arrive_copies(bar);  // of the asynchronous copies
         mbar_arrive(bar);         // and of the plain stores
@@ -313,7 +322,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
   };
 #pragma unroll
   for (int k = 0; k < S - 2; ++k) load(k);
-  if (tma) load(S - 2);
+  if (tma || kDirect) load(S - 2);
   const L nb = gate_offset<T, LAYOUT>(a, p.d0, lane);
   L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.init, p.b, a.nstates, p.d0, a.dim, lane);
   if (w == 0) common.handed[0][lane] = carry;
@@ -342,16 +351,21 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     Edges e;
     if constexpr (SEQ) {
       e = edges_of(lane < kRecSteps + 2 ? common.ids[k % 3][w * kRecSteps + lane] : -1);
-      if (e.valid != 0xffu) {  // rare: positions without a token pass the state on
-        set_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, ~e.valid, kHold);
-        set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, ~e.valid, 0.f);
-        __syncwarp();
-      }
+    }
+    // Rare: positions without a token pass the state on.  z as well: four positions share a
+    // reciprocal, and their roundings must not depend on what padding or old tiles hold (the
+    // TMA fills up with zeros).
+    const unsigned valid = SEQ ? e.valid : SKEW ? below(within(tw, a.seqlen, kRecSteps)) : 0xffu;
+    if (valid != 0xffu) {
+      set_steps<T, LAYOUT, SKEW>(now, gt, w, lane, ~valid, kHold);
+      set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, ~valid, 0.f);
+      if constexpr (Z) set_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, zt, w, lane, ~valid, 0.f);
+      __syncwarp();
     }
     // the 8 positions' maps and their composition
     L ga[kRecSteps], gb[kRecSteps];
-    read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, ga);
-    read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, gb);
+    read_steps<T, LAYOUT, SKEW>(now, gt, w, lane, ga);
+    read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, gb);
     sigmoids<T, V, false, true>(ga, nb, ga, nullptr);
     // 1 - a from a: a + (1 - a) is then exactly one, and the error of 2^-24 is that of a itself
 #pragma unroll
@@ -380,12 +394,13 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     const unsigned cuts = SEQ ? cuts_of(sum.cut, lane) : 0;
     if (CLUSTER) send_to_cluster<V, SEQ, true>(sum.A, sum.H, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), p, w, lane);
     copy_ids(k + 2);
-    if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
-    if (!tma) load(k + S - 2);  // into the slot that was stored a round ago
+    if (!kDirect && k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
+    if (kDirect) load(k + S - 1);       // into the last round's slot
+    else if (!tma) load(k + S - 2);     // into the slot that was stored a round ago
     L zs[kRecSteps];
     auto silu = [&] {
       L z[kRecSteps];
-      read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, zt, t0, w, lane, z);
+      read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, zt, w, lane, z);
       sigmoids<T, V, false, false>(z, splat(0.f, L{}), zs, nullptr);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) zs[j] = mul(zs[j], z[j]);
@@ -436,8 +451,12 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gb[j], zs[j]);
     }
-    write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gb);
-    if (SEQ && e.valid != 0xffu) clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~e.valid);
+    if constexpr (kDirect) {
+      store_halves<T>(ot, tw, lane, p.nd - 2 * lane, within(tw, a.seqlen, kRecSteps), SEQ ? ~e.valid & 0xffu : 0u, gb);
+    } else {
+      write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gb);
+      if (SEQ && e.valid != 0xffu) clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~e.valid);
+    }
     if (tma) {
       tma_fence();
       if (threadIdx.x == 0) tma_wait_read<0>();  // by now the last round's tiles have been stored
@@ -446,7 +465,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     if (++slot == S) slot = 0, parity ^= 1;
   }
   __syncthreads();
-  store(p.rounds - 1, slot == 0 ? S - 1 : slot - 1);
+  if (!kDirect) store(p.rounds - 1, slot == 0 ? S - 1 : slot - 1);
   if (tma && threadIdx.x == 0) tma_wait_read<0>();
   if (CLUSTER) cluster_sync();  // no CTA leaves while a partner may still write to it
 }
@@ -468,6 +487,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const Place p = place_of<C::kChannels, CLUSTER>(a);
   const bool tma = !SKEW && a.move == kTma;
+  constexpr bool kDirect = SKEW && !C::kRows;  // results are stored from registers
   start_barriers<S, CLUSTER>(bars, tma);
   grid_dependency_wait();
   const Strip<T> gt = strip_of<T>(a.gate, maps.gate, p.b, p.d0), xt = strip_of<T>(a.x, maps.x, p.b, p.d0);
@@ -496,13 +516,13 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
         }
       } else {
         if (nt > 0) {
-          load_tile<T, LAYOUT, SKEW>(smem + o, gt, t0, p.nd, nt);
-          load_tile<T, LAYOUT, SKEW>(smem + o + C::kBytes, xt, t0, p.nd, nt);
-          load_tile<T, LAYOUT, SKEW>(smem + o + 2 * C::kBytes, yt, t0, p.nd, nt);
-          if constexpr (Z) load_tile<T, LAYOUT, SKEW>(smem + o + 3 * C::kBytes, zt, t0, p.nd, nt);
+          load_by_threads<T, LAYOUT, SKEW>(smem + o, gt, t0, p.nd, nt);
+          load_by_threads<T, LAYOUT, SKEW>(smem + o + C::kBytes, xt, t0, p.nd, nt);
+          load_by_threads<T, LAYOUT, SKEW>(smem + o + 2 * C::kBytes, yt, t0, p.nd, nt);
+          if constexpr (Z) load_by_threads<T, LAYOUT, SKEW>(smem + o + 3 * C::kBytes, zt, t0, p.nd, nt);
         }
-        mbar_arrive_copies(bar);  // of the asynchronous copies
-        mbar_arrive(bar);         // and of the plain stores
+        mbar_arrive_copies(bar);
+        mbar_arrive(bar);
       }
     }
     if (++load_slot == S) load_slot = 0;
@@ -543,7 +563,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
   };
 #pragma unroll
   for (int k = 0; k < S - 2; ++k) load(k);
-  if (tma) load(S - 2);
+  if (tma || kDirect) load(S - 2);
   const L nb = gate_offset<T, LAYOUT>(a, p.d0, lane);
   L carry = SEQ ? splat(0.f, L{}) : load_state<T, LAYOUT>(a.dfinal, p.b, a.nstates, p.d0, a.dim, lane);
   if (w == 0) common.handed[0][lane] = carry;
@@ -568,27 +588,27 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
       valid = e.valid;
     }
     if (valid != 0xffu) {  // rare: positions without a token pass the gradient on
-      set_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, ~valid, kHold);
-      set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, ~valid, 0.f);
-      set_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, yt, t0, w, lane, ~valid, 0.f);
-      if constexpr (Z) set_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, t0, w, lane, ~valid, 0.f);
+      set_steps<T, LAYOUT, SKEW>(now, gt, w, lane, ~valid, kHold);
+      set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, ~valid, 0.f);
+      set_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, yt, w, lane, ~valid, 0.f);
+      if constexpr (Z) set_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, w, lane, ~valid, 0.f);
       __syncwarp();
     }
     L ga[kRecSteps], gc[kRecSteps], x[kRecSteps], gy[kRecSteps], dz[kRecSteps];
     {
       L g[kRecSteps];
-      read_steps<T, LAYOUT, SKEW>(now, gt, t0, w, lane, g);
+      read_steps<T, LAYOUT, SKEW>(now, gt, w, lane, g);
       // the gradients have 1 - a as a factor, so it is taken to full relative precision
       sigmoids<T, V, true, true>(g, nb, ga, gc);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) gc[j] = mul(gc[j], ga[j]);
       if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
     }
-    read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, t0, w, lane, x);
-    read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, yt, t0, w, lane, gy);
+    read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, x);
+    read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, yt, w, lane, gy);
     if constexpr (Z) {
       L z[kRecSteps], s[kRecSteps];
-      read_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, t0, w, lane, z);
+      read_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, w, lane, z);
       sigmoids<T, V, false, false>(z, splat(0.f, L{}), s, nullptr);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
@@ -635,8 +655,9 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     const unsigned cuts = SEQ ? cuts_of(sum_back.cut, lane) : 0;
     if (CLUSTER) send_to_cluster<V, SEQ, false>(sum.A, sum_back.B, cuts, far + buf * p.cluster * 32, bars + 8 * (S + buf), p, w, lane);
     copy_ahead(k + 2);
-    if (k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
-    if (!tma) load(k + S - 2);
+    if (!kDirect && k > 0) store(k - 1, slot == 0 ? S - 1 : slot - 1);
+    if (kDirect) load(k + S - 1);
+    else if (!tma) load(k + S - 2);
     L h = through_warps<V, SEQ, true>(sum.A, sum.H, SEQ ? cuts_of(sum.cut, lane) : 0, w, lane, common.start[k % 3][lane]);
 
     // forward through the positions: h before each, and dz
@@ -683,13 +704,21 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
       for (int j = kRecSteps - 1; j >= 0; --j) step_back(j);
     }
     if (!CLUSTER && w == 0) common.handed[buf ^ 1][lane] = s;
-    write_steps<T, LAYOUT, SKEW>(now, w, lane, prev);
-    write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gy);
-    if constexpr (Z) write_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, w, lane, dz);
-    if (SEQ && valid != 0xffu) {
-      clear_steps<T, LAYOUT, SKEW>(now, w, lane, ~valid);
-      clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~valid);
-      if constexpr (Z) clear_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, w, lane, ~valid);
+    if constexpr (kDirect) {
+      const int left = within(tw, a.seqlen, kRecSteps), n = p.nd - 2 * lane;
+      const unsigned clear = SEQ ? ~valid & 0xffu : 0u;
+      store_halves<T>(dgt, tw, lane, n, left, clear, prev);
+      store_halves<T>(dxt, tw, lane, n, left, clear, gy);
+      if constexpr (Z) store_halves<T>(dzt, tw, lane, n, left, clear, dz);
+    } else {
+      write_steps<T, LAYOUT, SKEW>(now, w, lane, prev);
+      write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gy);
+      if constexpr (Z) write_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, w, lane, dz);
+      if (SEQ && valid != 0xffu) {
+        clear_steps<T, LAYOUT, SKEW>(now, w, lane, ~valid);
+        clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~valid);
+        if constexpr (Z) clear_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, w, lane, ~valid);
+      }
     }
     if (tma) {
       tma_fence();
@@ -699,7 +728,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     if (++slot == S) slot = 0, parity ^= 1;
   }
   __syncthreads();
-  store(p.rounds - 1, slot == 0 ? S - 1 : slot - 1);
+  if (!kDirect) store(p.rounds - 1, slot == 0 ? S - 1 : slot - 1);
   if (!SEQ && w == 0 && p.rank == 0)
     store_state<T, LAYOUT>(a.dinit, p.b, a.nstates, p.d0, a.dim, lane, !CLUSTER ? common.handed[p.rounds & 1][lane] : carry);
   if (a.dbias) {
@@ -720,40 +749,6 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
   if (tma && threadIdx.x == 0) tma_wait_read<0>();
   if (CLUSTER) cluster_sync();
 }
-
-template <typename T>
-__device__ __forceinline__ float at(const TensorArg& t, int64_t b, int64_t d, int64_t l) {
-  return to_f32(static_cast<const T*>(t.data)[b * t.s0 + d * t.s1 + l * t.s2]);
-}
-template <typename T>
-__device__ __forceinline__ void put(const TensorArg& t, int64_t b, int64_t d, int64_t l, float v) {
-  static_cast<T*>(t.data)[b * t.s0 + d * t.s1 + l * t.s2] = from_f32<T>(v);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) rec_update_kernel(const RecUpdateArgs a) {
-  grid_dependency_wait();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= a.batch * a.dim) return;
-  const int64_t b = i / a.dim, d = i - b * a.dim;
-  const int64_t row = a.indices ? a.indices[b * a.indices_stride] : b;
-  if (row < 0 || row >= a.nstates) {
-    for (int64_t l = 0; l < a.seqlen; ++l) put<T>(a.out, b, d, l, 0.f);
-    return;
-  }
-  const float bias = a.bias.data ? load_any(a.bias.data, a.bias.dtype, d * a.bias.s0) : 0.f;
-  float* hp = static_cast<float*>(a.state.data) + row * a.state.s0 + d * a.state.s1;
-  float h = *hp;
-  for (int64_t l = 0; l < a.seqlen; ++l) {
-    float ga, gc;
-    sigmoid_pair<T>(at<T>(a.gate, b, d, l) + bias, ga, gc);
-    h = fmaf(ga, h, gc * at<T>(a.x, b, d, l));
-    put<T>(a.out, b, d, l, a.z.data ? h * silu_of<T>(at<T>(a.z, b, d, l)) : h);
-  }
-  *hp = h;
-}
-
-unsigned blocks_for(int64_t threads) { return static_cast<unsigned>((threads + kThreads - 1) / kThreads); }
 
 // The tensor map of a strip-wise aligned tensor; channel-last (dim, seqlen, batch), rows
 // (seqlen, dim, batch), boxes of a tile's strips.
@@ -786,7 +781,7 @@ template <typename T, int LAYOUT, bool SKEW, bool BWD, bool SEQ, bool Z, bool CL
 cudaError_t run(RecArgs& a, cudaStream_t s) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int NT = (BWD ? 3 : 2) + (Z ? 1 : 0);
-  constexpr int stages = BWD ? kBwdStages : kFwdStages;
+  constexpr int stages = BWD ? kBwdStages : kFwdStages<SKEW, LAYOUT>;
   RecMaps maps = {};
   if (a.move == kTma) {
     const bool ok = make_map<T, LAYOUT>(&maps.gate, a.gate, a) && make_map<T, LAYOUT>(&maps.x, a.x, a) && make_map<T, LAYOUT>(&maps.z, a.z, a) &&
@@ -848,8 +843,4 @@ cudaError_t CC1D_DT_NAME(rec_bwd)(RecArgs& a, cudaStream_t s) {
   if (e == cudaSuccess && a.dbias) e = sum_rows(a.partials, a.batch * a.cluster, a.dim, a.dbias, s);
   return e;
 }
-cudaError_t CC1D_DT_NAME(rec_update)(RecUpdateArgs& a, cudaStream_t s) {
-  return launch_dependent(rec_update_kernel<DT>, dim3(blocks_for(a.batch * a.dim)), dim3(kThreads), 0, s, static_cast<const RecUpdateArgs&>(a));
-}
-
 }  // namespace cc1d

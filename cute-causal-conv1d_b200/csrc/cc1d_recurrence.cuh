@@ -124,7 +124,7 @@ __device__ __forceinline__ int lane_channel(int lane, int i) {
 }
 
 // One of the (batch, dim, seqlen) tensors as a CTA sees it: its tile of channels in its batch
-// row.  `origin` is the tensor's first element: nothing before it is read.
+// row.  Nothing before `origin`, its first element, is read.
 template <typename T>
 struct Strip {
   T* origin;
@@ -159,61 +159,69 @@ template <int N> __device__ __forceinline__ void tma_wait_read() { asm volatile(
 // What this thread wrote to shared memory is there for the TMA.
 __device__ __forceinline__ void tma_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-// kPackets and kElements, all threads: positions t0 .. t0 + nt - 1 of nd channels; places
-// outside are zero.
-template <typename T, int LAYOUT, bool SKEW>
-__device__ __forceinline__ void load_tile(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
-  using C = Tile<T, LAYOUT, SKEW>;
-  const unsigned base = shared_addr(tile);
-  if constexpr (SKEW) {
-    constexpr int P = C::kPitch / 16, N = C::kStrips * P;
-    const int64_t step = (C::kRows ? t.s1 : t.s2) * C::kSize;
-    const int strips = C::kRows ? nd : nt, bytes = (C::kRows ? nt : nd) * C::kSize;
-    const char* const from = reinterpret_cast<const char*>(t.row + (C::kRows ? t0 : t0 * t.s2));
-    const char* const origin = reinterpret_cast<const char*>(t.origin);
-#pragma unroll
-    for (int k = 0; k < (N + kRecThreads - 1) / kRecThreads; ++k) {
-      const int i = threadIdx.x + k * kRecThreads, r = i / P, c = i % P * 16;
-      if (N % kRecThreads && i >= N) break;
-      const char* const strip = from + r * step;
-      const int off = static_cast<int>(reinterpret_cast<uintptr_t>(strip)) & 15;
-      const int n = r < strips ? max(0, min(16, off + bytes - c)) : 0;  // up to the strip's end
-      const char* const src = strip - off + c;
-      const unsigned dst = base + r * C::kPitch + c;
-      if (n > 0 && src < origin) {  // the tensor begins within the packet
-        for (int e = off; e < n; e += C::kSize)
-          *reinterpret_cast<uint16_t*>(tile + r * C::kPitch + e) = *reinterpret_cast<const uint16_t*>(src + e);
-      } else {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(n > 0 ? src : reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(origin) & ~uintptr_t{15})), "r"(n) : "memory");
-      }
-    }
+// kPackets, all threads: starts the copy of a chunk's strips into a tile, the packets that cover
+// each.  A thread has every second (rows) or fourth packet of one strip.  Places outside the
+// chunk's nt positions of nd channels are zero or left as they are.
+template <typename T, int LAYOUT>
+__device__ __forceinline__ void load_strips(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
+  using C = Tile<T, LAYOUT, true>;
+  constexpr int N = kRecThreads / C::kStrips;                      // threads of a strip
+  constexpr int K = (C::kPitch / 16 + N - 1) / N;                  // packets of a thread
+  const int r = threadIdx.x / N, c = threadIdx.x % N * 16;
+  const int64_t step = (C::kRows ? t.s1 : t.s2) * C::kSize;
+  const int bytes = r < (C::kRows ? nd : nt) ? (C::kRows ? nt : nd) * C::kSize : -16;
+  const char* const strip = reinterpret_cast<const char*>(t.row + (C::kRows ? t0 : t0 * t.s2)) + r * step;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(strip)) & 15;
+  const char* const src = strip - off + c;
+  unsigned char* const dst = tile + r * C::kPitch + c;
+  const unsigned to = shared_addr(dst);
+  const int left = off + bytes - c;  // up to the strip's end
+  if (bytes > 0 && c == 0 && src < reinterpret_cast<const char*>(t.origin)) {  // the tensor begins within the first packet
+    for (int e = off; e < min(16, left); e += C::kSize) *reinterpret_cast<uint16_t*>(dst + e) = *reinterpret_cast<const uint16_t*>(src + e);
   } else {
-    const T* const src = t.row + t0 * t.s2;
-    constexpr int N = C::kChannels * kRecChunk / kRecThreads;
+    const int n = max(0, min(16, left));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(n ? src : strip - off), "r"(n) : "memory");
+  }
+#pragma unroll
+  for (int k = 1; k < K; ++k) {
+    if ((k + 1) * N * 16 > C::kPitch && c + k * N * 16 >= C::kPitch) break;
+    const int n = max(0, min(16, left - k * N * 16));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to + k * N * 16), "l"(src + k * N * 16), "r"(n) : "memory");
+  }
+}
+
+// kElements, all threads: positions t0 .. t0 + nt - 1 of nd channels; places outside are zero.
+template <typename T, int LAYOUT>
+__device__ __forceinline__ void load_tile(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
+  using C = Tile<T, LAYOUT, false>;
+  const unsigned base = shared_addr(tile);
+  const T* const src = t.row + t0 * t.s2;
+  constexpr int N = C::kChannels * kRecChunk / kRecThreads;
 #pragma unroll 4
-    for (int k = 0; k < N; ++k) {
-      const int i = threadIdx.x + k * kRecThreads;
-      const int ch = C::kRows ? i / kRecChunk : i % C::kChannels, p = C::kRows ? i % kRecChunk : i / C::kChannels;
-      const bool in = ch < nd && p < nt;
-      const T* from = in ? src + ch * t.s1 + p * t.s2 : t.origin;
-      if constexpr (C::kSize == 4) {
-        cp4(base + C::at(ch, p), from, in ? 4 : 0);
-      } else {
-        *reinterpret_cast<T*>(tile + C::at(ch, p)) = in ? *from : from_f32<T>(0.f);
-      }
+  for (int k = 0; k < N; ++k) {
+    const int i = threadIdx.x + k * kRecThreads;
+    const int ch = C::kRows ? i / kRecChunk : i % C::kChannels, p = C::kRows ? i % kRecChunk : i / C::kChannels;
+    const bool in = ch < nd && p < nt;
+    const T* from = in ? src + ch * t.s1 + p * t.s2 : t.origin;
+    if constexpr (C::kSize == 4) {
+      cp4(base + C::at(ch, p), from, in ? 4 : 0);
+    } else {
+      *reinterpret_cast<T*>(tile + C::at(ch, p)) = in ? *from : from_f32<T>(0.f);
     }
   }
 }
 
-// The low half of the address of element p[i * step].
-template <typename T>
-__device__ __forceinline__ unsigned low_address(const T* p, int i, int64_t step) {
-  return static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)) + static_cast<unsigned>(i) * static_cast<unsigned>(step) * static_cast<unsigned>(sizeof(T));
+// kPackets: bytes that strip i of a chunk starts off a 16-byte boundary.  Chunks and warps are
+// 32 and 8 positions apart, multiples of 16 bytes in either layout, so neither matters.
+template <typename T, int LAYOUT>
+__device__ __forceinline__ unsigned offset_of(const Strip<T>& t, int i) {
+  const unsigned step = static_cast<unsigned>(LAYOUT == kLayoutRows ? t.s1 : t.s2) * static_cast<unsigned>(sizeof(T));
+  return (static_cast<unsigned>(reinterpret_cast<uintptr_t>(t.row)) + static_cast<unsigned>(i) * step) & 15u;
 }
 
 // The 8 positions of warp w and the lane's V channels, as fp32.
 template <typename T, int LAYOUT, bool SKEW>
-__device__ __forceinline__ void read_steps(const unsigned char* tile, const Strip<T>& t, int64_t t0, int w, int lane, Lane<4 / sizeof(T)> (&f)[kRecSteps]) {
+__device__ __forceinline__ void read_steps(const unsigned char* tile, const Strip<T>& t, int w, int lane, Lane<4 / sizeof(T)> (&f)[kRecSteps]) {
   using C = Tile<T, LAYOUT, SKEW>;
   if constexpr (C::kRows) {
 #pragma unroll
@@ -223,7 +231,7 @@ __device__ __forceinline__ void read_steps(const unsigned char* tile, const Stri
       for (int q = 0; q < kRecSteps / C::kPacket; ++q) {
         uint4 u;
         if constexpr (SKEW) {
-          const unsigned off = low_address(t.row + t0, ch, t.s1) & 15, sh = (off & 2) * 8;
+          const unsigned off = offset_of<T, LAYOUT>(t, ch), sh = (off & 2) * 8;
           const uint32_t* p = reinterpret_cast<const uint32_t*>(tile + ch * C::kPitch + w * 16 + (off & 12));
           const uint32_t w0 = p[0], w1 = p[1], w2 = p[2], w3 = p[3], w4 = p[4];
           u = make_uint4(__funnelshift_r(w0, w1, sh), __funnelshift_r(w1, w2, sh), __funnelshift_r(w2, w3, sh), __funnelshift_r(w3, w4, sh));
@@ -246,7 +254,7 @@ __device__ __forceinline__ void read_steps(const unsigned char* tile, const Stri
       if constexpr (C::V == 2) {
         uint32_t u;
         if constexpr (SKEW) {
-          const unsigned off = low_address(t.row + t0 * t.s2, w * kRecSteps + j, t.s2) & 15;
+          const unsigned off = offset_of<T, LAYOUT>(t, j);
           const uint32_t* q = reinterpret_cast<const uint32_t*>(p + j * C::kPitch + (off & 12));
           u = __funnelshift_r(q[0], q[1], (off & 2) * 8);
         } else {
@@ -294,7 +302,7 @@ __device__ __forceinline__ void write_steps(unsigned char* tile, int w, int lane
 
 // Sets the positions of `mask` among the warp's 8 to a value, in a tile as it was loaded.
 template <typename T, int LAYOUT, bool SKEW>
-__device__ __forceinline__ void set_steps(unsigned char* tile, const Strip<T>& t, int64_t t0, int w, int lane, unsigned mask, float value) {
+__device__ __forceinline__ void set_steps(unsigned char* tile, const Strip<T>& t, int w, int lane, unsigned mask, float value) {
   using C = Tile<T, LAYOUT, SKEW>;
 #pragma unroll 1
   for (int j = 0; j < kRecSteps; ++j) {
@@ -304,7 +312,7 @@ __device__ __forceinline__ void set_steps(unsigned char* tile, const Strip<T>& t
     for (int i = 0; i < C::V; ++i) {
       const int ch = lane_channel<T, LAYOUT>(lane, i);
       int o = C::at(ch, pos);
-      if constexpr (SKEW) o += C::kRows ? low_address(t.row + t0, ch, t.s1) & 15 : low_address(t.row + t0 * t.s2, pos, t.s2) & 15;
+      if constexpr (SKEW) o += offset_of<T, LAYOUT>(t, C::kRows ? ch : j);
       *reinterpret_cast<T*>(tile + o) = from_f32<T>(value);
     }
   }
@@ -322,28 +330,28 @@ __device__ __forceinline__ void clear_steps(unsigned char* tile, int w, int lane
   }
 }
 
-// kPackets and kElements, all threads: stores what write_steps put into a tile.
+// kElements and kPackets with rows, all threads: stores what write_steps put into a tile.
 template <typename T, int LAYOUT, bool SKEW>
 __device__ __forceinline__ void store_tile(const unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
   using C = Tile<T, LAYOUT, SKEW>;
   if constexpr (SKEW) {
-    constexpr int W = C::kStripBytes / 4;  // words of a strip, and one more where it starts within a word
-    const int64_t step = (C::kRows ? t.s1 : t.s2) * C::kSize;
-    const int strips = C::kRows ? nd : nt, len = C::kRows ? nt : nd;
-    char* const to = reinterpret_cast<char*>(t.row + (C::kRows ? t0 : t0 * t.s2));
+    // the 4-byte words of a strip as it lies in memory: 16, and one more where it starts within one
+    constexpr int W = C::kStripBytes / 4;
+    const int64_t step = t.s1 * C::kSize;
+    char* const to = reinterpret_cast<char*>(t.row + t0);
     auto word = [&](int r, int i) {
-      if (r >= strips) return;
+      if (r >= nd) return;
       char* const strip = to + r * step;
       const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(strip) >> 1) & 1, e = 2 * i - skew;
       const unsigned char* const s = tile + r * C::kPitch + 4 * i;  // the word that holds element 2i
-      if (e >= 0 && e + 1 < len) {
+      if (e >= 0 && e + 1 < nt) {
         uint32_t u = *reinterpret_cast<const uint32_t*>(s);
         if (skew) u = __funnelshift_r(*reinterpret_cast<const uint32_t*>(s - 4), u, 16);
         *reinterpret_cast<uint32_t*>(strip + 2 * e) = u;
       } else {
         const unsigned char* const f = s - 2 * skew;
-        if (e >= 0 && e < len) *reinterpret_cast<uint16_t*>(strip + 2 * e) = *reinterpret_cast<const uint16_t*>(f);
-        if (e + 1 >= 0 && e + 1 < len) *reinterpret_cast<uint16_t*>(strip + 2 * e + 2) = *reinterpret_cast<const uint16_t*>(f + 2);
+        if (e >= 0 && e < nt) *reinterpret_cast<uint16_t*>(strip + 2 * e) = *reinterpret_cast<const uint16_t*>(f);
+        if (e + 1 >= 0 && e + 1 < nt) *reinterpret_cast<uint16_t*>(strip + 2 * e + 2) = *reinterpret_cast<const uint16_t*>(f + 2);
       }
     };
 #pragma unroll
@@ -357,6 +365,31 @@ __device__ __forceinline__ void store_tile(const unsigned char* tile, const Stri
       const int ch = C::kRows ? i / kRecChunk : i % C::kChannels, p = C::kRows ? i % kRecChunk : i / C::kChannels;
       if (ch < nd && p < nt) dst[ch * t.s1 + p * t.s2] = *reinterpret_cast<const T*>(tile + C::at(ch, p));
     }
+  }
+}
+
+// kPackets, channel-last: stores a warp's 8 positions (from tw on, `left` of them in the sequence)
+// straight from registers, as 2-byte halves; `nch`: the lane's channels that there are.
+// `clear`: positions that get zeros.
+template <typename T>
+__device__ __forceinline__ void store_halves(const Strip<T>& t, int64_t tw, int lane, int nch, int left, unsigned clear, const Lane<2> (&f)[kRecSteps]) {
+  char* p = reinterpret_cast<char*>(t.row + tw * t.s2 + lane * 2);
+  const int64_t step = t.s2 * static_cast<int64_t>(sizeof(T));
+  const bool whole = left >= kRecSteps && nch >= 2 && !clear;
+#pragma unroll
+  for (int j = 0; j < kRecSteps; ++j) {
+    float2 v[1] = {f[j].v};
+    const Packet<T, 2> r = pack2<T, 2>(v);
+    uint32_t u = *reinterpret_cast<const uint32_t*>(&r);
+    if (whole) {
+      *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(u);
+      *reinterpret_cast<uint16_t*>(p + 2) = static_cast<uint16_t>(u >> 16);
+    } else if (j < left) {
+      if (clear >> j & 1u) u = 0;
+      if (nch > 0) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(u);
+      if (nch > 1) *reinterpret_cast<uint16_t*>(p + 2) = static_cast<uint16_t>(u >> 16);
+    }
+    p += step;
   }
 }
 
