@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
   copy_ahead(1);
   cp_async_wait<0>();
   __syncthreads();
-  L bias_sum = splat(0.f, L{});
+  L bias_sum = splat(0.f, L{}), bias_lost = bias_sum;
 
   int slot = 0;
   unsigned parity = 0;
@@ -688,7 +688,6 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
       gy[j] = mul(dh, gc[j]);
       s = mul(ga[j], dh);
       prev[j] = mul(mul(s, gc[j]), sub(prev[j], x[j]));
-      bias_sum = add(bias_sum, prev[j]);
     };
     if (SEQ && (e.first | e.last)) {
 #pragma unroll
@@ -704,6 +703,14 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
       for (int j = kRecSteps - 1; j >= 0; --j) step_back(j);
     }
     if (!CLUSTER && w == 0) common.handed[buf ^ 1][lane] = s;
+    // dbias, with the sum's own rounding carried along (Kahan): thousands of rounds add up
+    L round_sum = prev[0];
+#pragma unroll
+    for (int j = 1; j < kRecSteps; ++j) round_sum = add(round_sum, prev[j]);
+    round_sum = sub(round_sum, bias_lost);
+    const L new_sum = add(bias_sum, round_sum);
+    bias_lost = sub(sub(new_sum, bias_sum), round_sum);
+    bias_sum = new_sum;
     if constexpr (kDirect) {
       const int left = within(tw, a.seqlen, kRecSteps), n = p.nd - 2 * lane;
       const unsigned clear = SEQ ? ~valid & 0xffu : 0u;
