@@ -331,6 +331,7 @@ def fwd_varlen_states(x, weight, bias, seq_idx, cu_seqlens, states, out, silu: b
 RECURRENCE_CHUNK = 32  # CC1D_RECURRENCE_CHUNK
 _NONE = (0, 0, 0, 0, 0)
 _PAD = ((0, 0, 0), (0, 0), (0,), ())
+_NO_GRADIENTS = _NONE * 6 + (0,)  # the recurrence's dout .. dinitial_states and dbias
 RECURRENCE_PARAMS = struct.Struct("<78q")
 RECURRENCE_UPDATE_PARAMS = struct.Struct("<39q")
 ADD_NORM_PARAMS = struct.Struct("<55q2d")
@@ -395,17 +396,40 @@ def _recurrence_states(batch, seq_idx, states) -> int:
 
 
 def recurrence_fwd(x, gate, z, bias, seq_idx, initial_states, final_states, checkpoints, out) -> None:
-    _expect_dims("x", x, 3)
     shape = x.shape
+    if len(shape) != 3:
+        _expect_dims("x", x, 3)
     B, D, L = shape
+    dev = x.get_device()
+    # absent tensors cost nothing here; `same` stays true while all are on x's device
+    same = dev >= 0 and gate.get_device() == dev and out.get_device() == dev
+    if gate.shape != shape or out.shape != shape:
+        _expect("gate", gate, shape)
+        _expect("out", out, shape)
+    if z is not None:
+        _expect("z", z, shape)
+        same = same and z.get_device() == dev
+    if bias is not None:
+        _expect("gate_bias", bias, (D,))
+        same = same and bias.get_device() == dev
+    if seq_idx is not None:
+        _expect("seq_idx", seq_idx, (B, L))
+        same = same and seq_idx.get_device() == dev
     n = _recurrence_states(B, seq_idx, (initial_states, final_states))
-    dev = _check_all((("x", x, shape), ("gate", gate, shape), ("z", z, shape), ("gate_bias", bias, (D,)),
-                      ("seq_idx", seq_idx, (B, L)), ("initial_states", initial_states, (n, D)),
-                      ("final_states", final_states, (n, D)), ("out", out, shape),
-                      ("checkpoints", checkpoints, (B, -(-L // RECURRENCE_CHUNK), D))))
+    if initial_states is not None:
+        _expect("initial_states", initial_states, (n, D))
+        same = same and initial_states.get_device() == dev
+    if final_states is not None:
+        _expect("final_states", final_states, (n, D))
+        same = same and final_states.get_device() == dev
+    if checkpoints is not None:
+        _expect("checkpoints", checkpoints, (B, -(-L // RECURRENCE_CHUNK), D))
+        same = same and checkpoints.get_device() == dev
+    if not same:
+        _device_of(x, gate, z, bias, seq_idx, initial_states, final_states, checkpoints, out)
     p = RECURRENCE_PARAMS.pack(
         B, D, L, n, *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(seq_idx), *_words(initial_states),
-        *_words(final_states), *_words(out), *_NONE * 6, 0, 0 if checkpoints is None else checkpoints.data_ptr(), 0, 0)
+        *_words(final_states), *_words(out), *_NO_GRADIENTS, 0 if checkpoints is None else checkpoints.data_ptr(), 0, 0)
     lib = _lib or load_library()
     with _DeviceStream(dev) as stream:
         status = lib.cc1d_recurrence_fwd_launch(p, stream)

@@ -24,16 +24,22 @@ def _laid_out(x, *others):
     if s[1] != 1 and s[2] != 1:
         x = x.contiguous()
         s = x.stride()
-    return x, *(t if t is None or t.stride() == s or t.dim() != 3 else _like_layout(t, x) for t in others)
+    laid = [x]
+    for t in others:
+        if t is not None and t.stride() != s and t.dim() == 3:
+            t = _like_layout(t, x)
+        laid.append(t)
+    return laid
 
 
 def gated_recurrence_fwd_function(x, gate, z, gate_bias, seq_idx, initial_states, return_final_states,
                                   num_sequences, save_checkpoints):
     """One forward pass.  Returns (out, final_states or None, checkpoints or None)."""
-    if x.dim() != 3:
-        raise ValueError(f"x must have 3 dimensions, got shape {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) != 3:
+        raise ValueError(f"x must have 3 dimensions, got shape {tuple(shape)}")
     x, gate, z = _laid_out(x, gate, z)
-    batch, dim, seqlen = x.shape
+    batch, dim, seqlen = shape
     final = None
     if return_final_states:
         if seq_idx is None:

@@ -15,6 +15,15 @@ them.
 * ``update(x, conv_state, weight, bias, silu, cache_seqlens, conv_state_indices) -> out``
 * ``varlen_states(x, cu_seqlens, state_len) -> states``
 * ``fwd_varlen_states(x, weight, bias, seq_idx, cu_seqlens, state_len, silu) -> (out, states)``
+* ``gated_recurrence_fwd(x, gate, z, gate_bias, seq_idx, initial_states, return_final_states,
+  num_sequences, save_checkpoints) -> (out, final_states, checkpoints)``, empty where not asked for
+* ``gated_recurrence_bwd(x, gate, z, gate_bias, seq_idx, initial_states, checkpoints, dout,
+  dfinal_states, return_dbias, return_dinitial_states) -> (dx, dgate, dz, dbias, dinitial_states)``
+* ``gated_recurrence_update(x, state, gate, z, gate_bias, state_indices) -> out``
+* ``dropout_add_rms_norm_fwd(x, weight, residual, eps, dropout_p, rng_state, residual_in_fp32)
+  -> (out, residual_out)``
+* ``dropout_add_rms_norm_bwd(x_dtype, residual_out, weight, dout, dresidual_out, eps, dropout_p,
+  rng_state) -> (dx, dresidual, dweight)``
 
 The reference compiles its kernels with the CuTe DSL and registers no torch operators;
 these registrations are this package's equivalent of the C++ extension's op table.
@@ -25,7 +34,10 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
+from causal_conv1d import _abi
+from causal_conv1d import add_norm as _an
 from causal_conv1d import cpp_functions as _cf
+from causal_conv1d import gated_recurrence as _gr
 from causal_conv1d.causal_conv1d_varlen import causal_conv1d_fn_varlen_states as _fwd_varlen_states
 from causal_conv1d.causal_conv1d_varlen import causal_conv1d_varlen_states as _varlen_states
 
@@ -102,3 +114,92 @@ def _(x, weight, bias, seq_idx, cu_seqlens, state_len, silu):
     nseq = cu_seqlens.shape[0] - 1
     out = torch.empty_like(x) if (x.stride(2) == 1 or x.stride(1) == 1) else torch.empty_like(x.contiguous())
     return out, x.new_empty(nseq, state_len, x.shape[1]).transpose(1, 2)
+
+
+# -------------------------------------------------------- recurrent-block operators
+def _laid_out_like(x):
+    """An empty tensor with the layout that the recurrence gives its results."""
+    return torch.empty_like(x) if (x.stride(2) == 1 or x.stride(1) == 1) else torch.empty_like(x.contiguous())
+
+
+@torch.library.custom_op("causal_conv1d::gated_recurrence_fwd", mutates_args=())
+def gated_recurrence_fwd(x: Tensor, gate: Tensor, z: Tensor | None, gate_bias: Tensor | None, seq_idx: Tensor | None,
+                         initial_states: Tensor | None, return_final_states: bool, num_sequences: int,
+                         save_checkpoints: bool) -> tuple[Tensor, Tensor, Tensor]:
+    out, final, checkpoints = _gr.gated_recurrence_fwd_function(
+        x, gate, z, gate_bias, seq_idx, initial_states, return_final_states, num_sequences, save_checkpoints)
+    empty = x.new_empty(_EMPTY, dtype=torch.float32)
+    return out, empty if final is None else final, empty.clone() if checkpoints is None else checkpoints
+
+
+@gated_recurrence_fwd.register_fake
+def _(x, gate, z, gate_bias, seq_idx, initial_states, return_final_states, num_sequences, save_checkpoints):
+    batch, dim, seqlen = x.shape
+    n = batch if seq_idx is None else initial_states.shape[0] if initial_states is not None else num_sequences
+    final = x.new_empty((n, dim) if return_final_states else _EMPTY, dtype=torch.float32)
+    chunks = -(-seqlen // _abi.RECURRENCE_CHUNK)
+    return _laid_out_like(x), final, x.new_empty((batch, chunks, dim) if save_checkpoints else _EMPTY, dtype=torch.float32)
+
+
+@torch.library.custom_op("causal_conv1d::gated_recurrence_bwd", mutates_args=())
+def gated_recurrence_bwd(x: Tensor, gate: Tensor, z: Tensor | None, gate_bias: Tensor | None, seq_idx: Tensor | None,
+                         initial_states: Tensor | None, checkpoints: Tensor, dout: Tensor,
+                         dfinal_states: Tensor | None, return_dbias: bool,
+                         return_dinitial_states: bool) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    dx, dgate, dz, dbias, dinitial = _gr.gated_recurrence_bwd_function(
+        x, gate, z, gate_bias, seq_idx, initial_states, checkpoints, dout, dfinal_states, return_dbias,
+        return_dinitial_states)
+    if dz is None:
+        dz = x.new_empty(_EMPTY)
+    if dbias is None:
+        dbias = x.new_empty(_EMPTY, dtype=torch.float32)
+    if dinitial is None:
+        dinitial = x.new_empty(_EMPTY, dtype=torch.float32)
+    return dx, dgate, dz, dbias, dinitial
+
+
+@gated_recurrence_bwd.register_fake
+def _(x, gate, z, gate_bias, seq_idx, initial_states, checkpoints, dout, dfinal_states, return_dbias,
+      return_dinitial_states):
+    dz = _laid_out_like(x) if z is not None else x.new_empty(_EMPTY)
+    dbias = gate_bias.new_empty(x.shape[1]) if return_dbias else x.new_empty(_EMPTY, dtype=torch.float32)
+    dinitial = x.new_empty(initial_states.shape if return_dinitial_states else _EMPTY, dtype=torch.float32)
+    return _laid_out_like(x), _laid_out_like(x), dz, dbias, dinitial
+
+
+@torch.library.custom_op("causal_conv1d::gated_recurrence_update", mutates_args=("state",))
+def gated_recurrence_update(x: Tensor, state: Tensor, gate: Tensor, z: Tensor | None, gate_bias: Tensor | None,
+                            state_indices: Tensor | None) -> Tensor:
+    return _gr.gated_recurrence_update(x, state, gate, z, gate_bias, state_indices)
+
+
+@gated_recurrence_update.register_fake
+def _(x, state, gate, z, gate_bias, state_indices):
+    return torch.empty_like(x)
+
+
+@torch.library.custom_op("causal_conv1d::dropout_add_rms_norm_fwd", mutates_args=())
+def dropout_add_rms_norm_fwd(x: Tensor, weight: Tensor, residual: Tensor | None, eps: float, dropout_p: float,
+                             rng_state: Tensor | None, residual_in_fp32: bool) -> tuple[Tensor, Tensor]:
+    return _an.dropout_add_rms_norm_fwd_function(x, weight, residual, eps, dropout_p, rng_state, residual_in_fp32)
+
+
+@dropout_add_rms_norm_fwd.register_fake
+def _(x, weight, residual, eps, dropout_p, rng_state, residual_in_fp32):
+    dtype = residual.dtype if residual is not None else torch.float32 if residual_in_fp32 else x.dtype
+    return x.new_empty(x.shape), x.new_empty(x.shape, dtype=dtype)
+
+
+@torch.library.custom_op("causal_conv1d::dropout_add_rms_norm_bwd", mutates_args=())
+def dropout_add_rms_norm_bwd(x_dtype: torch.dtype, residual_out: Tensor, weight: Tensor, dout: Tensor | None,
+                             dresidual_out: Tensor | None, eps: float, dropout_p: float,
+                             rng_state: Tensor | None) -> tuple[Tensor, Tensor, Tensor]:
+    dx, dresidual, dweight = _an.dropout_add_rms_norm_bwd_function(
+        x_dtype, residual_out, weight, dout, dresidual_out, eps, dropout_p, rng_state, True, True, True)
+    return dx, dresidual.clone() if dresidual is dx else dresidual, dweight  # an operator's results may not alias
+
+
+@dropout_add_rms_norm_bwd.register_fake
+def _(x_dtype, residual_out, weight, dout, dresidual_out, eps, dropout_p, rng_state):
+    return (residual_out.new_empty(residual_out.shape, dtype=x_dtype), residual_out.new_empty(residual_out.shape),
+            weight.new_empty(weight.shape))

@@ -255,3 +255,24 @@ def test_params_layout(tmp_path):
     assert five == 40
     assert got == [_abi.RECURRENCE_PARAMS.size, _abi.RECURRENCE_UPDATE_PARAMS.size, _abi.ADD_NORM_PARAMS.size,
                    _abi.RECURRENCE_CHUNK, 32, 32 + 14 * five, 32 + 6 * five, _abi.ADD_NORM_PARAMS.size - 16]
+
+
+def test_torch_ops_registered_with_fake_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    ops = torch.ops.causal_conv1d
+    with FakeTensorMode():
+        x = torch.empty(2, 70, 64, dtype=torch.bfloat16).transpose(1, 2)
+        bias, init = torch.empty(64), torch.empty(2, 64)
+        out, final, ck = ops.gated_recurrence_fwd(x, x, x, bias, None, init, True, 0, True)
+        assert out.stride() == x.stride() and final.shape == (2, 64) and ck.shape == (2, 3, 64)
+        seq = torch.empty(2, 70, dtype=torch.int32)
+        assert ops.gated_recurrence_fwd(x, x, None, None, seq, None, True, 5, False)[1].shape == (5, 64)
+        dx, dg, dz, db, di = ops.gated_recurrence_bwd(x, x, None, bias, None, init, ck, x, final, True, True)
+        assert dx.stride() == x.stride() and dz.numel() == 0 and db.shape == (64,) and di.shape == (2, 64)
+        assert ops.gated_recurrence_update(x[..., 0], init, x[..., 0], None, None, None).shape == (2, 64)
+        m, w = torch.empty(3, 64, dtype=torch.float16), torch.empty(64)
+        out, res = ops.dropout_add_rms_norm_fwd(m, w, None, 1e-5, 0.0, None, True)
+        assert out.dtype == torch.float16 and res.dtype == torch.float32
+        dx, dres, dw = ops.dropout_add_rms_norm_bwd(torch.float16, res, w, out, res, 1e-5, 0.0, None)
+        assert dx.dtype == torch.float16 and dres.dtype == torch.float32 and dw.shape == (64,)
