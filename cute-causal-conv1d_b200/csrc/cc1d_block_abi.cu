@@ -2,6 +2,7 @@
 // update, and dropout + residual add + RMSNorm.  Argument checks happen here, before any
 // launch; include/causal_conv1d_b200.h states the contract.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -76,31 +77,55 @@ int sm_count() {
   return n;
 }
 
+// How many clusters of a.cluster CTAs (CTAs for 1) of this recurrence's kernel run at a time: the
+// driver's answer, asked once per kernel, size and device.
+int64_t clusters_at_a_time(RecArgs a, bool bwd) {
+  static std::atomic<int> known[64][2][3][3][2][2][2][17];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  const int dt = a.x.dtype;
+  std::atomic<int>& slot = known[dev][bwd][dt][a.move][a.rows][a.seq_idx.data != nullptr][a.z.data != nullptr][a.cluster];
+  int n = slot.load(std::memory_order_relaxed);
+  if (n == 0) {
+    int64_t count = 0;
+    a.capacity = &count;
+    const cudaError_t e = bwd ? by_type(dt, a, nullptr, rec_bwd_f32, rec_bwd_f16, rec_bwd_bf16) : by_type(dt, a, nullptr, rec_fwd_f32, rec_fwd_f16, rec_fwd_bf16);
+    if (e != cudaSuccess) cudaGetLastError();
+    n = e == cudaSuccess && count > 0 ? static_cast<int>(count) : -1;
+    slot.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 // CTAs that share a tile.  Each takes 1/cluster of the chunks, so a long sequence of few
-// channels fills the GPU, but the cluster's exchange lengthens every chunk.  Measured on a
-// B200, with n CTAs on an SM, a chunk takes base + n * more microseconds:
+// channels fills the GPU, but the cluster's exchange lengthens every chunk, and clusters that
+// do not all run at once take a second wave.  Measured on a B200 with n CTAs on an SM, a chunk
+// takes (microseconds, 16-bit, with z)
 //
-//   cluster           1            2            4            8            16
-//   forward    .75 + .21n  1.15 + .15n  1.30 + .13n  1.30 + .22n  1.30 + .45n
-//   backward   .75 + .52n  1.40 + .25n  1.60 + .28n  1.75 + .37n  1.75 + .65n
+//   forward  .75 + .21 n alone, .74 + .045 cluster + .34 n      backward  .75 + .52 n,
+//   .95 + .08 cluster + .42 n
 //
-// and a CTA about 6 microseconds to start.  As many fit an SM as their shared memory allows
-// (`smem`, and 1 KB for each CTA of the cluster), at most 4 (registers).  The estimate picks
-// the fastest: 256 tiles of 64 chunks run alone, 64 tiles of 256 chunks in clusters of 4
-// (forward 244 us alone, 100 in fours, 113 in eights).
-int choose_cluster(int64_t tiles, int64_t chunks, int64_t smem, bool bwd) {
-  static const double kBase[2][5] = {{.75, 1.15, 1.30, 1.30, 1.30}, {.75, 1.40, 1.60, 1.75, 1.75}};
-  static const double kMore[2][5] = {{.21, .15, .13, .22, .45}, {.52, .25, .28, .37, .65}};
-  const int64_t sms = sm_count();
+// and a CTA about 6 to start.  One sequence of 32768 positions and 5120 channels (80 tiles):
+// forward 949 us alone, 664 in twos, 418 in fours, 350 in fives, 409 in eights; backward 490 us
+// in fives, 589 in fours, 671 in sixes.
+int choose_cluster(RecArgs* a, int64_t tiles, bool bwd) {
+  const double sms = sm_count();
   double best = 0;
   int pick = 1;
-  for (int i = 0, c = 1; c <= 16 && (c == 1 || c <= chunks); ++i, c *= 2) {
-    const int64_t bytes = smem + (c > 1 ? c * 1024 : 0) + 1024;
-    const int64_t fit = std::max<int64_t>(1, std::min<int64_t>(4, 228 * 1024 / bytes)), slots = fit * sms;
-    const int64_t ctas = tiles * c, rest = ctas % slots;
-    const double rounds = static_cast<double>((chunks + c - 1) / c);
-    auto wave = [&](int64_t n) { return 6.0 + rounds * (kBase[bwd][i] + kMore[bwd][i] * static_cast<double>(n)); };
-    const double cost = static_cast<double>(ctas / slots) * wave(fit) + (rest ? wave((rest + sms - 1) / sms) : 0.0);
+  for (int c = 1; c <= 16 && (c == 1 || c <= a->nchunks); c += c < 8 ? 1 : 8) {
+    a->cluster = c;
+    const int64_t fit = clusters_at_a_time(*a, bwd);
+    if (fit <= 0) {
+      if (c == 1) return 1;
+      continue;
+    }
+    const double rounds = static_cast<double>((a->nchunks + c - 1) / c);
+    auto wave = [&](int64_t clusters) {
+      const double n = std::max(1.0, static_cast<double>(clusters * c) / sms);
+      const double t = c == 1 ? .75 + (bwd ? .52 : .21) * n : bwd ? .95 + .08 * c + .42 * n : .74 + .045 * c + .34 * n;
+      return 6.0 + rounds * t;
+    };
+    const double cost = static_cast<double>(tiles / fit) * wave(fit) + (tiles % fit ? wave(tiles % fit) : 0.0);
     if (c == 1 || cost < best) {
       best = cost;
       pick = c;
@@ -131,8 +156,7 @@ cc1d_status rec_plan(RecArgs* a, bool bwd) {
   const int64_t channels = a->x.dtype == CC1D_FLOAT32 ? 32 : 64;
   a->dtiles = (a->dim + channels - 1) / channels;
   const int64_t tiles = a->batch * a->dtiles;
-  const int64_t tile = 4096 + (a->move == kPackets ? (a->rows ? 1024 : 512) : 0), z = a->z.data ? 1 : 0;
-  a->cluster = choose_cluster(tiles, a->nchunks, bwd ? 3 * (3 + z) * tile + 8064 : (a->move == kPackets && !a->rows ? 3 : 4) * (2 + z) * tile + 6016, bwd);
+  a->cluster = choose_cluster(a, tiles, bwd);
   if (tiles * a->cluster > kMax31) return fail(CC1D_ERR_VALUE, "batch * dim is too large");
   return CC1D_OK;
 }

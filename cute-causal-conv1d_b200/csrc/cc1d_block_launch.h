@@ -20,6 +20,7 @@ struct RecArgs {
   int64_t dtiles;
   int cluster, move;
   bool rows;
+  int64_t* capacity = nullptr;  // if set nothing is launched: how many clusters run at a time
 };
 
 // How the recurrence's tensors move (RecArgs::move).  kTma: the TMA copies whole tiles both

@@ -30,8 +30,9 @@ namespace {
 
 // Ring slots: the chunk in work, the one before, whose results are still being stored from its
 // tiles, and one (backward) or two chunks that are being loaded.
-// (strips off their alignment have larger tiles, and channel-last none that are stored from).
-template <bool SKEW, int LAYOUT> constexpr int kFwdStages = SKEW && LAYOUT != kLayoutRows ? 3 : 4;
+// (strips off their alignment have larger tiles, and channel-last none that are stored from; a
+// cluster's rounds are longer, and one chunk ahead leaves room for a fourth CTA).
+template <bool SKEW, int LAYOUT, bool CLUSTER> constexpr int kFwdStages = CLUSTER || (SKEW && LAYOUT != kLayoutRows) ? 3 : 4;
 constexpr int kBwdStages = 3, kMostStages = 4;
 
 // s = 1 / (1 + exp(-v)) at a warp's 8 positions, and e = exp(-v) if wanted.  For 16-bit tensors
@@ -212,13 +213,14 @@ __device__ __forceinline__ Lane<V> from_cluster(const Map<V>* far, unsigned bar,
   Lane<V> h = mbar_wait(bar, parity) ? carry : splat(__int_as_float(0x7fc00000), carry);
   Lane<V> start = h;
   const int mine = FORWARD ? p.rank : p.cluster - 1 - p.rank;  // how many come before this CTA
-  for (int i = 0; i < p.cluster; i += 2) {                     // (a power of two)
+  for (int i = 0; i < p.cluster; i += 2) {
     const int r = FORWARD ? i : p.cluster - 1 - i;
-    const Map<V> m0 = far[r * 32 + lane], m1 = far[(FORWARD ? r + 1 : r - 1) * 32 + lane];
+    const bool two = i + 1 < p.cluster;
+    const Map<V> m0 = far[r * 32 + lane], m1 = far[(two ? FORWARD ? r + 1 : r - 1 : r) * 32 + lane];
     if (i == mine) start = h;
     h = apply<V, SEQ>(m0, h);
     if (i + 1 == mine) start = h;
-    h = apply<V, SEQ>(m1, h);
+    if (two) h = apply<V, SEQ>(m1, h);
   }
   carry = h;
   return start;
@@ -261,7 +263,7 @@ __device__ __forceinline__ void start_barriers(unsigned bars, bool tma) {
 template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z, bool CLUSTER>
 __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
   using C = Tile<T, LAYOUT, SKEW>;
-  constexpr int V = C::V, NT = Z ? 3 : 2, S = kFwdStages<SKEW, LAYOUT>;
+  constexpr int V = C::V, NT = Z ? 3 : 2, S = kFwdStages<SKEW, LAYOUT, CLUSTER>;
   using L = Lane<V>;
   extern __shared__ __align__(1024) unsigned char smem[];
   // ring of tiles (gate, x, z) | sums of the warps [2] | maps of the cluster [2][cluster][32] | common
@@ -784,13 +786,30 @@ bool make_map(CUtensorMap* map, const TensorArg& t, const RecArgs& a) {
                 CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Clusters (CTAs if there are none) of this launch that run at the same time on the device.
+template <bool CLUSTER>
+cudaError_t capacity_of(const void* kernel, const cudaLaunchConfig_t& cfg, int cluster, int64_t* out) {
+  int dev = 0, n = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if constexpr (CLUSTER) {
+    e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+  } else {
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kRecThreads, cfg.dynamicSmemBytes);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    n *= sms;
+  }
+  *out = n;
+  return e;
+}
+
 template <typename T, int LAYOUT, bool SKEW, bool BWD, bool SEQ, bool Z, bool CLUSTER>
 cudaError_t run(RecArgs& a, cudaStream_t s) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int NT = (BWD ? 3 : 2) + (Z ? 1 : 0);
-  constexpr int stages = BWD ? kBwdStages : kFwdStages<SKEW, LAYOUT>;
+  constexpr int stages = BWD ? kBwdStages : kFwdStages<SKEW, LAYOUT, CLUSTER>;
   RecMaps maps = {};
-  if (a.move == kTma) {
+  if (a.move == kTma && !a.capacity) {
     const bool ok = make_map<T, LAYOUT>(&maps.gate, a.gate, a) && make_map<T, LAYOUT>(&maps.x, a.x, a) && make_map<T, LAYOUT>(&maps.z, a.z, a) &&
                     (BWD ? make_map<T, LAYOUT>(&maps.dout, a.dout, a) && make_map<T, LAYOUT>(&maps.dx, a.dx, a) &&
                                make_map<T, LAYOUT>(&maps.dgate, a.dgate, a) && make_map<T, LAYOUT>(&maps.dz, a.dz, a)
@@ -817,6 +836,7 @@ cudaError_t run(RecArgs& a, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = CLUSTER ? 2 : 1;
+  if (a.capacity) return capacity_of<CLUSTER>(ptr, cfg, a.cluster, a.capacity);
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<const RecArgs&>(a), static_cast<const RecMaps&>(maps));
 }
 
@@ -847,6 +867,7 @@ cudaError_t CC1D_DT_NAME(rec_fwd)(RecArgs& a, cudaStream_t s) {
 }
 cudaError_t CC1D_DT_NAME(rec_bwd)(RecArgs& a, cudaStream_t s) {
   cudaError_t e = pick<DT, true>(a, s);
+  if (a.capacity) return e;
   if (e == cudaSuccess && a.dbias) e = sum_rows(a.partials, a.batch * a.cluster, a.dim, a.dbias, s);
   return e;
 }
