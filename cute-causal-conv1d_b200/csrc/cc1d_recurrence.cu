@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
 
     Edges e;
     if constexpr (SEQ) {
-      e = edges_of(lane < kRecSteps + 2 ? common.ids[k % 3][w * kRecSteps + lane] : -1);
+      e = edges_of(common.ids[k % 3][w * kRecSteps + min(lane, kRecSteps + 1)]);
     }
     // Rare: positions without a token pass the state on.  z as well: four positions share a
     // reciprocal, and their roundings must not depend on what padding or old tiles hold (the
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     Edges e;
     unsigned valid = below(within(tw, a.seqlen, kRecSteps));
     if constexpr (SEQ) {
-      e = edges_of(lane < kRecSteps + 2 ? common.ids[k % 3][w * kRecSteps + lane] : -1);
+      e = edges_of(common.ids[k % 3][w * kRecSteps + min(lane, kRecSteps + 1)]);
       valid = e.valid;
     }
     if (valid != 0xffu) {  // rare: positions without a token pass the gradient on

@@ -400,14 +400,16 @@ struct Edges {
   unsigned valid, first, last;
   int id;
 };
-// From the ids of positions t - 1 .. t + 8, in lanes 0 .. 9.
+// From the ids of positions t - 1 .. t + 8, in lanes 0 .. 9 (the others hold what lane 9 does).
+// Mostly one sequence covers them all, which one vote shows.
 __device__ __forceinline__ Edges edges_of(int id) {
   constexpr unsigned all = 0xffffffffu;
-  const int before = __shfl_up_sync(all, id, 1), after = __shfl_down_sync(all, id, 1);
-  Edges e;
-  e.id = id;
+  Edges e = {0xffu, 0u, 0u, id};
+  const int before = __shfl_up_sync(all, id, 1);
+  if (__all_sync(all, id == before && id >= 0)) return e;  // (lane 0 gets its own)
+  const int after = __shfl_down_sync(all, id, 1), lane = threadIdx.x & 31;
   e.valid = (__ballot_sync(all, id >= 0) >> 1) & 0xffu;
-  e.first = (__ballot_sync(all, id >= 0 && id != before) >> 1) & 0xffu;
+  e.first = (__ballot_sync(all, lane > 0 && id >= 0 && id != before) >> 1) & 0xffu;
   e.last = (__ballot_sync(all, id >= 0 && id != after) >> 1) & 0xffu;
   return e;
 }
