@@ -20,37 +20,41 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// exp(-u), at most 1e30.  For 16-bit tensors 2^v by the hardware's approximation (relative
-// error about 2^-22, plus the rounding of u log2(e)); for fp32 the library's exp.
+// exp(-u) for 16-bit tensors: 2^v by the hardware's approximation (relative error about 2^-22,
+// plus the rounding of v = -u log2(e)), at most 1e30.
+//
+// fp32 also takes what that rounding loses: -u log2(e) = t + r, with r from two fused
+// multiply-adds (the second for the part of log2(e) below fp32), and 2^r = 1 + r ln 2 to
+// 2^-40.  u is held within +-85, where sigmoids are 0 and 1 to working precision and neither
+// exp nor 1 / (1 + exp) leaves the normal numbers; a NaN passes.
 template <typename T>
 __device__ __forceinline__ float exp_minus(float u) {
-  if constexpr (std::is_same<T, float>::value) return clamp_exp(expf(-u), 1e30f);
-  else return clamp_exp(ex2_approx(-kLog2e * u), 1e30f);
-}
-template <typename T>
-__device__ __forceinline__ float reciprocal(float v) {
-  if constexpr (std::is_same<T, float>::value) return __frcp_rn(v);
-  else return rcp_approx(v);
+  if constexpr (std::is_same<T, float>::value) {
+    constexpr double kLog2eExact = 1.4426950408889634074;
+    constexpr float kLow = static_cast<float>(kLog2eExact - static_cast<double>(kLog2e));
+    u = clamp_exp(max_nan(u, -85.f), 85.f);
+    const float t = -kLog2e * u;
+    const float r = fmaf(-kLow, u, fmaf(-kLog2e, u, -t));
+    const float e = ex2_approx(t);
+    return fmaf(e, r * 0.693147181f, e);
+  } else {
+    return clamp_exp(ex2_approx(-kLog2e * u), 1e30f);
+  }
 }
 
 // a = sigmoid(u) and c = 1 - a = sigmoid(-u), each to full relative precision.
 template <typename T>
 __device__ __forceinline__ void sigmoid_pair(float u, float& a, float& c) {
   const float e = exp_minus<T>(u);
-  a = reciprocal<T>(1.f + e);
+  a = rcp_approx(1.f + e);
   c = e * a;
 }
 
-// sigmoid(z) alone needs no clamp: 1 / (1 + inf) is 0.
-template <typename T>
-__device__ __forceinline__ float sigmoid_of(float z) {
-  if constexpr (std::is_same<T, float>::value) return __frcp_rn(1.f + expf(-z));
-  else return rcp_approx(1.f + ex2_approx(-kLog2e * z));
-}
 template <typename T>
 __device__ __forceinline__ float silu_of(float z) {
-  return z * sigmoid_of<T>(z);
+  return z * rcp_approx(1.f + exp_minus<T>(z));
 }
+
 // ---------------------------------------------------------------------- Philox4x32-10
 // Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3" (2011):
 // four 32-bit words for a 128-bit counter under a 64-bit key.

@@ -51,9 +51,9 @@ __device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const La
     for (int j = 0; j < kRecSteps; ++j) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float x = clamp_exp(expf(-(el(v[j], i) + el(n, i))), 1e30f);
+        const float x = exp_minus<float>(el(v[j], i) + el(n, i));
         if constexpr (E) el(e[j], i) = x;
-        el(s[j], i) = __frcp_rn(1.f + x);
+        el(s[j], i) = rcp_approx(1.f + x);
       }
     }
   } else {

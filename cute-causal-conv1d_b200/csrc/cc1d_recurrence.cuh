@@ -74,19 +74,25 @@ __device__ __forceinline__ void mbar_arrive(unsigned bar) {
 __device__ __forceinline__ void mbar_arrive_copies(unsigned bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
 }
-// Waits for the phase of that parity, at most 2^20 tries of the hardware's own waiting time;
-// returns whether it came.  What is waited for was issued by this CTA or by CTAs of its
-// cluster, which run at the same time, so it does come.
+// Waits for the phase of that parity, about two seconds at most (the clock is looked at every
+// 65536 tries); returns whether it came.  What is waited for was issued by this CTA or by CTAs
+// of its cluster, which run at the same time, so it does come.
 __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
-  for (int i = 0; i < (1 << 20); ++i) {
+  uint64_t begin = 0;
+  for (unsigned i = 1;; ++i) {
     unsigned done;
     asm volatile(
         "{\n.reg .pred p;\n"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         "selp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     if (done) return true;
+    if ((i & 0xffffu) == 0) {
+      uint64_t now;
+      asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(now));
+      if (begin == 0) begin = now;
+      else if (now - begin > 2000000000ull) return false;
+    }
   }
-  return false;
 }
 
 // ----------------------------------------------------------------------------- the tiles
