@@ -279,13 +279,16 @@ template <typename T, typename R, int G, int VPT, int E, bool VEC>
 __global__ void __launch_bounds__(kThreads, bwd_ctas(VPT * E)) add_norm_bwd_kernel(const AddNormArgs a) {
   extern __shared__ float shares[];  // G == 32: [warps][columns]
   __shared__ float scratch[2][2][kThreads / 32];
+  // dresidual_out, which the sums do not need, is loaded with its own row where two rows of
+  // fp32 of it would not fit the registers
+  constexpr bool kAhead = sizeof(R) == 2;
   const int g = threadIdx.x % G;
   const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / G);
   int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
   grid_dependency_wait();
   const uint64_t key = a.rng ? static_cast<uint64_t>(a.rng[0]) : 0, stream = a.rng ? static_cast<uint64_t>(a.rng[a.rng_stride]) : 0;
   const float inv = 1.f / static_cast<float>(a.dim);
-  Cols<R, E> r[VPT], dres[VPT];
+  Cols<R, E> r[VPT], dres[kAhead ? VPT : 1];
   Cols<T, E> dy[VPT];
   auto load = [&](int64_t at) {
     if (at >= a.rows) return;
@@ -295,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, bwd_ctas(VPT * E)) add_norm_bwd_kern
       const int n = cols_left(a.dim, c);
       load_cols<R, E, VEC>(row_of<R>(a.residual_out, at) + c, n, r[v]);
       load_cols<T, E, VEC>(row_of<T>(a.dout, at) + c, a.dout.data ? n : 0, dy[v]);
-      load_cols<R, E, VEC>(row_of<R>(a.dresidual_out, at) + c, a.dresidual_out.data ? n : 0, dres[v]);
+      if constexpr (kAhead) load_cols<R, E, VEC>(row_of<R>(a.dresidual_out, at) + c, a.dresidual_out.data ? n : 0, dres[v]);
     }
   };
   load(row);
@@ -311,12 +314,19 @@ __global__ void __launch_bounds__(kThreads, bwd_ctas(VPT * E)) add_norm_bwd_kern
     float sum[2] = {0.f, 0.f};  // of r^2 and of q r
     Cols<R, E> rn[VPT], dresn[VPT];
     Cols<T, E> dyn[VPT];
+    if constexpr (!kAhead) {
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) {
+        const int64_t c = static_cast<int64_t>(v * G + g) * E;
+        load_cols<R, E, VEC>(row_of<R>(a.dresidual_out, row) + c, a.dresidual_out.data ? cols_left(a.dim, c) : 0, dresn[v]);
+      }
+    }
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       float rf[E], df[E];
       widen<R, E>(rn[v] = r[v], rf);
       widen<T, E>(dyn[v] = dy[v], df);
-      dresn[v] = dres[v];
+      if constexpr (kAhead) dresn[v] = dres[v];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         sum[0] = fmaf(rf[i], rf[i], sum[0]);

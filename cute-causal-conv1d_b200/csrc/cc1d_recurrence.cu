@@ -783,7 +783,7 @@ bool make_map(CUtensorMap* map, const TensorArg& t, const RecArgs& a) {
   const cuuint32_t one[3] = {1, 1, 1};
   return encode(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, t.data, dims, strides, box, one,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, !C::kRows ? CU_TENSOR_MAP_SWIZZLE_NONE : C::kStripBytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Clusters (CTAs if there are none) of this launch that run at the same time on the device.
