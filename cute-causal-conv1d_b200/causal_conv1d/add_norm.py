@@ -10,6 +10,7 @@ The dropout mask ``keep`` is a function of a generator state and the place alone
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from causal_conv1d import _abi
 
@@ -79,6 +80,7 @@ class DropoutAddRMSNormFn(torch.autograd.Function):
         return out, residual_out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, dresidual_out):
         if dout is None and dresidual_out is None:
             return (None,) * 7

@@ -13,6 +13,7 @@ carry h in fp32, and round once, on the stores.  States are fp32.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from causal_conv1d import _abi
 from causal_conv1d.cpp_functions import _like_layout
@@ -101,6 +102,7 @@ class GatedRecurrenceFn(torch.autograd.Function):
         return (out, final) if return_final_states else out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, dfinal_states=None):
         x, gate, z, gate_bias, seq_idx, initial_states, checkpoints = ctx.saved_tensors
         if dout is None and dfinal_states is None:

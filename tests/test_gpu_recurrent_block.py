@@ -85,3 +85,15 @@ def test_opcheck():
     m, w, rng = x[0].t().contiguous(), torch.ones(64, device="cuda"), torch.tensor([1, 2], device="cuda")
     torch.library.opcheck(ops.dropout_add_rms_norm_fwd, (m, w, m, 1e-5, 0.2, rng, False))
     torch.library.opcheck(ops.dropout_add_rms_norm_bwd, (m.dtype, m, w, m, m, 1e-5, 0.2, rng))
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(1, 8, 20, device="cuda", requires_grad=True)
+    out = causal_conv1d.gated_recurrence_fn(x, x)
+    (g,) = torch.autograd.grad(out.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(g.sum(), x)
+    m = torch.randn(3, 16, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(causal_conv1d.dropout_add_rms_norm_fn(m, torch.ones(16, device="cuda"))[0].sum(), m, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(g.sum(), m)
