@@ -8,6 +8,7 @@ missing or a tensor is not on a CUDA device, the call raises.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 import struct
 import threading
@@ -88,7 +89,7 @@ SIGNATURES = {
     "cc1d_update_launch": (c_i32, [ctypes.POINTER(UpdateParams), c_void_p]),
     "cc1d_varlen_states_launch": (c_i32, [ctypes.POINTER(VarlenParams), c_void_p]),
     "cc1d_fwd_varlen_states_launch": (c_i32, [ctypes.POINTER(FwdVarlenStatesParams), c_void_p]),
-    # the params of these are packed as flat 64-bit words (_words)
+    # the params of these are flat 64-bit words (RECURRENCE_PARAMS and the others below)
     "cc1d_recurrence_fwd_launch": (c_i32, [c_void_p, c_void_p]),
     "cc1d_recurrence_bwd_workspace_bytes": (c_i64, [c_void_p]),
     "cc1d_recurrence_bwd_launch": (c_i32, [c_void_p, c_void_p]),
@@ -324,203 +325,33 @@ def fwd_varlen_states(x, weight, bias, seq_idx, cu_seqlens, states, out, silu: b
 
 
 # ------------------------------------------------- recurrent-block operators
-# Their params structs are made of 64-bit words only (a cc1d_tensor is five: data, dtype
-# with the reserved half zero, three strides), so one struct.pack fills them, and the
-# checks below are written for few Python operations: a decode step is short enough for the
-# host's time per call to count.
+# Their PyTorch binding is the extension module _block.  Their params structs are made of
+# 64-bit words (a cc1d_tensor is five: data, dtype with the reserved half zero, three
+# strides), so a caller without it fills one with one struct.pack.
+class _Missing:
+    """Stands for the binding where it cannot be loaded: importing the package and the
+    convolution do not need it, and each use of it raises the reason."""
+
+    def __init__(self, reason: ImportError):
+        self._reason = reason
+
+    def __getattr__(self, name):
+        raise ImportError(
+            "causal_conv1d/_block.so cannot be loaded: build it with `python cute-causal-conv1d_b200/cc1d_build.py` "
+            f"against the installed PyTorch. causal_conv1d has no CPU fallback. ({self._reason})"
+        )
+
+
+try:
+    block = importlib.import_module("causal_conv1d._block")
+except ImportError as e:
+    block = _Missing(e)
+
 RECURRENCE_CHUNK = 32  # CC1D_RECURRENCE_CHUNK
-_NONE = (0, 0, 0, 0, 0)
-_PAD = ((0, 0, 0), (0, 0), (0,), ())
-_NO_GRADIENTS = _NONE * 6 + (0,)  # the recurrence's dout .. dinitial_states and dbias
+_NONE = (0, 0, 0, 0, 0)  # an absent tensor
 RECURRENCE_PARAMS = struct.Struct("<78q")
 RECURRENCE_UPDATE_PARAMS = struct.Struct("<39q")
 ADD_NORM_PARAMS = struct.Struct("<55q2d")
-_RECURRENCE_SCRATCH = struct.Struct("<2q")  # the last words: workspace, workspace_bytes
-_ADD_NORM_SCRATCH = struct.Struct("<2q2d")  # ... and eps, dropout_p
-
-
-def _words(t: torch.Tensor | None) -> tuple:
-    if t is None:
-        return _NONE
-    s = t.stride()
-    try:
-        return (t.data_ptr(), _DTYPES[t.dtype], *s, *_PAD[len(s)])
-    except KeyError:
-        raise TypeError(f"unsupported dtype {t.dtype}") from None
-
-
-def _check_all(tensors) -> int:
-    """The device index of (name, tensor, shape) triples after checking the shapes (as
-    ``_expect``) and that all are on one CUDA device.  The first must be there."""
-    dev = tensors[0][1].get_device()
-    same = dev >= 0
-    for name, t, shape in tensors:
-        if t is not None:
-            if t.shape != shape:
-                raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-            same = same and t.get_device() == dev
-    if not same:
-        _device_of(*(t for _, t, _ in tensors))  # raises with the reason
-    return dev
-
-
-class _DeviceStream:
-    """The current stream's handle on device ``index``, which is current meanwhile."""
-
-    __slots__ = ("index", "prev")
-
-    def __init__(self, index: int):
-        self.index = index
-
-    def __enter__(self):
-        self.prev = torch._C._cuda_getDevice()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
-        return False
-
-
-def _recurrence_states(batch, seq_idx, states) -> int:
-    """Rows of the states: the batch's, or with packed sequences as many as the first of
-    them has (0 if there are none)."""
-    if seq_idx is None:
-        return batch
-    for t in states:
-        if t is not None:
-            return t.shape[0]
-    return 0
-
-
-def recurrence_fwd(x, gate, z, bias, seq_idx, initial_states, final_states, checkpoints, out) -> None:
-    shape = x.shape
-    if len(shape) != 3:
-        _expect_dims("x", x, 3)
-    B, D, L = shape
-    dev = x.get_device()
-    # absent tensors cost nothing here; `same` stays true while all are on x's device
-    same = dev >= 0 and gate.get_device() == dev and out.get_device() == dev
-    if gate.shape != shape or out.shape != shape:
-        _expect("gate", gate, shape)
-        _expect("out", out, shape)
-    if z is not None:
-        _expect("z", z, shape)
-        same = same and z.get_device() == dev
-    if bias is not None:
-        _expect("gate_bias", bias, (D,))
-        same = same and bias.get_device() == dev
-    if seq_idx is not None:
-        _expect("seq_idx", seq_idx, (B, L))
-        same = same and seq_idx.get_device() == dev
-    n = _recurrence_states(B, seq_idx, (initial_states, final_states))
-    if initial_states is not None:
-        _expect("initial_states", initial_states, (n, D))
-        same = same and initial_states.get_device() == dev
-    if final_states is not None:
-        _expect("final_states", final_states, (n, D))
-        same = same and final_states.get_device() == dev
-    if checkpoints is not None:
-        _expect("checkpoints", checkpoints, (B, -(-L // RECURRENCE_CHUNK), D))
-        same = same and checkpoints.get_device() == dev
-    if not same:
-        _device_of(x, gate, z, bias, seq_idx, initial_states, final_states, checkpoints, out)
-    p = RECURRENCE_PARAMS.pack(
-        B, D, L, n, *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(seq_idx), *_words(initial_states),
-        *_words(final_states), *_words(out), *_NO_GRADIENTS, 0 if checkpoints is None else checkpoints.data_ptr(), 0, 0)
-    lib = _lib or load_library()
-    with _DeviceStream(dev) as stream:
-        status = lib.cc1d_recurrence_fwd_launch(p, stream)
-        if status:
-            _check(status)
-
-
-def recurrence_bwd(x, gate, z, bias, seq_idx, initial_states, checkpoints, dout, dfinal_states, dx, dgate, dz,
-                   dinitial_states, dbias) -> None:
-    _expect_dims("x", x, 3)
-    shape = x.shape
-    B, D, L = shape
-    n = _recurrence_states(B, seq_idx, (initial_states, dfinal_states, dinitial_states))
-    dev = _check_all((("x", x, shape), ("gate", gate, shape), ("z", z, shape), ("gate_bias", bias, (D,)),
-                      ("seq_idx", seq_idx, (B, L)), ("initial_states", initial_states, (n, D)),
-                      ("dout", dout, shape), ("dfinal_states", dfinal_states, (n, D)), ("dx", dx, shape),
-                      ("dgate", dgate, shape), ("dz", dz, shape), ("dinitial_states", dinitial_states, (n, D)),
-                      ("dbias", dbias, (D,)), ("checkpoints", checkpoints, (B, -(-L // RECURRENCE_CHUNK), D))))
-    p = RECURRENCE_PARAMS.pack(
-        B, D, L, n, *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(seq_idx), *_words(initial_states),
-        *_NONE * 2, *_words(dout), *_words(dfinal_states), *_words(dx), *_words(dgate), *_words(dz),
-        *_words(dinitial_states), 0 if dbias is None else dbias.data_ptr(), checkpoints.data_ptr(), 0, 0)
-    lib = _lib or load_library()
-    with _DeviceStream(dev) as stream:
-        need = lib.cc1d_recurrence_bwd_workspace_bytes(p)
-        if need > 0:
-            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-            p = p[:-16] + _RECURRENCE_SCRATCH.pack(workspace.data_ptr(), need)
-        status = lib.cc1d_recurrence_bwd_launch(p, stream)
-        if status:
-            _check(status)
-
-
-def recurrence_update(x, gate, z, bias, state, state_indices, out) -> None:
-    """x, gate, z, out: (batch, dim) or (batch, dim, tokens)."""
-    shape = x.shape
-    if len(shape) == 2:
-        B, D = shape
-        T = 1
-    else:
-        _expect_dims("x", x, 3)
-        B, D, T = shape
-    _expect_dims("state", state, 2)
-    n = B if state_indices is None else state.shape[0]
-    dev = _check_all((("x", x, shape), ("gate", gate, shape), ("z", z, shape), ("gate_bias", bias, (D,)),
-                      ("state", state, (n, D)), ("state_indices", state_indices, (B,)), ("out", out, shape)))
-    p = RECURRENCE_UPDATE_PARAMS.pack(
-        B, D, T, n, *_words(x), *_words(gate), *_words(z), *_words(bias), *_words(state), *_words(state_indices),
-        *_words(out))
-    lib = _lib or load_library()
-    with _DeviceStream(dev) as stream:
-        status = lib.cc1d_recurrence_update_launch(p, stream)
-        if status:
-            _check(status)
-
-
-def add_norm_fwd(x, residual, weight, rng_state, out, residual_out, eps: float, dropout_p: float) -> None:
-    _expect_dims("x", x, 2)
-    shape = x.shape
-    dev = _check_all((("x", x, shape), ("residual", residual, shape), ("weight", weight, (shape[1],)),
-                      ("rng_state", rng_state, (2,)), ("out", out, shape), ("residual_out", residual_out, shape)))
-    p = ADD_NORM_PARAMS.pack(
-        *shape, *_words(x), *_words(residual), *_words(weight), *_words(rng_state), *_words(out),
-        *_words(residual_out), *_NONE * 4, 0, 0, 0, eps, dropout_p)
-    lib = _lib or load_library()
-    with _DeviceStream(dev) as stream:
-        status = lib.cc1d_add_norm_fwd_launch(p, stream)
-        if status:
-            _check(status)
-
-
-def add_norm_bwd(x_dtype, residual_out, weight, rng_state, dout, dresidual_out, dx, dresidual, dweight,
-                 eps: float, dropout_p: float) -> None:
-    _expect_dims("residual_out", residual_out, 2)
-    shape = residual_out.shape
-    dev = _check_all((("residual_out", residual_out, shape), ("weight", weight, (shape[1],)),
-                      ("rng_state", rng_state, (2,)), ("dout", dout, shape), ("dresidual_out", dresidual_out, shape),
-                      ("dx", dx, shape), ("dresidual", dresidual, shape), ("dweight", dweight, (shape[1],))))
-    p = ADD_NORM_PARAMS.pack(
-        *shape, 0, _DTYPES[x_dtype], 0, 0, 0, *_NONE, *_words(weight), *_words(rng_state), *_NONE,
-        *_words(residual_out), *_words(dout), *_words(dresidual_out), *_words(dx), *_words(dresidual),
-        0 if dweight is None else dweight.data_ptr(), 0, 0, eps, dropout_p)
-    lib = _lib or load_library()
-    with _DeviceStream(dev) as stream:
-        need = lib.cc1d_add_norm_bwd_workspace_bytes(p)
-        if need > 0:
-            workspace = torch.empty(need, dtype=torch.uint8, device=weight.device)
-            p = p[:-32] + _ADD_NORM_SCRATCH.pack(workspace.data_ptr(), need, eps, dropout_p)
-        status = lib.cc1d_add_norm_bwd_launch(p, stream)
-        if status:
-            _check(status)
 
 
 def launch_count() -> int:

@@ -1,11 +1,14 @@
-"""Build libcc1d_b200.so (the C-ABI library of the causal_conv1d B200 kernels).
+"""Build libcc1d_b200.so (the C-ABI library of the causal_conv1d B200 kernels) and _block.so
+(the PyTorch binding of its recurrent-block operators).
 
     python cute-causal-conv1d_b200/cc1d_build.py [--force] [--verbose]
 
 Compiles every kernel file for sm_100a only (``-gencode arch=compute_100a,code=sm_100a``)
 with nvcc, in parallel; the per-element-type kernel files are compiled once per type.
 The library is written next to the Python package (``causal_conv1d/libcc1d_b200.so``),
-in the source tree, and is rebuilt only when a source or header is newer.
+in the source tree, and is rebuilt only when a source or header is newer.  So is the
+binding, which g++ compiles against the headers of the installed PyTorch; the library itself
+needs no PyTorch.
 """
 
 from __future__ import annotations
@@ -22,6 +25,8 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "causal_conv1d", "libcc1d_b200.so")
+# the PyTorch binding of the recurrent-block operators, an extension module on top of LIB
+BINDING = os.path.join(HERE, "causal_conv1d", "_block.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -59,10 +64,40 @@ def _inputs():
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(BINDING):
         return False
-    lib_mtime = os.path.getmtime(LIB)
+    lib_mtime = min(os.path.getmtime(LIB), os.path.getmtime(BINDING))
     return all(os.path.getmtime(f) <= lib_mtime for f in _inputs())
+
+
+def compile_binding(obj: str) -> None:
+    """cc1d_block_torch.cpp -> obj, with the installed PyTorch's headers and C++ ABI."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-c", os.path.join(CSRC, "cc1d_block_torch.cpp"), "-o", obj,
+           "-DTORCH_EXTENSION_NAME=_block", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + INCLUDE, "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_path("include")]
+    cmd += ["-isystem" + d for d in cpp_extension.include_paths()]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for cc1d_block_torch.cpp:\n{res.stdout}\n{res.stderr}")
+
+
+def link_binding(obj: str) -> None:
+    from torch.utils import cpp_extension
+
+    tmp = BINDING + ".tmp"
+    cmd = ["g++", "-shared", "-o", tmp, obj, "-Wl,-rpath,$ORIGIN"]
+    cmd += ["-L" + d for d in (os.path.dirname(LIB), *cpp_extension.library_paths())]
+    cmd += ["-l:" + os.path.basename(LIB), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"link of _block.so failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -82,8 +117,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return res.stderr
 
     workers = max(1, min(len(UNITS), os.cpu_count() or 4))
+    binding_obj = os.path.join(BUILD, "cc1d_block_torch.o")
     with ThreadPoolExecutor(workers) as pool:
+        binding = pool.submit(compile_binding, binding_obj)
         logs = list(pool.map(compile_unit, UNITS))
+        binding.result()
     if verbose:
         for log in logs:
             sys.stderr.write(log)
@@ -94,6 +132,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB)
+    link_binding(binding_obj)
     return LIB
 
 

@@ -276,3 +276,9 @@ def test_torch_ops_registered_with_fake_shapes():
         assert out.dtype == torch.float16 and res.dtype == torch.float32
         dx, dres, dw = ops.dropout_add_rms_norm_bwd(torch.float16, res, w, out, res, 1e-5, 0.0, None)
         assert dx.dtype == torch.float16 and dres.dtype == torch.float32 and dw.shape == (64,)
+
+
+def test_missing_binding_is_named_on_use():
+    missing = _abi._Missing(ImportError("no such file"))
+    with pytest.raises(ImportError, match="cc1d_build.*no such file"):
+        missing.recurrence(None)
