@@ -58,12 +58,12 @@ bool strips_ok(const TensorArg& t, const RecArgs& a) {
   const int64_t unit = a.rows ? t.s2 : t.s1, step = a.rows ? t.s1 : t.s2;
   return (unit == 1 || (a.rows ? a.seqlen : a.dim) == 1) && t.s0 >= 0 && ((a.rows ? a.dim : a.seqlen) <= 1 || step >= 0);
 }
-// Every strip of it starts on a 16-byte boundary.
-bool packets_ok(const TensorArg& t, const RecArgs& a) {
+// Every strip of it starts on a multiple of `bytes`.
+bool strips_start_on(int bytes, const TensorArg& t, const RecArgs& a) {
   if (!t.data) return true;
-  const int64_t n = t.dtype == CC1D_FLOAT32 ? 4 : 8;
+  const int64_t n = bytes / (t.dtype == CC1D_FLOAT32 ? 4 : 2);
   auto step_ok = [&](int64_t s, int64_t extent) { return extent <= 1 || s % n == 0; };
-  return (reinterpret_cast<uintptr_t>(t.data) & 15u) == 0 && step_ok(t.s0, a.batch) &&
+  return reinterpret_cast<uintptr_t>(t.data) % bytes == 0 && step_ok(t.s0, a.batch) &&
          (a.rows ? step_ok(t.s1, a.dim) : step_ok(t.s2, a.seqlen));
 }
 
@@ -80,7 +80,7 @@ int sm_count() {
 // How many clusters of a.cluster CTAs (CTAs for 1) of this recurrence's kernel run at a time: the
 // driver's answer, asked once per kernel, size and device.
 int64_t clusters_at_a_time(RecArgs a, bool bwd) {
-  static std::atomic<int> known[64][2][3][3][2][2][2][17];
+  static std::atomic<int> known[64][2][3][4][2][2][2][17];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   const int dt = a.x.dtype;
@@ -137,8 +137,8 @@ int choose_cluster(RecArgs* a, int64_t tiles, bool bwd) {
 // Layout, way of moving and cluster of a recurrence.  Rows: every tensor has unit stride along
 // the sequence; all others take the channel-last kernel.
 cc1d_status rec_plan(RecArgs* a, bool bwd) {
-  const TensorArg* const all[] = {&a->x, &a->gate, &a->z, bwd ? &a->dout : &a->out, bwd ? &a->dx : nullptr,
-                                  bwd ? &a->dgate : nullptr, bwd ? &a->dz : nullptr};
+  TensorArg* const all[] = {&a->x, &a->gate, &a->z, bwd ? &a->dout : &a->out, bwd ? &a->dx : nullptr,
+                            bwd ? &a->dgate : nullptr, bwd ? &a->dz : nullptr};
   bool last = true, rows = true;
   for (const TensorArg* t : all) {
     if (!t || !t->data) continue;
@@ -146,13 +146,19 @@ cc1d_status rec_plan(RecArgs* a, bool bwd) {
     rows = rows && (t->s2 == 1 || a->seqlen == 1);
   }
   a->rows = rows && (!last || a->dim == 1);
-  bool strips = true, packets = true;
-  for (const TensorArg* t : all) {
+  bool strips = true, packets = true, words = true;
+  for (TensorArg* t : all) {
     if (!t) continue;
+    // The stride of an extent of one may be anything, also one that is not checked below; tiles
+    // reach past such an extent, and where their strips start has to keep to the same rule.
+    if (a->batch <= 1) t->s0 = 0;
+    if (a->dim <= 1) t->s1 = 0;
+    if (a->seqlen <= 1) t->s2 = 0;
     strips = strips && strips_ok(*t, *a);
-    packets = packets && packets_ok(*t, *a);
+    packets = packets && strips_start_on(16, *t, *a);
+    words = words && strips_start_on(4, *t, *a);
   }
-  a->move = !strips ? kElements : packets ? kTma : a->x.dtype != CC1D_FLOAT32 ? kPackets : kElements;
+  a->move = !strips ? kElements : packets ? kTma : words ? kWords : kHalves;
   const int64_t channels = a->x.dtype == CC1D_FLOAT32 ? 32 : 64;
   a->dtiles = (a->dim + channels - 1) / channels;
   const int64_t tiles = a->batch * a->dtiles;

@@ -24,9 +24,9 @@ struct RecArgs {
 };
 
 // How the recurrence's tensors move (RecArgs::move).  kTma: the TMA copies whole tiles both
-// ways (strips aligned to 16 bytes).  kPackets: strips of 16-bit elements that may start
-// anywhere, by the 16-byte packets that cover them.  kElements: one by one, any strides.
-constexpr int kTma = 0, kPackets = 1, kElements = 2;
+// ways (strips aligned to 16 bytes).  kWords and kHalves: strips that start on 4 bytes or (16-bit
+// elements) anywhere, by the 16-byte packets that cover them.  kElements: one by one, any strides.
+constexpr int kTma = 0, kWords = 1, kHalves = 2, kElements = 3;
 
 struct RecUpdateArgs {
   int64_t batch, dim, seqlen, nstates;

@@ -37,7 +37,7 @@ namespace {
 // tiles, and one (backward) or two chunks that are being loaded.  A cluster's rounds are longer:
 // one chunk ahead is enough there and leaves room for a fourth CTA.  Off their alignment strips
 // have larger tiles, and channel-last none that are stored from.
-template <bool SKEW, int LAYOUT, bool CLUSTER> constexpr int kFwdStages = CLUSTER || (SKEW && LAYOUT != kLayoutRows) ? 3 : 4;
+template <int SKEW, int LAYOUT, bool CLUSTER> constexpr int kFwdStages = CLUSTER || (SKEW && LAYOUT != kLayoutRows) ? 3 : 4;
 constexpr int kBwdStages = 3, kMostStages = 4;
 
 // s = 1 / (1 + exp(-v)) at a warp's 8 positions, and e = exp(-v) if wanted.  For 16-bit tensors
@@ -111,7 +111,7 @@ __device__ __forceinline__ Lane<4 / sizeof(T)> gate_offset(const RecArgs& a, int
 // get it (and zeros for the rest), in shared memory, before they are read.
 constexpr float kHold = 60000.f;
 
-template <typename T, int LAYOUT, bool SKEW>
+template <typename T, int LAYOUT, int SKEW>
 __device__ __forceinline__ void load_by_threads(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
   if constexpr (SKEW) load_strips<T, LAYOUT>(tile, t, t0, nd, nt);
   else load_tile<T, LAYOUT>(tile, t, t0, nd, nt);
@@ -265,7 +265,7 @@ __device__ __forceinline__ void start_barriers(unsigned bars, bool tma) {
   else __syncthreads();
 }
 
-template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z, bool CLUSTER>
+template <typename T, int LAYOUT, int SKEW, bool SEQ, bool Z, bool CLUSTER>
 __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int V = C::V, NT = Z ? 3 : 2, S = kFwdStages<SKEW, LAYOUT, CLUSTER>;
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
       for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gb[j], zs[j]);
     }
     if constexpr (kDirect) {
-      store_halves<T>(ot, tw, lane, p.nd - 2 * lane, within(tw, a.seqlen, kRecSteps), SEQ ? ~e.valid & 0xffu : 0u, gb);
+      store_steps<T, SKEW>(ot, tw, lane, p.nd - V * lane, within(tw, a.seqlen, kRecSteps), SEQ ? ~e.valid & 0xffu : 0u, gb);
     } else {
       write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gb);
       if (SEQ && e.valid != 0xffu) clear_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, ~e.valid);
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
   if (CLUSTER) cluster_sync();  // no CTA leaves while a partner may still write to it
 }
 
-template <typename T, int LAYOUT, bool SKEW, bool SEQ, bool Z, bool CLUSTER>
+template <typename T, int LAYOUT, int SKEW, bool SEQ, bool Z, bool CLUSTER>
 __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_constant__ RecArgs a, const __grid_constant__ RecMaps maps) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int V = C::V, NT = Z ? 4 : 3, S = kBwdStages;
@@ -719,11 +719,11 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     bias_lost = sub(sub(new_sum, bias_sum), round_sum);
     bias_sum = new_sum;
     if constexpr (kDirect) {
-      const int left = within(tw, a.seqlen, kRecSteps), n = p.nd - 2 * lane;
+      const int left = within(tw, a.seqlen, kRecSteps), n = p.nd - V * lane;
       const unsigned clear = SEQ ? ~valid & 0xffu : 0u;
-      store_halves<T>(dgt, tw, lane, n, left, clear, prev);
-      store_halves<T>(dxt, tw, lane, n, left, clear, gy);
-      if constexpr (Z) store_halves<T>(dzt, tw, lane, n, left, clear, dz);
+      store_steps<T, SKEW>(dgt, tw, lane, n, left, clear, prev);
+      store_steps<T, SKEW>(dxt, tw, lane, n, left, clear, gy);
+      if constexpr (Z) store_steps<T, SKEW>(dzt, tw, lane, n, left, clear, dz);
     } else {
       write_steps<T, LAYOUT, SKEW>(now, w, lane, prev);
       write_steps<T, LAYOUT, SKEW>(now + C::kBytes, w, lane, gy);
@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
 template <typename T, int LAYOUT>
 bool make_map(CUtensorMap* map, const TensorArg& t, const RecArgs& a) {
   if (!t.data) return true;
-  using C = Tile<T, LAYOUT, false>;
+  using C = Tile<T, LAYOUT, 0>;
   static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
     void* f = nullptr;
     cudaDriverEntryPointQueryResult found;
@@ -808,7 +808,7 @@ cudaError_t capacity_of(const void* kernel, const cudaLaunchConfig_t& cfg, int c
   return e;
 }
 
-template <typename T, int LAYOUT, bool SKEW, bool BWD, bool SEQ, bool Z, bool CLUSTER>
+template <typename T, int LAYOUT, int SKEW, bool BWD, bool SEQ, bool Z, bool CLUSTER>
 cudaError_t run(RecArgs& a, cudaStream_t s) {
   using C = Tile<T, LAYOUT, SKEW>;
   constexpr int NT = (BWD ? 3 : 2) + (Z ? 1 : 0);
@@ -845,11 +845,11 @@ cudaError_t run(RecArgs& a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<const RecArgs&>(a), static_cast<const RecMaps&>(maps));
 }
 
-template <typename T, int LAYOUT, bool SKEW, bool BWD, bool SEQ, bool Z>
+template <typename T, int LAYOUT, int SKEW, bool BWD, bool SEQ, bool Z>
 cudaError_t pick_cluster(RecArgs& a, cudaStream_t s) {
   return a.cluster > 1 ? run<T, LAYOUT, SKEW, BWD, SEQ, Z, true>(a, s) : run<T, LAYOUT, SKEW, BWD, SEQ, Z, false>(a, s);
 }
-template <typename T, int LAYOUT, bool SKEW, bool BWD>
+template <typename T, int LAYOUT, int SKEW, bool BWD>
 cudaError_t pick_options(RecArgs& a, cudaStream_t s) {
   if (a.seq_idx.data)
     return a.z.data ? pick_cluster<T, LAYOUT, SKEW, BWD, true, true>(a, s) : pick_cluster<T, LAYOUT, SKEW, BWD, true, false>(a, s);
@@ -858,9 +858,10 @@ cudaError_t pick_options(RecArgs& a, cudaStream_t s) {
 template <typename T, bool BWD>
 cudaError_t pick(RecArgs& a, cudaStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    if (a.move == kPackets) return a.rows ? pick_options<T, kLayoutRows, true, BWD>(a, s) : pick_options<T, kLayoutChannelLast, true, BWD>(a, s);
+    if (a.move == kHalves) return a.rows ? pick_options<T, kLayoutRows, 2, BWD>(a, s) : pick_options<T, kLayoutChannelLast, 2, BWD>(a, s);
   }
-  return a.rows ? pick_options<T, kLayoutRows, false, BWD>(a, s) : pick_options<T, kLayoutChannelLast, false, BWD>(a, s);
+  if (a.move == kWords) return a.rows ? pick_options<T, kLayoutRows, 4, BWD>(a, s) : pick_options<T, kLayoutChannelLast, 4, BWD>(a, s);
+  return a.rows ? pick_options<T, kLayoutRows, 0, BWD>(a, s) : pick_options<T, kLayoutChannelLast, 0, BWD>(a, s);
 }
 
 }  // namespace

@@ -100,10 +100,10 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
 // rows: strips of 32 positions, one per channel, in 16-byte packets that are swapped around as
 // the TMA's swizzles do, so that 8 lanes reading the same packet of 8 channels use all banks.
 //
-// SKEW (kPackets): the aligned 16-byte packets that cover a strip, in order; the strip starts
+// SKEW (kWords: 4, kHalves: 2): the aligned 16-byte packets that cover a strip, in order; the strip starts
 // as many bytes into them as it lies off a 16-byte boundary in memory.  Results are put there
 // without that offset.
-template <typename T, int LAYOUT, bool SKEW> struct Tile {
+template <typename T, int LAYOUT, int SKEW> struct Tile {
   static constexpr int kSize = sizeof(T);
   static constexpr int V = 4 / kSize;                // channels per lane
   static constexpr int kChannels = 32 * V;           // 128 bytes
@@ -165,12 +165,12 @@ template <int N> __device__ __forceinline__ void tma_wait_read() { asm volatile(
 // What this thread wrote to shared memory is there for the TMA.
 __device__ __forceinline__ void tma_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-// kPackets, all threads: starts the copy of a chunk's strips into a tile, the packets that cover
+// kWords and kHalves, all threads: starts the copy of a chunk's strips into a tile, the packets that cover
 // each.  A thread has every second (rows) or fourth packet of one strip.  Places outside the
 // chunk's nt positions of nd channels are zero or left as they are.
 template <typename T, int LAYOUT>
 __device__ __forceinline__ void load_strips(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
-  using C = Tile<T, LAYOUT, true>;
+  using C = Tile<T, LAYOUT, 4>;
   constexpr int N = kRecThreads / C::kStrips;                      // threads of a strip
   constexpr int K = (C::kPitch / 16 + N - 1) / N;                  // packets of a thread
   const int r = threadIdx.x / N, c = threadIdx.x % N * 16;
@@ -183,7 +183,7 @@ __device__ __forceinline__ void load_strips(unsigned char* tile, const Strip<T>&
   const unsigned to = shared_addr(dst);
   const int left = off + bytes - c;  // up to the strip's end
   if (bytes > 0 && c == 0 && src < reinterpret_cast<const char*>(t.origin)) {  // the tensor begins within the first packet
-    for (int e = off; e < min(16, left); e += C::kSize) *reinterpret_cast<uint16_t*>(dst + e) = *reinterpret_cast<const uint16_t*>(src + e);
+    for (int e = off; e < min(16, left); e += C::kSize) *reinterpret_cast<T*>(dst + e) = *reinterpret_cast<const T*>(src + e);
   } else {
     const int n = max(0, min(16, left));
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(n ? src : strip - off), "r"(n) : "memory");
@@ -199,7 +199,7 @@ __device__ __forceinline__ void load_strips(unsigned char* tile, const Strip<T>&
 // kElements, all threads: positions t0 .. t0 + nt - 1 of nd channels; places outside are zero.
 template <typename T, int LAYOUT>
 __device__ __forceinline__ void load_tile(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
-  using C = Tile<T, LAYOUT, false>;
+  using C = Tile<T, LAYOUT, 0>;
   const unsigned base = shared_addr(tile);
   const T* const src = t.row + t0 * t.s2;
   constexpr int N = C::kChannels * kRecChunk / kRecThreads;
@@ -217,7 +217,7 @@ __device__ __forceinline__ void load_tile(unsigned char* tile, const Strip<T>& t
   }
 }
 
-// kPackets: bytes that strip i of a chunk starts off a 16-byte boundary.  Chunks and warps are
+// kWords and kHalves: bytes that strip i of a chunk starts off a 16-byte boundary.  Chunks and warps are
 // 32 and 8 positions apart, multiples of 16 bytes in either layout, so neither matters.
 template <typename T, int LAYOUT>
 __device__ __forceinline__ unsigned offset_of(const Strip<T>& t, int i) {
@@ -226,24 +226,43 @@ __device__ __forceinline__ unsigned offset_of(const Strip<T>& t, int i) {
 }
 
 // The 8 positions of warp w and the lane's V channels, as fp32.
-template <typename T, int LAYOUT, bool SKEW>
+template <typename T, int LAYOUT, int SKEW>
 __device__ __forceinline__ void read_steps(const unsigned char* tile, const Strip<T>& t, int w, int lane, Lane<4 / sizeof(T)> (&f)[kRecSteps]) {
   using C = Tile<T, LAYOUT, SKEW>;
   if constexpr (C::kRows) {
 #pragma unroll
     for (int i = 0; i < C::V; ++i) {
       const int ch = lane + 32 * i;
+      uint4 packets[kRecSteps / C::kPacket];
+      if constexpr (SKEW) {
+        // From the packets that cover them; single words would be four to a bank.
+        constexpr int N = kRecSteps * C::kSize / 4;
+        const unsigned off = offset_of<T, LAYOUT>(t, ch);
+        const uint4* p = reinterpret_cast<const uint4*>(tile + ch * C::kPitch + w * kRecSteps * C::kSize);
+        uint32_t u[N + 4];
+#pragma unroll
+        for (int q = 0; q <= N / 4; ++q) {
+          const uint4 c = p[q];
+          u[4 * q] = c.x, u[4 * q + 1] = c.y, u[4 * q + 2] = c.z, u[4 * q + 3] = c.w;
+        }
+#pragma unroll
+        for (int j = 0; j < N + 2; ++j) u[j] = off & 8 ? u[j + 2] : u[j];
+#pragma unroll
+        for (int j = 0; j < N + 1; ++j) u[j] = off & 4 ? u[j + 1] : u[j];
+        if constexpr (SKEW == 2) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) u[j] = __funnelshift_r(u[j], u[j + 1], off * 8);
+        }
+#pragma unroll
+        for (int q = 0; q < N / 4; ++q) packets[q] = make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < kRecSteps / C::kPacket; ++q)
+          packets[q] = *reinterpret_cast<const uint4*>(tile + C::at(ch, w * kRecSteps + q * C::kPacket));
+      }
 #pragma unroll
       for (int q = 0; q < kRecSteps / C::kPacket; ++q) {
-        uint4 u;
-        if constexpr (SKEW) {
-          const unsigned off = offset_of<T, LAYOUT>(t, ch), sh = (off & 2) * 8;
-          const uint32_t* p = reinterpret_cast<const uint32_t*>(tile + ch * C::kPitch + w * 16 + (off & 12));
-          const uint32_t w0 = p[0], w1 = p[1], w2 = p[2], w3 = p[3], w4 = p[4];
-          u = make_uint4(__funnelshift_r(w0, w1, sh), __funnelshift_r(w1, w2, sh), __funnelshift_r(w2, w3, sh), __funnelshift_r(w3, w4, sh));
-        } else {
-          u = *reinterpret_cast<const uint4*>(tile + C::at(ch, w * kRecSteps + q * C::kPacket));
-        }
+        const uint4 u = packets[q];
         float2 v[C::kPacket / 2];
         unpack2<T, C::kPacket>(*reinterpret_cast<const Packet<T, C::kPacket>*>(&u), v);
 #pragma unroll
@@ -257,27 +276,27 @@ __device__ __forceinline__ void read_steps(const unsigned char* tile, const Stri
     const unsigned char* p = tile + w * kRecSteps * C::kPitch + lane * 4;
 #pragma unroll
     for (int j = 0; j < kRecSteps; ++j) {
+      const unsigned off = SKEW ? offset_of<T, LAYOUT>(t, j) : 0;
       if constexpr (C::V == 2) {
         uint32_t u;
-        if constexpr (SKEW) {
-          const unsigned off = offset_of<T, LAYOUT>(t, j);
+        if constexpr (SKEW == 2) {
           const uint32_t* q = reinterpret_cast<const uint32_t*>(p + j * C::kPitch + (off & 12));
-          u = __funnelshift_r(q[0], q[1], (off & 2) * 8);
+          u = __funnelshift_r(q[0], q[1], off * 8);
         } else {
-          u = *reinterpret_cast<const uint32_t*>(p + j * C::kPitch);
+          u = *reinterpret_cast<const uint32_t*>(p + j * C::kPitch + off);
         }
         float2 v[1];
         unpack2<T, 2>(*reinterpret_cast<const Packet<T, 2>*>(&u), v);
         f[j].v = v[0];
       } else {
-        f[j].v = *reinterpret_cast<const float*>(p + j * C::kPitch);
+        f[j].v = *reinterpret_cast<const float*>(p + j * C::kPitch + off);
       }
     }
   }
 }
 
 // Puts 8 positions into a tile, without a skew.
-template <typename T, int LAYOUT, bool SKEW>
+template <typename T, int LAYOUT, int SKEW>
 __device__ __forceinline__ void write_steps(unsigned char* tile, int w, int lane, const Lane<4 / sizeof(T)> (&f)[kRecSteps]) {
   using C = Tile<T, LAYOUT, SKEW>;
   if constexpr (C::kRows) {
@@ -307,7 +326,7 @@ __device__ __forceinline__ void write_steps(unsigned char* tile, int w, int lane
 }
 
 // Sets the positions of `mask` among the warp's 8 to a value, in a tile as it was loaded.
-template <typename T, int LAYOUT, bool SKEW>
+template <typename T, int LAYOUT, int SKEW>
 __device__ __forceinline__ void set_steps(unsigned char* tile, const Strip<T>& t, int w, int lane, unsigned mask, float value) {
   using C = Tile<T, LAYOUT, SKEW>;
 #pragma unroll 1
@@ -324,7 +343,7 @@ __device__ __forceinline__ void set_steps(unsigned char* tile, const Strip<T>& t
   }
 }
 // Clears them in a tile of results.
-template <typename T, int LAYOUT, bool SKEW>
+template <typename T, int LAYOUT, int SKEW>
 __device__ __forceinline__ void clear_steps(unsigned char* tile, int w, int lane, unsigned mask) {
   using C = Tile<T, LAYOUT, SKEW>;
 #pragma unroll 1
@@ -336,33 +355,45 @@ __device__ __forceinline__ void clear_steps(unsigned char* tile, int w, int lane
   }
 }
 
-// kElements and kPackets with rows, all threads: stores what write_steps put into a tile.
-template <typename T, int LAYOUT, bool SKEW>
+// kElements, and kWords and kHalves with rows, all threads: stores what write_steps put into a tile.
+template <typename T, int LAYOUT, int SKEW>
 __device__ __forceinline__ void store_tile(const unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
   using C = Tile<T, LAYOUT, SKEW>;
   if constexpr (SKEW) {
-    // the 4-byte words of a strip as it lies in memory: 16, and one more where it starts within one
-    constexpr int W = C::kStripBytes / 4;
+    // The 4-byte words of a strip as it lies in memory: 64 or 128 bytes, and one more word where
+    // it starts within one.  Threads have the same word of every N-th strip, all of which start
+    // alike (N strips are a multiple of 16 bytes apart).
+    constexpr int W = C::kStripBytes / 4, N = kRecThreads / W, E = 4 / C::kSize;
+    const int i = threadIdx.x % W, r = threadIdx.x / W;
     const int64_t step = t.s1 * C::kSize;
-    char* const to = reinterpret_cast<char*>(t.row + t0);
-    auto word = [&](int r, int i) {
-      if (r >= nd) return;
-      char* const strip = to + r * step;
-      const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(strip) >> 1) & 1, e = 2 * i - skew;
-      const unsigned char* const s = tile + r * C::kPitch + 4 * i;  // the word that holds element 2i
-      if (e >= 0 && e + 1 < nt) {
-        uint32_t u = *reinterpret_cast<const uint32_t*>(s);
-        if (skew) u = __funnelshift_r(*reinterpret_cast<const uint32_t*>(s - 4), u, 16);
-        *reinterpret_cast<uint32_t*>(strip + 2 * e) = u;
-      } else {
-        const unsigned char* const f = s - 2 * skew;
-        if (e >= 0 && e < nt) *reinterpret_cast<uint16_t*>(strip + 2 * e) = *reinterpret_cast<const uint16_t*>(f);
-        if (e + 1 >= 0 && e + 1 < nt) *reinterpret_cast<uint16_t*>(strip + 2 * e + 2) = *reinterpret_cast<const uint16_t*>(f + 2);
-      }
-    };
+    char* to = reinterpret_cast<char*>(t.row + t0) + r * step + 4 * i;
+    const int skew = SKEW == 2 ? static_cast<int>(reinterpret_cast<uintptr_t>(to) >> 1) & 1 : 0, e = E * i - skew;
+    to -= 2 * skew;
+    const unsigned char* const s = tile + r * C::kPitch + 4 * i;  // the word that holds element E i
+    if (e >= 0 && e + E <= nt) {
+      const unsigned char* const low = s - 4 * skew;
 #pragma unroll
-    for (int k = 0; k < C::kStrips * W / kRecThreads; ++k) word((threadIdx.x + k * kRecThreads) / W, (threadIdx.x + k * kRecThreads) % W);
-    if (threadIdx.x < C::kStrips) word(threadIdx.x, W);
+      for (int k = 0; k < C::kStrips / N; ++k) {
+        if (r + k * N >= nd) break;
+        uint32_t u = *reinterpret_cast<const uint32_t*>(s + k * N * C::kPitch);
+        if constexpr (SKEW == 2) u = __funnelshift_rc(*reinterpret_cast<const uint32_t*>(low + k * N * C::kPitch), u, skew ? 16 : 32);
+        *reinterpret_cast<uint32_t*>(to) = u;
+        to += N * step;
+      }
+    } else if constexpr (E == 2) {
+      for (int k = r; k < nd; k += N, to += N * step) {
+        const uint16_t* const f = reinterpret_cast<const uint16_t*>(tile + k * C::kPitch);
+        if (e >= 0 && e < nt) *reinterpret_cast<uint16_t*>(to) = f[e];
+        if (e + 1 >= 0 && e + 1 < nt) *reinterpret_cast<uint16_t*>(to + 2) = f[e + 1];
+      }
+    }
+    if constexpr (SKEW == 2) {
+      constexpr int last = kRecChunk - 1;
+      if (threadIdx.x < nd && nt == kRecChunk) {
+        T* const at = t.row + t0 + threadIdx.x * t.s1 + last;
+        if (!(reinterpret_cast<uintptr_t>(at) & 2)) *at = *reinterpret_cast<const T*>(tile + threadIdx.x * C::kPitch + last * 2);
+      }
+    }
   } else {
     T* const dst = t.row + t0 * t.s2;
 #pragma unroll 4
@@ -374,26 +405,36 @@ __device__ __forceinline__ void store_tile(const unsigned char* tile, const Stri
   }
 }
 
-// kPackets, channel-last: stores a warp's 8 positions (from tw on, `left` of them in the sequence)
-// straight from registers, as 2-byte halves; `nch`: the lane's channels that there are.
-// `clear`: positions that get zeros.
-template <typename T>
-__device__ __forceinline__ void store_halves(const Strip<T>& t, int64_t tw, int lane, int nch, int left, unsigned clear, const Lane<2> (&f)[kRecSteps]) {
-  char* p = reinterpret_cast<char*>(t.row + tw * t.s2 + lane * 2);
+// kWords and kHalves, channel-last: stores a warp's 8 positions (from tw on, `left` of them in the
+// sequence) straight from registers, as words or halves; `nch`: the lane's channels that there
+// are.  `clear`: positions that get zeros.
+template <typename T, int SKEW>
+__device__ __forceinline__ void store_steps(const Strip<T>& t, int64_t tw, int lane, int nch, int left, unsigned clear,
+                                            const Lane<4 / sizeof(T)> (&f)[kRecSteps]) {
+  constexpr int V = 4 / sizeof(T);
+  char* p = reinterpret_cast<char*>(t.row + tw * t.s2 + lane * V);
   const int64_t step = t.s2 * static_cast<int64_t>(sizeof(T));
-  const bool whole = left >= kRecSteps && nch >= 2 && !clear;
+  const bool whole = left >= kRecSteps && nch >= V && !clear;
 #pragma unroll
   for (int j = 0; j < kRecSteps; ++j) {
-    float2 v[1] = {f[j].v};
-    const Packet<T, 2> r = pack2<T, 2>(v);
-    uint32_t u = *reinterpret_cast<const uint32_t*>(&r);
-    if (whole) {
+    uint32_t u;
+    if constexpr (V == 2) {
+      float2 v[1] = {f[j].v};
+      const Packet<T, 2> r = pack2<T, 2>(v);
+      u = *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+      u = __float_as_uint(f[j].v);
+    }
+    if (clear >> j & 1u) u = 0;
+    if (whole || (j < left && nch >= V)) {
+      if constexpr (SKEW == 4) {
+        *reinterpret_cast<uint32_t*>(p) = u;
+      } else {
+        *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(u);
+        *reinterpret_cast<uint16_t*>(p + 2) = static_cast<uint16_t>(u >> 16);
+      }
+    } else if (V == 2 && j < left && nch == 1) {
       *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(u);
-      *reinterpret_cast<uint16_t*>(p + 2) = static_cast<uint16_t>(u >> 16);
-    } else if (j < left) {
-      if (clear >> j & 1u) u = 0;
-      if (nch > 0) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(u);
-      if (nch > 1) *reinterpret_cast<uint16_t*>(p + 2) = static_cast<uint16_t>(u >> 16);
     }
     p += step;
   }

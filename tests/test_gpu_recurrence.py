@@ -112,6 +112,24 @@ def test_packed(B, D, L, nseq, states, dtype, layout):
     _run_and_check(_inputs(nseq, B, D, L, dtype, layout, nstates=B * nseq if states else None), ids)
 
 
+@pytest.mark.parametrize("inner,width", [(96, 96), (96, 104), (94, 98), (95, 103), (37, 41), (130, 133)])
+@pytest.mark.parametrize("rows", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strips_that_start_anywhere(dtype, rows, inner, width):
+    """Tensors within wider ones that are NaN around them, each with its own offset and pitch."""
+    D, L = (70, inner) if rows else (inner, 75)
+    for packed in (False, True):
+        t = _inputs(width, 2, D, L, dtype, "contiguous", nstates=6 if packed else 2)
+        for i, k in enumerate(("x", "gate", "z", "dout")):
+            v = t[k] if rows else t[k].transpose(1, 2)
+            pitch, off = width + i % 2 * 2, min(i, width - inner)
+            wide = torch.full((*v.shape[:2], pitch), float("nan"), device="cuda", dtype=dtype)
+            wide[:, :, off:off + inner] = v
+            v = wide[:, :, off:off + inner]
+            t[k] = v if rows else v.transpose(1, 2)
+        _run_and_check(t, _packing(inner, 2, L, 3) if packed else None)
+
+
 @pytest.mark.parametrize("layout", ["channel_last", "contiguous"])
 def test_padding_is_not_read(layout):
     """Whatever padding holds, NaN and infinities included, nothing depends on it; a batch row
