@@ -80,7 +80,7 @@ int sm_count() {
 // How many clusters of a.cluster CTAs (CTAs for 1) of this recurrence's kernel run at a time: the
 // driver's answer, asked once per kernel, size and device.
 int64_t clusters_at_a_time(RecArgs a, bool bwd) {
-  static std::atomic<int> known[64][2][3][4][2][2][2][17];
+  static std::atomic<int> known[64][2][3][5][2][2][2][17];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   const int dt = a.x.dtype;
@@ -146,7 +146,7 @@ cc1d_status rec_plan(RecArgs* a, bool bwd) {
     rows = rows && (t->s2 == 1 || a->seqlen == 1);
   }
   a->rows = rows && (!last || a->dim == 1);
-  bool strips = true, packets = true, words = true;
+  bool strips = true, packets = true, words = true, alike = true;
   for (TensorArg* t : all) {
     if (!t) continue;
     // The stride of an extent of one may be anything, also one that is not checked below; tiles
@@ -157,8 +157,12 @@ cc1d_status rec_plan(RecArgs* a, bool bwd) {
     strips = strips && strips_ok(*t, *a);
     packets = packets && strips_start_on(16, *t, *a);
     words = words && strips_start_on(4, *t, *a);
+    if (t->data && (t == &a->gate || t == &a->z || t == &a->dout))
+      alike = alike && t->s0 == a->x.s0 && t->s1 == a->x.s1 && t->s2 == a->x.s2;
+    if (t->data && (t == &a->x || t == &a->gate || t == &a->z || t == &a->dout))
+      alike = alike && reinterpret_cast<uintptr_t>(t->data) % 16 == 0;
   }
-  a->move = !strips ? kElements : packets ? kTma : words ? kWords : kHalves;
+  a->move = !strips ? kElements : packets ? kTma : !alike ? kOwn : words ? kWords : kHalves;
   const int64_t channels = a->x.dtype == CC1D_FLOAT32 ? 32 : 64;
   a->dtiles = (a->dim + channels - 1) / channels;
   const int64_t tiles = a->batch * a->dtiles;

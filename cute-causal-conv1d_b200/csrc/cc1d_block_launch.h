@@ -24,9 +24,10 @@ struct RecArgs {
 };
 
 // How the recurrence's tensors move (RecArgs::move).  kTma: the TMA copies whole tiles both
-// ways (strips aligned to 16 bytes).  kWords and kHalves: strips that start on 4 bytes or (16-bit
-// elements) anywhere, by the 16-byte packets that cover them.  kElements: one by one, any strides.
-constexpr int kTma = 0, kWords = 1, kHalves = 2, kElements = 3;
+// ways (strips aligned to 16 bytes).  By the 16-byte packets that cover a strip: kWords and kHalves
+// (strips on 4 bytes, or anywhere for 16-bit elements) where the inputs lie alike, so that one
+// offset serves them all; kOwn where each has its own.  kElements: one by one, any strides.
+constexpr int kTma = 0, kWords = 1, kHalves = 2, kOwn = 3, kElements = 4;
 
 struct RecUpdateArgs {
   int64_t batch, dim, seqlen, nstates;

@@ -111,10 +111,18 @@ __device__ __forceinline__ Lane<4 / sizeof(T)> gate_offset(const RecArgs& a, int
 // get it (and zeros for the rest), in shared memory, before they are read.
 constexpr float kHold = 60000.f;
 
+// `same`: the cover of a tensor that lies like t; with kOwn there is none.
 template <typename T, int LAYOUT, int SKEW>
-__device__ __forceinline__ void load_by_threads(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
-  if constexpr (SKEW) load_strips<T, LAYOUT>(tile, t, t0, nd, nt);
+__device__ __forceinline__ void load_by_threads(unsigned char* tile, const Strip<T>& t, const Cover<T, LAYOUT>& same, int64_t t0, int nd, int nt) {
+  if constexpr (SKEW & 1) load_strips<T, LAYOUT, true>(tile, t, Cover<T, LAYOUT>(t), t0, nd, nt);
+  else if constexpr (SKEW) load_strips<T, LAYOUT, false>(tile, t, same, t0, nd, nt);
   else load_tile<T, LAYOUT>(tile, t, t0, nd, nt);
+}
+// The tensor whose offsets tell those of t.
+template <int SKEW, typename T>
+__device__ __forceinline__ const Strip<T>& like(const Strip<T>& t, const Strip<T>& x) {
+  if constexpr (SKEW & 1) return t;
+  else return x;
 }
 
 // Positions of a chunk or of a warp, t .. t + n - 1, that lie within the sequence (may be <= 0).
@@ -286,6 +294,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
   const Strip<T> gt = strip_of<T>(a.gate, maps.gate, p.b, p.d0), xt = strip_of<T>(a.x, maps.x, p.b, p.d0);
   const Strip<T> zt = Z ? strip_of<T>(a.z, maps.z, p.b, p.d0) : gt, ot = strip_of<T>(a.out, maps.out, p.b, p.d0);
 
+  const Cover<T, LAYOUT> cover(xt);
   int load_slot = 0;
   auto load = [&](int k) {  // the tiles of round k
     if (k < p.rounds) {
@@ -305,9 +314,9 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
         }
       } else {
         if (nt > 0) {
-          load_by_threads<T, LAYOUT, SKEW>(smem + o, gt, t0, p.nd, nt);
-          load_by_threads<T, LAYOUT, SKEW>(smem + o + C::kBytes, xt, t0, p.nd, nt);
-          if constexpr (Z) load_by_threads<T, LAYOUT, SKEW>(smem + o + 2 * C::kBytes, zt, t0, p.nd, nt);
+          load_by_threads<T, LAYOUT, SKEW>(smem + o, gt, cover, t0, p.nd, nt);
+          load_by_threads<T, LAYOUT, SKEW>(smem + o + C::kBytes, xt, cover, t0, p.nd, nt);
+          if constexpr (Z) load_by_threads<T, LAYOUT, SKEW>(smem + o + 2 * C::kBytes, zt, cover, t0, p.nd, nt);
         }
         mbar_arrive_copies(bar);  // of the asynchronous copies
         mbar_arrive(bar);         // and of the plain stores
@@ -364,14 +373,14 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     // TMA fills up with zeros).
     const unsigned valid = SEQ ? e.valid : SKEW ? below(within(tw, a.seqlen, kRecSteps)) : 0xffu;
     if (valid != 0xffu) {
-      set_steps<T, LAYOUT, SKEW>(now, gt, w, lane, ~valid, kHold);
+      set_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, ~valid, kHold);
       set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, ~valid, 0.f);
-      if constexpr (Z) set_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, zt, w, lane, ~valid, 0.f);
+      if constexpr (Z) set_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(zt, xt), w, lane, ~valid, 0.f);
       __syncwarp();
     }
     // the 8 positions' maps and their composition
     L ga[kRecSteps], gb[kRecSteps];
-    read_steps<T, LAYOUT, SKEW>(now, gt, w, lane, ga);
+    read_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, ga);
     read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, gb);
     sigmoids<T, V, false, true>(ga, nb, ga, nullptr);
     // 1 - a from a: a + (1 - a) is then exactly one, and the error of 2^-24 is that of a itself
@@ -407,7 +416,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     L zs[kRecSteps];
     auto silu = [&] {
       L z[kRecSteps];
-      read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, zt, w, lane, z);
+      read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(zt, xt), w, lane, z);
       sigmoids<T, V, false, false>(z, splat(0.f, L{}), zs, nullptr);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) zs[j] = mul(zs[j], z[j]);
@@ -503,6 +512,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
   const Strip<T> dzt = Z ? strip_of<T>(a.dz, maps.dz, p.b, p.d0) : dgt;
 
   auto chunk_of = [&](int k) { return static_cast<int64_t>(p.rounds - 1 - k) * p.cluster + p.rank; };
+  const Cover<T, LAYOUT> cover(xt);
   int load_slot = 0;
   auto load = [&](int k) {
     if (k < p.rounds) {
@@ -523,10 +533,10 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
         }
       } else {
         if (nt > 0) {
-          load_by_threads<T, LAYOUT, SKEW>(smem + o, gt, t0, p.nd, nt);
-          load_by_threads<T, LAYOUT, SKEW>(smem + o + C::kBytes, xt, t0, p.nd, nt);
-          load_by_threads<T, LAYOUT, SKEW>(smem + o + 2 * C::kBytes, yt, t0, p.nd, nt);
-          if constexpr (Z) load_by_threads<T, LAYOUT, SKEW>(smem + o + 3 * C::kBytes, zt, t0, p.nd, nt);
+          load_by_threads<T, LAYOUT, SKEW>(smem + o, gt, cover, t0, p.nd, nt);
+          load_by_threads<T, LAYOUT, SKEW>(smem + o + C::kBytes, xt, cover, t0, p.nd, nt);
+          load_by_threads<T, LAYOUT, SKEW>(smem + o + 2 * C::kBytes, yt, cover, t0, p.nd, nt);
+          if constexpr (Z) load_by_threads<T, LAYOUT, SKEW>(smem + o + 3 * C::kBytes, zt, cover, t0, p.nd, nt);
         }
         mbar_arrive_copies(bar);
         mbar_arrive(bar);
@@ -595,16 +605,16 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
       valid = e.valid;
     }
     if (valid != 0xffu) {  // rare: positions without a token pass the gradient on
-      set_steps<T, LAYOUT, SKEW>(now, gt, w, lane, ~valid, kHold);
+      set_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, ~valid, kHold);
       set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, ~valid, 0.f);
-      set_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, yt, w, lane, ~valid, 0.f);
-      if constexpr (Z) set_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, w, lane, ~valid, 0.f);
+      set_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(yt, xt), w, lane, ~valid, 0.f);
+      if constexpr (Z) set_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, like<SKEW>(zt, xt), w, lane, ~valid, 0.f);
       __syncwarp();
     }
     L ga[kRecSteps], gc[kRecSteps], x[kRecSteps], gy[kRecSteps], dz[kRecSteps];
     {
       L g[kRecSteps];
-      read_steps<T, LAYOUT, SKEW>(now, gt, w, lane, g);
+      read_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, g);
       // the gradients have 1 - a as a factor, so it is taken to full relative precision
       sigmoids<T, V, true, true>(g, nb, ga, gc);
 #pragma unroll
@@ -612,10 +622,10 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
       if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
     }
     read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, x);
-    read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, yt, w, lane, gy);
+    read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(yt, xt), w, lane, gy);
     if constexpr (Z) {
       L z[kRecSteps], s[kRecSteps];
-      read_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, zt, w, lane, z);
+      read_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, like<SKEW>(zt, xt), w, lane, z);
       sigmoids<T, V, false, false>(z, splat(0.f, L{}), s, nullptr);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
@@ -857,9 +867,11 @@ cudaError_t pick_options(RecArgs& a, cudaStream_t s) {
 }
 template <typename T, bool BWD>
 cudaError_t pick(RecArgs& a, cudaStream_t s) {
+  constexpr int own = sizeof(T) == 2 ? 3 : 5;
   if constexpr (sizeof(T) == 2) {
     if (a.move == kHalves) return a.rows ? pick_options<T, kLayoutRows, 2, BWD>(a, s) : pick_options<T, kLayoutChannelLast, 2, BWD>(a, s);
   }
+  if (a.move == kOwn) return a.rows ? pick_options<T, kLayoutRows, own, BWD>(a, s) : pick_options<T, kLayoutChannelLast, own, BWD>(a, s);
   if (a.move == kWords) return a.rows ? pick_options<T, kLayoutRows, 4, BWD>(a, s) : pick_options<T, kLayoutChannelLast, 4, BWD>(a, s);
   return a.rows ? pick_options<T, kLayoutRows, 0, BWD>(a, s) : pick_options<T, kLayoutChannelLast, 0, BWD>(a, s);
 }

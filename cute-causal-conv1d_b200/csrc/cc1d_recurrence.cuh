@@ -100,9 +100,9 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
 // rows: strips of 32 positions, one per channel, in 16-byte packets that are swapped around as
 // the TMA's swizzles do, so that 8 lanes reading the same packet of 8 channels use all banks.
 //
-// SKEW (kWords: 4, kHalves: 2): the aligned 16-byte packets that cover a strip, in order; the strip starts
-// as many bytes into them as it lies off a 16-byte boundary in memory.  Results are put there
-// without that offset.
+// SKEW (4: kWords, 2: kHalves, with 1 added: kOwn): the aligned 16-byte packets that cover a
+// strip, in order; the strip starts as many bytes into them as it lies off a 16-byte boundary in
+// memory.  Results are put there without that offset.
 template <typename T, int LAYOUT, int SKEW> struct Tile {
   static constexpr int kSize = sizeof(T);
   static constexpr int V = 4 / kSize;                // channels per lane
@@ -165,34 +165,46 @@ template <int N> __device__ __forceinline__ void tma_wait_read() { asm volatile(
 // What this thread wrote to shared memory is there for the TMA.
 __device__ __forceinline__ void tma_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-// kWords and kHalves, all threads: starts the copy of a chunk's strips into a tile, the packets that cover
-// each.  A thread has every second (rows) or fourth packet of one strip.  Places outside the
-// chunk's nt positions of nd channels are zero or left as they are.
+// Strips off 16 bytes: the packets that a thread copies of each chunk, every second (rows) or
+// fourth of one strip.
 template <typename T, int LAYOUT>
-__device__ __forceinline__ void load_strips(unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
+struct Cover {
   using C = Tile<T, LAYOUT, 4>;
-  constexpr int N = kRecThreads / C::kStrips;                      // threads of a strip
-  constexpr int K = (C::kPitch / 16 + N - 1) / N;                  // packets of a thread
-  const int r = threadIdx.x / N, c = threadIdx.x % N * 16;
-  const int64_t step = (C::kRows ? t.s1 : t.s2) * C::kSize;
-  const int bytes = r < (C::kRows ? nd : nt) ? (C::kRows ? nt : nd) * C::kSize : -16;
-  const char* const strip = reinterpret_cast<const char*>(t.row + (C::kRows ? t0 : t0 * t.s2)) + r * step;
-  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(strip)) & 15;
-  const char* const src = strip - off + c;
-  unsigned char* const dst = tile + r * C::kPitch + c;
+  static constexpr int N = kRecThreads / C::kStrips;         // threads of a strip
+  static constexpr int K = (C::kPitch / 16 + N - 1) / N;     // packets of a thread
+  int r, c;     // the strip, and the first packet's bytes in it
+  int off;      // bytes that the strip starts into its first packet
+  int64_t rel;  // from the chunk's first element to the first packet
+  __device__ __forceinline__ explicit Cover(const Strip<T>& t) : r(threadIdx.x / N), c(threadIdx.x % N * 16) {
+    const int64_t step = (C::kRows ? t.s1 : t.s2) * C::kSize;
+    off = static_cast<int>(reinterpret_cast<uintptr_t>(t.row) + r * step) & 15;
+    rel = r * step - off + c;
+  }
+};
+// All threads: starts the copy of a chunk's packets into a tile.  Places outside the chunk's nt
+// positions of nd channels are zero or left as they are.  GUARD: the tensor may begin within a
+// packet, and what lies before is not read.
+template <typename T, int LAYOUT, bool GUARD>
+__device__ __forceinline__ void load_strips(unsigned char* tile, const Strip<T>& t, const Cover<T, LAYOUT>& m, int64_t t0, int nd, int nt) {
+  using C = Tile<T, LAYOUT, 4>;
+  using M = Cover<T, LAYOUT>;
+  const int bytes = m.r < (C::kRows ? nd : nt) ? (C::kRows ? nt : nd) * C::kSize : -16;
+  const char* const first = reinterpret_cast<const char*>(t.row + (C::kRows ? t0 : t0 * t.s2));
+  const char* const src = first + m.rel;
+  unsigned char* const dst = tile + m.r * C::kPitch + m.c;
   const unsigned to = shared_addr(dst);
-  const int left = off + bytes - c;  // up to the strip's end
-  if (bytes > 0 && c == 0 && src < reinterpret_cast<const char*>(t.origin)) {  // the tensor begins within the first packet
-    for (int e = off; e < min(16, left); e += C::kSize) *reinterpret_cast<T*>(dst + e) = *reinterpret_cast<const T*>(src + e);
+  const int left = m.off + bytes - m.c;  // up to the strip's end
+  if (GUARD && bytes > 0 && m.c == 0 && src < reinterpret_cast<const char*>(t.origin)) {
+    for (int e = m.off; e < min(16, left); e += C::kSize) *reinterpret_cast<T*>(dst + e) = *reinterpret_cast<const T*>(src + e);
   } else {
     const int n = max(0, min(16, left));
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(n ? src : strip - off), "r"(n) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(src), "r"(n) : "memory");
   }
 #pragma unroll
-  for (int k = 1; k < K; ++k) {
-    if ((k + 1) * N * 16 > C::kPitch && c + k * N * 16 >= C::kPitch) break;
-    const int n = max(0, min(16, left - k * N * 16));
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to + k * N * 16), "l"(src + k * N * 16), "r"(n) : "memory");
+  for (int k = 1; k < M::K; ++k) {
+    if ((k + 1) * M::N * 16 > C::kPitch && m.c + k * M::N * 16 >= C::kPitch) break;
+    const int n = max(0, min(16, left - k * M::N * 16));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to + k * M::N * 16), "l"(src + k * M::N * 16), "r"(n) : "memory");
   }
 }
 
@@ -217,7 +229,7 @@ __device__ __forceinline__ void load_tile(unsigned char* tile, const Strip<T>& t
   }
 }
 
-// kWords and kHalves: bytes that strip i of a chunk starts off a 16-byte boundary.  Chunks and warps are
+// Strips off 16 bytes: bytes that strip i of a chunk starts off a 16-byte boundary.  Chunks and warps are
 // 32 and 8 positions apart, multiples of 16 bytes in either layout, so neither matters.
 template <typename T, int LAYOUT>
 __device__ __forceinline__ unsigned offset_of(const Strip<T>& t, int i) {
@@ -249,7 +261,7 @@ __device__ __forceinline__ void read_steps(const unsigned char* tile, const Stri
         for (int j = 0; j < N + 2; ++j) u[j] = off & 8 ? u[j + 2] : u[j];
 #pragma unroll
         for (int j = 0; j < N + 1; ++j) u[j] = off & 4 ? u[j + 1] : u[j];
-        if constexpr (SKEW == 2) {
+        if constexpr ((SKEW & 6) == 2) {
 #pragma unroll
           for (int j = 0; j < N; ++j) u[j] = __funnelshift_r(u[j], u[j + 1], off * 8);
         }
@@ -279,7 +291,7 @@ __device__ __forceinline__ void read_steps(const unsigned char* tile, const Stri
       const unsigned off = SKEW ? offset_of<T, LAYOUT>(t, j) : 0;
       if constexpr (C::V == 2) {
         uint32_t u;
-        if constexpr (SKEW == 2) {
+        if constexpr ((SKEW & 6) == 2) {
           const uint32_t* q = reinterpret_cast<const uint32_t*>(p + j * C::kPitch + (off & 12));
           u = __funnelshift_r(q[0], q[1], off * 8);
         } else {
@@ -355,7 +367,7 @@ __device__ __forceinline__ void clear_steps(unsigned char* tile, int w, int lane
   }
 }
 
-// kElements, and kWords and kHalves with rows, all threads: stores what write_steps put into a tile.
+// kElements, and strips off 16 bytes with rows, all threads: stores what write_steps put into a tile.
 template <typename T, int LAYOUT, int SKEW>
 __device__ __forceinline__ void store_tile(const unsigned char* tile, const Strip<T>& t, int64_t t0, int nd, int nt) {
   using C = Tile<T, LAYOUT, SKEW>;
@@ -367,31 +379,31 @@ __device__ __forceinline__ void store_tile(const unsigned char* tile, const Stri
     const int i = threadIdx.x % W, r = threadIdx.x / W;
     const int64_t step = t.s1 * C::kSize;
     char* to = reinterpret_cast<char*>(t.row + t0) + r * step + 4 * i;
-    const int skew = SKEW == 2 ? static_cast<int>(reinterpret_cast<uintptr_t>(to) >> 1) & 1 : 0, e = E * i - skew;
-    to -= 2 * skew;
-    const unsigned char* const s = tile + r * C::kPitch + 4 * i;  // the word that holds element E i
-    if (e >= 0 && e + E <= nt) {
-      const unsigned char* const low = s - 4 * skew;
+    const int skew = (SKEW & 6) == 2 ? static_cast<int>(reinterpret_cast<uintptr_t>(to) >> 1) & 1 : 0, e = E * i - skew;
+    to -= 2 * skew;  // the word of elements e .. e + E - 1
+    if (nt == kRecChunk) {
+      const unsigned char* const s = tile + r * C::kPitch + 4 * i;  // the word that holds element E i
+      const unsigned char* const low = s - (e > 0 ? 4 * skew : 0);
 #pragma unroll
-      for (int k = 0; k < C::kStrips / N; ++k) {
+      for (int k = 0; k < C::kStrips / N; ++k, to += N * step) {
         if (r + k * N >= nd) break;
         uint32_t u = *reinterpret_cast<const uint32_t*>(s + k * N * C::kPitch);
-        if constexpr (SKEW == 2) u = __funnelshift_rc(*reinterpret_cast<const uint32_t*>(low + k * N * C::kPitch), u, skew ? 16 : 32);
-        *reinterpret_cast<uint32_t*>(to) = u;
-        to += N * step;
+        if constexpr ((SKEW & 6) == 2) u = __funnelshift_rc(*reinterpret_cast<const uint32_t*>(low + k * N * C::kPitch), u, skew ? 16 : 32);
+        if (e >= 0) *reinterpret_cast<uint32_t*>(to) = u;
+        else *reinterpret_cast<uint16_t*>(to + 2) = static_cast<uint16_t>(u >> 16);
       }
-    } else if constexpr (E == 2) {
+      if constexpr ((SKEW & 6) == 2) {  // a skewed strip's last element, in the word after its 16
+        constexpr int last = kRecChunk - 1;
+        if (threadIdx.x < nd) {
+          T* const at = t.row + t0 + threadIdx.x * t.s1 + last;
+          if (!(reinterpret_cast<uintptr_t>(at) & 2)) *at = *reinterpret_cast<const T*>(tile + threadIdx.x * C::kPitch + last * C::kSize);
+        }
+      }
+    } else {
       for (int k = r; k < nd; k += N, to += N * step) {
-        const uint16_t* const f = reinterpret_cast<const uint16_t*>(tile + k * C::kPitch);
-        if (e >= 0 && e < nt) *reinterpret_cast<uint16_t*>(to) = f[e];
-        if (e + 1 >= 0 && e + 1 < nt) *reinterpret_cast<uint16_t*>(to + 2) = f[e + 1];
-      }
-    }
-    if constexpr (SKEW == 2) {
-      constexpr int last = kRecChunk - 1;
-      if (threadIdx.x < nd && nt == kRecChunk) {
-        T* const at = t.row + t0 + threadIdx.x * t.s1 + last;
-        if (!(reinterpret_cast<uintptr_t>(at) & 2)) *at = *reinterpret_cast<const T*>(tile + threadIdx.x * C::kPitch + last * 2);
+#pragma unroll
+        for (int h = 0; h < E; ++h)
+          if (e + h >= 0 && e + h < nt) reinterpret_cast<T*>(to)[h] = reinterpret_cast<const T*>(tile + k * C::kPitch)[e + h];
       }
     }
   } else {
@@ -405,7 +417,7 @@ __device__ __forceinline__ void store_tile(const unsigned char* tile, const Stri
   }
 }
 
-// kWords and kHalves, channel-last: stores a warp's 8 positions (from tw on, `left` of them in the
+// Strips off 16 bytes, channel-last: stores a warp's 8 positions (from tw on, `left` of them in the
 // sequence) straight from registers, as words or halves; `nch`: the lane's channels that there
 // are.  `clear`: positions that get zeros.
 template <typename T, int SKEW>
@@ -427,7 +439,7 @@ __device__ __forceinline__ void store_steps(const Strip<T>& t, int64_t tw, int l
     }
     if (clear >> j & 1u) u = 0;
     if (whole || (j < left && nch >= V)) {
-      if constexpr (SKEW == 4) {
+      if constexpr ((SKEW & 6) == 4) {
         *reinterpret_cast<uint32_t*>(p) = u;
       } else {
         *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(u);
