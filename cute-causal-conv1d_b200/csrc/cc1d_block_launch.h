@@ -47,10 +47,10 @@ struct AddNormArgs {
   float eps, keep_scale;     // keep_scale = 1 / (1 - p)
   unsigned keep_from;        // a word below it is dropped
   // the plan (add_norm_plan): threads that share a row (0: rows too wide for the registers),
-  // columns that each of them holds, CTAs, and whether every row moves in 16-byte packets
-  int group, held;
+  // columns that each of them holds, CTAs, and the elements that every row starts on a multiple
+  // of: 8 (16-bit types), 4, 2 or 1
+  int group, held, aligned;
   int64_t ctas;
-  bool vectors;
 };
 
 // The launches of one element type.  Args& is changed only where a recurrence's tensor turns
