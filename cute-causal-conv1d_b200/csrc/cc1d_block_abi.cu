@@ -135,7 +135,10 @@ int choose_cluster(RecArgs* a, int64_t tiles, bool bwd) {
 }
 
 // Layout, way of moving and cluster of a recurrence.  Rows: every tensor has unit stride along
-// the sequence; all others take the channel-last kernel.
+// the sequence; all others take the channel-last kernel.  The first of the ways that the tensors
+// allow is the fastest; bf16, 8 sequences of 8192, forward and backward: 382 and 722 us for
+// 4096 channels (kTma), 642 and 1168 us for 4094 (kWords), 748 and 1318 us for 4095 (kHalves),
+// 764 and 1781 us with an offset for each input (kOwn).
 cc1d_status rec_plan(RecArgs* a, bool bwd) {
   TensorArg* const all[] = {&a->x, &a->gate, &a->z, bwd ? &a->dout : &a->out, bwd ? &a->dx : nullptr,
                             bwd ? &a->dgate : nullptr, bwd ? &a->dz : nullptr};
