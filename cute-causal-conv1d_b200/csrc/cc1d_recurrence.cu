@@ -107,10 +107,6 @@ __device__ __forceinline__ Lane<4 / sizeof(T)> gate_offset(const RecArgs& a, int
   return nb;
 }
 
-// A gate that holds the state: a = 1 and 1 - a = 0 whatever the bias.  Positions without a token
-// get it (and zeros for the rest), in shared memory, before they are read.
-constexpr float kHold = 60000.f;
-
 // `same`: the cover of a tensor that lies like t; with kOwn there is none.
 template <typename T, int LAYOUT, int SKEW>
 __device__ __forceinline__ void load_by_threads(unsigned char* tile, const Strip<T>& t, const Cover<T, LAYOUT>& same, int64_t t0, int nd, int nt) {
@@ -368,14 +364,14 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     if constexpr (SEQ) {
       e = edges_of(common.ids[k % 3][w * kRecSteps + min(lane, kRecSteps + 1)]);
     }
-    // Rare: positions without a token pass the state on.  z as well: four positions share a
-    // reciprocal, and their roundings must not depend on what padding or old tiles hold (the
-    // TMA fills up with zeros).
+    // Rare: positions without a token are cleared.  Nothing reads the state that leaves them, but
+    // four positions share a reciprocal, and their roundings must not depend on what padding or
+    // old tiles hold (the TMA fills up with zeros).
     const unsigned valid = SEQ ? e.valid : SKEW ? below(within(tw, a.seqlen, kRecSteps)) : 0xffu;
     if (valid != 0xffu) {
-      set_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, ~valid, kHold);
-      set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, ~valid, 0.f);
-      if constexpr (Z) set_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(zt, xt), w, lane, ~valid, 0.f);
+      zero_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, ~valid);
+      zero_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, ~valid);
+      if constexpr (Z) zero_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(zt, xt), w, lane, ~valid);
       __syncwarp();
     }
     // the 8 positions' maps and their composition
@@ -604,11 +600,11 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
       e = edges_of(common.ids[k % 3][w * kRecSteps + min(lane, kRecSteps + 1)]);
       valid = e.valid;
     }
-    if (valid != 0xffu) {  // rare: positions without a token pass the gradient on
-      set_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, ~valid, kHold);
-      set_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, ~valid, 0.f);
-      set_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(yt, xt), w, lane, ~valid, 0.f);
-      if constexpr (Z) set_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, like<SKEW>(zt, xt), w, lane, ~valid, 0.f);
+    if (valid != 0xffu) {  // rare: positions without a token are cleared
+      zero_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, ~valid);
+      zero_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, ~valid);
+      zero_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(yt, xt), w, lane, ~valid);
+      if constexpr (Z) zero_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, like<SKEW>(zt, xt), w, lane, ~valid);
       __syncwarp();
     }
     L ga[kRecSteps], gc[kRecSteps], x[kRecSteps], gy[kRecSteps], dz[kRecSteps];
@@ -619,6 +615,14 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
       sigmoids<T, V, true, true>(g, nb, ga, gc);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) gc[j] = mul(gc[j], ga[j]);
+      if (valid != 0xffu) {  // and hand the gradient on as it is, whatever the bias
+#pragma unroll
+        for (int j = 0; j < kRecSteps; ++j)
+          if (!(valid >> j & 1u)) {
+            ga[j] = splat(1.f, L{});
+            gc[j] = splat(0.f, L{});
+          }
+      }
       if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
     }
     read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, x);

@@ -337,9 +337,9 @@ __device__ __forceinline__ void write_steps(unsigned char* tile, int w, int lane
   }
 }
 
-// Sets the positions of `mask` among the warp's 8 to a value, in a tile as it was loaded.
+// Sets the positions of `mask` among the warp's 8 to zero, in a tile as it was loaded.
 template <typename T, int LAYOUT, int SKEW>
-__device__ __forceinline__ void set_steps(unsigned char* tile, const Strip<T>& t, int w, int lane, unsigned mask, float value) {
+__device__ __forceinline__ void zero_steps(unsigned char* tile, const Strip<T>& t, int w, int lane, unsigned mask) {
   using C = Tile<T, LAYOUT, SKEW>;
 #pragma unroll 1
   for (int j = 0; j < kRecSteps; ++j) {
@@ -350,7 +350,7 @@ __device__ __forceinline__ void set_steps(unsigned char* tile, const Strip<T>& t
       const int ch = lane_channel<T, LAYOUT>(lane, i);
       int o = C::at(ch, pos);
       if constexpr (SKEW) o += offset_of<T, LAYOUT>(t, C::kRows ? ch : j);
-      *reinterpret_cast<T*>(tile + o) = from_f32<T>(value);
+      *reinterpret_cast<T*>(tile + o) = from_f32<T>(0.f);
     }
   }
 }
