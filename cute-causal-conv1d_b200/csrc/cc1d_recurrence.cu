@@ -40,41 +40,48 @@ namespace {
 template <int SKEW, int LAYOUT, bool CLUSTER> constexpr int kFwdStages = CLUSTER || (SKEW && LAYOUT != kLayoutRows) ? 3 : 4;
 constexpr int kBwdStages = 3, kMostStages = 4;
 
-// s = 1 / (1 + exp(-v)) at a warp's 8 positions, and e = exp(-v) if wanted.  For 16-bit tensors
-// -v log2(e) = v m + n with m = -log2(e), for fp32 n is added to v.
+// s = sigmoid(v + bias) at a warp's 8 positions, and with GATE (where they weight a state) also
+// c = 1 - s = e s, e = exp(-v - bias).  For 16-bit tensors -v log2(e) = v m + n with m = -log2(e),
+// for fp32 n is added to v.
+//
+// 1 - s by subtraction would leave few bits of a slow channel's c (2e-3 off at v = 10, all of them
+// lost from 17 on); e s is relative to itself.  The same channel multiplies its state by thousands
+// of s, so the reciprocal's error is taken out with one step of Newton's iteration on the residual
+// 1 - s - e s: s is then rounded as near to one as fp32 allows, about 2^-25 of it.
 //
 // 16-bit: four positions share one reciprocal, of the product of their 1 + e (the special
 // function unit would bound the forward otherwise: 4 of its operations per element, now 2.5).
 // So that the product stays finite e is at most 2^30 and a sigmoid at least 2^-30, which is
-// zero next to the other terms of a sum; the three more roundings leave 2^-22.  A NaN must not
-// reach the others of its four: the minimum drops it, and KEEP puts it back into its own
-// sigmoid (silu has it from z).
-template <typename T, int V, bool E, bool KEEP>
-__device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const Lane<V>& n, Lane<V> (&s)[kRecSteps], Lane<V>* e) {
+// zero next to the other terms of a sum; the three more roundings leave 2^-22, which is enough
+// for silu.  A NaN must not reach the others of its four: the minimum drops it, and GATE puts it
+// back into its own sigmoid (silu has it from z).
+template <typename T, int V, bool GATE>
+__device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const Lane<V>& n, Lane<V> (&s)[kRecSteps], Lane<V>* c) {
+  const Lane<V> one = splat(1.f, n);
   if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
     for (int j = 0; j < kRecSteps; ++j) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float x = exp_minus<float>(el(v[j], i) + el(n, i));
-        if constexpr (E) el(e[j], i) = x;
-        el(s[j], i) = rcp_approx(1.f + x);
+        const float e = exp_minus<float>(el(v[j], i) + el(n, i));
+        const float r = rcp_approx(1.f + e);
+        el(s[j], i) = GATE ? fmaf(r, fmaf(-r, e, 1.f - r), r) : r;
+        if constexpr (GATE) el(c[j], i) = e * el(s[j], i);
       }
     }
   } else {
 #pragma unroll
     for (int q = 0; q < kRecSteps; q += 4) {
-      Lane<V> d[4], raw[4];
+      Lane<V> e[4], d[4], raw[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        Lane<V> x = fma(v[q + j], splat(-kLog2e, n), n);
+        e[j] = fma(v[q + j], splat(-kLog2e, n), n);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          el(raw[j], i) = ex2_approx(el(x, i));
-          el(x, i) = fminf(el(raw[j], i), 1073741824.f);
+          el(raw[j], i) = ex2_approx(el(e[j], i));
+          el(e[j], i) = fminf(el(raw[j], i), 1073741824.f);
         }
-        if constexpr (E) e[q + j] = x;
-        d[j] = add(x, splat(1.f, x));
+        d[j] = add(e[j], one);
       }
       const Lane<V> lo = mul(d[0], d[1]), hi = mul(d[2], d[3]);
       Lane<V> r = mul(lo, hi);
@@ -85,11 +92,15 @@ __device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const La
       s[q + 1] = mul(rlo, d[0]);
       s[q + 2] = mul(rhi, d[3]);
       s[q + 3] = mul(rhi, d[2]);
-      if constexpr (KEEP) {
+      if constexpr (GATE) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j) {
+          Lane<V>& a = s[q + j];
+          a = fma(a, sub(sub(one, a), mul(e[j], a)), a);
 #pragma unroll
-          for (int i = 0; i < V; ++i) el(s[q + j], i) = max_nan(el(s[q + j], i), -el(raw[j], i));
+          for (int i = 0; i < V; ++i) el(a, i) = max_nan(el(a, i), -el(raw[j], i));
+          c[q + j] = mul(e[j], a);
+        }
       }
     }
   }
@@ -378,10 +389,12 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     L ga[kRecSteps], gb[kRecSteps];
     read_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, ga);
     read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, gb);
-    sigmoids<T, V, false, true>(ga, nb, ga, nullptr);
-    // 1 - a from a: a + (1 - a) is then exactly one, and the error of 2^-24 is that of a itself
+    {
+      L gc[kRecSteps];
+      sigmoids<T, V, true>(ga, nb, ga, gc);
 #pragma unroll
-    for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(sub(splat(1.f, L{}), ga[j]), gb[j]);
+      for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gc[j], gb[j]);
+    }
     if (!there) ga[0] = splat(__int_as_float(0x7fc00000), L{});
     L A = ga[0], H = gb[0];
 #pragma unroll
@@ -413,7 +426,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     auto silu = [&] {
       L z[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(zt, xt), w, lane, z);
-      sigmoids<T, V, false, false>(z, splat(0.f, L{}), zs, nullptr);
+      sigmoids<T, V, false>(z, splat(0.f, L{}), zs, nullptr);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) zs[j] = mul(zs[j], z[j]);
     };
@@ -611,10 +624,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     {
       L g[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, g);
-      // the gradients have 1 - a as a factor, so it is taken to full relative precision
-      sigmoids<T, V, true, true>(g, nb, ga, gc);
-#pragma unroll
-      for (int j = 0; j < kRecSteps; ++j) gc[j] = mul(gc[j], ga[j]);
+      sigmoids<T, V, true>(g, nb, ga, gc);
       if (valid != 0xffu) {  // and hand the gradient on as it is, whatever the bias
 #pragma unroll
         for (int j = 0; j < kRecSteps; ++j)
@@ -630,7 +640,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     if constexpr (Z) {
       L z[kRecSteps], s[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, like<SKEW>(zt, xt), w, lane, z);
-      sigmoids<T, V, false, false>(z, splat(0.f, L{}), s, nullptr);
+      sigmoids<T, V, false>(z, splat(0.f, L{}), s, nullptr);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
         // silu(z) = z s and silu'(z) = s + z s (1 - s), s = sigmoid(z)
