@@ -5,54 +5,72 @@
 
 namespace cc1d {
 
-// min(v, most) that keeps a NaN: e / (1 + e) stays finite where exp overflows, and 1 / (1 + e)
-// is then zero to working precision.
-__device__ __forceinline__ float clamp_exp(float v, float most) {
+// The largest (smallest) of three, or NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
-// The larger of two, or NaN if one is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
+// Within +-87 neither exp nor 1 / (1 + exp) leaves the normal numbers; beyond, a sigmoid is 0 or 1
+// to within e^-87 = 1.6e-38.  An e of at most 2^30 has finite products of four 1 + e.
+constexpr float kMostExponent = 87.f, kMostBits = 30.f;
 
-// exp(-u) for 16-bit tensors: 2^v by the hardware's approximation (relative error about 2^-22,
-// plus the rounding of v = -u log2(e)), at most 1e30.
-//
-// fp32 also takes what that rounding loses: -u log2(e) = t + r, with r from two fused
-// multiply-adds (the second for the part of log2(e) below fp32), and 2^r = 1 + r ln 2 to
-// 2^-40.  u is held within +-85, where sigmoids are 0 and 1 to working precision and neither
-// exp nor 1 / (1 + exp) leaves the normal numbers; a NaN passes.
-template <typename T>
+// exp(-u) for |u| <= kMostExponent: 2^v by the hardware's approximation (relative error about
+// 2^-22) and what the rounding of v loses: -u log2(e) = t + r, with r from two fused
+// multiply-adds (the second for the part of log2(e) below fp32), and 2^r = 1 + r ln 2 to 2^-40.
 __device__ __forceinline__ float exp_minus(float u) {
-  if constexpr (std::is_same<T, float>::value) {
-    constexpr double kLog2eExact = 1.4426950408889634074;
-    constexpr float kLow = static_cast<float>(kLog2eExact - static_cast<double>(kLog2e));
-    u = clamp_exp(max_nan(u, -85.f), 85.f);
-    const float t = -kLog2e * u;
-    const float r = fmaf(-kLow, u, fmaf(-kLog2e, u, -t));
-    const float e = ex2_approx(t);
-    return fmaf(e, r * 0.693147181f, e);
+  constexpr double kLog2eExact = 1.4426950408889634074;
+  constexpr float kLow = static_cast<float>(kLog2eExact - static_cast<double>(kLog2e));
+  const float t = -kLog2e * u;
+  const float r = fmaf(-kLow, u, fmaf(-kLog2e, u, -t));
+  const float e = ex2_approx(t);
+  return fmaf(e, r * 0.693147181f, e);
+}
+
+// A step of Newton's iteration for s = 1 / (1 + e), whose residual takes no rounding of 1 + e.
+__device__ __forceinline__ float newton(float s, float e) { return fmaf(s, fmaf(-s, e, 1.f - s), s); }
+
+// a = 1 / (1 + e) and c = e / (1 + e), for any e >= 0 that exp may give, infinite or NaN as well.
+__device__ __forceinline__ void pair_of_exp(float e, float& a, float& c) {
+  a = rcp_approx(1.f + e);
+  if (e <= 1073741824.f) {  // 2^kMostBits
+    a = newton(a, e);
+    c = e * a;
   } else {
-    return clamp_exp(ex2_approx(-kLog2e * u), 1e30f);
+    c = 1.f - a;
   }
 }
 
-// a = sigmoid(u) and c = 1 - a = sigmoid(-u), each to full relative precision.
-template <typename T>
-__device__ __forceinline__ void sigmoid_pair(float u, float& a, float& c) {
-  const float e = exp_minus<T>(u);
+// a = sigmoid(u) and c = 1 - a = sigmoid(-u), each to full relative precision (to 2^-22 without
+// NEWTON), for |u| <= kMostExponent.
+template <bool NEWTON = true>
+__device__ __forceinline__ void sigmoid_within(float u, float& a, float& c) {
+  const float e = exp_minus(u);
   a = rcp_approx(1.f + e);
+  if constexpr (NEWTON) a = newton(a, e);
   c = e * a;
 }
+// The same for any u, NaN included: exactly 0 and 1 beyond +-kMostExponent.
+template <bool NEWTON = true>
+__device__ __forceinline__ void sigmoid_pair(float u, float& a, float& c) {
+  if (fabsf(u) <= kMostExponent) {
+    sigmoid_within<NEWTON>(u, a, c);
+  } else {
+    a = u > 0.f ? 1.f : u < 0.f ? 0.f : u;
+    c = 1.f - a;
+  }
+}
 
-template <typename T>
 __device__ __forceinline__ float silu_of(float z) {
-  return z * rcp_approx(1.f + exp_minus<T>(z));
+  float a, c;
+  sigmoid_pair(z, a, c);
+  return z * a;
 }
 
 // ---------------------------------------------------------------------- Philox4x32-10

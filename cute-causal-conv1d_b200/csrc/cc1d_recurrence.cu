@@ -51,37 +51,65 @@ constexpr int kBwdStages = 3, kMostStages = 4;
 //
 // 16-bit: four positions share one reciprocal, of the product of their 1 + e (the special
 // function unit would bound the forward otherwise: 4 of its operations per element, now 2.5).
-// So that the product stays finite e is at most 2^30 and a sigmoid at least 2^-30, which is
-// zero next to the other terms of a sum; the three more roundings leave 2^-22, which is enough
-// for silu.  A NaN must not reach the others of its four: the minimum drops it, and GATE puts it
-// back into its own sigmoid (silu has it from z).
+// Its three more roundings leave 2^-22, which is enough for c and for silu.  Where one of a lane's
+// e is above 2^30 or NaN the product might not be finite or the NaN reach its neighbours, and where
+// an fp32 exponent is beyond 87 exp leaves the normal numbers: such a lane's positions are taken
+// one by one.  That shows before any e is there, from the least argument of 8 positions (clamping
+// each e took more instructions, and left a sigmoid of 2^-30 where there should be none).
 template <typename T, int V, bool GATE>
 __device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const Lane<V>& n, Lane<V> (&s)[kRecSteps], Lane<V>* c) {
+  constexpr bool kWide = std::is_same<T, float>::value;
   const Lane<V> one = splat(1.f, n);
-  if constexpr (std::is_same<T, float>::value) {
+  Lane<V> e[kRecSteps];  // fp32: the arguments; 16-bit: exp of the negated ones
+  bool ordinary = true;
+  if constexpr (kWide) {
+#pragma unroll
+    for (int j = 0; j < kRecSteps; ++j) e[j] = add(v[j], n);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float far = 0.f;  // 16-bit: the least of v, fp32: the largest magnitude
+    if constexpr (!kWide) far = el(v[0], i);
+#pragma unroll
+    for (int j = 0; j < kRecSteps; j += 2)
+      far = kWide ? max_nan(far, fabsf(el(e[j], i)), fabsf(el(e[j + 1], i))) : min_nan(far, el(v[j], i), el(v[j + 1], i));
+    ordinary = ordinary && (kWide ? far <= kMostExponent : fmaf(far, -kLog2e, el(n, i)) <= kMostBits);
+  }
+  if (!ordinary) {
 #pragma unroll
     for (int j = 0; j < kRecSteps; ++j) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float e = exp_minus<float>(el(v[j], i) + el(n, i));
-        const float r = rcp_approx(1.f + e);
-        el(s[j], i) = GATE ? fmaf(r, fmaf(-r, e, 1.f - r), r) : r;
-        if constexpr (GATE) el(c[j], i) = e * el(s[j], i);
+        float a, b;
+        if constexpr (kWide) sigmoid_pair<GATE>(el(e[j], i), a, b);
+        else pair_of_exp(ex2_approx(fmaf(el(v[j], i), -kLog2e, el(n, i))), a, b);
+        el(s[j], i) = a;
+        if constexpr (GATE) el(c[j], i) = b;
+      }
+    }
+    return;
+  }
+  if constexpr (kWide) {
+#pragma unroll
+    for (int j = 0; j < kRecSteps; ++j) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float a, b;
+        sigmoid_within<GATE>(el(e[j], i), a, b);
+        el(s[j], i) = a;
+        if constexpr (GATE) el(c[j], i) = b;
       }
     }
   } else {
 #pragma unroll
     for (int q = 0; q < kRecSteps; q += 4) {
-      Lane<V> e[4], d[4], raw[4];
+      Lane<V> d[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        e[j] = fma(v[q + j], splat(-kLog2e, n), n);
+        e[q + j] = fma(v[q + j], splat(-kLog2e, n), n);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          el(raw[j], i) = ex2_approx(el(e[j], i));
-          el(e[j], i) = fminf(el(raw[j], i), 1073741824.f);
-        }
-        d[j] = add(e[j], one);
+        for (int i = 0; i < V; ++i) el(e[q + j], i) = ex2_approx(el(e[q + j], i));
+        d[j] = add(e[q + j], one);
       }
       const Lane<V> lo = mul(d[0], d[1]), hi = mul(d[2], d[3]);
       Lane<V> r = mul(lo, hi);
@@ -94,12 +122,9 @@ __device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const La
       s[q + 3] = mul(rhi, d[2]);
       if constexpr (GATE) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          Lane<V>& a = s[q + j];
-          a = fma(a, sub(sub(one, a), mul(e[j], a)), a);
-#pragma unroll
-          for (int i = 0; i < V; ++i) el(a, i) = max_nan(el(a, i), -el(raw[j], i));
-          c[q + j] = mul(e[j], a);
+        for (int j = q; j < q + 4; ++j) {
+          c[j] = mul(e[j], s[j]);
+          s[j] = fma(s[j], sub(sub(one, s[j]), c[j]), s[j]);
         }
       }
     }
