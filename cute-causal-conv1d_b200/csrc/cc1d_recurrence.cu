@@ -40,12 +40,12 @@ namespace {
 template <int SKEW, int LAYOUT, bool CLUSTER> constexpr int kFwdStages = CLUSTER || (SKEW && LAYOUT != kLayoutRows) ? 3 : 4;
 constexpr int kBwdStages = 3, kMostStages = 4;
 
-// s = sigmoid(v + bias) at a warp's 8 positions, and with GATE (where they weight a state) also
-// c = 1 - s = e s, e = exp(-v - bias).  For 16-bit tensors -v log2(e) = v m + n with m = -log2(e),
+// s = sigmoid(v + bias) at a warp's 8 positions, and if wanted c = 1 - s = e s, e = exp(-v - bias).
+// GATE: they weight a state.  For 16-bit tensors -v log2(e) = v m + n with m = -log2(e),
 // for fp32 n is added to v.
 //
-// 1 - s by subtraction would leave few bits of a slow channel's c (2e-3 off at v = 10, all of them
-// lost from 17 on); e s is relative to itself.  The same channel multiplies its state by thousands
+// 1 - s by subtraction would leave few bits of a slow channel's c, or of silu'(z) = s + z s c where
+// z is large (2e-3 off at v = 10, all of them lost from 17 on); e s is relative to itself.  A slow channel multiplies its state by thousands
 // of s, so the reciprocal's error is taken out with one step of Newton's iteration on the residual
 // 1 - s - e s: s is then rounded as near to one as fp32 allows, about 2^-25 of it.
 //
@@ -56,8 +56,9 @@ constexpr int kBwdStages = 3, kMostStages = 4;
 // an fp32 exponent is beyond 87 exp leaves the normal numbers: such a lane's positions are taken
 // one by one.  That shows before any e is there, from the least argument of 8 positions (clamping
 // each e took more instructions, and left a sigmoid of 2^-30 where there should be none).
-template <typename T, int V, bool GATE>
+template <typename T, int V, bool GATE, bool C>
 __device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const Lane<V>& n, Lane<V> (&s)[kRecSteps], Lane<V>* c) {
+  static_assert(C || !GATE, "the residual is taken from c");
   constexpr bool kWide = std::is_same<T, float>::value;
   const Lane<V> one = splat(1.f, n);
   Lane<V> e[kRecSteps];  // fp32: the arguments; 16-bit: exp of the negated ones
@@ -84,7 +85,7 @@ __device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const La
         if constexpr (kWide) sigmoid_pair<GATE>(el(e[j], i), a, b);
         else pair_of_exp(ex2_approx(fmaf(el(v[j], i), -kLog2e, el(n, i))), a, b);
         el(s[j], i) = a;
-        if constexpr (GATE) el(c[j], i) = b;
+        if constexpr (C) el(c[j], i) = b;
       }
     }
     return;
@@ -97,7 +98,7 @@ __device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const La
         float a, b;
         sigmoid_within<GATE>(el(e[j], i), a, b);
         el(s[j], i) = a;
-        if constexpr (GATE) el(c[j], i) = b;
+        if constexpr (C) el(c[j], i) = b;
       }
     }
   } else {
@@ -120,12 +121,10 @@ __device__ __forceinline__ void sigmoids(const Lane<V> (&v)[kRecSteps], const La
       s[q + 1] = mul(rlo, d[0]);
       s[q + 2] = mul(rhi, d[3]);
       s[q + 3] = mul(rhi, d[2]);
-      if constexpr (GATE) {
 #pragma unroll
-        for (int j = q; j < q + 4; ++j) {
-          c[j] = mul(e[j], s[j]);
-          s[j] = fma(s[j], sub(sub(one, s[j]), c[j]), s[j]);
-        }
+      for (int j = q; j < q + 4; ++j) {
+        if constexpr (C) c[j] = mul(e[j], s[j]);
+        if constexpr (GATE) s[j] = fma(s[j], sub(sub(one, s[j]), c[j]), s[j]);
       }
     }
   }
@@ -416,7 +415,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, gb);
     {
       L gc[kRecSteps];
-      sigmoids<T, V, true>(ga, nb, ga, gc);
+      sigmoids<T, V, true, true>(ga, nb, ga, gc);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) gb[j] = mul(gc[j], gb[j]);
     }
@@ -451,7 +450,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_fwd_kernel(const __grid_co
     auto silu = [&] {
       L z[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(zt, xt), w, lane, z);
-      sigmoids<T, V, false>(z, splat(0.f, L{}), zs, nullptr);
+      sigmoids<T, V, false, false>(z, splat(0.f, L{}), zs, nullptr);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) zs[j] = mul(zs[j], z[j]);
     };
@@ -649,7 +648,7 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     {
       L g[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now, like<SKEW>(gt, xt), w, lane, g);
-      sigmoids<T, V, true>(g, nb, ga, gc);
+      sigmoids<T, V, true, true>(g, nb, ga, gc);
       if (valid != 0xffu) {  // and hand the gradient on as it is, whatever the bias
 #pragma unroll
         for (int j = 0; j < kRecSteps; ++j)
@@ -663,14 +662,14 @@ __global__ void __launch_bounds__(kRecThreads, 4) rec_bwd_kernel(const __grid_co
     read_steps<T, LAYOUT, SKEW>(now + C::kBytes, xt, w, lane, x);
     read_steps<T, LAYOUT, SKEW>(now + 2 * C::kBytes, like<SKEW>(yt, xt), w, lane, gy);
     if constexpr (Z) {
-      L z[kRecSteps], s[kRecSteps];
+      L z[kRecSteps], s[kRecSteps], c[kRecSteps];
       read_steps<T, LAYOUT, SKEW>(now + 3 * C::kBytes, like<SKEW>(zt, xt), w, lane, z);
-      sigmoids<T, V, false>(z, splat(0.f, L{}), s, nullptr);
+      sigmoids<T, V, false, true>(z, splat(0.f, L{}), s, c);
 #pragma unroll
       for (int j = 0; j < kRecSteps; ++j) {
-        // silu(z) = z s and silu'(z) = s + z s (1 - s), s = sigmoid(z)
+        // silu(z) = z s and silu'(z) = s + z s c, s = sigmoid(z), c = 1 - s
         const L zs = mul(z[j], s[j]);
-        dz[j] = mul(gy[j], fma(zs, sub(splat(1.f, L{}), s[j]), s[j]));
+        dz[j] = mul(gy[j], fma(zs, c[j], s[j]));
         gy[j] = mul(gy[j], zs);
       }
     }

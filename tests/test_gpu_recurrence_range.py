@@ -119,10 +119,11 @@ def test_a_reset_leaves_nothing_behind(dtype, layout):
 # ------------------------------------------------------------- output gates of any size
 ORDINARY = [-1.5, 0.5, 2.0, 5.0]
 CLOSED = [-10.0, -19.0, -22.0, -30.0, -60.0, -100.0, -1e3, -6e4]
+OPEN = [10.0, 20.0, 40.0, 1e3, 1e4, 6e4]
 
 
 def _gates(dtype):
-    return torch.tensor([*ORDINARY, *CLOSED, torch.finfo(dtype).min])
+    return torch.tensor([*ORDINARY, *CLOSED, torch.finfo(dtype).min, *OPEN])
 
 
 @pytest.mark.parametrize("layout", LAYOUTS)
