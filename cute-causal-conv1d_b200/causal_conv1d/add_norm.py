@@ -38,6 +38,9 @@ def dropout_add_rms_norm_fn(x, weight, residual=None, eps=1e-5, dropout_p=0.0, r
     dropout_p: probability of dropping an element of x (0 outside training).  rng_state: (2,)
     int64 on x's device, a seed and an offset; the same state gives the same mask, whatever
     the strides (None draws one from the device's default generator).
+
+    Gradients flow back to x, weight and residual.  There is no second derivative and no
+    forward-mode one: both raise.
     """
     return _block.add_norm(x, weight, residual, eps, dropout_p, rng_state, residual_in_fp32)
 

@@ -46,6 +46,9 @@ def gated_recurrence_fn(x, gate, z=None, gate_bias=None, seq_idx=None, initial_s
     returned); num_sequences is needed only to return final states without initial ones.
     A negative id is padding: its out is 0 and nothing there is used.  A sequence without
     positions keeps its initial state.
+
+    Gradients flow back to x, gate, z, gate_bias and initial_states.  There is no second
+    derivative and no forward-mode one: both raise.
     """
     out, final = _block.recurrence(x, gate, z, gate_bias, seq_idx, initial_states, return_final_states,
                                    -1 if num_sequences is None else num_sequences)

@@ -98,6 +98,17 @@ Tensor fp32(at::IntArrayRef shape, const Tensor& like) {
   return at::empty(shape, like.options().dtype(at::kFloat));
 }
 
+// Refuses forward-mode tangents: a call that dropped one would pass for a function that does not
+// depend on that input.
+void no_tangents(const char* what, std::initializer_list<const Tensor*> all) {
+  for (const Tensor* t : all) {
+    if (!t->defined() || !t->_fw_grad(0).defined()) continue;
+    py::gil_scoped_acquire gil;
+    PyErr_SetString(PyExc_NotImplementedError, (std::string(what) + " has no forward-mode derivative").c_str());
+    throw py::error_already_set();
+  }
+}
+
 // The gradients of a node whose backward has no derivative of its own: a graph of them leads
 // to `inputs` through a node that raises.
 variable_list once(variable_list grads, const variable_list& inputs) {
@@ -267,6 +278,7 @@ std::tuple<Tensor, Tensor> recurrence(const Tensor& x, const Tensor& gate, const
                                       const Opt& seq_idx, const Opt& init, bool return_final,
                                       int64_t num_sequences) {
   const Tensor tz = or_none(z), tb = or_none(bias), ti = or_none(init);
+  no_tangents("gated_recurrence_fn", {&x, &gate, &tz, &tb, &ti});
   if (tracked({&x, &gate, &tz, &tb, &ti})) {
     const auto r = RecurrenceNode::apply(x, gate, z, bias, seq_idx, init, return_final, num_sequences);
     return {r[0], return_final ? r[1] : Tensor()};
@@ -282,6 +294,7 @@ Tensor recurrence_update(const Tensor& x, const Tensor& state, const Tensor& gat
   const Tensor tz = or_none(z), tb = or_none(bias);
   Tensor ti = or_none(index);
   if (ti.defined() && ti.scalar_type() != at::kInt) ti = ti.to(at::kInt);
+  no_tangents("gated_recurrence_update", {&x, &state, &gate, &tz, &tb});
   if (x.dim() != 2) expect_dims("x", x, 3);
   expect_dims("state", state, 2);
   cc1d_recurrence_update_params p = {};
@@ -413,6 +426,7 @@ std::tuple<Tensor, Tensor> add_norm(const Tensor& x, const Tensor& weight, const
                                     double dropout_p, const Opt& rng, bool residual_in_fp32) {
   if (!(dropout_p >= 0.0 && dropout_p < 1.0)) throw py::value_error("dropout_p must be in [0, 1)");
   const Tensor tr = or_none(residual);
+  no_tangents("dropout_add_rms_norm_fn", {&x, &weight, &tr});
   Tensor state = dropout_p > 0.0 ? or_none(rng) : Tensor();
   if (dropout_p > 0.0 && !state.defined())
     state = at::randint(int64_t{1} << 62, {2}, x.options().dtype(at::kLong));
