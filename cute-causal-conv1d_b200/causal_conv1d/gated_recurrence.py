@@ -62,6 +62,9 @@ def gated_recurrence_update(x, state, gate, z=None, gate_bias=None, state_indice
     state_indices (batch,) int32 a pool (nstates, dim) of which batch row b uses row
     state_indices[b]; an index outside the pool is padding (zero output, no state
     touched), and no row may be named twice.  Returns out with x's shape.
+
+    It has no derivative: a backward pass that reaches out raises, a state that requires grad
+    is refused outside torch.no_grad(), and the state never carries a graph.
     """
     return _block.recurrence_update(x, state, gate, z, gate_bias, state_indices)
 

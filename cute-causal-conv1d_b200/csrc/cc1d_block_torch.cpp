@@ -109,18 +109,19 @@ void no_tangents(const char* what, std::initializer_list<const Tensor*> all) {
   }
 }
 
-// The gradients of a node whose backward has no derivative of its own: a graph of them leads
-// to `inputs` through a node that raises.
-variable_list once(variable_list grads, const variable_list& inputs) {
-  if (!at::GradMode::is_enabled()) return grads;
-  auto node = std::make_shared<torch::autograd::Error>(
-      "trying to differentiate twice a function that was marked with once_differentiable",
-      torch::autograd::collect_next_edges(inputs));
-  for (Tensor& g : grads)
-    if (g.defined()) {
-      g = g.detach();
-      torch::autograd::set_history(g, node);
+// Makes results lead to `inputs` through a node that raises `why` when a derivative is asked for.
+void no_derivative(variable_list& results, const variable_list& inputs, const char* why) {
+  auto node = std::make_shared<torch::autograd::Error>(why, torch::autograd::collect_next_edges(inputs));
+  for (Tensor& r : results)
+    if (r.defined()) {
+      r = r.detach();
+      torch::autograd::set_history(r, node);
     }
+}
+// The gradients of a node whose backward has no derivative of its own.
+variable_list once(variable_list grads, const variable_list& inputs) {
+  if (at::GradMode::is_enabled())
+    no_derivative(grads, inputs, "trying to differentiate twice a function that was marked with once_differentiable");
   return grads;
 }
 
@@ -289,30 +290,42 @@ std::tuple<Tensor, Tensor> recurrence(const Tensor& x, const Tensor& gate, const
   return {out, final};
 }
 
-Tensor recurrence_update(const Tensor& x, const Tensor& state, const Tensor& gate, const Opt& z, const Opt& bias,
-                         const Opt& index) {
-  const Tensor tz = or_none(z), tb = or_none(bias);
-  Tensor ti = or_none(index);
-  if (ti.defined() && ti.scalar_type() != at::kInt) ti = ti.to(at::kInt);
-  no_tangents("gated_recurrence_update", {&x, &state, &gate, &tz, &tb});
+Tensor update_tokens(const Tensor& x, const Tensor& state, const Tensor& gate, const Tensor& z, const Tensor& bias,
+                     Tensor index) {
+  at::NoGradGuard no_grad;
+  if (index.defined() && index.scalar_type() != at::kInt) index = index.to(at::kInt);
   if (x.dim() != 2) expect_dims("x", x, 3);
   expect_dims("state", state, 2);
   cc1d_recurrence_update_params p = {};
   p.batch = x.size(0), p.dim = x.size(1), p.seqlen = x.dim() == 2 ? 1 : x.size(2);
-  p.nstates = ti.defined() ? state.size(0) : p.batch;
+  p.nstates = index.defined() ? state.size(0) : p.batch;
   expect("gate", gate, x.sizes());
-  expect("z", tz, x.sizes());
-  expect("gate_bias", tb, {p.dim});
+  expect("z", z, x.sizes());
+  expect("gate_bias", bias, {p.dim});
   expect("state", state, {p.nstates, p.dim});
-  expect("state_indices", ti, {p.batch});
-  one_device({&x, &gate, &tz, &tb, &state, &ti});
-  at::NoGradGuard no_grad;
+  expect("state_indices", index, {p.batch});
+  one_device({&x, &gate, &z, &bias, &state, &index});
   Tensor out = at::empty_like(x);
-  p.x = describe(x), p.gate = describe(gate), p.z = describe(tz), p.bias = describe(tb);
-  p.state = describe(state), p.state_indices = describe(ti), p.out = describe(out);
+  p.x = describe(x), p.gate = describe(gate), p.z = describe(z), p.bias = describe(bias);
+  p.state = describe(state), p.state_indices = describe(index), p.out = describe(out);
   Launch launch(x);
   check(cc1d_recurrence_update_launch(&p, launch.stream));
+  // a graph that saved this state notices; states made in inference mode have no version
+  if (x.numel() > 0 && !state.is_inference()) torch::autograd::impl::bump_version(state);
   return out;
+}
+
+Tensor recurrence_update(const Tensor& x, const Tensor& state, const Tensor& gate, const Opt& z, const Opt& bias,
+                         const Opt& index) {
+  const Tensor tz = or_none(z), tb = or_none(bias);
+  no_tangents("gated_recurrence_update", {&x, &state, &gate, &tz, &tb});
+  if (tracked({&state}))
+    throw std::runtime_error("gated_recurrence_update overwrites state and has no derivative: a state that requires "
+                             "grad needs torch.no_grad()");
+  variable_list out = {update_tokens(x, state, gate, tz, tb, or_none(index))};
+  if (tracked({&x, &gate, &tz, &tb}))
+    no_derivative(out, {x, gate, tz, tb}, "gated_recurrence_update has no derivative: use gated_recurrence_fn to train");
+  return out[0];
 }
 
 // --------------------------------------------------------------------------- add_norm
