@@ -5,7 +5,17 @@
 
 namespace cc1d {
 
-// The largest (smallest) of three, or NaN if one is.
+// The largest (smallest) of two or three, or NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -17,13 +27,13 @@ __device__ __forceinline__ float min_nan(float a, float b, float c) {
   return r;
 }
 
-// Within +-87 neither exp nor 1 / (1 + exp) leaves the normal numbers; beyond, a sigmoid is 0 or 1
-// to within e^-87 = 1.6e-38.  An e of at most 2^30 has finite products of four 1 + e.
+// Within +-87 neither exp nor 1 / (1 + exp) leaves the normal numbers.  An e of at most 2^30 has
+// finite products of four 1 + e.
 constexpr float kMostExponent = 87.f, kMostBits = 30.f;
 
-// exp(-u) for |u| <= kMostExponent: 2^v by the hardware's approximation (relative error about
-// 2^-22) and what the rounding of v loses: -u log2(e) = t + r, with r from two fused
-// multiply-adds (the second for the part of log2(e) below fp32), and 2^r = 1 + r ln 2 to 2^-40.
+// exp(-u) for |u| <= 88: 2^v by the hardware's approximation (relative error about 2^-22) and what
+// the rounding of v loses: -u log2(e) = t + r, with r from two fused multiply-adds (the second for
+// the part of log2(e) below fp32), and 2^r = 1 + r ln 2 to 2^-40.
 __device__ __forceinline__ float exp_minus(float u) {
   constexpr double kLog2eExact = 1.4426950408889634074;
   constexpr float kLow = static_cast<float>(kLog2eExact - static_cast<double>(kLog2e));
@@ -32,45 +42,41 @@ __device__ __forceinline__ float exp_minus(float u) {
   const float e = ex2_approx(t);
   return fmaf(e, r * 0.693147181f, e);
 }
+// Any u, NaN included, brought within +-88: exp(-88) is flushed to zero, as is 1 / (1 + exp(88)).
+__device__ __forceinline__ float clamp_exponent(float u) { return min_nan(max_nan(u, -88.f), 88.f); }
 
-// A step of Newton's iteration for s = 1 / (1 + e), whose residual takes no rounding of 1 + e.
-__device__ __forceinline__ float newton(float s, float e) { return fmaf(s, fmaf(-s, e, 1.f - s), s); }
-
-// a = 1 / (1 + e) and c = e / (1 + e), for any e >= 0 that exp may give, infinite or NaN as well.
+// a = 1 / (1 + e) and c = e / (1 + e), to 2^-22 or, with NEWTON, a step of Newton's iteration on
+// the residual 1 - a - e a, which takes no rounding of 1 + e, to 2^-24.
+template <bool NEWTON>
 __device__ __forceinline__ void pair_of_exp(float e, float& a, float& c) {
   a = rcp_approx(1.f + e);
-  if (e <= 1073741824.f) {  // 2^kMostBits
-    a = newton(a, e);
-    c = e * a;
-  } else {
-    c = 1.f - a;
-  }
-}
-
-// a = sigmoid(u) and c = 1 - a = sigmoid(-u), each to full relative precision (to 2^-22 without
-// NEWTON), for |u| <= kMostExponent.
-template <bool NEWTON = true>
-__device__ __forceinline__ void sigmoid_within(float u, float& a, float& c) {
-  const float e = exp_minus(u);
-  a = rcp_approx(1.f + e);
-  if constexpr (NEWTON) a = newton(a, e);
+  if constexpr (NEWTON) a = fmaf(a, fmaf(-a, e, 1.f - a), a);
   c = e * a;
 }
-// The same for any u, NaN included: exactly 0 and 1 beyond +-kMostExponent.
-template <bool NEWTON = true>
+
+// a = sigmoid(u) and c = 1 - a = sigmoid(-u) for any u, NaN included, each to full relative
+// precision and down to zero.
+template <bool NEWTON>
 __device__ __forceinline__ void sigmoid_pair(float u, float& a, float& c) {
-  if (fabsf(u) <= kMostExponent) {
-    sigmoid_within<NEWTON>(u, a, c);
-  } else {
-    a = u > 0.f ? 1.f : u < 0.f ? 0.f : u;
-    c = 1.f - a;
-  }
+  pair_of_exp<NEWTON>(exp_minus(clamp_exponent(u)), a, c);
+  if (u < -kMostExponent) a = 0.f, c = 1.f;
+}
+// The same for 16-bit tensors, from t = -u log2(e), whose rounding is left in exp.
+__device__ __forceinline__ void sigmoid_pair_of_bits(float t, float& a, float& c) {
+  pair_of_exp<true>(ex2_approx(min_nan(t, 126.f)), a, c);
+  if (t > 125.f) a = 0.f, c = 1.f;
+}
+template <typename T>
+__device__ __forceinline__ void sigmoid_pair_of(float u, float& a, float& c) {
+  if constexpr (std::is_same<T, float>::value) sigmoid_pair<true>(u, a, c);
+  else sigmoid_pair_of_bits(-kLog2e * u, a, c);
 }
 
+// z sigmoid(z); where exp(-z) is infinite, or large enough for its reciprocal to be flushed, zero.
+template <typename T>
 __device__ __forceinline__ float silu_of(float z) {
-  float a, c;
-  sigmoid_pair(z, a, c);
-  return z * a;
+  if constexpr (std::is_same<T, float>::value) return z * rcp_approx(1.f + exp_minus(clamp_exponent(z)));
+  else return z * rcp_approx(1.f + ex2_approx(-kLog2e * z));
 }
 
 // ---------------------------------------------------------------------- Philox4x32-10

@@ -1,8 +1,7 @@
 // The gated recurrence for a few tokens of each row against a pool of fp32 states (sm_100a).
 //
 // One thread takes VEC neighbouring channels of one batch row through its tokens, from the
-// state it reads to the one it writes back, so a state is read and written once.  The fp32
-// exponential serves all types: the states are fp32, and its instructions do not show in the time.  Bound by
+// state it reads to the one it writes back, so a state is read and written once.  Bound by
 // HBM for many rows and by the launch for few.  VEC = 4 (8 or 16 bytes of each tensor, 16 of
 // the state) where every tensor has unit channel stride and that alignment: (128, 8192) bf16
 // in a pool of 160 rows takes 4.7 us (55% of the copy rate, launches back to back), channel by
@@ -52,9 +51,9 @@ __global__ void __launch_bounds__(kThreads) rec_update_kernel(const RecUpdateArg
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
       float ga, gc;
-      sigmoid_pair(g[v] + bias[v], ga, gc);
+      sigmoid_pair_of<T>(g[v] + bias[v], ga, gc);
       h[v] = fmaf(ga, h[v], gc * x[v]);
-      y[v] = a.z.data ? h[v] * silu_of(z[v]) : h[v];
+      y[v] = a.z.data ? h[v] * silu_of<T>(z[v]) : h[v];
     }
     store_at<T, VEC>(a.out, b, d, l, y);
     if (++l == a.seqlen) break;
