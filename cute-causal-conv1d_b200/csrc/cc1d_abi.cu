@@ -9,6 +9,7 @@
 #include <string>
 
 #include "cc1d_launch.h"
+#include "cc1d_smem.h"
 #include "cc1d_update_launch.h"
 
 namespace cc1d {
@@ -383,22 +384,7 @@ cc1d_status check_conv_common(int64_t B, int64_t D, int64_t L, int64_t W, const 
 void set_last_error(const char* msg) { g_last_error = msg; }
 void count_launches(int n) { g_launches.fetch_add(n); }
 
-cudaError_t allow_dynamic_smem(const void* kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return cudaSuccess;
-  static std::mutex mu;
-  static struct Entry { const void* k; int dev; size_t bytes; } done[256];
-  static int n = 0;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < n; ++i)
-    if (done[i].k == kernel && done[i].dev == dev && done[i].bytes >= bytes) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-  if (e != cudaSuccess) return e;
-  if (n < 256) done[n++] = Entry{kernel, dev, bytes};
-  return cudaSuccess;
-}
+cudaError_t allow_dynamic_smem(const void* kernel, size_t bytes) { return raise_smem_limit(kernel, bytes); }
 
 }  // namespace cc1d
 

@@ -101,7 +101,7 @@ const void* rowwalk_kernel_ptr_f16(bool bwd, size_t smem);
 const void* rowwalk_kernel_ptr_bf16(bool bwd, size_t smem);
 
 // Lets `kernel` use `bytes` of dynamic shared memory (above the 48 KB default) on the
-// current device; the attribute is set once per kernel and device.
+// current device; a kernel's limit is only ever raised.
 cudaError_t allow_dynamic_smem(const void* kernel, size_t bytes);
 
 cudaError_t reduce_rows_f32(const ConvArgs&, int width, cudaStream_t);
