@@ -59,9 +59,10 @@ def gated_recurrence_update(x, state, gate, z=None, gate_bias=None, state_indice
     """One decode step (or a few tokens) of the recurrence; ``state`` is updated in place.
 
     x, gate, z: (batch, dim) or (batch, dim, seqlen).  state: (batch, dim) fp32, or with
-    state_indices (batch,) int32 a pool (nstates, dim) of which batch row b uses row
+    state_indices (batch,) a pool (nstates, dim) of which batch row b uses row
     state_indices[b]; an index outside the pool is padding (zero output, no state
-    touched), and no row may be named twice.  Returns out with x's shape.
+    touched), and no row may be named twice.  The indices are int32; other signed integers
+    and uint8 are converted.  Returns out with x's shape.
 
     It has no derivative: a backward pass that reaches out raises, a state that requires grad
     is refused outside torch.no_grad(), and the state never carries a graph.

@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
+#include <limits>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -290,10 +291,23 @@ std::tuple<Tensor, Tensor> recurrence(const Tensor& x, const Tensor& gate, const
   return {out, final};
 }
 
+// State indices as the C ABI takes them.  What 32 bits do not hold is outside any pool, and has
+// to stay so.
+Tensor indices32(const Tensor& t) {
+  if (!t.defined() || t.scalar_type() == at::kInt) return t;
+  switch (t.scalar_type()) {
+    case at::kLong: return t.clamp(-1, std::numeric_limits<int32_t>::max()).to(at::kInt);
+    case at::kShort:
+    case at::kChar:
+    case at::kByte: return t.to(at::kInt);
+    default: throw py::type_error(std::string("state_indices must be an integer tensor, got ") + c10::toString(t.scalar_type()));
+  }
+}
+
 Tensor update_tokens(const Tensor& x, const Tensor& state, const Tensor& gate, const Tensor& z, const Tensor& bias,
-                     Tensor index) {
+                     const Tensor& wide_index) {
   at::NoGradGuard no_grad;
-  if (index.defined() && index.scalar_type() != at::kInt) index = index.to(at::kInt);
+  const Tensor index = indices32(wide_index);
   if (x.dim() != 2) expect_dims("x", x, 3);
   expect_dims("state", state, 2);
   cc1d_recurrence_update_params p = {};
