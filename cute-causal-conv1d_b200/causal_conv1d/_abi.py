@@ -338,7 +338,8 @@ class _Missing:
     def __getattr__(self, name):
         raise ImportError(
             "causal_conv1d/_block.so cannot be loaded: build it with `python cute-causal-conv1d_b200/cc1d_build.py` "
-            f"against the installed PyTorch. causal_conv1d has no CPU fallback. ({self._reason})"
+            "against the installed PyTorch (with --force if that has changed since). causal_conv1d has no CPU "
+            f"fallback. ({self._reason})"
         )
 
 

@@ -8,12 +8,13 @@ with nvcc, in parallel; the per-element-type kernel files are compiled once per 
 The library is written next to the Python package (``causal_conv1d/libcc1d_b200.so``),
 in the source tree, and is rebuilt only when a source or header is newer.  So is the
 binding, which g++ compiles against the headers of the installed PyTorch; the library itself
-needs no PyTorch.
+needs no PyTorch, and is built alone where there is none.
 """
 
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -63,11 +64,16 @@ def _inputs():
     return files
 
 
+def has_torch() -> bool:
+    return importlib.util.find_spec("torch") is not None
+
+
 def up_to_date() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(BINDING):
+    built = [LIB, BINDING] if has_torch() else [LIB]
+    if not all(os.path.exists(f) for f in built):
         return False
-    lib_mtime = min(os.path.getmtime(LIB), os.path.getmtime(BINDING))
-    return all(os.path.getmtime(f) <= lib_mtime for f in _inputs())
+    oldest = min(os.path.getmtime(f) for f in built)
+    return all(os.path.getmtime(f) <= oldest for f in _inputs())
 
 
 def compile_binding(obj: str) -> None:
@@ -119,9 +125,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
     workers = max(1, min(len(UNITS), os.cpu_count() or 4))
     binding_obj = os.path.join(BUILD, "cc1d_block_torch.o")
     with ThreadPoolExecutor(workers) as pool:
-        binding = pool.submit(compile_binding, binding_obj)
+        binding = pool.submit(compile_binding, binding_obj) if has_torch() else None
         logs = list(pool.map(compile_unit, UNITS))
-        binding.result()
     if verbose:
         for log in logs:
             sys.stderr.write(log)
@@ -132,7 +137,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB)
-    link_binding(binding_obj)
+    if binding is None:
+        sys.stderr.write("cc1d_build: no PyTorch here, so its binding _block.so is not built\n")
+    else:
+        binding.result()
+        link_binding(binding_obj)
     return LIB
 
 
