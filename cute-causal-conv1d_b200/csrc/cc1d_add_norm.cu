@@ -13,9 +13,12 @@
 // computed where it is used, forward and backward.  CTAs stay (a few per SM) and load their
 // next row before they work on the present one.
 //
-// Bound by HBM without dropout (65536 x 4096 bf16: forward 338 us, backward 424 us, 98% of the
-// copy rate), by the mask's integer arithmetic with it (420 and 562 us).  Rows too wide for the registers (16384 columns, backward 8192, and 8192 in
-// fp32 or off the 16-byte alignment) are read a second time, from L2.
+// Bound by HBM without dropout (65536 x 4096 bf16: forward 334 us, 99% of the copy rate; backward
+// 362 us, 92%, with dx and dresidual one tensor as the Python function makes them), by the mask's
+// integer arithmetic with it (419 and 562 us).  Rows too wide for the registers (more than 16384
+// columns, backward 8192, and 8192 in fp32 or off the 16-byte alignment) are read a second time,
+// from L2, and move element by element whatever their alignment: 8192 x 20480 bf16 forward 442 us
+// (47%), 8192 x 16384 backward 843 us (20%).
 #include "cc1d_block_launch.h"
 #include "cc1d_block_math.cuh"
 

@@ -106,8 +106,11 @@ int64_t clusters_at_a_time(RecArgs a, bool bwd) {
 //   .95 + .08 cluster + .42 n
 //
 // and a CTA about 6 to start.  One sequence of 32768 positions and 5120 channels (80 tiles):
-// forward 949 us alone, 664 in twos, 418 in fours, 350 in fives, 409 in eights; backward 490 us
-// in fives, 589 in fours, 671 in sixes.
+// forward 1010 us alone, 684 in twos, 434 in fours, 363 in fives, 359 in sixes, 424 in eights;
+// backward 517 us in fives, 626 in fours, 714 in sixes.  The constants are those of the aligned
+// channel-last kernels of 16-bit tensors with z, but serve all.  Swept over every size, packed,
+// without z, off 16 bytes and with 16 to 256 tiles, the choice was the fastest or within 1% of it;
+// fp32 (1, 2560, 32768) backward takes 435 us in sixes and would take 409 in fives.
 int choose_cluster(RecArgs* a, int64_t tiles, bool bwd) {
   const double sms = sm_count();
   double best = 0;
@@ -136,9 +139,9 @@ int choose_cluster(RecArgs* a, int64_t tiles, bool bwd) {
 
 // Layout, way of moving and cluster of a recurrence.  Rows: every tensor has unit stride along
 // the sequence; all others take the channel-last kernel.  The first of the ways that the tensors
-// allow is the fastest; bf16, 8 sequences of 8192, forward and backward: 382 and 722 us for
-// 4096 channels (kTma), 642 and 1168 us for 4094 (kWords), 748 and 1318 us for 4095 (kHalves),
-// 764 and 1781 us with an offset for each input (kOwn).
+// allow is the fastest; bf16, 8 sequences of 8192, forward and backward: 408 and 718 us for
+// 4096 channels (kTma), 659 and 1248 us for 4094 (kWords), 752 and 1400 us for 4095 (kHalves),
+// 768 and 1586 us with an offset for each input (kOwn).
 cc1d_status rec_plan(RecArgs* a, bool bwd) {
   TensorArg* const all[] = {&a->x, &a->gate, &a->z, bwd ? &a->dout : &a->out, bwd ? &a->dx : nullptr,
                             bwd ? &a->dgate : nullptr, bwd ? &a->dz : nullptr};

@@ -21,11 +21,12 @@
 // take consecutive chunks and send each other the chunks' sums, one exchange per round.  No CTA
 // waits for another outside its cluster, and results do not depend on timing.
 //
-// Bound by HBM in the limit; at this writing by issue slots (29 and 43 instructions per
-// element, with z) and latency: bf16 (8, 4096, 8192) channel-last takes 382 us forward (88%
-// of the copy rate) and 722 us backward (81%), fp32 (8, 4096, 4096) 352 us (95%) and 646 us
-// (90%).  Off the 16-byte alignment, with (8, 4094, 8192), 642 and 1168 us (52 and 50%).  4 warps and 32 positions: more CTAs fit an SM than with 8 warps and 64 (445 us
-// forward), and a warp's 8 positions amortise the exchange better than 4 (545 us).
+// Bound by HBM in the limit; at this writing by issue slots (29 and 45 instructions per
+// element, with z) and latency: bf16 (8, 4096, 8192) channel-last takes 408 us forward (82%
+// of the copy rate) and 718 us backward (81%), fp32 (8, 4096, 4096) 358 us (93%) and 640 us
+// (91%).  Off the 16-byte alignment, with (8, 4094, 8192), 659 and 1248 us (51 and 47%).  4 warps
+// and 32 positions: more CTAs fit an SM than with 8 warps and 64 (445 us forward where this took
+// 405), and a warp's 8 positions amortise the exchange better than 4 (545 us).
 #include <cudaTypedefs.h>
 
 #include "cc1d_recurrence.cuh"

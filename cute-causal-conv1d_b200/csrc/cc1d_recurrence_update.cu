@@ -4,8 +4,8 @@
 // state it reads to the one it writes back, so a state is read and written once.  Bound by
 // HBM for many rows and by the launch for few.  VEC = 4 (8 or 16 bytes of each tensor, 16 of
 // the state) where every tensor has unit channel stride and that alignment: (128, 8192) bf16
-// in a pool of 160 rows takes 4.7 us (55% of the copy rate, launches back to back), channel by
-// channel (8191 of them) 11.1 us; else VEC = 1.
+// in a pool of 160 rows takes 4.4 us (60% of the copy rate, launches back to back), channel by
+// channel (8191 of them) 10.6 us; else VEC = 1.
 #include "cc1d_block_launch.h"
 #include "cc1d_block_math.cuh"
 
