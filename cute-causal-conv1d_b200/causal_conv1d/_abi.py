@@ -97,6 +97,14 @@ SIGNATURES = {
     "cc1d_add_norm_fwd_launch": (c_i32, [c_void_p, c_void_p]),
     "cc1d_add_norm_bwd_workspace_bytes": (c_i64, [c_void_p]),
     "cc1d_add_norm_bwd_launch": (c_i32, [c_void_p, c_void_p]),
+    "cc1d_selective_fwd_workspace_bytes": (c_i64, [c_void_p]),
+    "cc1d_selective_fwd_launch": (c_i32, [c_void_p, c_void_p]),
+    "cc1d_selective_bwd_workspace_bytes": (c_i64, [c_void_p]),
+    "cc1d_selective_bwd_launch": (c_i32, [c_void_p, c_void_p]),
+    "cc1d_selective_update_launch": (c_i32, [c_void_p, c_void_p]),
+    "cc1d_beam_select_workspace_bytes": (c_i64, [c_void_p]),
+    "cc1d_beam_select_launch": (c_i32, [c_void_p, c_void_p]),
+    "cc1d_beam_reorder_launch": (c_i32, [c_void_p, c_void_p]),
     "cc1d_last_error": (ctypes.c_char_p, []),
     "cc1d_status_string": (ctypes.c_char_p, [c_i32]),
     "cc1d_abi_version": (c_i32, []),
@@ -353,6 +361,12 @@ _NONE = (0, 0, 0, 0, 0)  # an absent tensor
 RECURRENCE_PARAMS = struct.Struct("<78q")
 RECURRENCE_UPDATE_PARAMS = struct.Struct("<39q")
 ADD_NORM_PARAMS = struct.Struct("<55q2d")
+SELECTIVE_CHUNK = 32  # CC1D_SELECTIVE_CHUNK
+SELECTIVE_PARAMS = struct.Struct("<117q")
+SELECTIVE_UPDATE_PARAMS = struct.Struct("<64q")
+BEAM_SELECT_PARAMS = struct.Struct("<23q")
+BEAM_ROWS = struct.Struct("<10q")
+BEAM_REORDER_PARAMS = struct.Struct("<14q")
 
 
 def launch_count() -> int:

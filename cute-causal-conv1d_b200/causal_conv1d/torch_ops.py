@@ -24,6 +24,16 @@ them.
   -> (out, residual_out)``
 * ``dropout_add_rms_norm_bwd(x_dtype, residual_out, weight, dout, dresidual_out, eps, dropout_p,
   rng_state) -> (dx, dresidual, dweight)``
+* ``selective_recurrence_fwd(x, delta, A, B, C, D, z, delta_bias, delta_softplus, seq_idx,
+  initial_states, return_final_states, num_sequences, save_checkpoints)
+  -> (out, final_states, checkpoints)``, ``selective_recurrence_bwd(..., checkpoints, dout,
+  dfinal_states, return_dbias, return_dinitial_states)`` -> the list of the gradients of x, delta,
+  A, B, C, D, z, delta_bias and initial_states, empty where there is none, and
+  ``selective_recurrence_update(x, state, delta, A, B, C, D, z, delta_bias, delta_softplus,
+  state_indices) -> out``
+* ``beam_search_select(logits, scores, finished, end_token, num_candidates)
+  -> (scores, parents, tokens)``
+* ``beam_search_reorder(states, parents, state_indices)``: states is a list, mutated
 
 The reference compiles its kernels with the CuTe DSL and registers no torch operators;
 these registrations are this package's equivalent of the C++ extension's op table.
@@ -36,8 +46,10 @@ from torch import Tensor
 
 from causal_conv1d import _abi
 from causal_conv1d import add_norm as _an
+from causal_conv1d import beam_search as _bs
 from causal_conv1d import cpp_functions as _cf
 from causal_conv1d import gated_recurrence as _gr
+from causal_conv1d import selective_recurrence as _sr
 from causal_conv1d.causal_conv1d_varlen import causal_conv1d_fn_varlen_states as _fwd_varlen_states
 from causal_conv1d.causal_conv1d_varlen import causal_conv1d_varlen_states as _varlen_states
 
@@ -203,3 +215,95 @@ def dropout_add_rms_norm_bwd(x_dtype: torch.dtype, residual_out: Tensor, weight:
 def _(x_dtype, residual_out, weight, dout, dresidual_out, eps, dropout_p, rng_state):
     return (residual_out.new_empty(residual_out.shape, dtype=x_dtype), residual_out.new_empty(residual_out.shape),
             weight.new_empty(weight.shape))
+
+
+# ------------------------------------------------- selective recurrence, beam search
+def _state_rows(x, seq_idx, initial_states, num_sequences):
+    return x.shape[0] if seq_idx is None else initial_states.shape[0] if initial_states is not None else num_sequences
+
+
+@torch.library.custom_op("causal_conv1d::selective_recurrence_fwd", mutates_args=())
+def selective_recurrence_fwd(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor | None, z: Tensor | None,
+                             delta_bias: Tensor | None, delta_softplus: bool, seq_idx: Tensor | None,
+                             initial_states: Tensor | None, return_final_states: bool, num_sequences: int,
+                             save_checkpoints: bool) -> tuple[Tensor, Tensor, Tensor]:
+    out, final, checkpoints = _sr.selective_recurrence_fwd_function(
+        x, delta, A, B, C, D, z, delta_bias, delta_softplus, seq_idx, initial_states, return_final_states, num_sequences,
+        save_checkpoints)
+    empty = x.new_empty(_EMPTY, dtype=torch.float32)
+    return out, empty if final is None else final, empty.clone() if checkpoints is None else checkpoints
+
+
+@selective_recurrence_fwd.register_fake
+def _(x, delta, A, B, C, D, z, delta_bias, delta_softplus, seq_idx, initial_states, return_final_states, num_sequences,
+      save_checkpoints):
+    batch, dim, seqlen = x.shape
+    dstate = A.shape[1]
+    n = _state_rows(x, seq_idx, initial_states, num_sequences)
+    final = x.new_empty((n, dim, dstate) if return_final_states else _EMPTY, dtype=torch.float32)
+    kept = (batch, -(-seqlen // _abi.SELECTIVE_CHUNK), dim, -(-dstate // 4) * 4)
+    return _laid_out_like(x), final, x.new_empty(kept if save_checkpoints else _EMPTY, dtype=torch.float32)
+
+
+@torch.library.custom_op("causal_conv1d::selective_recurrence_bwd", mutates_args=())
+def selective_recurrence_bwd(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor | None, z: Tensor | None,
+                             delta_bias: Tensor | None, delta_softplus: bool, seq_idx: Tensor | None,
+                             initial_states: Tensor | None, checkpoints: Tensor, dout: Tensor, dfinal_states: Tensor | None,
+                             return_dbias: bool, return_dinitial_states: bool) -> list[Tensor]:
+    """[dx, ddelta, dA, dB, dC, dD, dz, dbias, dinitial_states]; absent ones are empty."""
+    got = _sr.selective_recurrence_bwd_function(x, delta, A, B, C, D, z, delta_bias, delta_softplus, seq_idx, initial_states,
+                                                checkpoints, dout, dfinal_states, return_dbias, return_dinitial_states)
+    return [x.new_empty(_EMPTY) if g is None else g for g in got]
+
+
+@selective_recurrence_bwd.register_fake
+def _(x, delta, A, B, C, D, z, delta_bias, delta_softplus, seq_idx, initial_states, checkpoints, dout, dfinal_states,
+      return_dbias, return_dinitial_states):
+    def like(t, wanted=True):
+        return x.new_empty(t.shape, dtype=t.dtype) if wanted and t is not None else x.new_empty(_EMPTY)
+
+    along = B.stride(-2) == 1 or B.stride(-1) != 1
+
+    def coefficients(t):
+        return x.new_empty(*t.shape[:1], t.shape[-1], *t.shape[1:-1]).movedim(1, -1) if along else x.new_empty(t.shape)
+
+    init = x.new_empty(initial_states.shape if return_dinitial_states else _EMPTY,
+                       dtype=torch.float32 if return_dinitial_states else x.dtype)
+    dz = _laid_out_like(x) if z is not None else x.new_empty(_EMPTY)
+    return [_laid_out_like(x), _laid_out_like(x), like(A), coefficients(B), coefficients(C), like(D), dz,
+            like(delta_bias, return_dbias), init]
+
+
+@torch.library.custom_op("causal_conv1d::selective_recurrence_update", mutates_args=("state",))
+def selective_recurrence_update(x: Tensor, state: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor | None,
+                                z: Tensor | None, delta_bias: Tensor | None, delta_softplus: bool,
+                                state_indices: Tensor | None) -> Tensor:
+    return _sr.selective_recurrence_update(x, state, delta, A, B, C, D, z, delta_bias, delta_softplus, state_indices)
+
+
+@selective_recurrence_update.register_fake
+def _(x, state, delta, A, B, C, D, z, delta_bias, delta_softplus, state_indices):
+    return torch.empty_like(x)
+
+
+@torch.library.custom_op("causal_conv1d::beam_search_select", mutates_args=())
+def beam_search_select(logits: Tensor, scores: Tensor, finished: Tensor | None, end_token: int | None,
+                       num_candidates: int | None) -> tuple[Tensor, Tensor, Tensor]:
+    return _bs.beam_search_select(logits, scores, finished, end_token, num_candidates)
+
+
+@beam_search_select.register_fake
+def _(logits, scores, finished, end_token, num_candidates):
+    shape = (logits.shape[0], logits.shape[1] if num_candidates is None else num_candidates)
+    return (logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int64),
+            logits.new_empty(shape, dtype=torch.int64))
+
+
+@torch.library.custom_op("causal_conv1d::beam_search_reorder", mutates_args=("states",))
+def beam_search_reorder(states: list[Tensor], parents: Tensor, state_indices: Tensor | None) -> None:
+    _bs.beam_search_reorder(states, parents, state_indices)
+
+
+@beam_search_reorder.register_fake
+def _(states, parents, state_indices):
+    return None

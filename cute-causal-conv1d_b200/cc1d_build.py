@@ -42,10 +42,14 @@ UNITS = [
     ("cc1d_decode.cu", [], "cc1d_decode.o"),
     ("cc1d_static.cu", [], "cc1d_static.o"),
     ("cc1d_block_abi.cu", [], "cc1d_block_abi.o"),
+    ("cc1d_selective_abi.cu", [], "cc1d_selective_abi.o"),
+    ("cc1d_beam.cu", [], "cc1d_beam.o"),
+    ("cc1d_beam_abi.cu", [], "cc1d_beam_abi.o"),
 ] + [
     (src, [f"-DCC1D_DT={dt}"], f"{src[:-3]}_{name}.o")
     for src in ("cc1d_fwd.cu", "cc1d_bwd.cu", "cc1d_rows.cu", "cc1d_rowwalk.cu",
-                "cc1d_recurrence.cu", "cc1d_recurrence_update.cu", "cc1d_add_norm.cu")
+                "cc1d_recurrence.cu", "cc1d_recurrence_update.cu", "cc1d_add_norm.cu",
+                "cc1d_selective_fwd.cu", "cc1d_selective_bwd.cu", "cc1d_selective_update.cu")
     for dt, name in ((0, "f32"), (1, "f16"), (2, "bf16"))
 ]
 

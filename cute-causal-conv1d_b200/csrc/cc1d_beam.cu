@@ -1,0 +1,369 @@
+// Beam search (sm_100a): the best continuations of each request's beams over the vocabulary, and
+// the states that follow the choice.
+#include <climits>
+
+#include "cc1d_beam_launch.h"
+#include "cc1d_block_math.cuh"
+
+namespace cc1d {
+namespace {
+
+// ------------------------------------------------------------------------- selection
+// total[k, v] = scores[k] + logits[k, v] - log sum_w exp(logits[k, w]); the best `candidates` of
+// beams x vocabulary, equal ones by the lowest place.
+//
+// One pass over the logits: each warp walks a strip of a row with the running maximum and sum of
+// the softmax and a sorted list of the strip's best in registers, one or two entries a lane.  An
+// element is looked at one by one only if it beats the list's last entry, which becomes rare
+// after the first steps.  A second kernel joins the strips' lists, by beams, then over beams.
+constexpr int kWarps = kThreads / 32;
+constexpr int kEmpty = INT_MIN;  // below the order of every float
+
+// Order of floats as integers; -0 counts as 0.
+__device__ __forceinline__ int order_of(float f) {
+  const int b = __float_as_int(f + 0.f);
+  return b >= 0 ? b : b ^ 0x7fffffff;
+}
+__device__ __forceinline__ float value_of(int o) { return __int_as_float(o >= 0 ? o : o ^ 0x7fffffff); }
+
+// The `n` best of what a warp has seen, sorted: entry 32 q + lane in (key[q], at[q]).
+template <int Q>
+struct Best {
+  int key[Q], at[Q], last, n;
+  __device__ __forceinline__ void start(int count) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) key[q] = kEmpty, at[q] = INT_MAX;
+    n = count;
+    last = kEmpty;
+  }
+  // k > last, and behind all entries of the same key
+  __device__ __forceinline__ void insert(int k, int place, int lane) {
+    int pos = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) pos += __popc(__ballot_sync(~0u, key[q] >= k));
+#pragma unroll
+    for (int q = Q - 1; q >= 0; --q) {
+      int ku = __shfl_up_sync(~0u, key[q], 1), au = __shfl_up_sync(~0u, at[q], 1);
+      if (q > 0) {
+        const int kl = __shfl_sync(~0u, key[q - 1], 31), al = __shfl_sync(~0u, at[q - 1], 31);
+        if (lane == 0) ku = kl, au = al;
+      }
+      const int i = q * 32 + lane;
+      if (i > pos) key[q] = ku, at[q] = au;
+      else if (i == pos) key[q] = k, at[q] = place;
+    }
+    int l = key[0];
+#pragma unroll
+    for (int q = 1; q < Q; ++q)
+      if ((n - 1) / 32 == q) l = key[q];
+    last = __shfl_sync(~0u, l, (n - 1) & 31);
+  }
+};
+
+// The running maximum m and sum s + low of exp(x - m) of a lane or a part of a row.
+struct Soft {
+  float m = -INFINITY, s = 0.f, low = 0.f;
+};
+__device__ __forceinline__ float exp_of(float d) { return ex2_approx(d * kLog2e); }
+__device__ __forceinline__ void raise(Soft& a, float m) {
+  if (m > a.m) {
+    const float f = a.m > -INFINITY ? exp_of(a.m - m) : 0.f;
+    a.s *= f;
+    a.low *= f;
+    a.m = m;
+  }
+}
+// s + low with the rounding of the sum kept (Knuth's two-sum)
+__device__ __forceinline__ void add_to(Soft& a, float v) {
+  const float t = a.s + v, w = t - a.s;
+  a.low += (a.s - (t - w)) + (v - w);
+  a.s = t;
+}
+
+template <typename T, int Q>
+struct Strip {
+  Best<Q> best;
+  Soft soft;
+  int lane;
+  // E neighbouring elements of each lane from place `at` on, in the order of the lanes; `has` of them
+  template <int E>
+  __device__ __forceinline__ void step(const float (&x)[E], int at, int has) {
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
+    raise(soft, top);
+    const float m = soft.m > -INFINITY ? soft.m : 0.f;
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += exp_of(x[e] - m);
+    add_to(soft, s);
+    unsigned todo = __ballot_sync(~0u, has > 0 && order_of(top) > best.last);
+    while (todo) {
+      const int from = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const int start = __shfl_sync(~0u, at, from), count = __shfl_sync(~0u, has, from);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int k = order_of(__shfl_sync(~0u, x[e], from));
+        if (e < count && k > best.last) best.insert(k, start + e, lane);
+      }
+      todo &= __ballot_sync(~0u, order_of(top) > best.last);
+    }
+  }
+};
+
+template <typename T, int Q>
+__global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectArgs a) {
+  constexpr int E = 16 / sizeof(T);
+  __shared__ int2 lists[kWarps][Q * 32];
+  __shared__ Soft softs[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  const int n = static_cast<int>(a.candidates);
+  grid_dependency_wait();
+  const T* x = static_cast<const T*>(a.logits) + (row / a.beams) * a.logits_s0 + (row % a.beams) * a.logits_s1;
+  const int64_t begin = part * a.part, end = begin + a.part < a.vocab ? begin + a.part : a.vocab;
+  const int64_t strip = (end - begin + kWarps - 1) / kWarps;
+  int64_t i = begin + warp * strip;
+  const int64_t stop = i + strip < end ? i + strip : end;
+  Strip<T, Q> w;
+  w.lane = lane;
+  w.best.start(n);
+  // up to the first 16-byte boundary, element by element
+  const int64_t past = reinterpret_cast<uintptr_t>(x + i) % 16 / sizeof(T);
+  const int64_t head = past ? E - past : 0;
+  if (i < stop && head) {
+    const int64_t count = head < stop - i ? head : stop - i;
+    float v[1] = {lane < count ? to_f32(x[i + lane]) : -INFINITY};
+    w.step(v, static_cast<int>(i + lane), lane < count ? 1 : 0);
+    i += count;
+  }
+  for (; i < stop; i += 32 * E) {
+    const int64_t at = i + lane * E;
+    float v[E];
+    int has = 0;
+    if (at + E <= stop) {
+      unpack<T, E>(ld_packet<T, E>(x + at), v);
+      has = E;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = at + e < stop ? to_f32(x[at + e]) : -INFINITY;
+      has = at < stop ? static_cast<int>(stop - at) : 0;
+    }
+    w.step(v, static_cast<int>(at), has);
+  }
+#pragma unroll
+  for (int q = 0; q < Q; ++q) lists[warp][q * 32 + lane] = make_int2(w.best.key[q], w.best.at[q]);
+#pragma unroll
+  for (int bit = 1; bit < 32; bit *= 2) {
+    Soft o;
+    o.m = __shfl_xor_sync(~0u, w.soft.m, bit);
+    o.s = __shfl_xor_sync(~0u, w.soft.s, bit);
+    o.low = __shfl_xor_sync(~0u, w.soft.low, bit);
+    const float m = fmaxf(w.soft.m, o.m);
+    raise(w.soft, m);
+    raise(o, m);
+    add_to(w.soft, o.s);
+    w.soft.low += o.low;
+  }
+  if (lane == 0) softs[warp] = w.soft;
+  __syncthreads();
+  if (warp != 0) return;
+  // the other warps' lists behind this one's, each in its order until an entry does not fit
+  for (int o = 1; o < kWarps; ++o) {
+    for (int e = 0; e < n; ++e) {
+      const int2 c = lists[o][e];
+      if (c.x <= w.best.last) break;
+      w.best.insert(c.x, c.y, lane);
+    }
+    Soft s = softs[o];
+    const float m = fmaxf(w.soft.m, s.m);
+    raise(w.soft, m);
+    raise(s, m);
+    add_to(w.soft, s.s);
+    w.soft.low += s.low;
+  }
+  int2* out = a.best + static_cast<int64_t>(blockIdx.x) * n;
+#pragma unroll
+  for (int q = 0; q < Q; ++q)
+    if (q * 32 + lane < n) out[q * 32 + lane] = make_int2(w.best.key[q], w.best.at[q]);
+  if (lane == 0) a.sums[blockIdx.x] = make_float2(w.soft.m, w.soft.s + w.soft.low);
+}
+
+// One CTA for each request.  A warp joins a beam's parts and writes the beam's best with their
+// totals, in 64 bits, to shared memory; then the first warp takes the best head n times.
+template <int Q>
+__global__ void __launch_bounds__(kThreads) beam_join_kernel(const BeamSelectArgs a) {
+  extern __shared__ double totals[];  // (beams, n), then the tokens
+  const int n = static_cast<int>(a.candidates), beams = static_cast<int>(a.beams);
+  int* tokens = reinterpret_cast<int*>(totals + beams * n);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t b = blockIdx.x;
+  grid_dependency_wait();
+  for (int k = warp; k < beams; k += kWarps) {
+    const int64_t first = (b * beams + k) * a.parts;
+    Best<Q> best;
+    best.start(n);
+    float m = -INFINITY;
+    for (int64_t p = lane; p < a.parts; p += 32) m = fmaxf(m, a.sums[first + p].x);
+#pragma unroll
+    for (int bit = 1; bit < 32; bit *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, bit));
+    double s = 0.0;
+    for (int64_t p = lane; p < a.parts; p += 32) {
+      const float2 v = a.sums[first + p];
+      s += static_cast<double>(v.y) * (v.x > -INFINITY ? exp(static_cast<double>(v.x) - m) : 1.0);
+    }
+#pragma unroll
+    for (int bit = 1; bit < 32; bit *= 2) s += __shfl_xor_sync(~0u, s, bit);
+    const double lse = m + log(s);
+    for (int64_t p = 0; p < a.parts; ++p) {
+      const int2* list = a.best + (first + p) * n;
+      for (int e = 0; e < n; ++e) {
+        const int2 c = list[e];
+        if (c.x <= best.last) break;
+        best.insert(c.x, c.y, lane);
+      }
+    }
+    const float score = a.scores[b * a.scores_s0 + k * a.scores_s1];
+    const bool ended = a.finished && a.finished[b * a.finished_s0 + k * a.finished_s1];
+    // a row that is no distribution (a NaN, an infinity, nothing left) offers nothing
+    const bool sound = fabsf(score) < INFINITY && (ended || fabs(lse) < INFINITY);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int i = q * 32 + lane;
+      if (i >= n) continue;
+      double total = -INFINITY;
+      int token = i;  // nothing offered: the lowest places
+      if (sound && ended) {
+        if (i == 0) total = score, token = static_cast<int>(a.end_token);
+        else if (i <= a.end_token) token = i - 1;
+      } else if (sound && best.key[q] != kEmpty) {
+        total = static_cast<double>(score) + (static_cast<double>(value_of(best.key[q])) - lse);
+        token = best.at[q];
+      }
+      totals[k * n + i] = total;
+      tokens[k * n + i] = i < a.vocab ? token : -1;
+    }
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  // lane l has the beams l and l + 32, and where it stands in their lists
+  int at[2] = {0, 0};
+  for (int c = 0; c < n; ++c) {
+    double top = 0.0;
+    int from = INT_MAX;  // none
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int k = q * 32 + lane;
+      if (k >= beams || at[q] >= n || tokens[k * n + at[q]] < 0) continue;
+      const double t = totals[k * n + at[q]];
+      if (from == INT_MAX || t > top) top = t, from = k;
+    }
+#pragma unroll
+    for (int bit = 1; bit < 32; bit *= 2) {
+      const double t = __shfl_xor_sync(~0u, top, bit);
+      const int k = __shfl_xor_sync(~0u, from, bit);
+      if (k != INT_MAX && (from == INT_MAX || t > top || (t == top && k < from))) top = t, from = k;
+    }
+    const int place = __shfl_sync(~0u, from >= 32 ? at[1] : at[0], from & 31);
+    if (lane == 0) {
+      a.out_scores[b * n + c] = static_cast<float>(top);
+      a.parents[b * n + c] = from;
+      a.tokens[b * n + c] = tokens[from * n + place];
+    }
+    if (lane == (from & 31)) ++at[from >> 5];
+  }
+}
+
+template <typename T, int Q>
+cudaError_t run_select(const BeamSelectArgs& a, cudaStream_t s) {
+  cudaError_t e = launch_dependent(beam_parts_kernel<T, Q>, dim3(static_cast<unsigned>(a.batch * a.beams * a.parts)), dim3(kThreads), 0, s, a);
+  if (e != cudaSuccess) return e;
+  const size_t smem = static_cast<size_t>(a.beams * a.candidates) * 12;
+  e = allow_dynamic_smem(reinterpret_cast<const void*>(beam_join_kernel<Q>), smem);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(beam_join_kernel<Q>, dim3(static_cast<unsigned>(a.batch)), dim3(kThreads), smem, s, a);
+}
+template <typename T>
+cudaError_t run_select(const BeamSelectArgs& a, cudaStream_t s) {
+  return a.candidates <= 32 ? run_select<T, 1>(a, s) : run_select<T, 2>(a, s);
+}
+
+// ------------------------------------------------------------------------ reordering
+// A thread takes one column of a request's rows: it reads it from every parent that is needed,
+// then writes it to every beam whose parent is another one, so the rows change in place.
+template <int BEAMS, typename U>
+__device__ __forceinline__ void move_column(const BeamReorderArgs& a, const BeamRows& t, int64_t column, const int* source, const int* target) {
+  const int64_t u0 = column % t.size0, rest = column / t.size0;
+  const int64_t at = u0 * t.step0 + rest % t.size1 * t.step1 + rest / t.size1 * t.step2;
+  U v[BEAMS];
+#pragma unroll
+  for (int k = 0; k < BEAMS; ++k)
+    if (k < a.beams && source[k] >= 0) v[k] = *reinterpret_cast<const U*>(t.data + source[k] * t.row_bytes + at);
+#pragma unroll
+  for (int k = 0; k < BEAMS; ++k)
+    if (k < a.beams && source[k] >= 0) *reinterpret_cast<U*>(t.data + target[k] * t.row_bytes + at) = v[k];
+}
+
+template <int BEAMS>
+__global__ void __launch_bounds__(kThreads) beam_reorder_kernel(const __grid_constant__ BeamReorderArgs a) {
+  __shared__ int source[BEAMS], target[BEAMS];  // rows; source -1: the beam keeps its row
+  int64_t i = blockIdx.x;
+  int n = 0;
+  while (i >= a.batch * a.t[n].blocks) i -= a.batch * a.t[n++].blocks;
+  const BeamRows& t = a.t[n];
+  const int64_t b = i / t.blocks, block = i % t.blocks;
+  grid_dependency_wait();
+  if (threadIdx.x < a.beams) {
+    const int64_t k = threadIdx.x, at = b * a.parents_s0 + k * a.parents_s1;
+    const int64_t parent = a.wide_parents ? static_cast<const int64_t*>(a.parents)[at] : static_cast<const int32_t*>(a.parents)[at];
+    int64_t from = -1, to = b * a.beams + k;
+    if (parent >= 0 && parent < a.beams && parent != k) {
+      from = b * a.beams + parent;
+      if (a.indices) {
+        from = a.indices[from * a.indices_stride];
+        to = a.indices[to * a.indices_stride];
+      }
+      if (from < 0 || from >= t.rows || to < 0 || to >= t.rows) from = -1;
+    }
+    source[k] = static_cast<int>(from);
+    target[k] = static_cast<int>(to);
+  }
+  __syncthreads();
+  const int64_t column = block * kThreads + threadIdx.x;
+  if (column >= t.columns) return;
+  switch (t.unit) {
+    case 16:
+      if constexpr (BEAMS <= 16) move_column<BEAMS, uint4>(a, t, column, source, target);
+      break;
+    case 8:
+      if constexpr (BEAMS <= 32) move_column<BEAMS, uint2>(a, t, column, source, target);
+      break;
+    case 4: move_column<BEAMS, uint32_t>(a, t, column, source, target); break;
+    case 2: move_column<BEAMS, uint16_t>(a, t, column, source, target); break;
+    default: move_column<BEAMS, uint8_t>(a, t, column, source, target); break;
+  }
+}
+
+}  // namespace
+
+int64_t beam_most_unit(int64_t beams) { return beams <= 16 ? 16 : beams <= 32 ? 8 : 4; }
+
+cudaError_t beam_select(const BeamSelectArgs& a, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case CC1D_FLOAT32: return run_select<float>(a, s);
+    case CC1D_FLOAT16: return run_select<__half>(a, s);
+    default: return run_select<__nv_bfloat16>(a, s);
+  }
+}
+
+cudaError_t beam_reorder(const BeamReorderArgs& a, int64_t ctas, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(ctas));
+  if (a.beams <= 4) return launch_dependent(beam_reorder_kernel<4>, grid, dim3(kThreads), 0, s, a);
+  if (a.beams <= 8) return launch_dependent(beam_reorder_kernel<8>, grid, dim3(kThreads), 0, s, a);
+  if (a.beams <= 16) return launch_dependent(beam_reorder_kernel<16>, grid, dim3(kThreads), 0, s, a);
+  if (a.beams <= 32) return launch_dependent(beam_reorder_kernel<32>, grid, dim3(kThreads), 0, s, a);
+  return launch_dependent(beam_reorder_kernel<64>, grid, dim3(kThreads), 0, s, a);
+}
+
+}  // namespace cc1d

@@ -4,43 +4,12 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
 
 #include "cc1d_block_launch.h"
+#include "cc1d_check.h"
 
 namespace cc1d {
 namespace {
-
-cc1d_status fail(cc1d_status code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-cc1d_status fail(cc1d_status code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  try {
-    set_last_error(buf);
-  } catch (...) {  // out of memory for the message: the status alone has to do
-  }
-  return code;
-}
-
-cc1d_status launched(cudaError_t e, const char* what, int kernels) {
-  if (e != cudaSuccess)
-    return fail(CC1D_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorString(e), cudaGetErrorName(e));
-  count_launches(kernels);
-  return CC1D_OK;
-}
-
-bool is_float(int dt) { return dt == CC1D_FLOAT32 || dt == CC1D_FLOAT16 || dt == CC1D_BFLOAT16; }
-constexpr int64_t kMax31 = (int64_t{1} << 31) - 1;
-
-// Sizes whose products stay far inside 64 bits, so that the launchers' own arithmetic cannot wrap.
-bool sizes_ok(int64_t a, int64_t b, int64_t c) {
-  return a >= 0 && b >= 0 && c >= 0 && a <= kMax31 && b <= kMax31 && c <= kMax31 &&
-         static_cast<double>(a) * static_cast<double>(b) * static_cast<double>(c) < 4e18;
-}
 
 template <typename Args, typename Fn>
 cudaError_t by_type(int dtype, Args& a, cudaStream_t s, Fn f32, Fn f16, Fn bf16) {
@@ -181,13 +150,6 @@ int64_t rec_partial_bytes(const RecArgs& a) {
   return a.batch * a.cluster * a.dim * static_cast<int64_t>(sizeof(float));
 }
 
-#define CC1D_REQUIRE(t, name) \
-  if (!(t).data) return fail(CC1D_ERR_VALUE, "%s is required", name)
-#define CC1D_SAME_TYPE(t, name)                            \
-  if ((t).data && (t).dtype != p->x.dtype) return fail(CC1D_ERR_TYPE, "%s must have x's dtype", name)
-#define CC1D_FP32(t, name) \
-  if ((t).data && (t).dtype != CC1D_FLOAT32) return fail(CC1D_ERR_TYPE, "%s must be float32", name)
-
 cc1d_status rec_check(const cc1d_recurrence_params* p, bool bwd, RecArgs* a) {
   if (!p) return fail(CC1D_ERR_VALUE, "params is NULL");
   const int64_t B = p->batch, D = p->dim, L = p->seqlen, N = p->nstates;
@@ -300,13 +262,6 @@ cc1d_status add_norm_check(const cc1d_add_norm_params* p, bool bwd, AddNormArgs*
   a->keep_scale = static_cast<float>(1.0 / (1.0 - p->dropout_p));
   a->keep_from = static_cast<unsigned>(p->dropout_p * 4294967296.0);
   if (p->rows > 0 && p->dim > 0) add_norm_plan(a, p->x.dtype, sm_count(), bwd);
-  return CC1D_OK;
-}
-
-cc1d_status workspace_ok(const void* ws, int64_t bytes, int64_t need) {
-  if (need > 0 && (!ws || bytes < need))
-    return fail(CC1D_ERR_VALUE, "workspace too small: %lld bytes needed", (long long)need);
-  if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & 15u)) return fail(CC1D_ERR_VALUE, "workspace must be 16-byte aligned");
   return CC1D_OK;
 }
 

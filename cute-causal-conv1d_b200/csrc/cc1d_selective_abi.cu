@@ -1,0 +1,263 @@
+// extern "C" launchers of the selective recurrence and of its token update.  Argument checks
+// happen here, before any launch; include/causal_conv1d_b200.h states the contract.
+#include <algorithm>
+
+#include "cc1d_check.h"
+#include "cc1d_selective_launch.h"
+
+namespace cc1d {
+namespace {
+
+template <typename Args, typename Fn>
+cudaError_t by_type(int dtype, const Args& a, cudaStream_t s, Fn f32, Fn f16, Fn bf16) {
+  switch (dtype) {
+    case CC1D_FLOAT32: return f32(a, s);
+    case CC1D_FLOAT16: return f16(a, s);
+    default: return bf16(a, s);
+  }
+}
+
+constexpr int64_t kMostStates = CC1D_SELECTIVE_MAX_STATES;
+
+// What the sequence and the token form have in common.  p: either params struct.
+template <typename P>
+cc1d_status check_common(const P* p) {
+  const int64_t B = p->batch, D = p->dim, L = p->seqlen, N = p->dstate, G = p->groups;
+  if (!sizes_ok(B, D, L) || !sizes_ok(p->nstates, D, N) || !sizes_ok(B, L, N) || !sizes_ok(B, G, 1))
+    return fail(CC1D_ERR_VALUE, "sizes must be >= 0 and below 2^31");
+  if (N < 1 || N > kMostStates) return fail(CC1D_ERR_VALUE, "dstate must be in [1, %lld]", (long long)kMostStates);
+  if (G < 1 || D % G) return fail(CC1D_ERR_VALUE, "dim must be a multiple of groups");
+  if (!is_float(p->x.dtype)) return fail(CC1D_ERR_TYPE, "x must be float32, float16 or bfloat16");
+  CC1D_SAME_TYPE(p->delta, "delta");
+  CC1D_SAME_TYPE(p->B, "B");
+  CC1D_SAME_TYPE(p->C, "C");
+  CC1D_SAME_TYPE(p->z, "z");
+  CC1D_FLOAT(p->A, "A");
+  CC1D_FLOAT(p->D, "D");
+  CC1D_FLOAT(p->bias, "delta_bias");
+  return CC1D_OK;
+}
+
+cc1d_status check(const cc1d_selective_params* p, bool bwd, SelArgs* a) {
+  if (!p) return fail(CC1D_ERR_VALUE, "params is NULL");
+  const cc1d_status st = check_common(p);
+  if (st != CC1D_OK) return st;
+  if (p->seq_idx.data && p->seq_idx.dtype != CC1D_INT32) return fail(CC1D_ERR_TYPE, "seq_idx must be int32");
+  CC1D_FP32(p->initial_states, "initial_states");
+  if (!p->seq_idx.data && (p->initial_states.data || p->final_states.data || p->dfinal_states.data ||
+                           p->dinitial_states.data) && p->nstates != p->batch)
+    return fail(CC1D_ERR_VALUE, "without seq_idx there is one state for each batch row");
+  if (!bwd) {
+    CC1D_SAME_TYPE(p->out, "out");
+    CC1D_FP32(p->final_states, "final_states");
+  } else {
+    CC1D_SAME_TYPE(p->dout, "dout");
+    CC1D_SAME_TYPE(p->dx, "dx");
+    CC1D_SAME_TYPE(p->ddelta, "ddelta");
+    CC1D_SAME_TYPE(p->dB, "dB");
+    CC1D_SAME_TYPE(p->dC, "dC");
+    CC1D_SAME_TYPE(p->dz, "dz");
+    CC1D_FP32(p->dfinal_states, "dfinal_states");
+    CC1D_FP32(p->dinitial_states, "dinitial_states");
+  }
+  if (p->batch > 0 && p->dim > 0 && p->seqlen > 0) {
+    CC1D_REQUIRE(p->x, "x");
+    CC1D_REQUIRE(p->delta, "delta");
+    CC1D_REQUIRE(p->A, "A");
+    CC1D_REQUIRE(p->B, "B");
+    CC1D_REQUIRE(p->C, "C");
+    if (!bwd) {
+      CC1D_REQUIRE(p->out, "out");
+    } else {
+      CC1D_REQUIRE(p->dout, "dout");
+      CC1D_REQUIRE(p->dx, "dx");
+      CC1D_REQUIRE(p->ddelta, "ddelta");
+      CC1D_REQUIRE(p->dB, "dB");
+      CC1D_REQUIRE(p->dC, "dC");
+      if (p->z.data) CC1D_REQUIRE(p->dz, "dz");
+      if (!p->checkpoints) return fail(CC1D_ERR_VALUE, "checkpoints are required");
+    }
+    if (reinterpret_cast<uintptr_t>(p->checkpoints) & 15u) return fail(CC1D_ERR_VALUE, "checkpoints must be 16-byte aligned");
+  }
+  *a = SelArgs{};
+  a->batch = p->batch;
+  a->dim = p->dim;
+  a->seqlen = p->seqlen;
+  a->dstate = p->dstate;
+  a->groups = p->groups;
+  a->nstates = p->nstates;
+  a->x = tensor_arg(p->x);
+  a->delta = tensor_arg(p->delta);
+  a->A = tensor_arg(p->A);
+  a->B = tensor_arg(p->B);
+  a->C = tensor_arg(p->C);
+  a->D = tensor_arg(p->D);
+  a->z = tensor_arg(p->z);
+  a->bias = tensor_arg(p->bias);
+  a->seq_idx = tensor_arg(p->seq_idx);
+  a->init = tensor_arg(p->initial_states);
+  a->final_states = bwd ? TensorArg{} : tensor_arg(p->final_states);
+  a->out = tensor_arg(p->out);
+  a->dout = tensor_arg(p->dout);
+  a->dfinal = tensor_arg(p->dfinal_states);
+  a->dx = tensor_arg(p->dx);
+  a->ddelta = tensor_arg(p->ddelta);
+  a->dB = tensor_arg(p->dB);
+  a->dC = tensor_arg(p->dC);
+  a->dz = tensor_arg(p->dz);
+  a->dinit = tensor_arg(p->dinitial_states);
+  a->B_group = p->B_group_stride;
+  a->C_group = p->C_group_stride;
+  a->dB_group = p->dB_group_stride;
+  a->dC_group = p->dC_group_stride;
+  a->dA = p->dA;
+  a->dD = p->dD;
+  a->dbias = p->dbias;
+  a->checkpoints = p->checkpoints;
+  a->softplus = p->softplus != 0;
+  return CC1D_OK;
+}
+
+// Threads per channel, passes, tiles of channels, segments of the sequence, and which way the
+// threads go through a tile.
+cc1d_status plan(SelArgs* a, bool bwd) {
+  a->padded = (a->dstate + 3) / 4 * 4;
+  a->lanes = a->padded <= 4 ? 1 : a->padded <= 8 ? 2 : 4;
+  a->blocks = static_cast<int>((a->dstate + kSelBlock - 1) / kSelBlock);
+  a->nchunks = (a->seqlen + kSelChunk - 1) / kSelChunk;
+  a->gdim = a->dim / a->groups;
+  const int64_t channels = kSelThreads / a->lanes;
+  a->group_tiles = (a->gdim + channels - 1) / channels;
+  a->tiles = a->group_tiles * a->groups;
+  a->rows = a->x.s2 == 1 && a->x.s1 != 1 && a->seqlen > 1;
+  a->segments = 1;
+  a->segment_chunks = (a->nchunks + a->segments - 1) / a->segments;
+  a->segments = (a->nchunks + a->segment_chunks - 1) / a->segment_chunks;
+  if (a->batch * a->segments * a->tiles > kMax31 ||
+      static_cast<double>(a->batch) * a->seqlen * a->groups * 2 * a->padded / kThreads > kMax31)
+    return fail(CC1D_ERR_VALUE, "the problem is too large for one launch");
+  if (bwd && static_cast<double>(a->batch) * a->seqlen * a->tiles * 2 * a->padded > 1e17)
+    return fail(CC1D_ERR_VALUE, "the workspace would be too large");
+  return CC1D_OK;
+}
+
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// Lays the workspace out from `base` on and returns its size.
+int64_t lay_out(SelArgs* a, bool bwd, void* base) {
+  int64_t at = 0;
+  auto take = [&](float*& p, int64_t floats) {
+    p = base ? reinterpret_cast<float*>(static_cast<char*>(base) + at) : nullptr;
+    at += round16(floats * static_cast<int64_t>(sizeof(float)));
+  };
+  const int64_t parts = a->batch * a->segments * a->dim;
+  if (a->segments > 1) {
+    take(a->ends, parts * a->padded);
+    take(a->steps, parts);
+  }
+  if (bwd) {
+    take(a->parts_bc, a->batch * a->seqlen * a->tiles * 2 * a->padded);
+    take(a->parts_a, parts * a->padded);
+    take(a->parts_d, 2 * parts);
+  }
+  return at;
+}
+
+bool empty(const SelArgs& a) { return a.batch == 0 || a.dim == 0 || a.seqlen == 0; }
+
+int64_t workspace_bytes(const cc1d_selective_params* p, bool bwd) {
+  set_last_error("");
+  SelArgs a;
+  if (check(p, bwd, &a) != CC1D_OK) return -1;
+  if (empty(a)) return 0;
+  return plan(&a, bwd) == CC1D_OK ? lay_out(&a, bwd, nullptr) : -1;
+}
+
+}  // namespace
+}  // namespace cc1d
+
+using namespace cc1d;
+
+extern "C" {
+
+int64_t cc1d_selective_fwd_workspace_bytes(const cc1d_selective_params* p) { return workspace_bytes(p, false); }
+int64_t cc1d_selective_bwd_workspace_bytes(const cc1d_selective_params* p) { return workspace_bytes(p, true); }
+
+cc1d_status cc1d_selective_fwd_launch(const cc1d_selective_params* p, void* stream) {
+  set_last_error("");
+  SelArgs a;
+  cc1d_status st = check(p, false, &a);
+  if (st != CC1D_OK || empty(a)) return st;
+  if ((st = plan(&a, false)) != CC1D_OK) return st;
+  if ((st = workspace_ok(p->workspace, p->workspace_bytes, lay_out(&a, false, p->workspace))) != CC1D_OK) return st;
+  return launched(by_type(p->x.dtype, a, static_cast<cudaStream_t>(stream), sel_fwd_f32, sel_fwd_f16, sel_fwd_bf16),
+                  "selective recurrence forward launch", a.segments > 1 ? 2 : 1);
+}
+
+cc1d_status cc1d_selective_bwd_launch(const cc1d_selective_params* p, void* stream) {
+  set_last_error("");
+  SelArgs a;
+  cc1d_status st = check(p, true, &a);
+  if (st != CC1D_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (empty(a)) {
+    cudaError_t e = cudaSuccess;
+    if (a.dA && a.dim > 0) e = cudaMemsetAsync(a.dA, 0, a.dim * a.dstate * sizeof(float), s);
+    if (e == cudaSuccess && a.dD && a.dim > 0) e = cudaMemsetAsync(a.dD, 0, a.dim * sizeof(float), s);
+    if (e == cudaSuccess && a.dbias && a.dim > 0) e = cudaMemsetAsync(a.dbias, 0, a.dim * sizeof(float), s);
+    return launched(e, "selective recurrence zero fill", 0);
+  }
+  if ((st = plan(&a, true)) != CC1D_OK) return st;
+  if ((st = workspace_ok(p->workspace, p->workspace_bytes, lay_out(&a, true, p->workspace))) != CC1D_OK) return st;
+  return launched(by_type(p->x.dtype, a, s, sel_bwd_f32, sel_bwd_f16, sel_bwd_bf16), "selective recurrence backward launch",
+                  a.segments > 1 ? 4 : 3);
+}
+
+cc1d_status cc1d_selective_update_launch(const cc1d_selective_update_params* p, void* stream) {
+  set_last_error("");
+  if (!p) return fail(CC1D_ERR_VALUE, "params is NULL");
+  const cc1d_status st = check_common(p);
+  if (st != CC1D_OK) return st;
+  CC1D_SAME_TYPE(p->out, "out");
+  CC1D_FP32(p->state, "state");
+  if (p->state_indices.data && p->state_indices.dtype != CC1D_INT32)
+    return fail(CC1D_ERR_TYPE, "state_indices must be int32");
+  if (!p->state_indices.data && p->nstates != p->batch)
+    return fail(CC1D_ERR_VALUE, "without state_indices there is one state for each batch row");
+  if (p->batch == 0 || p->dim == 0 || p->seqlen == 0) return CC1D_OK;
+  CC1D_REQUIRE(p->x, "x");
+  CC1D_REQUIRE(p->delta, "delta");
+  CC1D_REQUIRE(p->A, "A");
+  CC1D_REQUIRE(p->B, "B");
+  CC1D_REQUIRE(p->C, "C");
+  CC1D_REQUIRE(p->out, "out");
+  if (p->nstates > 0) CC1D_REQUIRE(p->state, "state");
+  if (static_cast<double>(p->batch) * p->dim * 32 / kThreads > kMax31)
+    return fail(CC1D_ERR_VALUE, "batch * dim is too large");
+  SelUpdateArgs a;
+  a.batch = p->batch;
+  a.dim = p->dim;
+  a.seqlen = p->seqlen;
+  a.dstate = p->dstate;
+  a.groups = p->groups;
+  a.nstates = p->nstates;
+  a.x = tensor_arg(p->x);
+  a.delta = tensor_arg(p->delta);
+  a.A = tensor_arg(p->A);
+  a.B = tensor_arg(p->B);
+  a.C = tensor_arg(p->C);
+  a.D = tensor_arg(p->D);
+  a.z = tensor_arg(p->z);
+  a.bias = tensor_arg(p->bias);
+  a.state = tensor_arg(p->state);
+  a.out = tensor_arg(p->out);
+  a.B_group = p->B_group_stride;
+  a.C_group = p->C_group_stride;
+  a.indices = static_cast<const int32_t*>(p->state_indices.data);
+  a.indices_stride = p->state_indices.stride[0];
+  a.softplus = p->softplus != 0;
+  return launched(by_type(p->x.dtype, a, static_cast<cudaStream_t>(stream), sel_update_f32, sel_update_f16, sel_update_bf16),
+                  "selective recurrence update launch", 1);
+}
+
+}  // extern "C"

@@ -1,0 +1,128 @@
+// The selective recurrence for a few tokens of each row against a pool of fp32 states (sm_100a).
+//
+// LANES threads share a channel of one batch row; each takes VEC * 4 of its states through the
+// row's tokens, from the state it reads to the one it writes back, and the output is summed over
+// the threads by exchanges.  A state is read and written once; it is most of what moves.
+#include "cc1d_selective.cuh"
+
+namespace cc1d {
+namespace {
+
+// PACKED: states, A, B and C lie densely along dstate, a multiple of 4, and on 16 bytes (16-bit: 8).
+template <typename T, bool PACKED>
+__device__ __forceinline__ Four load_inputs(const TensorArg& t, int64_t group_stride, int64_t b, int64_t g, int64_t n0, int64_t l, int64_t dstate) {
+  const T* p = static_cast<const T*>(t.data) + b * t.s0 + g * group_stride + l * t.s2;
+  Four f;
+  if constexpr (PACKED) {
+    unpack<T, 4>(ld_packet<T, 4>(p + n0), f.v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.v[i] = n0 + i < dstate ? to_f32(p[(n0 + i) * t.s1]) : 0.f;
+  }
+  return f;
+}
+
+template <typename T, int LANES, int VEC, bool PACKED>
+__global__ void __launch_bounds__(kThreads) sel_update_kernel(const SelUpdateArgs a) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / LANES;
+  const int sl = threadIdx.x % LANES;
+  grid_dependency_wait();
+  const bool mine = i < a.batch * a.dim;
+  const int64_t b = mine ? i / a.dim : 0, d = mine ? i - b * a.dim : 0, g = d / (a.dim / a.groups);
+  const int64_t row = !mine ? -1 : a.indices ? a.indices[b * a.indices_stride] : b;
+  const bool live = row >= 0 && row < a.nstates;
+  Four h[VEC], rate[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    const int64_t n0 = (v * LANES + sl) * 4;
+    h[v] = rate[v] = zero4();
+    if (!live || n0 >= a.dstate) continue;
+    if constexpr (PACKED) {
+      h[v] = load4(static_cast<const float*>(a.state.data) + row * a.state.s0 + d * a.state.s1 + n0);
+      rate[v] = load4(static_cast<const float*>(a.A.data) + d * a.A.s0 + n0);
+    } else {
+      h[v] = load_state(a.state, row, d, n0, a.dstate);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (n0 + k < a.dstate) rate[v].v[k] = load_any(a.A.data, a.A.dtype, d * a.A.s0 + (n0 + k) * a.A.s1);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) rate[v].v[k] *= kLog2e;
+  }
+  const float bias = live && a.bias.data ? load_any(a.bias.data, a.bias.dtype, d * a.bias.s0) : 0.f;
+  const float skip = live && a.D.data ? load_any(a.D.data, a.D.dtype, d * a.D.s0) : 0.f;
+  for (int64_t l = 0; l < a.seqlen; ++l) {
+    float y = 0.f, x = 0.f;
+    if (live) {
+      x = load_el<T>(a.x, b, d, l);
+      float s = load_el<T>(a.delta, b, d, l) + bias, slope;
+      if (a.softplus) s = step_size(s, &slope);
+      const float sx = s * x;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        const int64_t n0 = (v * LANES + sl) * 4;
+        if (n0 >= a.dstate) continue;
+        const Four B = load_inputs<T, PACKED>(a.B, a.B_group, b, g, n0, l, a.dstate);
+        const Four C = load_inputs<T, PACKED>(a.C, a.C_group, b, g, n0, l, a.dstate);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          h[v].v[k] = fmaf(ex2_approx(s * rate[v].v[k]), h[v].v[k], sx * B.v[k]);
+          y = fmaf(C.v[k], h[v].v[k], y);
+        }
+      }
+    }
+#pragma unroll
+    for (int bit = 1; bit < LANES; bit *= 2) y += __shfl_xor_sync(~0u, y, bit);
+    if (!mine || sl != 0) continue;
+    if (live) {
+      y = fmaf(skip, x, y);
+      if (a.z.data) y *= silu_of<T>(load_el<T>(a.z, b, d, l));
+    }
+    store_el<T>(a.out, b, d, l, live ? y : 0.f);
+  }
+  if (!live) return;
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    const int64_t n0 = (v * LANES + sl) * 4;
+    if (n0 >= a.dstate) continue;
+    if constexpr (PACKED) store4(static_cast<float*>(a.state.data) + row * a.state.s0 + d * a.state.s1 + n0, h[v]);
+    else store_state(a.state, row, d, n0, a.dstate, h[v]);
+  }
+}
+
+// Packets of four states are legal.
+bool packed(const SelUpdateArgs& a) {
+  if (a.dstate % 4) return false;
+  auto on = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
+  auto step = [](int64_t s, int64_t extent) { return extent <= 1 || s % 4 == 0; };
+  if (a.state.s2 != 1 || !on(a.state.data, 16) || !step(a.state.s0, a.nstates) || !step(a.state.s1, a.dim)) return false;
+  if (a.A.dtype != CC1D_FLOAT32 || a.A.s1 != 1 || !on(a.A.data, 16) || !step(a.A.s0, a.dim)) return false;
+  const uintptr_t bytes = a.x.dtype == CC1D_FLOAT32 ? 16 : 8;
+  const struct { const TensorArg& t; int64_t group; } both[] = {{a.B, a.B_group}, {a.C, a.C_group}};
+  for (const auto& e : both)
+    if (e.t.s1 != 1 || !on(e.t.data, bytes) || !step(e.t.s0, a.batch) || !step(e.group, a.groups) || !step(e.t.s2, a.seqlen)) return false;
+  return true;
+}
+
+template <typename T, int LANES, int VEC>
+cudaError_t run(const SelUpdateArgs& a, cudaStream_t s) {
+  const int64_t threads = a.batch * a.dim * LANES;
+  const dim3 grid(static_cast<unsigned>((threads + kThreads - 1) / kThreads));
+  return packed(a) ? launch_dependent(sel_update_kernel<T, LANES, VEC, true>, grid, dim3(kThreads), 0, s, a)
+                   : launch_dependent(sel_update_kernel<T, LANES, VEC, false>, grid, dim3(kThreads), 0, s, a);
+}
+
+}  // namespace
+
+cudaError_t CC1D_DT_NAME(sel_update)(const SelUpdateArgs& a, cudaStream_t s) {
+  using T = CC1D_DT_TYPE;
+  return a.dstate <= 4    ? run<T, 1, 1>(a, s)
+         : a.dstate <= 8  ? run<T, 2, 1>(a, s)
+         : a.dstate <= 16 ? run<T, 4, 1>(a, s)
+         : a.dstate <= 32 ? run<T, 8, 1>(a, s)
+         : a.dstate <= 64 ? run<T, 16, 1>(a, s)
+         : a.dstate <= 128 ? run<T, 32, 1>(a, s)
+                           : run<T, 32, 2>(a, s);
+}
+
+}  // namespace cc1d

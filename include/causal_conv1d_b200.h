@@ -364,6 +364,170 @@ cc1d_status cc1d_add_norm_fwd_launch(const cc1d_add_norm_params* params, void* s
 int64_t cc1d_add_norm_bwd_workspace_bytes(const cc1d_add_norm_params* params);
 cc1d_status cc1d_add_norm_bwd_launch(const cc1d_add_norm_params* params, void* stream);
 
+/* ------------------------------------------------------ selective recurrence
+ * The selective state-space recurrence that follows the convolution in a state-space block:
+ *     s[b, d, t]    = softplus(delta[b, d, t] + bias[d])             (without softplus: delta + bias)
+ *     h[b, d, n, t] = exp(s A[d, n]) h[b, d, n, t-1] + s x[b, d, t] B[b, g, n, t]
+ *     out[b, d, t]  = (sum_n C[b, g, n, t] h[b, d, n, t] + D[d] x[b, d, t]) * silu(z[b, d, t])
+ * with g = d / (dim / groups), computed and carried in fp32 and rounded once, on the stores.
+ *
+ * Any strides are accepted.
+ *   x, delta, z, out (batch, dim, seqlen)           one float dtype; z optional
+ *   A               (dim, dstate)                   any float dtype; dstate <= CC1D_SELECTIVE_MAX_STATES
+ *   B, C            (batch, groups, dstate, seqlen) x's dtype; the tensors' three strides are those
+ *                                                   of batch, dstate and seqlen, B_group_stride and
+ *                                                   C_group_stride the others
+ *   D, bias         (dim,)                          any float dtype, optional
+ *   seq_idx         (batch, seqlen) int32           optional, as in the gated recurrence
+ *   initial_states  (nstates, dim, dstate) fp32     optional, h before the first position
+ *   final_states    (nstates, dim, dstate) fp32     optional output, h at the last position.  With
+ *                                                   seq_idx only the rows of sequences that have
+ *                                                   positions are written: fill the others beforehand
+ *   checkpoints     (batch, ceil(seqlen / CC1D_SELECTIVE_CHUNK), dim, dstate rounded up to a multiple
+ *                   of 4) fp32 contiguous, 16-byte aligned: h before each chunk; written by the
+ *                   forward if given, read by the backward
+ *   workspace       device scratch of cc1d_selective_{fwd,bwd}_workspace_bytes(params) bytes, 16-byte
+ *                   aligned, contents need not be initialised
+ * Without seq_idx nstates == batch.  At a padding position out is 0 and nothing that stands there is
+ * used.  The gradients of out and of final_states give
+ *   dx, ddelta, dz  (batch, dim, seqlen)            outputs, x's dtype (dz iff z)
+ *   dB, dC          (batch, groups, dstate, seqlen) outputs, x's dtype, summed in a fixed order
+ *   dinitial_states (nstates, dim, dstate) fp32     optional output; with seq_idx as final_states
+ *   dA              (dim, dstate) fp32 dense        optional outputs, summed in a fixed order
+ *   dD, dbias       (dim,) fp32 dense
+ * dout (batch, dim, seqlen) has x's dtype; dfinal_states (nstates, dim, dstate) fp32 is optional.
+ * The forward ignores the gradient fields and the backward final_states and out.
+ */
+#define CC1D_SELECTIVE_CHUNK 32
+#define CC1D_SELECTIVE_MAX_STATES 256
+
+typedef struct cc1d_selective_params {
+  int64_t batch, dim, seqlen, dstate, groups, nstates;
+  int64_t softplus; /* 0 or 1 */
+  cc1d_tensor x;
+  cc1d_tensor delta;
+  cc1d_tensor A;
+  cc1d_tensor B;
+  cc1d_tensor C;
+  cc1d_tensor D;
+  cc1d_tensor z;
+  cc1d_tensor bias;
+  cc1d_tensor seq_idx;
+  cc1d_tensor initial_states;
+  cc1d_tensor final_states;
+  cc1d_tensor out;
+  cc1d_tensor dout;
+  cc1d_tensor dfinal_states;
+  cc1d_tensor dx;
+  cc1d_tensor ddelta;
+  cc1d_tensor dB;
+  cc1d_tensor dC;
+  cc1d_tensor dz;
+  cc1d_tensor dinitial_states;
+  int64_t B_group_stride, C_group_stride, dB_group_stride, dC_group_stride;
+  float* dA;
+  float* dD;
+  float* dbias;
+  float* checkpoints;
+  void* workspace;
+  int64_t workspace_bytes;
+} cc1d_selective_params;
+
+/* Scratch bytes, or -1 with cc1d_last_error() set if the params are invalid. */
+int64_t cc1d_selective_fwd_workspace_bytes(const cc1d_selective_params* params);
+cc1d_status cc1d_selective_fwd_launch(const cc1d_selective_params* params, void* stream);
+int64_t cc1d_selective_bwd_workspace_bytes(const cc1d_selective_params* params);
+cc1d_status cc1d_selective_bwd_launch(const cc1d_selective_params* params, void* stream);
+
+/* ----------------------------------------------- selective recurrence, decoding
+ * The same recurrence for a few tokens of each row against a pool of states.
+ *   x, delta, z, out, A, B, C, D, bias    as above
+ *   state           (nstates, dim, dstate) fp32  updated in place
+ *   state_indices   (batch,) int32               optional: state row of each batch row; a row outside
+ *                                                [0, nstates) is padding: out = 0, no state is touched.
+ *                                                Two batch rows must not name the same state row.
+ * Without state_indices nstates == batch.
+ */
+typedef struct cc1d_selective_update_params {
+  int64_t batch, dim, seqlen, dstate, groups, nstates;
+  int64_t softplus; /* 0 or 1 */
+  cc1d_tensor x;
+  cc1d_tensor delta;
+  cc1d_tensor A;
+  cc1d_tensor B;
+  cc1d_tensor C;
+  cc1d_tensor D;
+  cc1d_tensor z;
+  cc1d_tensor bias;
+  cc1d_tensor state;
+  cc1d_tensor state_indices;
+  cc1d_tensor out;
+  int64_t B_group_stride, C_group_stride;
+} cc1d_selective_update_params;
+
+cc1d_status cc1d_selective_update_launch(const cc1d_selective_update_params* params, void* stream);
+
+/* -------------------------------------------------------- beam search, selection
+ * The best continuations of each request's beams:
+ *     total[b, k, v] = scores[b, k] + logits[b, k, v] - log sum_w exp(logits[b, k, w])
+ * and of each request the `candidates` largest in descending order, equal totals by the lowest
+ * place k * vocab + v.  Sums are taken in fp32 with their rounding kept, totals in fp64.
+ *   logits          (batch, beams, vocab)  float dtype, unit stride along the vocabulary
+ *   scores          (batch, beams) fp32    log-probabilities of the beams so far
+ *   finished        (batch, beams) bytes   optional; where not 0 the beam's only continuation is
+ *                                          end_token, at no cost
+ *   out_scores      (batch, candidates) fp32 dense
+ *   parents, tokens (batch, candidates) int64 dense: the beam k and the token v
+ * What is no number counts as -infinity: a NaN, a beam whose score is not finite, or whose logits
+ * have a NaN, an infinity or nothing above -infinity.  Tokens of one beam are ordered by their
+ * logits, also where a huge score leaves their totals equal.
+ * 1 <= candidates <= min(beams * vocab, CC1D_BEAM_MAX), beams <= CC1D_BEAM_MAX.
+ */
+#define CC1D_BEAM_MAX 64
+
+typedef struct cc1d_beam_select_params {
+  int64_t batch, beams, vocab, candidates;
+  int64_t end_token; /* in [0, vocab) with finished */
+  cc1d_tensor logits;
+  cc1d_tensor scores;
+  const uint8_t* finished;
+  int64_t finished_stride[2];
+  float* out_scores;
+  int64_t* parents;
+  int64_t* tokens;
+  void* workspace; /* cc1d_beam_select_workspace_bytes(params) bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+} cc1d_beam_select_params;
+
+int64_t cc1d_beam_select_workspace_bytes(const cc1d_beam_select_params* params);
+cc1d_status cc1d_beam_select_launch(const cc1d_beam_select_params* params, void* stream);
+
+/* ------------------------------------------------------- beam search, reordering
+ * The states of the beams follow the choice, in place:
+ *     row(b, k) <- row(b, parents[b, k]),   row(b, k) = b * beams + k, or state_indices[b * beams + k]
+ * for each of `count` tensors.  A beam whose parent is outside [0, beams), or whose row or parent's
+ * row is outside [0, rows), keeps its row.  No row may be named twice by state_indices.
+ *   parents         (batch, beams) int32 or int64
+ *   state_indices   (batch * beams,) int32, optional
+ * A row has up to three dimensions of elements; strides are in elements.
+ */
+typedef struct cc1d_beam_rows {
+  void* data;
+  int64_t rows, row_stride;
+  int64_t element_bytes; /* 1, 2, 4, 8 or 16 */
+  int64_t size[3];
+  int64_t stride[3];
+} cc1d_beam_rows;
+
+typedef struct cc1d_beam_reorder_params {
+  int64_t batch, beams, count;
+  cc1d_tensor parents;
+  cc1d_tensor state_indices;
+  const cc1d_beam_rows* tensors; /* on the host */
+} cc1d_beam_reorder_params;
+
+cc1d_status cc1d_beam_reorder_launch(const cc1d_beam_reorder_params* params, void* stream);
+
 /* ------------------------------------------------------------------- utility */
 /* Message of the last error on the calling thread ("" if none). */
 const char* cc1d_last_error(void);
