@@ -361,12 +361,16 @@ _NONE = (0, 0, 0, 0, 0)  # an absent tensor
 RECURRENCE_PARAMS = struct.Struct("<78q")
 RECURRENCE_UPDATE_PARAMS = struct.Struct("<39q")
 ADD_NORM_PARAMS = struct.Struct("<55q2d")
-SELECTIVE_CHUNK = 32  # CC1D_SELECTIVE_CHUNK
 SELECTIVE_PARAMS = struct.Struct("<117q")
 SELECTIVE_UPDATE_PARAMS = struct.Struct("<64q")
 BEAM_SELECT_PARAMS = struct.Struct("<23q")
 BEAM_ROWS = struct.Struct("<10q")
 BEAM_REORDER_PARAMS = struct.Struct("<14q")
+
+
+def selective_chunk(dstate: int) -> int:
+    """CC1D_SELECTIVE_CHUNK: positions between two checkpoints of the selective recurrence."""
+    return 8 if dstate <= 4 else 16 if dstate <= 8 else 32
 
 
 def launch_count() -> int:

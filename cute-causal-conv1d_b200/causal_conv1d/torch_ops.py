@@ -241,7 +241,7 @@ def _(x, delta, A, B, C, D, z, delta_bias, delta_softplus, seq_idx, initial_stat
     dstate = A.shape[1]
     n = _state_rows(x, seq_idx, initial_states, num_sequences)
     final = x.new_empty((n, dim, dstate) if return_final_states else _EMPTY, dtype=torch.float32)
-    kept = (batch, -(-seqlen // _abi.SELECTIVE_CHUNK), dim, -(-dstate // 4) * 4)
+    kept = (batch, -(-seqlen // _abi.selective_chunk(dstate)), dim, -(-dstate // 4) * 4)
     return _laid_out_like(x), final, x.new_empty(kept if save_checkpoints else _EMPTY, dtype=torch.float32)
 
 

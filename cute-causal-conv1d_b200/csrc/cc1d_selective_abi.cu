@@ -124,7 +124,8 @@ cc1d_status plan(SelArgs* a, bool bwd) {
   a->padded = (a->dstate + 3) / 4 * 4;
   a->lanes = a->padded <= 4 ? 1 : a->padded <= 8 ? 2 : 4;
   a->blocks = static_cast<int>((a->dstate + kSelBlock - 1) / kSelBlock);
-  a->nchunks = (a->seqlen + kSelChunk - 1) / kSelChunk;
+  const int64_t chunk = CC1D_SELECTIVE_CHUNK(a->dstate);
+  a->nchunks = (a->seqlen + chunk - 1) / chunk;
   a->gdim = a->dim / a->groups;
   const int64_t channels = kSelThreads / a->lanes;
   a->group_tiles = (a->gdim + channels - 1) / channels;

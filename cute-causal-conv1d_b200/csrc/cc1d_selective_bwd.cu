@@ -20,17 +20,23 @@ namespace cc1d {
 namespace {
 
 constexpr int kWarps = kSelThreads / 32;
+#ifndef BWDC
+#define BWDC 3
+#endif
+constexpr int kBwdCtas = BWDC;
 
+// Shared memory: flags; (s, x, dy, slope of the step size), replaced by (dx, ddelta, y), by position
+// and channel; the states before every fourth position; each warp's sums of dB and dC; B and C;
+// with several passes three sums by position and channel, and the states between two tiles.
 template <int LN>
 struct BwdSmem {
-  static constexpr int CH = kSelThreads / LN;
-  static constexpr int kFlags = 256;
-  static constexpr int kIo = kSelChunk * (CH + 1) * 16;
-  static constexpr int kSums = (kSelChunk * (CH + 1) * 12 + 15) / 16 * 16;  // several passes only
-  static constexpr int kSub = kSelChunk / 4 * kSelThreads * 16;
-  static constexpr int kSlab = kSelChunk * 8 * LN * 4;                       // one warp's sums of dB and dC
-  static __host__ __device__ int64_t bytes(const SelArgs& a) {
-    return kFlags + kIo + kSub + kWarps * kSlab + kSelChunk * 2 * a.padded * 4 +
+  static constexpr int kFlags = 256, T = Tile<LN, false>::T, PITCH = Tile<LN, false>::PITCH;
+  static constexpr int kIo = T * PITCH * 16;
+  static constexpr int kSums = (T * PITCH * 12 + 15) / 16 * 16;
+  static constexpr int kSub = T / 4 * kSelThreads * 16;
+  static constexpr int kSlab = T * 8 * LN * 4;  // one warp's
+  static int64_t bytes(const SelArgs& a) {
+    return kFlags + kIo + kSub + kWarps * kSlab + T * 8 * LN * a.blocks * 4 +
            (a.blocks > 1 ? kSums + 3ll * a.blocks * kSelThreads * 16 : 0);
   }
 };
@@ -42,42 +48,49 @@ __device__ __forceinline__ void add_to(float& hi, float& lo, float v) {
   lo += (hi - (s - w)) + (v - w);
   hi = s;
 }
+__device__ __forceinline__ void add_to(Four& hi, Four& lo, const Four& v) {
+  add_to(hi.lo.x, lo.lo.x, v.lo.x);
+  add_to(hi.lo.y, lo.lo.y, v.lo.y);
+  add_to(hi.hi.x, lo.hi.x, v.hi.x);
+  add_to(hi.hi.y, lo.hi.y, v.hi.y);
+}
 
-// The sums of v[0 .. 8) over the channels of a warp; a lane ends with one of them, the number of
-// which it returns (in v[0]); lanes that differ in further bits hold the same sums.
+// The sums of a's and b's four values over the channels of a warp.  A lane ends with one of the
+// eight, the number of which summed() tells; lanes that differ in further bits hold the same one.
 template <int LN>
-__device__ __forceinline__ int sum_channels(float (&v)[8], int lane) {
-  int which = 0;
+__device__ __forceinline__ float sum_channels(const Four& a, const Four& b, int lane) {
+  float v[8] = {a.lo.x, a.lo.y, a.hi.x, a.hi.y, b.lo.x, b.lo.y, b.hi.x, b.hi.y};
 #pragma unroll
   for (int half = 4; half >= 1; half /= 2) {
-    const int bit = half == 4 ? 16 : half == 2 ? 8 : 4;
+    const int bit = 4 * half;
     const bool hi = lane & bit;
 #pragma unroll
     for (int i = 0; i < half; ++i) {
       const float send = hi ? v[i] : v[half + i];
       v[i] = (hi ? v[half + i] : v[i]) + __shfl_xor_sync(~0u, send, bit);
     }
-    which = which * 2 + (hi ? 1 : 0);
   }
 #pragma unroll
   for (int bit = 2; bit >= LN; bit /= 2) v[0] += __shfl_xor_sync(~0u, v[0], bit);
-  return which;
+  return v[0];
 }
+__device__ __forceinline__ int summed(int lane) { return (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1); }
 
 // ENDS: only the gradient that each segment hands to the one before it.
-template <typename T, int LN, bool ENDS>
-__global__ void __launch_bounds__(kSelThreads) sel_bwd_kernel(const SelArgs a) {
-  constexpr int CH = kSelThreads / LN;
-  constexpr int PITCH = CH + 1;
+template <typename T, int LN, bool ROWS, bool ENDS>
+__global__ void __launch_bounds__(kSelThreads, ENDS ? 4 : kBwdCtas) sel_bwd_kernel(const __grid_constant__ SelArgs a) {
+  using Where = Tile<LN, ROWS>;
   using Smem = BwdSmem<LN>;
+  constexpr int PITCH = Where::PITCH, TT = Where::T;
   extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float biases[Where::CH];
   SelFlags& flags = *reinterpret_cast<SelFlags*>(smem);
-  float4* io = reinterpret_cast<float4*>(smem + Smem::kFlags);  // in: s, x, dy, sigmoid; out: dx, ddelta, y
+  float4* io = reinterpret_cast<float4*>(smem + Smem::kFlags);
   float* sub = reinterpret_cast<float*>(smem + Smem::kFlags + Smem::kIo);
   float* slabs = reinterpret_cast<float*>(smem + Smem::kFlags + Smem::kIo + Smem::kSub);
   float* bc = slabs + kWarps * Smem::kSlab / 4;
-  const int np = static_cast<int>(a.padded);
-  float* held = bc + kSelChunk * 2 * np;  // several passes: g carried, dA and its low part
+  const int np = static_cast<int>(a.padded), wide = 4 * LN * a.blocks;
+  float* held = bc + TT * 2 * wide;  // several passes: g carried, dA and its low part
   float* sums = held + 3 * a.blocks * kSelThreads * 4;
 
   const SelPlace p = sel_place<LN>(a);
@@ -85,6 +98,8 @@ __global__ void __launch_bounds__(kSelThreads) sel_bwd_kernel(const SelArgs a) {
   const bool mine = c < p.channels;
   const int64_t ch = p.ch0 + (mine ? c : 0);
   grid_dependency_wait();
+  for (int i = tid; i < Where::CH; i += kSelThreads)
+    biases[i] = i < p.channels && a.bias.data ? load_any(a.bias.data, a.bias.dtype, (p.ch0 + i) * a.bias.s0) : 0.f;
 
   const float skip = a.D.data && mine ? load_any(a.D.data, a.D.dtype, ch * a.D.s0) : 0.f;
   Four rate = zero4(), carry = zero4(), da = zero4(), da_low = zero4();
@@ -97,13 +112,8 @@ __global__ void __launch_bounds__(kSelThreads) sel_bwd_kernel(const SelArgs a) {
     rate = mine && has ? load_rates(a, ch, n0) : zero4();
     carry = zero4();
     if (!ENDS && mine && has)
-      for (int64_t s = a.segments - 1; s > p.seg; --s) {
-        const Four e = load4(a.ends + ends_at + s * a.dim * np + n0);
-        const float sum = a.steps[(p.b * a.segments + s) * a.dim + ch];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          carry.v[i] = sum < INFINITY && carry.v[i] != 0.f ? fmaf(exp2f(rate.v[i] * sum), carry.v[i], e.v[i]) : e.v[i];
-      }
+      for (int64_t s = a.segments - 1; s > p.seg; --s)
+        carry = handed_on(carry, rate, a.steps[(p.b * a.segments + s) * a.dim + ch], load4(a.ends + ends_at + s * a.dim * np + n0));
     if (a.blocks > 1) {
       store4(held + (nb * 3 * kSelThreads + tid) * 4, carry);
       store4(held + ((nb * 3 + 1) * kSelThreads + tid) * 4, zero4());
@@ -111,31 +121,56 @@ __global__ void __launch_bounds__(kSelThreads) sel_bwd_kernel(const SelArgs a) {
     }
   }
 
-  for (int64_t chunk = p.chunk1 - 1; chunk >= p.chunk0; --chunk) {
-    const int64_t t0 = chunk * kSelChunk;
+  const Walk<T, LN, ROWS> xs(a.x, p), deltas(a.delta, p), zs(a.z.data ? a.z : a.x, p), douts(a.dout, p);
+  const Walk<T, LN, ROWS> dxs(a.dx, p), ddeltas(a.ddelta, p), dzs(a.z.data ? a.dz : a.dx, p);
+  const bool all_channels = p.channels == Where::CH, packed = a.seq_idx.data != nullptr;
+  T next_x[8], next_delta[8], next_z[8], next_dout[8];
+  float dzf[8];  // dout silu'(z)
+  FlagFeed<TT> feed;
+  Coefficients<T, LN> next_bc;
+  auto inside = [&](int64_t i) { return all_channels && (i + 1) * TT <= a.seqlen; };
+  auto fetch = [&](int64_t i) {
+    const bool whole = inside(i);
+    xs.load(a, a.x, p, i, whole, next_x);
+    deltas.load(a, a.delta, p, i, whole, next_delta);
+    douts.load(a, a.dout, p, i, whole, next_dout);
+    if (a.z.data) zs.load(a, a.z, p, i, whole, next_z);
+    feed.load(a, p.b, i * TT);
+    next_bc.load(a, p, i * TT);
+  };
+  fetch(p.chunk1 - 1);
+  for (int64_t i = p.chunk1 - 1; i >= p.chunk0; --i) {
+    const int64_t t0 = i * TT;
+    const bool whole = inside(i);
+    feed.store(a, p.b, t0, flags);
     __syncthreads();
-    load_flags(a, p.b, t0, flags);
-    __syncthreads();
-#pragma unroll 4
-    for (int e = tid; e < kSelChunk * CH; e += kSelThreads) {
-      int t, cc;
-      tile_place<CH>(a.rows, e, t, cc);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (cc < p.channels && (reinterpret_cast<const uint8_t*>(flags.word)[t] & kValid)) {
-        const int64_t d = p.ch0 + cc;
-        float u = load_el<T>(a.delta, p.b, d, t0 + t);
-        v.y = load_el<T>(a.x, p.b, d, t0 + t);
-        v.z = load_el<T>(a.dout, p.b, d, t0 + t);
-        if (a.z.data) v.z *= silu_of<T>(load_el<T>(a.z, p.b, d, t0 + t));
-        if (a.bias.data) u += load_any(a.bias.data, a.bias.dtype, d * a.bias.s0);
-        v.x = u;
-        v.w = 1.f;
-        if (a.softplus) v.x = step_size(u, &v.w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
+      float4 v;
+      const float u = to_f32(next_delta[k]) + biases[cc];
+      v.x = u;
+      v.y = to_f32(next_x[k]);
+      v.z = to_f32(next_dout[k]);
+      v.w = 1.f;
+      if (a.softplus) v.x = step_size(u, &v.w);
+      if (a.z.data) {
+        // silu(z) = z s and silu'(z) = s + z s (1 - s)
+        float s, less;
+        const float z = to_f32(next_z[k]);
+        sigmoid_pair_of<T>(z, s, less);
+        dzf[k] = v.z * fmaf(z * s, less, s);
+        v.z *= z * s;
+      }
+      if ((packed || !whole) && !(flags.valid(t) && cc < p.channels)) {
+        v = make_float4(0.f, 0.f, 0.f, 0.f);
+        dzf[k] = 0.f;
       }
       io[t * PITCH + cc] = v;
     }
-    load_bc<T>(a, p, t0, np, flags, bc);
+    next_bc.store(a, p, t0, flags, bc);
     __syncthreads();
+    if (i > p.chunk0) fetch(i - 1);
 
     for (int nb = 0; nb < a.blocks; ++nb) {
       const int n0 = nb * kSelBlock + sl * kSelStates;
@@ -144,190 +179,162 @@ __global__ void __launch_bounds__(kSelThreads) sel_bwd_kernel(const SelArgs a) {
         carry = load4(held + (nb * 3 * kSelThreads + tid) * 4);
         rate = mine && has ? load_rates(a, ch, n0) : zero4();
       }
-      const float* row = bc + (has ? n0 : 0);
+      const float* row = bc + nb * 4 * LN + sl * 4;
       Four h = zero4();
-      if (!ENDS) {
-        if (mine && has) h = load4(a.checkpoints + ((p.b * a.nchunks + chunk) * a.dim + ch) * np + n0);
+      auto start = [&](int t) {
+        const int r = flags.row[t];
+        h = a.init.data && r >= 0 && mine && has ? load_state(a.init, r, ch, n0, a.dstate) : zero4();
+      };
+      if constexpr (!ENDS) {
+        if (mine && has) h = load4(a.checkpoints + ((p.b * a.nchunks + i) * a.dim + ch) * np + n0);
 #pragma unroll 1
-        for (int q = 0; q < kSelChunk / 4; ++q) {
+        for (int q = 0; q < TT / 4; ++q) {
           store4(sub + (q * kSelThreads + tid) * 4, h);
+          if (q == TT / 4 - 1) break;
           const uint32_t f = flags.word[q];
-          const bool inside = f == kAllInside;
+          const bool in = f == kAllInside;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int t = q * 4 + j;
-            const uint32_t fj = f >> (8 * j);
-            if (!inside) {
-              if (!(fj & kValid)) continue;
-              if (fj & kFirst) {
-                const int r = flags.row[t];
-                h = a.init.data && r >= 0 && mine && has ? load_state(a.init, r, ch, n0, a.dstate) : zero4();
-              }
-            }
+            if (!in && (f >> (8 * j) & kFirst)) start(t);
             const float4 v = io[t * PITCH + c];
             const float sx = v.x * v.y;
-            const Four B = load4(row + t * 2 * np);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) h.v[i] = fmaf(ex2_approx(v.x * rate.v[i]), h.v[i], sx * B.v[i]);
+            h = fma4(decays4(make_float2(v.x, v.x), rate), h, mul4(load4(row + t * 2 * wide), make_float2(sx, sx)));
           }
         }
       }
       Four da_tile = zero4();
 #pragma unroll 1
-      for (int q = kSelChunk / 4 - 1; q >= 0; --q) {
+      for (int q = TT / 4 - 1; q >= 0; --q) {
         const uint32_t f = flags.word[q];
-        const bool inside = f == kAllInside;
-        float decay[4][4], kept[4][4], now[4][4];  // a, a h_{t-1} and h of the four positions
+        const bool in = f == kAllInside;
+        Four decay[4], kept[4], now[4];  // a, a h_{t-1} and h of the four positions
         if (!ENDS) h = load4(sub + (q * kSelThreads + tid) * 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int t = q * 4 + j;
-          const uint32_t fj = f >> (8 * j);
-          if (!inside && !ENDS && (fj & kFirst)) {
-            const int r = flags.row[t];
-            h = a.init.data && r >= 0 && mine && has ? load_state(a.init, r, ch, n0, a.dstate) : zero4();
-          }
+          if (!in && !ENDS && (f >> (8 * j) & kFirst)) start(t);
           const float4 v = io[t * PITCH + c];
-          const float sx = v.x * v.y;
-          const Four B = load4(row + t * 2 * np);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            decay[j][i] = ex2_approx(v.x * rate.v[i]);
-            if (ENDS) continue;
-            kept[j][i] = decay[j][i] * h.v[i];
-            h.v[i] = fmaf(sx, B.v[i], kept[j][i]);
-            now[j][i] = h.v[i];
+          decay[j] = decays4(make_float2(v.x, v.x), rate);
+          if constexpr (!ENDS) {
+            const float sx = v.x * v.y;
+            kept[j] = mul4(decay[j], h);
+            h = now[j] = fma4(load4(row + t * 2 * wide), make_float2(sx, sx), kept[j]);
           }
         }
         float y[4], sa[4], sb[4];  // sums over the states of C h, g a h_{t-1} A and g B
 #pragma unroll
         for (int j = 3; j >= 0; --j) {
-          const int t = q * 4 + j;
+          const int t = q * 4 + j, r = in ? 0 : flags.row[t];
           const uint32_t fj = f >> (8 * j);
-          y[j] = sa[j] = sb[j] = 0.f;
-          float bcs[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) bcs[i] = 0.f;
-          if (inside || (fj & kValid)) {
-            if (!inside && (fj & kLast)) {
-              const int r = flags.row[t];
-              carry = a.dfinal.data && r >= 0 && mine && has ? load_state(a.dfinal, r, ch, n0, a.dstate) : zero4();
-            }
-            const float4 v = io[t * PITCH + c];
+          if (!in && (fj & kLast)) carry = a.dfinal.data && r >= 0 && mine && has ? load_state(a.dfinal, r, ch, n0, a.dstate) : zero4();
+          const float4 v = io[t * PITCH + c];
+          const float2 dy = make_float2(v.z, v.z);
+          const Four C = load4(row + t * 2 * wide + wide);
+          Four g = fma4(C, dy, carry);
+          Four dB, dC;
+          if constexpr (!ENDS) {
             const float sx = v.x * v.y;
-            const Four B = load4(row + t * 2 * np), C = load4(row + t * 2 * np + np);
-            if (ENDS && nb == 0) total += v.x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float g = fmaf(C.v[i], v.z, carry.v[i]);
-              carry.v[i] = decay[j][i] * g;
-              if (ENDS) continue;
-              bcs[i] = g * sx;
-              bcs[4 + i] = v.z * now[j][i];
-              y[j] = fmaf(C.v[i], now[j][i], y[j]);
-              sb[j] = fmaf(g, B.v[i], sb[j]);
-              const float w = g * kept[j][i];
-              sa[j] = fmaf(w, rate.v[i], sa[j]);
-              da_tile.v[i] = fmaf(w, v.x, da_tile.v[i]);
-            }
-            if (!inside && (fj & kFirst)) {
-              const int r = flags.row[t];
-              if (!ENDS && a.dinit.data && r >= 0 && mine && has) store_state(a.dinit, r, ch, n0, a.dstate, carry);
-              carry = zero4();
-              if (ENDS) total = INFINITY;
-            }
+            Four w = mul4(g, kept[j]);
+            dC = mul4(now[j], dy);
+            if (!in && !(fj & kValid)) g = w = dC = zero4();  // padding: h may hold what a NaN has left
+            dB = mul4(g, make_float2(sx, sx));
+            y[j] = dot4(C, now[j]);
+            sb[j] = dot4(load4(row + t * 2 * wide), g);
+            sa[j] = dot4(w, rate);
+            da_tile = fma4(w, make_float2(v.x, v.x), da_tile);
+          } else if (nb == 0) {
+            total += v.x;
           }
-          if (!ENDS) {
-            if (p.channels < CH && !mine)  // so that 0 * infinity of no channel does not count
-#pragma unroll
-              for (int i = 0; i < 8; ++i) bcs[i] = 0.f;
-            const int which = sum_channels<LN>(bcs, lane);
-            if ((lane & 3) < LN) slabs[warp * (Smem::kSlab / 4) + t * 8 * LN + (which >> 2) * 4 * LN + sl * 4 + (which & 3)] = bcs[0];
+          carry = mul4(decay[j], g);
+          if (!in && (fj & kFirst)) {
+            if (!ENDS && a.dinit.data && r >= 0 && mine && has) store_state(a.dinit, r, ch, n0, a.dstate, carry);
+            if (ENDS) total = INFINITY;
+          }
+          // a gradient reaches a position from the next one of its sequence only
+          if (!in && (!(fj & kValid) || (fj & kFirst))) carry = zero4();
+          if constexpr (!ENDS) {
+            if (!all_channels && !mine) dB = dC = zero4();  // so that 0 * infinity of no channel does not count
+            const float v8 = sum_channels<LN>(dB, dC, lane);
+            const int which = summed(lane);
+            if ((lane & 3) < LN) slabs[warp * (Smem::kSlab / 4) + t * 8 * LN + (which >> 2) * 4 * LN + sl * 4 + (which & 3)] = v8;
           }
         }
-        if (ENDS) continue;
-        if (!has)
+        if constexpr (!ENDS) {
+          sum_lanes<LN>(y, sl);
+          sum_lanes<LN>(sa, sl);
+          sum_lanes<LN>(sb, sl);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = sa[j] = sb[j] = 0.f;
-        sum_lanes<LN>(y, sl);
-        sum_lanes<LN>(sa, sl);
-        sum_lanes<LN>(sb, sl);
-#pragma unroll
-        for (int j = 0; j < 4 / LN; ++j) {
-          const int t = q * 4 + sl * (4 / LN) + j;
-          float* s = sums + (t * PITCH + c) * 3;
-          if (nb > 0) {
-            y[j] += s[0];
-            sa[j] += s[1];
-            sb[j] += s[2];
+          for (int j = 0; j < 4 / LN; ++j) {
+            const int t = q * 4 + sl * (4 / LN) + j;
+            float* s = sums + (t * PITCH + c) * 3;
+            if (nb > 0) {
+              y[j] += s[0];
+              sa[j] += s[1];
+              sb[j] += s[2];
+            }
+            if (nb + 1 < a.blocks) {
+              s[0] = y[j];
+              s[1] = sa[j];
+              s[2] = sb[j];
+              continue;
+            }
+            const float4 v = io[t * PITCH + c];
+            const float du = fmaf(sa[j], 0.693147181f, v.y * sb[j]) * v.w;
+            io[t * PITCH + c] = make_float4(fmaf(v.x, sb[j], skip * v.z), du, fmaf(skip, v.y, y[j]), 0.f);
+            add_to(dbias, dbias_low, du);
+            add_to(dskip, dskip_low, v.z * v.y);
           }
-          if (nb + 1 < a.blocks) {
-            s[0] = y[j];
-            s[1] = sa[j];
-            s[2] = sb[j];
-            continue;
-          }
-          const float4 v = io[t * PITCH + c];
-          const float du = fmaf(sa[j], 0.693147181f, v.y * sb[j]) * v.w;
-          __syncwarp();  // the channel's other lanes have read theirs
-          io[t * PITCH + c] = make_float4(fmaf(v.x, sb[j], skip * v.z), du, fmaf(skip, v.y, y[j]), 0.f);
-          add_to(dbias, dbias_low, du);
-          add_to(dskip, dskip_low, v.z * v.y);
         }
       }
       if (a.blocks > 1) store4(held + (nb * 3 * kSelThreads + tid) * 4, carry);
-      if (ENDS) continue;
-      if (a.blocks > 1) {
-        da = load4(held + ((nb * 3 + 1) * kSelThreads + tid) * 4);
-        da_low = load4(held + ((nb * 3 + 2) * kSelThreads + tid) * 4);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) add_to(da.v[i], da_low.v[i], da_tile.v[i]);
-      if (a.blocks > 1) {
-        store4(held + ((nb * 3 + 1) * kSelThreads + tid) * 4, da);
-        store4(held + ((nb * 3 + 2) * kSelThreads + tid) * 4, da_low);
-      }
-      __syncthreads();
-      // this pass's states of dB and dC: the warps' sums to the CTA's
-      for (int e = tid; e < kSelChunk * 8 * LN; e += kSelThreads) {
-        const int t = e / (8 * LN), v = e % (8 * LN), n = nb * kSelBlock + v % (4 * LN);
-        if (t0 + t >= a.seqlen || n >= np) continue;
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) s += slabs[w * (Smem::kSlab / 4) + e];
-        a.parts_bc[(((p.b * a.seqlen + t0 + t) * a.tiles + p.tile) * 2 + v / (4 * LN)) * np + n] = s;
-      }
-      if (nb + 1 < a.blocks) __syncthreads();
-    }
-    if (ENDS) continue;
-#pragma unroll 4
-    for (int e = tid; e < kSelChunk * CH; e += kSelThreads) {
-      int t, cc;
-      tile_place<CH>(a.rows, e, t, cc);
-      if (cc >= p.channels || t0 + t >= a.seqlen) continue;
-      const int64_t d = p.ch0 + cc;
-      const bool valid = reinterpret_cast<const uint8_t*>(flags.word)[t] & kValid;
-      const float4 v = valid ? io[t * PITCH + cc] : make_float4(0.f, 0.f, 0.f, 0.f);
-      store_el<T>(a.dx, p.b, d, t0 + t, v.x);
-      store_el<T>(a.ddelta, p.b, d, t0 + t, v.y);
-      if (a.z.data) {
-        float dz = 0.f;
-        if (valid) {
-          // silu'(z) = s + z s (1 - s)
-          const float z = load_el<T>(a.z, p.b, d, t0 + t);
-          float s, less;
-          sigmoid_pair_of<T>(z, s, less);
-          dz = load_el<T>(a.dout, p.b, d, t0 + t) * v.z * fmaf(z * s, less, s);
+      if constexpr (!ENDS) {
+        if (a.blocks > 1) {
+          da = load4(held + ((nb * 3 + 1) * kSelThreads + tid) * 4);
+          da_low = load4(held + ((nb * 3 + 2) * kSelThreads + tid) * 4);
         }
-        store_el<T>(a.dz, p.b, d, t0 + t, dz);
+        add_to(da, da_low, da_tile);
+        if (a.blocks > 1) {
+          store4(held + ((nb * 3 + 1) * kSelThreads + tid) * 4, da);
+          store4(held + ((nb * 3 + 2) * kSelThreads + tid) * 4, da_low);
+        }
+        __syncthreads();
+        // this pass's states of dB and dC: the warps' sums to the CTA's
+        for (int e = tid; e < TT * 8 * LN; e += kSelThreads) {
+          const int t = e / (8 * LN), v = e % (8 * LN), n = nb * kSelBlock + v % (4 * LN);
+          if (t0 + t >= a.seqlen || n >= np) continue;
+          float s = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) s += slabs[w * (Smem::kSlab / 4) + e];
+          a.parts_bc[(((p.b * a.seqlen + t0 + t) * a.tiles + p.tile) * 2 + v / (4 * LN)) * np + n] = s;
+        }
+        if (nb + 1 < a.blocks) __syncthreads();
       }
     }
+    if constexpr (!ENDS) {
+      float o[8];
+#pragma unroll
+      for (int part = 0; part < 3; ++part) {
+        if (part == 2 && !a.z.data) break;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
+          const float4 v = io[t * PITCH + cc];
+          o[k] = part == 0 ? v.x : part == 1 ? v.y : dzf[k] * v.z;
+          if (packed && !flags.valid(t)) o[k] = 0.f;
+        }
+        if (part == 0) dxs.store(a, a.dx, p, i, whole, o);
+        else if (part == 1) ddeltas.store(a, a.ddelta, p, i, whole, o);
+        else dzs.store(a, a.dz, p, i, whole, o);
+      }
+    }
+    __syncthreads();
   }
 
   for (int nb = 0; nb < a.blocks; ++nb) {
     const int n0 = nb * kSelBlock + sl * kSelStates;
     if (n0 >= np || !mine) continue;
-    if (ENDS) {
+    if constexpr (ENDS) {
       if (a.blocks > 1) carry = load4(held + (nb * 3 * kSelThreads + tid) * 4);
       store4(a.ends + ends_at + p.seg * a.dim * np + n0, carry);
     } else {
@@ -335,12 +342,11 @@ __global__ void __launch_bounds__(kSelThreads) sel_bwd_kernel(const SelArgs a) {
         da = load4(held + ((nb * 3 + 1) * kSelThreads + tid) * 4);
         da_low = load4(held + ((nb * 3 + 2) * kSelThreads + tid) * 4);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) da.v[i] += da_low.v[i];
-      store4(a.parts_a + ((p.b * a.segments + p.seg) * a.dim + ch) * np + n0, da);
+      store4(a.parts_a + ((p.b * a.segments + p.seg) * a.dim + ch) * np + n0,
+             Four{fadd2(da.lo, da_low.lo), fadd2(da.hi, da_low.hi)});
     }
   }
-  if (ENDS) {
+  if constexpr (ENDS) {
     if (mine && sl == 0) a.steps[(p.b * a.segments + p.seg) * a.dim + ch] = total;
     return;
   }
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(kSelThreads) sel_bwd_kernel(const SelArgs a) {
 
 // dB and dC: the sums over a group's CTAs.  A thread takes one state of one position.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sel_sum_bc_kernel(const SelArgs a) {
+__global__ void __launch_bounds__(kThreads) sel_sum_bc_kernel(const __grid_constant__ SelArgs a) {
   grid_dependency_wait();
   const int64_t per = 2 * a.padded;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
@@ -378,7 +384,7 @@ __global__ void __launch_bounds__(kThreads) sel_sum_bc_kernel(const SelArgs a) {
 }
 
 // dA, dD and dbias: the sums over batch rows and segments.
-__global__ void __launch_bounds__(kThreads) sel_sum_params_kernel(const SelArgs a) {
+__global__ void __launch_bounds__(kThreads) sel_sum_params_kernel(const __grid_constant__ SelArgs a) {
   grid_dependency_wait();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t na = a.dim * a.padded, rows = a.batch * a.segments;
@@ -400,19 +406,25 @@ __global__ void __launch_bounds__(kThreads) sel_sum_params_kernel(const SelArgs 
   }
 }
 
-template <typename T, int LN, bool ENDS>
+template <typename T, int LN, bool ROWS, bool ENDS>
 cudaError_t launch(const SelArgs& a, cudaStream_t s) {
   const size_t smem = static_cast<size_t>(BwdSmem<LN>::bytes(a));
-  const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(sel_bwd_kernel<T, LN, ENDS>), smem);
+  const auto kernel = sel_bwd_kernel<T, LN, ROWS, ENDS>;
+  const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  return launch_dependent(sel_bwd_kernel<T, LN, ENDS>, dim3(static_cast<unsigned>(a.batch * a.segments * a.tiles)), dim3(kSelThreads), smem, s, a);
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(a.batch * a.segments * a.tiles)), dim3(kSelThreads), smem, s, a);
+}
+
+template <typename T, int LN, bool ROWS>
+cudaError_t main_kernels(const SelArgs& a, cudaStream_t s) {
+  cudaError_t e = cudaSuccess;
+  if (a.segments > 1) e = launch<T, LN, ROWS, true>(a, s);
+  return e == cudaSuccess ? launch<T, LN, ROWS, false>(a, s) : e;
 }
 
 template <typename T, int LN>
 cudaError_t run(const SelArgs& a, cudaStream_t s) {
-  cudaError_t e = cudaSuccess;
-  if (a.segments > 1) e = launch<T, LN, true>(a, s);
-  if (e == cudaSuccess) e = launch<T, LN, false>(a, s);
+  cudaError_t e = a.rows ? main_kernels<T, LN, true>(a, s) : main_kernels<T, LN, false>(a, s);
   const int64_t bc = a.batch * a.seqlen * a.groups * 2 * a.padded, params = a.dim * (a.padded + 2);
   if (e == cudaSuccess)
     e = launch_dependent(sel_sum_bc_kernel<T>, dim3(static_cast<unsigned>((bc + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);

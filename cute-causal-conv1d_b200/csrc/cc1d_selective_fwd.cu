@@ -4,45 +4,55 @@
 //     y_t = sum_n C_t[n] h_t[n] + D x_t      out_t = y_t silu(z_t)
 //
 // A CTA of 128 threads owns up to 32 channels (64 or 128 for at most 8 or 4 states) of one batch
-// row and walks the sequence in tiles of 32 positions.  A thread holds four states of a channel
-// in registers; the step sizes of a tile are made once, by all threads, and with B and C lie in
-// shared memory as fp32.
+// row and walks the sequence in tiles of 32 (16, 8) positions.  A thread holds four states of a
+// channel in registers and goes through the tile one position after the other; the step sizes of
+// a tile are made once, by all threads, and with B and C lie in shared memory as fp32.  The
+// next tile's inputs are on their way to registers meanwhile.
 #include "cc1d_selective.cuh"
 
 namespace cc1d {
 namespace {
 
-// Shared memory: flags; (s, s x) by position and channel; B and C; y by position and channel; with
-// several passes the states between two tiles.
+#ifndef FWDC
+#define FWDC 4
+#endif
+constexpr int kFwdCtas = FWDC;
+// Shared memory: flags; (s, s, s x, s x) by position and channel; y by position and channel; B and
+// C; with several passes the states between two tiles.
 template <int LN>
 struct FwdSmem {
-  static constexpr int CH = kSelThreads / LN;
   static constexpr int kFlags = 256;
-  static constexpr int kIo = kSelChunk * (CH + 1) * 8;
-  static constexpr int kY = (kSelChunk * (CH + 1) * 4 + 15) / 16 * 16;
-  static __host__ __device__ int64_t bytes(const SelArgs& a) {
-    return kFlags + kIo + kY + kSelChunk * 2 * a.padded * 4 + (a.blocks > 1 ? a.blocks * kSelThreads * 16 : 0);
+  static constexpr int kIo = Tile<LN, false>::T * Tile<LN, false>::PITCH * 16;
+  static constexpr int kY = (Tile<LN, false>::T * Tile<LN, false>::PITCH * 4 + 15) / 16 * 16;
+  static int64_t bytes(const SelArgs& a) {
+    return kFlags + kIo + kY + Tile<LN, false>::T * 8 * LN * a.blocks * 4 + (a.blocks > 1 ? a.blocks * kSelThreads * 16 : 0);
   }
 };
 
 // ENDS: only what each segment carries out of itself, for the segments behind it.
-template <typename T, int LN, bool ENDS>
-__global__ void __launch_bounds__(kSelThreads) sel_fwd_kernel(const SelArgs a) {
-  constexpr int CH = kSelThreads / LN;
-  constexpr int PITCH = CH + 1;
+template <typename T, int LN, bool ROWS, bool ENDS>
+__global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __grid_constant__ SelArgs a) {
+  using Where = Tile<LN, ROWS>;
+  constexpr int PITCH = Where::PITCH, TT = Where::T;
   extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float biases[Where::CH], skips[Where::CH];
   SelFlags& flags = *reinterpret_cast<SelFlags*>(smem);
-  float2* io = reinterpret_cast<float2*>(smem + FwdSmem<LN>::kFlags);
+  float4* io = reinterpret_cast<float4*>(smem + FwdSmem<LN>::kFlags);
   float* ys = reinterpret_cast<float*>(smem + FwdSmem<LN>::kFlags + FwdSmem<LN>::kIo);
   float* bc = reinterpret_cast<float*>(smem + FwdSmem<LN>::kFlags + FwdSmem<LN>::kIo + FwdSmem<LN>::kY);
-  const int np = static_cast<int>(a.padded);
-  float* held = bc + kSelChunk * 2 * np;
+  const int np = static_cast<int>(a.padded), wide = 4 * LN * a.blocks;
+  float* held = bc + TT * 2 * wide;
 
   const SelPlace p = sel_place<LN>(a);
   const int tid = threadIdx.x, sl = tid % LN, c = tid / LN;
   const bool mine = c < p.channels;
   const int64_t ch = p.ch0 + (mine ? c : 0);
   grid_dependency_wait();
+  for (int i = tid; i < Where::CH; i += kSelThreads) {
+    const bool is = i < p.channels;
+    biases[i] = is && a.bias.data ? load_any(a.bias.data, a.bias.dtype, (p.ch0 + i) * a.bias.s0) : 0.f;
+    skips[i] = is && a.D.data ? load_any(a.D.data, a.D.dtype, (p.ch0 + i) * a.D.s0) : 0.f;
+  }
 
   Four h = zero4(), rate = zero4();
   float total = 0.f;  // ENDS: the sum of step sizes since the segment's start
@@ -53,38 +63,44 @@ __global__ void __launch_bounds__(kSelThreads) sel_fwd_kernel(const SelArgs a) {
     h = zero4();
     rate = mine && has ? load_rates(a, ch, n0) : zero4();
     if (!ENDS && mine && has)
-      for (int64_t s = 0; s < p.seg; ++s) {
-        const Four e = load4(a.ends + ends_at + s * a.dim * np + n0);
-        const float sum = a.steps[(p.b * a.segments + s) * a.dim + ch];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h.v[i] = sum < INFINITY && h.v[i] != 0.f ? fmaf(exp2f(rate.v[i] * sum), h.v[i], e.v[i]) : e.v[i];
-      }
+      for (int64_t s = 0; s < p.seg; ++s)
+        h = handed_on(h, rate, a.steps[(p.b * a.segments + s) * a.dim + ch], load4(a.ends + ends_at + s * a.dim * np + n0));
     if (a.blocks > 1) store4(held + (nb * kSelThreads + tid) * 4, h);
   }
 
-  for (int64_t chunk = p.chunk0; chunk < p.chunk1; ++chunk) {
-    const int64_t t0 = chunk * kSelChunk;
-    __syncthreads();  // the last tile's results have been read
-    load_flags(a, p.b, t0, flags);
-    __syncthreads();
-#pragma unroll 4
-    for (int e = tid; e < kSelChunk * CH; e += kSelThreads) {
-      int t, cc;
-      tile_place<CH>(a.rows, e, t, cc);
-      float2 v = make_float2(0.f, 0.f);
-      if (cc < p.channels && (reinterpret_cast<const uint8_t*>(flags.word)[t] & kValid)) {
-        const int64_t d = p.ch0 + cc;
-        float u = load_el<T>(a.delta, p.b, d, t0 + t);
-        const float x = load_el<T>(a.x, p.b, d, t0 + t);
-        if (a.bias.data) u += load_any(a.bias.data, a.bias.dtype, d * a.bias.s0);
-        float slope;
-        v.x = a.softplus ? step_size(u, &slope) : u;
-        v.y = v.x * x;
-      }
-      io[t * PITCH + cc] = v;
+  const Walk<T, LN, ROWS> xs(a.x, p), deltas(a.delta, p), zs(a.z.data ? a.z : a.x, p), outs(a.out, p);
+  const bool all_channels = p.channels == Where::CH, packed = a.seq_idx.data != nullptr;
+  T x[8], next_x[8], next_delta[8], z[8];
+  FlagFeed<TT> feed;
+  Coefficients<T, LN> next_bc;
+  auto inside = [&](int64_t i) { return all_channels && (i + 1) * TT <= a.seqlen; };
+  auto fetch = [&](int64_t i) {
+    const bool whole = inside(i);
+    xs.load(a, a.x, p, i, whole, next_x);
+    deltas.load(a, a.delta, p, i, whole, next_delta);
+    feed.load(a, p.b, i * TT);
+    next_bc.load(a, p, i * TT);
+  };
+  fetch(p.chunk0);
+  for (int64_t i = p.chunk0; i < p.chunk1; ++i) {
+    const int64_t t0 = i * TT;
+    const bool whole = inside(i);
+    feed.store(a, p.b, t0, flags);
+    __syncthreads();  // flags are there
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
+      x[k] = next_x[k];
+      float u = to_f32(next_delta[k]) + biases[cc];
+      float s = a.softplus ? step_size(u) : u;
+      float sx = s * to_f32(x[k]);
+      if ((packed || !whole) && !(flags.valid(t) && cc < p.channels)) s = sx = 0.f;
+      io[t * PITCH + cc] = make_float4(s, s, sx, sx);
     }
-    load_bc<T>(a, p, t0, np, flags, bc);
+    next_bc.store(a, p, t0, flags, bc);
     __syncthreads();
+    if (!ENDS && a.z.data) zs.load(a, a.z, p, i, whole, z);
+    if (i + 1 < p.chunk1) fetch(i + 1);
 
     for (int nb = 0; nb < a.blocks; ++nb) {
       const int n0 = nb * kSelBlock + sl * kSelStates;
@@ -93,39 +109,51 @@ __global__ void __launch_bounds__(kSelThreads) sel_fwd_kernel(const SelArgs a) {
         h = load4(held + (nb * kSelThreads + tid) * 4);
         rate = mine && has ? load_rates(a, ch, n0) : zero4();
       }
-      if (!ENDS && a.checkpoints && mine && has) store4(a.checkpoints + ((p.b * a.nchunks + chunk) * a.dim + ch) * np + n0, h);
-      const float* row = bc + (has ? n0 : 0);
+      if (!ENDS && a.checkpoints && mine && has)
+        store4(a.checkpoints + ((p.b * a.nchunks + i) * a.dim + ch) * np + n0, h);
+      const float* row = bc + nb * 4 * LN + sl * 4;
 #pragma unroll 1
-      for (int q = 0; q < kSelChunk / 4; ++q) {
+      for (int q = 0; q < TT / 4; ++q) {
         const uint32_t f = flags.word[q];
-        const bool inside = f == kAllInside;
         float y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        auto position = [&](int j) {
           const int t = q * 4 + j;
-          const uint32_t fj = f >> (8 * j);
-          y[j] = 0.f;
-          if (!inside) {
-            if (!(fj & kValid)) continue;
-            if (fj & kFirst) {
-              const int r = flags.row[t];
-              h = a.init.data && r >= 0 && mine && has ? load_state(a.init, r, ch, n0, a.dstate) : zero4();
-              if (ENDS) total = INFINITY;
-            }
+          const float4 v = io[t * PITCH + c];
+          const float2 s = make_float2(v.x, v.y), sx = make_float2(v.z, v.w);
+          h = fma4(decays4(s, rate), h, mul4(load4(row + t * 2 * wide), sx));
+          if constexpr (ENDS) {
+            if (nb == 0) total += v.x;
+          } else {
+            y[j] = dot4(load4(row + t * 2 * wide + wide), h);
           }
-          const float2 v = io[t * PITCH + c];
-          const Four B = load4(row + t * 2 * np), C = load4(row + t * 2 * np + np);
-          if (ENDS && nb == 0) total += v.x;
+        };
+        if (f == kAllInside) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            h.v[i] = fmaf(ex2_approx(v.x * rate.v[i]), h.v[i], v.y * B.v[i]);
-            if (!ENDS) y[j] = fmaf(C.v[i], h.v[i], y[j]);
+          for (int j = 0; j < 4; ++j) position(j);
+        } else {
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            const int t = q * 4 + j, r = flags.row[t];
+            const uint32_t fj = f >> (8 * j);
+            float yj = 0.f;
+            if (fj & kValid) {
+              if (fj & kFirst) {
+                h = a.init.data && r >= 0 && mine && has ? load_state(a.init, r, ch, n0, a.dstate) : zero4();
+                if (ENDS) total = INFINITY;
+              }
+              const float4 v = io[t * PITCH + c];
+              h = fma4(decays4(make_float2(v.x, v.y), rate), h, mul4(load4(row + t * 2 * wide), make_float2(v.z, v.w)));
+              if (ENDS && nb == 0) total += v.x;
+              if (!ENDS) yj = dot4(load4(row + t * 2 * wide + wide), h);
+              if (!ENDS && (fj & kLast) && a.final_states.data && r >= 0 && mine && has)
+                store_state(a.final_states, r, ch, n0, a.dstate, h);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e == j) y[e] = yj;
           }
-          if (!inside && !ENDS && (fj & kLast) && a.final_states.data && flags.row[t] >= 0 && mine && has)
-            store_state(a.final_states, flags.row[t], ch, n0, a.dstate, h);
         }
-        if (!ENDS) {
-          if (!has) y[0] = y[1] = y[2] = y[3] = 0.f;
+        if constexpr (!ENDS) {
           sum_lanes<LN>(y, sl);
 #pragma unroll
           for (int j = 0; j < 4 / LN; ++j) {
@@ -136,21 +164,19 @@ __global__ void __launch_bounds__(kSelThreads) sel_fwd_kernel(const SelArgs a) {
       }
       if (a.blocks > 1) store4(held + (nb * kSelThreads + tid) * 4, h);
     }
-    if (ENDS) continue;
     __syncthreads();
-#pragma unroll 4
-    for (int e = tid; e < kSelChunk * CH; e += kSelThreads) {
-      int t, cc;
-      tile_place<CH>(a.rows, e, t, cc);
-      if (cc >= p.channels || t0 + t >= a.seqlen) continue;
-      const int64_t d = p.ch0 + cc;
-      float y = 0.f;
-      if (reinterpret_cast<const uint8_t*>(flags.word)[t] & kValid) {
-        y = ys[t * PITCH + cc];
-        if (a.D.data) y = fmaf(load_any(a.D.data, a.D.dtype, d * a.D.s0), load_el<T>(a.x, p.b, d, t0 + t), y);
-        if (a.z.data) y *= silu_of<T>(load_el<T>(a.z, p.b, d, t0 + t));
+    if constexpr (!ENDS) {
+      float out[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
+        float y = fmaf(skips[cc], a.D.data ? to_f32(x[k]) : 0.f, ys[t * PITCH + cc]);
+        if (a.z.data) y *= silu_of<T>(to_f32(z[k]));
+        if (packed && !flags.valid(t)) y = 0.f;
+        out[k] = y;
       }
-      store_el<T>(a.out, p.b, d, t0 + t, y);
+      outs.store(a, a.out, p, i, whole, out);
+      __syncthreads();  // flags and y have been read
     }
   }
   if (ENDS && mine) {
@@ -164,21 +190,27 @@ __global__ void __launch_bounds__(kSelThreads) sel_fwd_kernel(const SelArgs a) {
   }
 }
 
-template <typename T, int LN, bool ENDS>
+template <typename T, int LN, bool ROWS, bool ENDS>
 cudaError_t launch(const SelArgs& a, cudaStream_t s) {
   const size_t smem = static_cast<size_t>(FwdSmem<LN>::bytes(a));
-  const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(sel_fwd_kernel<T, LN, ENDS>), smem);
+  const auto kernel = sel_fwd_kernel<T, LN, ROWS, ENDS>;
+  const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  return launch_dependent(sel_fwd_kernel<T, LN, ENDS>, dim3(static_cast<unsigned>(a.batch * a.segments * a.tiles)), dim3(kSelThreads), smem, s, a);
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(a.batch * a.segments * a.tiles)), dim3(kSelThreads), smem, s, a);
+}
+
+template <typename T, int LN, bool ROWS>
+cudaError_t run(const SelArgs& a, cudaStream_t s) {
+  if (a.segments > 1) {
+    const cudaError_t e = launch<T, LN, ROWS, true>(a, s);
+    if (e != cudaSuccess) return e;
+  }
+  return launch<T, LN, ROWS, false>(a, s);
 }
 
 template <typename T, int LN>
 cudaError_t run(const SelArgs& a, cudaStream_t s) {
-  if (a.segments > 1) {
-    const cudaError_t e = launch<T, LN, true>(a, s);
-    if (e != cudaSuccess) return e;
-  }
-  return launch<T, LN, false>(a, s);
+  return a.rows ? run<T, LN, true>(a, s) : run<T, LN, false>(a, s);
 }
 
 }  // namespace

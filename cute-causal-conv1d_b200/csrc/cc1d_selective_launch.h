@@ -6,7 +6,7 @@
 
 namespace cc1d {
 
-constexpr int kSelChunk = CC1D_SELECTIVE_CHUNK;  // positions between two checkpoints, and of a tile
+constexpr int kSelChunk = 32;                    // the most positions of a tile, and between two checkpoints
 constexpr int kSelThreads = 128;                 // a CTA of the sequence kernels
 constexpr int kSelStates = 4;                    // states of a channel that a thread holds
 constexpr int kSelBlock = 16;                    // states of a channel that a pass over a tile takes, at most
@@ -23,7 +23,7 @@ struct SelArgs {
   int lanes;                             // threads that share a channel: 1, 2 or 4
   int blocks;                            // passes over a tile: ceil(dstate / 16)
   int64_t padded;                        // dstate rounded up to a multiple of 4
-  int64_t nchunks;                       // ceil(seqlen / kSelChunk)
+  int64_t nchunks;                       // tiles along the sequence: ceil(seqlen / (8 lanes))
   int64_t gdim, group_tiles, tiles;      // channels of a group, CTAs that they take, CTAs of all groups
   int64_t segments, segment_chunks;      // parts of the sequence that run side by side, chunks of one
   bool rows;                             // unit stride along the sequence: threads go along it

@@ -63,6 +63,11 @@ void sel_describe(const SelInputs& v, int64_t n, cc1d_selective_params& p) {
   p.initial_states = describe(v.init);
 }
 
+std::vector<int64_t> kept_shape(int64_t batch, int64_t L, int64_t dim, int64_t N) {
+  const int64_t chunk = CC1D_SELECTIVE_CHUNK(N);
+  return {batch, (L + chunk - 1) / chunk, dim, (N + 3) / 4 * 4};
+}
+
 Tensor sel_workspace(int64_t need, const Tensor& like, cc1d_selective_params& p) {
   if (need < 0) check(CC1D_ERR_VALUE);
   if (need == 0) return Tensor();
@@ -95,7 +100,7 @@ std::tuple<Tensor, Tensor, Tensor> sel_forward(SelInputs v, bool return_final, i
     else final = fp32({n, dim, N}, v.x).zero_();
   }
   if (save)
-    kept = fp32({batch, (L + CC1D_SELECTIVE_CHUNK - 1) / CC1D_SELECTIVE_CHUNK, dim, (N + 3) / 4 * 4}, v.x);
+    kept = fp32(kept_shape(batch, L, dim, N), v.x);
   Tensor out = at::empty_like(v.x);
   cc1d_selective_params p = {};
   sel_describe(v, n, p);
@@ -123,7 +128,7 @@ SelGrads sel_backward(SelInputs v, const Tensor& kept, Tensor dout, const Tensor
   const int64_t G = v.B.size(1);
   expect("dout", dout, v.x.sizes());
   expect("dfinal_states", dfinal, {n, dim, N});
-  expect("checkpoints", kept, {batch, (L + CC1D_SELECTIVE_CHUNK - 1) / CC1D_SELECTIVE_CHUNK, dim, (N + 3) / 4 * 4});
+  expect("checkpoints", kept, kept_shape(batch, L, dim, N));
   one_device({&v.x, &v.delta, &v.A, &v.B, &v.C, &v.D, &v.z, &v.bias, &v.seq_idx, &v.init, &kept, &dout, &dfinal});
   Tensor dx = at::empty_like(v.x), ddelta = at::empty_like(v.x), dz, dD, dbias, dinit;
   Tensor dA = fp32({dim, N}, v.x);

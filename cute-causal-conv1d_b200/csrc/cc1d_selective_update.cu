@@ -12,14 +12,14 @@ namespace {
 template <typename T, bool PACKED>
 __device__ __forceinline__ Four load_inputs(const TensorArg& t, int64_t group_stride, int64_t b, int64_t g, int64_t n0, int64_t l, int64_t dstate) {
   const T* p = static_cast<const T*>(t.data) + b * t.s0 + g * group_stride + l * t.s2;
-  Four f;
+  float f[4];
   if constexpr (PACKED) {
-    unpack<T, 4>(ld_packet<T, 4>(p + n0), f.v);
+    unpack<T, 4>(ld_packet<T, 4>(p + n0), f);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f.v[i] = n0 + i < dstate ? to_f32(p[(n0 + i) * t.s1]) : 0.f;
+    for (int i = 0; i < 4; ++i) f[i] = n0 + i < dstate ? to_f32(p[(n0 + i) * t.s1]) : 0.f;
   }
-  return f;
+  return Four{make_float2(f[0], f[1]), make_float2(f[2], f[3])};
 }
 
 template <typename T, int LANES, int VEC, bool PACKED>
@@ -39,15 +39,11 @@ __global__ void __launch_bounds__(kThreads) sel_update_kernel(const SelUpdateArg
     if (!live || n0 >= a.dstate) continue;
     if constexpr (PACKED) {
       h[v] = load4(static_cast<const float*>(a.state.data) + row * a.state.s0 + d * a.state.s1 + n0);
-      rate[v] = load4(static_cast<const float*>(a.A.data) + d * a.A.s0 + n0);
+      rate[v] = mul4(load4(static_cast<const float*>(a.A.data) + d * a.A.s0 + n0), make_float2(kLog2e, kLog2e));
     } else {
       h[v] = load_state(a.state, row, d, n0, a.dstate);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (n0 + k < a.dstate) rate[v].v[k] = load_any(a.A.data, a.A.dtype, d * a.A.s0 + (n0 + k) * a.A.s1);
+      rate[v] = load_rates(a.A, d, n0, a.dstate);
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) rate[v].v[k] *= kLog2e;
   }
   const float bias = live && a.bias.data ? load_any(a.bias.data, a.bias.dtype, d * a.bias.s0) : 0.f;
   const float skip = live && a.D.data ? load_any(a.D.data, a.D.dtype, d * a.D.s0) : 0.f;
@@ -55,20 +51,17 @@ __global__ void __launch_bounds__(kThreads) sel_update_kernel(const SelUpdateArg
     float y = 0.f, x = 0.f;
     if (live) {
       x = load_el<T>(a.x, b, d, l);
-      float s = load_el<T>(a.delta, b, d, l) + bias, slope;
-      if (a.softplus) s = step_size(s, &slope);
-      const float sx = s * x;
+      float s = load_el<T>(a.delta, b, d, l) + bias;
+      if (a.softplus) s = step_size(s);
+      const float2 s2 = make_float2(s, s), sx = make_float2(s * x, s * x);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
         const int64_t n0 = (v * LANES + sl) * 4;
         if (n0 >= a.dstate) continue;
         const Four B = load_inputs<T, PACKED>(a.B, a.B_group, b, g, n0, l, a.dstate);
         const Four C = load_inputs<T, PACKED>(a.C, a.C_group, b, g, n0, l, a.dstate);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          h[v].v[k] = fmaf(ex2_approx(s * rate[v].v[k]), h[v].v[k], sx * B.v[k]);
-          y = fmaf(C.v[k], h[v].v[k], y);
-        }
+        h[v] = fma4(decays4(s2, rate[v]), h[v], mul4(B, sx));
+        y += dot4(C, h[v]);
       }
     }
 #pragma unroll

@@ -383,7 +383,7 @@ cc1d_status cc1d_add_norm_bwd_launch(const cc1d_add_norm_params* params, void* s
  *   final_states    (nstates, dim, dstate) fp32     optional output, h at the last position.  With
  *                                                   seq_idx only the rows of sequences that have
  *                                                   positions are written: fill the others beforehand
- *   checkpoints     (batch, ceil(seqlen / CC1D_SELECTIVE_CHUNK), dim, dstate rounded up to a multiple
+ *   checkpoints     (batch, ceil(seqlen / CC1D_SELECTIVE_CHUNK(dstate)), dim, dstate rounded up to a multiple
  *                   of 4) fp32 contiguous, 16-byte aligned: h before each chunk; written by the
  *                   forward if given, read by the backward
  *   workspace       device scratch of cc1d_selective_{fwd,bwd}_workspace_bytes(params) bytes, 16-byte
@@ -398,7 +398,7 @@ cc1d_status cc1d_add_norm_bwd_launch(const cc1d_add_norm_params* params, void* s
  * dout (batch, dim, seqlen) has x's dtype; dfinal_states (nstates, dim, dstate) fp32 is optional.
  * The forward ignores the gradient fields and the backward final_states and out.
  */
-#define CC1D_SELECTIVE_CHUNK 32
+#define CC1D_SELECTIVE_CHUNK(dstate) ((dstate) <= 4 ? 8 : (dstate) <= 8 ? 16 : 32)
 #define CC1D_SELECTIVE_MAX_STATES 256
 
 typedef struct cc1d_selective_params {

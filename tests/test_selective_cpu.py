@@ -355,8 +355,9 @@ C_PROBE = r"""
 #include <stdio.h>
 #include "causal_conv1d_b200.h"
 int main(void) {
-  printf("%zu %zu %zu %zu %zu %d %d %d\n", sizeof(cc1d_selective_params), sizeof(cc1d_selective_update_params),
-         sizeof(cc1d_beam_select_params), sizeof(cc1d_beam_rows), sizeof(cc1d_beam_reorder_params), CC1D_SELECTIVE_CHUNK,
+  printf("%zu %zu %zu %zu %zu %d %d %d %d %d\n", sizeof(cc1d_selective_params), sizeof(cc1d_selective_update_params),
+         sizeof(cc1d_beam_select_params), sizeof(cc1d_beam_rows), sizeof(cc1d_beam_reorder_params), CC1D_SELECTIVE_CHUNK(4),
+         CC1D_SELECTIVE_CHUNK(8), CC1D_SELECTIVE_CHUNK(9),
          CC1D_SELECTIVE_MAX_STATES, CC1D_BEAM_MAX);
   printf("%zu %zu %zu %zu\n", offsetof(cc1d_selective_params, x), offsetof(cc1d_selective_params, dA),
          offsetof(cc1d_selective_update_params, out), offsetof(cc1d_beam_select_params, out_scores));
@@ -374,7 +375,7 @@ def test_params_layout(tmp_path):
         pytest.skip("gcc unavailable")
     got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [_abi.SELECTIVE_PARAMS.size, _abi.SELECTIVE_UPDATE_PARAMS.size, _abi.BEAM_SELECT_PARAMS.size,
-                   _abi.BEAM_ROWS.size, _abi.BEAM_REORDER_PARAMS.size, _abi.SELECTIVE_CHUNK, 256, 64,
+                   _abi.BEAM_ROWS.size, _abi.BEAM_REORDER_PARAMS.size, *map(_abi.selective_chunk, (4, 8, 9)), 256, 64,
                    56, 56 + 20 * 40 + 32, 56 + 10 * 40, 40 + 80 + 24]
 
 
@@ -387,7 +388,7 @@ def test_torch_ops_registered_with_fake_shapes():
         A, D, init = torch.empty(64, 5), torch.empty(64), torch.empty(2, 64, 5)
         bc = torch.empty(2, 70, 5, dtype=torch.bfloat16).transpose(1, 2)
         out, final, ck = ops.selective_recurrence_fwd(x, x, A, bc, bc, D, x, D, True, None, init, True, 0, True)
-        assert out.stride() == x.stride() and final.shape == (2, 64, 5) and ck.shape == (2, 3, 64, 8)
+        assert out.stride() == x.stride() and final.shape == (2, 64, 5) and ck.shape == (2, 5, 64, 8)
         g = ops.selective_recurrence_bwd(x, x, A, bc, bc, None, None, D, True, None, init, ck, x, final, True, True)
         assert g[0].stride() == x.stride() and g[3].shape == bc.shape and g[3].stride() == bc.stride()
         assert g[2].shape == A.shape and g[5].numel() == 0 and g[6].numel() == 0 and g[8].shape == init.shape
