@@ -18,10 +18,18 @@ __device__ __forceinline__ float softplus_of_exp(float u, float e) {
   q = fmaf(q, w, 2.f);
   return fmaf(s, q, fmaxf(u, 0.f));
 }
-__device__ __forceinline__ float step_size(float u) { return softplus_of_exp(u, exp_minus(fabsf(clamp_exponent(u)))); }
+// exp(-|u|); for 16-bit tensors the rounding of the exponent is left in it (|u| 2^-24 of it).
+template <typename T>
+__device__ __forceinline__ float exp_of_size(float u) {
+  if constexpr (std::is_same<T, float>::value) return exp_minus(min_nan(fabsf(u), 88.f));
+  else return ex2_approx(-kLog2e * fabsf(u));
+}
+template <typename T>
+__device__ __forceinline__ float step_size(float u) { return softplus_of_exp(u, exp_of_size<T>(u)); }
 // The same, and its derivative sigmoid(u).
+template <typename T>
 __device__ __forceinline__ float step_size(float u, float* slope) {
-  const float e = exp_minus(fabsf(clamp_exponent(u)));
+  const float e = exp_of_size<T>(u);
   const float r = rcp_approx(1.f + e);
   *slope = u < 0.f ? e * r : r;
   return softplus_of_exp(u, e);
@@ -150,60 +158,79 @@ struct Walk {
   }
 };
 
-// B and C of a tile's positions as fp32 [position][B, C][wide], wide = 4 LN per pass; zero past
-// dstate and where a position is not valid, so that whatever stands there is not used.  A thread
-// has element e = threadIdx.x + 128 k, along the states or, where that is B's unit stride, along the
-// sequence; the eight of a single pass are loaded a tile ahead.
-template <typename T, int LN>
+// B and C of a tile's positions in shared memory, in their own type, since what a load from there
+// brings to registers is what it costs: [position][B, C][wide], wide = 4 LN per pass; zero past
+// dstate and where a position is not valid, so that whatever stands there is not used.  The threads
+// go along the states or, where that is B's unit stride, along the sequence; the eight elements
+// of a thread for a single pass are loaded a tile ahead.
+template <typename T, int LN, bool MULTI>
 struct Coefficients {
-  static constexpr int TT = 8 * LN, HELD = TT * 8 * LN / kSelThreads > 0 ? TT * 8 * LN / kSelThreads : 1;
+  static constexpr int TT = 8 * LN, ALL = TT * 8 * LN, HELD = MULTI || ALL < kSelThreads ? 1 : ALL / kSelThreads;
+  static constexpr int DT = kSelThreads / (8 * LN), DN = kSelThreads / TT, HALF = HELD > 1 ? HELD / 2 : 1;
   T v[HELD];
-  static __device__ __forceinline__ void place(const SelArgs& a, int e, int& t, int& n, bool& is_c) {
-    const int wide = 4 * LN * a.blocks;
+  const T *p, *pc;  // along the states: the thread's tensor; else B and C
+  int n, t;
+  bool along, is_c;
+  __device__ __forceinline__ Coefficients(const SelArgs& a, const SelPlace& at) {
+    along = a.B.s1 == 1 || a.B.s2 != 1;
+    const int e = threadIdx.x;
     int s;
-    if (a.B.s1 == 1 || a.B.s2 != 1) {
-      t = a.blocks == 1 ? e / (8 * LN) : e / (2 * wide);
-      s = a.blocks == 1 ? e % (8 * LN) : e - t * 2 * wide;
-    } else {
-      t = e % TT;
-      s = e / TT;
-    }
-    is_c = s >= wide;
-    n = is_c ? s - wide : s;
+    if (along) t = e / (8 * LN), s = e % (8 * LN);
+    else t = e % TT, s = e / TT;
+    is_c = s >= 4 * LN;
+    n = is_c ? s - 4 * LN : s;
+    const T* b = static_cast<const T*>(a.B.data) + at.b * a.B.s0 + at.group * a.B_group;
+    const T* c = static_cast<const T*>(a.C.data) + at.b * a.C.s0 + at.group * a.C_group;
+    p = is_c ? c + n * a.C.s1 + t * a.C.s2 : b + n * a.B.s1 + t * a.B.s2;
+    pc = c + n * a.C.s1 + t * a.C.s2;
   }
-  static __device__ __forceinline__ T fetch(const SelArgs& a, const SelPlace& p, int64_t t, int n, bool is_c) {
-    const TensorArg& x = is_c ? a.C : a.B;
-    if (n >= a.dstate || t >= a.seqlen) return from_f32<T>(0.f);
-    return static_cast<const T*>(x.data)[p.b * x.s0 + p.group * (is_c ? a.C_group : a.B_group) + n * x.s1 + t * x.s2];
-  }
-  __device__ __forceinline__ void load(const SelArgs& a, const SelPlace& p, int64_t t0) {
-    if (a.blocks != 1) return;
+  __device__ __forceinline__ void load(const SelArgs& a, int64_t t0, bool whole) {
+    if constexpr (MULTI) return;
+    if (ALL < kSelThreads && threadIdx.x >= ALL) return;
+    if (along) {
+      const int64_t s2 = is_c ? a.C.s2 : a.B.s2;
+      const T* q = p + t0 * s2;
+      if (n >= a.dstate) {
 #pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-      int t, n;
-      bool is_c;
-      const int e = threadIdx.x + k * kSelThreads;
-      place(a, e, t, n, is_c);
-      v[k] = e < TT * 8 * LN ? fetch(a, p, t0 + t, n, is_c) : from_f32<T>(0.f);
-    }
-  }
-  __device__ __forceinline__ void store(const SelArgs& a, const SelPlace& p, int64_t t0, const SelFlags& s, float* bc) const {
-    const int wide = 4 * LN * a.blocks;
-    if (a.blocks == 1) {
+        for (int k = 0; k < HELD; ++k) v[k] = from_f32<T>(0.f);
+      } else if (whole) {
 #pragma unroll
-      for (int k = 0; k < HELD; ++k) {
-        int t, n;
-        bool is_c;
-        const int e = threadIdx.x + k * kSelThreads;
-        place(a, e, t, n, is_c);
-        if (e < TT * 8 * LN) bc[(t * 2 + is_c) * 4 * LN + n] = s.valid(t) ? to_f32(v[k]) : 0.f;
+        for (int k = 0; k < HELD; ++k, q += DT * s2) v[k] = *q;
+      } else {
+#pragma unroll
+        for (int k = 0; k < HELD; ++k, q += DT * s2) v[k] = t0 + t + k * DT < a.seqlen ? *q : from_f32<T>(0.f);
       }
     } else {
+      const bool in = t0 + t < a.seqlen;
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) {
+        const bool c = k >= HALF || is_c;
+        const T* q = (k >= HALF ? pc : p) + t0 * (c ? a.C.s2 : a.B.s2) + k % HALF * DN * (c ? a.C.s1 : a.B.s1);
+        v[k] = in && n + k % HALF * DN < a.dstate ? *q : from_f32<T>(0.f);
+      }
+    }
+  }
+  // checked: a position may not be valid
+  __device__ __forceinline__ void store(const SelArgs& a, const SelPlace& at, int64_t t0, bool checked, const SelFlags& f, T* bc) const {
+    if constexpr (MULTI) {
+      const int wide = 4 * LN * a.blocks;
       for (int e = threadIdx.x; e < TT * 2 * wide; e += kSelThreads) {
-        int t, n;
-        bool is_c;
-        place(a, e, t, n, is_c);
-        bc[(t * 2 + is_c) * wide + n] = s.valid(t) ? to_f32(fetch(a, p, t0 + t, n, is_c)) : 0.f;
+        const int tt = along ? e / (2 * wide) : e % TT, s = along ? e - tt * 2 * wide : e / TT;
+        const bool c = s >= wide;
+        const int nn = c ? s - wide : s;
+        const TensorArg& x = c ? a.C : a.B;
+        T r = from_f32<T>(0.f);
+        if (nn < a.dstate && f.valid(tt))
+          r = static_cast<const T*>(x.data)[at.b * x.s0 + at.group * (c ? a.C_group : a.B_group) + nn * x.s1 + (t0 + tt) * x.s2];
+        bc[(tt * 2 + c) * wide + nn] = r;
+      }
+    } else {
+      if (ALL < kSelThreads && threadIdx.x >= ALL) return;
+      T* o = bc + (t * 2 + is_c) * 4 * LN + n;
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) {
+        const int at_k = along ? k * DT * 8 * LN : (k >= HALF) * 4 * LN + k % HALF * DN;
+        o[at_k] = checked && !f.valid(along ? t + k * DT : t) ? from_f32<T>(0.f) : v[k];
       }
     }
   }
@@ -229,6 +256,13 @@ __device__ __forceinline__ Four load4(const float* p) {
 }
 __device__ __forceinline__ void store4(float* p, const Four& f) {
   *reinterpret_cast<float4*>(p) = make_float4(f.lo.x, f.lo.y, f.hi.x, f.hi.y);
+}
+// Four neighbouring elements, on their alignment.
+template <typename T>
+__device__ __forceinline__ Four load4_of(const T* p) {
+  float v[4];
+  unpack<T, 4>(*reinterpret_cast<const Packet<T, 4>*>(p), v);
+  return Four{make_float2(v[0], v[1]), make_float2(v[2], v[3])};
 }
 __device__ __forceinline__ Four fma4(const Four& a, const Four& b, const Four& c) { return Four{ffma2(a.lo, b.lo, c.lo), ffma2(a.hi, b.hi, c.hi)}; }
 __device__ __forceinline__ Four mul4(const Four& a, const Four& b) { return Four{fmul2(a.lo, b.lo), fmul2(a.hi, b.hi)}; }

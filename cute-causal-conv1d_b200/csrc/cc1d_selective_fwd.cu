@@ -17,31 +17,31 @@ namespace {
 #define FWDC 4
 #endif
 constexpr int kFwdCtas = FWDC;
-// Shared memory: flags; (s, s, s x, s x) by position and channel; y by position and channel; B and
+// Shared memory: flags; (s, s x) by position and channel; y by position and channel; B and
 // C; with several passes the states between two tiles.
-template <int LN>
+template <typename T, int LN>
 struct FwdSmem {
   static constexpr int kFlags = 256;
-  static constexpr int kIo = Tile<LN, false>::T * Tile<LN, false>::PITCH * 16;
+  static constexpr int kIo = Tile<LN, false>::T * Tile<LN, false>::PITCH * 8;
   static constexpr int kY = (Tile<LN, false>::T * Tile<LN, false>::PITCH * 4 + 15) / 16 * 16;
   static int64_t bytes(const SelArgs& a) {
-    return kFlags + kIo + kY + Tile<LN, false>::T * 8 * LN * a.blocks * 4 + (a.blocks > 1 ? a.blocks * kSelThreads * 16 : 0);
+    return kFlags + kIo + kY + Tile<LN, false>::T * 8 * LN * a.blocks * sizeof(T) + (a.blocks > 1 ? a.blocks * kSelThreads * 16 : 0);
   }
 };
 
 // ENDS: only what each segment carries out of itself, for the segments behind it.
-template <typename T, int LN, bool ROWS, bool ENDS>
+template <typename T, int LN, bool ROWS, bool MULTI, bool ENDS>
 __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __grid_constant__ SelArgs a) {
   using Where = Tile<LN, ROWS>;
   constexpr int PITCH = Where::PITCH, TT = Where::T;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float biases[Where::CH], skips[Where::CH];
   SelFlags& flags = *reinterpret_cast<SelFlags*>(smem);
-  float4* io = reinterpret_cast<float4*>(smem + FwdSmem<LN>::kFlags);
-  float* ys = reinterpret_cast<float*>(smem + FwdSmem<LN>::kFlags + FwdSmem<LN>::kIo);
-  float* bc = reinterpret_cast<float*>(smem + FwdSmem<LN>::kFlags + FwdSmem<LN>::kIo + FwdSmem<LN>::kY);
-  const int np = static_cast<int>(a.padded), wide = 4 * LN * a.blocks;
-  float* held = bc + TT * 2 * wide;
+  float2* io = reinterpret_cast<float2*>(smem + FwdSmem<T, LN>::kFlags);
+  float* ys = reinterpret_cast<float*>(smem + FwdSmem<T, LN>::kFlags + FwdSmem<T, LN>::kIo);
+  T* bc = reinterpret_cast<T*>(smem + FwdSmem<T, LN>::kFlags + FwdSmem<T, LN>::kIo + FwdSmem<T, LN>::kY);
+  const int np = static_cast<int>(a.padded), blocks = MULTI ? a.blocks : 1, wide = 4 * LN * blocks;
+  float* held = reinterpret_cast<float*>(bc + TT * 2 * wide);
 
   const SelPlace p = sel_place<LN>(a);
   const int tid = threadIdx.x, sl = tid % LN, c = tid / LN;
@@ -54,10 +54,13 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
     skips[i] = is && a.D.data ? load_any(a.D.data, a.D.dtype, (p.ch0 + i) * a.D.s0) : 0.f;
   }
 
+  __syncthreads();
+  const float bias = biases[Where::c()], skip = skips[Where::c()];  // of the thread's channel, unless along the sequence
+
   Four h = zero4(), rate = zero4();
   float total = 0.f;  // ENDS: the sum of step sizes since the segment's start
   const int64_t ends_at = (p.b * a.segments * a.dim + ch) * np;  // of segment 0
-  for (int nb = 0; nb < a.blocks; ++nb) {
+  for (int nb = 0; nb < blocks; ++nb) {
     const int n0 = nb * kSelBlock + sl * kSelStates;
     const bool has = n0 < np;
     h = zero4();
@@ -65,21 +68,21 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
     if (!ENDS && mine && has)
       for (int64_t s = 0; s < p.seg; ++s)
         h = handed_on(h, rate, a.steps[(p.b * a.segments + s) * a.dim + ch], load4(a.ends + ends_at + s * a.dim * np + n0));
-    if (a.blocks > 1) store4(held + (nb * kSelThreads + tid) * 4, h);
+    if constexpr (MULTI) store4(held + (nb * kSelThreads + tid) * 4, h);
   }
 
   const Walk<T, LN, ROWS> xs(a.x, p), deltas(a.delta, p), zs(a.z.data ? a.z : a.x, p), outs(a.out, p);
   const bool all_channels = p.channels == Where::CH, packed = a.seq_idx.data != nullptr;
   T x[8], next_x[8], next_delta[8], z[8];
   FlagFeed<TT> feed;
-  Coefficients<T, LN> next_bc;
+  Coefficients<T, LN, MULTI> next_bc(a, p);
   auto inside = [&](int64_t i) { return all_channels && (i + 1) * TT <= a.seqlen; };
   auto fetch = [&](int64_t i) {
     const bool whole = inside(i);
     xs.load(a, a.x, p, i, whole, next_x);
     deltas.load(a, a.delta, p, i, whole, next_delta);
     feed.load(a, p.b, i * TT);
-    next_bc.load(a, p, i * TT);
+    next_bc.load(a, i * TT, whole);
   };
   fetch(p.chunk0);
   for (int64_t i = p.chunk0; i < p.chunk1; ++i) {
@@ -87,53 +90,78 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
     const bool whole = inside(i);
     feed.store(a, p.b, t0, flags);
     __syncthreads();  // flags are there
+    const bool checked = packed || !whole;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
       x[k] = next_x[k];
-      float u = to_f32(next_delta[k]) + biases[cc];
-      float s = a.softplus ? step_size(u) : u;
-      float sx = s * to_f32(x[k]);
-      if ((packed || !whole) && !(flags.valid(t) && cc < p.channels)) s = sx = 0.f;
-      io[t * PITCH + cc] = make_float4(s, s, sx, sx);
+      const float u = to_f32(next_delta[k]) + (ROWS ? biases[cc] : bias);
+      const float s = a.softplus ? step_size<T>(u) : u, sx = s * to_f32(x[k]);
+      io[t * PITCH + cc] = make_float2(s, sx);
     }
-    next_bc.store(a, p, t0, flags, bc);
+    if (checked)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
+        if (!flags.valid(t) || cc >= p.channels) io[t * PITCH + cc] = make_float2(0.f, 0.f);
+      }
+    next_bc.store(a, p, t0, checked, flags, bc);
     __syncthreads();
     if (!ENDS && a.z.data) zs.load(a, a.z, p, i, whole, z);
     if (i + 1 < p.chunk1) fetch(i + 1);
 
-    for (int nb = 0; nb < a.blocks; ++nb) {
+    for (int nb = 0; nb < blocks; ++nb) {
       const int n0 = nb * kSelBlock + sl * kSelStates;
       const bool has = n0 < np;
-      if (a.blocks > 1) {
+      if constexpr (MULTI) {
         h = load4(held + (nb * kSelThreads + tid) * 4);
         rate = mine && has ? load_rates(a, ch, n0) : zero4();
       }
       if (!ENDS && a.checkpoints && mine && has)
         store4(a.checkpoints + ((p.b * a.nchunks + i) * a.dim + ch) * np + n0, h);
-      const float* row = bc + nb * 4 * LN + sl * 4;
-#pragma unroll 1
-      for (int q = 0; q < TT / 4; ++q) {
-        const uint32_t f = flags.word[q];
-        float y[4];
-        auto position = [&](int j) {
-          const int t = q * 4 + j;
-          const float4 v = io[t * PITCH + c];
-          const float2 s = make_float2(v.x, v.y), sx = make_float2(v.z, v.w);
-          h = fma4(decays4(s, rate), h, mul4(load4(row + t * 2 * wide), sx));
-          if constexpr (ENDS) {
-            if (nb == 0) total += v.x;
-          } else {
-            y[j] = dot4(load4(row + t * 2 * wide + wide), h);
-          }
-        };
-        if (f == kAllInside) {
+      const T* row = bc + nb * 4 * LN + sl * 4;
+      // y of four positions from q * 4 on: over the states' threads, then to shared memory
+      auto keep = [&](int q, float (&y)[4]) {
+        sum_lanes<LN>(y, sl);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) position(j);
-        } else {
+        for (int j = 0; j < 4 / LN; ++j) {
+          float* o = ys + (q * 4 + sl * (4 / LN) + j) * PITCH + c;
+          *o = MULTI && nb > 0 ? *o + y[j] : y[j];
+        }
+      };
+#pragma unroll 1
+      for (int q = 0; q < TT / 4; q += 2) {
+        if (flags.word[q] == kAllInside && flags.word[q + 1] == kAllInside) {
+          // eight positions: all that does not wait for h first
+          Four decay[8], add[8], C[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int t = q * 4 + j;
+            const float2 v = io[t * PITCH + c];
+            decay[j] = decays4(make_float2(v.x, v.x), rate);
+            add[j] = mul4(load4_of(row + t * 2 * wide), make_float2(v.y, v.y));
+            if (ENDS && nb == 0) total += v.x;
+            if (!ENDS) C[j] = load4_of(row + t * 2 * wide + wide);
+          }
+          float y[2][4];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            h = fma4(decay[j], h, add[j]);
+            if (!ENDS) y[j / 4][j % 4] = dot4(C[j], h);
+          }
+          if constexpr (!ENDS) {
+            keep(q, y[0]);
+            keep(q + 1, y[1]);
+          }
+          continue;
+        }
+#pragma unroll 1
+        for (int half = q; half < q + 2; ++half) {
+          const uint32_t f = flags.word[half];
+          float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
           for (int j = 0; j < 4; ++j) {
-            const int t = q * 4 + j, r = flags.row[t];
+            const int t = half * 4 + j, r = flags.row[t];
             const uint32_t fj = f >> (8 * j);
             float yj = 0.f;
             if (fj & kValid) {
@@ -141,10 +169,10 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
                 h = a.init.data && r >= 0 && mine && has ? load_state(a.init, r, ch, n0, a.dstate) : zero4();
                 if (ENDS) total = INFINITY;
               }
-              const float4 v = io[t * PITCH + c];
-              h = fma4(decays4(make_float2(v.x, v.y), rate), h, mul4(load4(row + t * 2 * wide), make_float2(v.z, v.w)));
+              const float2 v = io[t * PITCH + c];
+              h = fma4(decays4(make_float2(v.x, v.x), rate), h, mul4(load4_of(row + t * 2 * wide), make_float2(v.y, v.y)));
               if (ENDS && nb == 0) total += v.x;
-              if (!ENDS) yj = dot4(load4(row + t * 2 * wide + wide), h);
+              if (!ENDS) yj = dot4(load4_of(row + t * 2 * wide + wide), h);
               if (!ENDS && (fj & kLast) && a.final_states.data && r >= 0 && mine && has)
                 store_state(a.final_states, r, ch, n0, a.dstate, h);
             }
@@ -152,17 +180,10 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
             for (int e = 0; e < 4; ++e)
               if (e == j) y[e] = yj;
           }
-        }
-        if constexpr (!ENDS) {
-          sum_lanes<LN>(y, sl);
-#pragma unroll
-          for (int j = 0; j < 4 / LN; ++j) {
-            float* o = ys + (q * 4 + sl * (4 / LN) + j) * PITCH + c;
-            *o = nb == 0 ? y[j] : *o + y[j];
-          }
+          if constexpr (!ENDS) keep(half, y);
         }
       }
-      if (a.blocks > 1) store4(held + (nb * kSelThreads + tid) * 4, h);
+      if constexpr (MULTI) store4(held + (nb * kSelThreads + tid) * 4, h);
     }
     __syncthreads();
     if constexpr (!ENDS) {
@@ -170,57 +191,63 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
-        float y = fmaf(skips[cc], a.D.data ? to_f32(x[k]) : 0.f, ys[t * PITCH + cc]);
-        if (a.z.data) y *= silu_of<T>(to_f32(z[k]));
-        if (packed && !flags.valid(t)) y = 0.f;
-        out[k] = y;
+        out[k] = ys[t * PITCH + cc];
       }
+      if (a.D.data)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) out[k] = fmaf(ROWS ? skips[Where::c() + k * Where::DC] : skip, to_f32(x[k]), out[k]);
+      if (a.z.data)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) out[k] *= silu_of<T>(to_f32(z[k]));
+      if (packed)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (!flags.valid(Where::t() + k * Where::DT)) out[k] = 0.f;
       outs.store(a, a.out, p, i, whole, out);
       __syncthreads();  // flags and y have been read
     }
   }
   if (ENDS && mine) {
-    for (int nb = 0; nb < a.blocks; ++nb) {
+    for (int nb = 0; nb < blocks; ++nb) {
       const int n0 = nb * kSelBlock + sl * kSelStates;
       if (n0 >= np) continue;
-      if (a.blocks > 1) h = load4(held + (nb * kSelThreads + tid) * 4);
+      if constexpr (MULTI) h = load4(held + (nb * kSelThreads + tid) * 4);
       store4(a.ends + ends_at + p.seg * a.dim * np + n0, h);
     }
     if (sl == 0) a.steps[(p.b * a.segments + p.seg) * a.dim + ch] = total;
   }
 }
 
-template <typename T, int LN, bool ROWS, bool ENDS>
+template <typename T, int LN, bool ROWS, bool MULTI, bool ENDS>
 cudaError_t launch(const SelArgs& a, cudaStream_t s) {
-  const size_t smem = static_cast<size_t>(FwdSmem<LN>::bytes(a));
-  const auto kernel = sel_fwd_kernel<T, LN, ROWS, ENDS>;
+  const size_t smem = static_cast<size_t>(FwdSmem<T, LN>::bytes(a));
+  const auto kernel = sel_fwd_kernel<T, LN, ROWS, MULTI, ENDS>;
   const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
   return launch_dependent(kernel, dim3(static_cast<unsigned>(a.batch * a.segments * a.tiles)), dim3(kSelThreads), smem, s, a);
 }
 
-template <typename T, int LN, bool ROWS>
+template <typename T, int LN, bool ROWS, bool MULTI = false>
 cudaError_t run(const SelArgs& a, cudaStream_t s) {
   if (a.segments > 1) {
-    const cudaError_t e = launch<T, LN, ROWS, true>(a, s);
+    const cudaError_t e = launch<T, LN, ROWS, MULTI, true>(a, s);
     if (e != cudaSuccess) return e;
   }
-  return launch<T, LN, ROWS, false>(a, s);
+  return launch<T, LN, ROWS, MULTI, false>(a, s);
 }
 
-template <typename T, int LN>
+template <typename T>
 cudaError_t run(const SelArgs& a, cudaStream_t s) {
-  return a.rows ? run<T, LN, true>(a, s) : run<T, LN, false>(a, s);
+  if (a.blocks > 1) return a.rows ? run<T, 4, true, true>(a, s) : run<T, 4, false, true>(a, s);
+  switch (a.lanes) {
+    case 1: return a.rows ? run<T, 1, true>(a, s) : run<T, 1, false>(a, s);
+    case 2: return a.rows ? run<T, 2, true>(a, s) : run<T, 2, false>(a, s);
+    default: return a.rows ? run<T, 4, true>(a, s) : run<T, 4, false>(a, s);
+  }
 }
 
 }  // namespace
 
-cudaError_t CC1D_DT_NAME(sel_fwd)(const SelArgs& a, cudaStream_t s) {
-  switch (a.lanes) {
-    case 1: return run<CC1D_DT_TYPE, 1>(a, s);
-    case 2: return run<CC1D_DT_TYPE, 2>(a, s);
-    default: return run<CC1D_DT_TYPE, 4>(a, s);
-  }
-}
+cudaError_t CC1D_DT_NAME(sel_fwd)(const SelArgs& a, cudaStream_t s) { return run<CC1D_DT_TYPE>(a, s); }
 
 }  // namespace cc1d

@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kThreads) sel_update_kernel(const SelUpdateArg
     if (live) {
       x = load_el<T>(a.x, b, d, l);
       float s = load_el<T>(a.delta, b, d, l) + bias;
-      if (a.softplus) s = step_size(s);
+      if (a.softplus) s = step_size<T>(s);
       const float2 s2 = make_float2(s, s), sx = make_float2(s * x, s * x);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
