@@ -36,16 +36,6 @@ bool strips_start_on(int bytes, const TensorArg& t, const RecArgs& a) {
          (a.rows ? step_ok(t.s1, a.dim) : step_ok(t.s2, a.seqlen));
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
-    cudaGetLastError();
-    return 148;
-  }
-  return n;
-}
-
 // How many clusters of a.cluster CTAs (CTAs for 1) of this recurrence's kernel run at a time: the
 // driver's answer, asked once per kernel, size and device.
 int64_t clusters_at_a_time(RecArgs a, bool bwd) {

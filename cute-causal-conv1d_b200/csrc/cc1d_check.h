@@ -45,6 +45,16 @@ inline cc1d_status workspace_ok(const void* ws, int64_t bytes, int64_t need) {
   return CC1D_OK;
 }
 
+inline int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return 148;
+  }
+  return n;
+}
+
 }  // namespace cc1d
 
 // For functions whose params are called p.

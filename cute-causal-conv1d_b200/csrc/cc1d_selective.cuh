@@ -6,32 +6,39 @@
 
 namespace cc1d {
 
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // softplus(u) = max(u, 0) + log(1 + e) with e = exp(-|u|), to full relative precision for u of any
-// size, NaN included.  log(1 + e) = 2 atanh(s) with s = e / (2 + e) <= 1/3, and 2 atanh(s) / s in
-// w = s^2 <= 1/9 by the polynomial that interpolates it at five Chebyshev points (off by 4e-9).
-__device__ __forceinline__ float softplus_of_exp(float u, float e) {
-  const float s = e * rcp_approx(2.f + e);
-  const float w = s * s;
-  float q = fmaf(0.281577796f, w, 0.279651582f);
-  q = fmaf(q, w, 0.400245965f);
-  q = fmaf(q, w, 0.666663229f);
-  q = fmaf(q, w, 2.f);
-  return fmaf(s, q, fmaxf(u, 0.f));
+// size, NaN included, for two values.  log(1 + e) = 2 atanh(s) with s = e / (2 + e) <= 1/3, and
+// 2 atanh(s) / s in w = s^2 <= 1/9 by the polynomial that interpolates it at five Chebyshev points
+// (off by 4e-9).
+__device__ __forceinline__ float2 softplus_of_exp(float2 u, float2 e) {
+  const float2 d = fadd2(both(2.f), e);
+  const float2 s = fmul2(e, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+  const float2 w = fmul2(s, s);
+  float2 q = ffma2(both(0.281577796f), w, both(0.279651582f));
+  q = ffma2(q, w, both(0.400245965f));
+  q = ffma2(q, w, both(0.666663229f));
+  q = ffma2(q, w, both(2.f));
+  return ffma2(s, q, make_float2(fmaxf(u.x, 0.f), fmaxf(u.y, 0.f)));
 }
 // exp(-|u|); for 16-bit tensors the rounding of the exponent is left in it (|u| 2^-24 of it).
 template <typename T>
-__device__ __forceinline__ float exp_of_size(float u) {
-  if constexpr (std::is_same<T, float>::value) return exp_minus(min_nan(fabsf(u), 88.f));
-  else return ex2_approx(-kLog2e * fabsf(u));
+__device__ __forceinline__ float2 exp_of_size(float2 u) {
+  if constexpr (std::is_same<T, float>::value)
+    return make_float2(exp_minus(min_nan(fabsf(u.x), 88.f)), exp_minus(min_nan(fabsf(u.y), 88.f)));
+  const float2 v = fmul2(both(-kLog2e), make_float2(fabsf(u.x), fabsf(u.y)));
+  return make_float2(ex2_approx(v.x), ex2_approx(v.y));
 }
 template <typename T>
-__device__ __forceinline__ float step_size(float u) { return softplus_of_exp(u, exp_of_size<T>(u)); }
+__device__ __forceinline__ float2 step_size(float2 u) { return softplus_of_exp(u, exp_of_size<T>(u)); }
 // The same, and its derivative sigmoid(u).
 template <typename T>
-__device__ __forceinline__ float step_size(float u, float* slope) {
-  const float e = exp_of_size<T>(u);
-  const float r = rcp_approx(1.f + e);
-  *slope = u < 0.f ? e * r : r;
+__device__ __forceinline__ float2 step_size(float2 u, float2* slope) {
+  const float2 e = exp_of_size<T>(u), d = fadd2(both(1.f), e);
+  const float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+  const float2 less = fmul2(e, r);
+  *slope = make_float2(u.x < 0.f ? less.x : r.x, u.y < 0.f ? less.y : r.y);
   return softplus_of_exp(u, e);
 }
 
@@ -57,7 +64,7 @@ struct SelPlace {
 
 template <int LN>
 __device__ __forceinline__ SelPlace sel_place(const SelArgs& a) {
-  constexpr int CH = kSelThreads / LN;
+  constexpr int CH = kSelChannels / LN;
   SelPlace p;
   int64_t i = blockIdx.x;
   p.tile = i % a.tiles;
@@ -73,15 +80,17 @@ __device__ __forceinline__ SelPlace sel_place(const SelArgs& a) {
   return p;
 }
 
-// A tile: T positions of CH channels of a batch row, and how the threads go through it, eight
-// elements each, along the dimension of unit stride: element k of a thread is position t + k DT,
-// channel c + k DC.
-template <int LN, bool ROWS>
+// A tile: T positions of PAIRS pairs of channels of a batch row, and how the threads go through it,
+// K pairs each, along the dimension of unit stride: the k-th of a thread is position t + k DT,
+// pair c + k DC.  NT: threads of the CTA.
+template <int NT, int LN, bool ROWS>
 struct Tile {
-  static constexpr int CH = kSelThreads / LN, T = 8 * LN, PITCH = CH + 1;
-  static constexpr int DT = ROWS ? 0 : LN, DC = ROWS ? kSelThreads / T : 0;
-  static __device__ __forceinline__ int t() { return ROWS ? threadIdx.x % T : threadIdx.x / CH; }
-  static __device__ __forceinline__ int c() { return ROWS ? threadIdx.x / T : threadIdx.x % CH; }
+  static constexpr int T = 8 * LN, PAIRS = kSelChannels / 2 / LN, K = T * PAIRS / NT;
+  static constexpr int DT = ROWS ? 0 : NT / PAIRS, DC = ROWS ? NT / T : 0;
+  static __device__ __forceinline__ int t() { return ROWS ? threadIdx.x % T : threadIdx.x / PAIRS; }
+  static __device__ __forceinline__ int c() { return ROWS ? threadIdx.x / T : threadIdx.x % PAIRS; }
+  static __device__ __forceinline__ int t(int k) { return t() + k * DT; }
+  static __device__ __forceinline__ int c(int k) { return c() + k * DC; }
 };
 
 // The flags and state rows (-1: none) of a tile's positions.
@@ -122,51 +131,90 @@ struct FlagFeed {
   }
 };
 
-// A thread's eight elements of one tensor, walked tile by tile.
-template <typename T, int LN, bool ROWS>
+// Two channels of a position as they were loaded.  Kept as words until they are used: taking them
+// apart at once would wait for the load.  16-bit: both in lo where they came as one word.
+struct Raw {
+  uint32_t lo, hi;
+};
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const Raw& r, bool pairs) {
+  if constexpr (std::is_same<T, float>::value) return make_float2(__uint_as_float(r.lo), __uint_as_float(r.hi));
+  const uint32_t word = pairs ? r.lo : __byte_perm(r.lo, r.hi, 0x5410);
+  float f[2];
+  unpack<T, 2>(*reinterpret_cast<const Packet<T, 2>*>(&word), f);
+  return make_float2(f[0], f[1]);
+}
+
+// A thread's pairs of one tensor, walked tile by tile.
+template <typename T, typename Where>
 struct Walk {
-  using Where = Tile<LN, ROWS>;
   T* p;  // of the thread's first element in tile 0
   __device__ __forceinline__ Walk(const TensorArg& t, const SelPlace& at) {
-    p = static_cast<T*>(t.data) + at.b * t.s0 + (at.ch0 + Where::c()) * t.s1 + Where::t() * t.s2;
+    p = static_cast<T*>(t.data) + at.b * t.s0 + (at.ch0 + 2 * Where::c()) * t.s1 + Where::t() * t.s2;
   }
-  // Whether element k of the tile at t0 exists.
-  static __device__ __forceinline__ bool has(const SelArgs& a, const SelPlace& at, int64_t t0, int k) {
-    return t0 + Where::t() + k * Where::DT < a.seqlen && Where::c() + k * Where::DC < at.channels;
+  // How many channels of pair k of the tile at t0 exist.
+  static __device__ __forceinline__ int has(const SelArgs& a, const SelPlace& at, int64_t t0, int k) {
+    return t0 + Where::t(k) < a.seqlen ? at.channels - 2 * Where::c(k) : 0;
   }
-  static __device__ __forceinline__ int64_t step(const TensorArg& t) { return ROWS ? Where::DC * t.s1 : Where::DT * t.s2; }
-  __device__ __forceinline__ void load(const SelArgs& a, const TensorArg& t, const SelPlace& at, int64_t index, bool whole, T (&v)[8]) const {
+  static __device__ __forceinline__ int64_t step(const TensorArg& t) { return Where::DC ? 2 * Where::DC * t.s1 : Where::DT * t.s2; }
+  static __device__ __forceinline__ uint32_t word(const T* q) {
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const uint32_t*>(q);
+    else return *reinterpret_cast<const uint16_t*>(q);
+  }
+  __device__ __forceinline__ void load(const SelArgs& a, const TensorArg& t, const SelPlace& at, int64_t index, bool whole, Raw (&v)[Where::K]) const {
     const T* q = p + index * (Where::T * t.s2);
-    if (whole) {
+    if (whole && a.pairs) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k, q += step(t)) v[k] = *q;
+      for (int k = 0; k < Where::K; ++k, q += step(t)) {
+        if constexpr (sizeof(T) == 4) {
+          const uint2 u = *reinterpret_cast<const uint2*>(q);
+          v[k].lo = u.x, v[k].hi = u.y;
+        } else {
+          v[k].lo = *reinterpret_cast<const uint32_t*>(q);
+        }
+      }
+    } else if (whole) {
+#pragma unroll
+      for (int k = 0; k < Where::K; ++k, q += step(t)) v[k].lo = word(q), v[k].hi = word(q + t.s1);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k, q += step(t)) v[k] = has(a, at, index * Where::T, k) ? *q : from_f32<T>(0.f);
+      for (int k = 0; k < Where::K; ++k, q += step(t)) {
+        const int n = has(a, at, index * Where::T, k);
+        if (a.pairs && sizeof(T) == 2) {  // both or none
+          v[k].lo = n > 0 ? *reinterpret_cast<const uint32_t*>(q) : 0;
+        } else {
+          v[k].lo = n > 0 ? word(q) : 0;
+          v[k].hi = n > 1 ? word(q + t.s1) : 0;
+        }
+      }
     }
   }
-  __device__ __forceinline__ void store(const SelArgs& a, const TensorArg& t, const SelPlace& at, int64_t index, bool whole, const float (&v)[8]) const {
-    T* q = p + index * (Where::T * t.s2);
-    if (whole) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k, q += step(t)) *q = from_f32<T>(v[k]);
+  __device__ __forceinline__ void store_one(const SelArgs& a, const TensorArg& t, const SelPlace& at, int64_t index, int k, bool whole, float2 v) const {
+    T* q = p + index * (Where::T * t.s2) + k * step(t);
+    const float f[2] = {v.x, v.y};
+    const Packet<T, 2> r = pack<T, 2>(f);
+    if (whole && a.pairs) {
+      *reinterpret_cast<Packet<T, 2>*>(q) = r;
     } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k, q += step(t))
-        if (has(a, at, index * Where::T, k)) *q = from_f32<T>(v[k]);
+      const int n = whole ? 2 : has(a, at, index * Where::T, k);
+      if (n > 0) q[0] = r.v[0];
+      if (n > 1) q[t.s1] = r.v[1];
     }
+  }
+  __device__ __forceinline__ void store(const SelArgs& a, const TensorArg& t, const SelPlace& at, int64_t index, bool whole, const float2 (&v)[Where::K]) const {
+#pragma unroll
+    for (int k = 0; k < Where::K; ++k) store_one(a, t, at, index, k, whole, v[k]);
   }
 };
-
-// B and C of a tile's positions in shared memory, in their own type, since what a load from there
-// brings to registers is what it costs: [position][B, C][wide], wide = 4 LN per pass; zero past
-// dstate and where a position is not valid, so that whatever stands there is not used.  The threads
-// go along the states or, where that is B's unit stride, along the sequence; the eight elements
-// of a thread for a single pass are loaded a tile ahead.
-template <typename T, int LN, bool MULTI>
+// B and C of a tile's positions as fp32 in shared memory: [position][B, C][wide], wide = 4 LN per
+// pass; zero past dstate and where a position is not valid, so that whatever stands there is not
+// used.  The threads
+// go along the states or, where that is B's unit stride, along the sequence; a thread's elements
+// for a single pass are loaded a tile ahead.
+template <typename T, int NT, int LN, bool MULTI>
 struct Coefficients {
-  static constexpr int TT = 8 * LN, ALL = TT * 8 * LN, HELD = MULTI || ALL < kSelThreads ? 1 : ALL / kSelThreads;
-  static constexpr int DT = kSelThreads / (8 * LN), DN = kSelThreads / TT, HALF = HELD > 1 ? HELD / 2 : 1;
+  static constexpr int TT = 8 * LN, ALL = TT * 8 * LN, HELD = MULTI || ALL < NT ? 1 : ALL / NT;
+  static constexpr int DT = NT / (8 * LN), DN = NT / TT, HALF = HELD > 1 ? HELD / 2 : 1;
   T v[HELD];
   const T *p, *pc;  // along the states: the thread's tensor; else B and C
   int n, t;
@@ -186,7 +234,7 @@ struct Coefficients {
   }
   __device__ __forceinline__ void load(const SelArgs& a, int64_t t0, bool whole) {
     if constexpr (MULTI) return;
-    if (ALL < kSelThreads && threadIdx.x >= ALL) return;
+    if (ALL < NT && threadIdx.x >= ALL) return;
     if (along) {
       const int64_t s2 = is_c ? a.C.s2 : a.B.s2;
       const T* q = p + t0 * s2;
@@ -211,26 +259,26 @@ struct Coefficients {
     }
   }
   // checked: a position may not be valid
-  __device__ __forceinline__ void store(const SelArgs& a, const SelPlace& at, int64_t t0, bool checked, const SelFlags& f, T* bc) const {
+  __device__ __forceinline__ void store(const SelArgs& a, const SelPlace& at, int64_t t0, bool checked, const SelFlags& f, float* bc) const {
     if constexpr (MULTI) {
       const int wide = 4 * LN * a.blocks;
-      for (int e = threadIdx.x; e < TT * 2 * wide; e += kSelThreads) {
+      for (int e = threadIdx.x; e < TT * 2 * wide; e += NT) {
         const int tt = along ? e / (2 * wide) : e % TT, s = along ? e - tt * 2 * wide : e / TT;
         const bool c = s >= wide;
         const int nn = c ? s - wide : s;
         const TensorArg& x = c ? a.C : a.B;
-        T r = from_f32<T>(0.f);
+        float r = 0.f;
         if (nn < a.dstate && f.valid(tt))
-          r = static_cast<const T*>(x.data)[at.b * x.s0 + at.group * (c ? a.C_group : a.B_group) + nn * x.s1 + (t0 + tt) * x.s2];
+          r = to_f32(static_cast<const T*>(x.data)[at.b * x.s0 + at.group * (c ? a.C_group : a.B_group) + nn * x.s1 + (t0 + tt) * x.s2]);
         bc[(tt * 2 + c) * wide + nn] = r;
       }
     } else {
-      if (ALL < kSelThreads && threadIdx.x >= ALL) return;
-      T* o = bc + (t * 2 + is_c) * 4 * LN + n;
+      if (ALL < NT && threadIdx.x >= ALL) return;
+      float* o = bc + (t * 2 + is_c) * 4 * LN + n;
 #pragma unroll
       for (int k = 0; k < HELD; ++k) {
         const int at_k = along ? k * DT * 8 * LN : (k >= HALF) * 4 * LN + k % HALF * DN;
-        o[at_k] = checked && !f.valid(along ? t + k * DT : t) ? from_f32<T>(0.f) : v[k];
+        o[at_k] = checked && !f.valid(along ? t + k * DT : t) ? 0.f : to_f32(v[k]);
       }
     }
   }
@@ -249,65 +297,121 @@ __device__ __forceinline__ void store_el(const TensorArg& t, int64_t b, int64_t 
 struct Four {
   float2 lo, hi;
 };
-__device__ __forceinline__ Four zero4() { return Four{make_float2(0.f, 0.f), make_float2(0.f, 0.f)}; }
-__device__ __forceinline__ Four load4(const float* p) {
-  const float4 f = *reinterpret_cast<const float4*>(p);
-  return Four{make_float2(f.x, f.y), make_float2(f.z, f.w)};
-}
-__device__ __forceinline__ void store4(float* p, const Four& f) {
-  *reinterpret_cast<float4*>(p) = make_float4(f.lo.x, f.lo.y, f.hi.x, f.hi.y);
-}
-// Four neighbouring elements, on their alignment.
-template <typename T>
-__device__ __forceinline__ Four load4_of(const T* p) {
-  float v[4];
-  unpack<T, 4>(*reinterpret_cast<const Packet<T, 4>*>(p), v);
-  return Four{make_float2(v[0], v[1]), make_float2(v[2], v[3])};
-}
+__device__ __forceinline__ Four of4(const float4& f) { return Four{make_float2(f.x, f.y), make_float2(f.z, f.w)}; }
+__device__ __forceinline__ float4 to4(const Four& f) { return make_float4(f.lo.x, f.lo.y, f.hi.x, f.hi.y); }
+__device__ __forceinline__ Four zero4() { return Four{both(0.f), both(0.f)}; }
+__device__ __forceinline__ Four load4(const float* p) { return of4(*reinterpret_cast<const float4*>(p)); }
+__device__ __forceinline__ void store4(float* p, const Four& f) { *reinterpret_cast<float4*>(p) = to4(f); }
 __device__ __forceinline__ Four fma4(const Four& a, const Four& b, const Four& c) { return Four{ffma2(a.lo, b.lo, c.lo), ffma2(a.hi, b.hi, c.hi)}; }
-__device__ __forceinline__ Four mul4(const Four& a, const Four& b) { return Four{fmul2(a.lo, b.lo), fmul2(a.hi, b.hi)}; }
 __device__ __forceinline__ Four mul4(const Four& a, float2 b) { return Four{fmul2(a.lo, b), fmul2(a.hi, b)}; }
-__device__ __forceinline__ Four fma4(const Four& a, float2 b, const Four& c) { return Four{ffma2(a.lo, b, c.lo), ffma2(a.hi, b, c.hi)}; }
-__device__ __forceinline__ float sum4(const Four& a) {
-  const float2 s = fadd2(a.lo, a.hi);
-  return s.x + s.y;
-}
 __device__ __forceinline__ float dot4(const Four& a, const Four& b) {
   const float2 s = ffma2(a.hi, b.hi, fmul2(a.lo, b.lo));
   return s.x + s.y;
 }
 __device__ __forceinline__ Four decays4(float2 s, const Four& rate) { return Four{decays(s, rate.lo), decays(s, rate.hi)}; }
+
+// Four states of two channels: v[i] is state i of both, as one operand of the instructions with
+// which sm_100a multiplies and adds two fp32 values at a time.
+struct Eight {
+  float2 v[4];
+};
+__device__ __forceinline__ Eight zero8() {
+  Eight r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = both(0.f);
+  return r;
+}
+__device__ __forceinline__ Eight of_channels(const float4& a, const float4& b) {
+  return Eight{{make_float2(a.x, b.x), make_float2(a.y, b.y), make_float2(a.z, b.z), make_float2(a.w, b.w)}};
+}
+__device__ __forceinline__ float4 channel0(const Eight& e) { return make_float4(e.v[0].x, e.v[1].x, e.v[2].x, e.v[3].x); }
+__device__ __forceinline__ float4 channel1(const Eight& e) { return make_float4(e.v[0].y, e.v[1].y, e.v[2].y, e.v[3].y); }
+// To and from a place of 32 bytes of each thread in shared memory, half of them `half` floats behind.
+__device__ __forceinline__ Eight take8(const float* p, int half) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + half);
+  return Eight{{make_float2(a.x, a.y), make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w)}};
+}
+__device__ __forceinline__ void put8(float* p, int half, const Eight& e) {
+  *reinterpret_cast<float4*>(p) = make_float4(e.v[0].x, e.v[0].y, e.v[1].x, e.v[1].y);
+  *reinterpret_cast<float4*>(p + half) = make_float4(e.v[2].x, e.v[2].y, e.v[3].x, e.v[3].y);
+}
+// To and from rows of `padded` fp32 for each channel, on 16 bytes.  n: channels that exist.
+__device__ __forceinline__ Eight load8(const float* p, int64_t padded, int n) {
+  const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+  return of_channels(n > 0 ? *reinterpret_cast<const float4*>(p) : z, n > 1 ? *reinterpret_cast<const float4*>(p + padded) : z);
+}
+__device__ __forceinline__ void store8(float* p, int64_t padded, int n, const Eight& e) {
+  if (n > 0) *reinterpret_cast<float4*>(p) = channel0(e);
+  if (n > 1) *reinterpret_cast<float4*>(p + padded) = channel1(e);
+}
 // A row of the states (rows, dim, dstate) at channel ch, states n0 .. n0 + 3.
-__device__ __forceinline__ Four load_state(const TensorArg& t, int64_t row, int64_t ch, int64_t n0, int64_t dstate) {
+__device__ __forceinline__ float4 load_state(const TensorArg& t, int64_t row, int64_t ch, int64_t n0, int64_t dstate) {
   const float* p = static_cast<const float*>(t.data) + row * t.s0 + ch * t.s1;
   float v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = n0 + i < dstate ? p[(n0 + i) * t.s2] : 0.f;
-  return Four{make_float2(v[0], v[1]), make_float2(v[2], v[3])};
+  return make_float4(v[0], v[1], v[2], v[3]);
 }
-__device__ __forceinline__ void store_state(const TensorArg& t, int64_t row, int64_t ch, int64_t n0, int64_t dstate, const Four& f) {
+__device__ __forceinline__ void store_state(const TensorArg& t, int64_t row, int64_t ch, int64_t n0, int64_t dstate, const float4& f) {
   float* p = static_cast<float*>(t.data) + row * t.s0 + ch * t.s1;
-  const float v[4] = {f.lo.x, f.lo.y, f.hi.x, f.hi.y};
+  const float v[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (n0 + i < dstate) p[(n0 + i) * t.s2] = v[i];
 }
+// The same for the channels ch and ch + 1, n of which exist; zero without the tensor or the row.
+__device__ __forceinline__ Eight load_states(const TensorArg& t, int64_t row, int64_t ch, int64_t n0, int64_t dstate, int n) {
+  const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool is = t.data && row >= 0;
+  return of_channels(is && n > 0 ? load_state(t, row, ch, n0, dstate) : z, is && n > 1 ? load_state(t, row, ch + 1, n0, dstate) : z);
+}
+__device__ __forceinline__ void store_states(const TensorArg& t, int64_t row, int64_t ch, int64_t n0, int64_t dstate, int n, const Eight& e) {
+  if (!t.data || row < 0) return;
+  if (n > 0) store_state(t, row, ch, n0, dstate, channel0(e));
+  if (n > 1) store_state(t, row, ch + 1, n0, dstate, channel1(e));
+}
 // A[ch, n0 .. n0 + 3] log2(e), so that exp(s A) = 2^(s A log2(e)).
-__device__ __forceinline__ Four load_rates(const TensorArg& A, int64_t ch, int64_t n0, int64_t dstate) {
+__device__ __forceinline__ float4 load_rates(const TensorArg& A, int64_t ch, int64_t n0, int64_t dstate) {
   float v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = n0 + i < dstate ? kLog2e * load_any(A.data, A.dtype, ch * A.s0 + (n0 + i) * A.s1) : 0.f;
-  return Four{make_float2(v[0], v[1]), make_float2(v[2], v[3])};
+  return make_float4(v[0], v[1], v[2], v[3]);
 }
-__device__ __forceinline__ Four load_rates(const SelArgs& a, int64_t ch, int64_t n0) { return load_rates(a.A, ch, n0, a.dstate); }
+__device__ __forceinline__ Eight load_rates(const SelArgs& a, int64_t ch, int64_t n0, int n) {
+  const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+  return of_channels(n > 0 ? load_rates(a.A, ch, n0, a.dstate) : z, n > 1 ? load_rates(a.A, ch + 1, n0, a.dstate) : z);
+}
+__device__ __forceinline__ Eight decays8(float2 s, const Eight& rate) {
+  Eight r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = decays(s, rate.v[i]);
+  return r;
+}
+// Four neighbouring values of shared memory (B or C of a position).
+struct Quad {
+  float v[4];
+};
+__device__ __forceinline__ Quad quad(const float* p) {
+  const float4 f = *reinterpret_cast<const float4*>(p);
+  return Quad{{f.x, f.y, f.z, f.w}};
+}
 // What a segment's neighbour and those beyond it hand on: x exp(A sum) + e, and e alone where the
 // sequence is cut between them (sum infinite) or nothing comes.
 __device__ __forceinline__ float handed_on(float x, float rate, float sum, float e) {
   return sum < INFINITY && x != 0.f ? fmaf(exp2f(rate * sum), x, e) : e;
 }
-__device__ __forceinline__ Four handed_on(const Four& x, const Four& rate, float sum, const Four& e) {
-  return Four{make_float2(handed_on(x.lo.x, rate.lo.x, sum, e.lo.x), handed_on(x.lo.y, rate.lo.y, sum, e.lo.y)),
-              make_float2(handed_on(x.hi.x, rate.hi.x, sum, e.hi.x), handed_on(x.hi.y, rate.hi.y, sum, e.hi.y))};
+// Over segments [from, to) upwards, or with step -1 downwards.
+__device__ __forceinline__ Eight handed_over(const SelArgs& a, int64_t b, int64_t from, int64_t to, int64_t step, int64_t ch, int64_t n0, int n, const Eight& rate) {
+  Eight x = zero8();
+  for (int64_t s = from; s != to; s += step) {
+    const int64_t at = (b * a.segments + s) * a.dim + ch;
+    const Eight e = load8(a.ends + at * a.padded + n0, a.padded, n);
+    const float s0 = n > 0 ? a.steps[at] : 0.f, s1 = n > 1 ? a.steps[at + 1] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x.v[i] = make_float2(handed_on(x.v[i].x, rate.v[i].x, s0, e.v[i].x), handed_on(x.v[i].y, rate.v[i].y, s1, e.v[i].y));
+  }
+  return x;
 }
 
 // The sums over the LN threads of a channel of four positions' values; afterwards thread sl has

@@ -118,6 +118,39 @@ cc1d_status check(const cc1d_selective_params* p, bool bwd, SelArgs* a) {
   return CC1D_OK;
 }
 
+// Neighbouring channels of it move two at a time.
+bool pairs_ok(const TensorArg& t, const SelArgs& a) {
+  const uintptr_t bytes = t.dtype == CC1D_FLOAT32 ? 8 : 4;
+  return t.s1 == 1 && reinterpret_cast<uintptr_t>(t.data) % bytes == 0 && (a.batch <= 1 || t.s0 % 2 == 0) &&
+         (a.seqlen <= 1 || t.s2 % 2 == 0);
+}
+
+// Parts of the sequence that run side by side.  One part needs no first pass over it; with more,
+// that pass finds what each part hands to the next one.  Four CTAs run on an SM (registers), and a
+// tile takes long because a thread's work is one chain: with n CTAs on an SM, measured on a B200
+// (microseconds, 32 positions, 16 states, bf16 with z)
+//
+//   forward  3.0 + .55 n, the first pass .66 of it      backward  13.7 + 1.2 n, .43
+//
+// and a part about two tiles' time to start.  One sequence of 16384 positions and 1024 channels:
+// forward 1587 us in one part, 660 in four; backward 7617 and 2729.
+int64_t choose_segments(const SelArgs& a, bool bwd) {
+  constexpr int kFit = 4;
+  const double sms = sm_count();
+  const int64_t ctas = a.batch * a.tiles, fit = static_cast<int64_t>(sms) * kFit;
+  const double base = bwd ? 13.7 : 3.0, more = bwd ? 1.2 : .55, first = bwd ? .43 : .66;
+  double best = 0;
+  int64_t pick = 1;
+  for (int64_t n = 1; n <= 64 && n <= a.nchunks; ++n) {
+    const double tiles = static_cast<double>((a.nchunks + n - 1) / n) + 2;
+    const int64_t waves = ctas * n / fit, rest = ctas * n % fit;
+    const auto tile = [&](int64_t running) { return base + more * std::max(1.0, static_cast<double>(running) / sms); };
+    const double cost = tiles * (n > 1 ? 1 + first : 1) * (static_cast<double>(waves) * tile(fit) + (rest ? tile(rest) : 0.0));
+    if (n == 1 || cost < best) best = cost, pick = n;
+  }
+  return pick;
+}
+
 // Threads per channel, passes, tiles of channels, segments of the sequence, and which way the
 // threads go through a tile.
 cc1d_status plan(SelArgs* a, bool bwd) {
@@ -127,11 +160,16 @@ cc1d_status plan(SelArgs* a, bool bwd) {
   const int64_t chunk = CC1D_SELECTIVE_CHUNK(a->dstate);
   a->nchunks = (a->seqlen + chunk - 1) / chunk;
   a->gdim = a->dim / a->groups;
-  const int64_t channels = kSelThreads / a->lanes;
+  const int64_t channels = kSelChannels / a->lanes;
   a->group_tiles = (a->gdim + channels - 1) / channels;
   a->tiles = a->group_tiles * a->groups;
   a->rows = a->x.s2 == 1 && a->x.s1 != 1 && a->seqlen > 1;
-  a->segments = 1;
+  a->pairs = !a->rows && a->gdim % 2 == 0;
+  const TensorArg* const moved[] = {&a->x, &a->delta, &a->z, bwd ? &a->dout : &a->out, bwd ? &a->dx : nullptr,
+                                    bwd ? &a->ddelta : nullptr, bwd ? &a->dz : nullptr};
+  for (const TensorArg* t : moved)
+    if (t && t->data) a->pairs = a->pairs && pairs_ok(*t, *a);
+  a->segments = choose_segments(*a, bwd);
   a->segment_chunks = (a->nchunks + a->segments - 1) / a->segments;
   a->segments = (a->nchunks + a->segment_chunks - 1) / a->segment_chunks;
   if (a->batch * a->segments * a->tiles > kMax31 ||

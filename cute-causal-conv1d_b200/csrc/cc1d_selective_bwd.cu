@@ -8,36 +8,36 @@
 //     dA[n] = sum_t g_t[n] a_t[n] h_{t-1}[n] s_t
 // and ddelta = ds sigmoid(delta + bias), dz = dout y silu'(z).
 //
-// CTAs, threads and tiles are the forward's; a CTA goes through its tiles from the last one back.
-// From the state that the forward kept before a tile it runs forward, keeping the state before
-// every fourth position, then takes the groups of four positions from the last one back: states
-// again, then gradients.  dB and dC are summed over the warp's channels by exchanges between
-// lanes, over the CTA's warps in shared memory and over CTAs by a second kernel, all in a fixed
-// order.
+// CTAs and threads are the forward's; tiles have 32 (16, 8) positions, and a CTA goes through them
+// from the last one back.  From the state that the forward kept before a tile it runs forward,
+// keeping the state before every fourth position, then takes the groups of four positions from the
+// last one back: states again, then gradients.  dB and dC are summed over a thread's two channels,
+// over the warp's by exchanges between lanes, over the CTA's warps in shared memory and over CTAs
+// by a second kernel, all in a fixed order.
 #include "cc1d_selective.cuh"
 
 namespace cc1d {
 namespace {
 
-constexpr int kWarps = kSelThreads / 32;
+constexpr int kSelThreads = 64, kWarps = kSelThreads / 32, kHalf = kSelThreads * 4;
 #ifndef BWDC
-#define BWDC 3
+#define BWDC 4
 #endif
 constexpr int kBwdCtas = BWDC;
 
-// Shared memory: flags; (s, x, dy, slope of the step size), replaced by (dx, ddelta, y), by position
-// and channel; the states before every fourth position; each warp's sums of dB and dC; B and C;
-// with several passes three sums by position and channel, and the states between two tiles.
-template <typename T, int LN>
+// Shared memory: flags; (s, x) of a pair by position, replaced by (dx, ddelta), and (dy, slope of the
+// step size), replaced by (y, -), and dout silu'(z); the states before every fourth position; each warp's sums of dB
+// and dC; B and C; of each pass g carried, dA and its low part; with several passes three sums by
+// position and pair.
+template <int LN>
 struct BwdSmem {
-  static constexpr int kFlags = 256, TT = Tile<LN, false>::T, PITCH = Tile<LN, false>::PITCH;
-  static constexpr int kIo = TT * PITCH * 16;
-  static constexpr int kSums = (TT * PITCH * 12 + 15) / 16 * 16;
-  static constexpr int kSub = TT / 4 * kSelThreads * 16;
-  static constexpr int kSlab = TT * 8 * LN * 4;  // one warp's
+  static constexpr int T = 8 * LN, PAIRS = kSelThreads / LN, PITCH = PAIRS + 1;
+  static constexpr int kFlags = 256, kIo = T * PITCH * 16, kDz = (T * PITCH * 8 + 15) / 16 * 16, kSub = T / 4 * kSelThreads * 32;
+  static constexpr int kSlab = T * 8 * LN * 4;  // one warp's
+  static constexpr int kSums = T * PITCH * 24;
   static int64_t bytes(const SelArgs& a) {
-    return kFlags + kIo + kSub + kWarps * kSlab + TT * 8 * LN * a.blocks * static_cast<int>(sizeof(T)) +
-           (a.blocks > 1 ? kSums + 3ll * a.blocks * kSelThreads * 16 : 0);
+    return kFlags + 2 * kIo + kDz + kSub + kWarps * kSlab + T * 8 * LN * a.blocks * 4 + 3ll * a.blocks * kSelThreads * 32 +
+           (a.blocks > 1 ? kSums : 0);
   }
 };
 
@@ -48,18 +48,15 @@ __device__ __forceinline__ void add_to(float& hi, float& lo, float v) {
   lo += (hi - (s - w)) + (v - w);
   hi = s;
 }
-__device__ __forceinline__ void add_to(Four& hi, Four& lo, const Four& v) {
-  add_to(hi.lo.x, lo.lo.x, v.lo.x);
-  add_to(hi.lo.y, lo.lo.y, v.lo.y);
-  add_to(hi.hi.x, lo.hi.x, v.hi.x);
-  add_to(hi.hi.y, lo.hi.y, v.hi.y);
+__device__ __forceinline__ void add_to(float2& hi, float2& lo, float2 v) {
+  add_to(hi.x, lo.x, v.x);
+  add_to(hi.y, lo.y, v.y);
 }
 
-// The sums of a's and b's four values over the channels of a warp.  A lane ends with one of the
-// eight, the number of which summed() tells; lanes that differ in further bits hold the same one.
+// The sums of eight values over the channels of a warp.  A lane ends with one of them, the number
+// of which summed() tells; lanes that differ in further bits hold the same one.
 template <int LN>
-__device__ __forceinline__ float sum_channels(const Four& a, const Four& b, int lane) {
-  float v[8] = {a.lo.x, a.lo.y, a.hi.x, a.hi.y, b.lo.x, b.lo.y, b.hi.x, b.hi.y};
+__device__ __forceinline__ float sum_channels(float (&v)[8], int lane) {
 #pragma unroll
   for (int half = 4; half >= 1; half /= 2) {
     const int bit = 4 * half;
@@ -78,61 +75,60 @@ __device__ __forceinline__ int summed(int lane) { return (lane >> 4 & 1) * 4 + (
 
 // ENDS: only the gradient that each segment hands to the one before it.
 template <typename T, int LN, bool ROWS, bool MULTI, bool ENDS>
-__global__ void __launch_bounds__(kSelThreads, ENDS ? 4 : kBwdCtas) sel_bwd_kernel(const __grid_constant__ SelArgs a) {
-  using Where = Tile<LN, ROWS>;
-  using Smem = BwdSmem<T, LN>;
-  constexpr int PITCH = Where::PITCH, TT = Where::T;
+__global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __grid_constant__ SelArgs a) {
+  using Smem = BwdSmem<LN>;
+  constexpr int TT = Smem::T, PITCH = Smem::PITCH;
+  using Where = Tile<kSelThreads, LN, ROWS>;
+  constexpr int K = Where::K;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float biases[Where::CH];
+  __shared__ float biases[2 * Where::PAIRS];
   SelFlags& flags = *reinterpret_cast<SelFlags*>(smem);
   float4* io = reinterpret_cast<float4*>(smem + Smem::kFlags);
-  float* sub = reinterpret_cast<float*>(smem + Smem::kFlags + Smem::kIo);
-  float* slabs = reinterpret_cast<float*>(smem + Smem::kFlags + Smem::kIo + Smem::kSub);
-  T* bc = reinterpret_cast<T*>(slabs + kWarps * Smem::kSlab / 4);
+  float4* io2 = reinterpret_cast<float4*>(smem + Smem::kFlags + Smem::kIo);
+  float2* dzfs = reinterpret_cast<float2*>(smem + Smem::kFlags + 2 * Smem::kIo);  // dout silu'(z)
+  float* sub = reinterpret_cast<float*>(smem + Smem::kFlags + 2 * Smem::kIo + Smem::kDz) + threadIdx.x * 4;
+  float* slabs = reinterpret_cast<float*>(smem + Smem::kFlags + 2 * Smem::kIo + Smem::kDz + Smem::kSub);
+  float* bc = slabs + kWarps * Smem::kSlab / 4;
   const int np = static_cast<int>(a.padded), blocks = MULTI ? a.blocks : 1, wide = 4 * LN * blocks;
-  float* held = reinterpret_cast<float*>(bc + TT * 2 * wide);  // several passes: g carried, dA and its low part
-  float* sums = held + 3 * blocks * kSelThreads * 4;
+  float* held = bc + TT * 2 * wide + threadIdx.x * 4;  // of each pass: g carried, dA, its low part
+  float2* sums = reinterpret_cast<float2*>(bc + TT * 2 * wide + blocks * 6 * kHalf);
 
   const SelPlace p = sel_place<LN>(a);
+  if (ENDS && p.seg == 0) return;  // nothing is before it
   const int tid = threadIdx.x, sl = tid % LN, c = tid / LN, lane = tid & 31, warp = tid >> 5;
-  const bool mine = c < p.channels;
-  const int64_t ch = p.ch0 + (mine ? c : 0);
+  const int mine = p.channels - 2 * c;  // of the thread's two channels, those that exist
+  const int64_t ch = p.ch0 + (mine > 0 ? 2 * c : 0);
   grid_dependency_wait();
-  for (int i = tid; i < Where::CH; i += kSelThreads)
+  for (int i = tid; i < 2 * Where::PAIRS; i += kSelThreads)
     biases[i] = i < p.channels && a.bias.data ? load_any(a.bias.data, a.bias.dtype, (p.ch0 + i) * a.bias.s0) : 0.f;
-
   __syncthreads();
-  const float bias = biases[Where::c()];  // of the thread's channel, unless along the sequence
-  const float skip = a.D.data && mine ? load_any(a.D.data, a.D.dtype, ch * a.D.s0) : 0.f;
-  Four rate = zero4(), carry = zero4(), da = zero4(), da_low = zero4();
-  float dbias = 0.f, dbias_low = 0.f, dskip = 0.f, dskip_low = 0.f;
-  float total = 0.f;
-  const int64_t ends_at = (p.b * a.segments * a.dim + ch) * np;
+  auto of_pair = [](const float* v, int k) { return make_float2(v[2 * Where::c(k)], v[2 * Where::c(k) + 1]); };
+  const float2 bias = of_pair(biases, 0);  // unless along the sequence
+  float2 skip = both(0.f);
+  if (a.D.data && mine > 0) skip.x = load_any(a.D.data, a.D.dtype, ch * a.D.s0);
+  if (a.D.data && mine > 1) skip.y = load_any(a.D.data, a.D.dtype, (ch + 1) * a.D.s0);
+
+  Eight rate, carry;
+  float2 dbias = both(0.f), dbias_low = both(0.f), dskip = both(0.f), dskip_low = both(0.f);
+  float2 total = both(0.f);
   for (int nb = 0; nb < blocks; ++nb) {
-    const int n0 = nb * kSelBlock + sl * kSelStates;
-    const bool has = n0 < np;
-    rate = mine && has ? load_rates(a, ch, n0) : zero4();
-    carry = zero4();
-    if (!ENDS && mine && has)
-      for (int64_t s = a.segments - 1; s > p.seg; --s)
-        carry = handed_on(carry, rate, a.steps[(p.b * a.segments + s) * a.dim + ch], load4(a.ends + ends_at + s * a.dim * np + n0));
-    if constexpr (MULTI) {
-      store4(held + (nb * 3 * kSelThreads + tid) * 4, carry);
-      store4(held + ((nb * 3 + 1) * kSelThreads + tid) * 4, zero4());
-      store4(held + ((nb * 3 + 2) * kSelThreads + tid) * 4, zero4());
-    }
+    const int n0 = nb * kSelBlock + sl * kSelStates, n = n0 < np ? mine : 0;
+    rate = load_rates(a, ch, n0, n);
+    carry = ENDS ? zero8() : handed_over(a, p.b, a.segments - 1, p.seg, -1, ch, n0, n, rate);
+    if constexpr (MULTI) put8(held + nb * 6 * kHalf, kHalf, carry);
+    put8(held + (nb * 6 + 2) * kHalf, kHalf, zero8());
+    put8(held + (nb * 6 + 4) * kHalf, kHalf, zero8());
   }
 
   // where this lane's sums over channels of the first position go
   const int which = summed(lane);
   float* slab = slabs + warp * (Smem::kSlab / 4) + (which >> 2) * 4 * LN + sl * 4 + (which & 3);
-  const Walk<T, LN, ROWS> xs(a.x, p), deltas(a.delta, p), zs(a.z.data ? a.z : a.x, p), douts(a.dout, p);
-  const Walk<T, LN, ROWS> dxs(a.dx, p), ddeltas(a.ddelta, p), dzs(a.z.data ? a.dz : a.dx, p);
-  const bool all_channels = p.channels == Where::CH, packed = a.seq_idx.data != nullptr;
-  T next_x[8], next_delta[8], next_z[8], next_dout[8];
-  float dzf[8];  // dout silu'(z)
+  const Walk<T, Where> xs(a.x, p), deltas(a.delta, p), zs(a.z.data ? a.z : a.x, p), douts(a.dout, p);
+  const Walk<T, Where> dxs(a.dx, p), ddeltas(a.ddelta, p), dzs(a.z.data ? a.dz : a.dx, p);
+  const bool all_channels = p.channels == 2 * Where::PAIRS, packed = a.seq_idx.data != nullptr;
+  Raw next_x[K], next_delta[K], next_z[K], next_dout[K];
   FlagFeed<TT> feed;
-  Coefficients<T, LN, MULTI> next_bc(a, p);
+  Coefficients<T, kSelThreads, LN, MULTI> next_bc(a, p);
   auto inside = [&](int64_t i) { return all_channels && (i + 1) * TT <= a.seqlen; };
   auto fetch = [&](int64_t i) {
     const bool whole = inside(i);
@@ -143,65 +139,63 @@ __global__ void __launch_bounds__(kSelThreads, ENDS ? 4 : kBwdCtas) sel_bwd_kern
     feed.load(a, p.b, i * TT);
     next_bc.load(a, i * TT, whole);
   };
-  fetch(p.chunk1 - 1);
   for (int64_t i = p.chunk1 - 1; i >= p.chunk0; --i) {
+    // one latency of memory for 32 positions, which the CTAs beside this one fill: registers for
+    // inputs that are loaded ahead would cost more
+    fetch(i);
     const int64_t t0 = i * TT;
-    const bool whole = inside(i);
+    const bool whole = inside(i), checked = packed || !whole;
     feed.store(a, p.b, t0, flags);
-    __syncthreads();
-    const bool checked = packed || !whole;
+    if (checked) __syncthreads();  // flags are there
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
-      const float u = to_f32(next_delta[k]) + (ROWS ? biases[cc] : bias);
-      float slope = 1.f, dy = to_f32(next_dout[k]);
-      const float s = a.softplus ? step_size<T>(u, &slope) : u;
+    for (int k = 0; k < K; ++k) {
+      const float2 u = fadd2(pair_of<T>(next_delta[k], a.pairs), ROWS ? of_pair(biases, k) : bias), x = pair_of<T>(next_x[k], a.pairs);
+      float2 slope = both(1.f), dzf = both(0.f), dy = pair_of<T>(next_dout[k], a.pairs);
+      const float2 s = a.softplus ? step_size<T>(u, &slope) : u;
       if (a.z.data) {
         // silu(z) = z r and silu'(z) = r + z r (1 - r)
-        float r, less;
-        const float z = to_f32(next_z[k]);
-        sigmoid_pair_of<T>(z, r, less);
-        dzf[k] = dy * fmaf(z * r, less, r);
-        dy *= z * r;
+        float2 r, less;
+        const float2 z = pair_of<T>(next_z[k], a.pairs);
+        sigmoid_pair_of<T>(z.x, r.x, less.x);
+        sigmoid_pair_of<T>(z.y, r.y, less.y);
+        const float2 zr = fmul2(z, r);
+        dzf = fmul2(dy, ffma2(zr, less, r));
+        dy = fmul2(dy, zr);
       }
-      io[t * PITCH + cc] = make_float4(s, to_f32(next_x[k]), dy, slope);
+      float4 v = make_float4(s.x, s.y, x.x, x.y), w = make_float4(dy.x, dy.y, slope.x, slope.y);
+      if (checked) {
+        const int has = flags.valid(Where::t(k)) ? p.channels - 2 * Where::c(k) : 0;
+        if (has < 1) v.x = v.z = w.x = w.z = dzf.x = 0.f;
+        if (has < 2) v.y = v.w = w.y = w.w = dzf.y = 0.f;
+      }
+      io[Where::t(k) * PITCH + Where::c(k)] = v;
+      io2[Where::t(k) * PITCH + Where::c(k)] = w;
+      if (a.z.data) dzfs[Where::t(k) * PITCH + Where::c(k)] = dzf;
     }
-    if (checked)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
-        if (!flags.valid(t) || cc >= p.channels) {
-          io[t * PITCH + cc] = make_float4(0.f, 0.f, 0.f, 0.f);
-          dzf[k] = 0.f;
-        }
-      }
     next_bc.store(a, p, t0, checked, flags, bc);
     __syncthreads();
-    if (i > p.chunk0) fetch(i - 1);
 
     for (int nb = 0; nb < blocks; ++nb) {
-      const int n0 = nb * kSelBlock + sl * kSelStates;
-      const bool has = n0 < np;
+      const int n0 = nb * kSelBlock + sl * kSelStates, n = n0 < np ? mine : 0;
       if constexpr (MULTI) {
-        carry = load4(held + (nb * 3 * kSelThreads + tid) * 4);
-        rate = mine && has ? load_rates(a, ch, n0) : zero4();
+        carry = take8(held + nb * 6 * kHalf, kHalf);
+        rate = load_rates(a, ch, n0, n);
       }
-      const T* row = bc + nb * 4 * LN + sl * 4;
-      Four h = zero4();
-      auto start = [&](int t) {
-        const int r = flags.row[t];
-        h = a.init.data && r >= 0 && mine && has ? load_state(a.init, r, ch, n0, a.dstate) : zero4();
-      };
+      const float* row = bc + nb * 4 * LN + sl * 4;
+      Eight h;
       auto advance = [&](int t) {
         const float4 v = io[t * PITCH + c];
-        const float sx = v.x * v.y;
-        h = fma4(decays4(make_float2(v.x, v.x), rate), h, mul4(load4_of(row + t * 2 * wide), make_float2(sx, sx)));
+        const float2 s = make_float2(v.x, v.y), sx = fmul2(s, make_float2(v.z, v.w));
+        const Eight decay = decays8(s, rate);
+        const Quad B = quad(row + t * 2 * wide);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h.v[e] = ffma2(decay.v[e], h.v[e], fmul2(both(B.v[e]), sx));
       };
       if constexpr (!ENDS) {
-        if (mine && has) h = load4(a.checkpoints + ((p.b * a.nchunks + i) * a.dim + ch) * np + n0);
+        h = load8(a.checkpoints + ((p.b * a.nchunks + i) * a.dim + ch) * np + n0, np, n);
 #pragma unroll 1
         for (int q = 0; q < TT / 4; ++q) {
-          store4(sub + (q * kSelThreads + tid) * 4, h);
+          put8(sub + q * 2 * kHalf, kHalf, h);
           if (q == TT / 4 - 1) break;
           const uint32_t f = flags.word[q];
           if (f == kAllInside) {
@@ -210,55 +204,84 @@ __global__ void __launch_bounds__(kSelThreads, ENDS ? 4 : kBwdCtas) sel_bwd_kern
           } else {
 #pragma unroll 1
             for (int j = 0; j < 4; ++j) {
-              if (f >> (8 * j) & kFirst) start(q * 4 + j);
+              if (f >> (8 * j) & kFirst) h = load_states(a.init, flags.row[q * 4 + j], ch, n0, a.dstate, n);
               advance(q * 4 + j);
             }
           }
         }
       }
-      Four da_tile = zero4();
+      Eight da = zero8();  // of this tile
+      float2 tile_bias = both(0.f), tile_skip = both(0.f);
       // The sums of a position's dB and dC over the warp's channels, to the warp's slab.
-      auto keep_channels = [&](int t, Four dB, Four dC) {
-        if (!all_channels && !mine) dB = dC = zero4();  // so that 0 * infinity of no channel does not count
-        const float v = sum_channels<LN>(dB, dC, lane);
-        if ((lane & 3) < LN) slab[t * 8 * LN] = v;
+      auto keep_channels = [&](int t, float2 (&b)[8]) {
+        if (!all_channels) {  // so that 0 * infinity of no channel does not count
+#pragma unroll
+          for (int e = 0; e < 8; ++e) b[e] = make_float2(mine > 0 ? b[e].x : 0.f, mine > 1 ? b[e].y : 0.f);
+        }
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = b[e].x + b[e].y;
+        const float r = sum_channels<LN>(v, lane);
+        if ((lane & 3) < LN) slab[t * 8 * LN] = r;
+      };
+      // One position, from the gradient carried to it: h before it in `kept` times its decay.
+      // y, sa, sb: the thread's parts of the sums over the states of C h, g a h_{t-1} A and g B.
+      auto retreat = [&](int t, const Eight& decay, const Eight& kept, float2& y, float2& sa, float2& sb, float2 (&v)[8]) {
+        const float4 in = io[t * PITCH + c];
+        const float2 s = make_float2(in.x, in.y), x = make_float2(in.z, in.w);
+        const float2 dy = *reinterpret_cast<const float2*>(&io2[t * PITCH + c]);
+        const Quad B = quad(row + t * 2 * wide), C = quad(row + t * 2 * wide + wide);
+        const float2 sx = fmul2(s, x);
+        y = sa = sb = both(0.f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 g = ffma2(both(C.v[e]), dy, carry.v[e]);
+          const float2 now = ffma2(both(B.v[e]), sx, kept.v[e]);
+          const float2 w = fmul2(g, kept.v[e]);
+          carry.v[e] = fmul2(decay.v[e], g);
+          v[e] = fmul2(g, sx);
+          v[4 + e] = fmul2(now, dy);
+          y = ffma2(both(C.v[e]), now, y);
+          sb = ffma2(both(B.v[e]), g, sb);
+          sa = ffma2(w, rate.v[e], sa);
+          da.v[e] = ffma2(w, s, da.v[e]);
+        }
       };
 #pragma unroll 1
       for (int q = TT / 4 - 1; q >= 0; --q) {
         const uint32_t f = flags.word[q];
-        float y[4], sa[4], sb[4];  // sums over the states of C h, g a h_{t-1} A and g B
+        float2 y[4], sa[4], sb[4];
         if (f == kAllInside) {
-          Four decay[4], kept[4], now[4];  // a, a h_{t-1} and h of the four positions
-          if (!ENDS) h = load4(sub + (q * kSelThreads + tid) * 4);
+          Eight decay[4], kept[4];  // a and a h_{t-1} of the four positions
+          if (!ENDS) h = take8(sub + q * 2 * kHalf, kHalf);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int t = q * 4 + j;
-            const float4 v = io[t * PITCH + c];
-            decay[j] = decays4(make_float2(v.x, v.x), rate);
+            const float4 v = io[(q * 4 + j) * PITCH + c];
+            const float2 s = make_float2(v.x, v.y), sx = fmul2(s, make_float2(v.z, v.w));
+            decay[j] = decays8(s, rate);
             if constexpr (!ENDS) {
-              const float sx = v.x * v.y;
-              kept[j] = mul4(decay[j], h);
-              h = now[j] = fma4(load4_of(row + t * 2 * wide), make_float2(sx, sx), kept[j]);
+              const Quad B = quad(row + (q * 4 + j) * 2 * wide);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                kept[j].v[e] = fmul2(decay[j].v[e], h.v[e]);
+                h.v[e] = ffma2(both(B.v[e]), sx, kept[j].v[e]);
+              }
             }
           }
 #pragma unroll
           for (int j = 3; j >= 0; --j) {
             const int t = q * 4 + j;
-            const float4 v = io[t * PITCH + c];
-            const float2 dy = make_float2(v.z, v.z);
-            const Four C = load4_of(row + t * 2 * wide + wide);
-            const Four g = fma4(C, dy, carry);
-            carry = mul4(decay[j], g);
             if constexpr (!ENDS) {
-              const float sx = v.x * v.y;
-              const Four w = mul4(g, kept[j]);
-              y[j] = dot4(C, now[j]);
-              sb[j] = dot4(load4_of(row + t * 2 * wide), g);
-              sa[j] = dot4(w, rate);
-              da_tile = fma4(w, make_float2(v.x, v.x), da_tile);
-              keep_channels(t, mul4(g, make_float2(sx, sx)), mul4(now[j], dy));
+              float2 v[8];
+              retreat(t, decay[j], kept[j], y[j], sa[j], sb[j], v);
+              keep_channels(t, v);
             } else {
-              if (nb == 0) total += v.x;
+              const float4 in = io[t * PITCH + c];
+              const float2 dy = *reinterpret_cast<const float2*>(&io2[t * PITCH + c]);
+              const Quad C = quad(row + t * 2 * wide + wide);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) carry.v[e] = fmul2(decay[j].v[e], ffma2(both(C.v[e]), dy, carry.v[e]));
+              if (nb == 0) total = fadd2(total, make_float2(in.x, in.y));
             }
           }
         } else {
@@ -267,41 +290,41 @@ __global__ void __launch_bounds__(kSelThreads, ENDS ? 4 : kBwdCtas) sel_bwd_kern
           for (int j = 3; j >= 0; --j) {
             const int t = q * 4 + j, r = flags.row[t];
             const uint32_t fj = f >> (8 * j);
-            float yj = 0.f, saj = 0.f, sbj = 0.f;
-            Four dB = zero4(), dC = zero4();
+            float2 yj = both(0.f), saj = both(0.f), sbj = both(0.f);
+            float2 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = both(0.f);
             if (fj & kValid) {
-              const float4 v = io[t * PITCH + c];
-              const Four decay = decays4(make_float2(v.x, v.x), rate), C = load4_of(row + t * 2 * wide + wide);
-              if (fj & kLast) carry = a.dfinal.data && r >= 0 && mine && has ? load_state(a.dfinal, r, ch, n0, a.dstate) : zero4();
-              const Four g = fma4(C, make_float2(v.z, v.z), carry);
+              const float4 in = io[t * PITCH + c];
+              const Eight decay = decays8(make_float2(in.x, in.y), rate);
+              if (fj & kLast) carry = load_states(a.dfinal, r, ch, n0, a.dstate, n);
               if constexpr (!ENDS) {
-                h = load4(sub + (q * kSelThreads + tid) * 4);
+                h = take8(sub + q * 2 * kHalf, kHalf);
 #pragma unroll 1
                 for (int k = 0; k < j; ++k) {
-                  if (f >> (8 * k) & kFirst) start(q * 4 + k);
+                  if (f >> (8 * k) & kFirst) h = load_states(a.init, flags.row[q * 4 + k], ch, n0, a.dstate, n);
                   advance(q * 4 + k);
                 }
-                if (fj & kFirst) start(t);
-                const float sx = v.x * v.y;
-                const Four B = load4_of(row + t * 2 * wide), kept = mul4(decay, h), now = fma4(B, make_float2(sx, sx), kept), w = mul4(g, kept);
-                yj = dot4(C, now);
-                sbj = dot4(B, g);
-                saj = dot4(w, rate);
-                da_tile = fma4(w, make_float2(v.x, v.x), da_tile);
-                dB = mul4(g, make_float2(sx, sx));
-                dC = mul4(now, make_float2(v.z, v.z));
+                if (fj & kFirst) h = load_states(a.init, r, ch, n0, a.dstate, n);
+                Eight kept;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) kept.v[e] = fmul2(decay.v[e], h.v[e]);
+                retreat(t, decay, kept, yj, saj, sbj, v);
               } else {
-                if (nb == 0) total += v.x;
+                const float2 dy = *reinterpret_cast<const float2*>(&io2[t * PITCH + c]);
+                const Quad C = quad(row + t * 2 * wide + wide);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) carry.v[e] = fmul2(decay.v[e], ffma2(both(C.v[e]), dy, carry.v[e]));
+                if (nb == 0) total = fadd2(total, make_float2(in.x, in.y));
               }
-              carry = mul4(decay, g);
               if (fj & kFirst) {
-                if (!ENDS && a.dinit.data && r >= 0 && mine && has) store_state(a.dinit, r, ch, n0, a.dstate, carry);
-                if (ENDS) total = INFINITY;
-                carry = zero4();
+                if (!ENDS) store_states(a.dinit, r, ch, n0, a.dstate, n, carry);
+                if (ENDS) total = both(INFINITY);
+                carry = zero8();
               }
             }
             if constexpr (!ENDS) {
-              keep_channels(t, dB, dC);
+              keep_channels(t, v);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (e == j) y[e] = yj, sa[e] = saj, sb[e] = sbj;
@@ -309,71 +332,84 @@ __global__ void __launch_bounds__(kSelThreads, ENDS ? 4 : kBwdCtas) sel_bwd_kern
           }
         }
         if constexpr (!ENDS) {
-          sum_lanes<LN>(y, sl);
-          sum_lanes<LN>(sa, sl);
-          sum_lanes<LN>(sb, sl);
+          float l[3][2][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            l[0][0][j] = y[j].x, l[0][1][j] = y[j].y;
+            l[1][0][j] = sa[j].x, l[1][1][j] = sa[j].y;
+            l[2][0][j] = sb[j].x, l[2][1][j] = sb[j].y;
+          }
+#pragma unroll
+          for (int e = 0; e < 6; ++e) sum_lanes<LN>(l[e / 2][e % 2], sl);
 #pragma unroll
           for (int j = 0; j < 4 / LN; ++j) {
             const int t = q * 4 + sl * (4 / LN) + j;
-            float* s = sums + (t * PITCH + c) * 3;
-            if (MULTI && nb > 0) {
-              y[j] += s[0];
-              sa[j] += s[1];
-              sb[j] += s[2];
+            float2 yt = make_float2(l[0][0][j], l[0][1][j]), sat = make_float2(l[1][0][j], l[1][1][j]), sbt = make_float2(l[2][0][j], l[2][1][j]);
+            if constexpr (MULTI) {
+              float2* s = sums + (t * PITCH + c) * 3;
+              if (nb > 0) yt = fadd2(yt, s[0]), sat = fadd2(sat, s[1]), sbt = fadd2(sbt, s[2]);
+              if (nb + 1 < blocks) {
+                s[0] = yt, s[1] = sat, s[2] = sbt;
+                continue;
+              }
             }
-            if (MULTI && nb + 1 < blocks) {
-              s[0] = y[j];
-              s[1] = sa[j];
-              s[2] = sb[j];
-              continue;
-            }
-            const float4 v = io[t * PITCH + c];
-            const float du = fmaf(sa[j], 0.693147181f, v.y * sb[j]) * v.w;
-            io[t * PITCH + c] = make_float4(fmaf(v.x, sb[j], skip * v.z), du, fmaf(skip, v.y, y[j]), 0.f);
-            add_to(dbias, dbias_low, du);
-            add_to(dskip, dskip_low, v.z * v.y);
+            const float4 in = io[t * PITCH + c], in2 = io2[t * PITCH + c];
+            const float2 s = make_float2(in.x, in.y), x = make_float2(in.z, in.w), dy = make_float2(in2.x, in2.y);
+            const float2 du = fmul2(ffma2(sat, both(0.693147181f), fmul2(x, sbt)), make_float2(in2.z, in2.w));
+            const float2 dx = ffma2(s, sbt, fmul2(skip, dy));
+            io[t * PITCH + c] = make_float4(dx.x, dx.y, du.x, du.y);
+            *reinterpret_cast<float2*>(&io2[t * PITCH + c]) = ffma2(skip, x, yt);
+            tile_bias = fadd2(tile_bias, du);
+            tile_skip = ffma2(dy, x, tile_skip);
           }
         }
       }
-      if constexpr (MULTI) store4(held + (nb * 3 * kSelThreads + tid) * 4, carry);
+      if constexpr (MULTI) put8(held + nb * 6 * kHalf, kHalf, carry);
       if constexpr (!ENDS) {
-        if constexpr (MULTI) {
-          da = load4(held + ((nb * 3 + 1) * kSelThreads + tid) * 4);
-          da_low = load4(held + ((nb * 3 + 2) * kSelThreads + tid) * 4);
-        }
-        add_to(da, da_low, da_tile);
-        if constexpr (MULTI) {
-          store4(held + ((nb * 3 + 1) * kSelThreads + tid) * 4, da);
-          store4(held + ((nb * 3 + 2) * kSelThreads + tid) * 4, da_low);
-        }
-        __syncthreads();
-        // this pass's states of dB and dC: the warps' sums to the CTA's
-        for (int e = tid; e < TT * 8 * LN; e += kSelThreads) {
-          const int t = e / (8 * LN), v = e % (8 * LN), n = nb * kSelBlock + v % (4 * LN);
-          if (t0 + t >= a.seqlen || n >= np) continue;
-          float s = 0.f;
+        add_to(dbias, dbias_low, tile_bias);
+        add_to(dskip, dskip_low, tile_skip);
+        Eight hi = take8(held + (nb * 6 + 2) * kHalf, kHalf), lo = take8(held + (nb * 6 + 4) * kHalf, kHalf);
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) s += slabs[w * (Smem::kSlab / 4) + e];
-          a.parts_bc[(((p.b * a.seqlen + t0 + t) * a.tiles + p.tile) * 2 + v / (4 * LN)) * np + n] = s;
+        for (int e = 0; e < 4; ++e) add_to(hi.v[e], lo.v[e], da.v[e]);
+        put8(held + (nb * 6 + 2) * kHalf, kHalf, hi);
+        put8(held + (nb * 6 + 4) * kHalf, kHalf, lo);
+        __syncthreads();
+        // this pass's states of dB and dC: the warps' sums to the CTA's, one value of every
+        // kSelThreads / (8 LN)-th position for each thread
+        constexpr int STEP = kSelThreads / (8 * LN);
+        const int v = tid % (8 * LN), m = nb * kSelBlock + v % (4 * LN), first = tid / (8 * LN);
+        if (m < np) {
+          const float* from = slabs + first * 8 * LN + v;
+          const int64_t row_size = a.tiles * 2 * np;
+          float* to = a.parts_bc + (p.b * a.seqlen + t0 + first) * row_size + (p.tile * 2 + v / (4 * LN)) * np + m;
+          const int count = static_cast<int>(a.seqlen - t0 < TT ? a.seqlen - t0 : TT);
+#pragma unroll 4
+          for (int t = first; t < count; t += STEP, to += STEP * row_size, from += STEP * 8 * LN) {
+            float r = from[0];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) r += from[w * (Smem::kSlab / 4)];
+            *to = r;
+          }
         }
         if (nb + 1 < blocks) __syncthreads();
       }
     }
     if constexpr (!ENDS) {
-      float o[8];
+      float2 o[K];
 #pragma unroll
       for (int part = 0; part < 3; ++part) {
         if (part == 2 && !a.z.data) break;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
-          const float4 v = io[t * PITCH + cc];
-          o[k] = part == 0 ? v.x : part == 1 ? v.y : dzf[k] * v.z;
+        for (int k = 0; k < K; ++k) {
+          const int at = Where::t(k) * PITCH + Where::c(k);
+          const float4* from = part == 2 ? &io2[at] : &io[at];
+          o[k] = reinterpret_cast<const float2*>(from)[part == 1];
+          if (part == 2) o[k] = fmul2(o[k], dzfs[at]);
         }
         if (packed)
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (!flags.valid(Where::t() + k * Where::DT)) o[k] = 0.f;
+          for (int k = 0; k < K; ++k)
+            if (!flags.valid(Where::t(k))) o[k] = both(0.f);
         if (part == 0) dxs.store(a, a.dx, p, i, whole, o);
         else if (part == 1) ddeltas.store(a, a.ddelta, p, i, whole, o);
         else dzs.store(a, a.dz, p, i, whole, o);
@@ -382,37 +418,36 @@ __global__ void __launch_bounds__(kSelThreads, ENDS ? 4 : kBwdCtas) sel_bwd_kern
     __syncthreads();
   }
 
+  const int64_t part = p.b * a.segments + p.seg;
   for (int nb = 0; nb < blocks; ++nb) {
-    const int n0 = nb * kSelBlock + sl * kSelStates;
-    if (n0 >= np || !mine) continue;
+    const int n0 = nb * kSelBlock + sl * kSelStates, n = n0 < np ? mine : 0;
     if constexpr (ENDS) {
-      if constexpr (MULTI) carry = load4(held + (nb * 3 * kSelThreads + tid) * 4);
-      store4(a.ends + ends_at + p.seg * a.dim * np + n0, carry);
+      if constexpr (MULTI) carry = take8(held + nb * 6 * kHalf, kHalf);
+      store8(a.ends + (part * a.dim + ch) * np + n0, np, n, carry);
     } else {
-      if constexpr (MULTI) {
-        da = load4(held + ((nb * 3 + 1) * kSelThreads + tid) * 4);
-        da_low = load4(held + ((nb * 3 + 2) * kSelThreads + tid) * 4);
-      }
-      store4(a.parts_a + ((p.b * a.segments + p.seg) * a.dim + ch) * np + n0,
-             Four{fadd2(da.lo, da_low.lo), fadd2(da.hi, da_low.hi)});
+      Eight hi = take8(held + (nb * 6 + 2) * kHalf, kHalf);
+      const Eight lo = take8(held + (nb * 6 + 4) * kHalf, kHalf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) hi.v[e] = fadd2(hi.v[e], lo.v[e]);
+      store8(a.parts_a + (part * a.dim + ch) * np + n0, np, n, hi);
     }
   }
-  if constexpr (ENDS) {
-    if (mine && sl == 0) a.steps[(p.b * a.segments + p.seg) * a.dim + ch] = total;
-    return;
-  }
-  dskip += dskip_low;
-  dbias += dbias_low;
+  float2 one = total, two = both(0.f);
+  if constexpr (!ENDS) {
+    one = fadd2(dskip, dskip_low);
+    two = fadd2(dbias, dbias_low);
 #pragma unroll
-  for (int bit = 1; bit < LN; bit *= 2) {
-    dskip += __shfl_xor_sync(~0u, dskip, bit);
-    dbias += __shfl_xor_sync(~0u, dbias, bit);
+    for (int bit = 1; bit < LN; bit *= 2) {
+      one = fadd2(one, make_float2(__shfl_xor_sync(~0u, one.x, bit), __shfl_xor_sync(~0u, one.y, bit)));
+      two = fadd2(two, make_float2(__shfl_xor_sync(~0u, two.x, bit), __shfl_xor_sync(~0u, two.y, bit)));
+    }
   }
-  if (mine && sl == 0) {
-    float* d = a.parts_d + (p.b * a.segments + p.seg) * 2 * a.dim + ch;
-    d[0] = dskip;
-    d[a.dim] = dbias;
-  }
+  if (sl != 0) return;
+  float* d = ENDS ? a.steps + part * a.dim + ch : a.parts_d + part * 2 * a.dim + ch;
+  if (mine > 0) d[0] = one.x;
+  if (mine > 1) d[1] = one.y;
+  if (!ENDS && mine > 0) d[a.dim] = two.x;
+  if (!ENDS && mine > 1) d[a.dim + 1] = two.y;
 }
 
 // dB and dC: the sums over a group's CTAs.  A thread takes one state of one position.
@@ -459,7 +494,7 @@ __global__ void __launch_bounds__(kThreads) sel_sum_params_kernel(const __grid_c
 
 template <typename T, int LN, bool ROWS, bool MULTI, bool ENDS>
 cudaError_t launch(const SelArgs& a, cudaStream_t s) {
-  const size_t smem = static_cast<size_t>(BwdSmem<T, LN>::bytes(a));
+  const size_t smem = static_cast<size_t>(BwdSmem<LN>::bytes(a));
   const auto kernel = sel_bwd_kernel<T, LN, ROWS, MULTI, ENDS>;
   const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;

@@ -17,65 +17,72 @@ namespace {
 #define FWDC 4
 #endif
 constexpr int kFwdCtas = FWDC;
-// Shared memory: flags; (s, s x) by position and channel; y by position and channel; B and
-// C; with several passes the states between two tiles.
-template <typename T, int LN>
+constexpr int kSelThreads = 128;
+
+// Shared memory: flags; (s, s x) by position and channel; y by position and channel; B and C; with
+// several passes the states between two tiles.
+template <int LN>
 struct FwdSmem {
-  static constexpr int kFlags = 256;
-  static constexpr int kIo = Tile<LN, false>::T * Tile<LN, false>::PITCH * 8;
-  static constexpr int kY = (Tile<LN, false>::T * Tile<LN, false>::PITCH * 4 + 15) / 16 * 16;
+  static constexpr int T = 8 * LN, CH = kSelChannels / LN, PITCH = CH + 2;
+  static constexpr int kFlags = 256, kIo = T * PITCH * 8, kY = (T * PITCH * 4 + 15) / 16 * 16;
   static int64_t bytes(const SelArgs& a) {
-    return kFlags + kIo + kY + Tile<LN, false>::T * 8 * LN * a.blocks * sizeof(T) + (a.blocks > 1 ? a.blocks * kSelThreads * 16 : 0);
+    return kFlags + kIo + kY + T * 8 * LN * a.blocks * 4 + (a.blocks > 1 ? a.blocks * kSelThreads * 16 : 0);
   }
 };
 
 // ENDS: only what each segment carries out of itself, for the segments behind it.
 template <typename T, int LN, bool ROWS, bool MULTI, bool ENDS>
 __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __grid_constant__ SelArgs a) {
-  using Where = Tile<LN, ROWS>;
-  constexpr int PITCH = Where::PITCH, TT = Where::T;
+  using Smem = FwdSmem<LN>;
+  using Where = Tile<kSelThreads, LN, ROWS>;
+  constexpr int K = Where::K, PITCH = Smem::PITCH, TT = Where::T;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float biases[Where::CH], skips[Where::CH];
+  __shared__ float biases[Smem::CH], skips[Smem::CH];
   SelFlags& flags = *reinterpret_cast<SelFlags*>(smem);
-  float2* io = reinterpret_cast<float2*>(smem + FwdSmem<T, LN>::kFlags);
-  float* ys = reinterpret_cast<float*>(smem + FwdSmem<T, LN>::kFlags + FwdSmem<T, LN>::kIo);
-  T* bc = reinterpret_cast<T*>(smem + FwdSmem<T, LN>::kFlags + FwdSmem<T, LN>::kIo + FwdSmem<T, LN>::kY);
+  float2* io = reinterpret_cast<float2*>(smem + Smem::kFlags);
+  float* ys = reinterpret_cast<float*>(smem + Smem::kFlags + Smem::kIo);
+  float* bc = reinterpret_cast<float*>(smem + Smem::kFlags + Smem::kIo + Smem::kY);
   const int np = static_cast<int>(a.padded), blocks = MULTI ? a.blocks : 1, wide = 4 * LN * blocks;
-  float* held = reinterpret_cast<float*>(bc + TT * 2 * wide);
+  float* held = bc + TT * 2 * wide;
 
   const SelPlace p = sel_place<LN>(a);
+  if (ENDS && p.seg + 1 == a.segments) return;  // nothing is behind it
   const int tid = threadIdx.x, sl = tid % LN, c = tid / LN;
-  const bool mine = c < p.channels;
+  const int mine = c < p.channels ? 1 : 0;
   const int64_t ch = p.ch0 + (mine ? c : 0);
   grid_dependency_wait();
-  for (int i = tid; i < Where::CH; i += kSelThreads) {
+  for (int i = tid; i < Smem::CH; i += kSelThreads) {
     const bool is = i < p.channels;
     biases[i] = is && a.bias.data ? load_any(a.bias.data, a.bias.dtype, (p.ch0 + i) * a.bias.s0) : 0.f;
     skips[i] = is && a.D.data ? load_any(a.D.data, a.D.dtype, (p.ch0 + i) * a.D.s0) : 0.f;
   }
-
   __syncthreads();
-  const float bias = biases[Where::c()], skip = skips[Where::c()];  // of the thread's channel, unless along the sequence
+  auto of_pair = [](const float* v, int k) { return make_float2(v[2 * Where::c(k)], v[2 * Where::c(k) + 1]); };
+  const float2 bias = of_pair(biases, 0), skip = of_pair(skips, 0);  // unless along the sequence
 
   Four h = zero4(), rate = zero4();
   float total = 0.f;  // ENDS: the sum of step sizes since the segment's start
-  const int64_t ends_at = (p.b * a.segments * a.dim + ch) * np;  // of segment 0
+  auto rates = [&](int n0) { return mine && n0 < np ? of4(load_rates(a.A, ch, n0, a.dstate)) : zero4(); };
   for (int nb = 0; nb < blocks; ++nb) {
     const int n0 = nb * kSelBlock + sl * kSelStates;
-    const bool has = n0 < np;
+    rate = rates(n0);
     h = zero4();
-    rate = mine && has ? load_rates(a, ch, n0) : zero4();
-    if (!ENDS && mine && has)
-      for (int64_t s = 0; s < p.seg; ++s)
-        h = handed_on(h, rate, a.steps[(p.b * a.segments + s) * a.dim + ch], load4(a.ends + ends_at + s * a.dim * np + n0));
+    if (!ENDS && mine && n0 < np)
+      for (int64_t s = 0; s < p.seg; ++s) {
+        const int64_t at = (p.b * a.segments + s) * a.dim + ch;
+        const float sum = a.steps[at];
+        const float4 e = *reinterpret_cast<const float4*>(a.ends + at * np + n0);
+        h.lo = make_float2(handed_on(h.lo.x, rate.lo.x, sum, e.x), handed_on(h.lo.y, rate.lo.y, sum, e.y));
+        h.hi = make_float2(handed_on(h.hi.x, rate.hi.x, sum, e.z), handed_on(h.hi.y, rate.hi.y, sum, e.w));
+      }
     if constexpr (MULTI) store4(held + (nb * kSelThreads + tid) * 4, h);
   }
 
-  const Walk<T, LN, ROWS> xs(a.x, p), deltas(a.delta, p), zs(a.z.data ? a.z : a.x, p), outs(a.out, p);
-  const bool all_channels = p.channels == Where::CH, packed = a.seq_idx.data != nullptr;
-  T x[8], next_x[8], next_delta[8], z[8];
+  const Walk<T, Where> xs(a.x, p), deltas(a.delta, p), zs(a.z.data ? a.z : a.x, p), outs(a.out, p);
+  const bool all_channels = p.channels == Smem::CH, packed = a.seq_idx.data != nullptr;
+  Raw x[K], next_x[K], next_delta[K], z[K];
   FlagFeed<TT> feed;
-  Coefficients<T, LN, MULTI> next_bc(a, p);
+  Coefficients<T, kSelThreads, LN, MULTI> next_bc(a, p);
   auto inside = [&](int64_t i) { return all_channels && (i + 1) * TT <= a.seqlen; };
   auto fetch = [&](int64_t i) {
     const bool whole = inside(i);
@@ -87,24 +94,22 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
   fetch(p.chunk0);
   for (int64_t i = p.chunk0; i < p.chunk1; ++i) {
     const int64_t t0 = i * TT;
-    const bool whole = inside(i);
+    const bool whole = inside(i), checked = packed || !whole;
     feed.store(a, p.b, t0, flags);
-    __syncthreads();  // flags are there
-    const bool checked = packed || !whole;
+    if (checked) __syncthreads();  // flags are there
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
+    for (int k = 0; k < K; ++k) {
       x[k] = next_x[k];
-      const float u = to_f32(next_delta[k]) + (ROWS ? biases[cc] : bias);
-      const float s = a.softplus ? step_size<T>(u) : u, sx = s * to_f32(x[k]);
-      io[t * PITCH + cc] = make_float2(s, sx);
-    }
-    if (checked)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
-        if (!flags.valid(t) || cc >= p.channels) io[t * PITCH + cc] = make_float2(0.f, 0.f);
+      const float2 u = fadd2(pair_of<T>(next_delta[k], a.pairs), ROWS ? of_pair(biases, k) : bias);
+      const float2 s = a.softplus ? step_size<T>(u) : u, sx = fmul2(s, pair_of<T>(x[k], a.pairs));
+      float4 v = make_float4(s.x, sx.x, s.y, sx.y);
+      if (checked) {
+        const int has = flags.valid(Where::t(k)) ? p.channels - 2 * Where::c(k) : 0;
+        if (has < 1) v.x = v.y = 0.f;
+        if (has < 2) v.z = v.w = 0.f;
       }
+      *reinterpret_cast<float4*>(&io[Where::t(k) * PITCH + 2 * Where::c(k)]) = v;
+    }
     next_bc.store(a, p, t0, checked, flags, bc);
     __syncthreads();
     if (!ENDS && a.z.data) zs.load(a, a.z, p, i, whole, z);
@@ -112,14 +117,14 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
 
     for (int nb = 0; nb < blocks; ++nb) {
       const int n0 = nb * kSelBlock + sl * kSelStates;
-      const bool has = n0 < np;
+      const bool has = n0 < np && mine;
       if constexpr (MULTI) {
         h = load4(held + (nb * kSelThreads + tid) * 4);
-        rate = mine && has ? load_rates(a, ch, n0) : zero4();
+        rate = rates(n0);
       }
-      if (!ENDS && a.checkpoints && mine && has)
+      if (!ENDS && a.checkpoints && has)
         store4(a.checkpoints + ((p.b * a.nchunks + i) * a.dim + ch) * np + n0, h);
-      const T* row = bc + nb * 4 * LN + sl * 4;
+      const float* row = bc + nb * 4 * LN + sl * 4;
       // y of four positions from q * 4 on: over the states' threads, then to shared memory
       auto keep = [&](int q, float (&y)[4]) {
         sum_lanes<LN>(y, sl);
@@ -139,9 +144,9 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
             const int t = q * 4 + j;
             const float2 v = io[t * PITCH + c];
             decay[j] = decays4(make_float2(v.x, v.x), rate);
-            add[j] = mul4(load4_of(row + t * 2 * wide), make_float2(v.y, v.y));
+            add[j] = mul4(load4(row + t * 2 * wide), make_float2(v.y, v.y));
             if (ENDS && nb == 0) total += v.x;
-            if (!ENDS) C[j] = load4_of(row + t * 2 * wide + wide);
+            if (!ENDS) C[j] = load4(row + t * 2 * wide + wide);
           }
           float y[2][4];
 #pragma unroll
@@ -166,15 +171,15 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
             float yj = 0.f;
             if (fj & kValid) {
               if (fj & kFirst) {
-                h = a.init.data && r >= 0 && mine && has ? load_state(a.init, r, ch, n0, a.dstate) : zero4();
+                h = a.init.data && r >= 0 && has ? of4(load_state(a.init, r, ch, n0, a.dstate)) : zero4();
                 if (ENDS) total = INFINITY;
               }
               const float2 v = io[t * PITCH + c];
-              h = fma4(decays4(make_float2(v.x, v.x), rate), h, mul4(load4_of(row + t * 2 * wide), make_float2(v.y, v.y)));
+              h = fma4(decays4(make_float2(v.x, v.x), rate), h, mul4(load4(row + t * 2 * wide), make_float2(v.y, v.y)));
               if (ENDS && nb == 0) total += v.x;
-              if (!ENDS) yj = dot4(load4_of(row + t * 2 * wide + wide), h);
-              if (!ENDS && (fj & kLast) && a.final_states.data && r >= 0 && mine && has)
-                store_state(a.final_states, r, ch, n0, a.dstate, h);
+              if (!ENDS) yj = dot4(load4(row + t * 2 * wide + wide), h);
+              if (!ENDS && (fj & kLast) && a.final_states.data && r >= 0 && has)
+                store_state(a.final_states, r, ch, n0, a.dstate, to4(h));
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -187,24 +192,25 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
     }
     __syncthreads();
     if constexpr (!ENDS) {
-      float out[8];
+      float2 out[K];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int t = Where::t() + k * Where::DT, cc = Where::c() + k * Where::DC;
-        out[k] = ys[t * PITCH + cc];
-      }
+      for (int k = 0; k < K; ++k) out[k] = *reinterpret_cast<const float2*>(&ys[Where::t(k) * PITCH + 2 * Where::c(k)]);
       if (a.D.data)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) out[k] = fmaf(ROWS ? skips[Where::c() + k * Where::DC] : skip, to_f32(x[k]), out[k]);
+        for (int k = 0; k < K; ++k) out[k] = ffma2(ROWS ? of_pair(skips, k) : skip, pair_of<T>(x[k], a.pairs), out[k]);
       if (a.z.data)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) out[k] *= silu_of<T>(to_f32(z[k]));
-      if (packed)
+        for (int k = 0; k < K; ++k) {
+          const float2 v = pair_of<T>(z[k], a.pairs);
+          out[k] = fmul2(out[k], make_float2(silu_of<T>(v.x), silu_of<T>(v.y)));
+        }
+      if (packed) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (!flags.valid(Where::t() + k * Where::DT)) out[k] = 0.f;
+        for (int k = 0; k < K; ++k)
+          if (!flags.valid(Where::t(k))) out[k] = both(0.f);
+        __syncthreads();  // flags have been read
+      }
       outs.store(a, a.out, p, i, whole, out);
-      __syncthreads();  // flags and y have been read
     }
   }
   if (ENDS && mine) {
@@ -212,7 +218,7 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
       const int n0 = nb * kSelBlock + sl * kSelStates;
       if (n0 >= np) continue;
       if constexpr (MULTI) h = load4(held + (nb * kSelThreads + tid) * 4);
-      store4(a.ends + ends_at + p.seg * a.dim * np + n0, h);
+      store4(a.ends + ((p.b * a.segments + p.seg) * a.dim + ch) * np + n0, h);
     }
     if (sl == 0) a.steps[(p.b * a.segments + p.seg) * a.dim + ch] = total;
   }
@@ -220,7 +226,7 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
 
 template <typename T, int LN, bool ROWS, bool MULTI, bool ENDS>
 cudaError_t launch(const SelArgs& a, cudaStream_t s) {
-  const size_t smem = static_cast<size_t>(FwdSmem<T, LN>::bytes(a));
+  const size_t smem = static_cast<size_t>(FwdSmem<LN>::bytes(a));
   const auto kernel = sel_fwd_kernel<T, LN, ROWS, MULTI, ENDS>;
   const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;

@@ -7,7 +7,7 @@
 namespace cc1d {
 
 constexpr int kSelChunk = 32;                    // the most positions of a tile, and between two checkpoints
-constexpr int kSelThreads = 128;                 // a CTA of the sequence kernels
+constexpr int kSelChannels = 128;                // channels of a CTA times the threads that share one state vector
 constexpr int kSelStates = 4;                    // states of a channel that a thread holds
 constexpr int kSelBlock = 16;                    // states of a channel that a pass over a tile takes, at most
 
@@ -20,13 +20,14 @@ struct SelArgs {
   float* checkpoints;
   bool softplus;
   // the plan (sel_plan)
-  int lanes;                             // threads that share a channel: 1, 2 or 4
+  int lanes;                             // threads that share a channel's states: 1, 2 or 4
   int blocks;                            // passes over a tile: ceil(dstate / 16)
   int64_t padded;                        // dstate rounded up to a multiple of 4
   int64_t nchunks;                       // tiles along the sequence: ceil(seqlen / (8 lanes))
   int64_t gdim, group_tiles, tiles;      // channels of a group, CTAs that they take, CTAs of all groups
   int64_t segments, segment_chunks;      // parts of the sequence that run side by side, chunks of one
   bool rows;                             // unit stride along the sequence: threads go along it
+  bool pairs;                            // two neighbouring channels move as one word, in every tensor
   // workspace
   float* ends;      // (batch, segments, dim, padded): what a segment alone carries out of itself
   float* steps;     // (batch, segments, dim): the sum of its step sizes, or infinity if it is cut

@@ -38,11 +38,13 @@ __global__ void __launch_bounds__(kThreads) sel_update_kernel(const SelUpdateArg
     h[v] = rate[v] = zero4();
     if (!live || n0 >= a.dstate) continue;
     if constexpr (PACKED) {
-      h[v] = load4(static_cast<const float*>(a.state.data) + row * a.state.s0 + d * a.state.s1 + n0);
-      rate[v] = mul4(load4(static_cast<const float*>(a.A.data) + d * a.A.s0 + n0), make_float2(kLog2e, kLog2e));
+      h[v] = of4(*reinterpret_cast<const float4*>(static_cast<const float*>(a.state.data) + row * a.state.s0 + d * a.state.s1 + n0));
+      rate[v] = of4(*reinterpret_cast<const float4*>(static_cast<const float*>(a.A.data) + d * a.A.s0 + n0));
+      rate[v].lo = fmul2(rate[v].lo, both(kLog2e));
+      rate[v].hi = fmul2(rate[v].hi, both(kLog2e));
     } else {
-      h[v] = load_state(a.state, row, d, n0, a.dstate);
-      rate[v] = load_rates(a.A, d, n0, a.dstate);
+      h[v] = of4(load_state(a.state, row, d, n0, a.dstate));
+      rate[v] = of4(load_rates(a.A, d, n0, a.dstate));
     }
   }
   const float bias = live && a.bias.data ? load_any(a.bias.data, a.bias.dtype, d * a.bias.s0) : 0.f;
@@ -51,17 +53,19 @@ __global__ void __launch_bounds__(kThreads) sel_update_kernel(const SelUpdateArg
     float y = 0.f, x = 0.f;
     if (live) {
       x = load_el<T>(a.x, b, d, l);
-      float s = load_el<T>(a.delta, b, d, l) + bias;
+      float2 s = both(load_el<T>(a.delta, b, d, l) + bias);
       if (a.softplus) s = step_size<T>(s);
-      const float2 s2 = make_float2(s, s), sx = make_float2(s * x, s * x);
+      const float2 sx = fmul2(s, both(x));
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
         const int64_t n0 = (v * LANES + sl) * 4;
         if (n0 >= a.dstate) continue;
         const Four B = load_inputs<T, PACKED>(a.B, a.B_group, b, g, n0, l, a.dstate);
         const Four C = load_inputs<T, PACKED>(a.C, a.C_group, b, g, n0, l, a.dstate);
-        h[v] = fma4(decays4(s2, rate[v]), h[v], mul4(B, sx));
-        y += dot4(C, h[v]);
+        h[v].lo = ffma2(decays(s, rate[v].lo), h[v].lo, fmul2(B.lo, sx));
+        h[v].hi = ffma2(decays(s, rate[v].hi), h[v].hi, fmul2(B.hi, sx));
+        const float2 sum = ffma2(C.hi, h[v].hi, fmul2(C.lo, h[v].lo));
+        y += sum.x + sum.y;
       }
     }
 #pragma unroll
@@ -78,8 +82,8 @@ __global__ void __launch_bounds__(kThreads) sel_update_kernel(const SelUpdateArg
   for (int v = 0; v < VEC; ++v) {
     const int64_t n0 = (v * LANES + sl) * 4;
     if (n0 >= a.dstate) continue;
-    if constexpr (PACKED) store4(static_cast<float*>(a.state.data) + row * a.state.s0 + d * a.state.s1 + n0, h[v]);
-    else store_state(a.state, row, d, n0, a.dstate, h[v]);
+    if constexpr (PACKED) *reinterpret_cast<float4*>(static_cast<float*>(a.state.data) + row * a.state.s0 + d * a.state.s1 + n0) = to4(h[v]);
+    else store_state(a.state, row, d, n0, a.dstate, to4(h[v]));
   }
 }
 
