@@ -15,7 +15,9 @@ namespace {
 // One pass over the logits: each warp walks a strip of a row with the running maximum and sum of
 // the softmax and a sorted list of the strip's best in registers, one or two entries a lane.  An
 // element is looked at one by one only if it beats the list's last entry, which becomes rare
-// after the first steps.  A second kernel joins the strips' lists, by beams, then over beams.
+// after the first steps; the first step takes the n-th largest of the lanes' maxima for a floor,
+// since n elements are at least that.  A second kernel joins the strips' lists, by beams, then over
+// beams.
 constexpr int kWarps = kThreads / 32;
 constexpr int kEmpty = INT_MIN;  // below the order of every float
 
@@ -26,21 +28,23 @@ __device__ __forceinline__ int order_of(float f) {
 }
 __device__ __forceinline__ float value_of(int o) { return __int_as_float(o >= 0 ? o : o ^ 0x7fffffff); }
 
-// The `n` best of what a warp has seen, sorted: entry 32 q + lane in (key[q], at[q]).
+// The `n` best of what a warp has seen, sorted by key and then by place: entry 32 q + lane in
+// (key[q], at[q]); the last one that counts in (last, last_at).
 template <int Q>
 struct Best {
-  int key[Q], at[Q], last, n;
+  int key[Q], at[Q], last, last_at, n;
   __device__ __forceinline__ void start(int count) {
 #pragma unroll
     for (int q = 0; q < Q; ++q) key[q] = kEmpty, at[q] = INT_MAX;
     n = count;
     last = kEmpty;
+    last_at = INT_MAX;
   }
-  // k > last, and behind all entries of the same key
+  __device__ __forceinline__ bool takes(int k, int place) const { return k > last || (k == last && place < last_at); }
   __device__ __forceinline__ void insert(int k, int place, int lane) {
     int pos = 0;
 #pragma unroll
-    for (int q = 0; q < Q; ++q) pos += __popc(__ballot_sync(~0u, key[q] >= k));
+    for (int q = 0; q < Q; ++q) pos += __popc(__ballot_sync(~0u, key[q] > k || (key[q] == k && at[q] < place)));
 #pragma unroll
     for (int q = Q - 1; q >= 0; --q) {
       int ku = __shfl_up_sync(~0u, key[q], 1), au = __shfl_up_sync(~0u, at[q], 1);
@@ -52,11 +56,35 @@ struct Best {
       if (i > pos) key[q] = ku, at[q] = au;
       else if (i == pos) key[q] = k, at[q] = place;
     }
-    int l = key[0];
+    int l = key[0], la = at[0];
 #pragma unroll
     for (int q = 1; q < Q; ++q)
-      if ((n - 1) / 32 == q) l = key[q];
-    last = __shfl_sync(~0u, l, (n - 1) & 31);
+      if ((n - 1) / 32 == q) l = key[q], la = at[q];
+    const int nl = __shfl_sync(~0u, l, (n - 1) & 31), na = __shfl_sync(~0u, la, (n - 1) & 31);
+    if (nl != kEmpty) last = nl, last_at = na;  // a floor stays until the list is full
+  }
+  // One entry of each lane that has one.
+  __device__ __forceinline__ void offer(int k, int place, bool has, int lane) {
+    unsigned todo = __ballot_sync(~0u, has && takes(k, place));
+    while (todo) {
+      const int from = __ffs(todo) - 1;
+      insert(__shfl_sync(~0u, k, from), __shfl_sync(~0u, place, from), lane);
+      todo &= todo - 1;
+      todo &= __ballot_sync(~0u, takes(k, place));
+    }
+  }
+  // Nothing below the n-th largest of the lanes' keys can be among the best; n <= 32.
+  __device__ __forceinline__ void floor_of(int k, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+      for (int step = size / 2; step > 0; step /= 2) {  // bitonic, descending
+        const int o = __shfl_xor_sync(~0u, k, step);
+        const bool low = (lane & step) == 0, down = (lane & size) == 0;
+        k = low == down ? max(k, o) : min(k, o);
+      }
+    k = __shfl_sync(~0u, k, n - 1);
+    if (k > last) last = k, last_at = INT_MAX;
   }
 };
 
@@ -85,7 +113,8 @@ struct Strip {
   Best<Q> best;
   Soft soft;
   int lane;
-  // E neighbouring elements of each lane from place `at` on, in the order of the lanes; `has` of them
+  bool fresh = true;
+  // E neighbouring elements of each lane from place `at` on; `has` of them
   template <int E>
   __device__ __forceinline__ void step(const float (&x)[E], int at, int has) {
     float top = x[0];
@@ -93,22 +122,22 @@ struct Strip {
     for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
     raise(soft, top);
     const float m = soft.m > -INFINITY ? soft.m : 0.f;
-    float s = 0.f;
+    float s[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += exp_of(x[e] - m);
-    add_to(soft, s);
-    unsigned todo = __ballot_sync(~0u, has > 0 && order_of(top) > best.last);
-    while (todo) {
-      const int from = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const int start = __shfl_sync(~0u, at, from), count = __shfl_sync(~0u, has, from);
+    for (int e = 0; e < E; ++e) s[e] = exp_of(x[e] - m);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int k = order_of(__shfl_sync(~0u, x[e], from));
-        if (e < count && k > best.last) best.insert(k, start + e, lane);
-      }
-      todo &= __ballot_sync(~0u, order_of(top) > best.last);
+    for (int w = E / 2; w > 0; w /= 2)
+#pragma unroll
+      for (int e = 0; e < w; ++e) s[e] += s[e + w];
+    add_to(soft, s[0]);
+    const int key = order_of(top);
+    if (Q == 1 && E > 1 && fresh) {
+      fresh = false;
+      best.floor_of(has > 0 ? key : kEmpty, lane);
     }
+    if (!__any_sync(~0u, has > 0 && key >= best.last)) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) best.offer(order_of(x[e]), at + e, e < has, lane);
   }
 };
 
@@ -138,18 +167,31 @@ __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectAr
     w.step(v, static_cast<int>(i + lane), lane < count ? 1 : 0);
     i += count;
   }
-  for (; i < stop; i += 32 * E) {
+  // whole steps, the next two on their way, then the rest
+  constexpr int STEP = 32 * E, AHEAD = 2;
+  const T* q = x + i + lane * E;
+  const int64_t whole = i < stop ? (stop - i) / STEP : 0;
+  Packet<T, E> next[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (k < whole) next[k] = ld_packet<T, E>(q + k * STEP);
+  for (int64_t n0 = 0; n0 < whole; n0 += AHEAD) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (n0 + k >= whole) break;
+      float v[E];
+      unpack<T, E>(next[k], v);
+      if (n0 + k + AHEAD < whole) next[k] = ld_packet<T, E>(q + (n0 + k + AHEAD) * STEP);
+      w.step(v, static_cast<int>(i + (n0 + k) * STEP + lane * E), E);
+    }
+  }
+  i += whole * STEP;
+  if (i < stop) {
     const int64_t at = i + lane * E;
     float v[E];
-    int has = 0;
-    if (at + E <= stop) {
-      unpack<T, E>(ld_packet<T, E>(x + at), v);
-      has = E;
-    } else {
+    const int has = at < stop ? static_cast<int>(stop - at < E ? stop - at : E) : 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = at + e < stop ? to_f32(x[at + e]) : -INFINITY;
-      has = at < stop ? static_cast<int>(stop - at) : 0;
-    }
+    for (int e = 0; e < E; ++e) v[e] = e < has ? to_f32(x[at + e]) : -INFINITY;
     w.step(v, static_cast<int>(at), has);
   }
 #pragma unroll
@@ -169,12 +211,11 @@ __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectAr
   if (lane == 0) softs[warp] = w.soft;
   __syncthreads();
   if (warp != 0) return;
-  // the other warps' lists behind this one's, each in its order until an entry does not fit
   for (int o = 1; o < kWarps; ++o) {
-    for (int e = 0; e < n; ++e) {
-      const int2 c = lists[o][e];
-      if (c.x <= w.best.last) break;
-      w.best.insert(c.x, c.y, lane);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int2 c = lists[o][q * 32 + lane];
+      w.best.offer(c.x, c.y, q * 32 + lane < n && c.x != kEmpty, lane);
     }
     Soft s = softs[o];
     const float m = fmaxf(w.soft.m, s.m);
@@ -216,13 +257,10 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(const BeamSelectArg
 #pragma unroll
     for (int bit = 1; bit < 32; bit *= 2) s += __shfl_xor_sync(~0u, s, bit);
     const double lse = m + log(s);
-    for (int64_t p = 0; p < a.parts; ++p) {
-      const int2* list = a.best + (first + p) * n;
-      for (int e = 0; e < n; ++e) {
-        const int2 c = list[e];
-        if (c.x <= best.last) break;
-        best.insert(c.x, c.y, lane);
-      }
+    const int64_t entries = a.parts * n;
+    for (int64_t e = lane; e - lane < entries; e += 32) {
+      const int2 c = e < entries ? a.best[first * n + e] : make_int2(kEmpty, INT_MAX);
+      best.offer(c.x, c.y, c.x != kEmpty, lane);
     }
     const float score = a.scores[b * a.scores_s0 + k * a.scores_s1];
     const bool ended = a.finished && a.finished[b * a.finished_s0 + k * a.finished_s1];
@@ -294,8 +332,11 @@ cudaError_t run_select(const BeamSelectArgs& a, cudaStream_t s) {
 // then writes it to every beam whose parent is another one, so the rows change in place.
 template <int BEAMS, typename U>
 __device__ __forceinline__ void move_column(const BeamReorderArgs& a, const BeamRows& t, int64_t column, const int* source, const int* target) {
-  const int64_t u0 = column % t.size0, rest = column / t.size0;
-  const int64_t at = u0 * t.step0 + rest % t.size1 * t.step1 + rest / t.size1 * t.step2;
+  int64_t at = column * t.step0;
+  if (t.size0 < t.columns) {
+    const int64_t rest = column / t.size0;
+    at += (rest % t.size1) * t.step1 + rest / t.size1 * t.step2 - rest * t.size0 * t.step0;
+  }
   U v[BEAMS];
 #pragma unroll
   for (int k = 0; k < BEAMS; ++k)
@@ -312,14 +353,15 @@ __global__ void __launch_bounds__(kThreads) beam_reorder_kernel(const __grid_con
   int n = 0;
   while (i >= a.batch * a.t[n].blocks) i -= a.batch * a.t[n++].blocks;
   const BeamRows& t = a.t[n];
-  const int64_t b = i / t.blocks, block = i % t.blocks;
+  const uint32_t b = static_cast<uint32_t>(i) / static_cast<uint32_t>(t.blocks);  // grids are below 2^31
+  const int64_t block = i - static_cast<int64_t>(b) * t.blocks;
   grid_dependency_wait();
   if (threadIdx.x < a.beams) {
-    const int64_t k = threadIdx.x, at = b * a.parents_s0 + k * a.parents_s1;
+    const int64_t k = threadIdx.x, at = static_cast<int64_t>(b) * a.parents_s0 + k * a.parents_s1;
     const int64_t parent = a.wide_parents ? static_cast<const int64_t*>(a.parents)[at] : static_cast<const int32_t*>(a.parents)[at];
-    int64_t from = -1, to = b * a.beams + k;
+    int64_t from = -1, to = static_cast<int64_t>(b) * a.beams + k;
     if (parent >= 0 && parent < a.beams && parent != k) {
-      from = b * a.beams + parent;
+      from = static_cast<int64_t>(b) * a.beams + parent;
       if (a.indices) {
         from = a.indices[from * a.indices_stride];
         to = a.indices[to * a.indices_stride];

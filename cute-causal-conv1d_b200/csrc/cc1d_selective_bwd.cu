@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
     const int64_t t0 = i * TT;
     const bool whole = inside(i), checked = packed || !whole;
     feed.store(a, p.b, t0, flags);
-    if (checked) __syncthreads();  // flags are there
+    if (checked || MULTI) __syncthreads();  // flags are there
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const float2 u = fadd2(pair_of<T>(next_delta[k], a.pairs), ROWS ? of_pair(biases, k) : bias), x = pair_of<T>(next_x[k], a.pairs);

@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
     const int64_t t0 = i * TT;
     const bool whole = inside(i), checked = packed || !whole;
     feed.store(a, p.b, t0, flags);
-    if (checked) __syncthreads();  // flags are there
+    if (checked || MULTI) __syncthreads();  // flags are there
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       x[k] = next_x[k];

@@ -22,14 +22,12 @@ __device__ __forceinline__ Four load_inputs(const TensorArg& t, int64_t group_st
   return Four{make_float2(f[0], f[1]), make_float2(f[2], f[3])};
 }
 
+// Channel d of batch row b.  Every thread of a warp comes here.
 template <typename T, int LANES, int VEC, bool PACKED>
-__global__ void __launch_bounds__(kThreads) sel_update_kernel(const SelUpdateArgs a) {
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / LANES;
-  const int sl = threadIdx.x % LANES;
-  grid_dependency_wait();
-  const bool mine = i < a.batch * a.dim;
-  const int64_t b = mine ? i / a.dim : 0, d = mine ? i - b * a.dim : 0, g = d / (a.dim / a.groups);
+__device__ __forceinline__ void update_row(const SelUpdateArgs& a, int64_t b, int64_t d, int sl) {
+  const bool mine = d < a.dim;
   const int64_t row = !mine ? -1 : a.indices ? a.indices[b * a.indices_stride] : b;
+  const int64_t g = a.groups == 1 ? 0 : static_cast<uint32_t>(d) / static_cast<uint32_t>(a.dim / a.groups);
   const bool live = row >= 0 && row < a.nstates;
   Four h[VEC], rate[VEC];
 #pragma unroll
@@ -87,6 +85,14 @@ __global__ void __launch_bounds__(kThreads) sel_update_kernel(const SelUpdateArg
   }
 }
 
+template <typename T, int LANES, int VEC, bool PACKED>
+__global__ void __launch_bounds__(kThreads) sel_update_kernel(const __grid_constant__ SelUpdateArgs a) {
+  const int sl = threadIdx.x % LANES;
+  const int64_t d = static_cast<int64_t>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
+  grid_dependency_wait();
+  for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) update_row<T, LANES, VEC, PACKED>(a, b, d, sl);
+}
+
 // Packets of four states are legal.
 bool packed(const SelUpdateArgs& a) {
   if (a.dstate % 4) return false;
@@ -103,8 +109,8 @@ bool packed(const SelUpdateArgs& a) {
 
 template <typename T, int LANES, int VEC>
 cudaError_t run(const SelUpdateArgs& a, cudaStream_t s) {
-  const int64_t threads = a.batch * a.dim * LANES;
-  const dim3 grid(static_cast<unsigned>((threads + kThreads - 1) / kThreads));
+  const int64_t per = kThreads / LANES;
+  const dim3 grid(static_cast<unsigned>((a.dim + per - 1) / per), static_cast<unsigned>(a.batch < 65535 ? a.batch : 65535));
   return packed(a) ? launch_dependent(sel_update_kernel<T, LANES, VEC, true>, grid, dim3(kThreads), 0, s, a)
                    : launch_dependent(sel_update_kernel<T, LANES, VEC, false>, grid, dim3(kThreads), 0, s, a);
 }
