@@ -73,6 +73,24 @@ struct Best {
       todo &= __ballot_sync(~0u, takes(k, place));
     }
   }
+  // The first entries, one of each lane (none: kEmpty): sorted by exchanges.
+  __device__ __forceinline__ void fill(int k, int place, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+      for (int step = size / 2; step > 0; step /= 2) {  // bitonic, the better ones first
+        const int ok = __shfl_xor_sync(~0u, k, step), op = __shfl_xor_sync(~0u, place, step);
+        const bool low = (lane & step) == 0, down = (lane & size) == 0;
+        const bool mine = k > ok || (k == ok && place < op), same = k == ok && place == op;
+        if (!same && mine != (low == down)) k = ok, place = op;
+      }
+    key[0] = k;
+    at[0] = place;
+    if (n <= 32) {
+      last = __shfl_sync(~0u, k, n - 1);
+      last_at = __shfl_sync(~0u, place, n - 1);
+    }
+  }
   // Nothing below the n-th largest of the lanes' keys can be among the best; n <= 32.
   __device__ __forceinline__ void floor_of(int k, int lane) {
 #pragma unroll
@@ -113,6 +131,7 @@ struct Strip {
   Best<Q> best;
   Soft soft;
   int lane;
+  int* floor;  // of the CTA: n elements of the row are at least that
   bool fresh = true;
   // E neighbouring elements of each lane from place `at` on; `has` of them
   template <int E>
@@ -135,9 +154,15 @@ struct Strip {
       fresh = false;
       best.floor_of(has > 0 ? key : kEmpty, lane);
     }
-    if (!__any_sync(~0u, has > 0 && key >= best.last)) return;
+    const int least = max(best.last, *static_cast<volatile int*>(floor));
+    if (!__any_sync(~0u, has > 0 && key >= least)) return;
+    const int before = best.last;
 #pragma unroll
-    for (int e = 0; e < E; ++e) best.offer(order_of(x[e]), at + e, e < has, lane);
+    for (int e = 0; e < E; ++e) {
+      const int k = order_of(x[e]);
+      best.offer(k, at + e, e < has && k >= least, lane);
+    }
+    if (lane == 0 && best.last != before) atomicMax(floor, best.last);
   }
 };
 
@@ -146,6 +171,9 @@ __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectAr
   constexpr int E = 16 / sizeof(T);
   __shared__ int2 lists[kWarps][Q * 32];
   __shared__ Soft softs[kWarps];
+  __shared__ int floor;
+  if (threadIdx.x == 0) floor = kEmpty;
+  __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int n = static_cast<int>(a.candidates);
@@ -157,6 +185,7 @@ __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectAr
   const int64_t stop = i + strip < end ? i + strip : end;
   Strip<T, Q> w;
   w.lane = lane;
+  w.floor = &floor;
   w.best.start(n);
   // up to the first 16-byte boundary, element by element
   const int64_t past = reinterpret_cast<uintptr_t>(x + i) % 16 / sizeof(T);
@@ -232,7 +261,7 @@ __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectAr
 }
 
 // One CTA for each request.  A warp joins a beam's parts and writes the beam's best with their
-// totals, in 64 bits, to shared memory; then the first warp takes the best head n times.
+// totals, in 64 bits, to shared memory; then every candidate finds its rank.
 template <int Q>
 __global__ void __launch_bounds__(kThreads) beam_join_kernel(const BeamSelectArgs a) {
   extern __shared__ double totals[];  // (beams, n), then the tokens
@@ -260,7 +289,8 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(const BeamSelectArg
     const int64_t entries = a.parts * n;
     for (int64_t e = lane; e - lane < entries; e += 32) {
       const int2 c = e < entries ? a.best[first * n + e] : make_int2(kEmpty, INT_MAX);
-      best.offer(c.x, c.y, c.x != kEmpty, lane);
+      if (e < 32) best.fill(c.x, c.y, lane);
+      else best.offer(c.x, c.y, c.x != kEmpty, lane);
     }
     const float score = a.scores[b * a.scores_s0 + k * a.scores_s1];
     const bool ended = a.finished && a.finished[b * a.finished_s0 + k * a.finished_s1];
@@ -284,32 +314,30 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(const BeamSelectArg
     }
   }
   __syncthreads();
-  if (warp != 0) return;
-  // lane l has the beams l and l + 32, and where it stands in their lists
-  int at[2] = {0, 0};
-  for (int c = 0; c < n; ++c) {
-    double top = 0.0;
-    int from = INT_MAX;  // none
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int k = q * 32 + lane;
-      if (k >= beams || at[q] >= n || tokens[k * n + at[q]] < 0) continue;
-      const double t = totals[k * n + at[q]];
-      if (from == INT_MAX || t > top) top = t, from = k;
+  // Each candidate's rank: how many of its own beam stand before it, and how many of each other
+  // beam are better, by bisection of that beam's descending totals.
+  for (int i = threadIdx.x; i < beams * n; i += kThreads) {
+    const int k = i / n, e = i - k * n;
+    if (tokens[i] < 0) continue;
+    const double t = totals[i];
+    int rank = e;
+    for (int o = 0; o < beams && rank < n; ++o) {
+      if (o == k) continue;
+      const double* list = totals + o * n;
+      const int* names = tokens + o * n;
+      int low = 0, high = n;  // entries before `low` are better, those from `high` on are not
+      while (low < high) {
+        const int m = (low + high) / 2;
+        const bool better = names[m] >= 0 && (list[m] > t || (list[m] == t && o < k));
+        if (better) low = m + 1;
+        else high = m;
+      }
+      rank += low;
     }
-#pragma unroll
-    for (int bit = 1; bit < 32; bit *= 2) {
-      const double t = __shfl_xor_sync(~0u, top, bit);
-      const int k = __shfl_xor_sync(~0u, from, bit);
-      if (k != INT_MAX && (from == INT_MAX || t > top || (t == top && k < from))) top = t, from = k;
-    }
-    const int place = __shfl_sync(~0u, from >= 32 ? at[1] : at[0], from & 31);
-    if (lane == 0) {
-      a.out_scores[b * n + c] = static_cast<float>(top);
-      a.parents[b * n + c] = from;
-      a.tokens[b * n + c] = tokens[from * n + place];
-    }
-    if (lane == (from & 31)) ++at[from >> 5];
+    if (rank >= n) continue;
+    a.out_scores[b * n + rank] = static_cast<float>(t);
+    a.parents[b * n + rank] = k;
+    a.tokens[b * n + rank] = tokens[i];
   }
 }
 

@@ -93,6 +93,87 @@ __global__ void __launch_bounds__(kThreads) sel_update_kernel(const __grid_const
   for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) update_row<T, LANES, VEC, PACKED>(a, b, d, sl);
 }
 
+// One token of rows whose states are packed: a thread takes its four states of a channel through
+// kRows batch rows, all of whose loads it makes first, and loads what the rows have in common once.
+// What a thread multiplies by its channel is below 2^32 (thin()).
+constexpr int kRows = 4;
+
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kThreads) sel_step_kernel(const __grid_constant__ SelUpdateArgs a) {
+  const int sl = threadIdx.x % LANES;
+  const uint32_t d = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  const int n0 = sl * 4;
+  const bool mine = d < a.dim && n0 < a.dstate;
+  grid_dependency_wait();
+  auto times = [&](int64_t stride) { return static_cast<int64_t>(static_cast<uint64_t>(d) * static_cast<uint32_t>(stride)); };
+  const uint32_t g = a.groups == 1 ? 0 : d / static_cast<uint32_t>(a.dim / a.groups);
+  const int64_t b0 = static_cast<int64_t>(blockIdx.y) * kRows;
+  int64_t row[kRows];
+  float4 h[kRows];
+  Packet<T, 4> B[kRows], C[kRows];
+  T x[kRows], delta[kRows], z[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    row[r] = -1;
+    if (mine && b0 + r < a.batch) row[r] = a.indices ? a.indices[(b0 + r) * a.indices_stride] : b0 + r;
+    if (row[r] >= a.nstates) row[r] = -1;
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    if (row[r] < 0) continue;
+    const int64_t b = b0 + r;
+    h[r] = *reinterpret_cast<const float4*>(static_cast<const float*>(a.state.data) + row[r] * a.state.s0 + times(a.state.s1) + n0);
+    x[r] = (static_cast<const T*>(a.x.data) + b * a.x.s0)[times(a.x.s1)];
+    delta[r] = (static_cast<const T*>(a.delta.data) + b * a.delta.s0)[times(a.delta.s1)];
+    if (a.z.data) z[r] = (static_cast<const T*>(a.z.data) + b * a.z.s0)[times(a.z.s1)];
+    B[r] = ld_packet<T, 4>(static_cast<const T*>(a.B.data) + b * a.B.s0 + g * a.B_group + n0);
+    C[r] = ld_packet<T, 4>(static_cast<const T*>(a.C.data) + b * a.C.s0 + g * a.C_group + n0);
+  }
+  Four rate = zero4();
+  float bias = 0.f, skip = 0.f;
+  if (mine) {
+    rate = of4(*reinterpret_cast<const float4*>(static_cast<const float*>(a.A.data) + times(a.A.s0) + n0));
+    rate.lo = fmul2(rate.lo, both(kLog2e));
+    rate.hi = fmul2(rate.hi, both(kLog2e));
+    if (a.bias.data) bias = load_any(a.bias.data, a.bias.dtype, d * a.bias.s0);
+    if (a.D.data) skip = load_any(a.D.data, a.D.dtype, d * a.D.s0);
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    if (b0 + r >= a.batch) return;  // every thread of the CTA
+    float y = 0.f;
+    if (row[r] >= 0) {
+      float2 s = both(to_f32(delta[r]) + bias);
+      if (a.softplus) s = step_size<T>(s);
+      const float2 sx = fmul2(s, both(to_f32(x[r])));
+      float vb[4], vc[4];
+      unpack<T, 4>(B[r], vb);
+      unpack<T, 4>(C[r], vc);
+      Four f = of4(h[r]);
+      f.lo = ffma2(decays(s, rate.lo), f.lo, fmul2(make_float2(vb[0], vb[1]), sx));
+      f.hi = ffma2(decays(s, rate.hi), f.hi, fmul2(make_float2(vb[2], vb[3]), sx));
+      *reinterpret_cast<float4*>(static_cast<float*>(a.state.data) + row[r] * a.state.s0 + times(a.state.s1) + n0) = to4(f);
+      const float2 sum = ffma2(make_float2(vc[2], vc[3]), f.hi, fmul2(make_float2(vc[0], vc[1]), f.lo));
+      y = sum.x + sum.y;
+    }
+#pragma unroll
+    for (int bit = 1; bit < LANES; bit *= 2) y += __shfl_xor_sync(~0u, y, bit);
+    if (sl != 0 || !mine) continue;
+    if (row[r] >= 0) {
+      y = fmaf(skip, to_f32(x[r]), y);
+      if (a.z.data) y *= silu_of<T>(to_f32(z[r]));
+    }
+    (static_cast<T*>(a.out.data) + (b0 + r) * a.out.s0)[times(a.out.s1)] = from_f32<T>(row[r] < 0 ? 0.f : y);
+  }
+}
+
+// Strides between channels that 32 bits hold.
+bool thin(const SelUpdateArgs& a) {
+  for (int64_t s : {a.x.s1, a.delta.s1, a.z.s1, a.out.s1, a.state.s1, a.A.s0})
+    if (s < 0 || s >= int64_t{1} << 32) return false;
+  return true;
+}
+
 // Packets of four states are legal.
 bool packed(const SelUpdateArgs& a) {
   if (a.dstate % 4) return false;
@@ -111,6 +192,9 @@ template <typename T, int LANES, int VEC>
 cudaError_t run(const SelUpdateArgs& a, cudaStream_t s) {
   const int64_t per = kThreads / LANES;
   const dim3 grid(static_cast<unsigned>((a.dim + per - 1) / per), static_cast<unsigned>(a.batch < 65535 ? a.batch : 65535));
+  if constexpr (VEC == 1)
+    if (a.seqlen == 1 && packed(a) && thin(a) && a.batch <= 65535 * kRows)
+      return launch_dependent(sel_step_kernel<T, LANES>, dim3(grid.x, static_cast<unsigned>((a.batch + kRows - 1) / kRows)), dim3(kThreads), 0, s, a);
   return packed(a) ? launch_dependent(sel_update_kernel<T, LANES, VEC, true>, grid, dim3(kThreads), 0, s, a)
                    : launch_dependent(sel_update_kernel<T, LANES, VEC, false>, grid, dim3(kThreads), 0, s, a);
 }

@@ -191,6 +191,33 @@ def test_update_pool(index_dtype, groups):
     assert torch.equal(pool[others], before[others])
 
 
+@pytest.mark.parametrize("N", [4, 8, 12, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_update_packed(dtype, N):
+    """States, B and C on 16 bytes, which move four at a time; batches that do not fill the last rows."""
+    for batch, groups, z, pool in ((1, 0, True, False), (3, 0, False, True), (4, 2, True, True), (9, 0, True, False), (6, 1, True, True)):
+        t = _inputs(N + batch, batch, 38, 1, N, dtype, "contiguous", groups, z, nstates=batch)
+        state = torch.randn(batch + 5, 38, N, generator=_gen(3), device="cuda") if pool else t["init"].clone()
+        index = torch.randperm(batch + 5, generator=_gen(4), device="cuda")[:batch] if pool else None
+        if pool:
+            index[batch // 2] = -1
+            t["init"] = state[index.clamp(min=0)]
+        before = state.clone()
+        one = {k: (v[..., 0].contiguous() if k in ("x", "delta", "B", "C", "z") and v is not None else v) for k, v in t.items()}
+        out = selective_recurrence_update(*(one[k] if k != "state" else state for k in ("x", "state", "delta", "A", "B", "C", "D", "z", "bias")),
+                                          state_indices=index)
+        t["dout"] = None
+        e = S.statement(S.fp64(t))
+        rows = list(range(batch)) if index is None else [k for k in range(batch) if k != batch // 2]
+        S.check(out[rows], tuple(v[rows, :, 0] for v in e["out"]), "out")
+        at = rows if index is None else index[rows].tolist()
+        S.check(state[at], tuple(v[rows] for v in e["final"]), "state")
+        if pool:
+            assert (out[batch // 2] == 0).all()
+            others = [i for i in range(batch + 5) if i not in at]
+            assert torch.equal(state[others], before[others])
+
+
 def test_update_continues_prefill():
     """The steps after a prefill give what one longer pass gives."""
     t = _inputs(3, 2, 70, 60, 16, torch.float32)
