@@ -15,8 +15,8 @@ namespace {
 // One pass over the logits: each warp walks a strip of a row with the running maximum and sum of
 // the softmax and a sorted list of the strip's best in registers, one or two entries a lane.  An
 // element is looked at one by one only if it beats the list's last entry, which becomes rare
-// after the first steps; the first step takes the n-th largest of the lanes' maxima for a floor,
-// since n elements are at least that.  A second kernel joins the strips' lists, by beams, then over
+// after the first steps; a floor from all warps of a CTA (the n-th largest of their elements' maxima,
+// later of their lists) keeps out most of the others.  A second kernel joins the strips' lists, by beams, then over
 // beams.
 constexpr int kWarps = kThreads / 32;
 constexpr int kEmpty = INT_MIN;  // below the order of every float
@@ -91,29 +91,18 @@ struct Best {
       last_at = __shfl_sync(~0u, place, n - 1);
     }
   }
-  // Nothing below the n-th largest of the lanes' keys can be among the best; n <= 32.
-  __device__ __forceinline__ void floor_of(int k, int lane) {
-#pragma unroll
-    for (int size = 2; size <= 32; size *= 2)
-#pragma unroll
-      for (int step = size / 2; step > 0; step /= 2) {  // bitonic, descending
-        const int o = __shfl_xor_sync(~0u, k, step);
-        const bool low = (lane & step) == 0, down = (lane & size) == 0;
-        k = low == down ? max(k, o) : min(k, o);
-      }
-    k = __shfl_sync(~0u, k, n - 1);
-    if (k > last) last = k, last_at = INT_MAX;
-  }
 };
 
-// The running maximum m and sum s + low of exp(x - m) of a lane or a part of a row.
+// The running maximum m and sum s + low of 2^(x L - c), L = kLog2e, of a lane or a part of a row.
+// c = m L as it is rounded (0 before there is an m): one multiply-add makes the exponent, and
+// log sum exp(x) = m + log(sum) + (c - m L) log(2) puts the rounding back.
 struct Soft {
   float m = -INFINITY, s = 0.f, low = 0.f;
 };
-__device__ __forceinline__ float exp_of(float d) { return ex2_approx(d * kLog2e); }
+__device__ __forceinline__ float scale_of(float m) { return m > -INFINITY ? m * kLog2e : 0.f; }
 __device__ __forceinline__ void raise(Soft& a, float m) {
   if (m > a.m) {
-    const float f = a.m > -INFINITY ? exp_of(a.m - m) : 0.f;
+    const float f = a.m > -INFINITY ? ex2_approx(scale_of(a.m) - scale_of(m)) : 0.f;
     a.s *= f;
     a.low *= f;
     a.m = m;
@@ -131,8 +120,7 @@ struct Strip {
   Best<Q> best;
   Soft soft;
   int lane;
-  int* floor;  // of the CTA: n elements of the row are at least that
-  bool fresh = true;
+  int floor = kEmpty;  // n elements of the CTA's part are at least that
   // E neighbouring elements of each lane from place `at` on; `has` of them
   template <int E>
   __device__ __forceinline__ void step(const float (&x)[E], int at, int has) {
@@ -140,40 +128,66 @@ struct Strip {
 #pragma unroll
     for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
     raise(soft, top);
-    const float m = soft.m > -INFINITY ? soft.m : 0.f;
+    const float c = scale_of(soft.m);
     float s[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) s[e] = exp_of(x[e] - m);
+    for (int e = 0; e < E; ++e) s[e] = ex2_approx(fmaf(x[e], kLog2e, -c));
 #pragma unroll
     for (int w = E / 2; w > 0; w /= 2)
 #pragma unroll
       for (int e = 0; e < w; ++e) s[e] += s[e + w];
     add_to(soft, s[0]);
     const int key = order_of(top);
-    if (Q == 1 && E > 1 && fresh) {
-      fresh = false;
-      best.floor_of(has > 0 ? key : kEmpty, lane);
-    }
-    const int least = max(best.last, *static_cast<volatile int*>(floor));
+    const int least = max(best.last, floor);
     if (!__any_sync(~0u, has > 0 && key >= least)) return;
-    const int before = best.last;
+    // the lanes' elements that may count, one after the other
+    unsigned mine = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int k = order_of(x[e]);
-      best.offer(k, at + e, e < has && k >= least, lane);
+    for (int e = 0; e < E; ++e) mine |= (e < has && order_of(x[e]) >= least ? 1u : 0u) << e;
+    while (true) {
+      const unsigned todo = __ballot_sync(~0u, mine != 0);
+      if (!todo) break;
+      const int from = __ffs(todo) - 1, first = __ffs(mine) - 1;
+      float v = x[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) v = e == first ? x[e] : v;
+      const int k = __shfl_sync(~0u, order_of(v), from), place = __shfl_sync(~0u, at + first, from);
+      if (best.takes(k, place)) best.insert(k, place, lane);
+      if (lane == from) mine &= mine - 1;
     }
-    if (lane == 0 && best.last != before) atomicMax(floor, best.last);
   }
 };
+
+// One step of a bitonic network on the lanes' keys: lanes `step` apart, the larger first where `down`.
+__device__ __forceinline__ int exchange(int k, int step, bool down, int lane) {
+  const int o = __shfl_xor_sync(~0u, k, step);
+  return ((lane & step) == 0) == down ? max(k, o) : min(k, o);
+}
+__device__ __forceinline__ int sorted_down(int k, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int step = size / 2; step > 0; step /= 2) k = exchange(k, step, (lane & size) == 0, lane);
+  return k;
+}
+// The n-th largest (n <= 32) of kWarps descending lists of 32 keys in shared memory.  Of two
+// descending lists a and b the larger of a[i] and b[31 - i] are the 32 largest, in a bitonic order.
+__device__ __forceinline__ int nth_of_lists(const int* keys, int n, int lane) {
+  int k = keys[lane];
+  for (int w = 1; w < kWarps; ++w) {
+    k = max(k, keys[w * 32 + 31 - lane]);
+#pragma unroll
+    for (int step = 16; step > 0; step /= 2) k = exchange(k, step, true, lane);
+  }
+  return __shfl_sync(~0u, k, n - 1);
+}
 
 template <typename T, int Q>
 __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectArgs a) {
   constexpr int E = 16 / sizeof(T);
   __shared__ int2 lists[kWarps][Q * 32];
   __shared__ Soft softs[kWarps];
-  __shared__ int floor;
-  if (threadIdx.x == 0) floor = kEmpty;
-  __syncthreads();
+  __shared__ int keys[2][kThreads];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int n = static_cast<int>(a.candidates);
@@ -185,7 +199,6 @@ __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectAr
   const int64_t stop = i + strip < end ? i + strip : end;
   Strip<T, Q> w;
   w.lane = lane;
-  w.floor = &floor;
   w.best.start(n);
   // up to the first 16-byte boundary, element by element
   const int64_t past = reinterpret_cast<uintptr_t>(x + i) % 16 / sizeof(T);
@@ -196,33 +209,65 @@ __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectAr
     w.step(v, static_cast<int>(i + lane), lane < count ? 1 : 0);
     i += count;
   }
-  // whole steps, the next two on their way, then the rest
+  // steps of 32 E elements, the next two on their way; the last one may be short
   constexpr int STEP = 32 * E, AHEAD = 2;
-  const T* q = x + i + lane * E;
-  const int64_t whole = i < stop ? (stop - i) / STEP : 0;
-  Packet<T, E> next[AHEAD];
+  const int size = i < stop ? static_cast<int>(stop - i) : 0, from = lane * E, steps = (size + STEP - 1) / STEP;
+  const T* q = x + i;
+  // Kept as words until they are used: taking them apart at once would wait for the load.
+  uint4 next[AHEAD];
+  auto fetch = [&](int n) {
+    const int at = from + n * STEP;
+    return at + E <= size ? *reinterpret_cast<const uint4*>(q + at) : make_uint4(0, 0, 0, 0);
+  };
+  auto count = [&](int n) { return min(max(size - from - n * STEP, 0), E); };
+  auto values = [&](int n, const uint4& u, float (&v)[E]) {
+    unpack<T, E>(*reinterpret_cast<const Packet<T, E>*>(&u), v);
+    if ((n + 1) * STEP > size) {
+      const int at = from + n * STEP;
+      if (at + E > size)
 #pragma unroll
-  for (int k = 0; k < AHEAD; ++k)
-    if (k < whole) next[k] = ld_packet<T, E>(q + k * STEP);
-  for (int64_t n0 = 0; n0 < whole; n0 += AHEAD) {
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      if (n0 + k >= whole) break;
-      float v[E];
-      unpack<T, E>(next[k], v);
-      if (n0 + k + AHEAD < whole) next[k] = ld_packet<T, E>(q + (n0 + k + AHEAD) * STEP);
-      w.step(v, static_cast<int>(i + (n0 + k) * STEP + lane * E), E);
+        for (int e = 0; e < E; ++e) v[e] = at + e < size ? to_f32(q[at + e]) : -INFINITY;
     }
-  }
-  i += whole * STEP;
-  if (i < stop) {
-    const int64_t at = i + lane * E;
-    float v[E];
-    const int has = at < stop ? static_cast<int>(stop - at < E ? stop - at : E) : 0;
+  };
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = e < has ? to_f32(x[at + e]) : -INFINITY;
-    w.step(v, static_cast<int>(at), has);
+  for (int k = 0; k < AHEAD; ++k) next[k] = fetch(k);
+  auto run = [&](int first, int end) {  // first: a multiple of AHEAD
+    for (int n0 = first; n0 < end; n0 += AHEAD) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (n0 + k >= end) break;
+        float v[E];
+        values(n0 + k, next[k], v);
+        next[k] = fetch(n0 + k + AHEAD);
+        w.step(v, static_cast<int>(i) + from + (n0 + k) * STEP, count(n0 + k));
+      }
+    }
+  };
+  // A floor before the first step: the n-th largest of the threads' maxima of it.  For long strips
+  // another one after eight steps: the n-th largest of the warps' lists.
+  constexpr int FIRST = 8;
+  if constexpr (Q == 1) {
+    int top = kEmpty;
+    if (count(0) > 0) {
+      float v[E];
+      values(0, next[0], v);
+      float m = v[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) m = fmaxf(m, v[e]);
+      top = order_of(m);
+    }
+    keys[0][threadIdx.x] = sorted_down(top, lane);
+    __syncthreads();
+    w.floor = nth_of_lists(keys[0], n, lane);
   }
+  run(0, steps < FIRST ? steps : FIRST);
+  if constexpr (Q == 1)
+    if (strip >= 2 * FIRST * STEP) {  // the same for all warps
+      keys[1][threadIdx.x] = lane < n ? w.best.key[0] : kEmpty;
+      __syncthreads();
+      w.floor = max(w.floor, nth_of_lists(keys[1], n, lane));
+    }
+  run(FIRST, steps);
 #pragma unroll
   for (int q = 0; q < Q; ++q) lists[warp][q * 32 + lane] = make_int2(w.best.key[q], w.best.at[q]);
 #pragma unroll
@@ -281,11 +326,11 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(const BeamSelectArg
     double s = 0.0;
     for (int64_t p = lane; p < a.parts; p += 32) {
       const float2 v = a.sums[first + p];
-      s += static_cast<double>(v.y) * (v.x > -INFINITY ? exp(static_cast<double>(v.x) - m) : 1.0);
+      s += static_cast<double>(v.y) * exp2(static_cast<double>(scale_of(v.x)) - scale_of(m));
     }
 #pragma unroll
     for (int bit = 1; bit < 32; bit *= 2) s += __shfl_xor_sync(~0u, s, bit);
-    const double lse = m + log(s);
+    const double lse = m + log(s) + (scale_of(m) - static_cast<double>(m) * kLog2e) * 0.69314718055994531;
     const int64_t entries = a.parts * n;
     for (int64_t e = lane; e - lane < entries; e += 32) {
       const int2 c = e < entries ? a.best[first * n + e] : make_int2(kEmpty, INT_MAX);
