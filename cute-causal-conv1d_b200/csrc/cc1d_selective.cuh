@@ -85,7 +85,7 @@ __device__ __forceinline__ SelPlace sel_place(const SelArgs& a) {
 // pair c + k DC.  NT: threads of the CTA.
 template <int NT, int LN, bool ROWS>
 struct Tile {
-  static constexpr int T = 8 * LN, PAIRS = kSelChannels / 2 / LN, K = T * PAIRS / NT;
+  static constexpr int T = sel_tile(LN), PAIRS = kSelChannels / 2 / LN, K = T * PAIRS / NT;
   static constexpr int DT = ROWS ? 0 : NT / PAIRS, DC = ROWS ? NT / T : 0;
   static __device__ __forceinline__ int t() { return ROWS ? threadIdx.x % T : threadIdx.x / PAIRS; }
   static __device__ __forceinline__ int c() { return ROWS ? threadIdx.x / T : threadIdx.x % PAIRS; }
@@ -213,17 +213,19 @@ struct Walk {
 // for a single pass are loaded a tile ahead.
 template <typename T, int NT, int LN, bool MULTI>
 struct Coefficients {
-  static constexpr int TT = 8 * LN, ALL = TT * 8 * LN, HELD = MULTI || ALL < NT ? 1 : ALL / NT;
-  static constexpr int DT = NT / (8 * LN), DN = NT / TT, HALF = HELD > 1 ? HELD / 2 : 1;
+  static constexpr int TT = sel_tile(LN), WIDE = 8 * LN, ALL = TT * WIDE, HELD = MULTI || ALL < NT ? 1 : ALL / NT;
+  // positions, or states, between two elements of a thread; half the elements are B's
+  static constexpr int DT = WIDE <= NT ? NT / WIDE : 1, DN = NT / TT, HALF = HELD > 1 ? HELD / 2 : 1;
+  static_assert(WIDE <= 2 * NT, "a thread has one place of B and C, or one of each");
   T v[HELD];
-  const T *p, *pc;  // along the states: the thread's tensor; else B and C
+  const T *p, *pc;  // along the states: the thread's tensor, or B; else B and C
   int n, t;
   bool along, is_c;
   __device__ __forceinline__ Coefficients(const SelArgs& a, const SelPlace& at) {
     along = a.B.s1 == 1 || a.B.s2 != 1;
     const int e = threadIdx.x;
     int s;
-    if (along) t = e / (8 * LN), s = e % (8 * LN);
+    if (along) t = e / WIDE, s = e % WIDE;
     else t = e % TT, s = e / TT;
     is_c = s >= 4 * LN;
     n = is_c ? s - 4 * LN : s;
@@ -232,27 +234,40 @@ struct Coefficients {
     p = is_c ? c + n * a.C.s1 + t * a.C.s2 : b + n * a.B.s1 + t * a.B.s2;
     pc = c + n * a.C.s1 + t * a.C.s2;
   }
+  // Element k's position in the tile, and whether it is C's.
+  __device__ __forceinline__ int position(int k) const { return !along ? t : WIDE <= NT ? t + k * DT : k / 2; }
+  __device__ __forceinline__ bool of_c(int k) const { return along ? (WIDE <= NT ? is_c : k % 2 != 0) : k >= HALF || is_c; }
   __device__ __forceinline__ void load(const SelArgs& a, int64_t t0, bool whole) {
     if constexpr (MULTI) return;
     if (ALL < NT && threadIdx.x >= ALL) return;
     if (along) {
-      const int64_t s2 = is_c ? a.C.s2 : a.B.s2;
-      const T* q = p + t0 * s2;
       if (n >= a.dstate) {
 #pragma unroll
         for (int k = 0; k < HELD; ++k) v[k] = from_f32<T>(0.f);
-      } else if (whole) {
-#pragma unroll
-        for (int k = 0; k < HELD; ++k, q += DT * s2) v[k] = *q;
-      } else {
-#pragma unroll
-        for (int k = 0; k < HELD; ++k, q += DT * s2) v[k] = t0 + t + k * DT < a.seqlen ? *q : from_f32<T>(0.f);
+        return;
       }
+      const int64_t step = is_c ? a.C.s2 : a.B.s2;
+      const T* q = p + t0 * step;
+      const T* qc = pc + t0 * a.C.s2;
+      auto each = [&](auto in) {
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) {
+          if (WIDE > NT && k % 2) {
+            v[k] = in(k) ? *qc : from_f32<T>(0.f);
+            qc += a.C.s2;
+          } else {
+            v[k] = in(k) ? *q : from_f32<T>(0.f);
+            q += DT * step;
+          }
+        }
+      };
+      if (whole) each([](int) { return true; });
+      else each([&](int k) { return t0 + (WIDE <= NT ? t + k * DT : k / 2) < a.seqlen; });
     } else {
       const bool in = t0 + t < a.seqlen;
 #pragma unroll
       for (int k = 0; k < HELD; ++k) {
-        const bool c = k >= HALF || is_c;
+        const bool c = of_c(k);
         const T* q = (k >= HALF ? pc : p) + t0 * (c ? a.C.s2 : a.B.s2) + k % HALF * DN * (c ? a.C.s1 : a.B.s1);
         v[k] = in && n + k % HALF * DN < a.dstate ? *q : from_f32<T>(0.f);
       }
@@ -274,12 +289,17 @@ struct Coefficients {
       }
     } else {
       if (ALL < NT && threadIdx.x >= ALL) return;
-      float* o = bc + (t * 2 + is_c) * 4 * LN + n;
+      auto each = [&](auto valid) {
+        float* o = bc + (t * 2 + is_c) * 4 * LN + n;
 #pragma unroll
-      for (int k = 0; k < HELD; ++k) {
-        const int at_k = along ? k * DT * 8 * LN : (k >= HALF) * 4 * LN + k % HALF * DN;
-        o[at_k] = checked && !f.valid(along ? t + k * DT : t) ? 0.f : to_f32(v[k]);
-      }
+        for (int k = 0; k < HELD; ++k) {
+          // from the thread's first element on
+          const int at_k = !along ? (k >= HALF) * 4 * LN + k % HALF * DN : WIDE <= NT ? k * DT * 8 * LN : k * 4 * LN;
+          o[at_k] = valid(position(k)) ? to_f32(v[k]) : 0.f;
+        }
+      };
+      if (checked) each([&](int at_t) { return f.valid(at_t); });
+      else each([](int) { return true; });
     }
   }
 };
@@ -415,10 +435,10 @@ __device__ __forceinline__ Eight handed_over(const SelArgs& a, int64_t b, int64_
 }
 
 // The sums over the LN threads of a channel of four positions' values; afterwards thread sl has
-// those of positions sl * 4 / LN on, in v[0 .. 4 / LN).
+// those of positions sl * 4 / LN on, in v[0 .. 4 / LN), or with LN >= 4 that of position sl % 4.
 template <int LN>
 __device__ __forceinline__ void sum_lanes(float (&v)[4], int sl) {
-  if constexpr (LN == 4) {
+  if constexpr (LN >= 4) {
     const bool hi = sl & 2;
     const float s0 = hi ? v[0] : v[2], s1 = hi ? v[1] : v[3];
     v[0] = (hi ? v[2] : v[0]) + __shfl_xor_sync(~0u, s0, 2);
@@ -426,6 +446,8 @@ __device__ __forceinline__ void sum_lanes(float (&v)[4], int sl) {
     const bool odd = sl & 1;
     const float s = odd ? v[0] : v[1];
     v[0] = (odd ? v[1] : v[0]) + __shfl_xor_sync(~0u, s, 1);
+#pragma unroll
+    for (int bit = 4; bit < LN; bit *= 2) v[0] += __shfl_xor_sync(~0u, v[0], bit);
   } else if constexpr (LN == 2) {
     const bool hi = sl & 1;
     const float s0 = hi ? v[0] : v[2], s1 = hi ? v[1] : v[3];
@@ -433,5 +455,10 @@ __device__ __forceinline__ void sum_lanes(float (&v)[4], int sl) {
     v[1] = (hi ? v[3] : v[1]) + __shfl_xor_sync(~0u, s1, 1);
   }
 }
+// Of four positions those that a thread has then, and the first of them; whether it stores them.
+template <int LN>
+constexpr int kSums = LN >= 4 ? 1 : 4 / LN;
+template <int LN>
+__device__ __forceinline__ int first_sum(int sl) { return LN >= 4 ? sl & 3 : sl * kSums<LN>; }
 
 }  // namespace cc1d

@@ -155,8 +155,8 @@ int64_t choose_segments(const SelArgs& a, bool bwd) {
 // threads go through a tile.
 cc1d_status plan(SelArgs* a, bool bwd) {
   a->padded = (a->dstate + 3) / 4 * 4;
-  a->lanes = a->padded <= 4 ? 1 : a->padded <= 8 ? 2 : 4;
-  a->blocks = static_cast<int>((a->dstate + kSelBlock - 1) / kSelBlock);
+  for (a->lanes = 1; a->lanes < kSelLanes && a->lanes * kSelStates < a->dstate;) a->lanes *= 2;
+  a->blocks = static_cast<int>((a->dstate + a->lanes * kSelStates - 1) / (a->lanes * kSelStates));
   const int64_t chunk = CC1D_SELECTIVE_CHUNK(a->dstate);
   a->nchunks = (a->seqlen + chunk - 1) / chunk;
   a->gdim = a->dim / a->groups;

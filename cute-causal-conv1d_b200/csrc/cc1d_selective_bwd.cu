@@ -31,13 +31,13 @@ constexpr int kBwdCtas = BWDC;
 // position and pair.
 template <int LN>
 struct BwdSmem {
-  static constexpr int T = 8 * LN, PAIRS = kSelThreads / LN, PITCH = PAIRS + 1;
+  static constexpr int T = sel_tile(LN), PAIRS = kSelThreads / LN, PITCH = PAIRS + 1;
   static constexpr int kFlags = 256, kIo = T * PITCH * 16, kDz = (T * PITCH * 8 + 15) / 16 * 16, kSub = T / 4 * kSelThreads * 32;
   static constexpr int kSlab = T * 8 * LN * 4;  // one warp's
-  static constexpr int kSums = T * PITCH * 24;
+  static constexpr int kThree = T * PITCH * 24;
   static int64_t bytes(const SelArgs& a) {
     return kFlags + 2 * kIo + kDz + kSub + kWarps * kSlab + T * 8 * LN * a.blocks * 4 + 3ll * a.blocks * kSelThreads * 32 +
-           (a.blocks > 1 ? kSums : 0);
+           (a.blocks > 1 ? kThree : 0);
   }
 };
 
@@ -53,12 +53,14 @@ __device__ __forceinline__ void add_to(float2& hi, float2& lo, float2 v) {
   add_to(hi.y, lo.y, v.y);
 }
 
-// The sums of eight values over the channels of a warp.  A lane ends with one of them, the number
-// of which summed() tells; lanes that differ in further bits hold the same one.
+// The sums of eight values over the channels of a warp.  A lane ends with kLeft<LN> of them, the
+// first of which summed() tells; lanes that differ in further bits hold the same ones.
 template <int LN>
-__device__ __forceinline__ float sum_channels(float (&v)[8], int lane) {
+constexpr int kLeft = LN >= 4 ? LN / 4 : 1;
+template <int LN>
+__device__ __forceinline__ void sum_channels(float (&v)[8], int lane) {
 #pragma unroll
-  for (int half = 4; half >= 1; half /= 2) {
+  for (int half = 4; half >= kLeft<LN>; half /= 2) {
     const int bit = 4 * half;
     const bool hi = lane & bit;
 #pragma unroll
@@ -69,9 +71,11 @@ __device__ __forceinline__ float sum_channels(float (&v)[8], int lane) {
   }
 #pragma unroll
   for (int bit = 2; bit >= LN; bit /= 2) v[0] += __shfl_xor_sync(~0u, v[0], bit);
-  return v[0];
 }
-__device__ __forceinline__ int summed(int lane) { return (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1); }
+template <int LN>
+__device__ __forceinline__ int summed(int lane) {
+  return (lane >> 4 & 1) * 4 + (LN <= 8 ? (lane >> 3 & 1) * 2 : 0) + (LN <= 4 ? lane >> 2 & 1 : 0);
+}
 
 // ENDS: only the gradient that each segment hands to the one before it.
 template <typename T, int LN, bool ROWS, bool MULTI, bool ENDS>
@@ -112,7 +116,7 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
   float2 dbias = both(0.f), dbias_low = both(0.f), dskip = both(0.f), dskip_low = both(0.f);
   float2 total = both(0.f);
   for (int nb = 0; nb < blocks; ++nb) {
-    const int n0 = nb * kSelBlock + sl * kSelStates, n = n0 < np ? mine : 0;
+    const int n0 = nb * 4 * LN + sl * kSelStates, n = n0 < np ? mine : 0;
     rate = load_rates(a, ch, n0, n);
     carry = ENDS ? zero8() : handed_over(a, p.b, a.segments - 1, p.seg, -1, ch, n0, n, rate);
     if constexpr (MULTI) put8(held + nb * 6 * kHalf, kHalf, carry);
@@ -121,7 +125,7 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
   }
 
   // where this lane's sums over channels of the first position go
-  const int which = summed(lane);
+  const int which = summed<LN>(lane);
   float* slab = slabs + warp * (Smem::kSlab / 4) + (which >> 2) * 4 * LN + sl * 4 + (which & 3);
   const Walk<T, Where> xs(a.x, p), deltas(a.delta, p), zs(a.z.data ? a.z : a.x, p), douts(a.dout, p);
   const Walk<T, Where> dxs(a.dx, p), ddeltas(a.ddelta, p), dzs(a.z.data ? a.dz : a.dx, p);
@@ -176,7 +180,7 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
     __syncthreads();
 
     for (int nb = 0; nb < blocks; ++nb) {
-      const int n0 = nb * kSelBlock + sl * kSelStates, n = n0 < np ? mine : 0;
+      const int n0 = nb * 4 * LN + sl * kSelStates, n = n0 < np ? mine : 0;
       if constexpr (MULTI) {
         carry = take8(held + nb * 6 * kHalf, kHalf);
         rate = load_rates(a, ch, n0, n);
@@ -221,8 +225,10 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = b[e].x + b[e].y;
-        const float r = sum_channels<LN>(v, lane);
-        if ((lane & 3) < LN) slab[t * 8 * LN] = r;
+        sum_channels<LN>(v, lane);
+#pragma unroll
+        for (int e = 0; e < kLeft<LN>; ++e)
+          if ((lane & 3) < LN) slab[t * 8 * LN + e] = v[e];
       };
       // One position, from the gradient carried to it: h before it in `kept` times its decay.
       // y, sa, sb: the thread's parts of the sums over the states of C h, g a h_{t-1} A and g B.
@@ -342,8 +348,9 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
 #pragma unroll
           for (int e = 0; e < 6; ++e) sum_lanes<LN>(l[e / 2][e % 2], sl);
 #pragma unroll
-          for (int j = 0; j < 4 / LN; ++j) {
-            const int t = q * 4 + sl * (4 / LN) + j;
+          for (int j = 0; j < kSums<LN>; ++j) {
+            if (sl >= 4) break;
+            const int t = q * 4 + first_sum<LN>(sl) + j;
             float2 yt = make_float2(l[0][0][j], l[0][1][j]), sat = make_float2(l[1][0][j], l[1][1][j]), sbt = make_float2(l[2][0][j], l[2][1][j]);
             if constexpr (MULTI) {
               float2* s = sums + (t * PITCH + c) * 3;
@@ -374,15 +381,17 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
         put8(held + (nb * 6 + 2) * kHalf, kHalf, hi);
         put8(held + (nb * 6 + 4) * kHalf, kHalf, lo);
         __syncthreads();
-        // this pass's states of dB and dC: the warps' sums to the CTA's, one value of every
-        // kSelThreads / (8 LN)-th position for each thread
-        constexpr int STEP = kSelThreads / (8 * LN);
-        const int v = tid % (8 * LN), m = nb * kSelBlock + v % (4 * LN), first = tid / (8 * LN);
-        if (m < np) {
+        // this pass's states of dB and dC: the warps' sums to the CTA's.  A thread has the same values
+        // of every STEP-th position, one or two of them.
+        constexpr int STEP = 8 * LN < kSelThreads ? kSelThreads / (8 * LN) : 1;
+        const int count = static_cast<int>(a.seqlen - t0 < TT ? a.seqlen - t0 : TT);
+#pragma unroll
+        for (int more = 0; more < 8 * LN; more += kSelThreads) {
+          const int v = tid % (8 * LN) + more, m = nb * 4 * LN + v % (4 * LN), first = tid / (8 * LN);
+          if (m >= np) continue;
           const float* from = slabs + first * 8 * LN + v;
           const int64_t row_size = a.tiles * 2 * np;
           float* to = a.parts_bc + (p.b * a.seqlen + t0 + first) * row_size + (p.tile * 2 + v / (4 * LN)) * np + m;
-          const int count = static_cast<int>(a.seqlen - t0 < TT ? a.seqlen - t0 : TT);
 #pragma unroll 4
           for (int t = first; t < count; t += STEP, to += STEP * row_size, from += STEP * 8 * LN) {
             float r = from[0];
@@ -420,7 +429,7 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
 
   const int64_t part = p.b * a.segments + p.seg;
   for (int nb = 0; nb < blocks; ++nb) {
-    const int n0 = nb * kSelBlock + sl * kSelStates, n = n0 < np ? mine : 0;
+    const int n0 = nb * 4 * LN + sl * kSelStates, n = n0 < np ? mine : 0;
     if constexpr (ENDS) {
       if constexpr (MULTI) carry = take8(held + nb * 6 * kHalf, kHalf);
       store8(a.ends + (part * a.dim + ch) * np + n0, np, n, carry);
@@ -454,19 +463,24 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sel_sum_bc_kernel(const __grid_constant__ SelArgs a) {
   grid_dependency_wait();
-  const int64_t per = 2 * a.padded;
+  const int64_t per = 2 * a.padded, rows = a.group_tiles;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (i >= a.batch * a.seqlen * a.groups * per) return;
   const int64_t v = i % per, r = i / per, g = r % a.groups, bt = r / a.groups;
-  const float* part = a.parts_bc + (bt * a.tiles + g * a.group_tiles) * per + v;
-  float s = 0.f;
+  const float* part = a.parts_bc + (bt * a.tiles + g * rows) * per + v;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  int64_t k = 0;
 #pragma unroll 4
-  for (int64_t k = 0; k < a.group_tiles; ++k) s += part[k * per];
+  for (; k + 4 <= rows; k += 4)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += part[(k + e) * per];
+  for (; k < rows; ++k) s[0] += part[k * per];
+  const float sum = (s[0] + s[1]) + (s[2] + s[3]);
   const bool is_c = v >= a.padded;
   const int64_t n = is_c ? v - a.padded : v;
   if (n >= a.dstate) return;
   const TensorArg& t = is_c ? a.dC : a.dB;
-  static_cast<T*>(t.data)[(bt / a.seqlen) * t.s0 + g * (is_c ? a.dC_group : a.dB_group) + n * t.s1 + (bt % a.seqlen) * t.s2] = from_f32<T>(s);
+  static_cast<T*>(t.data)[(bt / a.seqlen) * t.s0 + g * (is_c ? a.dC_group : a.dB_group) + n * t.s1 + (bt % a.seqlen) * t.s2] = from_f32<T>(sum);
 }
 
 // dA, dD and dbias: the sums over batch rows and segments.
@@ -509,11 +523,13 @@ cudaError_t walk(const SelArgs& a, cudaStream_t s) {
 }
 template <typename T>
 cudaError_t walk(const SelArgs& a, cudaStream_t s) {
-  if (a.blocks > 1) return a.rows ? walk<T, 4, true, true>(a, s) : walk<T, 4, false, true>(a, s);
+  if (a.blocks > 1) return a.rows ? walk<T, kSelLanes, true, true>(a, s) : walk<T, kSelLanes, false, true>(a, s);
   switch (a.lanes) {
     case 1: return a.rows ? walk<T, 1, true>(a, s) : walk<T, 1, false>(a, s);
     case 2: return a.rows ? walk<T, 2, true>(a, s) : walk<T, 2, false>(a, s);
-    default: return a.rows ? walk<T, 4, true>(a, s) : walk<T, 4, false>(a, s);
+    case 4: return a.rows ? walk<T, 4, true>(a, s) : walk<T, 4, false>(a, s);
+    case 8: return a.rows ? walk<T, 8, true>(a, s) : walk<T, 8, false>(a, s);
+    default: return a.rows ? walk<T, 16, true>(a, s) : walk<T, 16, false>(a, s);
   }
 }
 

@@ -23,7 +23,7 @@ constexpr int kSelThreads = 128;
 // several passes the states between two tiles.
 template <int LN>
 struct FwdSmem {
-  static constexpr int T = 8 * LN, CH = kSelChannels / LN, PITCH = CH + 2;
+  static constexpr int T = sel_tile(LN), CH = kSelChannels / LN, PITCH = CH + 2;
   static constexpr int kFlags = 256, kIo = T * PITCH * 8, kY = (T * PITCH * 4 + 15) / 16 * 16;
   static int64_t bytes(const SelArgs& a) {
     return kFlags + kIo + kY + T * 8 * LN * a.blocks * 4 + (a.blocks > 1 ? a.blocks * kSelThreads * 16 : 0);
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
   float total = 0.f;  // ENDS: the sum of step sizes since the segment's start
   auto rates = [&](int n0) { return mine && n0 < np ? of4(load_rates(a.A, ch, n0, a.dstate)) : zero4(); };
   for (int nb = 0; nb < blocks; ++nb) {
-    const int n0 = nb * kSelBlock + sl * kSelStates;
+    const int n0 = nb * 4 * LN + sl * kSelStates;
     rate = rates(n0);
     h = zero4();
     if (!ENDS && mine && n0 < np)
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
     if (i + 1 < p.chunk1) fetch(i + 1);
 
     for (int nb = 0; nb < blocks; ++nb) {
-      const int n0 = nb * kSelBlock + sl * kSelStates;
+      const int n0 = nb * 4 * LN + sl * kSelStates;
       const bool has = n0 < np && mine;
       if constexpr (MULTI) {
         h = load4(held + (nb * kSelThreads + tid) * 4);
@@ -129,9 +129,9 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
       auto keep = [&](int q, float (&y)[4]) {
         sum_lanes<LN>(y, sl);
 #pragma unroll
-        for (int j = 0; j < 4 / LN; ++j) {
-          float* o = ys + (q * 4 + sl * (4 / LN) + j) * PITCH + c;
-          *o = MULTI && nb > 0 ? *o + y[j] : y[j];
+        for (int j = 0; j < kSums<LN>; ++j) {
+          float* o = ys + (q * 4 + first_sum<LN>(sl) + j) * PITCH + c;
+          if (sl < 4) *o = MULTI && nb > 0 ? *o + y[j] : y[j];
         }
       };
 #pragma unroll 1
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kSelThreads, kFwdCtas) sel_fwd_kernel(const __
   }
   if (ENDS && mine) {
     for (int nb = 0; nb < blocks; ++nb) {
-      const int n0 = nb * kSelBlock + sl * kSelStates;
+      const int n0 = nb * 4 * LN + sl * kSelStates;
       if (n0 >= np) continue;
       if constexpr (MULTI) h = load4(held + (nb * kSelThreads + tid) * 4);
       store4(a.ends + ((p.b * a.segments + p.seg) * a.dim + ch) * np + n0, h);
@@ -244,11 +244,13 @@ cudaError_t run(const SelArgs& a, cudaStream_t s) {
 
 template <typename T>
 cudaError_t run(const SelArgs& a, cudaStream_t s) {
-  if (a.blocks > 1) return a.rows ? run<T, 4, true, true>(a, s) : run<T, 4, false, true>(a, s);
+  if (a.blocks > 1) return a.rows ? run<T, kSelLanes, true, true>(a, s) : run<T, kSelLanes, false, true>(a, s);
   switch (a.lanes) {
     case 1: return a.rows ? run<T, 1, true>(a, s) : run<T, 1, false>(a, s);
     case 2: return a.rows ? run<T, 2, true>(a, s) : run<T, 2, false>(a, s);
-    default: return a.rows ? run<T, 4, true>(a, s) : run<T, 4, false>(a, s);
+    case 4: return a.rows ? run<T, 4, true>(a, s) : run<T, 4, false>(a, s);
+    case 8: return a.rows ? run<T, 8, true>(a, s) : run<T, 8, false>(a, s);
+    default: return a.rows ? run<T, 16, true>(a, s) : run<T, 16, false>(a, s);
   }
 }
 

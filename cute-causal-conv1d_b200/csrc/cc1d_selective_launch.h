@@ -9,7 +9,8 @@ namespace cc1d {
 constexpr int kSelChunk = 32;                    // the most positions of a tile, and between two checkpoints
 constexpr int kSelChannels = 128;                // channels of a CTA times the threads that share one state vector
 constexpr int kSelStates = 4;                    // states of a channel that a thread holds
-constexpr int kSelBlock = 16;                    // states of a channel that a pass over a tile takes, at most
+constexpr int kSelLanes = 16;                    // the most threads that share a channel's states
+constexpr int sel_tile(int lanes) { return lanes < 4 ? 8 * lanes : 32; }  // positions of a tile
 
 struct SelArgs {
   int64_t batch, dim, seqlen, dstate, groups, nstates;
@@ -20,10 +21,10 @@ struct SelArgs {
   float* checkpoints;
   bool softplus;
   // the plan (sel_plan)
-  int lanes;                             // threads that share a channel's states: 1, 2 or 4
-  int blocks;                            // passes over a tile: ceil(dstate / 16)
+  int lanes;                             // threads that share a channel's states: 1, 2, 4, 8 or 16
+  int blocks;                            // passes over a tile: ceil(dstate / (4 lanes))
   int64_t padded;                        // dstate rounded up to a multiple of 4
-  int64_t nchunks;                       // tiles along the sequence: ceil(seqlen / (8 lanes))
+  int64_t nchunks;                       // tiles along the sequence: ceil(seqlen / sel_tile(lanes))
   int64_t gdim, group_tiles, tiles;      // channels of a group, CTAs that they take, CTAs of all groups
   int64_t segments, segment_chunks;      // parts of the sequence that run side by side, chunks of one
   bool rows;                             // unit stride along the sequence: threads go along it
