@@ -70,7 +70,7 @@ __device__ __forceinline__ SelPlace sel_place(const SelArgs& a) {
   p.tile = i % a.tiles;
   i /= a.tiles;
   p.seg = i % a.segments;
-  p.b = i / a.segments;
+  p.b = a.row0 + i / a.segments;
   p.group = p.tile / a.group_tiles;
   const int64_t in_group = (p.tile - p.group * a.group_tiles) * CH;
   p.ch0 = p.group * a.gdim + in_group;

@@ -137,7 +137,7 @@ bool pairs_ok(const TensorArg& t, const SelArgs& a) {
 int64_t choose_segments(const SelArgs& a, bool bwd) {
   constexpr int kFit = 4;
   const double sms = sm_count();
-  const int64_t ctas = a.batch * a.tiles, fit = static_cast<int64_t>(sms) * kFit;
+  const int64_t ctas = a.launch_rows * a.tiles, fit = static_cast<int64_t>(sms) * kFit;
   const double base = bwd ? 13.7 : 3.0, more = bwd ? 1.2 : .55, first = bwd ? .43 : .66;
   double best = 0;
   int64_t pick = 1;
@@ -169,13 +169,18 @@ cc1d_status plan(SelArgs* a, bool bwd) {
                                     bwd ? &a->ddelta : nullptr, bwd ? &a->dz : nullptr};
   for (const TensorArg* t : moved)
     if (t && t->data) a->pairs = a->pairs && pairs_ok(*t, *a);
+  // The backward's sums of dB and dC take 8 padded / CTA's channels bytes per element, so that many
+  // states of a large batch would take more than the tensors: as many batch rows at a time as 2 GB hold.
+  const double row_bytes = 8.0 * a->seqlen * a->tiles * a->padded;
+  a->row0 = 0;
+  a->launch_rows = bwd && row_bytes * a->batch > 2e9 ? std::max<int64_t>(1, static_cast<int64_t>(2e9 / row_bytes)) : a->batch;
   a->segments = choose_segments(*a, bwd);
   a->segment_chunks = (a->nchunks + a->segments - 1) / a->segments;
   a->segments = (a->nchunks + a->segment_chunks - 1) / a->segment_chunks;
-  if (a->batch * a->segments * a->tiles > kMax31 ||
-      static_cast<double>(a->batch) * a->seqlen * a->groups * 2 * a->padded / kThreads > kMax31)
+  if (a->launch_rows * a->segments * a->tiles > kMax31 ||
+      static_cast<double>(a->launch_rows) * a->seqlen * a->groups * 2 * a->padded / kThreads > kMax31)
     return fail(CC1D_ERR_VALUE, "the problem is too large for one launch");
-  if (bwd && static_cast<double>(a->batch) * a->seqlen * a->tiles * 2 * a->padded > 1e17)
+  if (bwd && row_bytes * a->launch_rows > 1e17)
     return fail(CC1D_ERR_VALUE, "the workspace would be too large");
   return CC1D_OK;
 }
@@ -195,7 +200,7 @@ int64_t lay_out(SelArgs* a, bool bwd, void* base) {
     take(a->steps, parts);
   }
   if (bwd) {
-    take(a->parts_bc, a->batch * a->seqlen * a->tiles * 2 * a->padded);
+    take(a->parts_bc, a->launch_rows * a->seqlen * a->tiles * 2 * a->padded);
     take(a->parts_a, parts * a->padded);
     take(a->parts_d, 2 * parts);
   }
@@ -248,8 +253,9 @@ cc1d_status cc1d_selective_bwd_launch(const cc1d_selective_params* p, void* stre
   }
   if ((st = plan(&a, true)) != CC1D_OK) return st;
   if ((st = workspace_ok(p->workspace, p->workspace_bytes, lay_out(&a, true, p->workspace))) != CC1D_OK) return st;
+  const int64_t times = (a.batch + a.launch_rows - 1) / a.launch_rows;
   return launched(by_type(p->x.dtype, a, s, sel_bwd_f32, sel_bwd_f16, sel_bwd_bf16), "selective recurrence backward launch",
-                  a.segments > 1 ? 4 : 3);
+                  static_cast<int>(times * (a.segments > 1 ? 3 : 2) + 1));
 }
 
 cc1d_status cc1d_selective_update_launch(const cc1d_selective_update_params* p, void* stream) {

@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
           if (m >= np) continue;
           const float* from = slabs + first * 8 * LN + v;
           const int64_t row_size = a.tiles * 2 * np;
-          float* to = a.parts_bc + (p.b * a.seqlen + t0 + first) * row_size + (p.tile * 2 + v / (4 * LN)) * np + m;
+          float* to = a.parts_bc + ((p.b - a.row0) * a.seqlen + t0 + first) * row_size + (p.tile * 2 + v / (4 * LN)) * np + m;
 #pragma unroll 4
           for (int t = first; t < count; t += STEP, to += STEP * row_size, from += STEP * 8 * LN) {
             float r = from[0];
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) sel_sum_bc_kernel(const __grid_const
   grid_dependency_wait();
   const int64_t per = 2 * a.padded, rows = a.group_tiles;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= a.batch * a.seqlen * a.groups * per) return;
+  if (i >= a.launch_rows * a.seqlen * a.groups * per) return;
   const int64_t v = i % per, r = i / per, g = r % a.groups, bt = r / a.groups;
   const float* part = a.parts_bc + (bt * a.tiles + g * rows) * per + v;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kThreads) sel_sum_bc_kernel(const __grid_const
   const int64_t n = is_c ? v - a.padded : v;
   if (n >= a.dstate) return;
   const TensorArg& t = is_c ? a.dC : a.dB;
-  static_cast<T*>(t.data)[(bt / a.seqlen) * t.s0 + g * (is_c ? a.dC_group : a.dB_group) + n * t.s1 + (bt % a.seqlen) * t.s2] = from_f32<T>(sum);
+  static_cast<T*>(t.data)[(a.row0 + bt / a.seqlen) * t.s0 + g * (is_c ? a.dC_group : a.dB_group) + n * t.s1 + (bt % a.seqlen) * t.s2] = from_f32<T>(sum);
 }
 
 // dA, dD and dbias: the sums over batch rows and segments.
@@ -512,7 +512,7 @@ cudaError_t launch(const SelArgs& a, cudaStream_t s) {
   const auto kernel = sel_bwd_kernel<T, LN, ROWS, MULTI, ENDS>;
   const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kernel, dim3(static_cast<unsigned>(a.batch * a.segments * a.tiles)), dim3(kSelThreads), smem, s, a);
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(a.launch_rows * a.segments * a.tiles)), dim3(kSelThreads), smem, s, a);
 }
 
 template <typename T, int LN, bool ROWS, bool MULTI = false>
@@ -534,11 +534,17 @@ cudaError_t walk(const SelArgs& a, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t run(const SelArgs& a, cudaStream_t s) {
-  cudaError_t e = walk<T>(a, s);
-  const int64_t bc = a.batch * a.seqlen * a.groups * 2 * a.padded, params = a.dim * (a.padded + 2);
-  if (e == cudaSuccess)
-    e = launch_dependent(sel_sum_bc_kernel<T>, dim3(static_cast<unsigned>((bc + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);
+cudaError_t run(const SelArgs& all, cudaStream_t s) {
+  SelArgs a = all;
+  cudaError_t e = cudaSuccess;
+  const int64_t params = a.dim * (a.padded + 2);
+  for (a.row0 = 0; e == cudaSuccess && a.row0 < a.batch; a.row0 += all.launch_rows) {
+    if (a.launch_rows > a.batch - a.row0) a.launch_rows = a.batch - a.row0;
+    const int64_t bc = a.launch_rows * a.seqlen * a.groups * 2 * a.padded;
+    e = walk<T>(a, s);
+    if (e == cudaSuccess)
+      e = launch_dependent(sel_sum_bc_kernel<T>, dim3(static_cast<unsigned>((bc + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);
+  }
   if (e == cudaSuccess)
     e = launch_dependent(sel_sum_params_kernel, dim3(static_cast<unsigned>((params + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);
   return e;

@@ -230,7 +230,7 @@ cudaError_t launch(const SelArgs& a, cudaStream_t s) {
   const auto kernel = sel_fwd_kernel<T, LN, ROWS, MULTI, ENDS>;
   const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kernel, dim3(static_cast<unsigned>(a.batch * a.segments * a.tiles)), dim3(kSelThreads), smem, s, a);
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(a.launch_rows * a.segments * a.tiles)), dim3(kSelThreads), smem, s, a);
 }
 
 template <typename T, int LN, bool ROWS, bool MULTI = false>

@@ -29,10 +29,11 @@ struct SelArgs {
   int64_t segments, segment_chunks;      // parts of the sequence that run side by side, chunks of one
   bool rows;                             // unit stride along the sequence: threads go along it
   bool pairs;                            // two neighbouring channels move as one word, in every tensor
+  int64_t row0, launch_rows;             // batch rows of a launch; the backward takes some at a time
   // workspace
   float* ends;      // (batch, segments, dim, padded): what a segment alone carries out of itself
   float* steps;     // (batch, segments, dim): the sum of its step sizes, or infinity if it is cut
-  float* parts_bc;  // backward: (batch, seqlen, tiles, 2, padded) sums of dB and dC over a tile's channels
+  float* parts_bc;  // backward: (launch_rows, seqlen, tiles, 2, padded) sums of dB and dC over a tile's channels
   float* parts_a;   // backward: (batch * segments, dim, padded) sums of dA over a segment
   float* parts_d;   // backward: (batch * segments, 2, dim), of dD and dbias
 };

@@ -5,12 +5,14 @@ fp64).  Beside each value it carries the same expression of the magnitudes (H fo
 gradient g of h: every product and sum of absolute values) and a first-order bound of the error
 that fp32 makes of it.
 
-An fp32 kernel takes s and a = exp(s A) to EPS = 2^-20 relative: the hardware's 2^v is within
-2^-22, the rounding of v = s A log2(e) and the error of s move a by |s A| 2^-21 of itself, and
-|s A| exp(-|s A|) < 0.37.  Each product and sum after that rounds by 2^-24.  So, with b = s x B,
+An fp32 kernel takes s to 2^-21 relative (an approximate exponential and reciprocal within 2^-22,
+and a handful of roundings).  a = exp(s A) is 2^v with v = s A log2(e): the hardware's 2^v is within
+2^-22, the roundings of log2(e) A and of v move it by up to 2^-24 |v| ln 2 = 2^-24 |s A| each, and
+the error of s by 2^-21 |s A|.  So a is within EPS (1 + |s A|) relative, EPS = 2^-20.  Each product
+and sum after that rounds by 2^-24.  With b = s x B,
 
-    E_t = a E_{t-1} + EPS (a H_{t-1} + |b|) + 2^-23 H_t           (error of h)
-    F_t = a_{t+1} F_{t+1} + EPS (a_{t+1} G_{t+1} + |C dy|)        (error of g)
+    E_t = a E_{t-1} + EPS ((1 + |s A|) a H_{t-1} + |b|) + 2^-23 H_t           (error of h)
+    F_t = a_{t+1} F_{t+1} + EPS ((1 + |s A|) a_{t+1} G_{t+1} + |C dy|)        (error of g)
 
 and the error of a sum of products is the sum of its factors' errors times the other factors,
 plus EPS for the factors' own roundings and its additions: up to 256 states in a chain of 8 and
@@ -66,6 +68,7 @@ def statement(v, ids=None, nstates=None, use_softplus=True):
     D = v["D"] if v.get("D") is not None else np.zeros(dim)
     a = np.exp(s[..., None] * A)
     b = (s * x)[..., None] * Bf
+    rough = EPS * (1.0 + np.abs(s[..., None] * A))  # relative error of a
     shape = (L, batch, dim, N)
     h, H, E, prev, pH, pE = (np.zeros(shape) for _ in range(6))
     final, final_e = init.copy(), np.zeros_like(init)
@@ -82,7 +85,7 @@ def statement(v, ids=None, nstates=None, use_softplus=True):
             at = a[t, bi]
             prev[t, bi], pH[t, bi], pE[t, bi] = p, P, e
             p = at * p + b[t, bi]
-            e = at * e + EPS * (at * P + np.abs(b[t, bi])) + 2.0 ** -23 * (at * P + np.abs(b[t, bi]))
+            e = at * e + rough[t, bi] * at * P + EPS * np.abs(b[t, bi]) + 2.0 ** -23 * (at * P + np.abs(b[t, bi]))
             P = at * P + np.abs(b[t, bi])
             h[t, bi], H[t, bi], E[t, bi] = p, P, e
             if last[t, bi] and k < n:
@@ -124,7 +127,7 @@ def statement(v, ids=None, nstates=None, use_softplus=True):
             g[t, bi], G[t, bi] = c + cd, cG + np.abs(cd)
             F[t, bi] = cF + EPS * np.abs(cd) + 2.0 ** -23 * G[t, bi]
             at = a[t, bi]
-            c, cG, cF = at * g[t, bi], at * G[t, bi], at * F[t, bi] + EPS * at * G[t, bi]
+            c, cG, cF = at * g[t, bi], at * G[t, bi], at * F[t, bi] + rough[t, bi] * at * G[t, bi]
             if first[t, bi] and k < n:
                 dinit[k], dinit_e[k] = c, cF
 
@@ -139,7 +142,7 @@ def statement(v, ids=None, nstates=None, use_softplus=True):
     gb, GB = (g * Bf).sum(-1), (G * np.abs(Bf)).sum(-1)
     gbe = (F * np.abs(Bf)).sum(-1) + EPS * GB
     w, W = g * a * prev, G * a * pH
-    we = F * a * pH + G * a * pE + 2 * EPS * W
+    we = F * a * pH + G * a * pE + 2 * rough * W
     res["dA"] = ((w * s[..., None]).sum((0, 1)), (we * np.abs(s)[..., None] + EPS * W * np.abs(s)[..., None]).sum((0, 1)))
     aA = np.abs(A)
     ds, DS = (w * A).sum(-1) + x * gb, (W * aA).sum(-1) + np.abs(x) * GB

@@ -374,3 +374,166 @@ def test_parameters_of_other_types():
     for k, dtype in (("A", torch.bfloat16), ("D", torch.float16), ("bias", torch.bfloat16)):
         t[k] = t[k].to(dtype)
     _run_and_check(t)
+
+
+@pytest.mark.parametrize("rows", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("start,D", [(1, 64), (2, 64), (3, 96), (1, 63)])
+def test_tensors_that_start_anywhere(start, D, dtype, rows):
+    """Slices of wider tensors that are NaN around them, off the alignment of pairs of channels."""
+    t = _inputs(start + D, 2, D, 70, 16, dtype, "contiguous" if rows else "channel_last", nstates=2)
+    for k in ("x", "delta", "z", "dout"):
+        v = t[k] if rows else t[k].transpose(1, 2)
+        wide = torch.full((v.shape[0], v.shape[1], v.shape[2] + 7), float("nan"), device="cuda", dtype=dtype)
+        wide[..., start:start + v.shape[2]] = v
+        view = wide[..., start:start + v.shape[2]]
+        t[k] = view if rows else view.transpose(1, 2)
+    leaves = {k: t[k].detach().requires_grad_() for k in NAMES}
+    out, final = selective_recurrence_fn(*[leaves[k] for k in ("x", "delta", "A", "B", "C", "D", "z", "bias")],
+                                         initial_states=leaves["init"], return_final_states=True)
+    found = dict(zip(leaves, torch.autograd.grad([out, final], list(leaves.values()), [t["dout"], t["dfinal"]])))
+    e = S.statement(S.fp64(t))
+    S.check(out, e["out"], "out")
+    S.check(final, e["final"], "final")
+    for k, g in found.items():
+        S.check(g, e["d" + k], "d" + k)
+
+
+def test_mixed_layouts_and_broadcast_inputs():
+    t = _inputs(6, 3, 40, 50, 16, torch.float16, "channel_last", nstates=3)
+    t["delta"] = t["delta"].contiguous()
+    t["B"] = t["B"].contiguous()                                   # along the sequence, C along the states
+    t["z"] = t["z"][:1].expand(3, -1, -1)                          # one output gate for all rows
+    t["C"] = t["C"][:1].expand(3, -1, -1)
+    t["dout"] = t["dout"][:, :, :1].expand(-1, -1, 50)
+    leaves = {k: t[k].detach().requires_grad_() for k in NAMES}
+    out = selective_recurrence_fn(*[leaves[k] for k in ("x", "delta", "A", "B", "C", "D", "z", "bias")], initial_states=leaves["init"])
+    found = dict(zip(leaves, torch.autograd.grad(out, list(leaves.values()), t["dout"])))
+    t["dfinal"] = None
+    e = S.statement(S.fp64(t))
+    S.check(out, e["out"], "out")
+    for k, g in found.items():
+        assert g.shape == t[k].shape
+        S.check(g, e["d" + k], "d" + k)
+    # a leaf that is broadcast gets the sum
+    z = t["z"][:1].detach().clone().requires_grad_()
+    out = selective_recurrence_fn(*[t[k] for k in ("x", "delta", "A", "B", "C", "D")], z.expand(3, -1, -1), t["bias"], initial_states=t["init"])
+    (g,) = torch.autograd.grad(out, z, t["dout"])
+    want, bound = e["dz"]
+    # each of the three is rounded to fp16 before torch adds them there
+    S.check(g, (want.sum(0, keepdims=True), bound.sum(0, keepdims=True) + 4 * 2.0 ** -11 * np.abs(want).sum(0, keepdims=True)), "dz")
+
+
+def test_slow_and_fast_states():
+    """Memories of thousands of steps and of less than one, steps from 1e-4 to 30."""
+    t = _inputs(7, 1, 64, 4000, 8, torch.float32, nstates=1)
+    t["A"] = -torch.logspace(-4, 2, 8, device="cuda").repeat(64, 1)
+    t["bias"] = torch.linspace(-9, 3, 64, device="cuda")
+    t["delta"] = t["delta"] * 0.3
+    _run_and_check(t)
+
+
+@pytest.mark.parametrize("u", [-100.0, -60.0, -20.0, -1e-3, 0.0, 15.0, 40.0, 100.0])
+def test_step_sizes(u):
+    """softplus and its slope to full relative precision: small steps count over long sequences."""
+    D, L = 32, 8
+    delta = torch.linspace(u - 0.5, u + 0.5, D * L, device="cuda").view(1, D, L)
+    x, A = torch.ones(1, D, L, device="cuda"), torch.zeros(D, 1, device="cuda")
+    bc = torch.ones(1, 1, L, device="cuda")
+    leaf = delta.clone().requires_grad_()
+    out = selective_recurrence_fn(x, leaf, A, bc, bc)  # the running sum of the steps
+    w = delta.double()
+    step = torch.clamp(w, min=0) + torch.log1p(torch.exp(-w.abs()))
+    # eight positive terms: each to 2^-21 of itself, the sum's roundings 8 2^-24; below 2^-126 all is zero
+    want = step.cumsum(2)
+    assert ((out.double() - want).abs() <= 2.0 ** -19 * want + 2.0 ** -125 * 8).all()
+    (g,) = torch.autograd.grad(out[..., -1].sum(), leaf)
+    slope = torch.sigmoid(w)
+    assert ((g.double() - slope).abs() <= 2.0 ** -19 * slope + 2.0 ** -125).all()
+
+
+def test_batches_that_the_backward_splits():
+    """The sums of dB and dC of all rows would take over 2 GB: some rows at a time."""
+    t = _inputs(5, 9, 512, 8192, 64, torch.bfloat16, nstates=None)
+    t["z"], args = None, ("x", "delta", "A", "B", "C", "D", "z", "bias")
+
+    def grads(w):
+        leaves = {k: w[k].detach().requires_grad_() for k in args if w[k] is not None}
+        out = selective_recurrence_fn(*[leaves.get(k) for k in args])
+        return dict(zip(leaves, torch.autograd.grad(out, list(leaves.values()), w["dout"])))
+
+    whole = grads(t)
+    total = {k: torch.zeros_like(t[k], dtype=torch.float64) for k in ("A", "D", "bias")}
+    for b in (0, 3, 6, 7, 8):  # on both sides of the splits
+        part = grads({k: (v[b:b + 1] if v is not None and v.dim() == 3 else v) for k, v in t.items()})
+        for k in ("x", "delta", "B", "C"):
+            # the same sums over other parts of the sequence: fp32 roundings, then bf16's
+            torch.testing.assert_close(whole[k][b:b + 1], part[k], rtol=2.0 ** -7, atol=2.0 ** -16 * part[k].abs().max().item())
+    for b in range(9):
+        part = grads({k: (v[b:b + 1] if v is not None and v.dim() == 3 else v) for k, v in t.items()})
+        for k in total:
+            total[k] += part[k].double()
+    for k in total:
+        torch.testing.assert_close(whole[k].double(), total[k], rtol=1e-4, atol=1e-4 * total[k].abs().max().item())
+
+
+@pytest.mark.parametrize("layout", ["channel_last", "contiguous"])
+@pytest.mark.parametrize("D,L", [(72, 30_000_128), (71, 30_300_007)])
+def test_offsets_past_32_bits(D, L, layout):
+    """The ends of a long sequence are what the statements of short stretches give."""
+    g = _gen(D)
+    x = torch.randn(1, L, D, generator=g, device="cuda", dtype=torch.bfloat16)
+    x = x.transpose(1, 2) if layout == "channel_last" else x.view(1, D, L)
+    bc = torch.randn(1, L, 2, generator=g, device="cuda", dtype=torch.bfloat16).transpose(1, 2)
+    A = -torch.exp(torch.randn(D, 2, generator=g, device="cuda"))
+    dfinal = torch.randn(1, D, 2, generator=g, device="cuda")
+    args = (x, x, A, bc, bc, None, None, None, True, None)
+    _, _, kept = selective_recurrence_fwd_function(*args, None, False, None, True)
+    dx, ddelta, _, dB, dC, _, _, _, _ = selective_recurrence_bwd_function(*args, None, kept, x, dfinal, False, False)
+    n = 501
+    cut = (x[:, :, :L - n], x[:, :, :L - n], A, bc[:, :, :L - n], bc[:, :, :L - n], None, None, None, True, None)
+    out, mid, _ = selective_recurrence_fwd_function(*cut, None, True, None, False)
+    del out
+
+    def stretch(lo, hi, init, last):
+        v = {k: S.wide(w[:, :, lo:hi]) for k, w in (("x", x), ("delta", x), ("B", bc), ("C", bc), ("dout", x))}
+        return S.statement({**v, "A": S.wide(A), "init": None if init is None else S.wide(init), "dfinal": None if last is None else S.wide(last)})
+
+    e = stretch(L - n, L, mid, dfinal)
+    for k, got in (("dx", dx), ("ddelta", ddelta), ("dB", dB), ("dC", dC)):
+        S.check(got[:, :, L - n:], e[k], k + ", tail")
+    # the first ones, whose gradients forget what lies 400 positions on (steps of 0.7 and more on average)
+    e = stretch(0, n + 400, None, None)
+    for k, got in (("dx", dx), ("ddelta", ddelta), ("dB", dB), ("dC", dC)):
+        S.check(got[:, :, :n], tuple(w[:, :, :n] for w in e[k]), k + ", head")
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, and two graphs that are replayed in turn, have workspaces of their own."""
+    ts = [_inputs(s, 1, 64, 2000, 16, torch.bfloat16, nstates=1) for s in (1, 2)]
+
+    def both(t):
+        args = [t[k] for k in ("x", "delta", "A", "B", "C", "D", "z", "bias")]
+        out, final, kept = selective_recurrence_fwd_function(*args, True, None, t["init"], True, None, True)
+        return [out, final, *selective_recurrence_bwd_function(*args, True, None, t["init"], kept, t["dout"], t["dfinal"], True, True)]
+
+    want = [both(t) for t in ts]
+    streams = [torch.cuda.Stream() for _ in ts]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for t, stream in zip(ts, streams):
+            with torch.cuda.stream(stream):
+                got.append(both(t))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+    graphs = []
+    for t in ts:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0][0].pool() if graphs else None):
+            graphs.append((graph, both(t)))
+    for i in (0, 1, 1, 0):
+        graphs[i][0].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(graphs[i][1], want[i]))
