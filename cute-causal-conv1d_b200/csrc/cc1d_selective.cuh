@@ -32,7 +32,19 @@ __device__ __forceinline__ float2 exp_of_size(float2 u) {
 }
 template <typename T>
 __device__ __forceinline__ float2 step_size(float2 u) { return softplus_of_exp(u, exp_of_size<T>(u)); }
-// The same, and its derivative sigmoid(u).
+template <typename T>
+__device__ __forceinline__ float step_size(float u) {
+  float e;
+  if constexpr (std::is_same<T, float>::value) e = exp_minus(min_nan(fabsf(u), 88.f));
+  else e = ex2_approx(-kLog2e * fabsf(u));
+  const float s = e * rcp_approx(2.f + e), w = s * s;
+  float q = fmaf(0.281577796f, w, 0.279651582f);
+  q = fmaf(q, w, 0.400245965f);
+  q = fmaf(q, w, 0.666663229f);
+  q = fmaf(q, w, 2.f);
+  return fmaf(s, q, fmaxf(u, 0.f));
+}
+// The same of two, and the derivative sigmoid(u).
 template <typename T>
 __device__ __forceinline__ float2 step_size(float2 u, float2* slope) {
   const float2 e = exp_of_size<T>(u), d = fadd2(both(1.f), e);
