@@ -46,7 +46,7 @@ def beam_search_reorder(states, parents, state_indices=None):
     other signed integers and uint8 are converted.
 
     At most 64 beams.  No two elements of a tensor may lie at the same place, and no two of the
-    tensors may share memory.  States that require grad are refused outside torch.no_grad().
+    tensors may share memory (two that start at one place are refused).  States that require grad are refused outside torch.no_grad().
     """
     _block.beam_reorder([states] if isinstance(states, torch.Tensor) else list(states), parents, state_indices)
 

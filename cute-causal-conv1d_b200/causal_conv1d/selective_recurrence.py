@@ -31,7 +31,8 @@ def selective_recurrence_fwd_function(x, delta, A, B, C, D, z, delta_bias, delta
 def selective_recurrence_bwd_function(x, delta, A, B, C, D, z, delta_bias, delta_softplus, seq_idx, initial_states,
                                       checkpoints, dout, dfinal_states, return_dbias, return_dinitial_states):
     """One backward pass.  Returns (dx, ddelta, dA, dB, dC, dD, dz, dbias, dinitial_states):
-    dD and dz are None without D and z, each gradient has its input's dtype."""
+    dD and dz are None without D and z, each gradient has its input's dtype (fp32 where the input,
+    delta_bias or initial_states, is absent)."""
     return _block.selective_bwd(x, delta, A, B, C, D, z, delta_bias, delta_softplus, seq_idx, initial_states, checkpoints,
                                 dout, dfinal_states, return_dbias, return_dinitial_states)
 

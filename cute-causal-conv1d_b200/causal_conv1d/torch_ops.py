@@ -267,11 +267,15 @@ def _(x, delta, A, B, C, D, z, delta_bias, delta_softplus, seq_idx, initial_stat
     def coefficients(t):
         return x.new_empty(*t.shape[:1], t.shape[-1], *t.shape[1:-1]).movedim(1, -1) if along else x.new_empty(t.shape)
 
-    init = x.new_empty(initial_states.shape if return_dinitial_states else _EMPTY,
-                       dtype=torch.float32 if return_dinitial_states else x.dtype)
+    def full(shape):
+        return x.new_empty(shape, dtype=torch.float32)
+
+    bias = full(x.shape[1]) if delta_bias is None else delta_bias
+    n = next((t.shape[0] for t in (initial_states, dfinal_states) if t is not None), 0) if seq_idx is not None else x.shape[0]
+    init = full((n, *A.shape)) if return_dinitial_states else x.new_empty(_EMPTY)
     dz = _laid_out_like(x) if z is not None else x.new_empty(_EMPTY)
     return [_laid_out_like(x), _laid_out_like(x), like(A), coefficients(B), coefficients(C), like(D), dz,
-            like(delta_bias, return_dbias), init]
+            like(bias, return_dbias), init]
 
 
 @torch.library.custom_op("causal_conv1d::selective_recurrence_update", mutates_args=("state",))

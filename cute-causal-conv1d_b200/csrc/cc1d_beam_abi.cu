@@ -156,6 +156,11 @@ cc1d_status cc1d_beam_reorder_launch(const cc1d_beam_reorder_params* p, void* st
   a.wide_parents = p->parents.dtype == CC1D_INT64;
   a.indices = static_cast<const int32_t*>(p->state_indices.data);
   a.indices_stride = p->state_indices.stride[0];
+  const auto full = [](const cc1d_beam_rows& r) { return r.rows && r.size[0] && r.size[1] && r.size[2]; };
+  for (int64_t i = 0; i < p->count; ++i)
+    for (int64_t j = 0; j < i; ++j)
+      if (p->tensors[i].data == p->tensors[j].data && full(p->tensors[i]) && full(p->tensors[j]))
+        return fail(CC1D_ERR_VALUE, "two of the states start at one place");
   // every tensor is checked before the first one changes
   for (int pass = 0; pass < 2; ++pass) {
     a.count = 0;

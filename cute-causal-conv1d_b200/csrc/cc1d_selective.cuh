@@ -32,6 +32,7 @@ __device__ __forceinline__ float2 exp_of_size(float2 u) {
 }
 template <typename T>
 __device__ __forceinline__ float2 step_size(float2 u) { return softplus_of_exp(u, exp_of_size<T>(u)); }
+// The same of one.
 template <typename T>
 __device__ __forceinline__ float step_size(float u) {
   float e;
@@ -220,9 +221,8 @@ struct Walk {
 };
 // B and C of a tile's positions as fp32 in shared memory: [position][B, C][wide], wide = 4 LN per
 // pass; zero past dstate and where a position is not valid, so that whatever stands there is not
-// used.  The threads
-// go along the states or, where that is B's unit stride, along the sequence; a thread's elements
-// for a single pass are loaded a tile ahead.
+// used.  The threads go along the states or, where that is B's unit stride, along the sequence; a
+// thread's elements for a single pass are loaded a tile ahead.
 template <typename T, int NT, int LN, bool MULTI>
 struct Coefficients {
   static constexpr int TT = sel_tile(LN), WIDE = 8 * LN, ALL = TT * WIDE, HELD = MULTI || ALL < NT ? 1 : ALL / NT;

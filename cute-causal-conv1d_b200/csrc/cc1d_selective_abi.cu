@@ -127,13 +127,23 @@ bool pairs_ok(const TensorArg& t, const SelArgs& a) {
 
 // Parts of the sequence that run side by side.  One part needs no first pass over it; with more,
 // that pass finds what each part hands to the next one.  Four CTAs run on an SM (registers), and a
-// tile takes long because a thread's work is one chain: with n CTAs on an SM, measured on a B200
+// tile takes long because a thread's work is one chain: with n CTAs on an SM its time is about
 // (microseconds, 32 positions, 16 states, bf16 with z)
 //
 //   forward  3.0 + .55 n, the first pass .66 of it      backward  13.7 + 1.2 n, .43
 //
-// and a part about two tiles' time to start.  One sequence of 16384 positions and 1024 channels:
-// forward 1587 us in one part, 660 in four; backward 7617 and 2729.
+// and a part about two tiles' time to start.  Measured on a B200, bf16 with z, 16 states, microseconds
+// in one part, in the parts chosen, and in the best of thirteen counts from 1 to 64:
+//
+//   batch x dim x seqlen   forward              backward
+//   1 x 1024 x 16384       1543, 253, 253       7700, 742, 742
+//   1 x 64 x 16384         1521, 58, 58         7032, 193, 193
+//   1 x 4096 x 2048        197, 131, 130        1017, 431, 431
+//   2 x 4096 x 2048        235, 235, 235        1026, 819, 768
+//   4 x 4096 x 2048        322, 322, 322        1197, 1197, 1197
+//   8 x 8192 x 128         85, 85, 85           346, 346, 346
+//   1 x 5120 x 8192        915, 584, 581        3986, 1819, 1819
+//   1 x 1024 x 4096 x 64   356, 255, 243        1648, 1153, 1055    (64 states)
 int64_t choose_segments(const SelArgs& a, bool bwd) {
   constexpr int kFit = 4;
   const double sms = sm_count();

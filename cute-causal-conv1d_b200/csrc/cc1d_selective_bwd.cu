@@ -8,27 +8,36 @@
 //     dA[n] = sum_t g_t[n] a_t[n] h_{t-1}[n] s_t
 // and ddelta = ds sigmoid(delta + bias), dz = dout y silu'(z).
 //
-// CTAs and threads are the forward's; tiles have 32 (16, 8) positions, and a CTA goes through them
-// from the last one back.  From the state that the forward kept before a tile it runs forward,
-// keeping the state before every fourth position, then takes the groups of four positions from the
-// last one back: states again, then gradients.  dB and dC are summed over a thread's two channels,
-// over the warp's by exchanges between lanes, over the CTA's warps in shared memory and over CTAs
-// by a second kernel, all in a fixed order.
+// A CTA owns the channels that a forward CTA owns, with half the threads: a thread holds four states
+// of two neighbouring channels, so that the sums of dB and dC start in its registers.  It goes through
+// the tiles from the last one back.  From the state that the forward kept before a tile it runs
+// forward, keeping the state before every fourth position, then takes the groups of four positions
+// from the last one back: states again, then gradients.  dB and dC are summed over a thread's two
+// channels, over the warp's by exchanges between lanes, over the CTA's warps in shared memory and
+// over CTAs by a second kernel, all in a fixed order: two calls give the same bits.
+//
+// What bounds it: an element takes two exponentials (238 us for the 537 M elements of 4 x 4096 x 2048
+// x 16, which takes 1197; its memory 82) and 28 instructions, most of them the gradients' FMAs and the
+// exchanges that sum dB, dC over channels and ds, dx over states.  Eight warps an SM are what the
+// registers leave; a scheduler issues .35 a cycle.  Of the 1197 us the pass to the states takes 180,
+// the gradients 570 (their sums over channels 180, over states 100), and what is done once per
+// position and channel (step sizes, gates, loads, stores) 440.
+//
+// Sums straight to memory for each warp and half the groups took 1372 us, loads ahead of the tile
+// 1266, B and C doubled in shared memory 2107, prefetches of the next tile into L2 1217.
 #include "cc1d_selective.cuh"
 
 namespace cc1d {
 namespace {
 
 constexpr int kSelThreads = 64, kWarps = kSelThreads / 32, kHalf = kSelThreads * 4;
-#ifndef BWDC
-#define BWDC 4
-#endif
-constexpr int kBwdCtas = BWDC;
+// CTAs of an SM: all 255 registers of a thread are in use.  With 168, and six CTAs, 1550 us.
+constexpr int kBwdCtas = 4;
 
 // Shared memory: flags; (s, x) of a pair by position, replaced by (dx, ddelta), and (dy, slope of the
-// step size), replaced by (y, -), and dout silu'(z); the states before every fourth position; each warp's sums of dB
-// and dC; B and C; of each pass g carried, dA and its low part; with several passes three sums by
-// position and pair.
+// step size), replaced by (y, -), and dout silu'(z); the states before every fourth position; each
+// warp's sums of dB and dC; B and C; of each pass g carried, dA and its low part; with several passes
+// three sums by position and pair.
 template <int LN>
 struct BwdSmem {
   static constexpr int T = sel_tile(LN), PAIRS = kSelThreads / LN, PITCH = PAIRS + 1;

@@ -3,20 +3,29 @@
 //     s_t = softplus(delta_t + bias)         h_t[n] = exp(s_t A[n]) h_{t-1}[n] + s_t x_t B_t[n]
 //     y_t = sum_n C_t[n] h_t[n] + D x_t      out_t = y_t silu(z_t)
 //
-// A CTA of 128 threads owns up to 32 channels (64 or 128 for at most 8 or 4 states) of one batch
-// row and walks the sequence in tiles of 32 (16, 8) positions.  A thread holds four states of a
-// channel in registers and goes through the tile one position after the other; the step sizes of
-// a tile are made once, by all threads, and with B and C lie in shared memory as fp32.  The
-// next tile's inputs are on their way to registers meanwhile.
+// A CTA of 128 threads walks the sequence of a batch row in tiles of 32 positions (8 for at most 4
+// states, 16 for at most 8).  A thread holds four states of a channel in registers; LN = 1 to 16
+// threads share a channel, a CTA owns 128 / LN channels, and more than 64 states take several passes
+// over a tile.  The step sizes of a tile are made once, by all threads, and with B and C lie in
+// shared memory as fp32; the next tile's inputs are on their way to registers, as the words that
+// they arrive in, meanwhile.
+//
+// What bounds it: an element of h takes one exponential (MUFU, 16 a cycle and SM) and about six
+// instructions in all, two values at a time where sm_100a can.  4 x 4096 x 2048 x 16 bf16 with z
+// (537 M elements, 268 MB without the checkpoints) takes 318 us: its exponentials alone 119, its
+// memory 41.  Its 512 CTAs are 3.5 an SM, so the longest wait is a thread's chain of dependent
+// positions; the MUFU is busy 47 % of the time.
+//
+// Eight positions are unrolled, with their loads first.  Two channels a thread took 502 us (half the
+// warps), three tiles in flight in one unrolled loop 420 to 550 (the instruction cache), 64 or 96
+// registers a thread 360 to 450.
 #include "cc1d_selective.cuh"
 
 namespace cc1d {
 namespace {
 
-#ifndef FWDC
-#define FWDC 4
-#endif
-constexpr int kFwdCtas = FWDC;
+// CTAs of an SM, which bounds the registers: three took 449 us above, four 318, five 364 (spills).
+constexpr int kFwdCtas = 4;
 constexpr int kSelThreads = 128;
 
 // Shared memory: flags; (s, s x) by position and channel; y by position and channel; B and C; with

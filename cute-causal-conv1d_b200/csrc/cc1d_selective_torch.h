@@ -165,7 +165,7 @@ SelGrads sel_backward(SelInputs v, const Tensor& kept, Tensor dout, const Tensor
   };
   as(dA, v.A);
   if (dD.defined()) as(dD, v.D);
-  if (dbias.defined()) as(dbias, v.bias);
+  if (dbias.defined() && v.bias.defined()) as(dbias, v.bias);
   if (!grouped) dB = dB.squeeze(1);
   if (!grouped_c) dC = dC.squeeze(1);
   return {dx, ddelta, dA, dB, dC, dD, dz, dbias, dinit};

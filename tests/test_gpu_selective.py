@@ -331,6 +331,20 @@ def test_captured():
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(state, after)
 
 
+def test_gradients_of_absent_inputs():
+    """Without delta_bias and initial_states the backward pass gives the gradients of zeros, if it is asked for them."""
+    t = _inputs(4, 2, 34, 45, 5, torch.bfloat16, nstates=2)
+    args = [t[k] for k in ("x", "delta", "A", "B", "C", "D", "z")]
+    zeros = [torch.zeros(34, device="cuda"), torch.zeros_like(t["init"])]
+    found = []
+    for bias, init in ((None, None), zeros):
+        kept = selective_recurrence_fwd_function(*args, bias, True, None, init, False, None, True)[2]
+        found.append(selective_recurrence_bwd_function(*args, bias, True, None, init, kept, t["dout"], None, True, True))
+        fewer = selective_recurrence_bwd_function(*args, bias, True, None, init, kept, t["dout"], None, False, False)
+        assert fewer[7] is None and fewer[8] is None
+    assert all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(*found))
+
+
 def test_derivatives_are_refused():
     t = _inputs(1, 1, 8, 20, 4, torch.float32, nstates=1)
     args = [t[k] for k in ("x", "delta", "A", "B", "C")]

@@ -340,6 +340,7 @@ def test_beam_abi_refusals_need_no_gpu():
     _refused(fn, reorder([good], sizes=(2, 65)), 1, b"beams")
     _refused(fn, reorder([good], parents=_tensor(dtype=0)), 2, b"parents")
     _refused(fn, reorder([good], index=_tensor(dtype=4)), 2, b"state_indices")
+    _refused(fn, reorder([good, (4096, *good[1:]), good]), 1, b"start at one place")
     _refused(fn, reorder([(16, 6, 4, 3, 4, 1, 1, 1, 1, 1)]), 1, b"element_bytes")
     _refused(fn, reorder([(16, 5, 4, 4, 4, 1, 1, 1, 1, 1)]), 1, b"one row")
     for bad in ((16, 6, 3, 4, 4, 1, 1, 1, 1, 1),     # a row reaches into the next one
@@ -392,6 +393,8 @@ def test_torch_ops_registered_with_fake_shapes():
         g = ops.selective_recurrence_bwd(x, x, A, bc, bc, None, None, D, True, None, init, ck, x, final, True, True)
         assert g[0].stride() == x.stride() and g[3].shape == bc.shape and g[3].stride() == bc.stride()
         assert g[2].shape == A.shape and g[5].numel() == 0 and g[6].numel() == 0 and g[8].shape == init.shape
+        g = ops.selective_recurrence_bwd(x, x, A, bc, bc, None, None, None, True, None, None, ck, x, None, True, True)
+        assert g[7].shape == (64,) and g[7].dtype == torch.float32 and g[8].shape == init.shape
         assert ops.selective_recurrence_update(x[..., 0], init, x[..., 0], A, bc[..., 0], bc[..., 0], None, None, None, True, None).shape == (2, 64)
         s, p, t = ops.beam_search_select(torch.empty(3, 4, 9), torch.empty(3, 4), None, None, 6)
         assert s.shape == p.shape == t.shape == (3, 6) and p.dtype == torch.int64
