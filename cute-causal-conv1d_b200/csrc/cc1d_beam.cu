@@ -12,19 +12,20 @@ namespace {
 // total[k, v] = scores[k] + logits[k, v] - log sum_w exp(logits[k, w]); the best `candidates` of
 // beams x vocabulary, equal ones by the lowest place.
 //
-// One pass over the logits: each warp walks a strip of a row with the running maximum and sum of
-// the softmax and a sorted list of the strip's best in registers, one or two entries a lane.  An
-// element is looked at one by one only if it beats the list's last entry, which becomes rare
-// after the first steps; a floor from all warps of a CTA (the n-th largest of their elements' maxima,
-// later of their lists) keeps out most of the others.  A second kernel joins the strips' lists, by
-// beams, then over beams.
+// One pass over the logits: each warp walks a strip of a row with the running maximum and sum of the
+// softmax, and keeps each lane's largest element in each of up to 32 chunks of the strip.  The n-th
+// largest of the threads' maxima is a floor of the best n; the few chunks that reach it (about n of a
+// CTA's) are read again, and the elements above it enter a sorted list of each warp, one or two entries
+// a lane.  The warps' lists are joined, and a second kernel joins those of a row's parts, then ranks
+// the beams' lists.  Beams that are at their end, or not in use, are not read.
 //
-// What bounds it: 512 rows of 128000 bf16 logits (131 MB, 20 us of memory) take 78 us, mostly the
-// instructions of the exponentials' sums and comparisons, two per element, and the insertions before
-// the floors are known; without the floors 180 us, with one made once from the threads' maxima 116.
-// Four rows of 32000 take 12.7 us: two kernels of which the second waits for the first, and in them
-// chains of exchanges and barriers rather than data.
+// What bounds it: 512 rows of 128000 bf16 logits (131 MB, 20 us of memory) take 53 us, 7 instructions
+// an element in the walk (one exponential, 15 us of all) and chains of exchanges behind it; with lists
+// kept during the walk 66 us, and with a floor from its first step alone 116.  Four rows of 32000 take
+// 11 us: two kernels of which the second waits for the first, and in them exchanges and barriers
+// rather than data.
 constexpr int kWarps = kThreads / 32;
+constexpr int kAhead = 2, kChunks = 32;
 constexpr int kEmpty = INT_MIN;  // below the order of every float
 
 // Order of floats as integers; -0 counts as 0.
@@ -79,6 +80,21 @@ struct Best {
       todo &= __ballot_sync(~0u, takes(k, place));
     }
   }
+  // The list of 32 entries that stands in `other` is joined to this one (Q = 1).  Of two descending
+  // lists a and b the better of a[i] and b[31 - i] are the 32 best, in a bitonic order.
+  __device__ __forceinline__ void join(const int2* other, int lane) {
+    const int2 o = other[31 - lane];
+    int k = key[0], place = at[0];
+    if (o.x > k || (o.x == k && o.y < place)) k = o.x, place = o.y;
+#pragma unroll
+    for (int step = 16; step > 0; step /= 2) {
+      const int ok = __shfl_xor_sync(~0u, k, step), op = __shfl_xor_sync(~0u, place, step);
+      const bool mine = k > ok || (k == ok && place < op), same = k == ok && place == op;
+      if (!same && mine != ((lane & step) == 0)) k = ok, place = op;
+    }
+    key[0] = k;
+    at[0] = place;
+  }
   // The first entries, one of each lane (none: kEmpty): sorted by exchanges.
   __device__ __forceinline__ void fill(int k, int place, int lane) {
 #pragma unroll
@@ -121,48 +137,35 @@ __device__ __forceinline__ void add_to(Soft& a, float v) {
   a.s = t;
 }
 
-template <typename T, int Q>
-struct Strip {
-  Best<Q> best;
-  Soft soft;
-  int lane;
-  int floor = kEmpty;  // n elements of the CTA's part are at least that
-  // E neighbouring elements of each lane from place `at` on; `has` of them
-  template <int E>
-  __device__ __forceinline__ void step(const float (&x)[E], int at, int has) {
-    float top = x[0];
+// The largest of 2 P elements, two neighbouring ones in one float2.
+template <int P>
+__device__ __forceinline__ float top_of(const float2 (&x)[P]) {
+  float top = fmaxf(x[0].x, x[0].y);
 #pragma unroll
-    for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
-    raise(soft, top);
-    const float c = scale_of(soft.m);
-    float s[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) s[e] = ex2_approx(fmaf(x[e], kLog2e, -c));
-#pragma unroll
-    for (int w = E / 2; w > 0; w /= 2)
-#pragma unroll
-      for (int e = 0; e < w; ++e) s[e] += s[e + w];
-    add_to(soft, s[0]);
-    const int key = order_of(top);
-    const int least = max(best.last, floor);
-    if (!__any_sync(~0u, has > 0 && key >= least)) return;
-    // the lanes' elements that may count, one after the other
-    unsigned mine = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) mine |= (e < has && order_of(x[e]) >= least ? 1u : 0u) << e;
-    while (true) {
-      const unsigned todo = __ballot_sync(~0u, mine != 0);
-      if (!todo) break;
-      const int from = __ffs(todo) - 1, first = __ffs(mine) - 1;
-      float v = x[0];
-#pragma unroll
-      for (int e = 1; e < E; ++e) v = e == first ? x[e] : v;
-      const int k = __shfl_sync(~0u, order_of(v), from), place = __shfl_sync(~0u, at + first, from);
-      if (best.takes(k, place)) best.insert(k, place, lane);
-      if (lane == from) mine &= mine - 1;
-    }
+  for (int p = 1; p < P; ++p) top = fmaxf(top, fmaxf(x[p].x, x[p].y));
+  return top;
+}
+// Adds the exponentials of 2 P H elements, of which `top` is the largest; c = scale_of(a.m).
+template <int H, int P>
+__device__ __forceinline__ void add_exps(Soft& a, float& c, const float2 (&x)[H][P], float top) {
+  if (top > a.m) {
+    raise(a, top);
+    c = scale_of(top);
   }
-};
+  float2 s[H * P];
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const float2 v = ffma2(x[h][p], make_float2(kLog2e, kLog2e), make_float2(-c, -c));
+      s[h * P + p] = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+    }
+#pragma unroll
+  for (int w = H * P / 2; w > 0; w /= 2)
+#pragma unroll
+    for (int i = 0; i < w; ++i) s[i] = fadd2(s[i], s[i + w]);
+  add_to(a, s[0].x + s[0].y);
+}
 
 // One step of a bitonic network on the lanes' keys: lanes `step` apart, the larger first where `down`.
 __device__ __forceinline__ int exchange(int k, int step, bool down, int lane) {
@@ -176,47 +179,38 @@ __device__ __forceinline__ int sorted_down(int k, int lane) {
     for (int step = size / 2; step > 0; step /= 2) k = exchange(k, step, (lane & size) == 0, lane);
   return k;
 }
-// The n-th largest (n <= 32) of kWarps descending lists of 32 keys in shared memory.  Of two
-// descending lists a and b the larger of a[i] and b[31 - i] are the 32 largest, in a bitonic order.
-__device__ __forceinline__ int nth_of_lists(const int* keys, int n, int lane) {
-  int k = keys[lane];
-  for (int w = 1; w < kWarps; ++w) {
-    k = max(k, keys[w * 32 + 31 - lane]);
-#pragma unroll
-    for (int step = 16; step > 0; step /= 2) k = exchange(k, step, true, lane);
-  }
-  return __shfl_sync(~0u, k, n - 1);
+// A beam at its end, or without a finite score, has no use for its logits.
+__device__ __forceinline__ bool beam_done(const BeamSelectArgs& a, int64_t b, int64_t k, float* score) {
+  *score = a.scores[b * a.scores_s0 + k * a.scores_s1];
+  return a.finished && a.finished[b * a.finished_s0 + k * a.finished_s1];
 }
 
+// Four CTAs an SM leave 64 registers; three with four steps on their way take 65 us above (two waves),
+// five and six, which spill, 57 and 72.
 template <typename T, int Q>
-__global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectArgs a) {
-  constexpr int E = 16 / sizeof(T);
+__global__ void __launch_bounds__(kThreads, kBeamCtas) beam_parts_kernel(const BeamSelectArgs a) {
+  constexpr int E = 16 / sizeof(T), P = E / 2;
   __shared__ int2 lists[kWarps][Q * 32];
   __shared__ Soft softs[kWarps];
-  __shared__ int keys[2][kThreads];
+  __shared__ int keys[kThreads], floor;
+  __shared__ float maxima[kChunks][kThreads];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int n = static_cast<int>(a.candidates);
   grid_dependency_wait();
+  float score;
+  const bool ended = beam_done(a, row / a.beams, row % a.beams, &score);
   const T* x = static_cast<const T*>(a.logits) + (row / a.beams) * a.logits_s0 + (row % a.beams) * a.logits_s1;
   const int64_t begin = part * a.part, end = begin + a.part < a.vocab ? begin + a.part : a.vocab;
   const int64_t strip = (end - begin + kWarps - 1) / kWarps;
   int64_t i = begin + warp * strip;
   const int64_t stop = i + strip < end ? i + strip : end;
-  Strip<T, Q> w;
-  w.lane = lane;
-  w.best.start(n);
   // up to the first 16-byte boundary, element by element
   const int64_t past = reinterpret_cast<uintptr_t>(x + i) % 16 / sizeof(T);
-  const int64_t head = past ? E - past : 0;
-  if (i < stop && head) {
-    const int64_t count = head < stop - i ? head : stop - i;
-    float v[1] = {lane < count ? to_f32(x[i + lane]) : -INFINITY};
-    w.step(v, static_cast<int>(i + lane), lane < count ? 1 : 0);
-    i += count;
-  }
-  // steps of 32 E elements, the next two on their way; the last one may be short
-  constexpr int STEP = 32 * E, AHEAD = 2;
+  const int64_t head = past && i < stop ? (E - past < stop - i ? E - past : stop - i) : 0, start = i;
+  i += head;
+  // Steps of 32 E elements; AHEAD of them are on their way, and are taken two at a time.
+  constexpr int STEP = 32 * E, AHEAD = kAhead;
   const int size = i < stop ? static_cast<int>(stop - i) : 0, from = lane * E, steps = (size + STEP - 1) / STEP;
   const T* q = x + i;
   // Kept as words until they are used: taking them apart at once would wait for the load.
@@ -225,90 +219,137 @@ __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const BeamSelectAr
     const int at = from + n * STEP;
     return at + E <= size ? *reinterpret_cast<const uint4*>(q + at) : make_uint4(0, 0, 0, 0);
   };
-  auto count = [&](int n) { return min(max(size - from - n * STEP, 0), E); };
-  auto values = [&](int n, const uint4& u, float (&v)[E]) {
-    unpack<T, E>(*reinterpret_cast<const Packet<T, E>*>(&u), v);
+  auto values = [&](int n, const uint4& u, float2 (&v)[P]) {
+    unpack2<T, E>(*reinterpret_cast<const Packet<T, E>*>(&u), v);
     if ((n + 1) * STEP > size) {
       const int at = from + n * STEP;
       if (at + E > size)
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = at + e < size ? to_f32(q[at + e]) : -INFINITY;
+        for (int p = 0; p < P; ++p)
+          v[p] = make_float2(at + 2 * p < size ? to_f32(q[at + 2 * p]) : -INFINITY,
+                             at + 2 * p + 1 < size ? to_f32(q[at + 2 * p + 1]) : -INFINITY);
     }
   };
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k) next[k] = fetch(k);
-  auto run = [&](int first, int end) {  // first: a multiple of AHEAD
-    for (int n0 = first; n0 < end; n0 += AHEAD) {
+  if (ended || !(fabsf(score) < INFINITY)) return;
+  // The sums, and the largest element of each lane in each of up to kChunks chunks of the strip.
+  Soft soft;
+  float c = 0.f, most = -INFINITY;
+  const float2 first[1][1] = {{make_float2(lane < head ? to_f32(x[start + lane]) : -INFINITY, -INFINITY)}};
+  if (head) add_exps(soft, c, first, first[0][0].x);
+  const int groups = (steps + AHEAD - 1) / AHEAD, chunk = (groups + kChunks - 1) / kChunks;
+  for (int g = 0, at = 0; g < groups; ++at) {
+    float most_here = -INFINITY;
+    for (const int till = min(g + chunk, groups); g < till; ++g) {
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        if (n0 + k >= end) break;
-        float v[E];
-        values(n0 + k, next[k], v);
-        next[k] = fetch(n0 + k + AHEAD);
-        w.step(v, static_cast<int>(i) + from + (n0 + k) * STEP, count(n0 + k));
+      for (int k = 0; k < AHEAD; k += 2) {
+        const int n0 = g * AHEAD + k;
+        if (n0 >= steps) break;
+        float2 v[2][P];
+        values(n0, next[k], v[0]);
+        values(n0 + 1, next[k + 1], v[1]);
+        next[k] = fetch(n0 + AHEAD);
+        next[k + 1] = fetch(n0 + 1 + AHEAD);
+        const float top = fmaxf(top_of(v[0]), top_of(v[1]));
+        add_exps(soft, c, v, top);
+        most_here = fmaxf(most_here, top);
       }
     }
-  };
-  // A floor before the first step: the n-th largest of the threads' maxima of it.  For long strips
-  // another one after eight steps: the n-th largest of the warps' lists.
-  constexpr int FIRST = 8;
-  if constexpr (Q == 1) {
-    int top = kEmpty;
-    if (count(0) > 0) {
-      float v[E];
-      values(0, next[0], v);
-      float m = v[0];
-#pragma unroll
-      for (int e = 1; e < E; ++e) m = fmaxf(m, v[e]);
-      top = order_of(m);
-    }
-    keys[0][threadIdx.x] = sorted_down(top, lane);
-    __syncthreads();
-    w.floor = nth_of_lists(keys[0], n, lane);
+    maxima[at][threadIdx.x] = most_here;
+    most = fmaxf(most, most_here);
   }
-  run(0, steps < FIRST ? steps : FIRST);
-  if constexpr (Q == 1)
-    if (strip >= 2 * FIRST * STEP) {  // the same for all warps
-      keys[1][threadIdx.x] = lane < n ? w.best.key[0] : kEmpty;
-      __syncthreads();
-      w.floor = max(w.floor, nth_of_lists(keys[1], n, lane));
-    }
-  run(FIRST, steps);
+  // The n-th largest of the threads' maxima: n elements of the CTA's part are at least that.  A warp
+  // sorts its own, and each finds its rank among all by bisection of the other warps' lists.
+  const int key = sorted_down(order_of(most), lane);
+  keys[threadIdx.x] = key;
+  __syncthreads();
+  int rank = lane;
 #pragma unroll
-  for (int q = 0; q < Q; ++q) lists[warp][q * 32 + lane] = make_int2(w.best.key[q], w.best.at[q]);
+  for (int o = 1; o < kWarps; ++o) {
+    const int other = (warp + o) % kWarps;
+    const int* list = keys + other * 32;
+    const int least = other < warp ? key : key + 1;  // the lower warp's first
+    int low = 0;  // entries that stand before
+#pragma unroll
+    for (int step = 16; step > 0; step /= 2)
+      if (list[low + step - 1] >= least) low += step;
+    rank += low + (low == 31 && list[31] >= least ? 1 : 0);
+  }
+  if (rank == n - 1) floor = key;
+  __syncthreads();
+  // The elements that may be among the n best, by places.
+  Best<Q> best;
+  best.start(n);
+  float least;  // elements below it do not count; one that equals the list's last entry comes too late
+  auto set_least = [&](int k) { least = k <= order_of(-INFINITY) ? -INFINITY : value_of(k); };
+  set_least(floor);
+  // `has` lanes' elements v at place + lane
+  auto offer = [&](float v, int place, int has) {
+    best.offer(order_of(v), place + lane, lane < has && v >= least, lane);
+    set_least(max(best.last + 1, floor));
+  };
+  if (head) offer(first[0][0].x, static_cast<int>(start), static_cast<int>(head));
+  for (int g = 0, at = 0; g < groups; g += chunk, ++at) {
+    if (!__any_sync(~0u, maxima[at][threadIdx.x] >= least)) continue;
+    const int till = min((g + chunk) * AHEAD, steps);
+    for (int n0 = g * AHEAD; n0 < till; ++n0) {
+      float2 v[P];
+      values(n0, fetch(n0), v);
+      // the lanes that have some, one after the other: its elements to the first E lanes
+      unsigned todo = __ballot_sync(~0u, top_of(v) >= least);
+      for (; todo; todo &= todo - 1) {
+        const int of = __ffs(todo) - 1;
+        float mine = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float f = __shfl_sync(~0u, e % 2 ? v[e / 2].y : v[e / 2].x, of);
+          if (lane == e) mine = f;
+        }
+        const int here = n0 * STEP + of * E;
+        offer(mine, static_cast<int>(i) + here, min(size - here, E));
+      }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < Q; ++q) lists[warp][q * 32 + lane] = make_int2(best.key[q], best.at[q]);
 #pragma unroll
   for (int bit = 1; bit < 32; bit *= 2) {
     Soft o;
-    o.m = __shfl_xor_sync(~0u, w.soft.m, bit);
-    o.s = __shfl_xor_sync(~0u, w.soft.s, bit);
-    o.low = __shfl_xor_sync(~0u, w.soft.low, bit);
-    const float m = fmaxf(w.soft.m, o.m);
-    raise(w.soft, m);
+    o.m = __shfl_xor_sync(~0u, soft.m, bit);
+    o.s = __shfl_xor_sync(~0u, soft.s, bit);
+    o.low = __shfl_xor_sync(~0u, soft.low, bit);
+    const float m = fmaxf(soft.m, o.m);
+    raise(soft, m);
     raise(o, m);
-    add_to(w.soft, o.s);
-    w.soft.low += o.low;
+    add_to(soft, o.s);
+    soft.low += o.low;
   }
-  if (lane == 0) softs[warp] = w.soft;
+  if (lane == 0) softs[warp] = soft;
   __syncthreads();
   if (warp != 0) return;
   for (int o = 1; o < kWarps; ++o) {
+    if constexpr (Q == 1) {
+      best.join(lists[o], lane);
+    } else {
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int2 c = lists[o][q * 32 + lane];
-      w.best.offer(c.x, c.y, q * 32 + lane < n && c.x != kEmpty, lane);
+      for (int q = 0; q < Q; ++q) {
+        const int2 c = lists[o][q * 32 + lane];
+        best.offer(c.x, c.y, q * 32 + lane < n && c.x != kEmpty, lane);
+      }
     }
     Soft s = softs[o];
-    const float m = fmaxf(w.soft.m, s.m);
-    raise(w.soft, m);
+    const float m = fmaxf(soft.m, s.m);
+    raise(soft, m);
     raise(s, m);
-    add_to(w.soft, s.s);
-    w.soft.low += s.low;
+    add_to(soft, s.s);
+    soft.low += s.low;
   }
   int2* out = a.best + static_cast<int64_t>(blockIdx.x) * n;
 #pragma unroll
   for (int q = 0; q < Q; ++q)
-    if (q * 32 + lane < n) out[q * 32 + lane] = make_int2(w.best.key[q], w.best.at[q]);
-  if (lane == 0) a.sums[blockIdx.x] = make_float2(w.soft.m, w.soft.s + w.soft.low);
+    if (q * 32 + lane < n) out[q * 32 + lane] = make_int2(best.key[q], best.at[q]);
+  if (lane == 0) a.sums[blockIdx.x] = make_float2(soft.m, soft.s + soft.low);
 }
 
 // One CTA for each request.  A warp joins a beam's parts and writes the beam's best with their
@@ -323,28 +364,28 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(const BeamSelectArg
   grid_dependency_wait();
   for (int k = warp; k < beams; k += kWarps) {
     const int64_t first = (b * beams + k) * a.parts;
+    float score;
+    const bool ended = beam_done(a, b, k, &score), read = !ended && fabsf(score) < INFINITY;  // the parts are there
+    const int64_t parts = read ? a.parts : 0, entries = parts * n;
     Best<Q> best;
     best.start(n);
     float m = -INFINITY;
-    for (int64_t p = lane; p < a.parts; p += 32) m = fmaxf(m, a.sums[first + p].x);
+    for (int64_t p = lane; p < parts; p += 32) m = fmaxf(m, a.sums[first + p].x);
 #pragma unroll
     for (int bit = 1; bit < 32; bit *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, bit));
     double s = 0.0;
-    for (int64_t p = lane; p < a.parts; p += 32) {
+    for (int64_t p = lane; p < parts; p += 32) {
       const float2 v = a.sums[first + p];
       s += static_cast<double>(v.y) * exp2(static_cast<double>(scale_of(v.x)) - scale_of(m));
     }
 #pragma unroll
     for (int bit = 1; bit < 32; bit *= 2) s += __shfl_xor_sync(~0u, s, bit);
     const double lse = m + log(s) + (scale_of(m) - static_cast<double>(m) * kLog2e) * 0.69314718055994531;
-    const int64_t entries = a.parts * n;
     for (int64_t e = lane; e - lane < entries; e += 32) {
       const int2 c = e < entries ? a.best[first * n + e] : make_int2(kEmpty, INT_MAX);
       if (e < 32) best.fill(c.x, c.y, lane);
       else best.offer(c.x, c.y, c.x != kEmpty, lane);
     }
-    const float score = a.scores[b * a.scores_s0 + k * a.scores_s1];
-    const bool ended = a.finished && a.finished[b * a.finished_s0 + k * a.finished_s1];
     // a row that is no distribution (a NaN, an infinity, nothing left) offers nothing
     const bool sound = fabsf(score) < INFINITY && (ended || fabs(lse) < INFINITY);
 #pragma unroll

@@ -43,10 +43,13 @@ cc1d_status check_select(const cc1d_beam_select_params* p, BeamSelectArgs* a) {
   a->out_scores = p->out_scores;
   a->parents = p->parents;
   a->tokens = p->tokens;
-  // As many CTAs as run at a time (four on an SM), each with at least 2048 elements of a row: 512
-  // rows of 128000 take 78 us in one part and 83 us in two, of which some wait for the others.
-  const int64_t rows = p->batch * p->beams, want = rows > 0 ? 4 * sm_count() / rows : 1;
-  a->parts = std::max<int64_t>(1, std::min(want, (p->vocab + 2047) / 2048));
+  // As many CTAs as run at a time, but no part so short that joining the parts' lists takes longer
+  // than it saves: 1024 elements for each candidate.  512 rows of 128000 take 53 us in one part and
+  // 58 in two.  Parts of 2048, 1024 n and 2048 n elements: 4 rows of 32000, n = 4: 12.5, 11.1, 11.6 us;
+  // 16 rows of 128000, n = 32: 45.8, 24.7, 26.3; 8 rows, n = 16: 37.6, 21.0, 20.6.
+  const int64_t rows = p->batch * p->beams, want = rows > 0 ? kBeamCtas * sm_count() / rows : 1;
+  const int64_t least = std::max<int64_t>(2048, 1024 * p->candidates);
+  a->parts = std::max<int64_t>(1, std::min(want, (p->vocab + least - 1) / least));
   a->part = (p->vocab + a->parts - 1) / a->parts;
   a->part = (a->part + 7) / 8 * 8;
   a->parts = (p->vocab + a->part - 1) / a->part;

@@ -24,6 +24,7 @@ struct BeamSelectArgs {
   float2* sums;
 };
 
+constexpr int kBeamCtas = 4;      // CTAs of the selection's first kernel on an SM
 constexpr int kBeamTensors = 24;  // tensors of one reordering launch
 
 // Rows that follow the beams.  Row r starts at data + r * row_bytes.  A row is `columns` units of

@@ -57,6 +57,26 @@ def test_large():
     _select_and_check(logits, scores, n=16)
 
 
+@pytest.mark.parametrize("kind", ["any", "masked", "rising", "few values"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_rows(dtype, kind):
+    """Rows of several steps in each part of a strip, whose largest elements stand at the end, at few places or at many."""
+    logits, scores = _case(5, 300, 1, 300_001, dtype)
+    if kind == "masked":
+        kept = torch.rand(logits.shape, generator=_gen(6), device="cuda") < 1e-5
+        logits.masked_fill_(~kept, -INF)
+    elif kind == "rising":
+        logits = torch.sort(logits, dim=-1).values
+    elif kind == "few values":
+        logits = logits.round()
+    finished = torch.zeros(300, 1, dtype=torch.bool, device="cuda")
+    finished[::7] = True
+    logits[::7, 0, 1000:] = float("nan")  # not looked at
+    scores[1::7] = -INF
+    logits[1::7] = float("inf")
+    _select_and_check(logits, scores, finished, 3, n=33 if kind == "any" else 8)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_ties_go_to_the_lowest_place(dtype):
     logits = torch.zeros(2, 3, 500, device="cuda", dtype=dtype)
