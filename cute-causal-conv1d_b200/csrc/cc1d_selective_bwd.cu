@@ -17,9 +17,9 @@
 // over CTAs by a second kernel, all in a fixed order: two calls give the same bits.
 //
 // What bounds it: an element takes two exponentials (238 us for the 537 M elements of 4 x 4096 x 2048
-// x 16, which takes 1197; its memory 82) and 28 instructions, most of them the gradients' FMAs and the
+// x 16, which takes 1188; its memory 82) and 28 instructions, most of them the gradients' FMAs and the
 // exchanges that sum dB, dC over channels and ds, dx over states.  Eight warps an SM are what the
-// registers leave; a scheduler issues .35 a cycle.  Of the 1197 us the pass to the states takes 180,
+// registers leave; a scheduler issues .35 a cycle.  Of the 1188 us the pass to the states takes 180,
 // the gradients 570 (their sums over channels 180, over states 100), and what is done once per
 // position and channel (step sizes, gates, loads, stores) 440.
 //
@@ -468,26 +468,40 @@ __global__ void __launch_bounds__(kSelThreads, kBwdCtas) sel_bwd_kernel(const __
   if (!ENDS && mine > 1) d[a.dim + 1] = two.y;
 }
 
-// dB and dC: the sums over a group's CTAs.  A thread takes one state of one position.
+// dB and dC: the sums over a group's CTAs.  Four threads take four states of a position, each of them
+// every fourth CTA, in loads of 16 bytes of which eight are on their way.  One state and all CTAs a
+// thread made the backward of 4 x 4096 x 1024 x 16 take 613 us, this 599.
+constexpr int kSumQuads = kThreads / 4;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sel_sum_bc_kernel(const __grid_constant__ SelArgs a) {
   grid_dependency_wait();
-  const int64_t per = 2 * a.padded, rows = a.group_tiles;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= a.launch_rows * a.seqlen * a.groups * per) return;
-  const int64_t v = i % per, r = i / per, g = r % a.groups, bt = r / a.groups;
+  const int64_t per = 2 * a.padded, quads = per / 4, rows = a.group_tiles;
+  const int lane = threadIdx.x & 31, share = lane >> 3;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kSumQuads + (threadIdx.x >> 5) * 8 + (lane & 7);
+  const bool is = i < a.launch_rows * a.seqlen * a.groups * quads;
+  const int64_t v = is ? i % quads * 4 : 0, r = is ? i / quads : 0, g = r % a.groups, bt = r / a.groups;
   const float* part = a.parts_bc + (bt * a.tiles + g * rows) * per + v;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
-  int64_t k = 0;
-#pragma unroll 4
-  for (; k + 4 <= rows; k += 4)
+  if (is) {
+#pragma unroll 8
+    for (int64_t k = share; k < rows; k += 4) {
+      const float4 p = *reinterpret_cast<const float4*>(part + k * per);
+      s[0] += p.x;
+      s[1] += p.y;
+      s[2] += p.z;
+      s[3] += p.w;
+    }
+  }
+  float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] += part[(k + e) * per];
-  for (; k < rows; ++k) s[0] += part[k * per];
-  const float sum = (s[0] + s[1]) + (s[2] + s[3]);
+  for (int e = 0; e < 4; ++e) {
+    s[e] += __shfl_xor_sync(~0u, s[e], 8);
+    s[e] += __shfl_xor_sync(~0u, s[e], 16);
+    if (e == share) sum = s[e];
+  }
   const bool is_c = v >= a.padded;
-  const int64_t n = is_c ? v - a.padded : v;
-  if (n >= a.dstate) return;
+  const int64_t n = (is_c ? v - a.padded : v) + share;
+  if (!is || n >= a.dstate) return;
   const TensorArg& t = is_c ? a.dC : a.dB;
   static_cast<T*>(t.data)[(a.row0 + bt / a.seqlen) * t.s0 + g * (is_c ? a.dC_group : a.dB_group) + n * t.s1 + (bt % a.seqlen) * t.s2] = from_f32<T>(sum);
 }
@@ -549,10 +563,10 @@ cudaError_t run(const SelArgs& all, cudaStream_t s) {
   const int64_t params = a.dim * (a.padded + 2);
   for (a.row0 = 0; e == cudaSuccess && a.row0 < a.batch; a.row0 += all.launch_rows) {
     if (a.launch_rows > a.batch - a.row0) a.launch_rows = a.batch - a.row0;
-    const int64_t bc = a.launch_rows * a.seqlen * a.groups * 2 * a.padded;
+    const int64_t quads = a.launch_rows * a.seqlen * a.groups * a.padded / 2;
     e = walk<T>(a, s);
     if (e == cudaSuccess)
-      e = launch_dependent(sel_sum_bc_kernel<T>, dim3(static_cast<unsigned>((bc + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);
+      e = launch_dependent(sel_sum_bc_kernel<T>, dim3(static_cast<unsigned>((quads + kSumQuads - 1) / kSumQuads)), dim3(kThreads), 0, s, a);
   }
   if (e == cudaSuccess)
     e = launch_dependent(sel_sum_params_kernel, dim3(static_cast<unsigned>((params + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);

@@ -10,11 +10,11 @@
 // shared memory as fp32; the next tile's inputs are on their way to registers, as the words that
 // they arrive in, meanwhile.
 //
-// What bounds it: an element of h takes one exponential (MUFU, 16 a cycle and SM) and about six
-// instructions in all, two values at a time where sm_100a can.  4 x 4096 x 2048 x 16 bf16 with z
-// (537 M elements, 268 MB without the checkpoints) takes 318 us: its exponentials alone 119, its
-// memory 41.  Its 512 CTAs are 3.5 an SM, so the longest wait is a thread's chain of dependent
-// positions; the MUFU is busy 47 % of the time.
+// What bounds it: an element of h takes one exponential (MUFU, 16 a cycle and SM) and about eleven
+// instructions in all, a third of them for what is done once per position and channel.  4 x 4096 x
+// 2048 x 16 bf16 with z (537 M elements, 268 MB without the checkpoints) takes 318 us: its
+// exponentials alone 119, its memory 41.  Its 512 CTAs are 3.5 an SM, so the longest wait is a
+// thread's chain of dependent positions; a scheduler issues .55 a cycle, the MUFU is busy 48 % of it.
 //
 // Eight positions are unrolled, with their loads first.  Two channels a thread took 502 us (half the
 // warps), three tiles in flight in one unrolled loop 420 to 550 (the instruction cache), 64 or 96
