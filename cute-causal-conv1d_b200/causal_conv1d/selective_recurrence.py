@@ -71,7 +71,8 @@ def selective_recurrence_update(x, state, delta, A, B, C, D=None, z=None, delta_
     fp32, or with state_indices (batch,) a pool (nstates, dim, dstate) of which batch row b uses
     row state_indices[b]; an index outside the pool is padding (zero output, no state touched),
     and no row may be named twice.  The indices are int32; other signed integers and uint8 are
-    converted.  The rest is as in :func:`selective_recurrence_fn`.  Returns out with x's shape.
+    converted.  No two elements of state may lie at one place, as an expanded tensor's do.  The
+    rest is as in :func:`selective_recurrence_fn`.  Returns out with x's shape.
 
     It has no derivative: a backward pass that reaches out raises, a state that requires grad
     is refused outside torch.no_grad(), and the state never carries a graph.

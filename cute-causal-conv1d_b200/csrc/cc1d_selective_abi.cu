@@ -38,6 +38,20 @@ cc1d_status check_common(const P* p) {
   return CC1D_OK;
 }
 
+// The elements of a tensor that is written lie at places of their own, each dimension beyond the reach
+// of those with smaller strides.
+bool apart(const cc1d_tensor& t, int64_t n0, int64_t n1, int64_t n2) {
+  struct { int64_t size, step; } d[3] = {{n0, t.stride[0]}, {n1, t.stride[1]}, {n2, t.stride[2]}};
+  std::sort(d, d + 3, [](const auto& a, const auto& b) { return a.step < b.step; });
+  int64_t reach = 1;
+  for (const auto& e : d) {
+    if (e.size <= 1) continue;
+    if (e.step < reach) return false;
+    reach = e.step * e.size;
+  }
+  return true;
+}
+
 cc1d_status check(const cc1d_selective_params* p, bool bwd, SelArgs* a) {
   if (!p) return fail(CC1D_ERR_VALUE, "params is NULL");
   const cc1d_status st = check_common(p);
@@ -287,6 +301,7 @@ cc1d_status cc1d_selective_update_launch(const cc1d_selective_update_params* p, 
   CC1D_REQUIRE(p->C, "C");
   CC1D_REQUIRE(p->out, "out");
   if (p->nstates > 0) CC1D_REQUIRE(p->state, "state");
+  if (!apart(p->state, p->nstates, p->dim, p->dstate)) return fail(CC1D_ERR_VALUE, "the state's elements must not overlap");
   if (static_cast<double>(p->batch) * p->dim * 32 / kThreads > kMax31)
     return fail(CC1D_ERR_VALUE, "batch * dim is too large");
   SelUpdateArgs a;

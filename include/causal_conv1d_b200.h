@@ -442,7 +442,7 @@ cc1d_status cc1d_selective_bwd_launch(const cc1d_selective_params* params, void*
 /* ----------------------------------------------- selective recurrence, decoding
  * The same recurrence for a few tokens of each row against a pool of states.
  *   x, delta, z, out, A, B, C, D, bias    as above
- *   state           (nstates, dim, dstate) fp32  updated in place
+ *   state           (nstates, dim, dstate) fp32  updated in place; its elements must not overlap
  *   state_indices   (batch,) int32               optional: state row of each batch row; a row outside
  *                                                [0, nstates) is padding: out = 0, no state is touched.
  *                                                Two batch rows must not name the same state row.

@@ -301,6 +301,8 @@ def test_selective_abi_refusals_need_no_gpu():
     _refused(upd, update(sizes=(2, 2, 1, 3, 1, 3), **ins, state=t, out=t), 1, b"one state")
     _refused(upd, update(**ins, out=t), 1, b"state is required")
     _refused(upd, update(sizes=(2, 2, 1, 300, 1, 2), **ins, state=t, out=t), 1, b"dstate")
+    for strides in ((0, 3, 1), (6, 0, 1), (6, 3, 0), (6, 2, 1), (5, 3, 1), (1, 1, 1), (-6, 3, 1)):
+        _refused(upd, update(**ins, state=_tensor(strides=strides), out=t), 1, b"overlap")
     assert upd(update(sizes=(0, 2, 1, 3, 1, 0)), None) == 0
 
 
