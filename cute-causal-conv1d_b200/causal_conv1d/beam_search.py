@@ -55,8 +55,10 @@ def beam_search_select_ref(logits, scores, finished=None, end_token=None, num_ca
     """PyTorch statement of :func:`beam_search_select`, in fp64."""
     batch, beams, vocab = logits.shape
     x = logits.double()
-    logp = x - torch.logsumexp(x, -1, keepdim=True)
-    sound = torch.isfinite(torch.logsumexp(x, -1))
+    top = x.amax(-1, keepdim=True)  # taken off first: a large one would swallow the sum
+    above = torch.log(torch.exp(x - top).sum(-1, keepdim=True))
+    logp = x - top - above
+    sound = torch.isfinite(above.squeeze(-1))
     if finished is not None:
         only = torch.full((vocab,), float("-inf"), dtype=x.dtype, device=x.device)
         only[end_token] = 0.0

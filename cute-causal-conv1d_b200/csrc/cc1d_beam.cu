@@ -115,16 +115,28 @@ struct Best {
   }
 };
 
-// The running maximum m and sum s + low of 2^(x L - c), L = kLog2e, of a lane or a part of a row.
-// c = m L as it is rounded (0 before there is an m): one multiply-add makes the exponent, and
-// log sum exp(x) = m + log(sum) + (c - m L) log(2) puts the rounding back.
+// The sum s + low of 2^(x L - r), L = kLog2e, of a lane or a part of a row.  m is an element that none
+// exceeds by more than kRise: rows that rise would else scale their sums down hundreds of times, each
+// time off by a rounding.  The reference r is m L as it is rounded, c, where |m| is at most 2^20: one
+// multiply-add makes the exponent, and c is off by at most 2^-4, so that no sum leaves the normal numbers;
+// log sum exp(x) = m + (log2(sum) + r - m L) log(2) puts the rounding back.  Beyond that the rounding
+// would be of any size, and m L itself may overflow: there r is m L, and the exponent (x - m) L.
 struct Soft {
   float m = -INFINITY, s = 0.f, low = 0.f;
 };
-__device__ __forceinline__ float scale_of(float m) { return m > -INFINITY ? m * kLog2e : 0.f; }
+constexpr float kRise = 4.f, kMostFused = 1048576.f;
+__device__ __forceinline__ bool is_fused(float m) { return fabsf(m) <= kMostFused; }
+// c, or none; rounded wherever it is used (a product is otherwise joined with the sum behind it)
+__device__ __forceinline__ float scale_of(float m) { return is_fused(m) ? __fmul_rn(m, kLog2e) : 0.f; }
+__device__ __forceinline__ float rest_of(float m) { return is_fused(m) ? fmaf(-m, kLog2e, scale_of(m)) : 0.f; }  // r - m L
+__device__ __forceinline__ double reference_of(float m) {
+  return is_fused(m) ? static_cast<double>(scale_of(m)) : static_cast<double>(m) * kLog2e;
+}
 __device__ __forceinline__ void raise(Soft& a, float m) {
   if (m > a.m) {
-    const float f = a.m > -INFINITY ? ex2_approx(scale_of(a.m) - scale_of(m)) : 0.f;
+    float f = 0.f;
+    if (is_fused(a.m) && is_fused(m)) f = ex2_approx(scale_of(a.m) - scale_of(m));
+    else if (a.m > -INFINITY) f = ex2_approx(fmaf(a.m - m, kLog2e, rest_of(a.m) - rest_of(m)));
     a.s *= f;
     a.low *= f;
     a.m = m;
@@ -145,12 +157,24 @@ __device__ __forceinline__ float top_of(const float2 (&x)[P]) {
   for (int p = 1; p < P; ++p) top = fmaxf(top, fmaxf(x[p].x, x[p].y));
   return top;
 }
-// Adds the exponentials of 2 P H elements, of which `top` is the largest; c = scale_of(a.m).
+// Adds the exponentials of 2 P H elements, of which `top` is the largest; c = scale_of(a.m).  Steps whose
+// top is not above `limit` need nothing else: the limit is kRise above m, or, where m is beyond 2^20 and
+// c is 0, below everything, and the elements become their difference from m.
 template <int H, int P>
-__device__ __forceinline__ void add_exps(Soft& a, float& c, const float2 (&x)[H][P], float top) {
-  if (top > a.m) {
-    raise(a, top);
-    c = scale_of(top);
+__device__ __forceinline__ void add_exps(Soft& a, float& c, float& limit, float2 (&x)[H][P], float top) {
+  if (top > limit) {
+    if (top > a.m + kRise) {
+      raise(a, top);
+      c = scale_of(top);
+    }
+    limit = a.m + kRise;
+    if (!is_fused(a.m)) {
+      limit = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int p = 0; p < P; ++p) x[h][p] = fadd2(x[h][p], make_float2(-a.m, -a.m));
+    }
   }
   float2 s[H * P];
 #pragma unroll
@@ -235,9 +259,12 @@ __global__ void __launch_bounds__(kThreads, kBeamCtas) beam_parts_kernel(const B
   if (ended || !(fabsf(score) < INFINITY)) return;
   // The sums, and the largest element of each lane in each of up to kChunks chunks of the strip.
   Soft soft;
-  float c = 0.f, most = -INFINITY;
-  const float2 first[1][1] = {{make_float2(lane < head ? to_f32(x[start + lane]) : -INFINITY, -INFINITY)}};
-  if (head) add_exps(soft, c, first, first[0][0].x);
+  float c = 0.f, limit = -INFINITY, most = -INFINITY;
+  const float first = lane < head ? to_f32(x[start + lane]) : -INFINITY;
+  if (head) {
+    float2 v[1][1] = {{make_float2(first, -INFINITY)}};
+    add_exps(soft, c, limit, v, first);
+  }
   const int groups = (steps + AHEAD - 1) / AHEAD, chunk = (groups + kChunks - 1) / kChunks;
   for (int g = 0, at = 0; g < groups; ++at) {
     float most_here = -INFINITY;
@@ -252,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, kBeamCtas) beam_parts_kernel(const B
         next[k] = fetch(n0 + AHEAD);
         next[k + 1] = fetch(n0 + 1 + AHEAD);
         const float top = fmaxf(top_of(v[0]), top_of(v[1]));
-        add_exps(soft, c, v, top);
+        add_exps(soft, c, limit, v, top);
         most_here = fmaxf(most_here, top);
       }
     }
@@ -289,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, kBeamCtas) beam_parts_kernel(const B
     best.offer(order_of(v), place + lane, lane < has && v >= least, lane);
     set_least(max(best.last + 1, floor));
   };
-  if (head) offer(first[0][0].x, static_cast<int>(start), static_cast<int>(head));
+  if (head) offer(first, static_cast<int>(start), static_cast<int>(head));
   for (int g = 0, at = 0; g < groups; g += chunk, ++at) {
     if (!__any_sync(~0u, maxima[at][threadIdx.x] >= least)) continue;
     const int till = min((g + chunk) * AHEAD, steps);
@@ -376,18 +403,20 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(const BeamSelectArg
     double s = 0.0;
     for (int64_t p = lane; p < parts; p += 32) {
       const float2 v = a.sums[first + p];
-      s += static_cast<double>(v.y) * exp2(static_cast<double>(scale_of(v.x)) - scale_of(m));
+      // a part without anything above -inf has the sum 0, or NaN
+      s += static_cast<double>(v.y) * (v.x > -INFINITY ? exp2(reference_of(v.x) - reference_of(m)) : 1.0);
     }
 #pragma unroll
     for (int bit = 1; bit < 32; bit *= 2) s += __shfl_xor_sync(~0u, s, bit);
-    const double lse = m + log(s) + (scale_of(m) - static_cast<double>(m) * kLog2e) * 0.69314718055994531;
+    // log sum exp(x) = m + above; m is taken from the logits first, since a large one would swallow the rest
+    const double above = log(s) + (reference_of(m) - static_cast<double>(m) * kLog2e) * 0.69314718055994531;
     for (int64_t e = lane; e - lane < entries; e += 32) {
       const int2 c = e < entries ? a.best[first * n + e] : make_int2(kEmpty, INT_MAX);
       if (e < 32) best.fill(c.x, c.y, lane);
       else best.offer(c.x, c.y, c.x != kEmpty, lane);
     }
     // a row that is no distribution (a NaN, an infinity, nothing left) offers nothing
-    const bool sound = fabsf(score) < INFINITY && (ended || fabs(lse) < INFINITY);
+    const bool sound = fabsf(score) < INFINITY && (ended || fabs(above) < INFINITY);
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int i = q * 32 + lane;
@@ -398,7 +427,7 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(const BeamSelectArg
         if (i == 0) total = score, token = static_cast<int>(a.end_token);
         else if (i <= a.end_token) token = i - 1;
       } else if (sound && best.key[q] != kEmpty) {
-        total = static_cast<double>(score) + (static_cast<double>(value_of(best.key[q])) - lse);
+        total = static_cast<double>(score) + (static_cast<double>(value_of(best.key[q])) - m - above);
         token = best.at[q];
       }
       totals[k * n + i] = total;
