@@ -273,7 +273,13 @@ cc1d_status cc1d_selective_bwd_launch(const cc1d_selective_params* p, void* stre
     if (a.dA && a.dim > 0) e = cudaMemsetAsync(a.dA, 0, a.dim * a.dstate * sizeof(float), s);
     if (e == cudaSuccess && a.dD && a.dim > 0) e = cudaMemsetAsync(a.dD, 0, a.dim * sizeof(float), s);
     if (e == cudaSuccess && a.dbias && a.dim > 0) e = cudaMemsetAsync(a.dbias, 0, a.dim * sizeof(float), s);
-    return launched(e, "selective recurrence zero fill", 0);
+    // without channels B and C reach nothing: the sums over no CTA
+    const bool sums = a.dim == 0 && a.batch > 0 && a.seqlen > 0 && a.dB.data && a.dC.data;
+    if (e == cudaSuccess && sums) {
+      if ((st = plan(&a, true)) != CC1D_OK) return st;
+      e = by_type(p->x.dtype, a, s, sel_bwd_f32, sel_bwd_f16, sel_bwd_bf16);
+    }
+    return launched(e, "selective recurrence zero fill", sums);
   }
   if ((st = plan(&a, true)) != CC1D_OK) return st;
   if ((st = workspace_ok(p->workspace, p->workspace_bytes, lay_out(&a, true, p->workspace))) != CC1D_OK) return st;

@@ -564,11 +564,11 @@ cudaError_t run(const SelArgs& all, cudaStream_t s) {
   for (a.row0 = 0; e == cudaSuccess && a.row0 < a.batch; a.row0 += all.launch_rows) {
     if (a.launch_rows > a.batch - a.row0) a.launch_rows = a.batch - a.row0;
     const int64_t quads = a.launch_rows * a.seqlen * a.groups * a.padded / 2;
-    e = walk<T>(a, s);
+    if (a.dim > 0) e = walk<T>(a, s);
     if (e == cudaSuccess)
       e = launch_dependent(sel_sum_bc_kernel<T>, dim3(static_cast<unsigned>((quads + kSumQuads - 1) / kSumQuads)), dim3(kThreads), 0, s, a);
   }
-  if (e == cudaSuccess)
+  if (e == cudaSuccess && a.dim > 0)
     e = launch_dependent(sel_sum_params_kernel, dim3(static_cast<unsigned>((params + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);
   return e;
 }

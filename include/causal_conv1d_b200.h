@@ -391,7 +391,8 @@ cc1d_status cc1d_add_norm_bwd_launch(const cc1d_add_norm_params* params, void* s
  * Without seq_idx nstates == batch.  At a padding position out is 0 and nothing that stands there is
  * used.  The gradients of out and of final_states give
  *   dx, ddelta, dz  (batch, dim, seqlen)            outputs, x's dtype (dz iff z)
- *   dB, dC          (batch, groups, dstate, seqlen) outputs, x's dtype, summed in a fixed order
+ *   dB, dC          (batch, groups, dstate, seqlen) outputs, x's dtype, summed in a fixed order; zero
+ *                                                   where dim is 0
  *   dinitial_states (nstates, dim, dstate) fp32     optional output; with seq_idx as final_states
  *   dA              (dim, dstate) fp32 dense        optional outputs, summed in a fixed order
  *   dD, dbias       (dim,) fp32 dense
