@@ -80,7 +80,7 @@ cc1d_status describe_rows(const cc1d_beam_rows& r, int64_t most_unit, BeamRows* 
   int m = n;
   if (r.rows > 1) all[m++] = {r.rows, r.row_stride * e};
   std::sort(all, all + m, by_step);
-  for (int64_t i = 0, reach = e; i < m; reach = all[i].step * all[i].size, ++i)
+  for (int64_t i = 0, reach = e; i < m; reach += all[i].step * (all[i].size - 1), ++i)  // up to the last element
     if (all[i].step < reach) return fail(CC1D_ERR_VALUE, "the states' elements must not overlap");
   std::sort(d, d + n, by_step);
   // an element is a run of bytes; runs that follow one another are one

@@ -47,7 +47,7 @@ bool apart(const cc1d_tensor& t, int64_t n0, int64_t n1, int64_t n2) {
   for (const auto& e : d) {
     if (e.size <= 1) continue;
     if (e.step < reach) return false;
-    reach = e.step * e.size;
+    reach += e.step * (e.size - 1);  // up to the last element
   }
   return true;
 }
