@@ -484,8 +484,9 @@ template <int BEAMS, typename U>
 __device__ __forceinline__ void move_column(const BeamReorderArgs& a, const BeamRows& t, int64_t column, const int* source, const int* target) {
   int64_t at = column * t.step0;
   if (t.size0 < t.columns) {
-    const int64_t rest = column / t.size0;
-    at += (rest % t.size1) * t.step1 + rest / t.size1 * t.step2 - rest * t.size0 * t.step0;
+    const int64_t rest = column / t.size0, outer = rest / t.size1;
+    at += (rest - outer * t.size1) * t.step1 - rest * t.size0 * t.step0;
+    at += outer < t.size2 ? outer * t.step2 : outer % t.size2 * t.step2 + outer / t.size2 * t.step3;
   }
   U v[BEAMS];
 #pragma unroll

@@ -93,21 +93,19 @@ cc1d_status describe_rows(const cc1d_beam_rows& r, int64_t most_unit, BeamRows* 
   fits(reinterpret_cast<uintptr_t>(r.data));
   if (r.rows > 1) fits(r.row_stride * e);
   for (int i = first; i < n; ++i) fits(d[i].step);
-  Dim out[3] = {{run / unit, unit}, {1, 0}, {1, 0}};
-  if (n - first < 3) {
-    for (int i = first; i < n; ++i) out[1 + i - first] = d[i];
-  } else {  // single elements in three dimensions
-    if (unit > e) unit = e;
-    if (unit < e) return fail(CC1D_ERR_NOT_IMPLEMENTED, "states of this layout must lie on their elements' size");
-    std::copy(d, d + 3, out);
-  }
+  // the run in its units, then what is left: four dimensions where three are of elements wider than a unit
+  Dim out[4] = {{1, 0}, {1, 0}, {1, 0}, {1, 0}};
+  const int outer = n - first == 3 && run == unit ? 0 : 1;
+  if (outer) out[0] = {run / unit, unit};
+  std::copy(d + first, d + n, out + outer);
   t->data = static_cast<char*>(r.data);
   t->rows = r.rows;
   t->row_bytes = r.row_stride * e;
   t->columns = total * e / unit;
   t->size0 = out[0].size, t->step0 = out[0].step;
   t->size1 = out[1].size, t->step1 = out[1].step;
-  t->step2 = out[2].step;
+  t->size2 = out[2].size, t->step2 = out[2].step;
+  t->step3 = out[3].step;
   t->unit = static_cast<int32_t>(unit);
   const int64_t blocks = (t->columns + kThreads - 1) / kThreads;
   if (blocks > kMax31) return fail(CC1D_ERR_VALUE, "a row is too large");

@@ -28,10 +28,11 @@ constexpr int kBeamCtas = 4;      // CTAs of the selection's first kernel on an 
 constexpr int kBeamTensors = 24;  // tensors of one reordering launch
 
 // Rows that follow the beams.  Row r starts at data + r * row_bytes.  A row is `columns` units of
-// `unit` bytes; unit u lies at (u % size0) * step0 + (u / size0 % size1) * step1 + (u / size0 / size1) * step2.
+// `unit` bytes in up to four dimensions: unit u = ((i3 size2 + i2) size1 + i1) size0 + i0 lies at
+// i0 step0 + i1 step1 + i2 step2 + i3 step3.
 struct BeamRows {
   char* data;
-  int64_t rows, row_bytes, columns, size0, size1, step0, step1, step2;
+  int64_t rows, row_bytes, columns, size0, size1, size2, step0, step1, step2, step3;
   int32_t unit, blocks;  // blocks: CTAs of one request
 };
 

@@ -52,3 +52,18 @@ def test_reorder(dtype):
         before, want = whole.clone(), beam_search_reorder_ref(state, parents)
         beam_search_reorder(state, parents)
         assert torch.equal(state, want) and torch.equal(whole[~inside], before[~inside])
+
+
+@pytest.mark.parametrize("beams", [2, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.float16, torch.float32, torch.float64, torch.complex128])
+def test_reorder_elements_in_three_dimensions(dtype, beams):
+    """Single elements of any size, with fewer and with more beams than move whole elements."""
+    values = torch.randint(0, 200, (2 * beams, 5, 12, 13), generator=_gen(beams), device="cuda").to(dtype)
+    wide = values[:, ::2, ::3, ::2]
+    parents = torch.randint(0, beams, (2, beams), generator=_gen(1), device="cuda")
+    for state in (wide, values.flatten()[1:1 + 2 * beams * 64].view(2 * beams, 64)[:, :60].unflatten(1, (5, 3, 4))[..., ::2]):
+        before, rest = values.clone(), torch.ones_like(values, dtype=torch.bool)
+        rest.as_strided(state.shape, state.stride(), state.storage_offset()).fill_(False)
+        want = beam_search_reorder_ref(state, parents)
+        beam_search_reorder(state, parents)
+        assert torch.equal(state, want) and torch.equal(values[rest], before[rest])
