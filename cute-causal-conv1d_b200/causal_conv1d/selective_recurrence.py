@@ -54,6 +54,11 @@ def selective_recurrence_fn(x, delta, A, B, C, D=None, z=None, delta_bias=None, 
     sequence, its id the row of initial_states and final_states; a negative id is padding, whose
     out is 0 and where nothing is used; a sequence without positions keeps its initial state.
 
+    Memory of training, for each position and channel, beside the inputs: dstate / 8 bytes (dstate / 4
+    up to 8 states, dstate / 2 up to 4) are kept until the backward pass, which takes about 4 bytes of
+    scratch at 16 states, 16 at 32 and dstate bytes at 64 and more, of as many batch rows as 2 GB hold,
+    but of one row at least.
+
     Gradients flow back to x, delta, A, B, C, D, z, delta_bias and initial_states; they are
     summed in a fixed order.  There is no second derivative and no forward-mode one: both raise.
     """

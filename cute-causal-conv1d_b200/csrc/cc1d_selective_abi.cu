@@ -193,8 +193,10 @@ cc1d_status plan(SelArgs* a, bool bwd) {
                                     bwd ? &a->ddelta : nullptr, bwd ? &a->dz : nullptr};
   for (const TensorArg* t : moved)
     if (t && t->data) a->pairs = a->pairs && pairs_ok(*t, *a);
-  // The backward's sums of dB and dC take 8 padded / CTA's channels bytes per element, so that many
-  // states of a large batch would take more than the tensors: as many batch rows at a time as 2 GB hold.
+  // The backward's sums of dB and dC take 8 padded bytes for each position and CTA, which has 128 / lanes
+  // channels: 4 bytes for each position and channel at 16 states, 16 at 32, 64 at 64, 256 at 256.  So that a
+  // large batch does not take more than its tensors, as many rows go at a time as 2 GB hold.  One row always
+  // goes as a whole, and may take more: 8.6 GB for 8192 channels x 16384 positions x 64 states.
   const double row_bytes = 8.0 * a->seqlen * a->tiles * a->padded;
   a->row0 = 0;
   a->launch_rows = bwd && row_bytes * a->batch > 2e9 ? std::max<int64_t>(1, static_cast<int64_t>(2e9 / row_bytes)) : a->batch;

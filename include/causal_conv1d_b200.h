@@ -387,7 +387,9 @@ cc1d_status cc1d_add_norm_bwd_launch(const cc1d_add_norm_params* params, void* s
  *                   of 4) fp32 contiguous, 16-byte aligned: h before each chunk; written by the
  *                   forward if given, read by the backward
  *   workspace       device scratch of cc1d_selective_{fwd,bwd}_workspace_bytes(params) bytes, 16-byte
- *                   aligned, contents need not be initialised
+ *                   aligned, contents need not be initialised.  The backward takes, for each position
+ *                   and channel of a batch row, about 4 bytes at 16 states, 16 at 32 and dstate bytes at
+ *                   64 and more, of as many rows as 2 GB hold, but of one row at least
  * Without seq_idx nstates == batch.  At a padding position out is 0 and nothing that stands there is
  * used.  The gradients of out and of final_states give
  *   dx, ddelta, dz  (batch, dim, seqlen)            outputs, x's dtype (dz iff z)
