@@ -8,8 +8,10 @@ namespace cc1d {
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// softplus(u) = max(u, 0) + log(1 + e) with e = exp(-|u|), to full relative precision for u of any
-// size, NaN included, for two values.  log(1 + e) = 2 atanh(s) with s = e / (2 + e) <= 1/3, and
+// softplus(u) = max(u, 0) + log(1 + e) with e = exp(-|u|), for two values of any size, NaN included: within
+// 2^-20 of itself (e 2^-22, the reciprocal 2^-23, five roundings), and (2^-24 + 2^-26) |u| more for 16-bit
+// tensors, whose e keeps the rounding of its exponent.  Below 2^-126, u < -87.3, it is zero, as is e.
+// log(1 + e) = 2 atanh(s) with s = e / (2 + e) <= 1/3, and
 // 2 atanh(s) / s in w = s^2 <= 1/9 by the polynomial that interpolates it at five Chebyshev points
 // (off by 4e-9).
 __device__ __forceinline__ float2 softplus_of_exp(float2 u, float2 e) {
@@ -22,7 +24,7 @@ __device__ __forceinline__ float2 softplus_of_exp(float2 u, float2 e) {
   q = ffma2(q, w, both(2.f));
   return ffma2(s, q, make_float2(fmaxf(u.x, 0.f), fmaxf(u.y, 0.f)));
 }
-// exp(-|u|); for 16-bit tensors the rounding of the exponent is left in it (|u| 2^-24 of it).
+// exp(-|u|); for 16-bit tensors the roundings of the exponent and of log2(e) are left in it, (2^-24 + 2^-26) |u| of it.
 template <typename T>
 __device__ __forceinline__ float2 exp_of_size(float2 u) {
   if constexpr (std::is_same<T, float>::value)
