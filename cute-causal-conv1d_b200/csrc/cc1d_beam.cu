@@ -17,13 +17,14 @@ namespace {
 // largest of the threads' maxima is a floor of the best n; the few chunks that reach it (about n of a
 // CTA's) are read again, and the elements above it enter a sorted list of each warp, one or two entries
 // a lane.  The warps' lists are joined, and a second kernel joins those of a row's parts, then ranks
-// the beams' lists.  Beams that are at their end, or not in use, are not read.
+// the beams' lists.  Beams that are at their end, or not in use, are not walked.
 //
-// What bounds it: 512 rows of 128000 bf16 logits (131 MB, 20 us of memory) take 53 us, 7 instructions
-// an element in the walk (one exponential, 15 us of all) and chains of exchanges behind it; with lists
-// kept during the walk 66 us, and with a floor from its first step alone 116.  Four rows of 32000 take
-// 11 us: two kernels of which the second waits for the first, and in them exchanges and barriers
-// rather than data.
+// What bounds it: 512 rows of 128000 bf16 logits (131 MB, 20 us of memory) take 53 us, of which the join
+// takes 11: 12.8 instructions an element in walk, second look and lists (one exponential, 15 us of all),
+// and chains of exchanges; with lists kept during the walk 66 us, and with a floor from its first step
+// alone 116.  Beyond the 592 CTAs that run at a time rows wait for a second wave: 592 rows take 54 us,
+// 600 take 75, 1024 take 90.  Four rows of 32000 take 12 us: two kernels of which the second waits for
+// the first, and in them exchanges and barriers rather than data.
 constexpr int kWarps = kThreads / 32;
 constexpr int kAhead = 2, kChunks = 32;
 constexpr int kEmpty = INT_MIN;  // below the order of every float
@@ -209,8 +210,8 @@ __device__ __forceinline__ bool beam_done(const BeamSelectArgs& a, int64_t b, in
   return a.finished && a.finished[b * a.finished_s0 + k * a.finished_s1];
 }
 
-// Four CTAs an SM leave 64 registers; three with four steps on their way take 65 us above (two waves),
-// five and six, which spill, 57 and 72.
+// Four CTAs an SM leave 64 registers.  When the walk took 54 us, three with four steps on their way took 65
+// (two waves), five and six, which spill, 57 and 72.
 template <typename T, int Q>
 __global__ void __launch_bounds__(kThreads, kBeamCtas) beam_parts_kernel(const BeamSelectArgs a) {
   constexpr int E = 16 / sizeof(T), P = E / 2;

@@ -45,8 +45,8 @@ cc1d_status check_select(const cc1d_beam_select_params* p, BeamSelectArgs* a) {
   a->tokens = p->tokens;
   // As many CTAs as run at a time, but no part so short that joining the parts' lists takes longer
   // than it saves: 1024 elements for each candidate.  512 rows of 128000 take 53 us in one part and
-  // 58 in two.  Parts of 2048, 1024 n and 2048 n elements: 4 rows of 32000, n = 4: 12.5, 11.1, 11.6 us;
-  // 16 rows of 128000, n = 32: 45.8, 24.7, 26.3; 8 rows, n = 16: 37.6, 21.0, 20.6.
+  // 61 in two.  Parts of 2048, 1024 n and 2048 n elements: 4 rows of 32000, n = 4: 12.3, 11.8, 11.9 us;
+  // 16 rows of 128000, n = 32: 44.3, 23.9, 25.3; 8 rows of one request, n = 16: 38.7, 21.8, 21.6.
   const int64_t rows = p->batch * p->beams, want = rows > 0 ? kBeamCtas * sm_count() / rows : 1;
   const int64_t least = std::max<int64_t>(2048, 1024 * p->candidates);
   a->parts = std::max<int64_t>(1, std::min(want, (p->vocab + least - 1) / least));

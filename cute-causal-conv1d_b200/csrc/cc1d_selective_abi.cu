@@ -140,13 +140,15 @@ bool pairs_ok(const TensorArg& t, const SelArgs& a) {
 }
 
 // Parts of the sequence that run side by side.  One part needs no first pass over it; with more,
-// that pass finds what each part hands to the next one.  Four CTAs run on an SM (registers), and a
-// tile takes long because a thread's work is one chain: with n CTAs on an SM its time is about
-// (microseconds, 32 positions, 16 states, bf16 with z)
+// that pass finds what each part hands to the next one.  Up to 16 states four CTAs run on an SM
+// (registers), and a tile takes long because a thread's work is one chain: with n CTAs on an SM its time
+// is about (microseconds, 32 positions, 16 states, bf16 with z)
 //
 //   forward  3.0 + .55 n, the first pass .66 of it      backward  13.7 + 1.2 n, .43
 //
-// and a part about two tiles' time to start.  Measured on a B200, bf16 with z, 16 states, microseconds
+// and a part about two tiles' time to start.  The same rule stands for other types and numbers of states.  It is
+// off where the backward's shared memory lets fewer CTAs run (59 KB and three of them at 32 states, 78 and
+// 105 KB and two at 64 and 128, 150 KB and one at 256), as the last line shows.  Measured on a B200, bf16 with z, 16 states, microseconds
 // in one part, in the parts chosen, and in the best of thirteen counts from 1 to 64:
 //
 //   batch x dim x seqlen   forward              backward

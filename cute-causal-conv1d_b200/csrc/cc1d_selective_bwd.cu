@@ -19,7 +19,7 @@
 // What bounds it: an element takes two exponentials (238 us for the 537 M elements of 4 x 4096 x 2048
 // x 16, which takes 1188; its memory 82) and 28 instructions, most of them the gradients' FMAs and the
 // exchanges that sum dB, dC over channels and ds, dx over states.  Eight warps an SM are what the
-// registers leave; a scheduler issues .35 a cycle.  Of the 1188 us the pass to the states takes 180,
+// registers leave (above 16 states shared memory leaves six to two); a scheduler issues .35 a cycle.  Of the 1188 us the pass to the states takes 180,
 // the gradients 570 (their sums over channels 180, over states 100), and what is done once per
 // position and channel (step sizes, gates, loads, stores) 440.
 //

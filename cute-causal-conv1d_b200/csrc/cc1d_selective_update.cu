@@ -96,9 +96,11 @@ __global__ void __launch_bounds__(kThreads) sel_update_kernel(const __grid_const
 // One token of rows whose states are packed: the threads of a channel take it through four batch
 // rows.  All loads of states, B and C come first; what belongs to a row and channel (step size, output
 // gate, output) is one thread's work for each row, and goes to the others by exchanges.
-// (128, 8192, 16) bf16 in a pool of 160 rows moves 143 MB in 25 us (22 us at the copy's rate); with
-// the step sizes, gates and outputs made by every thread it took 40 us, bound by its instructions, and
-// without the packets and rows in flight 66 us.  In that form two rows a thread took 42 us with cold
+// (128, 8192, 16) bf16 in a pool of 160 rows moves 143 MB (22 us at the copy's rate) in 34 us where no state
+// lies in L2: a thread's loads are on their way once, and DRAM is busy a third of the time.  Again and again
+// on the same states, part of which L2 holds, it takes 25 us; there, with the step sizes, gates and outputs
+// made by every thread it took 40 us, bound by its instructions, and without the packets and rows in
+// flight 66 us.  In that form two rows a thread took 42 us with cold
 // states, four 43, eight 49; four rows give each thread of four (16 states) one row's scalars.
 constexpr int kRows = 4;
 
